@@ -290,6 +290,73 @@ VERACE_API int verace_decode_step(const void* sssd_q, const void* sssd_k, const 
                                   int b, int h, int d, int D, int dtype, int mode,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * Products with 4-bit weights.  No counterpart in the reference, whose projections and LM
+ * head are dense torch.nn.Linear products (e.g. verace_v1/modules/backbone.py:202).
+ *   y[i][j] = sum_k x[i][k] W[j][k] (+ bias[j]),  W[j][k] = s[k/group][j] (q[j][k] - z[k/group][j])
+ * x      : [m, k] (dtype), rows ldx elements apart, each 16-byte aligned
+ * qweight: [n, k/2] bytes, two codes q in [0, 15] to a byte along k, the even k in the low
+ *          half; 16-byte aligned
+ * scales : [ceil(k/group), n] (dtype)
+ * zeros  : [ceil(k/group), n] bytes in [0, 15], or NULL (8 everywhere)
+ * bias   : [n] (dtype), or NULL
+ * y      : [m, n] (out_dtype: dtype or VERACE_F32), dense
+ * k % 32 == 0; group 32, 64 or 128 (the last group of a row may be short).  All sums are
+ * fp32; the integers q - z enter them exactly and each group's sum is scaled once.
+ * ---------------------------------------------------------------------------- */
+VERACE_API int verace_int4_linear(const void* x, long long ldx, const void* qweight, const void* scales,
+                                  const void* zeros, const void* bias, void* y, long long m, int n, int k,
+                                  int group, int dtype, int out_dtype, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * Logits before the choice of a token.  The reference's generator takes the arg-max of the
+ * raw logits (verace_v1/serving/hyper_generate.py:58-77); these are the usual controls.
+ * Per row, with c the count of a token among the row's generated tokens and "seen" any
+ * occurrence in its history, the prompt's included, in this order:
+ *   l <- l / r if l > 0 else l r   where seen             (rep)
+ *   l <- l - freq c - pres         where c > 0
+ *   l <- l + bias                  where the row's bias list names the token
+ *   l <- -inf                      where the mask's bit is 0 (whatever l was, NaN included)
+ * in fp32, rounded once to out_dtype.
+ * logits: [b, v] (dtype), row stride ld;  out: [b, v] (out_dtype: dtype or VERACE_F32), row
+ *   stride out_ld; out may be logits (one type, one row stride).
+ * tokens: [b, length] int32 or int64 (tokens_i64), row stride tokens_ld, or NULL.  Row i's
+ *   history is its first lengths[i] tokens (NULL: length; clamped to [0, length]), the
+ *   first prompt_lengths[i] (NULL: 0) of them the prompt.  Values outside [0, v) are skipped.
+ * rep_rows, pres_rows, freq_rows: [b] fp32, or NULL for the scalar beside each.
+ * bias_ids [b, n_bias] int32 or int64 (bias_i64), bias_values [b, n_bias] fp32, dense: ids
+ *   outside [0, v) are skipped; of entries with the same id the last one holds.
+ * allowed: 32-bit words, bit t % 32 of word t / 32 is token t's, row stride allowed_ld words
+ *   (0: one row for all), or NULL.
+ * ---------------------------------------------------------------------------- */
+VERACE_API int verace_logits_process(const void* logits, long long ld, void* out, long long out_ld, int b, int v,
+                                     int dtype, int out_dtype, const void* tokens, long long tokens_ld,
+                                     int tokens_i64, int length, const int* lengths, const int* prompt_lengths,
+                                     const float* rep_rows, float rep, const float* pres_rows, float pres,
+                                     const float* freq_rows, float freq, const void* bias_ids,
+                                     const float* bias_values, int n_bias, int bias_i64,
+                                     const uint32_t* allowed, long long allowed_ld, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * The choice of a token (the reference's generator: argmax, hyper_generate.py:58-77).
+ * Per row z = (l - max l) / T; kept are the tokens with z at least the k-th largest (k <= 0 or >= v:
+ * all), then those with less than p of the kept mass strictly above them (p >= 1: all; the
+ * largest is always kept), and exp(z) >= minp (the largest is
+ *   always kept); NaN and -inf are never kept.
+ *   token   = argmax over the kept of z - log(noise), the lowest index on ties: with noise
+ *             drawn from Exp(1), a draw from the softmax over the kept tokens.
+ *             T = 0 (or not above 0): the largest logit, without truncation or noise.
+ *   logprob = log softmax(z)[token] over the whole row (T = 0: of l).
+ * A row that leaves no token gives token -1 and logprob -inf.
+ * logits [b, v] (dtype), row stride ld; noise [b, v] fp32, row stride noise_ld, read only
+ * where a token is kept (NULL only with t_rows NULL and t <= 0); *_rows: [b], or NULL for
+ * the scalar; tokens [b] int64, logprobs [b] fp32.
+ * ---------------------------------------------------------------------------- */
+VERACE_API int verace_sample(const void* logits, long long ld, const float* noise, long long noise_ld, int b, int v,
+                             int dtype, const float* t_rows, float t, const int* k_rows, int k,
+                             const float* p_rows, float p, const float* minp_rows, float minp, long long* tokens,
+                             float* logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,344 @@
+"""process_logits and sample_logits against their formulas in 64 bits.
+
+Tolerances.  process: at most five fp32 operations, each off by half an ulp of a value no
+larger than |l| max(r, 1/r) + f c + p + |bias|: 6 * 2^-24 of that, plus the output's rounding.
+sample: the token has to be the 64-bit formula's wherever that is clear of ties (its key ahead
+of the next by 1e-4, the same token with either cut moved by 1e-5); a log-probability is z - max - log sum
+with fp32 z, exp and log, each within a few 2^-24 of the sizes involved."""
+import numpy as np
+import pytest
+import torch
+
+import verace_v1_b200 as V
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+HALF_ULP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+# ------------------------------------------------------------------ process
+def process_reference(l, tokens, lengths, prompts, r, p, f, ids, values, words):
+    b, v = l.shape
+    y, size = l.double().numpy().copy(), np.abs(l.double().numpy())
+    for i in range(b):
+        if tokens is not None:
+            n = tokens.shape[1] if lengths is None else max(0, min(int(lengths[i]), tokens.shape[1]))
+            seen, count = set(), {}
+            for j in range(n):
+                t = int(tokens[i, j])
+                if 0 <= t < v:
+                    seen.add(t)
+                    if j >= (0 if prompts is None else int(prompts[i])):
+                        count[t] = count.get(t, 0) + 1
+            for t in seen:
+                y[i, t] = y[i, t] / r[i] if y[i, t] > 0 else y[i, t] * r[i]
+                size[i, t] *= max(r[i], 1 / r[i])
+            for t, c in count.items():
+                y[i, t] -= f[i] * c + p[i]
+                size[i, t] += abs(f[i]) * c + abs(p[i])
+        if ids is not None:
+            last = {int(t): float(x) for t, x in zip(ids[i], values[i]) if 0 <= int(t) < v}
+            for t, x in last.items():
+                y[i, t] += x
+                size[i, t] += abs(x)
+        if words is not None:
+            w = words[i if words.shape[0] > 1 else 0].numpy().view(np.uint32)
+            ok = (w[np.arange(v) // 32] >> (np.arange(v) % 32).astype(np.uint32)) & 1
+            y[i, ok == 0] = -np.inf
+    return torch.from_numpy(y), torch.from_numpy(size)
+
+
+def check_process(out, ref, size, dtype):
+    out = out.cpu().double()
+    fine = torch.isfinite(ref)
+    assert torch.equal(out[~fine], ref[~fine])
+    tol = 6 * 2.0 ** -24 * size + HALF_ULP[dtype] * ref.abs() + 1e-7 * (dtype == torch.float16)
+    assert ((out - ref).abs()[fine] <= tol[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,v,length", [(1, 1, 1), (1, 33, 5), (3, 1000, 64), (2, 4097, 300), (5, 32000, 1000),
+                                        (2, 32001, 1), (64, 513, 37), (1, 163840, 20000), (40, 20011, 129),
+                                        (9, 65600, 777), (300, 96, 40)])
+def test_process_matches_formula(b, v, length, dtype):
+    g = torch.Generator().manual_seed(b * 7 + v + length)
+    l = (3 * torch.randn(b, v, generator=g)).to(dtype)
+    tokens = torch.randint(-2, v + 2, (b, length), generator=g)
+    tokens[:, ::3] = tokens[:, :1].clone()                       # one token many times
+    lengths = torch.randint(0, length + 1, (b,), generator=g)
+    prompts = torch.randint(0, length + 1, (b,), generator=g)
+    lengths[0], prompts[0] = length, length // 2
+    if b > 1:
+        lengths[1], prompts[1] = 0, 0
+    if b > 2:
+        lengths[2], prompts[2] = length + 9, -4
+    r, p, f = 1 + torch.rand(b, generator=g), torch.rand(b, generator=g), 0.3 * torch.rand(b, generator=g) - 0.1
+    n = min(v, 20)
+    ids = torch.stack([torch.randperm(v, generator=g)[:n] for _ in range(b)])
+    ids[:, -1] = -1
+    values = 5 * torch.randn(b, n, generator=g)
+    words = torch.randint(-2 ** 31, 2 ** 31, (b, (v + 31) // 32), generator=g).int()
+    if b > 1:
+        words[1] = 0                                     # nothing left
+    for kw in ({}, {"bias": 1}, {"mask": 1}, {"bias": 1, "mask": 1, "i32": 1}, {"out32": 1, "mask": 1}):
+        i = ids if kw.get("bias") else None
+        x = values if kw.get("bias") else None
+        w = words if kw.get("mask") else None
+        cast = (lambda t: t.int()) if kw.get("i32") else (lambda t: t)
+        ref, size = process_reference(l, tokens, lengths, prompts, r.double().numpy(), p.double().numpy(),
+                                      f.double().numpy(), i, x, w)
+        odt = torch.float32 if kw.get("out32") else dtype
+        out = V.process_logits(l.cuda(), cast(tokens).cuda(), cast(lengths).cuda(), cast(prompts).cuda(),
+                               repetition_penalty=r.cuda(), presence_penalty=p.cuda(), frequency_penalty=f.cuda(),
+                               bias_ids=None if i is None else cast(i).cuda(), bias_values=None if x is None else x.cuda(),
+                               allowed=None if w is None else w.cuda(), out_dtype=odt)
+        assert out.dtype == odt
+        check_process(out, ref, size, odt)
+
+
+def test_process_parts_alone_and_scalars():
+    g = torch.Generator().manual_seed(5)
+    l = torch.randn(4, 700, generator=g)
+    tokens = torch.randint(0, 700, (4, 50), generator=g)
+    ld, td = l.cuda(), tokens.cuda()
+    assert torch.equal(V.process_logits(ld), ld)                       # nothing asked: the same values
+    assert torch.equal(V.process_logits(ld, td), ld)                   # neutral penalties
+    ones = np.ones(4)
+    ref, size = process_reference(l, tokens, None, None, 1.5 * ones, 0.25 * ones, 0.5 * ones, None, None, None)
+    check_process(V.process_logits(ld, td, repetition_penalty=1.5, presence_penalty=0.25, frequency_penalty=0.5),
+                  ref, size, torch.float32)
+    word = torch.randint(-2 ** 31, 2 ** 31, (1, 22), generator=g).int()   # one mask for every row
+    ref, size = process_reference(l, None, None, None, ones, ones, ones, None, None, word)
+    check_process(V.process_logits(ld, allowed=word.cuda()), ref, size, torch.float32)
+    empty = torch.empty(4, 0, dtype=torch.long, device="cuda")
+    assert torch.equal(V.process_logits(ld, empty, repetition_penalty=2.0, bias_ids=empty,
+                                        bias_values=empty.float()), ld)
+    assert V.process_logits(ld[:0], td[:0]).shape == (0, 700) and V.process_logits(ld[:, :0]).shape == (4, 0)
+
+
+def test_process_equal_bias_ids_the_last_holds():
+    l = torch.zeros(2, 64, device="cuda")
+    ids = torch.tensor([[3, 5, 3, 3], [7, 7, 8, -1]], device="cuda")
+    values = torch.tensor([[1.0, 2.0, 4.0, 8.0], [1.0, -3.0, 5.0, 9.0]], device="cuda")
+    out = V.process_logits(l, bias_ids=ids, bias_values=values).cpu()
+    assert out[0, 3] == 8 and out[0, 5] == 2 and out[1, 7] == -3 and out[1, 8] == 5 and out.abs().sum() == 18
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_process_special_values(dtype):
+    v = 70
+    l = torch.zeros(1, v)
+    l[0, :6] = torch.tensor([float("nan"), INF, -INF, float("nan"), torch.finfo(dtype).min, torch.finfo(dtype).max])
+    l[0, 6] = -0.0
+    l = l.to(dtype).cuda()
+    words = torch.full((1, 3), -1, dtype=torch.int32)
+    words[0, 0] = ~1                                                   # token 0 (a NaN) is masked
+    tokens = torch.tensor([[1, 2, 3, 6, 20]], device="cuda")
+    out = V.process_logits(l, tokens, repetition_penalty=2.0, allowed=words.cuda()).cpu().float()[0]
+    assert out[0] == -INF and out[1] == INF and out[2] == -INF and torch.isnan(out[3])
+    assert out[4] == torch.finfo(dtype).min and out[5] == torch.finfo(dtype).max
+    assert (out[6:] == 0).all()
+    low = torch.full((1, 1), torch.finfo(torch.float32).min, device="cuda")   # an additive mask's lowest value
+    out = V.process_logits(l, bias_ids=torch.tensor([[20]], device="cuda"), bias_values=low).cpu().float()[0, 20]
+    assert out == (torch.finfo(torch.float32).min if dtype == torch.float32 else -INF)
+
+
+def test_process_strides_in_place_and_streams():
+    g = torch.Generator().manual_seed(6)
+    l = torch.randn(3, 900, generator=g)
+    tokens = torch.randint(0, 900, (3, 80), generator=g)
+    ones = np.ones(3)
+    ref, size = process_reference(l, tokens, None, None, 1.3 * ones, 0.5 * ones, 0.1 * ones, None, None, None)
+    kw = dict(repetition_penalty=1.3, presence_penalty=0.5, frequency_penalty=0.1)
+    for dtype in TYPES:
+        ref, size = process_reference(l.to(dtype), tokens, None, None, 1.3 * ones, 0.5 * ones, 0.1 * ones, None, None,
+                                      None)
+        for lo, ld in ((0, 912), (1, 903), (4, 928)):
+            wide = torch.zeros(3, ld, dtype=dtype, device="cuda")
+            wide[:, lo:lo + 900] = l.to(dtype).cuda()
+            view = wide[:, lo:lo + 900]
+            tw = torch.zeros(3, 101, dtype=torch.long, device="cuda")
+            tw[:, 7:87] = tokens.cuda()
+            check_process(V.process_logits(view, tw[:, 7:87], **kw), ref, size, dtype)
+            check_process(V.process_logits(view, tokens.t().contiguous().t().cuda(), **kw), ref, size, dtype)
+            before = wide.clone()
+            assert V.process_logits(view, tw[:, 7:87], out=view, **kw) is view
+            check_process(view, ref, size, dtype)
+            assert torch.equal(wide[:, :lo], before[:, :lo]) and torch.equal(wide[:, lo + 900:], before[:, lo + 900:])
+    st = torch.cuda.Stream()
+    ld, td = l.cuda(), tokens.cuda()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        out = V.process_logits(ld, td, **kw)
+    st.synchronize()
+    ref, size = process_reference(l, tokens, None, None, 1.3 * ones, 0.5 * ones, 0.1 * ones, None, None, None)
+    check_process(out, ref, size, torch.float32)
+
+
+# ------------------------------------------------------------------ sample
+def sample_reference(l, noise, t, k, p, minp):
+    """(token, logprob, clear) of one row in 64 bits; clear: the same token with the cuts by mass
+    and by min_p moved by 1e-5 either way, and its key ahead of the next by 1e-4."""
+    l = np.where(np.isnan(l), -np.inf, l)
+    z = l / t if t > 0 else l
+    top = z.max()
+    if top == -np.inf:
+        return -1, -np.inf, True
+    with np.errstate(invalid="ignore"):
+        w = np.where(z == top, 1.0, np.exp(z - top))
+    chosen, clear = [], True
+    for eps in (0.0, 1e-5, -1e-5):
+        keep = z > -np.inf
+        key = z
+        if t > 0:
+            if 0 < k < len(z):
+                keep &= z >= np.sort(z)[::-1][k - 1]
+            if p < 1:
+                values, at = np.unique(z[keep], return_inverse=True)
+                masses = np.bincount(at, weights=w[keep])[::-1]              # by value, descending
+                above = np.concatenate([[0.0], np.cumsum(masses)[:-1]])
+                inside = above < p * masses.sum() * (1 + eps)
+                inside[0] = True
+                keep &= z >= values[::-1][inside].min()
+            keep &= (w >= minp * (1 + eps)) | (z == top)
+            key = np.where(keep, z - np.log(noise), -np.inf)
+        chosen.append(int(np.argmax(key)))
+        if t > 0:
+            others = np.delete(key, chosen[-1])
+            clear &= len(others) == 0 or not (key[chosen[-1]] - others.max() < 1e-4)
+    token = chosen[0]
+    return token, (0.0 if z[token] == top else z[token] - top) - np.log(w.sum()), clear and len(set(chosen)) == 1
+
+
+def check_sample(l, noise, t, k, p, minp, most_clear=True, **kw):
+    b, v = l.shape
+    args = [x if isinstance(x, torch.Tensor) else torch.full((b,), float(x)) for x in (t, k, p, minp)]
+    tok, lp = V.sample_logits(l.cuda(), None if noise is None else noise.cuda(),
+                              temperature=t.cuda() if isinstance(t, torch.Tensor) else t,
+                              top_k=k.cuda() if isinstance(k, torch.Tensor) else k,
+                              top_p=p.cuda() if isinstance(p, torch.Tensor) else p,
+                              min_p=minp.cuda() if isinstance(minp, torch.Tensor) else minp)
+    assert tok.dtype == torch.int64 and lp.dtype == torch.float32 and tok.shape == lp.shape == (b,)
+    tok, lp, clears = tok.cpu(), lp.cpu(), 0
+    ln = l.double().numpy()
+    nn = None if noise is None else noise.double().numpy()
+    for i in range(b):
+        ti = float(args[0][i])
+        token, ref, clear = sample_reference(ln[i], None if nn is None else nn[i], ti, int(args[1][i]),
+                                             float(args[2][i]), float(args[3][i]))
+        if not clear:
+            continue
+        clears += 1
+        assert int(tok[i]) == token, (i, int(tok[i]), token)
+        if ref == -np.inf:
+            assert lp[i] == -INF
+        else:
+            size = np.abs(np.where(np.isfinite(ln[i]), ln[i], 0)).max() / (ti or 1)
+            assert abs(float(lp[i]) - ref) <= 2.0 ** -21 * (2 + 2 * size + abs(ref))
+    assert clears >= 0.8 * b or not most_clear
+    return tok, lp
+
+
+def draw(b, v, seed, masked=0.0, dtype=torch.float32, std=2.5):
+    g = torch.Generator().manual_seed(seed)
+    l = std * torch.randn(b, v, generator=g)
+    if masked:
+        l[torch.rand(b, v, generator=g) < masked] = -INF
+    return l.to(dtype), torch.empty(b, v).exponential_(generator=g)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,v", [(1, 1), (2, 3), (5, 31), (3, 1000), (4, 4099), (2, 32000), (7, 32001), (1, 163840),
+                                 (40, 20011), (300, 130)])
+def test_sample_matches_formula(b, v, dtype):
+    for seed, (t, k, p, minp, masked) in enumerate([
+            (0.0, 0, 1.0, 0.0, 0.0), (1.0, 0, 1.0, 0.0, 0.0), (0.7, 50, 1.0, 0.0, 0.3), (1.3, 0, 0.9, 0.0, 0.0),
+            (1.0, 1, 1.0, 0.0, 0.0), (0.8, 40, 0.6, 0.05, 0.5), (1.0, 0, 1.0, 0.1, 0.9), (1.0, 1000, 0.5, 0.0, 0.0)]):
+        l, noise = draw(b, v, 100 * seed + b + v, masked, dtype)
+        check_sample(l, noise if t else None, t, k, p, minp, most_clear=b * v > 100)
+
+
+def test_sample_per_row_controls():
+    b, v = 24, 5000
+    l, noise = draw(b, v, 1, 0.2)
+    g = torch.Generator().manual_seed(2)
+    t = torch.rand(b, generator=g) * 2
+    t[::5] = 0
+    k = torch.randint(0, 60, (b,), generator=g)
+    p = torch.rand(b, generator=g) * 1.2
+    minp = torch.rand(b, generator=g) * 0.1
+    l[3] = -INF
+    l[4] = float("nan")
+    check_sample(l, noise, t, k, p, minp)
+
+
+def test_sample_ties_and_extremes():
+    v = 300
+    flat = torch.zeros(4, v)
+    noise = torch.empty(4, v).exponential_(generator=torch.Generator().manual_seed(3))
+    tok, lp = V.sample_logits(flat.cuda(), temperature=0)
+    assert (tok == 0).all() and torch.allclose(lp.cpu(), torch.full((4,), -float(np.log(v))), rtol=1e-6)
+    # k = 5 over equal values keeps them all: the draw is the smallest noise
+    tok, _ = V.sample_logits(flat.cuda(), noise.cuda(), top_k=5)
+    assert torch.equal(tok.cpu(), noise.argmin(1))
+    tok, _ = V.sample_logits(flat.cuda(), noise.cuda(), top_p=0.1)
+    assert torch.equal(tok.cpu(), noise.argmin(1))
+    zeros = flat.clone()
+    zeros[:, ::2] = -0.0                                               # -0 and 0 are one value
+    tok, _ = V.sample_logits(zeros.cuda(), noise.cuda(), top_k=1)
+    assert torch.equal(tok.cpu(), noise.argmin(1))
+    tok, _ = V.sample_logits(flat.cuda(), torch.ones(4, v).cuda())     # equal keys: the lowest index
+    assert (tok == 0).all()
+    l, noise = draw(3, v, 4)
+    l[0, 17], l[1, 5], l[1, 250] = INF, INF, INF
+    l[2] = -INF
+    l[2, 299] = torch.finfo(torch.float32).min
+    for kw in ({"temperature": 0.0}, {"temperature": 1.0}, {"temperature": 0.5, "top_p": 0.5}, {"top_k": 1}):
+        tok, lp = V.sample_logits(l.cuda(), noise.cuda(), **kw)
+        tok, lp = tok.cpu(), lp.cpu()
+        assert tok[0] == 17 and tok[1] in (5, 250) and tok[2] == 299
+        assert lp[0] == 0 and abs(lp[1] + np.log(2)) < 1e-6 and lp[2] == 0
+    # top_p = 0 keeps the largest; a temperature that sends z out of range still chooses it
+    l, noise = draw(6, 1000, 5)
+    for kw in ({"top_p": 0.0}, {"min_p": 1.0}, {"temperature": 1e-30}):
+        tok, _ = V.sample_logits(l.cuda(), noise.cuda(), **kw)
+        if "temperature" not in kw:
+            assert torch.equal(tok.cpu(), l.argmax(1))
+        else:
+            assert (l.gather(1, tok.cpu()[:, None]) > 0).all()
+    peaked = torch.full((1, 1000), -12.0)
+    peaked[0, 3] = 3.0                                                 # log p near 0 keeps its digits
+    _, lp = V.sample_logits(peaked.cuda(), temperature=0)
+    assert abs(float(lp) / -np.log1p(999 * np.exp(-15.0)) - 1) < 1e-5
+    assert V.sample_logits(l[:0].cuda(), temperature=0)[0].shape == (0,)
+
+
+def test_sample_draws_follow_the_softmax():
+    l = torch.tensor([2.0, 1.0, 0.0, -1.0, 3.0, -INF, 0.5, 2.5])
+    n = 20000
+    noise = torch.empty(n, 8).exponential_(generator=torch.Generator().manual_seed(7)).cuda()
+    for kw, keep in (({}, torch.tensor([1, 1, 1, 1, 1, 0, 1, 1.])), ({"top_k": 3}, torch.tensor([1, 0, 0, 0, 1, 0, 0, 1.]))):
+        tok, _ = V.sample_logits(l.expand(n, 8).cuda(), noise, **kw)
+        prob = torch.softmax(l, 0) * keep
+        prob = prob / prob.sum()
+        freq = torch.bincount(tok.cpu(), minlength=8).double() / n
+        # six standard deviations of a count
+        assert ((freq - prob).abs() <= 6 * (prob * (1 - prob) / n).sqrt()).all()
+
+
+def test_sample_strides_and_streams():
+    l, noise = draw(5, 777, 8, 0.1)
+    lw, nw = torch.zeros(5, 800, device="cuda"), torch.ones(5, 779, device="cuda")
+    lw[:, 3:780], nw[:, 1:778] = l.cuda(), noise.cuda()
+    kw = dict(temperature=0.9, top_k=30, top_p=0.8, min_p=0.01)
+    want = V.sample_logits(l.cuda(), noise.cuda(), **kw)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = V.sample_logits(lw[:, 3:780], nw[:, 1:778], **kw)
+    st.synchronize()
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    got = V.sample_logits(l.t().contiguous().t().cuda(), noise.cuda(), **kw)
+    assert torch.equal(want[0], got[0])
+    check_sample(l, noise, 0.9, 30, 0.8, 0.01)

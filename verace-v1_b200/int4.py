@@ -1,0 +1,170 @@
+"""Products with 4-bit weights for the decode step (``verace_int4_linear``).
+
+The reference's projections and LM head are dense ``torch.nn.Linear`` products
+(verace_v1/modules/backbone.py:202, sssd_attention.py:116-126).  A decode step of a few
+sequences reads every weight for a handful of multiplications, so its time is the weights'
+bytes; codes of 4 bits with one scale (and zero) per group of 32, 64 or 128 inputs are a
+quarter of bf16's.
+
+Layout, as :func:`quantize_int4` makes it: ``qweight`` uint8 [n, k/2], two codes to a byte
+along k, the even k in the low half; ``scales`` [ceil(k/group), n] in the activations'
+dtype; ``zeros`` uint8 [ceil(k/group), n] or None (8 everywhere).
+W[n, k] = scales[k // group, n] * (code - zero).
+"""
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+
+from ._lib import check, lib
+from .kernels import _DTYPE
+from ._launch import launch
+
+GROUP_SIZES = (32, 64, 128)
+
+
+def _require_no_grad(x: torch.Tensor, who: str):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{who} runs for inference (no autograd path): call it under torch.no_grad()")
+
+
+def _check_packed(qweight, scales, zeros, bias, k, group_size, dtype):
+    if group_size not in GROUP_SIZES:
+        raise ValueError(f"group_size {group_size}: expected one of {GROUP_SIZES}")
+    n = qweight.shape[0]
+    groups = -(-k // group_size)
+    assert k % 32 == 0, "the input width must be a multiple of 32"
+    assert qweight.dtype == torch.uint8 and qweight.dim() == 2 and qweight.shape[1] * 2 == k, \
+        "qweight must be uint8 [n, k / 2]"
+    assert scales.dtype == dtype and scales.dim() == 2 and scales.shape[0] == groups and scales.shape[1] == n, \
+        "scales must be [ceil(k / group_size), n] in the activations' dtype"
+    assert zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape), \
+        "zeros must be uint8 in the shape of scales"
+    assert bias is None or (bias.dtype == dtype and bias.dim() == 1 and bias.shape[0] == n), \
+        "bias must be [n] in the activations' dtype"
+
+
+def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
+                zeros: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+                group_size: int = 128, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x [..., k] (fp32, bf16 or fp16) times the 4-bit weight's transpose, plus bias: [..., n]
+    in x's dtype or, with ``out_dtype=torch.float32``, in fp32.  Sums are fp32, the output is
+    rounded once.  Any number of rows; meant for the few of a decode step."""
+    assert x.is_cuda, "This kernel requires CUDA tensors"
+    _require_no_grad(x, "int4_linear")
+    dt = x.dtype
+    code = _DTYPE.get(dt)
+    if code is None:
+        raise ValueError(f"int4_linear: {dt} activations (expected fp32, bf16 or fp16)")
+    odt = dt if out_dtype is None else out_dtype
+    if odt is not dt and odt is not torch.float32:
+        raise ValueError(f"int4_linear: out_dtype {odt} (expected {dt} or torch.float32)")
+    k = x.shape[-1]
+    _check_packed(qweight, scales, zeros, bias, k, group_size, dt)
+    dev = x.device
+    n = qweight.shape[0]
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    m = x2.shape[0]
+    if (m > 1 and x2.stride(0) * x2.element_size() % 16) or (k > 1 and x2.stride(1) != 1) or x2.data_ptr() % 16 \
+            or (m > 1 and x2.stride(0) < k):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if not qweight.is_contiguous() or qweight.data_ptr() % 16:
+        qweight = qweight.clone(memory_format=torch.contiguous_format)
+    if not scales.is_contiguous():
+        scales = scales.contiguous()
+    if zeros is not None and not zeros.is_contiguous():
+        zeros = zeros.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    assert qweight.device == dev and scales.device == dev and (zeros is None or zeros.device == dev) \
+        and (bias is None or bias.device == dev), "all tensors must be on one device"
+    y = torch.empty((m, n), dtype=odt, device=dev)
+    rc = launch(dev, lib().verace_int4_linear, x2.data_ptr(), x2.stride(0) if m > 1 else k, qweight.data_ptr(),
+                scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
+                None if bias is None else bias.data_ptr(), y.data_ptr(), m, n, k, group_size, code, _DTYPE[odt])
+    if rc:
+        check(rc, "verace_int4_linear")
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
+
+
+def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool = True
+                  ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(qweight, scales, zeros) of weight [n, k]: round-to-nearest codes per group of
+    ``group_size`` along k.  Symmetric: scale = max |w| / 7, no zeros.  Otherwise the range
+    [min(w, 0), max(w, 0)] on 15 steps with an integer zero.  The scales are rounded to the
+    weight's dtype before the codes are taken."""
+    if group_size not in GROUP_SIZES:
+        raise ValueError(f"group_size {group_size}: expected one of {GROUP_SIZES}")
+    assert weight.dim() == 2 and weight.shape[1] % 32 == 0, "weight must be [n, k] with k a multiple of 32"
+    n, k = weight.shape
+    groups = -(-k // group_size)
+    w = weight.detach().float()
+    pad = groups * group_size - k
+    w = torch.nn.functional.pad(w, (0, pad)).view(n, groups, group_size)
+    if symmetric:
+        s = w.abs().amax(-1) / 7
+    else:
+        lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+        s = (hi - lo) / 15
+    s = s.to(weight.dtype)
+    sf = s.float()
+    inv = torch.where(sf > 0, 1 / sf, torch.zeros_like(sf))
+    z = torch.full_like(sf, 8.0) if symmetric else torch.round(-lo * inv).clamp_(0, 15)
+    q = (torch.round(w * inv.unsqueeze(-1)) + z.unsqueeze(-1)).clamp_(0, 15).to(torch.uint8)
+    q = q.view(n, -1)[:, :k]
+    packed = q[:, 0::2] | (q[:, 1::2] << 4)
+    return packed.contiguous(), s.t().contiguous(), None if symmetric else z.to(torch.uint8).t().contiguous()
+
+
+def dequantize_int4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
+                    group_size: int = 128) -> torch.Tensor:
+    """The weight [n, k] that the codes stand for, in the scales' dtype (computed in fp32)."""
+    n, k = qweight.shape[0], qweight.shape[1] * 2
+    _check_packed(qweight, scales, zeros, None, k, group_size, scales.dtype)
+    q = torch.stack((qweight & 15, qweight >> 4), dim=-1).view(n, k).float()
+    of = torch.arange(k, device=q.device) // group_size
+    z = 8.0 if zeros is None else zeros.float().t()[:, of]
+    return ((q - z) * scales.float().t()[:, of]).to(scales.dtype)
+
+
+class Int4Linear(nn.Module):
+    """A linear layer with 4-bit weights (buffers ``qweight``, ``scales``, ``zeros``, ``bias``)
+    in place of a ``torch.nn.Linear``."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, group_size: int = 128,
+                 symmetric: bool = True, dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        if group_size not in GROUP_SIZES:
+            raise ValueError(f"group_size {group_size}: expected one of {GROUP_SIZES}")
+        if in_features % 32:
+            raise ValueError(f"in_features {in_features}: expected a multiple of 32")
+        self.in_features, self.out_features, self.group_size = in_features, out_features, group_size
+        groups = -(-in_features // group_size)
+        self.register_buffer("qweight", torch.zeros(out_features, in_features // 2, dtype=torch.uint8, device=device))
+        self.register_buffer("scales", torch.zeros(groups, out_features, dtype=dtype, device=device))
+        self.register_buffer("zeros", None if symmetric else
+                             torch.zeros(groups, out_features, dtype=torch.uint8, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=dtype, device=device) if bias else None)
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, group_size: int = 128,
+                    symmetric: bool = True) -> "Int4Linear":
+        n, k = weight.shape
+        m = cls(k, n, bias is not None, group_size, symmetric, weight.dtype, device="meta")
+        m.qweight, m.scales, m.zeros = quantize_int4(weight, group_size, symmetric)
+        m.bias = None if bias is None else bias.detach().clone()
+        return m
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, group_size: int = 128, symmetric: bool = True) -> "Int4Linear":
+        return cls.from_weight(linear.weight, linear.bias, group_size, symmetric)
+
+    def dequantized(self) -> torch.Tensor:
+        return dequantize_int4(self.qweight, self.scales, self.zeros, group_size=self.group_size)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int4_linear(x, self.qweight, self.scales, self.zeros, self.bias, group_size=self.group_size)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, group_size={self.group_size}, "
+                f"zeros={self.zeros is not None}, bias={self.bias is not None}")
