@@ -302,11 +302,15 @@ VERACE_API int verace_decode_step(const void* sssd_q, const void* sssd_k, const 
  * bias   : [n] (dtype), or NULL
  * y      : [m, n] (out_dtype: dtype or VERACE_F32), dense
  * k % 32 == 0; group 32, 64 or 128 (the last group of a row may be short).  All sums are
- * fp32; the integers q - z enter them exactly and each group's sum is scaled once.
+ * fp32; codes, zeros and inputs enter them exactly and each group's sum is scaled once.
+ * Workspace: verace_int4_linear_workspace(m, n, k, group, dtype) bytes, 0 for short inputs;
+ * calls sharing a workspace must not overlap.
  * ---------------------------------------------------------------------------- */
+VERACE_API size_t verace_int4_linear_workspace(long long m, int n, int k, int group, int dtype);
 VERACE_API int verace_int4_linear(const void* x, long long ldx, const void* qweight, const void* scales,
                                   const void* zeros, const void* bias, void* y, long long m, int n, int k,
-                                  int group, int dtype, int out_dtype, void* stream);
+                                  int group, int dtype, int out_dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 /* ------------------------------------------------------------------------------
  * Logits before the choice of a token.  The reference's generator takes the arg-max of the

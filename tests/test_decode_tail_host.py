@@ -73,10 +73,12 @@ def test_python_api_requires_cuda_tensors():
 @host_only
 def test_int4_linear_rejects_bad_arguments_without_a_device():
     f = _lib.lib().verace_int4_linear
-    ok = [FAKE, 64, FAKE, FAKE, None, None, FAKE, 1, 8, 64, 32, 1, 1, None]
+    ok = [FAKE, 64, FAKE, FAKE, None, None, FAKE, 1, 8, 64, 32, 1, 1, None, 0, None]
 
     def call(**kw):
-        names = ["x", "ldx", "q", "s", "z", "bias", "y", "m", "n", "k", "group", "dtype", "out", "stream"]
+        names = ["x", "ldx", "q", "s", "z", "bias", "y", "m", "n", "k", "group", "dtype", "out", "ws",
+                 "nws", "stream"]
+        assert set(kw) <= set(names)
         return f(*[kw.get(n, v) for n, v in zip(names, ok)])
 
     assert call(group=48) == 2 and "group size 48" in _err()
@@ -89,6 +91,12 @@ def test_int4_linear_rejects_bad_arguments_without_a_device():
     assert call(y=None) == 1 and "NULL" in _err()
     assert call(q=ctypes.c_void_p(264)) == 1 and "aligned" in _err()
     assert call(ldx=68) == 1 and "aligned" in _err()
+    size = _lib.lib().verace_int4_linear_workspace
+    need = size(64, 4096, 4096, 128, 1)
+    assert need > size(64, 4096, 2048, 128, 1) > 0 and size(1, 4096, 1024, 128, 1) == 0 and size(0, 8, 64, 32, 1) == 0
+    big = dict(m=64, n=4096, k=4096, ldx=4096, group=128)
+    assert call(**big) == 4 and "workspace" in _err()
+    assert call(**big, ws=FAKE, nws=need - 1) == 4
     assert call(m=0, x=None, y=None) == 0 and call(n=0, q=None, y=None) == 0       # nothing to do
 
 

@@ -51,7 +51,8 @@ _SIGNATURES = {
     "verace_mcmoe_projection": (_i, [_p] * 6 + [_i, _p, ctypes.c_longlong, _i, _i, _i, _i, _i, _p, _c_size, _p]),
     "verace_situ_glu": (_i, [_p, _p, ctypes.c_longlong, _p, ctypes.c_longlong, _i, ctypes.c_float, ctypes.c_float,
                              _i, _p]),
-    "verace_int4_linear": (_i, [_p, ctypes.c_longlong] + [_p] * 5 + [ctypes.c_longlong] + [_i] * 5 + [_p]),
+    "verace_int4_linear_workspace": (_c_size, [ctypes.c_longlong, _i, _i, _i, _i]),
+    "verace_int4_linear": (_i, [_p, ctypes.c_longlong] + [_p] * 5 + [ctypes.c_longlong] + [_i] * 5 + [_p, _c_size, _p]),
     "verace_logits_process": (_i, [_p, ctypes.c_longlong, _p, ctypes.c_longlong, _i, _i, _i, _i, _p, ctypes.c_longlong,
                                    _i, _i, _p, _p] + [_p, ctypes.c_float] * 3 + [_p, _p, _i, _i, _p,
                                                                                  ctypes.c_longlong, _p]),

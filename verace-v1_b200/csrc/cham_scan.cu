@@ -46,6 +46,7 @@ int tc_read_status(cudaStream_t st, int* status);
 int sssd_tc_read_status(int* status);
 int decode_read_status(unsigned int* status);
 int mcmoe_read_status(int* status);
+int int4_read_status(int* status);
 
 namespace {
 
@@ -788,6 +789,9 @@ extern "C" int verace_device_status(void* stream) {
   if (rc) return rc;
   status |= status2;
   rc = cgemm_tc_read_status(&status2);
+  if (rc) return rc;
+  status |= status2;
+  rc = int4_read_status(&status2);
   if (rc) return rc;
   status |= status2;
   unsigned int dstat = 0;   // bit 0: a hologram far from unitary; bit 1: a decode wait gave up

@@ -1,51 +1,78 @@
 // Product of a few tokens with 4-bit weights:
 //     y[i][n] = sum_k x[i][k] W[n][k] (+ bias[n]),   W[n][k] = s[k/G][n] (q[n][k] - z[k/G][n])
 // q in [0, 15], two to a byte along k (the even k in the low half); z in [0, 15], 8 when no
-// zeros are given.  One group's terms are summed with the integers q - z, exact in bf16 and
-// fp16, and scaled once: y = sum_g s_g (sum_{k in g} x_k (q_k - z_g)), all sums in fp32.  No
-// weight is ever rounded.
+// zeros are given.
 //
-// Bound: the weights' bytes (half a byte for 2 m operations), as long as the tensor cores keep
-// up.  So the weights stream through shared memory once, each warp on its own: 32 output rows
-// by a chunk of 128 inputs at a time, three chunks in flight by cp.async, no barrier between
-// warps.  mma.sync with the weights as the 16-row operand fits few tokens better than a
-// 128-row tile: eight tokens are one instruction's columns.  The order of k inside a chunk is
-// free (both operands use the same one): lane t of a row's four takes one 32-bit word of
-// every 16 bytes, whose nibbles i and i + 4 unpack as a pair with one logic operation, and x
-// is staged in that order, so that a lane's operand is one 16-byte load.
-// fp32 inputs are cut into three bf16 columns of 8 significant bits each (exact).
+// Bound: the weights' bytes (half a byte for 2 m operations), if nothing else is slower.  A
+// first version unpacked the codes to bf16 (11 instructions for 8 codes) for mma.sync and ran
+// at a quarter of the memory rate, bound by instructions.  Here the tensor cores take a code as
+// it is: the bit pattern of an e4m3 number in [0, 15] reads code * 2^-9 (subnormal below 8, the
+// first binade from 8 on, with the same step), so a word of 8 codes becomes 8 operands with one
+// shift and two masks.  x goes in as fp8 pieces that add up to it, exactly:
+//   * few tokens: e4m3 pieces, each the rest of the one before times 2^5, in columns of their
+//     own (a 128-row MMA takes 50 clocks for anything up to 64 columns): y = d0 + 2^-5 d1 + ...
+//     bf16's 8 bits are 2 pieces, fp16's 11 are 3, fp32's 24 are 5;
+//   * up to 64 tokens of 16-bit types: an e4m3 piece and one or two e5m2 pieces of the rest, one
+//     MMA after the other into the same columns.
+// Each token is scaled by a power of two, its largest input to [2^7, 2^8); inputs 2^-22 of that
+// and smaller lose digits.  tcgen05.mma adds fp8 products in full fp32 (measured: 2^23 + 1 is
+// exact).  The zeros are one more MMA per group: 32 inputs that hold X = sum of the group's
+// scaled x in 6 e5m2 pieces, against -z.  So D = 2^-9 (sum q x - z X) per group, and a row's
+// thread adds s D in fp32.  No weight and no input is rounded.
+// What q x and z X lose by cancelling is 2^-24 of the group's largest input.  Where at most a
+// sixteenth of a group is 2^12 above all the rest, that could show in the outputs whose q = z
+// there, so those inputs (and infinities and NaN) are left out of the pieces and added one by
+// one as (q - z) x s at the end (rare).
+//
+// One CTA per SM, 128 output rows at a time, 16 warps: one feeds the weights by TMA (128 rows x
+// 256 codes a stage, 128-byte swizzle: a row's thread reads 16 bytes without bank conflicts),
+// one the staged x, two issue the MMAs, eight unpack codes into TMEM (the MMA's A operand; two
+// sets of four take a stage's halves), four hold the rows' sums.  Few row tiles: k is split over
+// a cluster and the partial sums are joined through distributed shared memory in rank order.
 #include "common.cuh"
 #include "tc.cuh"
+#include "tmap.cuh"
 
 #include <cooperative_groups.h>
+#include <cuda_fp8.h>
 
 #include <atomic>
+#include <mutex>
 
 namespace verace {
+
+__device__ int g_int4_status = 0;   // non-zero after a bounded wait gave up
+
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int NT = 256;           // threads per CTA: 8 warps
-constexpr int WARPS = NT / 32;
-constexpr int ROWS = 32;          // output rows per warp
-constexpr int KC = 128;           // inputs per chunk (64 bytes of a weight row)
-constexpr int STAGES = 3;         // chunks in flight per warp
-// A row's 64 bytes at a pitch of 80: the word loads of a fragment (8 rows x 4 lanes) hit 32 banks.
-constexpr int PITCH = 80;
-constexpr int STAGE_BYTES = ROWS * PITCH;
-constexpr int RPITCH = 36;        // row pitch (floats) of the partial tiles, conflict-free likewise
-constexpr int XSTREAM = 16384;    // bytes of x in one of the two streamed buffers, before padding
+constexpr uint32_t POLLS = 1u << 22;
+constexpr int NT = 512;                  // threads: 16 warps
+constexpr int ROWS = 128;                // output rows per tile
+constexpr int KC = 128;                  // inputs per chunk
+constexpr int SW = 5;                    // weight stages of two chunks
+constexpr int W_STAGE = ROWS * KC;       // bytes: 128 rows x 256 codes
+constexpr int NA = 4;                    // A operands (one chunk each) in TMEM
+constexpr int D_COL = 256;               // first TMEM column of the accumulators
+constexpr int MAX_SB = 64;
+constexpr int B_SMEM = 136 * 1024;
+constexpr float FINITE = 3.4028235e38f;
+constexpr float APART = 1.f / 4096.f;
 
-// A group's unscaled sum reaches 128 * 15 times its largest input: bf16 and fp32 inputs are
-// brought down by 2^12 (exact) and the result back up, so that sums of any finite inputs stay
-// finite.  fp16 inputs are below 2^16 and need none.
-template <typename T> constexpr float down() { return std::is_same<T, __half>::value ? 1.f : 1.f / 4096.f; }
-template <typename T> constexpr float up() { return std::is_same<T, __half>::value ? 1.f : 4096.f; }
-
-// operand type of the products, and columns of the product per token
-template <typename T> struct Op { using type = T; static constexpr int cols = 1; };
-template <> struct Op<float> { using type = __nv_bfloat16; static constexpr int cols = 3; };
+// How a token tile's x is laid out.  MP tokens per tile; COLS: the pieces in columns of their own.
+template <typename T, int MP_>
+struct Shape {
+  static constexpr bool IS32 = std::is_same<T, float>::value;
+  static constexpr int MP = MP_;
+  static constexpr bool COLS = IS32 || MP <= (std::is_same<T, __half>::value ? 16 : 32);
+  static constexpr int P = IS32 ? 5 : std::is_same<T, __half>::value ? 3 : 2;    // pieces
+  static constexpr int N = COLS ? (P * MP + 15) / 16 * 16 : MP;                  // MMA columns
+  static constexpr int PASSES = COLS ? 1 : P;
+  static constexpr int ND = 128 / N < 2 ? 1 : 2;                                 // accumulators per MMA warp
+  // bytes of a chunk's B operands: the passes' [128 / 16][N][16], then per group the zeros' [2][N][16]
+  static constexpr int block(int gpc) { return PASSES * KC * N + gpc * 32 * N; }
+};
 
 struct Int4Args {
   const void* x;
@@ -57,437 +84,793 @@ struct Int4Args {
   void* y;
   long long m;
   int n, k, out_f32;
-  int wk;        // warps of a CTA that share a row tile, interleaved along k
-  int ck;        // CTAs of a cluster that share a row tile, each with a range of k
-  int per;       // chunks in a CTA's range of k
-  int resident;  // the whole range's x staged once (else 16 KB at a time, double-buffered)
-  int x_bytes;   // shared memory of x
+  int tiles, ytiles;   // row tiles and token tiles
+  int ck, per;         // CTAs that share a tile, each with `per` chunks of k
+  int staged;          // x comes from the workspace (else every CTA stages its own)
+  int sb;              // chunks of x in shared memory
+  int resident;        // all of the CTA's chunks, loaded once
+  const uint8_t* ws;   // staged x: blocks [token tile][chunk], then scales, then left-out masks
+  const float* ws_scale;
+  const uint32_t* ws_mask;
 };
 
+// ------------------------------------------------------------------ staging x
+// Eight consecutive inputs of one token; out-of-range ones are 0.
 template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Nibbles i and i + 4 of w (already shifted down by 4 i) minus the zero, as a pair: the code in
-// the low mantissa bits of 128 (bf16) or 1024 (fp16) is that number plus the code.
-template <typename T>
-__device__ __forceinline__ uint32_t unpack(uint32_t w, uint32_t zero2) {
-  constexpr uint32_t magic = std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
-  const uint32_t c = (w & 0x000f000fu) | magic;
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&zero2));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const __nv_bfloat162 r =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(&zero2));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
-  return ((std::is_same<T, __half>::value ? 0x6400u : 0x4300u) | z) * 0x10001u;
-}
-
-// Eight consecutive inputs as loaded, and their staging: pairs (0,4) (1,5) (2,6) (3,7).
-template <typename T> struct Raw { uint4 u[sizeof(T) / 2]; };
-
-template <typename T>
-__device__ __forceinline__ void load_raw(Raw<T>& r, const T* p, bool valid) {
+__device__ __forceinline__ void load8(const T* p, bool valid, float (&v)[8]) {
+  uint4 u[sizeof(T) / 2];
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-    r.u[i] = valid ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
-}
-
-__device__ __forceinline__ uint4 pair_up(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  // words (0,1) (2,3) (4,5) (6,7) -> (0,4) (1,5) (2,6) (3,7)
-  return make_uint4(__byte_perm(a, c, 0x5410), __byte_perm(a, c, 0x7632), __byte_perm(b, d, 0x5410),
-                    __byte_perm(b, d, 0x7632));
-}
-
-__device__ __forceinline__ uint32_t bf16_down(uint32_t w) {
-  const __nv_bfloat162 f = __float2bfloat162_rn(1.f / 4096.f);
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), f);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-template <typename T>
-__device__ __forceinline__ void store_staged(uint8_t* dst, int pitch, const Raw<T>& r) {
+    u[i] = valid ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
   if constexpr (std::is_same<T, float>::value) {
-    // x = h + m + l exactly: the top 8 significant bits, the next 8, the rest (truncated, so
-    // that nothing rounds up past the range; an infinity or NaN stays whole in h)
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.u);
-    uint32_t h[4], m[4], l[4];
+    const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t p[2][3];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float x = __uint_as_float(w[i + 4 * e]) * down<float>();
-        const bool fin = fabsf(x) <= 3.4e38f;
-        // a NaN keeps a bit in its top half
-        const uint32_t hb = fin ? __float_as_uint(x) & 0xffff0000u
-                                : (x != x ? 0x7fc00000u : __float_as_uint(x));
-        const float rest = fin ? x - __uint_as_float(hb) : 0.f;
-        const uint32_t mb = __float_as_uint(rest) & 0xffff0000u;
-        const float last = rest - __uint_as_float(mb);
-        p[e][0] = hb; p[e][1] = mb; p[e][2] = __float_as_uint(last);
-      }
-      h[i] = __byte_perm(p[0][0], p[1][0], 0x7632);
-      m[i] = __byte_perm(p[0][1], p[1][1], 0x7632);
-      l[i] = __byte_perm(p[0][2], p[1][2], 0x7632);
-    }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(dst + pitch) = make_uint4(m[0], m[1], m[2], m[3]);
-    *reinterpret_cast<uint4*>(dst + 2 * pitch) = make_uint4(l[0], l[1], l[2], l[3]);
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
   } else {
-    uint4 u = r.u[0];
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-      u = make_uint4(bf16_down(u.x), bf16_down(u.y), bf16_down(u.z), bf16_down(u.w));
-    *reinterpret_cast<uint4*>(dst) = pair_up(u.x, u.y, u.z, u.w);
+    unpack8<T>(u[0], v);
   }
 }
 
-// scale bits and zero of one output row and group, carried by the row's lane
-template <typename T> struct Scale { uint32_t v; };            // scale | zero << 16
-template <> struct Scale<float> { uint32_t v; uint32_t zero; };
+// Zeroes the inputs that are added one by one; `LANES` lanes in a row hold one group.  Returns the
+// lane's largest remaining |input|.
+template <int LANES>
+__device__ __forceinline__ float leave_out(float (&v)[8], bool& out) {
+  float mine = 0.f;
+  out = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!(fabsf(v[i]) <= FINITE)) out = true, v[i] = 0.f;
+    mine = fmaxf(mine, fabsf(v[i]));
+  }
+  float top = mine;
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // a lane whose inputs are all far below the largest: perhaps that one stands alone
+  if (__any_sync(0xffffffffu, mine > 0.f && mine < top * APART)) {
+    int high = 0, low = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      high += fabsf(v[i]) >= top * APART;
+      low |= fabsf(v[i]) < top * APART && v[i] != 0.f;
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      high += __shfl_xor_sync(0xffffffffu, high, o);
+      low |= __shfl_xor_sync(0xffffffffu, low, o);
+    }
+    if (low && high <= LANES * 8 / 16) {
+      mine = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (fabsf(v[i]) >= top * APART) out = true, v[i] = 0.f;
+        mine = fmaxf(mine, fabsf(v[i]));
+      }
+    }
+  }
+  return mine;
+}
 
-// C8: columns in tiles of 8.  GPC: groups per chunk.
-template <typename T, int C8, int GPC>
-__global__ void __launch_bounds__(NT, C8 <= 2 ? 2 : 1) int4_linear_mma(Int4Args a) {
-  using O = typename Op<T>::type;
-  constexpr int PER_TOK = Op<T>::cols;
-  constexpr int TOK = 8 * C8 / PER_TOK;          // tokens per CTA
-  extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* xs = smem;
-  uint8_t* ws = smem + a.x_bytes;
-  const int tid = threadIdx.x, lane = tid % 32, w = tid / 32, g = lane / 4, t = lane % 4;
-  const int wk = w % a.wk, wr = w / a.wk;
-  const int rank = blockIdx.x % a.ck;
-  const long long tile0 = (long long)(blockIdx.x / a.ck) * (WARPS / a.wk) * ROWS;   // the CTA's first row
-  const long long row0 = tile0 + wr * ROWS;
-  const long long m0 = (long long)blockIdx.y * TOK;
-  const int toks = (int)(a.m - m0 < TOK ? a.m - m0 : TOK);
-  const int cols = toks * PER_TOK;
-  const int chunks = (a.k + KC - 1) / KC;
-  const int c0 = rank * a.per, c1 = min(chunks, c0 + a.per);
-  const int steps = (max(c1 - c0, 0) + a.wk - 1) / a.wk;
-  const size_t qrow = a.k / 2;
+// The exponent that brings `top` to [2^7, 2^8), at most 100.
+__device__ __forceinline__ int shift_of(float top) {
+  return min(7 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-  // ---- weights: this warp's ring
-  uint8_t* ring = ws + w * STAGES * STAGE_BYTES;
-  const bool rows_live = row0 < a.n;
-  const uint8_t* qp = a.q + (rows_live ? row0 + g : 0) * qrow + t * 16;
-  auto load_stage = [&](int j) {
-    const int c = c0 + j * a.wk + wk;
-    if (rows_live && c < c1) {
-      uint8_t* d = ring + (j % STAGES) * STAGE_BYTES + g * PITCH + t * 16;
-      const bool in_k = c * 64 + t * 16 < (int)qrow;
+// Writes the pieces of lane l16's eight inputs of a chunk (token row t of the tile) and, from a
+// group's first lane, X.  A word's codes 0, 2, 4, 6 unpack before 1, 3, 5, 7, and so do x's bytes.
+template <typename T, typename S, int GPC>
+__device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* block, int t, int l16) {
+  constexpr int LANES = 16 / GPC;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= scale, sum += v[i];
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  constexpr int at[4][2] = {{0, 2}, {4, 6}, {1, 3}, {5, 7}};
+  uint8_t* d = block + ((l16 / 2) * S::N + t) * 16 + (l16 % 2) * 8;
+  auto put = [&](int p, const uint32_t (&b)[4]) {
+    uint8_t* to = d + (S::COLS ? p * S::MP * 16 : p * KC * S::N);
+    *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
+  };
+  if constexpr (S::IS32) {
+#pragma unroll
+    for (int p = 0; p < S::P; ++p) {
+      uint32_t b[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool v = in_k && row0 + g + 8 * i < a.n;
-        tc::cp_async16(d + 8 * i * PITCH, v ? qp + 8 * i * qrow + (size_t)c * 64 : a.q, v);
+        b[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[at[i][0]], v[at[i][1]]), __NV_SATFINITE, __NV_E4M3);
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b[i], __NV_E4M3);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        v[at[i][0]] = (v[at[i][0]] - f.x) * 32.f;
+        v[at[i][1]] = (v[at[i][1]] - f.y) * 32.f;
       }
-    }
-    tc::cp_async_commit();
-  };
-  // ---- scales and zeros: lane l carries row l's
-  const T* sp = static_cast<const T*>(a.s) + row0 + lane;
-  const uint8_t* zp = a.z ? a.z + row0 + lane : nullptr;
-  const int groups = (a.k + KC / GPC - 1) / (KC / GPC);
-  Scale<T> next[GPC];
-  auto load_scales = [&](int j) {
-    const int c = c0 + j * a.wk + wk;
-#pragma unroll
-    for (int i = 0; i < GPC; ++i) {
-      const long long gi = (long long)c * GPC + i;
-      const bool v = c < c1 && gi < groups && row0 + lane < a.n;
-      const uint32_t zero = v && zp ? __ldg(zp + gi * a.n) : 8u;
-      if constexpr (std::is_same<T, float>::value) {
-        next[i].v = v ? __float_as_uint(__ldg(sp + gi * a.n)) : 0u;
-        next[i].zero = zero;
-      } else {
-        next[i].v = (v ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(sp) + gi * a.n) : 0u) | (zero << 16);
-      }
-    }
-  };
-#pragma unroll
-  for (int j = 0; j < STAGES; ++j) load_stage(j);
-  load_scales(0);
-
-  // ---- x: staged whole, or streamed XSTREAM bytes at a time
-  const int sx = a.resident ? max(steps, 1) : (8 / C8) / a.wk;      // steps per buffer
-  const int xk = sx * a.wk * KC;                                    // inputs per buffer
-  const int xpitch = xk * 2 + 64;
-  const int xbuf = 8 * C8 * xpitch;
-  const T* x = static_cast<const T*>(a.x) + m0 * a.ldx;
-  const int units_k = xk / 8;
-  constexpr int XR = (XSTREAM / 16 + NT - 1) / NT;                  // units per thread and buffer, at most
-  Raw<T> xr[XR];
-  auto fetch_x = [&](int b) {
-    const int kb = (c0 * KC) + b * xk;
-#pragma unroll
-    for (int i = 0; i < XR; ++i) {
-      const int u = tid + i * NT, tok = u / units_k, k = kb + (u - tok * units_k) * 8;
-      if (tok < toks) load_raw(xr[i], x + (long long)min(tok, toks - 1) * a.ldx + k, k < a.k);
-    }
-  };
-  auto store_x = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < XR; ++i) {
-      const int u = tid + i * NT, tok = u / units_k;
-      if (tok < toks)
-        store_staged<T>(xs + (b & 1) * xbuf + tok * PER_TOK * xpitch + (u - tok * units_k) * 16, xpitch, xr[i]);
-    }
-  };
-  if (a.resident) {
-    const int units = toks * units_k;
-    for (int u0 = 0; u0 < units; u0 += 4 * NT) {
-      Raw<T> r[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int u = u0 + tid + i * NT, tok = u / units_k, k = c0 * KC + (u - tok * units_k) * 8;
-        if (u < units) load_raw(r[i], x + (long long)tok * a.ldx + k, k < a.k);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int u = u0 + tid + i * NT, tok = u / units_k;
-        if (u < units) store_staged<T>(xs + tok * PER_TOK * xpitch + (u - tok * units_k) * 16, xpitch, r[i]);
-      }
+      put(p, b);
     }
   } else {
-    fetch_x(0);
-    store_x(0);
+    // 8 or 11 bits: fp16 holds them
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[at[i][0]], v[at[i][1]]);
+#pragma unroll
+    for (int p = 0; p < S::P; ++p) {
+      uint32_t b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2_raw hr = *reinterpret_cast<const __half2_raw*>(&h[i]);
+        __half2_raw r;
+        if (S::COLS || p == 0) {
+          b[i] = __nv_cvt_halfraw2_to_fp8x2(hr, __NV_SATFINITE, __NV_E4M3);
+          r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b[i], __NV_E4M3);
+        } else {
+          b[i] = __nv_cvt_halfraw2_to_fp8x2(hr, __NV_SATFINITE, __NV_E5M2);
+          r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b[i], __NV_E5M2);
+        }
+        h[i] = __hsub2(h[i], *reinterpret_cast<const __half2*>(&r));
+        if (S::COLS) h[i] = __hmul2(h[i], __float2half2_rn(32.f));
+      }
+      put(p, b);
+    }
+  }
+  if (l16 % LANES == 0) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int p = 0; p < 6; ++p) {
+      const uint32_t b = __nv_cvt_float_to_fp8(sum, __NV_SATFINITE, __NV_E5M2);
+      w[p / 4] |= b << (8 * (p % 4));
+      const __half_raw r = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E5M2);
+      sum -= __half2float(*reinterpret_cast<const __half*>(&r));
+    }
+    uint4* z = reinterpret_cast<uint4*>(block + S::PASSES * KC * S::N + (l16 / LANES) * 32 * S::N) + t;
+    z[0] = make_uint4(w[0], w[1], 0, 0);
+    z[S::N] = make_uint4(0, 0, 0, 0);
+    if constexpr (S::COLS) {
+#pragma unroll
+      for (int p = 1; p < S::P; ++p) z[p * S::MP] = z[S::N + p * S::MP] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// The staging kernel: one CTA per token.
+template <typename T, int MP, int GPC>
+__global__ void __launch_bounds__(NT) int4_stage_x(const T* __restrict__ x, long long ldx, int k, int chunks,
+                                                   uint8_t* __restrict__ ws, float* __restrict__ scales,
+                                                   uint32_t* __restrict__ masks) {
+  using S = Shape<T, MP>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int s_top;
+  __shared__ uint32_t s_mask;
+  const int tid = threadIdx.x, l16 = tid % 16;
+  const long long tok = blockIdx.x;
+  const T* row = x + tok * ldx;
+  const int span = (chunks * GPC + 31) / 32;
+  if (tid == 0) s_top = 0, s_mask = 0;
+  __syncthreads();
+  for (int c0 = 0; c0 < chunks; c0 += NT / 16) {
+    const int c = c0 + tid / 16, at = c * KC + l16 * 8;
+    float v[8];
+    load8(row + at, c < chunks && at < k, v);
+    bool out;
+    float mine = leave_out<16 / GPC>(v, out);
+    if (out) atomicOr(&s_mask, 1u << ((c * GPC + l16 / (16 / GPC)) / span));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if (tid % 32 == 0) atomicMax(&s_top, __float_as_int(mine));
   }
   __syncthreads();
-
-  float acc[2][C8][4];
+  const int sh = shift_of(__int_as_float(s_top));
+  uint8_t* base = ws + (tok / MP) * (long long)chunks * S::block(GPC);
+  for (int c0 = 0; c0 < chunks; c0 += NT / 16) {
+    const int c = c0 + tid / 16, at = c * KC + l16 * 8;
+    float v[8];
+    load8(row + at, c < chunks && at < k, v);
+    bool out;
+    leave_out<16 / GPC>(v, out);
+    // (whole warps: a warp's two chunks are both in range or its second is dropped after the shuffles)
+    uint8_t* block = base + (long long)min(c, chunks - 1) * S::block(GPC);
+    if (__all_sync(0xffffffffu, c < chunks)) {
+      stage8<T, S, GPC>(v, pow2(sh), block, (int)(tok % MP), l16);
+    } else if (__any_sync(0xffffffffu, c < chunks)) {
+      // the last, odd chunk: its lanes' twins write the same bytes
+      float u[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int c = 0; c < C8; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][c][e] = 0.f;
-
-  // a lane's columns (clamped: what a column without a token computes is not stored)
-  int xcol[C8];
-#pragma unroll
-  for (int c = 0; c < C8; ++c) xcol[c] = min(8 * c + g, cols - 1) * xpitch + t * 16;
-
-  for (int j = 0; j < steps; ++j) {
-    const int b = j / sx, jb = j - b * sx;
-    if (!a.resident && jb == 0) {
-      if (j > 0) {
-        store_x(b);
-        __syncthreads();
-      }
-      if ((b + 1) * sx < steps) fetch_x(b + 1);
+      for (int i = 0; i < 8; ++i) u[i] = __shfl_sync(0xffffffffu, v[i], l16);
+      stage8<T, S, GPC>(u, pow2(sh), base + (long long)(chunks - 1) * S::block(GPC), (int)(tok % MP), l16);
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    __syncwarp();
-    Scale<T> sc[GPC];
+  }
+  if (tid == 0) {
+    scales[tok] = pow2(-sh);
+    masks[tok] = s_mask;
+  }
+}
+
+// The terms of one output that leave_out zeroed, over the group that starts at input k0.
+template <typename T>
+__device__ __noinline__ float left_out(const Int4Args& a, const T* x, long long row, int k0, int group) {
+  const int k1 = min(k0 + group, a.k);
+  float top = 0.f;
+  for (int k = k0; k < k1; ++k) {
+    const float m = fabsf(to_f32(x[k]));
+    if (m <= FINITE) top = fmaxf(top, m);
+  }
+  int high = 0, low = 0;
+  for (int k = k0; k < k1; ++k) {
+    const float m = fabsf(to_f32(x[k]));
+    if (m <= FINITE) {
+      high += m >= top * APART;
+      low |= m < top * APART && m != 0.f;
+    }
+  }
+  const bool alone = low && high <= group / 16;
+  const long long at = (long long)(k0 / group) * a.n + row;
+  const float zero = a.z ? (float)a.z[at] : 8.f, scale = to_f32(static_cast<const T*>(a.s)[at]);
+  float v = 0.f;
+  for (int k = k0; k < k1; ++k) {
+    const float xv = to_f32(x[k]);
+    if (fabsf(xv) <= FINITE && !(alone && fabsf(xv) >= top * APART)) continue;
+    const uint8_t by = a.q[row * (a.k / 2) + k / 2];
+    v += xv * (((float)(k & 1 ? by >> 4 : by & 15) - zero) * scale);
+  }
+  return v;
+}
+
+// ------------------------------------------------------------------ TMEM and MMA
+__device__ __forceinline__ void mma_f8(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__host__ __device__ constexpr uint32_t idesc_f8(int n, int b_e5m2) {
+  return (1u << 4) | ((uint32_t)b_e5m2 << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t a, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// keeps the uses of loaded values behind the wait
+__device__ __forceinline__ void pin16(float* v) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+               "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
+
+struct Bars {
+  uint64_t wfull[SW], wempty[SW], afull[NA], aempty[NA], dfull[4], dempty[4], bfull[MAX_SB], bempty[MAX_SB], drain;
+};
+
+__device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done)
+               : "r"(tc::smem_addr(bar)), "r"(parity)
+               : "memory");
+  return done;
+}
+// One lane of a converged warp.  (With `lane == 0` instead, the MMAs' and copies' operands are
+// moved to uniform registers lane by lane: 114 clocks an MMA against 52.)
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p;
+}
+
+// Waits for completion number `it` (0, 1, ...) of a barrier.
+struct Waiter {
+  volatile int* fail;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t it) const {
+    if (ready(bar, it & 1) || (!*fail && tc::mbar_wait(bar, it & 1, POLLS))) return true;
+    *fail = 1;
+    atomicExch(&g_int4_status, 1);
+    return false;
+  }
+  // the same answer for a whole warp
+  __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t it) const {
+    return __all_sync(0xffffffffu, (*this)(bar, it));
+  }
+};
+
+template <typename T, int MP, int GPC>
+__global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constant__ CUtensorMap wmap, Int4Args a) {
+  using S = Shape<T, MP>;
+  constexpr int BLK = S::block(GPC), N = S::N, G = KC / GPC;
+  constexpr int A_COLS = 32 + 8 * GPC;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ Bars bar;
+  __shared__ uint32_t s_slot;
+  __shared__ int s_fail;
+  __shared__ int s_top[MP];
+  __shared__ uint32_t s_mask[MP];
+  __shared__ float s_scale[MP];
+  uint8_t* wst = smem;
+  uint8_t* bst = smem + SW * W_STAGE;
+  const int tid = threadIdx.x, lane = tid % 32, w = __shfl_sync(0xffffffffu, tid / 32, 0);
+  const int rank = a.ck > 1 ? blockIdx.x % a.ck : 0;
+  const int chunks = (a.k + KC - 1) / KC;
+  const int c0 = min(rank * a.per, chunks), c1 = min(c0 + a.per, chunks), nc = c1 - c0;
+  const int stages = (nc + 1) / 2;
+  const int unit0 = blockIdx.x / a.ck, units = a.tiles * a.ytiles, step = gridDim.x / a.ck;
+  const int span = ((a.staged ? chunks : a.per) * GPC + 31) / 32;     // groups per bit of a left-out mask
+
+  if (w == 1) tc::tmem_alloc(&s_slot, 512);
+  if (tid == 0) {
+    for (int i = 0; i < SW; ++i) tc::mbar_init(&bar.wfull[i], 1), tc::mbar_init(&bar.wempty[i], 8);
+    for (int i = 0; i < NA; ++i) tc::mbar_init(&bar.afull[i], 4), tc::mbar_init(&bar.aempty[i], 1);
+    for (int i = 0; i < 4; ++i) tc::mbar_init(&bar.dfull[i], 1), tc::mbar_init(&bar.dempty[i], 4);
+    for (int i = 0; i < a.sb; ++i) tc::mbar_init(&bar.bfull[i], 1), tc::mbar_init(&bar.bempty[i], 1);
+    tc::mbar_init(&bar.drain, 2);
+    tc::fence_mbar_init();
+    s_fail = 0;
+    // the first weights, before anything else
+    for (int i = 0; i < SW && i < stages; ++i) {
+      tc::mbar_expect_tx(&bar.wfull[i], W_STAGE);
+      tc::tma_load_2d(wst + i * W_STAGE, &wmap, (c0 + 2 * i) * (KC / 2), unit0 % a.tiles * ROWS, &bar.wfull[i]);
+    }
+  }
+  if (tid < MP) s_top[tid] = 0, s_mask[tid] = 0, s_scale[tid] = 0.f;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_slot, 0);
+  const Waiter wait{&s_fail};
+
+  if (!a.staged && nc > 0) {
+    // every thread stages the CTA's range of x: the tokens' largest inputs, then the pieces
+    const T* x = static_cast<const T*>(a.x);
+    const int toks = (int)a.m, total = toks * nc, l16 = tid % 16;
+    for (int u0 = 0; u0 < total; u0 += NT / 16) {
+      const int u = u0 + tid / 16, tok = u / nc, c = u - tok * nc, at = (c0 + c) * KC + l16 * 8;
+      float v[8];
+      load8(x + (long long)tok * a.ldx + at, u < total && at < a.k, v);
+      bool out;
+      float mine = leave_out<16 / GPC>(v, out);
+      if (out) atomicOr(&s_mask[tok], 1u << ((c * GPC + l16 / (16 / GPC)) / span));
 #pragma unroll
-    for (int i = 0; i < GPC; ++i) sc[i] = next[i];
-    if (j + 1 < steps) load_scales(j + 1);
-    if (rows_live && c0 + j * a.wk + wk < c1) {
-      const uint8_t* st = ring + (j % STAGES) * STAGE_BYTES + g * PITCH + t * 4;
-      const uint8_t* xb = xs + (a.resident ? 0 : (b & 1) * xbuf) + (jb * a.wk + wk) * KC * 2;
+      for (int o = 8; o > 0; o >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+      if (l16 == 0 && u < total) atomicMax(&s_top[tok], __float_as_int(mine));
+    }
+    __syncthreads();
+    for (int u0 = 0; u0 < total; u0 += NT / 16) {
+      const int u = u0 + tid / 16, tok = min(u / nc, toks - 1), c = u - u / nc * nc, at = (c0 + c) * KC + l16 * 8;
+      float v[8];
+      load8(x + (long long)tok * a.ldx + at, u < total && at < a.k, v);
+      bool out;
+      leave_out<16 / GPC>(v, out);
+      const int sh = shift_of(__int_as_float(s_top[tok]));
+      if (__all_sync(0xffffffffu, u < total)) {
+        stage8<T, S, GPC>(v, pow2(sh), bst + c * BLK, tok, l16);
+      } else if (__any_sync(0xffffffffu, u < total)) {     // the last, odd one: both halves of the warp write it
+        float d[8];
 #pragma unroll
-      for (int gi = 0; gi < GPC; ++gi) {
-        uint32_t zero[4];
-        float scale[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t v = __shfl_sync(0xffffffffu, sc[gi].v, 8 * r + g);
-          if constexpr (std::is_same<T, float>::value) {
-            scale[r] = __uint_as_float(v);
-            zero[r] = zero_pair<O>(__shfl_sync(0xffffffffu, sc[gi].zero, 8 * r + g));
-          } else {
-            scale[r] = std::is_same<T, __half>::value
-                           ? __half2float(__ushort_as_half((unsigned short)(v & 0xffffu)))
-                           : __uint_as_float(v << 16);
-            zero[r] = zero_pair<O>(v >> 16);
-          }
+        for (int i = 0; i < 8; ++i) d[i] = __shfl_sync(0xffffffffu, v[i], l16);
+        stage8<T, S, GPC>(d, pow2(shift_of(__int_as_float(s_top[toks - 1]))), bst + (nc - 1) * BLK, toks - 1, l16);
+      }
+    }
+    if (tid < toks) s_scale[tid] = pow2(-shift_of(__int_as_float(s_top[tid])));
+    tc::fence_proxy_async();
+    __syncthreads();
+  }
+
+  if (w == 0) {
+    if (elect()) {   // ---- weights
+      int it = 0;
+      bool ok = true;
+      for (int u = unit0; ok && u < units; u += step)
+        for (int i = 0; i < stages; ++i, ++it) {
+          if (it < SW && u == unit0) continue;             // loaded above
+          const int sl = it % SW;
+          if (it >= SW && !wait(&bar.wempty[sl], it / SW - 1)) { ok = false; break; }
+          tc::mbar_expect_tx(&bar.wfull[sl], W_STAGE);
+          tc::tma_load_2d(wst + sl * W_STAGE, &wmap, (c0 + 2 * i) * (KC / 2), u % a.tiles * ROWS, &bar.wfull[sl]);
         }
-        float part[2][C8][4];
+      // copies still in flight land before the CTA may exit
+      for (int j = it - SW < 0 ? 0 : it - SW; j < it; ++j) tc::mbar_wait(&bar.wfull[j % SW], j / SW & 1, POLLS);
+    }
+  } else if (w == 1) {
+    if (a.staged && elect()) {   // ---- staged x
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      int it = 0;
+      bool ok = true;
+      for (int u = unit0; ok && u < units && !(a.resident && u > unit0); u += step)
+        for (int c = 0; c < nc; ++c, ++it) {
+          const int sl = it % a.sb;
+          if (it >= a.sb && !wait(&bar.bempty[sl], it / a.sb - 1)) { ok = false; break; }
+          tc::mbar_expect_tx(&bar.bfull[sl], BLK);
+          tc::bulk_load(bst + sl * BLK, a.ws + ((long long)(u / a.tiles) * chunks + c0 + c) * BLK, BLK, &bar.bfull[sl]);
+        }
+      for (int j = it - a.sb < 0 ? 0 : it - a.sb; j < it; ++j)
+        tc::mbar_wait(&bar.bfull[j % a.sb], j / a.sb & 1, POLLS);
+    }
+  } else if (w < 4) {
+    // ---- MMAs: two warps, every other chunk each.  A chunk takes a thread 50 clocks an MMA and
+    // 100 a wait to issue, more than the chunk's share of time.
+    if (elect()) {
+      const int mine = w - 2;
+      int ia = 0;
+      bool ok = true;
+      for (int u = unit0; ok && u < units; u += step)
+        for (int c = 0; c < nc; ++c, ++ia) {
+          if (ia % 2 != mine) continue;
+          const int sl = a.resident ? c : ia % a.sb;
+          if (!wait(&bar.afull[ia % NA], ia / NA) ||
+              (a.staged && !wait(&bar.bfull[sl], a.resident ? 0 : ia / a.sb))) { ok = false; break; }
+          const uint32_t A = tmem + ia % NA * A_COLS;
+          const uint64_t B = tc::sdesc(tc::smem_addr(bst + sl * BLK), N * 16, 128);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+          for (int gi = 0; gi < GPC; ++gi) {
+            // each warp's accumulators are its own: it meets their every turn in order
+            const int i = ia / 2 * GPC + gi, e = mine * S::ND + i % S::ND, turn = i / S::ND;
+            if (turn > 0 && !wait(&bar.dempty[e], turn - 1)) { ok = false; break; }
+            tc::fence_after_sync();
+            const uint32_t D = tmem + D_COL + e * N;
 #pragma unroll
-          for (int c = 0; c < C8; ++c)
+            for (int p = 0; p < S::PASSES; ++p)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part[i][c][e] = 0.f;
+              for (int b = gi * (4 / GPC); b < (gi + 1) * (4 / GPC); ++b)
+                mma_f8(D, A + 8 * b, B + (uint64_t)((p * KC * N + b * 32 * N) >> 4), idesc_f8(N, p > 0),
+                       p > 0 || b > gi * (4 / GPC));
+            mma_f8(D, A + 32 + 8 * gi, B + (uint64_t)((S::PASSES * KC * N + gi * 32 * N) >> 4), idesc_f8(N, 1), true);
+            tc::commit(&bar.dfull[e]);
+          }
+          tc::commit(&bar.aempty[ia % NA]);
+          if (a.staged && !a.resident) tc::commit(&bar.bempty[sl]);
+        }
+      tc::commit(&bar.drain);        // every MMA issued is done before the TMEM goes
+      tc::mbar_wait(&bar.drain, 0, POLLS);
+    }
+  } else if (w >= 4 && w < 12) {
+    // ---- unpacking: set `half` takes that half of each weight stage; a thread is a row
+    const int half = (w - 4) / 4, r = w % 4 * 32 + lane;
+    const uint32_t at = tmem + ((uint32_t)(w % 4 * 32) << 16);
+    int it = 0, ia = 0;
+    bool ok = true;
+    uint32_t zc[8];
 #pragma unroll
-        for (int kb = 0; kb < 4 / GPC; ++kb) {
-          const int i = gi * (4 / GPC) + kb;     // 16-byte block of the chunk: 32 inputs
-          uint4 xf[C8];
+    for (int i = 0; i < 8; ++i) zc[i] = 0x88888888u;
+    for (int u = unit0; ok && u < units; u += step, ia += nc) {
+      const long long row = (long long)(u % a.tiles) * ROWS + r;
+      const uint8_t* zp = a.z && row < a.n ? a.z + row : nullptr;
+      const int groups = (a.k + G - 1) / G;
+      uint8_t zn[GPC];
+      auto load_zeros = [&](int c) {
 #pragma unroll
-          for (int c = 0; c < C8; ++c) xf[c] = *reinterpret_cast<const uint4*>(xb + xcol[c] + i * 64);
+        for (int gi = 0; gi < GPC; ++gi) {
+          const int g = (c0 + c) * GPC + gi;
+          zn[gi] = zp && c < nc && g < groups ? __ldg(zp + (long long)g * a.n) : 8;
+        }
+      };
+      load_zeros(half);
+      for (int i = 0; i < stages; ++i, ++it) {
+        const int sl = it % SW, c = 2 * i + half, e = (ia + c) % NA, en = (ia + c) / NA;
+        if (!wait.warp(&bar.wfull[sl], it / SW)) { ok = false; break; }
+        if (c < nc) {
+          uint4 raw[4];
+          const uint8_t* src = wst + sl * W_STAGE + r * KC;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + mt * 16 * PITCH + i * 16);
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (mt * 16 + 8) * PITCH + i * 16);
-            const uint32_t z0 = zero[2 * mt], z1 = zero[2 * mt + 1];
-            const uint32_t a0[4] = {unpack<O>(w0, z0), unpack<O>(w1, z1), unpack<O>(w0 >> 4, z0),
-                                    unpack<O>(w1 >> 4, z1)};
-            const uint32_t a1[4] = {unpack<O>(w0 >> 8, z0), unpack<O>(w1 >> 8, z1), unpack<O>(w0 >> 12, z0),
-                                    unpack<O>(w1 >> 12, z1)};
+          for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + (((half * 4 + j) ^ (r & 7)) * 16));
+          if (en > 0 && !wait.warp(&bar.aempty[e], en - 1)) { ok = false; break; }
+          tc::fence_after_sync();
+          const uint32_t A = at + e * A_COLS;
 #pragma unroll
-            for (int c = 0; c < C8; ++c) {
-              mma<O>(part[mt][c], a0, xf[c].x, xf[c].y);
-              mma<O>(part[mt][c], a1, xf[c].z, xf[c].w);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t b[8] = {raw[j].x & 0x0f0f0f0fu, (raw[j].x >> 4) & 0x0f0f0f0fu,
+                                   raw[j].y & 0x0f0f0f0fu, (raw[j].y >> 4) & 0x0f0f0f0fu,
+                                   raw[j].z & 0x0f0f0f0fu, (raw[j].z >> 4) & 0x0f0f0f0fu,
+                                   raw[j].w & 0x0f0f0f0fu, (raw[j].w >> 4) & 0x0f0f0f0fu};
+            tmem_st8(A + 8 * j, b);
+          }
+          if (a.z || en == 0) {        // without zeros, -8 stays where the first round wrote it
+#pragma unroll
+            for (int gi = 0; gi < GPC; ++gi) {
+              if (a.z) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) zc[j] = (0x80u | zn[gi]) * 0x01010101u;
+              }
+              tmem_st8(A + 32 + 8 * gi, zc);
+            }
+            if (a.z) load_zeros(c + 2);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc::fence_before_sync();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(&bar.wempty[sl]);
+          if (c < nc) tc::mbar_arrive(&bar.afull[e]);
+        }
+      }
+    }
+  } else if (w >= 12) {
+    // ---- sums: a thread is an output row
+    const int r = w % 4 * 32 + lane;
+    const uint32_t at = tmem + D_COL + ((uint32_t)(w % 4 * 32) << 16);
+    const T* sp = static_cast<const T*>(a.s);
+    const int groups = (a.k + G - 1) / G, ng = nc * GPC;
+    if (a.staged) asm volatile("griddepcontrol.wait;" ::: "memory");
+    int ia = 0;
+    bool ok = true;
+    for (int u = unit0; ok && u < units; u += step, ia += nc) {
+      const long long row = (long long)(u % a.tiles) * ROWS + r, m0 = (long long)(u / a.tiles) * MP;
+      const int toks = (int)min((long long)MP, a.m - m0);
+      float acc[MP];
+#pragma unroll
+      for (int t = 0; t < MP; ++t) acc[t] = 0.f;
+      auto scale_of = [&](int g) {
+        const int gg = c0 * GPC + g;
+        return row < a.n && g < ng && gg < groups ? __ldg(sp + (long long)gg * a.n + row) : from_f32<T>(0.f);
+      };
+      T sq[4];                          // the scales of the next four groups, as loaded (a conversion would wait)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sq[i] = scale_of(i);
+      for (int g0 = 0; ok && g0 < ng; g0 += 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (g0 + i >= ng) break;
+          const int ca = ia + (g0 + i) / GPC, di = ca / 2 * GPC + (g0 + i) % GPC, e = ca % 2 * S::ND + di % S::ND;
+          if (!wait.warp(&bar.dfull[e], di / S::ND)) { ok = false; break; }
+          tc::fence_after_sync();
+          const uint32_t D = at + e * N;
+          const float s = to_f32(sq[i]);
+          sq[i] = scale_of(g0 + i + 4);
+          if constexpr (S::COLS) {
+            float d[N];
+#pragma unroll
+            for (int j = 0; j < N; j += 16) tmem_ld16_issue(D + j, d + j);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < N; j += 16) pin16(d + j);
+#pragma unroll
+            for (int t = 0; t < MP; ++t) {
+              float v = d[(S::P - 1) * MP + t];
+#pragma unroll
+              for (int p = S::P - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[p * MP + t]);
+              acc[t] = fmaf(s, v, acc[t]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < N; j += 32) {
+              float d[32];
+              tmem_ld16_issue(D + j, d);
+              tmem_ld16_issue(D + j + 16, d + 16);
+              tmem_wait_ld();
+              pin16(d);
+              pin16(d + 16);
+#pragma unroll
+              for (int t = 0; t < 32; ++t) acc[j + t] = fmaf(s, d[t], acc[j + t]);
+            }
+          }
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&bar.dempty[e]);
+        }
+      }
+      // the tile's outputs (or this CTA's part of them)
+      if (ok) {
+        const T* x = static_cast<const T*>(a.x);
+        const T* bias = static_cast<const T*>(a.bias);
+        float* red = reinterpret_cast<float*>(wst);
+#pragma unroll
+        for (int t = 0; t < MP; ++t) {
+          if (t < toks && (row < a.n || a.ck > 1)) {
+            const uint32_t mask = a.staged ? a.ws_mask[m0 + t] : s_mask[t];
+            float v = acc[t] * 512.f * (a.staged ? a.ws_scale[m0 + t] : s_scale[t]);
+            if (mask && row < a.n)
+              for (int g = 0; g < ng; ++g)
+                if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
+                  v += left_out<T>(a, x + (m0 + t) * a.ldx, row, (c0 * GPC + g) * G, G);
+            if (a.ck > 1) {
+              red[t * ROWS + r] = v;    // (all stages are consumed: every group's sum is in)
+            } else {
+              if (bias) v += to_f32(bias[row]);
+              const long long o = (m0 + t) * a.n + row;
+              if (a.out_f32) static_cast<float*>(a.y)[o] = v;
+              else static_cast<T*>(a.y)[o] = from_f32<T>(v);
             }
           }
         }
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int c = 0; c < C8; ++c) {
-            acc[mt][c][0] = fmaf(scale[2 * mt], part[mt][c][0], acc[mt][c][0]);
-            acc[mt][c][1] = fmaf(scale[2 * mt], part[mt][c][1], acc[mt][c][1]);
-            acc[mt][c][2] = fmaf(scale[2 * mt + 1], part[mt][c][2], acc[mt][c][2]);
-            acc[mt][c][3] = fmaf(scale[2 * mt + 1], part[mt][c][3], acc[mt][c][3]);
-          }
       }
     }
-    __syncwarp();                  // every lane has read the slot
-    load_stage(j + STAGES);
   }
-  tc::cp_async_wait_all();
+  tc::fence_before_sync();
   __syncthreads();
-
-  // ---- partial tiles [warp][column][row] over the rings, summed in a fixed order
-  float* red = reinterpret_cast<float*>(ws);
-  float* mine = red + w * 8 * C8 * RPITCH;
-#pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-    for (int c = 0; c < C8; ++c) {
-      float* d = mine + (8 * c + 2 * t) * RPITCH + 16 * mt + g;
-      d[0] = acc[mt][c][0];
-      d[RPITCH] = acc[mt][c][1];
-      d[8] = acc[mt][c][2];
-      d[RPITCH + 8] = acc[mt][c][3];
-    }
-  __syncthreads();
-  const int nrows = WARPS / a.wk * ROWS;
-  const int total = toks * nrows;
-  const T* bias = static_cast<const T*>(a.bias);
-  auto local = [&](const float* r, int tok, int row) {
-    float v = 0.f;
-    for (int i = 0; i < a.wk; ++i) {
-      const float* p = r + ((row / ROWS) * a.wk + i) * 8 * C8 * RPITCH + tok * PER_TOK * RPITCH + row % ROWS;
-#pragma unroll
-      for (int e = 0; e < PER_TOK; ++e) v += p[e * RPITCH];
-    }
-    return v;
-  };
-  auto write = [&](int tok, int row, float v) {
-    const long long r = tile0 + row;
-    if (r < a.n) {
-      v = v * up<T>() + (bias ? to_f32(bias[r]) : 0.f);
-      const long long at = (m0 + tok) * a.n + r;
-      if (a.out_f32) static_cast<float*>(a.y)[at] = v;
-      else static_cast<T*>(a.y)[at] = from_f32<T>(v);
-    }
-  };
-  if (a.ck == 1) {
-    for (int e = tid; e < total; e += NT) write(e / nrows, e % nrows, local(red, e / nrows, e % nrows));
-  } else {
+  if (w == 1) tc::tmem_dealloc(tmem, 512);
+  if (a.ck > 1) {
     cg::cluster_group cl = cg::this_cluster();
-    float* sum = reinterpret_cast<float*>(xs);      // the CTA's own tile [token][row]
-    for (int e = tid; e < total; e += NT) sum[e] = local(red, e / nrows, e % nrows);
     cl.sync();
+    const float* red = reinterpret_cast<const float*>(wst);
+    const T* bias = static_cast<const T*>(a.bias);
+    const long long row0 = (long long)(unit0 % a.tiles) * ROWS, m0 = (long long)(unit0 / a.tiles) * MP;
+    const int total = (int)min((long long)MP, a.m - m0) * ROWS;
     for (int e = rank * NT + tid; e < total; e += a.ck * NT) {
+      const long long row = row0 + e % ROWS;
+      if (row >= a.n) continue;
       float v = 0.f;
-      for (int i = 0; i < a.ck; ++i) v += cl.map_shared_rank(sum, i)[e];
-      write(e / nrows, e % nrows, v);
+      for (int i = 0; i < a.ck; ++i) v += cl.map_shared_rank(red, i)[e];
+      if (bias) v += to_f32(bias[row]);
+      const long long o = (m0 + e / ROWS) * a.n + row;
+      if (a.out_f32) static_cast<float*>(a.y)[o] = v;
+      else static_cast<T*>(a.y)[o] = from_f32<T>(v);
     }
     cl.sync();
   }
 }
 
-constexpr int SMS = 148;
-constexpr int SMEM_MAX = 112 * 1024;   // two CTAs an SM
+// ------------------------------------------------------------------ host
+int sm_count() {
+  static std::atomic<int> sms{0};
+  int v = sms.load(std::memory_order_relaxed);
+  if (v == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      v = 148;
+    sms.store(v, std::memory_order_relaxed);
+  }
+  return v;
+}
 
-template <typename T, int C8, int GPC>
-int launch(Int4Args a, cudaStream_t st) {
-  constexpr int PER_TOK = Op<T>::cols;
-  constexpr int TOK = 8 * C8 / PER_TOK;
-  auto kern = int4_linear_mma<T, C8, GPC>;
+// Sizes of a call; the same for the workspace query and the launch.
+struct Plan {
+  int tiles, ytiles, ck, per, staged, sb, resident;
+  size_t ws_blocks, ws_total;
+};
+
+template <typename T, int MP, int GPC>
+Plan plan(long long m, int n, int k) {
+  using S = Shape<T, MP>;
+  constexpr int BLK = S::block(GPC);
+  Plan p{};
+  const int chunks = (k + KC - 1) / KC;
+  p.tiles = (n + ROWS - 1) / ROWS;
+  p.ytiles = (int)((m + MP - 1) / MP);
+  const long long units = (long long)p.tiles * p.ytiles;
+  p.ck = 1;
+  while (p.ck < 8 && units * p.ck * 2 <= 148 && chunks >= p.ck * 4) p.ck *= 2;
+  p.per = (chunks + p.ck - 1) / p.ck;
+  if (p.ck > 1) p.per = (p.per + 1) / 2 * 2;
+  const bool fits = (long long)p.per * BLK <= B_SMEM && p.per <= MAX_SB;
+  // every CTA stages x itself while that is at most four rounds of its threads
+  p.staged = !(fits && p.ytiles == 1 && m * p.per * 16 <= 4 * NT);
+  p.resident = fits && p.ytiles == 1;
+  p.sb = p.resident ? (p.per > 0 ? p.per : 1) : (B_SMEM / BLK < 8 ? B_SMEM / BLK / 2 * 2 : 8);   // (even: each MMA warp has its own)
+  p.ws_blocks = align_up((size_t)p.ytiles * chunks * BLK, 256);
+  p.ws_total = p.staged ? p.ws_blocks + align_up((size_t)p.ytiles * MP * 8, 256) + 256 : 0;
+  return p;
+}
+
+int weight_map(CUtensorMap* map, const void* q, int n, int k) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tmap_encoder();
+  VERACE_REQUIRE(enc, VERACE_ERR_CUDA, "int4_linear: the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)k / 2, (cuuint64_t)n}, strides[1] = {(cuuint64_t)k / 2};
+  const cuuint32_t box[2] = {KC, ROWS}, el[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(q), dims, strides, box, el,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  VERACE_REQUIRE(r == CUDA_SUCCESS, VERACE_ERR_CUDA, "int4_linear: tensor map of n=%d k=%d refused (%d)", n, k, (int)r);
+  return VERACE_OK;
+}
+
+template <typename T, int MP, int GPC>
+int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
+  using S = Shape<T, MP>;
+  constexpr int BLK = S::block(GPC);
+  const Plan p = plan<T, MP, GPC>(a.m, a.n, a.k);
+  VERACE_REQUIRE(!p.staged || (workspace && ws_bytes >= p.ws_total), VERACE_ERR_WORKSPACE,
+                 "int4_linear: workspace of %zu bytes required, %zu given", p.ws_total, workspace ? ws_bytes : (size_t)0);
+  a.tiles = p.tiles; a.ytiles = p.ytiles; a.ck = p.ck; a.per = p.per;
+  a.staged = p.staged; a.sb = p.sb; a.resident = p.resident;
   const int chunks = (a.k + KC - 1) / KC;
-  const int tiles = (a.n + ROWS - 1) / ROWS;
-  const long long ytiles = (a.m + TOK - 1) / TOK;
-  // split k over warps, then over CTAs, while the device has room for more warps (16 an SM)
-  // and every warp keeps a chunk; a streamed buffer holds wk chunks of every column
-  int wk = 1, ck = 1;
-  while (wk * 2 * C8 <= 8 && wk * 2 <= chunks && (long long)tiles * ytiles * wk * 2 <= SMS * 16) wk *= 2;
-  while (ck < 8 && wk * ck * 4 <= chunks && (long long)tiles * ytiles * wk * ck * 2 <= SMS * 16) ck *= 2;
-  a.wk = wk;
-  a.ck = ck;
-  a.per = (chunks + ck - 1) / ck;
-  a.per = (a.per + wk - 1) / wk * wk;
-  const int nrows = WARPS / wk * ROWS;
-  const long long whole = 8LL * C8 * (a.per * KC * 2 + 64);
-  a.resident = whole <= 32768;
-  const int streamed = 2 * 8 * C8 * ((8 / C8) * KC * 2 + 64);
-  a.x_bytes = a.resident ? (int)whole : streamed;
-  if (ck > 1 && a.x_bytes < TOK * nrows * 4) a.x_bytes = TOK * nrows * 4;
-  a.x_bytes = (int)align_up(a.x_bytes, 128);
-  const int smem = a.x_bytes + WARPS * STAGES * STAGE_BYTES;
-  static_assert(WARPS * 8 * C8 * RPITCH * 4 <= WARPS * STAGES * STAGE_BYTES, "partial tiles fit the rings");
-  static_assert(32768 + 8192 + WARPS * STAGES * STAGE_BYTES <= SMEM_MAX, "x and the rings fit");
+  if (p.staged) {
+    uint8_t* base = reinterpret_cast<uint8_t*>(align_up((size_t)workspace, 256));
+    float* scales = reinterpret_cast<float*>(base + p.ws_blocks);
+    a.ws = base;
+    a.ws_scale = scales;
+    a.ws_mask = reinterpret_cast<uint32_t*>(scales + (size_t)p.ytiles * MP);
+    int4_stage_x<T, MP, GPC><<<(unsigned)a.m, NT, 0, st>>>(static_cast<const T*>(a.x), a.ldx, a.k, chunks, base, scales,
+                                                         const_cast<uint32_t*>(a.ws_mask));
+    const int rc = check_launch("int4_stage_x");
+    if (rc) return rc;
+  }
+  CUtensorMap map;
+  if (a.k > 0) {
+    const int rc = weight_map(&map, a.q, a.n, a.k);
+    if (rc) return rc;
+  }
+  auto kern = int4_linear_kernel<T, MP, GPC>;
+  const int smem = SW * W_STAGE + p.sb * BLK;
   static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
   int dev = 0;
   VERACE_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SW * W_STAGE + B_SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles * wk + WARPS - 1) / WARPS * ck), (unsigned)ytiles);
+  const int units = p.tiles * p.ytiles;
+  cfg.gridDim = dim3((unsigned)(p.ck > 1 ? units * p.ck : units < sm_count() ? units : sm_count()));
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ck;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (p.ck > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = p.ck;
+    attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  if (p.staged) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = ck > 1 ? 1 : 0;
-  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  cfg.numAttrs = na;
+  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, map, a));
   return check_launch("int4_linear");
 }
 
-template <typename T, int GPC>
-int by_columns(const Int4Args& a, cudaStream_t st) {
-  const long long cols = a.m * Op<T>::cols;
-  if (cols <= 8 / Op<T>::cols * Op<T>::cols) return launch<T, 1, GPC>(a, st);
-  if (cols <= 16 / Op<T>::cols * Op<T>::cols) return launch<T, 2, GPC>(a, st);
-  return launch<T, 4, GPC>(a, st);
-}
-
-template <typename T>
-int by_group(const Int4Args& a, int group, cudaStream_t st) {
-  if (group == 128) return by_columns<T, 1>(a, st);
-  if (group == 64) return by_columns<T, 2>(a, st);
-  return by_columns<T, 4>(a, st);
+// Calls f with the (type, tokens per tile, groups per chunk) of a problem.
+template <typename F>
+auto dispatch(long long m, int group, int dtype, F f) {
+  auto by_group = [&](auto t, auto mp) {
+    if (group == 128) return f(t, mp, std::integral_constant<int, 1>());
+    if (group == 64) return f(t, mp, std::integral_constant<int, 2>());
+    return f(t, mp, std::integral_constant<int, 4>());
+  };
+  auto by_tokens = [&](auto t) {
+    if (m <= 8) return by_group(t, std::integral_constant<int, 8>());
+    if (m <= 16) return by_group(t, std::integral_constant<int, 16>());
+    if (m <= 32) return by_group(t, std::integral_constant<int, 32>());
+    return by_group(t, std::integral_constant<int, 64>());
+  };
+  if (dtype == VERACE_F32) {
+    if (m <= 3) return by_group(float(), std::integral_constant<int, 3>());
+    if (m <= 8) return by_group(float(), std::integral_constant<int, 8>());
+    return by_group(float(), std::integral_constant<int, 16>());
+  }
+  if (dtype == VERACE_BF16) return by_tokens(__nv_bfloat16());
+  return by_tokens(__half());
 }
 
 }  // namespace
+
+int int4_read_status(int* status) {
+  int h = 0;
+  VERACE_CUDA(cudaMemcpyFromSymbol(&h, g_int4_status, sizeof(int)));
+  if (h) {
+    const int zero = 0;
+    VERACE_CUDA(cudaMemcpyToSymbol(g_int4_status, &zero, sizeof(int)));
+  }
+  *status = h;
+  return VERACE_OK;
+}
+
 }  // namespace verace
 
 using namespace verace;
 
+extern "C" size_t verace_int4_linear_workspace(long long m, int n, int k, int group, int dtype) {
+  if (m <= 0 || n <= 0 || k < 0 || k % 32 || (group != 32 && group != 64 && group != 128) || dtype < VERACE_F32 ||
+      dtype > VERACE_F16)
+    return 0;
+  return dispatch(m, group, dtype, [&](auto t, auto mp, auto gpc) {
+    return plan<decltype(t), decltype(mp)::value, decltype(gpc)::value>(m, n, k).ws_total;
+  });
+}
+
 extern "C" int verace_int4_linear(const void* x, long long ldx, const void* qweight, const void* scales,
                                   const void* zeros, const void* bias, void* y, long long m, int n, int k,
-                                  int group, int dtype, int out_dtype, void* stream) {
+                                  int group, int dtype, int out_dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   VERACE_REQUIRE(m >= 0 && n >= 0 && k >= 0, VERACE_ERR_INVALID, "int4_linear: negative size");
   VERACE_REQUIRE(dtype == VERACE_F32 || dtype == VERACE_BF16 || dtype == VERACE_F16, VERACE_ERR_INVALID,
                  "int4_linear: dtype %d", dtype);
@@ -502,13 +885,14 @@ extern "C" int verace_int4_linear(const void* x, long long ldx, const void* qwei
   const size_t esz = dtype == VERACE_F32 ? 4 : 2;
   VERACE_REQUIRE((size_t)x % 16 == 0 && ldx * esz % 16 == 0 && (size_t)qweight % 16 == 0, VERACE_ERR_INVALID,
                  "int4_linear: x rows and qweight must be 16-byte aligned");
-  VERACE_REQUIRE(m <= 65535LL * 8, VERACE_ERR_UNSUPPORTED, "int4_linear: m %lld too large", m);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  VERACE_REQUIRE(m <= 1LL << 20 && n <= 1 << 28 && (m + 2) / 3 * ((n + ROWS - 1) / ROWS) < 1LL << 30,
+                 VERACE_ERR_UNSUPPORTED, "int4_linear: m %lld, n %d too large", m, n);
   Int4Args a{};
   a.x = x; a.ldx = ldx; a.q = static_cast<const uint8_t*>(qweight); a.s = scales;
   a.z = static_cast<const uint8_t*>(zeros); a.bias = bias; a.y = y; a.m = m; a.n = n; a.k = k;
   a.out_f32 = out_dtype == VERACE_F32;
-  if (dtype == VERACE_F32) return by_group<float>(a, group, st);
-  if (dtype == VERACE_BF16) return by_group<__nv_bfloat16>(a, group, st);
-  return by_group<__half>(a, group, st);
+  return dispatch(m, group, dtype, [&](auto t, auto mp, auto gpc) {
+    return launch<decltype(t), decltype(mp)::value, decltype(gpc)::value>(a, workspace, workspace_bytes,
+                                                                          static_cast<cudaStream_t>(stream));
+  });
 }

@@ -79,9 +79,13 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     assert qweight.device == dev and scales.device == dev and (zeros is None or zeros.device == dev) \
         and (bias is None or bias.device == dev), "all tensors must be on one device"
     y = torch.empty((m, n), dtype=odt, device=dev)
-    rc = launch(dev, lib().verace_int4_linear, x2.data_ptr(), x2.stride(0) if m > 1 else k, qweight.data_ptr(),
+    L = lib()
+    nws = L.verace_int4_linear_workspace(m, n, k, group_size, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    rc = launch(dev, L.verace_int4_linear, x2.data_ptr(), x2.stride(0) if m > 1 else k, qweight.data_ptr(),
                 scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
-                None if bias is None else bias.data_ptr(), y.data_ptr(), m, n, k, group_size, code, _DTYPE[odt])
+                None if bias is None else bias.data_ptr(), y.data_ptr(), m, n, k, group_size, code, _DTYPE[odt],
+                None if ws is None else ws.data_ptr(), nws)
     if rc:
         check(rc, "verace_int4_linear")
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
