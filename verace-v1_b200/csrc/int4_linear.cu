@@ -24,10 +24,11 @@
 // there, so those inputs (and infinities and NaN) are left out of the pieces and added one by
 // one as (q - z) x s at the end (rare).
 //
-// One CTA per SM, 128 output rows at a time, 16 warps: one feeds the weights by TMA (128 rows x
+// One CTA per SM, 128 output rows at a time, 20 warps: one feeds the weights by TMA (128 rows x
 // 256 codes a stage, 128-byte swizzle: a row's thread reads 16 bytes without bank conflicts),
 // one the staged x, two issue the MMAs, eight unpack codes into TMEM (the MMA's A operand; two
-// sets of four take a stage's halves), four hold the rows' sums.  Few row tiles: k is split over
+// sets of four take a chunk's halves), eight hold the rows' sums (two sets: half of the tokens
+// each).  Every role is a chain of short dependent steps, hence the two of each.  Few row tiles: k is split over
 // a cluster and the partial sums are joined through distributed shared memory in rank order.
 #include "common.cuh"
 #include "tc.cuh"
@@ -48,30 +49,32 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr uint32_t POLLS = 1u << 22;
-constexpr int NT = 512;                  // threads: 16 warps
+constexpr int NT = 640;                  // threads: 20 warps
 constexpr int ROWS = 128;                // output rows per tile
-constexpr int KC = 128;                  // inputs per chunk
-constexpr int SW = 5;                    // weight stages of two chunks
-constexpr int W_STAGE = ROWS * KC;       // bytes: 128 rows x 256 codes
-constexpr int NA = 4;                    // A operands (one chunk each) in TMEM
+constexpr int KC = 256;                  // inputs per chunk
+constexpr int SW = 5;                    // weight stages of one chunk
+constexpr int W_STAGE = ROWS * KC / 2;   // bytes: 128 rows x 256 codes
 constexpr int D_COL = 256;               // first TMEM column of the accumulators
-constexpr int MAX_SB = 64;
+constexpr int MAX_SB = 32;
 constexpr int B_SMEM = 136 * 1024;
 constexpr float FINITE = 3.4028235e38f;
 constexpr float APART = 1.f / 4096.f;
 
 // How a token tile's x is laid out.  MP tokens per tile; COLS: the pieces in columns of their own.
-template <typename T, int MP_>
+// GPC: groups per chunk.
+template <typename T, int MP_, int GPC_>
 struct Shape {
   static constexpr bool IS32 = std::is_same<T, float>::value;
-  static constexpr int MP = MP_;
+  static constexpr int MP = MP_, GPC = GPC_;
   static constexpr bool COLS = IS32 || MP <= (std::is_same<T, __half>::value ? 16 : 32);
   static constexpr int P = IS32 ? 5 : std::is_same<T, __half>::value ? 3 : 2;    // pieces
   static constexpr int N = COLS ? (P * MP + 15) / 16 * 16 : MP;                  // MMA columns
   static constexpr int PASSES = COLS ? 1 : P;
   static constexpr int ND = 128 / N < 2 ? 1 : 2;                                 // accumulators per MMA warp
-  // bytes of a chunk's B operands: the passes' [128 / 16][N][16], then per group the zeros' [2][N][16]
-  static constexpr int block(int gpc) { return PASSES * KC * N + gpc * 32 * N; }
+  static constexpr int A_COLS = KC / 4 + 8 * GPC;                                // TMEM columns of a chunk's A
+  static constexpr int NA = 256 / A_COLS;
+  // bytes of a chunk's B operands: the passes' [256 / 16][N][16], then per group the zeros' [2][N][16]
+  static constexpr int BLK = PASSES * KC * N + GPC * 32 * N;
 };
 
 struct Int4Args {
@@ -156,18 +159,18 @@ __device__ __forceinline__ int shift_of(float top) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// Writes the pieces of lane l16's eight inputs of a chunk (token row t of the tile) and, from a
-// group's first lane, X.  A word's codes 0, 2, 4, 6 unpack before 1, 3, 5, 7, and so do x's bytes.
-template <typename T, typename S, int GPC>
-__device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* block, int t, int l16) {
-  constexpr int LANES = 16 / GPC;
+// Writes the pieces of a lane's eight inputs of a chunk (token row t of the tile; a warp holds the
+// chunk) and, from a group's first lane, X.  A word's codes 0, 2, 4, 6 unpack before 1, 3, 5, 7, and so do x's bytes.
+template <typename T, typename S>
+__device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* block, int t, int lane) {
+  constexpr int LANES = 32 / S::GPC;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= scale, sum += v[i];
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   constexpr int at[4][2] = {{0, 2}, {4, 6}, {1, 3}, {5, 7}};
-  uint8_t* d = block + ((l16 / 2) * S::N + t) * 16 + (l16 % 2) * 8;
+  uint8_t* d = block + ((lane / 2) * S::N + t) * 16 + (lane % 2) * 8;
   auto put = [&](int p, const uint32_t (&b)[4]) {
     uint8_t* to = d + (S::COLS ? p * S::MP * 16 : p * KC * S::N);
     *reinterpret_cast<uint2*>(to) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
@@ -211,7 +214,7 @@ __device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* bloc
       put(p, b);
     }
   }
-  if (l16 % LANES == 0) {
+  if (lane % LANES == 0) {
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int p = 0; p < 6; ++p) {
@@ -220,7 +223,7 @@ __device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* bloc
       const __half_raw r = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E5M2);
       sum -= __half2float(*reinterpret_cast<const __half*>(&r));
     }
-    uint4* z = reinterpret_cast<uint4*>(block + S::PASSES * KC * S::N + (l16 / LANES) * 32 * S::N) + t;
+    uint4* z = reinterpret_cast<uint4*>(block + S::PASSES * KC * S::N + (lane / LANES) * 32 * S::N) + t;
     z[0] = make_uint4(w[0], w[1], 0, 0);
     z[S::N] = make_uint4(0, 0, 0, 0);
     if constexpr (S::COLS) {
@@ -230,52 +233,42 @@ __device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* bloc
   }
 }
 
-// The staging kernel: one CTA per token.
-template <typename T, int MP, int GPC>
-__global__ void __launch_bounds__(NT) int4_stage_x(const T* __restrict__ x, long long ldx, int k, int chunks,
-                                                   uint8_t* __restrict__ ws, float* __restrict__ scales,
-                                                   uint32_t* __restrict__ masks) {
-  using S = Shape<T, MP>;
+// The staging kernel: one CTA per token, a warp per chunk.
+constexpr int STAGE_NT = 512;
+template <typename T, typename S>
+__global__ void __launch_bounds__(STAGE_NT) int4_stage_x(const T* __restrict__ x, long long ldx, int k, int chunks,
+                                                         uint8_t* __restrict__ ws, float* __restrict__ scales,
+                                                         uint32_t* __restrict__ masks) {
+  constexpr int LANES = 32 / S::GPC;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int s_top;
   __shared__ uint32_t s_mask;
-  const int tid = threadIdx.x, l16 = tid % 16;
+  const int tid = threadIdx.x, lane = tid % 32;
   const long long tok = blockIdx.x;
   const T* row = x + tok * ldx;
-  const int span = (chunks * GPC + 31) / 32;
+  const int span = (chunks * S::GPC + 31) / 32;
   if (tid == 0) s_top = 0, s_mask = 0;
   __syncthreads();
-  for (int c0 = 0; c0 < chunks; c0 += NT / 16) {
-    const int c = c0 + tid / 16, at = c * KC + l16 * 8;
+  float most = 0.f;
+  for (int c = tid / 32; c < chunks; c += STAGE_NT / 32) {
+    const int at = c * KC + lane * 8;
     float v[8];
-    load8(row + at, c < chunks && at < k, v);
+    load8(row + at, at < k, v);
     bool out;
-    float mine = leave_out<16 / GPC>(v, out);
-    if (out) atomicOr(&s_mask, 1u << ((c * GPC + l16 / (16 / GPC)) / span));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-    if (tid % 32 == 0) atomicMax(&s_top, __float_as_int(mine));
+    most = fmaxf(most, leave_out<LANES>(v, out));
+    if (out) atomicOr(&s_mask, 1u << ((c * S::GPC + lane / LANES) / span));
   }
+  atomicMax(&s_top, __reduce_max_sync(0xffffffffu, __float_as_int(most)));
   __syncthreads();
   const int sh = shift_of(__int_as_float(s_top));
-  uint8_t* base = ws + (tok / MP) * (long long)chunks * S::block(GPC);
-  for (int c0 = 0; c0 < chunks; c0 += NT / 16) {
-    const int c = c0 + tid / 16, at = c * KC + l16 * 8;
+  uint8_t* block = ws + (tok / S::MP) * (long long)chunks * S::BLK;
+  for (int c = tid / 32; c < chunks; c += STAGE_NT / 32) {
+    const int at = c * KC + lane * 8;
     float v[8];
-    load8(row + at, c < chunks && at < k, v);
+    load8(row + at, at < k, v);
     bool out;
-    leave_out<16 / GPC>(v, out);
-    // (whole warps: a warp's two chunks are both in range or its second is dropped after the shuffles)
-    uint8_t* block = base + (long long)min(c, chunks - 1) * S::block(GPC);
-    if (__all_sync(0xffffffffu, c < chunks)) {
-      stage8<T, S, GPC>(v, pow2(sh), block, (int)(tok % MP), l16);
-    } else if (__any_sync(0xffffffffu, c < chunks)) {
-      // the last, odd chunk: its lanes' twins write the same bytes
-      float u[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = __shfl_sync(0xffffffffu, v[i], l16);
-      stage8<T, S, GPC>(u, pow2(sh), base + (long long)(chunks - 1) * S::block(GPC), (int)(tok % MP), l16);
-    }
+    leave_out<LANES>(v, out);
+    stage8<T, S>(v, pow2(sh), block + (long long)c * S::BLK, (int)(tok % S::MP), lane);
   }
   if (tid == 0) {
     scales[tok] = pow2(-sh);
@@ -329,22 +322,48 @@ __device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* r) {
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void tmem_ld16_issue(uint32_t a, float* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-      : "r"(a));
+// Issues the load of n consecutive columns of this thread's lane; pin() keeps the uses behind the wait.
+template <int n>
+__device__ __forceinline__ void tmem_ld(uint32_t a, float* v) {
+  static_assert(n == 2 || n == 4 || n == 8 || n == 16 || n == 32, "columns");
+  if constexpr (n == 2) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(a));
+  } else if constexpr (n == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(a));
+  } else if constexpr (n == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(a));
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; i += 16)
+      asm volatile(
+          "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+          : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]), "=f"(v[i + 4]), "=f"(v[i + 5]),
+            "=f"(v[i + 6]), "=f"(v[i + 7]), "=f"(v[i + 8]), "=f"(v[i + 9]), "=f"(v[i + 10]), "=f"(v[i + 11]),
+            "=f"(v[i + 12]), "=f"(v[i + 13]), "=f"(v[i + 14]), "=f"(v[i + 15])
+          : "r"(a + i));
+  }
+}
+template <int n>
+__device__ __forceinline__ void pin(float* v) {
+#pragma unroll
+  for (int i = 0; i < n; i += 2) asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// keeps the uses of loaded values behind the wait
-__device__ __forceinline__ void pin16(float* v) {
-  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-               "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
-}
-
 struct Bars {
-  uint64_t wfull[SW], wempty[SW], afull[NA], aempty[NA], dfull[4], dempty[4], bfull[MAX_SB], bempty[MAX_SB], drain;
+  uint64_t wfull[SW], wempty[SW], afull[3], aempty[3], dfull[4], dempty[4], bfull[MAX_SB], bempty[MAX_SB], drain;
+};
+
+// A place in a ring of barriers, and the parity of the completion awaited there: `phase` for one
+// that fills, phase ^ 1 for one that empties (which passes on the first turn).
+struct Turn {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++slot == n) slot = 0, phase ^= 1;
+  }
 };
 
 __device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
@@ -355,34 +374,30 @@ __device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
                : "memory");
   return done;
 }
-// One lane of a converged warp.  (With `lane == 0` instead, the MMAs' and copies' operands are
-// moved to uniform registers lane by lane: 114 clocks an MMA against 52.)
+// One lane of a converged warp.
 __device__ __forceinline__ bool elect() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p;
 }
 
-// Waits for completion number `it` (0, 1, ...) of a barrier.
 struct Waiter {
   volatile int* fail;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t it) const {
-    if (ready(bar, it & 1) || (!*fail && tc::mbar_wait(bar, it & 1, POLLS))) return true;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    if (ready(bar, parity) || (!*fail && tc::mbar_wait(bar, parity, POLLS))) return true;
     *fail = 1;
     atomicExch(&g_int4_status, 1);
     return false;
   }
   // the same answer for a whole warp
-  __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t it) const {
-    return __all_sync(0xffffffffu, (*this)(bar, it));
+  __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
+    return __all_sync(0xffffffffu, (*this)(bar, parity));
   }
 };
 
-template <typename T, int MP, int GPC>
+template <typename T, typename S>
 __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constant__ CUtensorMap wmap, Int4Args a) {
-  using S = Shape<T, MP>;
-  constexpr int BLK = S::block(GPC), N = S::N, G = KC / GPC;
-  constexpr int A_COLS = 32 + 8 * GPC;
+  constexpr int BLK = S::BLK, N = S::N, MP = S::MP, GPC = S::GPC, G = KC / GPC, KB = 8 / GPC;   // KB: k blocks a group
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bar;
   __shared__ uint32_t s_slot;
@@ -390,69 +405,67 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
   __shared__ int s_top[MP];
   __shared__ uint32_t s_mask[MP];
   __shared__ float s_scale[MP];
+  __shared__ float s_scales[8][MP];            // of the token tile at hand, a copy for each summing warp
+  __shared__ uint32_t s_masks[8][MP];
   uint8_t* wst = smem;
   uint8_t* bst = smem + SW * W_STAGE;
   const int tid = threadIdx.x, lane = tid % 32, w = __shfl_sync(0xffffffffu, tid / 32, 0);
   const int rank = a.ck > 1 ? blockIdx.x % a.ck : 0;
   const int chunks = (a.k + KC - 1) / KC;
-  const int c0 = min(rank * a.per, chunks), c1 = min(c0 + a.per, chunks), nc = c1 - c0;
-  const int stages = (nc + 1) / 2;
+  const int c0 = min(rank * a.per, chunks), nc = min(a.per, chunks - c0);
   const int unit0 = blockIdx.x / a.ck, units = a.tiles * a.ytiles, step = gridDim.x / a.ck;
   const int span = ((a.staged ? chunks : a.per) * GPC + 31) / 32;     // groups per bit of a left-out mask
 
   if (w == 1) tc::tmem_alloc(&s_slot, 512);
   if (tid == 0) {
     for (int i = 0; i < SW; ++i) tc::mbar_init(&bar.wfull[i], 1), tc::mbar_init(&bar.wempty[i], 8);
-    for (int i = 0; i < NA; ++i) tc::mbar_init(&bar.afull[i], 4), tc::mbar_init(&bar.aempty[i], 1);
-    for (int i = 0; i < 4; ++i) tc::mbar_init(&bar.dfull[i], 1), tc::mbar_init(&bar.dempty[i], 4);
-    for (int i = 0; i < a.sb; ++i) tc::mbar_init(&bar.bfull[i], 1), tc::mbar_init(&bar.bempty[i], 1);
+    for (int i = 0; i < S::NA; ++i) tc::mbar_init(&bar.afull[i], 8), tc::mbar_init(&bar.aempty[i], 2);
+    for (int i = 0; i < 4; ++i) tc::mbar_init(&bar.dfull[i], 1), tc::mbar_init(&bar.dempty[i], 8);
+    for (int i = 0; i < a.sb; ++i) tc::mbar_init(&bar.bfull[i], 1), tc::mbar_init(&bar.bempty[i], 2);
     tc::mbar_init(&bar.drain, 2);
     tc::fence_mbar_init();
     s_fail = 0;
     // the first weights, before anything else
-    for (int i = 0; i < SW && i < stages; ++i) {
+    for (int i = 0; i < SW && i < nc; ++i) {
       tc::mbar_expect_tx(&bar.wfull[i], W_STAGE);
-      tc::tma_load_2d(wst + i * W_STAGE, &wmap, (c0 + 2 * i) * (KC / 2), unit0 % a.tiles * ROWS, &bar.wfull[i]);
+      tc::tma_load_2d(wst + i * W_STAGE, &wmap, (c0 + i) * (KC / 2), unit0 % a.tiles * ROWS, &bar.wfull[i]);
     }
   }
   if (tid < MP) s_top[tid] = 0, s_mask[tid] = 0, s_scale[tid] = 0.f;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, s_slot, 0);
+  // all 512 columns are this CTA's, so they start at column 0 (addresses without the base stay
+  // in uniform registers)
   const Waiter wait{&s_fail};
+  if (tid == 0 && s_slot != 0) {
+    s_fail = 1;
+    atomicExch(&g_int4_status, 1);
+  }
 
   if (!a.staged && nc > 0) {
-    // every thread stages the CTA's range of x: the tokens' largest inputs, then the pieces
-    const T* x = static_cast<const T*>(a.x);
-    const int toks = (int)a.m, total = toks * nc, l16 = tid % 16;
-    for (int u0 = 0; u0 < total; u0 += NT / 16) {
-      const int u = u0 + tid / 16, tok = u / nc, c = u - tok * nc, at = (c0 + c) * KC + l16 * 8;
+    // every warp stages the CTA's range of x: the tokens' largest inputs, then the pieces
+    constexpr int LANES = 32 / GPC;
+    const T* x = static_cast<const T*>(a.x) + c0 * KC + lane * 8;
+    const int toks = (int)a.m, total = toks * nc;
+    for (int u = w; u < total; u += NT / 32) {
+      const int tok = u / nc, c = u - tok * nc;
       float v[8];
-      load8(x + (long long)tok * a.ldx + at, u < total && at < a.k, v);
+      load8(x + (long long)tok * a.ldx + c * KC, (c0 + c) * KC + lane * 8 < a.k, v);
       bool out;
-      float mine = leave_out<16 / GPC>(v, out);
-      if (out) atomicOr(&s_mask[tok], 1u << ((c * GPC + l16 / (16 / GPC)) / span));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-      if (l16 == 0 && u < total) atomicMax(&s_top[tok], __float_as_int(mine));
+      const float most = leave_out<LANES>(v, out);
+      if (out) atomicOr(&s_mask[tok], 1u << ((c * GPC + lane / LANES) / span));
+      const int m = __reduce_max_sync(0xffffffffu, __float_as_int(most));
+      if (lane == 0) atomicMax(&s_top[tok], m);
     }
     __syncthreads();
-    for (int u0 = 0; u0 < total; u0 += NT / 16) {
-      const int u = u0 + tid / 16, tok = min(u / nc, toks - 1), c = u - u / nc * nc, at = (c0 + c) * KC + l16 * 8;
+    for (int u = w; u < total; u += NT / 32) {
+      const int tok = u / nc, c = u - tok * nc;
       float v[8];
-      load8(x + (long long)tok * a.ldx + at, u < total && at < a.k, v);
+      load8(x + (long long)tok * a.ldx + c * KC, (c0 + c) * KC + lane * 8 < a.k, v);
       bool out;
-      leave_out<16 / GPC>(v, out);
-      const int sh = shift_of(__int_as_float(s_top[tok]));
-      if (__all_sync(0xffffffffu, u < total)) {
-        stage8<T, S, GPC>(v, pow2(sh), bst + c * BLK, tok, l16);
-      } else if (__any_sync(0xffffffffu, u < total)) {     // the last, odd one: both halves of the warp write it
-        float d[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = __shfl_sync(0xffffffffu, v[i], l16);
-        stage8<T, S, GPC>(d, pow2(shift_of(__int_as_float(s_top[toks - 1]))), bst + (nc - 1) * BLK, toks - 1, l16);
-      }
+      leave_out<LANES>(v, out);
+      stage8<T, S>(v, pow2(shift_of(__int_as_float(s_top[tok]))), bst + c * BLK, tok, lane);
     }
     if (tid < toks) s_scale[tid] = pow2(-shift_of(__int_as_float(s_top[tid])));
     tc::fence_proxy_async();
@@ -460,197 +473,205 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
   }
 
   if (w == 0) {
-    if (elect()) {   // ---- weights
+    // ---- weights
+    if (elect()) {
+      Turn tw;
       int it = 0;
       bool ok = true;
-      for (int u = unit0; ok && u < units; u += step)
-        for (int i = 0; i < stages; ++i, ++it) {
+      for (int u = unit0; ok && u < units; u += step) {
+        const int y = u % a.tiles * ROWS;
+        for (int c = 0; c < nc; ++c, ++it, tw.next(SW)) {
           if (it < SW && u == unit0) continue;             // loaded above
-          const int sl = it % SW;
-          if (it >= SW && !wait(&bar.wempty[sl], it / SW - 1)) { ok = false; break; }
-          tc::mbar_expect_tx(&bar.wfull[sl], W_STAGE);
-          tc::tma_load_2d(wst + sl * W_STAGE, &wmap, (c0 + 2 * i) * (KC / 2), u % a.tiles * ROWS, &bar.wfull[sl]);
+          if (!wait(&bar.wempty[tw.slot], tw.phase ^ 1)) { ok = false; break; }
+          tc::mbar_expect_tx(&bar.wfull[tw.slot], W_STAGE);
+          tc::tma_load_2d(wst + tw.slot * W_STAGE, &wmap, (c0 + c) * (KC / 2), y, &bar.wfull[tw.slot]);
         }
+      }
       // copies still in flight land before the CTA may exit
       for (int j = it - SW < 0 ? 0 : it - SW; j < it; ++j) tc::mbar_wait(&bar.wfull[j % SW], j / SW & 1, POLLS);
     }
   } else if (w == 1) {
-    if (a.staged && elect()) {   // ---- staged x
+    // ---- staged x
+    if (a.staged && elect()) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
+      Turn tb;
       int it = 0;
       bool ok = true;
-      for (int u = unit0; ok && u < units && !(a.resident && u > unit0); u += step)
-        for (int c = 0; c < nc; ++c, ++it) {
-          const int sl = it % a.sb;
-          if (it >= a.sb && !wait(&bar.bempty[sl], it / a.sb - 1)) { ok = false; break; }
-          tc::mbar_expect_tx(&bar.bfull[sl], BLK);
-          tc::bulk_load(bst + sl * BLK, a.ws + ((long long)(u / a.tiles) * chunks + c0 + c) * BLK, BLK, &bar.bfull[sl]);
+      for (int u = unit0; ok && u < units && !(a.resident && u > unit0); u += step) {
+        const uint8_t* src = a.ws + ((long long)(u / a.tiles) * chunks + c0) * BLK;
+        for (int c = 0; c < nc; ++c, ++it, tb.next(a.sb), src += BLK) {
+          if (!wait(&bar.bempty[tb.slot], tb.phase ^ 1)) { ok = false; break; }
+          tc::mbar_expect_tx(&bar.bfull[tb.slot], BLK);
+          tc::bulk_load(bst + tb.slot * BLK, src, BLK, &bar.bfull[tb.slot]);
         }
+      }
       for (int j = it - a.sb < 0 ? 0 : it - a.sb; j < it; ++j)
         tc::mbar_wait(&bar.bfull[j % a.sb], j / a.sb & 1, POLLS);
     }
   } else if (w < 4) {
-    // ---- MMAs: two warps, every other chunk each.  A chunk takes a thread 50 clocks an MMA and
-    // 100 a wait to issue, more than the chunk's share of time.
-    if (elect()) {
-      const int mine = w - 2;
-      int ia = 0;
-      bool ok = true;
-      for (int u = unit0; ok && u < units; u += step)
-        for (int c = 0; c < nc; ++c, ++ia) {
-          if (ia % 2 != mine) continue;
-          const int sl = a.resident ? c : ia % a.sb;
-          if (!wait(&bar.afull[ia % NA], ia / NA) ||
-              (a.staged && !wait(&bar.bfull[sl], a.resident ? 0 : ia / a.sb))) { ok = false; break; }
-          const uint32_t A = tmem + ia % NA * A_COLS;
-          const uint64_t B = tc::sdesc(tc::smem_addr(bst + sl * BLK), N * 16, 128);
+    // ---- MMAs: two warps, every other group each (an MMA takes a warp 33 clocks to issue, a wait
+    // 100).  The whole warp walks the loop, so that the operands sit in uniform registers.
+    const bool lead = elect();
+    const int mine = w - 2;
+    Turn ta, tb, td;
+    bool ok = true;
+    for (int u = unit0; ok && u < units; u += step) {
+      if (a.resident) tb.slot = 0;
+      for (int c = 0; c < nc; ++c) {
+        if (!wait.warp(&bar.afull[ta.slot], ta.phase) ||
+            (a.staged && !wait.warp(&bar.bfull[tb.slot], tb.phase))) { ok = false; break; }
+        const uint32_t A = ta.slot * S::A_COLS;
+        const uint64_t B = tc::sdesc(tc::smem_addr(bst + tb.slot * BLK), N * 16, 128);
 #pragma unroll
-          for (int gi = 0; gi < GPC; ++gi) {
-            // each warp's accumulators are its own: it meets their every turn in order
-            const int i = ia / 2 * GPC + gi, e = mine * S::ND + i % S::ND, turn = i / S::ND;
-            if (turn > 0 && !wait(&bar.dempty[e], turn - 1)) { ok = false; break; }
-            tc::fence_after_sync();
-            const uint32_t D = tmem + D_COL + e * N;
+        for (int gj = 0; gj < GPC / 2; ++gj) {
+          const int gi = 2 * gj + mine, e = mine * S::ND + td.slot;
+          if (!wait.warp(&bar.dempty[e], td.phase ^ 1)) { ok = false; break; }
+          tc::fence_after_sync();
+          const uint32_t D = D_COL + e * N, Ag = A + gi * (8 * KB);
+          const uint64_t Bg = B + (uint64_t)(gi * (KB * 32 * N >> 4));
+          if (lead) {
+            constexpr uint32_t first = idesc_f8(N, 0), rest = idesc_f8(N, 1);
 #pragma unroll
             for (int p = 0; p < S::PASSES; ++p)
 #pragma unroll
-              for (int b = gi * (4 / GPC); b < (gi + 1) * (4 / GPC); ++b)
-                mma_f8(D, A + 8 * b, B + (uint64_t)((p * KC * N + b * 32 * N) >> 4), idesc_f8(N, p > 0),
-                       p > 0 || b > gi * (4 / GPC));
-            mma_f8(D, A + 32 + 8 * gi, B + (uint64_t)((S::PASSES * KC * N + gi * 32 * N) >> 4), idesc_f8(N, 1), true);
+              for (int b = 0; b < KB; ++b)
+                mma_f8(D, Ag + 8 * b, Bg + (uint64_t)((p * KC * N + b * 32 * N) >> 4), p > 0 ? rest : first, p + b > 0);
+            mma_f8(D, A + KC / 4 + 8 * gi, B + (uint64_t)((S::PASSES * KC * N >> 4) + gi * (32 * N >> 4)), rest, true);
             tc::commit(&bar.dfull[e]);
           }
-          tc::commit(&bar.aempty[ia % NA]);
-          if (a.staged && !a.resident) tc::commit(&bar.bempty[sl]);
+          td.next(S::ND);
         }
+        if (lead) {
+          tc::commit(&bar.aempty[ta.slot]);
+          if (a.staged && !a.resident) tc::commit(&bar.bempty[tb.slot]);
+        }
+        ta.next(S::NA);
+        if (a.resident) ++tb.slot;
+        else tb.next(a.sb);
+      }
+    }
+    if (lead) {
       tc::commit(&bar.drain);        // every MMA issued is done before the TMEM goes
       tc::mbar_wait(&bar.drain, 0, POLLS);
     }
-  } else if (w >= 4 && w < 12) {
-    // ---- unpacking: set `half` takes that half of each weight stage; a thread is a row
+  } else if (w < 12) {
+    // ---- unpacking: two sets of four warps, a half of every chunk each; a thread is a row
     const int half = (w - 4) / 4, r = w % 4 * 32 + lane;
-    const uint32_t at = tmem + ((uint32_t)(w % 4 * 32) << 16);
-    int it = 0, ia = 0;
-    bool ok = true;
-    uint32_t zc[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) zc[i] = 0x88888888u;
-    for (int u = unit0; ok && u < units; u += step, ia += nc) {
+    const uint32_t at = ((uint32_t)(w % 4 * 32) << 16) + half * 32;
+    constexpr int GH = GPC / 2;        // groups per half
+    Turn tw, ta;
+    bool ok = true, fresh = true;
+    int seen = 0;
+    const int groups = (a.k + G - 1) / G;
+    for (int u = unit0; ok && u < units; u += step) {
       const long long row = (long long)(u % a.tiles) * ROWS + r;
-      const uint8_t* zp = a.z && row < a.n ? a.z + row : nullptr;
-      const int groups = (a.k + G - 1) / G;
-      uint8_t zn[GPC];
+      int g = c0 * GPC + half * GH;
+      const uint8_t* zp = a.z && row < a.n ? a.z + (long long)g * a.n + row : nullptr;
+      uint8_t zn[GH];
       auto load_zeros = [&](int c) {
 #pragma unroll
-        for (int gi = 0; gi < GPC; ++gi) {
-          const int g = (c0 + c) * GPC + gi;
-          zn[gi] = zp && c < nc && g < groups ? __ldg(zp + (long long)g * a.n) : 8;
-        }
+        for (int gi = 0; gi < GH; ++gi) zn[gi] = zp && c < nc && g + gi < groups ? __ldg(zp + (long long)gi * a.n) : 8;
+        g += GPC;
+        if (zp) zp += (long long)GPC * a.n;
       };
-      load_zeros(half);
-      for (int i = 0; i < stages; ++i, ++it) {
-        const int sl = it % SW, c = 2 * i + half, e = (ia + c) % NA, en = (ia + c) / NA;
-        if (!wait.warp(&bar.wfull[sl], it / SW)) { ok = false; break; }
-        if (c < nc) {
-          uint4 raw[4];
-          const uint8_t* src = wst + sl * W_STAGE + r * KC;
+      if (a.z) load_zeros(0);
+      for (int c = 0; c < nc; ++c) {
+        if (!wait.warp(&bar.wfull[tw.slot], tw.phase)) { ok = false; break; }
+        uint4 raw[4];
+        const uint8_t* src = wst + tw.slot * W_STAGE + r * (KC / 2);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + (((half * 4 + j) ^ (r & 7)) * 16));
-          if (en > 0 && !wait.warp(&bar.aempty[e], en - 1)) { ok = false; break; }
-          tc::fence_after_sync();
-          const uint32_t A = at + e * A_COLS;
+        for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + (((half * 4 + j) ^ (r & 7)) * 16));
+        if (!wait.warp(&bar.aempty[ta.slot], ta.phase ^ 1)) { ok = false; break; }
+        tc::fence_after_sync();
+        const uint32_t A = at + ta.slot * S::A_COLS;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t b[8] = {raw[j].x & 0x0f0f0f0fu, (raw[j].x >> 4) & 0x0f0f0f0fu,
-                                   raw[j].y & 0x0f0f0f0fu, (raw[j].y >> 4) & 0x0f0f0f0fu,
-                                   raw[j].z & 0x0f0f0f0fu, (raw[j].z >> 4) & 0x0f0f0f0fu,
-                                   raw[j].w & 0x0f0f0f0fu, (raw[j].w >> 4) & 0x0f0f0f0fu};
-            tmem_st8(A + 8 * j, b);
-          }
-          if (a.z || en == 0) {        // without zeros, -8 stays where the first round wrote it
-#pragma unroll
-            for (int gi = 0; gi < GPC; ++gi) {
-              if (a.z) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) zc[j] = (0x80u | zn[gi]) * 0x01010101u;
-              }
-              tmem_st8(A + 32 + 8 * gi, zc);
-            }
-            if (a.z) load_zeros(c + 2);
-          }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          tc::fence_before_sync();
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b[8] = {raw[j].x & 0x0f0f0f0fu, (raw[j].x >> 4) & 0x0f0f0f0fu,
+                                 raw[j].y & 0x0f0f0f0fu, (raw[j].y >> 4) & 0x0f0f0f0fu,
+                                 raw[j].z & 0x0f0f0f0fu, (raw[j].z >> 4) & 0x0f0f0f0fu,
+                                 raw[j].w & 0x0f0f0f0fu, (raw[j].w >> 4) & 0x0f0f0f0fu};
+          tmem_st8(A + 8 * j, b);
         }
+        if (a.z || fresh) {            // without zeros, -8 stays where the first round wrote it
+#pragma unroll
+          for (int gi = 0; gi < GH; ++gi) {
+            uint32_t zc[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) zc[j] = a.z ? (0x80u | zn[gi]) * 0x01010101u : 0x88888888u;
+            tmem_st8(A - half * 32 + KC / 4 + 8 * (half * GH + gi), zc);
+          }
+          if (a.z) load_zeros(c + 1);
+          if (++seen == S::NA) fresh = false;
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          tc::mbar_arrive(&bar.wempty[sl]);
-          if (c < nc) tc::mbar_arrive(&bar.afull[e]);
+          tc::mbar_arrive(&bar.wempty[tw.slot]);
+          tc::mbar_arrive(&bar.afull[ta.slot]);
         }
+        tw.next(SW);
+        ta.next(S::NA);
       }
     }
-  } else if (w >= 12) {
-    // ---- sums: a thread is an output row
-    const int r = w % 4 * 32 + lane;
-    const uint32_t at = tmem + D_COL + ((uint32_t)(w % 4 * 32) << 16);
-    const T* sp = static_cast<const T*>(a.s);
+  } else {
+    // ---- sums: two sets of four warps, half of the tokens each; a thread is an output row
+    constexpr int TH = MP / 2;
+    const int set = (w - 12) / 4, t0 = set * TH, r = w % 4 * 32 + lane;
+    const uint32_t at = D_COL + ((uint32_t)(w % 4 * 32) << 16) + t0;
     const int groups = (a.k + G - 1) / G, ng = nc * GPC;
     if (a.staged) asm volatile("griddepcontrol.wait;" ::: "memory");
-    int ia = 0;
+    Turn td;                            // a pair of groups: one accumulator of each MMA warp
     bool ok = true;
-    for (int u = unit0; ok && u < units; u += step, ia += nc) {
+    for (int u = unit0; ok && u < units; u += step) {
       const long long row = (long long)(u % a.tiles) * ROWS + r, m0 = (long long)(u / a.tiles) * MP;
       const int toks = (int)min((long long)MP, a.m - m0);
-      float acc[MP];
+      __syncwarp();
+      for (int t = lane; t < toks; t += 32) {
+        s_scales[w - 12][t] = a.staged ? a.ws_scale[m0 + t] : s_scale[t];
+        s_masks[w - 12][t] = a.staged ? a.ws_mask[m0 + t] : s_mask[t];
+      }
+      __syncwarp();
+      float acc[TH];
 #pragma unroll
-      for (int t = 0; t < MP; ++t) acc[t] = 0.f;
-      auto scale_of = [&](int g) {
-        const int gg = c0 * GPC + g;
-        return row < a.n && g < ng && gg < groups ? __ldg(sp + (long long)gg * a.n + row) : from_f32<T>(0.f);
-      };
+      for (int t = 0; t < TH; ++t) acc[t] = 0.f;
+      const T* sp = static_cast<const T*>(a.s) + (long long)c0 * GPC * a.n + row;
+      const int have = row < a.n ? min(ng, groups - c0 * GPC) : 0;
       T sq[4];                          // the scales of the next four groups, as loaded (a conversion would wait)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq[i] = scale_of(i);
+      for (int i = 0; i < 4; ++i) sq[i] = i < have ? __ldg(sp + (long long)i * a.n) : from_f32<T>(0.f);
+      sp += 4LL * a.n;
       for (int g0 = 0; ok && g0 < ng; g0 += 4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (g0 + i >= ng) break;
-          const int ca = ia + (g0 + i) / GPC, di = ca / 2 * GPC + (g0 + i) % GPC, e = ca % 2 * S::ND + di % S::ND;
-          if (!wait.warp(&bar.dfull[e], di / S::ND)) { ok = false; break; }
+          if (i % 2 == 0 && g0 + i >= ng) break;          // (ng is even)
+          const int e = i % 2 * S::ND + td.slot;
+          if (!wait.warp(&bar.dfull[e], td.phase)) { ok = false; break; }
           tc::fence_after_sync();
           const uint32_t D = at + e * N;
           const float s = to_f32(sq[i]);
-          sq[i] = scale_of(g0 + i + 4);
-          if constexpr (S::COLS) {
-            float d[N];
+          if (g0 + i + 4 < have) sq[i] = __ldg(sp + (long long)i * a.n);
+          else sq[i] = from_f32<T>(0.f);
+          constexpr int NP = S::COLS ? S::P : 1;          // columns of a token
+          float d[NP][TH];
 #pragma unroll
-            for (int j = 0; j < N; j += 16) tmem_ld16_issue(D + j, d + j);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < N; j += 16) pin16(d + j);
-#pragma unroll
-            for (int t = 0; t < MP; ++t) {
-              float v = d[(S::P - 1) * MP + t];
-#pragma unroll
-              for (int p = S::P - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[p * MP + t]);
-              acc[t] = fmaf(s, v, acc[t]);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < N; j += 32) {
-              float d[32];
-              tmem_ld16_issue(D + j, d);
-              tmem_ld16_issue(D + j + 16, d + 16);
-              tmem_wait_ld();
-              pin16(d);
-              pin16(d + 16);
-#pragma unroll
-              for (int t = 0; t < 32; ++t) acc[j + t] = fmaf(s, d[t], acc[j + t]);
-            }
-          }
+          for (int p = 0; p < NP; ++p) tmem_ld<TH>(D + p * MP, d[p]);
+          tmem_wait_ld();
           tc::fence_before_sync();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&bar.dempty[e]);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) pin<TH>(d[p]);
+#pragma unroll
+          for (int t = 0; t < TH; ++t) {
+            float v = d[NP - 1][t];
+#pragma unroll
+            for (int p = NP - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[p][t]);
+            acc[t] = fmaf(s, v, acc[t]);
+          }
+          if (i % 2) td.next(S::ND);
         }
+        sp += 4LL * a.n;
       }
       // the tile's outputs (or this CTA's part of them)
       if (ok) {
@@ -658,19 +679,20 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
         const T* bias = static_cast<const T*>(a.bias);
         float* red = reinterpret_cast<float*>(wst);
 #pragma unroll
-        for (int t = 0; t < MP; ++t) {
-          if (t < toks && (row < a.n || a.ck > 1)) {
-            const uint32_t mask = a.staged ? a.ws_mask[m0 + t] : s_mask[t];
-            float v = acc[t] * 512.f * (a.staged ? a.ws_scale[m0 + t] : s_scale[t]);
+        for (int t = 0; t < TH; ++t) {
+          const int tok = t0 + t;
+          if (tok < toks && (row < a.n || a.ck > 1)) {
+            const uint32_t mask = s_masks[w - 12][tok];
+            float v = acc[t] * 512.f * s_scales[w - 12][tok];
             if (mask && row < a.n)
               for (int g = 0; g < ng; ++g)
                 if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
-                  v += left_out<T>(a, x + (m0 + t) * a.ldx, row, (c0 * GPC + g) * G, G);
+                  v += left_out<T>(a, x + (m0 + tok) * a.ldx, row, (c0 * GPC + g) * G, G);
             if (a.ck > 1) {
-              red[t * ROWS + r] = v;    // (all stages are consumed: every group's sum is in)
+              red[tok * ROWS + r] = v;    // (all stages are consumed: every group's sum is in)
             } else {
               if (bias) v += to_f32(bias[row]);
-              const long long o = (m0 + t) * a.n + row;
+              const long long o = (m0 + tok) * a.n + row;
               if (a.out_f32) static_cast<float*>(a.y)[o] = v;
               else static_cast<T*>(a.y)[o] = from_f32<T>(v);
             }
@@ -681,7 +703,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (w == 1) tc::tmem_dealloc(tmem, 512);
+  if (w == 1) tc::tmem_dealloc(s_slot, 512);
   if (a.ck > 1) {
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
@@ -723,26 +745,23 @@ struct Plan {
   size_t ws_blocks, ws_total;
 };
 
-template <typename T, int MP, int GPC>
+template <typename T, typename S>
 Plan plan(long long m, int n, int k) {
-  using S = Shape<T, MP>;
-  constexpr int BLK = S::block(GPC);
   Plan p{};
   const int chunks = (k + KC - 1) / KC;
   p.tiles = (n + ROWS - 1) / ROWS;
-  p.ytiles = (int)((m + MP - 1) / MP);
+  p.ytiles = (int)((m + S::MP - 1) / S::MP);
   const long long units = (long long)p.tiles * p.ytiles;
   p.ck = 1;
-  while (p.ck < 8 && units * p.ck * 2 <= 148 && chunks >= p.ck * 4) p.ck *= 2;
+  while (p.ck < 8 && units * p.ck * 2 <= 148 && chunks >= p.ck * 2) p.ck *= 2;
   p.per = (chunks + p.ck - 1) / p.ck;
-  if (p.ck > 1) p.per = (p.per + 1) / 2 * 2;
-  const bool fits = (long long)p.per * BLK <= B_SMEM && p.per <= MAX_SB;
-  // every CTA stages x itself while that is at most four rounds of its threads
-  p.staged = !(fits && p.ytiles == 1 && m * p.per * 16 <= 4 * NT);
+  const bool fits = (long long)p.per * S::BLK <= B_SMEM && p.per <= MAX_SB;
+  // every CTA stages x itself while that is at most two rounds of its warps
+  p.staged = !(fits && p.ytiles == 1 && m * p.per <= 2 * NT / 32);
   p.resident = fits && p.ytiles == 1;
-  p.sb = p.resident ? (p.per > 0 ? p.per : 1) : (B_SMEM / BLK < 8 ? B_SMEM / BLK / 2 * 2 : 8);   // (even: each MMA warp has its own)
-  p.ws_blocks = align_up((size_t)p.ytiles * chunks * BLK, 256);
-  p.ws_total = p.staged ? p.ws_blocks + align_up((size_t)p.ytiles * MP * 8, 256) + 256 : 0;
+  p.sb = p.resident ? (p.per > 0 ? p.per : 1) : (B_SMEM / S::BLK < 8 ? B_SMEM / S::BLK : 8);
+  p.ws_blocks = align_up((size_t)p.ytiles * chunks * S::BLK, 256);
+  p.ws_total = p.staged ? p.ws_blocks + align_up((size_t)p.ytiles * S::MP * 8, 256) + 256 : 0;
   return p;
 }
 
@@ -750,7 +769,7 @@ int weight_map(CUtensorMap* map, const void* q, int n, int k) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tmap_encoder();
   VERACE_REQUIRE(enc, VERACE_ERR_CUDA, "int4_linear: the driver has no cuTensorMapEncodeTiled");
   const cuuint64_t dims[2] = {(cuuint64_t)k / 2, (cuuint64_t)n}, strides[1] = {(cuuint64_t)k / 2};
-  const cuuint32_t box[2] = {KC, ROWS}, el[2] = {1, 1};
+  const cuuint32_t box[2] = {KC / 2, ROWS}, el[2] = {1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(q), dims, strides, box, el,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -758,11 +777,10 @@ int weight_map(CUtensorMap* map, const void* q, int n, int k) {
   return VERACE_OK;
 }
 
-template <typename T, int MP, int GPC>
+template <typename T, typename S>
 int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
-  using S = Shape<T, MP>;
-  constexpr int BLK = S::block(GPC);
-  const Plan p = plan<T, MP, GPC>(a.m, a.n, a.k);
+  constexpr int BLK = S::BLK;
+  const Plan p = plan<T, S>(a.m, a.n, a.k);
   VERACE_REQUIRE(!p.staged || (workspace && ws_bytes >= p.ws_total), VERACE_ERR_WORKSPACE,
                  "int4_linear: workspace of %zu bytes required, %zu given", p.ws_total, workspace ? ws_bytes : (size_t)0);
   a.tiles = p.tiles; a.ytiles = p.ytiles; a.ck = p.ck; a.per = p.per;
@@ -773,8 +791,8 @@ int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
     float* scales = reinterpret_cast<float*>(base + p.ws_blocks);
     a.ws = base;
     a.ws_scale = scales;
-    a.ws_mask = reinterpret_cast<uint32_t*>(scales + (size_t)p.ytiles * MP);
-    int4_stage_x<T, MP, GPC><<<(unsigned)a.m, NT, 0, st>>>(static_cast<const T*>(a.x), a.ldx, a.k, chunks, base, scales,
+    a.ws_mask = reinterpret_cast<uint32_t*>(scales + (size_t)p.ytiles * S::MP);
+    int4_stage_x<T, S><<<(unsigned)a.m, STAGE_NT, 0, st>>>(static_cast<const T*>(a.x), a.ldx, a.k, chunks, base, scales,
                                                          const_cast<uint32_t*>(a.ws_mask));
     const int rc = check_launch("int4_stage_x");
     if (rc) return rc;
@@ -784,7 +802,7 @@ int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
     const int rc = weight_map(&map, a.q, a.n, a.k);
     if (rc) return rc;
   }
-  auto kern = int4_linear_kernel<T, MP, GPC>;
+  auto kern = int4_linear_kernel<T, S>;
   const int smem = SW * W_STAGE + p.sb * BLK;
   static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
   int dev = 0;
@@ -818,13 +836,15 @@ int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
   return check_launch("int4_linear");
 }
 
-// Calls f with the (type, tokens per tile, groups per chunk) of a problem.
+// Calls f with a problem's type and shape.
 template <typename F>
 auto dispatch(long long m, int group, int dtype, F f) {
   auto by_group = [&](auto t, auto mp) {
-    if (group == 128) return f(t, mp, std::integral_constant<int, 1>());
-    if (group == 64) return f(t, mp, std::integral_constant<int, 2>());
-    return f(t, mp, std::integral_constant<int, 4>());
+    using T = decltype(t);
+    constexpr int MP = decltype(mp)::value;
+    if (group == 128) return f(t, Shape<T, MP, 2>());
+    if (group == 64) return f(t, Shape<T, MP, 4>());
+    return f(t, Shape<T, MP, 8>());
   };
   auto by_tokens = [&](auto t) {
     if (m <= 8) return by_group(t, std::integral_constant<int, 8>());
@@ -833,7 +853,7 @@ auto dispatch(long long m, int group, int dtype, F f) {
     return by_group(t, std::integral_constant<int, 64>());
   };
   if (dtype == VERACE_F32) {
-    if (m <= 3) return by_group(float(), std::integral_constant<int, 3>());
+    if (m <= 4) return by_group(float(), std::integral_constant<int, 4>());
     if (m <= 8) return by_group(float(), std::integral_constant<int, 8>());
     return by_group(float(), std::integral_constant<int, 16>());
   }
@@ -862,8 +882,8 @@ extern "C" size_t verace_int4_linear_workspace(long long m, int n, int k, int gr
   if (m <= 0 || n <= 0 || k < 0 || k % 32 || (group != 32 && group != 64 && group != 128) || dtype < VERACE_F32 ||
       dtype > VERACE_F16)
     return 0;
-  return dispatch(m, group, dtype, [&](auto t, auto mp, auto gpc) {
-    return plan<decltype(t), decltype(mp)::value, decltype(gpc)::value>(m, n, k).ws_total;
+  return dispatch(m, group, dtype, [&](auto t, auto s) {
+    return plan<decltype(t), decltype(s)>(m, n, k).ws_total;
   });
 }
 
@@ -885,14 +905,13 @@ extern "C" int verace_int4_linear(const void* x, long long ldx, const void* qwei
   const size_t esz = dtype == VERACE_F32 ? 4 : 2;
   VERACE_REQUIRE((size_t)x % 16 == 0 && ldx * esz % 16 == 0 && (size_t)qweight % 16 == 0, VERACE_ERR_INVALID,
                  "int4_linear: x rows and qweight must be 16-byte aligned");
-  VERACE_REQUIRE(m <= 1LL << 20 && n <= 1 << 28 && (m + 2) / 3 * ((n + ROWS - 1) / ROWS) < 1LL << 30,
+  VERACE_REQUIRE(m <= 1LL << 20 && n <= 1 << 28 && (m + 3) / 4 * ((n + ROWS - 1) / ROWS) < 1LL << 30,
                  VERACE_ERR_UNSUPPORTED, "int4_linear: m %lld, n %d too large", m, n);
   Int4Args a{};
   a.x = x; a.ldx = ldx; a.q = static_cast<const uint8_t*>(qweight); a.s = scales;
   a.z = static_cast<const uint8_t*>(zeros); a.bias = bias; a.y = y; a.m = m; a.n = n; a.k = k;
   a.out_f32 = out_dtype == VERACE_F32;
-  return dispatch(m, group, dtype, [&](auto t, auto mp, auto gpc) {
-    return launch<decltype(t), decltype(mp)::value, decltype(gpc)::value>(a, workspace, workspace_bytes,
-                                                                          static_cast<cudaStream_t>(stream));
+  return dispatch(m, group, dtype, [&](auto t, auto s) {
+    return launch<decltype(t), decltype(s)>(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
   });
 }
