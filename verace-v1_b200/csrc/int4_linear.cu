@@ -48,7 +48,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t POLLS = 1u << 22;
+constexpr uint32_t POLLS = 1u << 16;     // of 64 polls each
 constexpr int NT = 640;                  // threads: 20 warps
 constexpr int ROWS = 128;                // output rows per tile
 constexpr int KC = 256;                  // inputs per chunk
@@ -70,7 +70,7 @@ struct Shape {
   static constexpr int P = IS32 ? 5 : std::is_same<T, __half>::value ? 3 : 2;    // pieces
   static constexpr int N = COLS ? (P * MP + 15) / 16 * 16 : MP;                  // MMA columns
   static constexpr int PASSES = COLS ? 1 : P;
-  static constexpr int ND = 128 / N < 2 ? 1 : 2;                                 // accumulators per MMA warp
+  static constexpr int ND = 128 / N < 2 ? 1 : 2;                                 // pairs of accumulators (one per MMA warp)
   static constexpr int A_COLS = KC / 4 + 8 * GPC;                                // TMEM columns of a chunk's A
   static constexpr int NA = 256 / A_COLS;
   // bytes of a chunk's B operands: the passes' [256 / 16][N][16], then per group the zeros' [2][N][16]
@@ -322,6 +322,16 @@ __device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* r) {
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 // Issues the load of n consecutive columns of this thread's lane; pin() keeps the uses behind the wait.
 template <int n>
 __device__ __forceinline__ void tmem_ld(uint32_t a, float* v) {
@@ -353,7 +363,7 @@ __device__ __forceinline__ void pin(float* v) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 struct Bars {
-  uint64_t wfull[SW], wempty[SW], afull[3], aempty[3], dfull[4], dempty[4], bfull[MAX_SB], bempty[MAX_SB], drain;
+  uint64_t wfull[SW], wempty[SW], afull[3], aempty[3], dfull[2], dempty[2], bfull[MAX_SB], bempty[MAX_SB], drain;
 };
 
 // A place in a ring of barriers, and the parity of the completion awaited there: `phase` for one
@@ -366,9 +376,9 @@ struct Turn {
   }
 };
 
-__device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(done)
                : "r"(tc::smem_addr(bar)), "r"(parity)
                : "memory");
@@ -381,17 +391,22 @@ __device__ __forceinline__ bool elect() {
   return p;
 }
 
+// Waits for a completion, but not for ever: when one does not come, the status word is set and no
+// wait of the CTA blocks any more.  The roles then run to their ends on whatever is there (every
+// address stays in range), the copies and MMAs in flight are waited for with the same bound, and
+// the TMEM is freed.
+__device__ __noinline__ void wait_longer(uint64_t* bar, uint32_t parity, volatile int* fail) {
+  for (uint32_t i = 0; i < POLLS; ++i) {
+    if (tc::mbar_wait(bar, parity, 64)) return;
+    if (*fail) return;
+  }
+  *fail = 1;
+  atomicExch(&g_int4_status, 1);
+}
 struct Waiter {
   volatile int* fail;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-    if (ready(bar, parity) || (!*fail && tc::mbar_wait(bar, parity, POLLS))) return true;
-    *fail = 1;
-    atomicExch(&g_int4_status, 1);
-    return false;
-  }
-  // the same answer for a whole warp
-  __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
-    return __all_sync(0xffffffffu, (*this)(bar, parity));
+  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) const {
+    if (!try_wait(bar, parity)) wait_longer(bar, parity, fail);
   }
 };
 
@@ -420,7 +435,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
   if (tid == 0) {
     for (int i = 0; i < SW; ++i) tc::mbar_init(&bar.wfull[i], 1), tc::mbar_init(&bar.wempty[i], 8);
     for (int i = 0; i < S::NA; ++i) tc::mbar_init(&bar.afull[i], 8), tc::mbar_init(&bar.aempty[i], 2);
-    for (int i = 0; i < 4; ++i) tc::mbar_init(&bar.dfull[i], 1), tc::mbar_init(&bar.dempty[i], 8);
+    for (int i = 0; i < S::ND; ++i) tc::mbar_init(&bar.dfull[i], 2), tc::mbar_init(&bar.dempty[i], 8);
     for (int i = 0; i < a.sb; ++i) tc::mbar_init(&bar.bfull[i], 1), tc::mbar_init(&bar.bempty[i], 2);
     tc::mbar_init(&bar.drain, 2);
     tc::fence_mbar_init();
@@ -477,18 +492,17 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
     if (elect()) {
       Turn tw;
       int it = 0;
-      bool ok = true;
-      for (int u = unit0; ok && u < units; u += step) {
+      for (int u = unit0; u < units; u += step) {
         const int y = u % a.tiles * ROWS;
         for (int c = 0; c < nc; ++c, ++it, tw.next(SW)) {
           if (it < SW && u == unit0) continue;             // loaded above
-          if (!wait(&bar.wempty[tw.slot], tw.phase ^ 1)) { ok = false; break; }
+          wait(&bar.wempty[tw.slot], tw.phase ^ 1);
           tc::mbar_expect_tx(&bar.wfull[tw.slot], W_STAGE);
           tc::tma_load_2d(wst + tw.slot * W_STAGE, &wmap, (c0 + c) * (KC / 2), y, &bar.wfull[tw.slot]);
         }
       }
       // copies still in flight land before the CTA may exit
-      for (int j = it - SW < 0 ? 0 : it - SW; j < it; ++j) tc::mbar_wait(&bar.wfull[j % SW], j / SW & 1, POLLS);
+      for (int j = it - SW < 0 ? 0 : it - SW; j < it; ++j) wait(&bar.wfull[j % SW], j / SW & 1);
     }
   } else if (w == 1) {
     // ---- staged x
@@ -496,17 +510,16 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
       asm volatile("griddepcontrol.wait;" ::: "memory");
       Turn tb;
       int it = 0;
-      bool ok = true;
-      for (int u = unit0; ok && u < units && !(a.resident && u > unit0); u += step) {
+      for (int u = unit0; u < units && !(a.resident && u > unit0); u += step) {
         const uint8_t* src = a.ws + ((long long)(u / a.tiles) * chunks + c0) * BLK;
         for (int c = 0; c < nc; ++c, ++it, tb.next(a.sb), src += BLK) {
-          if (!wait(&bar.bempty[tb.slot], tb.phase ^ 1)) { ok = false; break; }
+          wait(&bar.bempty[tb.slot], tb.phase ^ 1);
           tc::mbar_expect_tx(&bar.bfull[tb.slot], BLK);
           tc::bulk_load(bst + tb.slot * BLK, src, BLK, &bar.bfull[tb.slot]);
         }
       }
       for (int j = it - a.sb < 0 ? 0 : it - a.sb; j < it; ++j)
-        tc::mbar_wait(&bar.bfull[j % a.sb], j / a.sb & 1, POLLS);
+        wait(&bar.bfull[j % a.sb], j / a.sb & 1);
     }
   } else if (w < 4) {
     // ---- MMAs: two warps, every other group each (an MMA takes a warp 33 clocks to issue, a wait
@@ -514,20 +527,20 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
     const bool lead = elect();
     const int mine = w - 2;
     Turn ta, tb, td;
-    bool ok = true;
-    for (int u = unit0; ok && u < units; u += step) {
+    for (int u = unit0; u < units; u += step) {
       if (a.resident) tb.slot = 0;
+      const bool new_x = a.staged && !(a.resident && u > unit0);
       for (int c = 0; c < nc; ++c) {
-        if (!wait.warp(&bar.afull[ta.slot], ta.phase) ||
-            (a.staged && !wait.warp(&bar.bfull[tb.slot], tb.phase))) { ok = false; break; }
+        wait(&bar.afull[ta.slot], ta.phase);
+        if (new_x) wait(&bar.bfull[tb.slot], tb.phase);
         const uint32_t A = ta.slot * S::A_COLS;
         const uint64_t B = tc::sdesc(tc::smem_addr(bst + tb.slot * BLK), N * 16, 128);
 #pragma unroll
         for (int gj = 0; gj < GPC / 2; ++gj) {
-          const int gi = 2 * gj + mine, e = mine * S::ND + td.slot;
-          if (!wait.warp(&bar.dempty[e], td.phase ^ 1)) { ok = false; break; }
+          wait(&bar.dempty[td.slot], td.phase ^ 1);
           tc::fence_after_sync();
-          const uint32_t D = D_COL + e * N, Ag = A + gi * (8 * KB);
+          const int gi = 2 * gj + mine;
+          const uint32_t D = D_COL + (2 * td.slot + mine) * N, Ag = A + gi * (8 * KB);
           const uint64_t Bg = B + (uint64_t)(gi * (KB * 32 * N >> 4));
           if (lead) {
             constexpr uint32_t first = idesc_f8(N, 0), rest = idesc_f8(N, 1);
@@ -537,7 +550,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
               for (int b = 0; b < KB; ++b)
                 mma_f8(D, Ag + 8 * b, Bg + (uint64_t)((p * KC * N + b * 32 * N) >> 4), p > 0 ? rest : first, p + b > 0);
             mma_f8(D, A + KC / 4 + 8 * gi, B + (uint64_t)((S::PASSES * KC * N >> 4) + gi * (32 * N >> 4)), rest, true);
-            tc::commit(&bar.dfull[e]);
+            tc::commit(&bar.dfull[td.slot]);
           }
           td.next(S::ND);
         }
@@ -552,7 +565,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
     }
     if (lead) {
       tc::commit(&bar.drain);        // every MMA issued is done before the TMEM goes
-      tc::mbar_wait(&bar.drain, 0, POLLS);
+      wait(&bar.drain, 0);
     }
   } else if (w < 12) {
     // ---- unpacking: two sets of four warps, a half of every chunk each; a thread is a row
@@ -560,10 +573,10 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
     const uint32_t at = ((uint32_t)(w % 4 * 32) << 16) + half * 32;
     constexpr int GH = GPC / 2;        // groups per half
     Turn tw, ta;
-    bool ok = true, fresh = true;
+    bool fresh = true;
     int seen = 0;
     const int groups = (a.k + G - 1) / G;
-    for (int u = unit0; ok && u < units; u += step) {
+    for (int u = unit0; u < units; u += step) {
       const long long row = (long long)(u % a.tiles) * ROWS + r;
       int g = c0 * GPC + half * GH;
       const uint8_t* zp = a.z && row < a.n ? a.z + (long long)g * a.n + row : nullptr;
@@ -576,22 +589,26 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
       };
       if (a.z) load_zeros(0);
       for (int c = 0; c < nc; ++c) {
-        if (!wait.warp(&bar.wfull[tw.slot], tw.phase)) { ok = false; break; }
+        wait(&bar.wfull[tw.slot], tw.phase);
         uint4 raw[4];
         const uint8_t* src = wst + tw.slot * W_STAGE + r * (KC / 2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + (((half * 4 + j) ^ (r & 7)) * 16));
-        if (!wait.warp(&bar.aempty[ta.slot], ta.phase ^ 1)) { ok = false; break; }
+        wait(&bar.aempty[ta.slot], ta.phase ^ 1);
+        __syncwarp();
         tc::fence_after_sync();
         const uint32_t A = at + ta.slot * S::A_COLS;
+        uint32_t code[32];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t b[8] = {raw[j].x & 0x0f0f0f0fu, (raw[j].x >> 4) & 0x0f0f0f0fu,
-                                 raw[j].y & 0x0f0f0f0fu, (raw[j].y >> 4) & 0x0f0f0f0fu,
-                                 raw[j].z & 0x0f0f0f0fu, (raw[j].z >> 4) & 0x0f0f0f0fu,
-                                 raw[j].w & 0x0f0f0f0fu, (raw[j].w >> 4) & 0x0f0f0f0fu};
-          tmem_st8(A + 8 * j, b);
+          const uint32_t word[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            code[8 * j + 2 * i] = word[i] & 0x0f0f0f0fu;
+            code[8 * j + 2 * i + 1] = (word[i] >> 4) & 0x0f0f0f0fu;
+          }
         }
+        tmem_st32(A, code);
         if (a.z || fresh) {            // without zeros, -8 stays where the first round wrote it
 #pragma unroll
           for (int gi = 0; gi < GH; ++gi) {
@@ -622,8 +639,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
     const int groups = (a.k + G - 1) / G, ng = nc * GPC;
     if (a.staged) asm volatile("griddepcontrol.wait;" ::: "memory");
     Turn td;                            // a pair of groups: one accumulator of each MMA warp
-    bool ok = true;
-    for (int u = unit0; ok && u < units; u += step) {
+    for (int u = unit0; u < units; u += step) {
       const long long row = (long long)(u % a.tiles) * ROWS + r, m0 = (long long)(u / a.tiles) * MP;
       const int toks = (int)min((long long)MP, a.m - m0);
       __syncwarp();
@@ -637,65 +653,104 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
       for (int t = 0; t < TH; ++t) acc[t] = 0.f;
       const T* sp = static_cast<const T*>(a.s) + (long long)c0 * GPC * a.n + row;
       const int have = row < a.n ? min(ng, groups - c0 * GPC) : 0;
-      T sq[4];                          // the scales of the next four groups, as loaded (a conversion would wait)
+      // the scales of the next four groups, as loaded: 16-bit ones in words of their own, since a
+      // conversion or a packed pair would wait for the load
+      using Raw = typename std::conditional<S::IS32, uint32_t, unsigned short>::type;
+      const Raw* sr = reinterpret_cast<const Raw*>(sp);
+      uint32_t sq[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq[i] = i < have ? __ldg(sp + (long long)i * a.n) : from_f32<T>(0.f);
-      sp += 4LL * a.n;
-      for (int g0 = 0; ok && g0 < ng; g0 += 4) {
+      for (int i = 0; i < 4; ++i) sq[i] = i < have ? (uint32_t)__ldg(sr + (long long)i * a.n) : 0u;
+      sr += 4LL * a.n;
+      float bv = 0.f;
+      if (a.bias && row < a.n) bv = to_f32(static_cast<const T*>(a.bias)[row]);
+      for (int g0 = 0; g0 < ng; g0 += 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i % 2 == 0 && g0 + i >= ng) break;          // (ng is even)
-          const int e = i % 2 * S::ND + td.slot;
-          if (!wait.warp(&bar.dfull[e], td.phase)) { ok = false; break; }
-          tc::fence_after_sync();
-          const uint32_t D = at + e * N;
-          const float s = to_f32(sq[i]);
-          if (g0 + i + 4 < have) sq[i] = __ldg(sp + (long long)i * a.n);
-          else sq[i] = from_f32<T>(0.f);
-          constexpr int NP = S::COLS ? S::P : 1;          // columns of a token
-          float d[NP][TH];
-#pragma unroll
-          for (int p = 0; p < NP; ++p) tmem_ld<TH>(D + p * MP, d[p]);
-          tmem_wait_ld();
-          tc::fence_before_sync();
+        for (int i = 0; i < 4; i += 2) {
+          if (g0 + i >= ng) break;          // (ng is even)
+          wait(&bar.dfull[td.slot], td.phase);
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&bar.dempty[e]);
+          tc::fence_after_sync();
+          const uint32_t D = at + 2 * td.slot * N;
+          constexpr int NP = S::COLS ? S::P : 1;          // columns of a token
+          // both of the pair at once, where the registers hold them
+          constexpr int ONCE = 2 * NP * TH <= 40 ? 2 : 1;
 #pragma unroll
-          for (int p = 0; p < NP; ++p) pin<TH>(d[p]);
+          for (int j0 = 0; j0 < 2; j0 += ONCE) {
+            float d[ONCE][NP][TH];
 #pragma unroll
-          for (int t = 0; t < TH; ++t) {
-            float v = d[NP - 1][t];
+            for (int j = 0; j < ONCE; ++j)
 #pragma unroll
-            for (int p = NP - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[p][t]);
-            acc[t] = fmaf(s, v, acc[t]);
+              for (int p = 0; p < NP; ++p) tmem_ld<TH>(D + (j0 + j) * N + p * MP, d[j][p]);
+            tmem_wait_ld();
+            if (j0 + ONCE == 2) {
+              tc::fence_before_sync();
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(&bar.dempty[td.slot]);
+            }
+#pragma unroll
+            for (int j = 0; j < ONCE; ++j) {
+              const uint32_t raw = sq[i + j0 + j];
+              float s;
+              if constexpr (S::IS32) s = __uint_as_float(raw);
+              else if constexpr (std::is_same<T, __half>::value) s = __half2float(__ushort_as_half((unsigned short)raw));
+              else s = __uint_as_float(raw << 16);
+#pragma unroll
+              for (int p = 0; p < NP; ++p) pin<TH>(d[j][p]);
+#pragma unroll
+              for (int t = 0; t < TH; ++t) {
+                float v = d[j][NP - 1][t];
+#pragma unroll
+                for (int p = NP - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[j][p][t]);
+                acc[t] = fmaf(s, v, acc[t]);
+              }
+            }
           }
-          if (i % 2) td.next(S::ND);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            sq[i + j] = 0;
+            if (g0 + i + j + 4 < have) sq[i + j] = __ldg(sr + (long long)(i + j) * a.n);
+          }
+          td.next(S::ND);
         }
-        sp += 4LL * a.n;
+        sr += 4LL * a.n;
       }
       // the tile's outputs (or this CTA's part of them)
-      if (ok) {
-        const T* x = static_cast<const T*>(a.x);
-        const T* bias = static_cast<const T*>(a.bias);
-        float* red = reinterpret_cast<float*>(wst);
+      {
+        uint32_t any = 0;
 #pragma unroll
         for (int t = 0; t < TH; ++t) {
-          const int tok = t0 + t;
-          if (tok < toks && (row < a.n || a.ck > 1)) {
-            const uint32_t mask = s_masks[w - 12][tok];
-            float v = acc[t] * 512.f * s_scales[w - 12][tok];
-            if (mask && row < a.n)
-              for (int g = 0; g < ng; ++g)
-                if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
-                  v += left_out<T>(a, x + (m0 + tok) * a.ldx, row, (c0 * GPC + g) * G, G);
-            if (a.ck > 1) {
-              red[tok * ROWS + r] = v;    // (all stages are consumed: every group's sum is in)
-            } else {
-              if (bias) v += to_f32(bias[row]);
-              const long long o = (m0 + tok) * a.n + row;
-              if (a.out_f32) static_cast<float*>(a.y)[o] = v;
-              else static_cast<T*>(a.y)[o] = from_f32<T>(v);
-            }
+          if (t0 + t < toks) {
+            acc[t] *= 512.f * s_scales[w - 12][t0 + t];
+            any |= s_masks[w - 12][t0 + t];
+          }
+        }
+        if (any && row < a.n) {
+          const T* x = static_cast<const T*>(a.x);
+#pragma unroll
+          for (int t = 0; t < TH; ++t) {
+            const uint32_t mask = t0 + t < toks ? s_masks[w - 12][t0 + t] : 0u;
+            for (int g = 0; mask && g < ng; ++g)
+              if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
+                acc[t] += left_out<T>(a, x + (m0 + t0 + t) * a.ldx, row, (c0 * GPC + g) * G, G);
+          }
+        }
+        if (a.ck > 1) {
+          float* red = reinterpret_cast<float*>(wst) + t0 * ROWS + r;   // (all stages are consumed: every sum is in)
+#pragma unroll
+          for (int t = 0; t < TH; ++t)
+            if (t0 + t < toks) red[t * ROWS] = acc[t];
+        } else if (row < a.n) {
+          const long long o = (m0 + t0) * a.n + row;
+          if (a.out_f32) {
+            float* y = static_cast<float*>(a.y) + o;
+#pragma unroll
+            for (int t = 0; t < TH; ++t, y += a.n)
+              if (t0 + t < toks) *y = acc[t] + bv;
+          } else {
+            T* y = static_cast<T*>(a.y) + o;
+#pragma unroll
+            for (int t = 0; t < TH; ++t, y += a.n)
+              if (t0 + t < toks) *y = from_f32<T>(acc[t] + bv);
           }
         }
       }
