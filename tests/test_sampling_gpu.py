@@ -327,6 +327,33 @@ def test_sample_draws_follow_the_softmax():
         assert ((freq - prob).abs() <= 6 * (prob * (1 - prob) / n).sqrt()).all()
 
 
+def test_sample_vocabularies_of_any_size():
+    """Rows for one CTA, for clusters of up to sixteen, and beyond what a cluster holds."""
+    for b, v, dtype in ((200, 20000, torch.float32), (3, 262144, torch.bfloat16), (2, 400001, torch.float32),
+                        (2, 800003, torch.float32)):
+        l, noise = draw(b, v, v, 0.1, dtype)
+        check_sample(l, noise, 1.0, 0, 0.95, 0.0)
+        check_sample(l, noise, 0.7, 200, 0.8, 0.001)
+        check_sample(l, noise, 1.5, 0, 1.0, 0.0)
+        check_sample(l, None, 0.0, 0, 1.0, 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_cuts_among_many_equal_values(dtype):
+    """Few distinct values, values around zero and of every size: the cut falls into crowded bins."""
+    g = torch.Generator().manual_seed(9)
+    v = 30000
+    rows = [torch.randint(0, 6, (v,), generator=g).float(), torch.randn(v, generator=g) * 1e-4,
+            10.0 ** (torch.rand(v, generator=g) * 8 - 6) * torch.randn(v, generator=g).sign(),
+            torch.randn(v, generator=g) * 200, torch.full((v,), 1.5), 100 + torch.rand(v, generator=g) * 1e-3,
+            torch.randint(0, 2, (v,), generator=g).float() * 1e4]
+    l = torch.stack(rows).to(dtype)
+    noise = torch.empty(l.shape).exponential_(generator=g)
+    for t, k, p, minp in ((1.0, 1000, 1.0, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 7, 0.5, 0.0), (50.0, 20000, 0.9, 0.0),
+                          (0.01, 100, 0.7, 0.0)):
+        check_sample(l, noise, t, k, p, minp, most_clear=False)
+
+
 def test_sample_strides_and_streams():
     l, noise = draw(5, 777, 8, 0.1)
     lw, nw = torch.zeros(5, 800, device="cuda"), torch.ones(5, 779, device="cuda")

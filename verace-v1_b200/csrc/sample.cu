@@ -6,15 +6,28 @@
 // smallest of exponentials with rates w_i is i with probability w_i / sum w).  T = 0 takes
 // the largest logit.  logprob = log softmax(z)[token] over the whole row (T = 0: of l).
 //
-// The thresholds come from a radix selection on the values' order-preserving 32-bit keys,
-// eight bits at a time: by count for k, by mass for p.  Mass is summed in 2^-40 fixed point,
-// so that the order of the atomics changes nothing.
+// Two kernels.  sample_cluster: a cluster of CTAs per row, the row read once and kept in shared
+// memory, where the passes after the first run.  The cuts by count (k) and by mass (p) come from
+// histograms in shared memory, joined over the cluster: first 1024 bins linear in z (values
+// near the top spread over many bins; bins of the float's bits would put most of a row into a
+// handful), then within the bin of the cut 1024 bins of the values' order-preserving 32-bit
+// keys, until a bin holds one value or one key: two levels for most rows, five at worst.
+// sample_rows: one CTA per row that reads it again for every pass; for rows that no cluster
+// holds.  Mass is summed in 2^-40 fixed point, so that the order of the atomics changes nothing.
 #include "common.cuh"
+
+#include <cooperative_groups.h>
+
+#include <atomic>
 
 namespace verace {
 namespace {
 
-constexpr int NT = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int NT = 1024;       // threads of sample_rows
+constexpr int CT = 512;        // threads of sample_cluster's CTAs: two or three of them share an SM
+constexpr int BINS = 1024;
 
 struct SampleArgs {
   const void* logits;
@@ -46,7 +59,7 @@ __device__ __forceinline__ float value(T l) {
 // z of a value against the row's largest (equal infinities: 0)
 __device__ __forceinline__ float scaled(float x, float top, float t) { return x == top ? 0.f : (x - top) / t; }
 
-template <typename F>
+template <int WARPS = NT / 32, typename F>
 __device__ __forceinline__ float block_reduce(float x, float* s, F f) {
   const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
 #pragma unroll
@@ -54,14 +67,14 @@ __device__ __forceinline__ float block_reduce(float x, float* s, F f) {
   __syncthreads();
   if (lane == 0) s[w] = x;
   __syncthreads();
-  x = s[lane];
+  x = s[lane % WARPS];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, o));
+  for (int o = WARPS / 2; o > 0; o >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, o));
   return x;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
   __shared__ float red[32];
   __shared__ unsigned long long hist[256];
   __shared__ uint32_t s_prefix;
@@ -157,6 +170,323 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ a cluster per row
+struct Hist {
+  uint32_t count[BINS];
+  unsigned long long mass[BINS];
+};
+struct Shared {
+  Hist hist[2];                        // of alternate levels: a level clears the next one's
+  float top, ties, rest;
+  unsigned long long best;
+  float red[32];
+  unsigned long long red64[32];
+  int bin;
+  uint32_t found;                      // the values in it
+  unsigned long long left;             // of the target, before that bin
+};
+
+// Every CTA's copy of one field, combined in rank order.
+template <typename V, typename F>
+__device__ __forceinline__ V over_cluster(cg::cluster_group& cl, V* field, F f) {
+  const int n = cl.num_blocks();
+  V v = *cl.map_shared_rank(field, 0);
+  for (int i = 1; i < n; ++i) v = f(v, *cl.map_shared_rank(field, i));
+  return v;
+}
+
+__device__ __forceinline__ unsigned long long fixed_mass(float z) {
+  return (unsigned long long)(expf(z) * 1099511627776.f + 0.5f);
+}
+
+// The cluster's histogram h: the first bin at which the running count (or mass) reaches `left`,
+// the last one if none does.  Thread i has bins 2 i and 2 i + 1.  Sets s.bin, s.found and s.left.
+__device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, bool first, float p,
+                         unsigned long long left) {
+  static_assert(BINS == 2 * CT, "two bins a thread");
+  const int tid = threadIdx.x, lane = tid % 32, w = tid / 32, n = cl.num_blocks();
+  uint32_t count[2] = {0, 0};
+  unsigned long long mass[2] = {0, 0};
+  for (int i = 0; i < n; ++i) {
+    const Hist* r = &cl.map_shared_rank(&s, i)->hist[h];
+    const uint2 c = *reinterpret_cast<const uint2*>(&r->count[2 * tid]);
+    count[0] += c.x, count[1] += c.y;
+    if (by_mass) {
+      const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(&r->mass[2 * tid]);
+      mass[0] += m.x, mass[1] += m.y;
+    }
+  }
+  const unsigned long long m0 = by_mass ? mass[0] : count[0], m1 = by_mass ? mass[1] : count[1];
+  unsigned long long run = m0 + m1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  if (lane == 31) s.red64[w] = run;
+  __syncthreads();
+  unsigned long long before = 0, total = 0;
+  for (int i = 0; i < CT / 32; ++i) {
+    const unsigned long long v = s.red64[i];
+    before += i < w ? v : 0;
+    total += v;
+  }
+  run += before;
+  if (by_mass && first) {
+    // a token is kept while the mass strictly above it is below p * total
+    left = (unsigned long long)ceil((double)p * (double)total);
+    if (left < 1) left = 1;
+  }
+  const unsigned long long upto[2] = {run - m1, run}, mine[2] = {m0, m1};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const bool at = upto[e] >= left && upto[e] - mine[e] < left;
+    const bool last = 2 * tid + e == BINS - 1 && upto[e] < left;
+    if (at || last) {
+      s.bin = 2 * tid + e;
+      s.found = count[e];
+      s.left = left - (upto[e] - mine[e]);
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ __align__(16) Shared s;
+  T* xs = reinterpret_cast<T*>(raw);
+  cg::cluster_group cl = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid % 32, rank = cl.block_rank();
+  const int row = blockIdx.x / cl.num_blocks();
+  const T* l = static_cast<const T*>(a.logits) + row * a.ld;
+  const float t = a.t_rows ? a.t_rows[row] : a.t;
+  const bool greedy = !(t > 0.f);
+  const float ts = greedy ? 1.f : t;
+  const int k = a.k_rows ? a.k_rows[row] : a.k;
+  const float p = a.p_rows ? a.p_rows[row] : a.p;
+  const float minp = a.minp_rows ? a.minp_rows[row] : a.minp;
+
+  // ---- this CTA's part of the row
+  const int i0 = rank * chunk, n = max(0, min(chunk, a.v - i0));
+  const T* src = l + i0;
+  float top = -INFINITY;
+  constexpr int E = 16 / sizeof(T);
+  int done = 0;
+  if (reinterpret_cast<size_t>(src) % 16 == 0) {
+    done = n / E * E;
+#pragma unroll 4
+    for (int j = tid * E; j < done; j += CT * E) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(src + j));
+      *reinterpret_cast<uint4*>(xs + j) = u;
+      if constexpr (sizeof(T) == 4) {
+        top = fmaxf(fmaxf(top, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),      // (fmaxf passes over a NaN)
+                    fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+      } else {
+        float f[8];
+        unpack8<T>(u, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, f[e]);
+      }
+    }
+  }
+#pragma unroll 8
+  for (int j = done + tid; j < n; j += CT) {
+    const T u = src[j];
+    xs[j] = u;
+    top = fmaxf(top, to_f32(u));
+  }
+  top = top + 0.f;
+  for (int i = tid; i < BINS; i += CT) s.hist[0].count[i] = 0, s.hist[0].mass[i] = 0;
+  if (tid == 0) s.best = 0;
+  top = block_reduce<CT / 32>(top, s.red, [](float u, float v) { return fmaxf(u, v); });
+  if (tid == 0) s.top = top;
+  cl.sync();
+  top = over_cluster(cl, &s.top, [](float u, float v) { return fmaxf(u, v); });
+  if (top == -INFINITY) {              // (the same for every CTA of the cluster)
+    if (rank == 0 && tid == 0) a.tokens[row] = -1, a.logprobs[row] = -INFINITY;
+    cl.sync();
+    return;
+  }
+
+  // ---- log sum, and the first histogram
+  const bool cut_k = !greedy && k > 0 && k < a.v, cut_p = !greedy && p < 1.f;
+  const float per = 16.f / ts;         // bins of 1/16 in z
+  auto bin_of = [&](float v) { return (int)fminf((top - v) * per, (float)(BINS - 1)); };    // (v finite or top)
+  auto bin0 = [&](float v) { return v == top ? 0 : bin_of(v); };
+  float ties = 0.f, rest = 0.f;
+#pragma unroll 4
+  for (int j = tid; j < n; j += CT) {
+    const float x = value(xs[j]);
+    const float e = expf(scaled(x, top, ts));
+    if (x == top) ties += 1.f;
+    else rest += e;
+    if ((cut_k || cut_p) && x > -INFINITY) {
+      const int b = bin0(x);
+      atomicAdd(&s.hist[0].count[b], 1u);
+      if (cut_p && !cut_k) atomicAdd(&s.hist[0].mass[b], (unsigned long long)(e * 1099511627776.f + 0.5f));
+    }
+  }
+  ties = block_reduce<CT / 32>(ties, s.red, [](float u, float v) { return u + v; });
+  rest = block_reduce<CT / 32>(rest, s.red, [](float u, float v) { return u + v; });
+  if (tid == 0) s.ties = ties, s.rest = rest;
+  cl.sync();
+  ties = over_cluster(cl, &s.ties, [](float u, float v) { return u + v; });
+  rest = over_cluster(cl, &s.rest, [](float u, float v) { return u + v; });
+  const float lse = logf(ties) + log1pf(rest / ties);
+
+  // ---- the cuts: what is kept is every value in a bin before `edge`, and in it the keys from
+  // `least` on
+  int edge = BINS;
+  uint32_t least = 0;
+  int h = 0;
+  for (int by_mass = 0; by_mass < 2; ++by_mass) {
+    if (by_mass ? !cut_p : !cut_k) continue;
+    if (by_mass && cut_k) {            // the mass of what k kept
+      h ^= 1;
+      for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].mass[i] = 0;
+      __syncthreads();
+      for (int j = tid; j < n; j += CT) {
+        const float x = value(xs[j]);
+        if (x > -INFINITY) {
+          const int b = bin0(x);
+          if (b < edge || (b == edge && key_of(x) >= least)) {
+            atomicAdd(&s.hist[h].count[b], 1u);
+            atomicAdd(&s.hist[h].mass[b], fixed_mass(scaled(x, top, ts)));
+          }
+        }
+      }
+      cl.sync();
+    }
+    find_bin(cl, s, h, by_mass, true, p, (unsigned long long)k);
+    int cut = s.bin;
+    uint32_t from = 0;
+    unsigned long long left = s.left;
+    bool more = s.found > 1 && !(!by_mass && left >= s.found);
+    const int kept_edge = edge;
+    const uint32_t kept_least = least;
+    if (more) {
+      // the keys that bin `cut` can hold (its bounds, widened by the roundings of bin_of)
+      const float wide = 1.f / per, slack = (fabsf(top) + (cut + 1) * wide) * 1e-6f;
+      uint32_t lo = cut == BINS - 1 ? key_of(-INFINITY) + 1 : key_of(value(top - (cut + 1) * wide - slack));
+      uint32_t hi = key_of(fminf(top, top - cut * wide + slack));
+      if (!(fabsf(top) <= 3.4028235e38f)) lo = key_of(-INFINITY) + 1, hi = key_of(top);
+      if (lo > hi) lo = hi;
+      while (more) {
+        const int bits = 32 - __clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;
+        h ^= 1;
+        // (find_bin's barriers are behind every CTA's reads of the other histogram only after the
+        // cluster's next one: this one was last read a level ago)
+        for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].mass[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < n; j += CT) {
+          const float x = value(xs[j]);
+          if (x > -INFINITY && bin0(x) == cut) {
+            const uint32_t key = key_of(x);
+            if (key >= lo && key <= hi && (cut < kept_edge || key >= kept_least)) {
+              const int b = BINS - 1 - (int)((key - lo) >> shift);      // descending, as the first level
+              atomicAdd(&s.hist[h].count[b], 1u);
+              if (by_mass) atomicAdd(&s.hist[h].mass[b], fixed_mass(scaled(x, top, ts)));
+            }
+          }
+        }
+        cl.sync();
+        find_bin(cl, s, h, by_mass, false, p, left);
+        const uint32_t b = BINS - 1 - s.bin;
+        left = s.left;
+        from = lo + (b << shift);
+        more = shift > 0 && s.found > 1 && !(!by_mass && left >= s.found);
+        if (shift > 0) hi = min(hi, from + ((1u << shift) - 1));
+        lo = from;
+        __syncthreads();
+      }
+    }
+    if (cut < edge) edge = cut, least = from;
+    else if (cut == edge) least = max(least, from);
+    cl.sync();                         // before the histograms are used again
+  }
+
+  // ---- the choice
+  const float* noise = a.noise + row * a.noise_ld;
+  unsigned long long best = 0;
+#pragma unroll 4
+  for (int j = tid; j < n; j += CT) {
+    const float x = value(xs[j]);
+    if (!(x > -INFINITY)) continue;
+    float score = x;
+    if (!greedy) {
+      if (edge < BINS) {
+        const int b = bin0(x);
+        if (b > edge || (b == edge && key_of(x) < least)) continue;
+      }
+      const float z = scaled(x, top, ts);
+      if (minp > 0.f && x != top && !(expf(z) >= minp)) continue;
+      score = z - logf(__ldg(noise + i0 + j));
+      if (!(score > -INFINITY)) continue;
+    }
+    const unsigned long long c = ((unsigned long long)key_of(score + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + j));
+    if (c > best) best = c;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long v = __shfl_xor_sync(0xffffffffu, best, o);
+    if (v > best) best = v;
+  }
+  if (lane == 0 && best) atomicMax(&s.best, best);
+  cl.sync();
+  if (rank == 0 && tid == 0) {
+    const unsigned long long c = over_cluster(
+        cl, &s.best, [](unsigned long long u, unsigned long long v) { return u > v ? u : v; });
+    if (c == 0) {
+      a.tokens[row] = -1, a.logprobs[row] = -INFINITY;
+    } else {
+      const int i = (int)(0xffffffffu - (uint32_t)c);
+      a.tokens[row] = i;
+      a.logprobs[row] = scaled(value(to_f32(l[i])), top, ts) - lse;
+    }
+  }
+  cl.sync();
+}
+
+constexpr int CHUNK_MAX = 176 * 1024;   // bytes of a row in a CTA (one an SM beyond 80 KB)
+
+template <typename T>
+int run(const SampleArgs& a, cudaStream_t st) {
+  auto chunk_of = [&](int c) { return ((a.v + c - 1) / c + 7) / 8 * 8; };
+  // CTAs per row: as few as two CTAs an SM hold it with, more (of 2048 values at least) while
+  // the rows alone leave the device empty
+  int c = 1;
+  while (c < 16 && (size_t)chunk_of(c) * sizeof(T) > 80 * 1024) c *= 2;
+  while (c < 8 && (long long)a.b * c * 2 <= 296 && chunk_of(2 * c) >= 2048) c *= 2;
+  const size_t bytes = (size_t)chunk_of(c) * sizeof(T);
+  if (bytes > CHUNK_MAX || (long long)a.b * c > 0x7fffffffLL) {
+    sample_rows<T><<<a.b, NT, 0, st>>>(a);
+    return check_launch("sample");
+  }
+  auto kern = sample_cluster<T>;
+  static std::atomic<uint64_t> ready{0};      // devices whose limits are raised
+  int dev = 0;
+  VERACE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_MAX));
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.b * c));
+  cfg.blockDim = dim3(CT);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, a, chunk_of(c)));
+  return check_launch("sample");
+}
+
 }  // namespace
 }  // namespace verace
 
@@ -178,8 +508,7 @@ extern "C" int verace_sample(const void* logits, long long ld, const float* nois
                  "sample: noise is needed unless every row has temperature 0");
   SampleArgs a{logits, ld, noise, noise_ld, b, v, t_rows, k_rows, p_rows, minp_rows, t, p, minp, k, tokens, logprobs};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == VERACE_F32) sample_kernel<float><<<b, NT, 0, st>>>(a);
-  else if (dtype == VERACE_BF16) sample_kernel<__nv_bfloat16><<<b, NT, 0, st>>>(a);
-  else sample_kernel<__half><<<b, NT, 0, st>>>(a);
-  return check_launch("sample");
+  if (dtype == VERACE_F32) return run<float>(a, st);
+  if (dtype == VERACE_BF16) return run<__nv_bfloat16>(a, st);
+  return run<__half>(a, st);
 }
