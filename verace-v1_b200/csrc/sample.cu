@@ -171,9 +171,11 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
 }
 
 // ------------------------------------------------------------------ a cluster per row
+// A histogram over a CTA's part of the row.  The mass of a bin is in 2^-32 of a unit, the halves
+// of each addend summed apart (a 64-bit atomic in shared memory is a loop): at the first level the
+// unit of bin i is exp(-i / 16), the largest weight in it, at the others 1 at half the digits.
 struct Hist {
-  uint32_t count[BINS];
-  unsigned long long mass[BINS];
+  uint32_t count[BINS], high[BINS], low[BINS];
 };
 struct Shared {
   Hist hist[2];                        // of alternate levels: a level clears the next one's
@@ -191,32 +193,44 @@ template <typename V, typename F>
 __device__ __forceinline__ V over_cluster(cg::cluster_group& cl, V* field, F f) {
   const int n = cl.num_blocks();
   V v = *cl.map_shared_rank(field, 0);
+#pragma unroll 8
   for (int i = 1; i < n; ++i) v = f(v, *cl.map_shared_rank(field, i));
   return v;
 }
 
-__device__ __forceinline__ unsigned long long fixed_mass(float z) {
-  return (unsigned long long)(expf(z) * 1099511627776.f + 0.5f);
+__device__ __forceinline__ void add_mass(Hist& h, int b, float part) {
+  const uint32_t u = (uint32_t)fminf(part * 4294967296.f, 4294967040.f);
+  atomicAdd(&h.high[b], u >> 16);
+  atomicAdd(&h.low[b], u & 0xffffu);
 }
 
 // The cluster's histogram h: the first bin at which the running count (or mass) reaches `left`,
-// the last one if none does.  Thread i has bins 2 i and 2 i + 1.  Sets s.bin, s.found and s.left.
+// the last one if none does.  Thread i has bins 2 i and 2 i + 1.  Masses are in units of exp(-bin /
+// 16) (`first`) or of `weight`.  Sets s.bin, s.found and s.left.
 __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, bool first, float p,
-                         unsigned long long left) {
+                         unsigned long long left, float weight) {
   static_assert(BINS == 2 * CT, "two bins a thread");
   const int tid = threadIdx.x, lane = tid % 32, w = tid / 32, n = cl.num_blocks();
+  // a unit of a bin's mass, in 2^-8 of the largest weight's 2^-32
+  const double unit[2] = {256.0 * (first ? expf(-0.125f * tid) : weight),
+                          256.0 * (first ? expf(-0.125f * tid - 0.0625f) : weight)};
   uint32_t count[2] = {0, 0};
-  unsigned long long mass[2] = {0, 0};
+  unsigned long long part[2] = {0, 0};
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
     const Hist* r = &cl.map_shared_rank(&s, i)->hist[h];
     const uint2 c = *reinterpret_cast<const uint2*>(&r->count[2 * tid]);
     count[0] += c.x, count[1] += c.y;
     if (by_mass) {
-      const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(&r->mass[2 * tid]);
-      mass[0] += m.x, mass[1] += m.y;
+      const uint2 u = *reinterpret_cast<const uint2*>(&r->high[2 * tid]);
+      const uint2 v = *reinterpret_cast<const uint2*>(&r->low[2 * tid]);
+      part[0] += ((unsigned long long)u.x << 16) + v.x;
+      part[1] += ((unsigned long long)u.y << 16) + v.y;
     }
   }
-  const unsigned long long m0 = by_mass ? mass[0] : count[0], m1 = by_mass ? mass[1] : count[1];
+  // in 2^-40 of the largest weight
+  const unsigned long long m0 = by_mass ? (unsigned long long)((double)part[0] * unit[0]) : count[0];
+  const unsigned long long m1 = by_mass ? (unsigned long long)((double)part[1] * unit[1]) : count[1];
   unsigned long long run = m0 + m1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -266,38 +280,66 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   const int k = a.k_rows ? a.k_rows[row] : a.k;
   const float p = a.p_rows ? a.p_rows[row] : a.p;
   const float minp = a.minp_rows ? a.minp_rows[row] : a.minp;
+  const float log_minp = minp > 0.f ? logf(minp) : -INFINITY;
 
   // ---- this CTA's part of the row
   const int i0 = rank * chunk, n = max(0, min(chunk, a.v - i0));
   const T* src = l + i0;
   float top = -INFINITY;
   constexpr int E = 16 / sizeof(T);
+  const T none = from_f32<T>(-INFINITY);
   int done = 0;
   if (reinterpret_cast<size_t>(src) % 16 == 0) {
     done = n / E * E;
 #pragma unroll 4
     for (int j = tid * E; j < done; j += CT * E) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(src + j));
-      *reinterpret_cast<uint4*>(xs + j) = u;
-      if constexpr (sizeof(T) == 4) {
-        top = fmaxf(fmaxf(top, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),      // (fmaxf passes over a NaN)
-                    fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+      uint4 u = __ldg(reinterpret_cast<const uint4*>(src + j));
+      float f[E];
+      if constexpr (E == 4) {
+        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y);
+        f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
       } else {
-        float f[8];
         unpack8<T>(u, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, f[e]);
       }
+      float most = f[0];                        // (fmaxf passes over a NaN)
+      bool nan = f[0] != f[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) most = fmaxf(most, f[e]), nan |= f[e] != f[e];
+      *reinterpret_cast<uint4*>(xs + j) = u;
+      if (nan) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (f[e] != f[e]) xs[j + e] = none;
+      }
+      top = fmaxf(top, most);
     }
   }
 #pragma unroll 8
   for (int j = done + tid; j < n; j += CT) {
     const T u = src[j];
-    xs[j] = u;
-    top = fmaxf(top, to_f32(u));
+    const float f = to_f32(u);
+    xs[j] = f != f ? none : u;
+    top = fmaxf(top, f);
   }
-  top = top + 0.f;
-  for (int i = tid; i < BINS; i += CT) s.hist[0].count[i] = 0, s.hist[0].mass[i] = 0;
+  const int n4 = (n + 3) / 4;
+  if (tid < n4 * 4 - n) xs[n + tid] = none;
+  // f(value, index in the CTA's part) for a thread's values, four at a time
+  auto each = [&](auto f) {
+    for (int j = tid; j < n4; j += CT) {
+      float v[4];
+      if constexpr (sizeof(T) == 4) {
+        const float4 u = reinterpret_cast<const float4*>(xs)[j];
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      } else {
+        const uint2 u = reinterpret_cast<const uint2*>(xs)[j];
+        const float2 g = unpack2<T>(u.x), h = unpack2<T>(u.y);
+        v[0] = g.x; v[1] = g.y; v[2] = h.x; v[3] = h.y;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(v[e], 4 * j + e);
+    }
+  };
+  for (int i = tid; i < BINS; i += CT) s.hist[0].count[i] = 0, s.hist[0].high[i] = 0, s.hist[0].low[i] = 0;
   if (tid == 0) s.best = 0;
   top = block_reduce<CT / 32>(top, s.red, [](float u, float v) { return fmaxf(u, v); });
   if (tid == 0) s.top = top;
@@ -311,21 +353,32 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
 
   // ---- log sum, and the first histogram
   const bool cut_k = !greedy && k > 0 && k < a.v, cut_p = !greedy && p < 1.f;
-  const float per = 16.f / ts;         // bins of 1/16 in z
-  auto bin_of = [&](float v) { return (int)fminf((top - v) * per, (float)(BINS - 1)); };    // (v finite or top)
-  auto bin0 = [&](float v) { return v == top ? 0 : bin_of(v); };
+  const float inv = 1.f / ts, per = 16.f * inv;         // bins of 1/16 in z
+  auto below = [&](float x) { return x == top ? 0.f : top - x; };
+  auto bin_of = [&](float d) { return (int)fminf(d * per, (float)(BINS - 1)); };
+  auto bin0 = [&](float x) { return bin_of(below(x)); };
+  auto weight = [&](float d) { return __expf(-d * inv); };
+  // a weight in units of its first-level bin's largest (the last bin's, below exp(-64), is left out)
+  auto part_of = [&](float d, int b) { return b == BINS - 1 ? 0.f : __expf(0.0625f * b - d * inv); };
   float ties = 0.f, rest = 0.f;
-#pragma unroll 4
-  for (int j = tid; j < n; j += CT) {
-    const float x = value(xs[j]);
-    const float e = expf(scaled(x, top, ts));
-    if (x == top) ties += 1.f;
-    else rest += e;
-    if ((cut_k || cut_p) && x > -INFINITY) {
-      const int b = bin0(x);
-      atomicAdd(&s.hist[0].count[b], 1u);
-      if (cut_p && !cut_k) atomicAdd(&s.hist[0].mass[b], (unsigned long long)(e * 1099511627776.f + 0.5f));
-    }
+  if (cut_k || cut_p) {
+    const bool mass = cut_p && !cut_k;
+    each([&](float x, int) {
+      const float d = below(x);
+      if (d == 0.f) ties += 1.f;
+      else rest += weight(d);
+      if (x > -INFINITY) {
+        const int b = bin_of(d);
+        atomicAdd(&s.hist[0].count[b], 1u);
+        if (mass) add_mass(s.hist[0], b, part_of(d, b));
+      }
+    });
+  } else {
+    each([&](float x, int) {
+      const float d = below(x);
+      if (d == 0.f) ties += 1.f;
+      else rest += weight(d);
+    });
   }
   ties = block_reduce<CT / 32>(ties, s.red, [](float u, float v) { return u + v; });
   rest = block_reduce<CT / 32>(rest, s.red, [](float u, float v) { return u + v; });
@@ -344,21 +397,21 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     if (by_mass ? !cut_p : !cut_k) continue;
     if (by_mass && cut_k) {            // the mass of what k kept
       h ^= 1;
-      for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].mass[i] = 0;
+      for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].high[i] = 0, s.hist[h].low[i] = 0;
       __syncthreads();
-      for (int j = tid; j < n; j += CT) {
-        const float x = value(xs[j]);
+      each([&](float x, int) {
         if (x > -INFINITY) {
-          const int b = bin0(x);
-          if (b < edge || (b == edge && key_of(x) >= least)) {
+          const float d = below(x);
+          const int b = bin_of(d);
+          if (b < edge || (b == edge && key_of(x + 0.f) >= least)) {
             atomicAdd(&s.hist[h].count[b], 1u);
-            atomicAdd(&s.hist[h].mass[b], fixed_mass(scaled(x, top, ts)));
+            add_mass(s.hist[h], b, part_of(d, b));
           }
         }
-      }
+      });
       cl.sync();
     }
-    find_bin(cl, s, h, by_mass, true, p, (unsigned long long)k);
+    find_bin(cl, s, h, by_mass, true, p, (unsigned long long)k, 1.f);
     int cut = s.bin;
     uint32_t from = 0;
     unsigned long long left = s.left;
@@ -377,21 +430,21 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
         h ^= 1;
         // (find_bin's barriers are behind every CTA's reads of the other histogram only after the
         // cluster's next one: this one was last read a level ago)
-        for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].mass[i] = 0;
+        for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].high[i] = 0, s.hist[h].low[i] = 0;
         __syncthreads();
-        for (int j = tid; j < n; j += CT) {
-          const float x = value(xs[j]);
-          if (x > -INFINITY && bin0(x) == cut) {
-            const uint32_t key = key_of(x);
+        each([&](float x, int) {
+          const float d = below(x);
+          if (x > -INFINITY && bin_of(d) == cut) {
+            const uint32_t key = key_of(x + 0.f);
             if (key >= lo && key <= hi && (cut < kept_edge || key >= kept_least)) {
               const int b = BINS - 1 - (int)((key - lo) >> shift);      // descending, as the first level
               atomicAdd(&s.hist[h].count[b], 1u);
-              if (by_mass) atomicAdd(&s.hist[h].mass[b], fixed_mass(scaled(x, top, ts)));
+              if (by_mass) add_mass(s.hist[h], b, part_of(d, cut));
             }
           }
-        }
+        });
         cl.sync();
-        find_bin(cl, s, h, by_mass, false, p, left);
+        find_bin(cl, s, h, by_mass, false, p, left, expf(-0.0625f * cut));
         const uint32_t b = BINS - 1 - s.bin;
         left = s.left;
         from = lo + (b << shift);
@@ -407,32 +460,43 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   }
 
   // ---- the choice
-  const float* noise = a.noise + row * a.noise_ld;
-  unsigned long long best = 0;
-#pragma unroll 4
-  for (int j = tid; j < n; j += CT) {
-    const float x = value(xs[j]);
-    if (!(x > -INFINITY)) continue;
-    float score = x;
-    if (!greedy) {
+  // The score is l / T - log(noise) where that is in range, z - log(noise) where it is not.  Most
+  // values are far from the best so far: fast arithmetic (off by less than 1e-4 and 1e-5 of its
+  // terms) passes over them.
+  const float* noise = a.noise + row * a.noise_ld + i0;
+  const float shift = top * inv;
+  const bool direct = fabsf(top / ts) <= 3.4028235e38f;
+  float best = -INFINITY;
+  int at = -1;
+  if (greedy) {
+    each([&](float x, int j) {
+      if (x > best) best = x, at = j;
+    });
+  } else {
+    each([&](float x, int j) {
+      if (!(x > -INFINITY)) return;
+      const float d = below(x);
       if (edge < BINS) {
-        const int b = bin0(x);
-        if (b > edge || (b == edge && key_of(x) < least)) continue;
+        const int b = bin_of(d);
+        if (b > edge || (b == edge && key_of(x + 0.f) < least)) return;
       }
-      const float z = scaled(x, top, ts);
-      if (minp > 0.f && x != top && !(expf(z) >= minp)) continue;
-      score = z - logf(__ldg(noise + i0 + j));
-      if (!(score > -INFINITY)) continue;
-    }
-    const unsigned long long c = ((unsigned long long)key_of(score + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + j));
-    if (c > best) best = c;
+      const float z = -d * inv;
+      if (minp > 0.f && d != 0.f && !(z >= log_minp)) return;
+      const float r = __ldg(noise + j);
+      const float l = __logf(r), near = (direct ? shift + z : z) - l;
+      if (near + 1e-4f + 1e-5f * (fabsf(shift) + fabsf(z) + fabsf(l)) < best) return;
+      const float score = (direct ? x / ts : -(d / ts)) - logf(r);
+      if (score > best) best = score, at = j;           // (a thread's indices rise: the lowest on ties)
+    });
   }
+  unsigned long long choice =
+      at < 0 ? 0 : ((unsigned long long)key_of(best + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + at));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long v = __shfl_xor_sync(0xffffffffu, best, o);
-    if (v > best) best = v;
+    const unsigned long long v = __shfl_xor_sync(0xffffffffu, choice, o);
+    if (v > choice) choice = v;
   }
-  if (lane == 0 && best) atomicMax(&s.best, best);
+  if (lane == 0 && choice) atomicMax(&s.best, choice);
   cl.sync();
   if (rank == 0 && tid == 0) {
     const unsigned long long c = over_cluster(
