@@ -8,10 +8,10 @@
 //
 // Two kernels.  sample_cluster: a cluster of CTAs per row, the row read once and kept in shared
 // memory, where the passes after the first run.  The cuts by count (k) and by mass (p) come from
-// histograms in shared memory, joined over the cluster: first 1024 bins linear in z (values
+// histograms in shared memory, joined over the cluster: first 512 bins linear in z (values
 // near the top spread over many bins; bins of the float's bits would put most of a row into a
-// handful), then within the bin of the cut 1024 bins of the values' order-preserving 32-bit
-// keys, until a bin holds one value or one key: two levels for most rows, five at worst.
+// handful), then within the bin of the cut 512 bins of the values' order-preserving keys, until
+// a bin holds one value or one key: two or three levels for most rows, five at worst.
 // sample_rows: one CTA per row that reads it again for every pass; for rows that no cluster
 // holds.  Mass is summed in 2^-40 fixed point, so that the order of the atomics changes nothing.
 #include "common.cuh"
@@ -27,7 +27,7 @@ namespace cg = cooperative_groups;
 
 constexpr int NT = 1024;       // threads of sample_rows
 constexpr int CT = 512;        // threads of sample_cluster's CTAs: two or three of them share an SM
-constexpr int BINS = 1024;
+constexpr int BINS = 512;
 
 struct SampleArgs {
   const void* logits;
@@ -205,33 +205,24 @@ __device__ __forceinline__ void add_mass(Hist& h, int b, float part) {
 }
 
 // The cluster's histogram h: the first bin at which the running count (or mass) reaches `left`,
-// the last one if none does.  Thread i has bins 2 i and 2 i + 1.  Masses are in units of exp(-bin /
+// the last one if none does.  Thread i has bin i.  Masses are in units of exp(-bin /
 // 16) (`first`) or of `weight`.  Sets s.bin, s.found and s.left.
 __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, bool first, float p,
                          unsigned long long left, float weight) {
-  static_assert(BINS == 2 * CT, "two bins a thread");
+  static_assert(BINS == CT, "a bin a thread");
   const int tid = threadIdx.x, lane = tid % 32, w = tid / 32, n = cl.num_blocks();
-  // a unit of a bin's mass, in 2^-8 of the largest weight's 2^-32
-  const double unit[2] = {256.0 * (first ? expf(-0.125f * tid) : weight),
-                          256.0 * (first ? expf(-0.125f * tid - 0.0625f) : weight)};
-  uint32_t count[2] = {0, 0};
-  unsigned long long part[2] = {0, 0};
-#pragma unroll 4
+  uint32_t count = 0;
+  unsigned long long part = 0;
+#pragma unroll 8
   for (int i = 0; i < n; ++i) {
     const Hist* r = &cl.map_shared_rank(&s, i)->hist[h];
-    const uint2 c = *reinterpret_cast<const uint2*>(&r->count[2 * tid]);
-    count[0] += c.x, count[1] += c.y;
-    if (by_mass) {
-      const uint2 u = *reinterpret_cast<const uint2*>(&r->high[2 * tid]);
-      const uint2 v = *reinterpret_cast<const uint2*>(&r->low[2 * tid]);
-      part[0] += ((unsigned long long)u.x << 16) + v.x;
-      part[1] += ((unsigned long long)u.y << 16) + v.y;
-    }
+    count += r->count[tid];
+    if (by_mass) part += ((unsigned long long)r->high[tid] << 16) + r->low[tid];
   }
   // in 2^-40 of the largest weight
-  const unsigned long long m0 = by_mass ? (unsigned long long)((double)part[0] * unit[0]) : count[0];
-  const unsigned long long m1 = by_mass ? (unsigned long long)((double)part[1] * unit[1]) : count[1];
-  unsigned long long run = m0 + m1;
+  const unsigned long long mine =
+      by_mass ? (unsigned long long)((double)part * (256.0 * (first ? expf(-0.0625f * tid) : weight))) : count;
+  unsigned long long run = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned long long v = __shfl_up_sync(0xffffffffu, run, o);
@@ -240,6 +231,7 @@ __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, 
   if (lane == 31) s.red64[w] = run;
   __syncthreads();
   unsigned long long before = 0, total = 0;
+#pragma unroll
   for (int i = 0; i < CT / 32; ++i) {
     const unsigned long long v = s.red64[i];
     before += i < w ? v : 0;
@@ -251,16 +243,10 @@ __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, 
     left = (unsigned long long)ceil((double)p * (double)total);
     if (left < 1) left = 1;
   }
-  const unsigned long long upto[2] = {run - m1, run}, mine[2] = {m0, m1};
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const bool at = upto[e] >= left && upto[e] - mine[e] < left;
-    const bool last = 2 * tid + e == BINS - 1 && upto[e] < left;
-    if (at || last) {
-      s.bin = 2 * tid + e;
-      s.found = count[e];
-      s.left = left - (upto[e] - mine[e]);
-    }
+  if ((run >= left && run - mine < left) || (tid == BINS - 1 && run < left)) {
+    s.bin = tid;
+    s.found = count;
+    s.left = left - (run - mine);
   }
   __syncthreads();
 }
@@ -321,22 +307,20 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     xs[j] = f != f ? none : u;
     top = fmaxf(top, f);
   }
-  const int n4 = (n + 3) / 4;
-  if (tid < n4 * 4 - n) xs[n + tid] = none;
-  // f(value, index in the CTA's part) for a thread's values, four at a time
+  const int n8 = (n + 7) / 8;
+  if (tid < n8 * 8 - n) xs[n + tid] = none;
+  // f(eight values, the first one's index in the CTA's part)
   auto each = [&](auto f) {
-    for (int j = tid; j < n4; j += CT) {
-      float v[4];
+    for (int j = tid; j < n8; j += CT) {
+      float v[8];
       if constexpr (sizeof(T) == 4) {
-        const float4 u = reinterpret_cast<const float4*>(xs)[j];
+        const float4 u = reinterpret_cast<const float4*>(xs)[2 * j], g = reinterpret_cast<const float4*>(xs)[2 * j + 1];
         v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+        v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
       } else {
-        const uint2 u = reinterpret_cast<const uint2*>(xs)[j];
-        const float2 g = unpack2<T>(u.x), h = unpack2<T>(u.y);
-        v[0] = g.x; v[1] = g.y; v[2] = h.x; v[3] = h.y;
+        unpack8<T>(reinterpret_cast<const uint4*>(xs)[j], v);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f(v[e], 4 * j + e);
+      f(v, 8 * j);
     }
   };
   for (int i = tid; i < BINS; i += CT) s.hist[0].count[i] = 0, s.hist[0].high[i] = 0, s.hist[0].low[i] = 0;
@@ -355,34 +339,60 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   const bool cut_k = !greedy && k > 0 && k < a.v, cut_p = !greedy && p < 1.f;
   const float inv = 1.f / ts, per = 16.f * inv;         // bins of 1/16 in z
   auto below = [&](float x) { return x == top ? 0.f : top - x; };
-  auto bin_of = [&](float d) { return (int)fminf(d * per, (float)(BINS - 1)); };
-  auto bin0 = [&](float x) { return bin_of(below(x)); };
+  // the first-level bin of a value, not yet cut to a whole number
+  auto place = [&](float x) { return fminf(below(x) * per, (float)(BINS - 1)); };
   auto weight = [&](float d) { return __expf(-d * inv); };
-  // a weight in units of its first-level bin's largest (the last bin's, below exp(-64), is left out)
+  // a weight in units of its first-level bin's largest (the last bin's, below exp(-31), is left out)
   auto part_of = [&](float d, int b) { return b == BINS - 1 ? 0.f : __expf(0.0625f * b - d * inv); };
+  // keys: order-preserving, without the bits that a 16-bit type leaves empty
+  constexpr int EMPTY = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+  auto key = [&](float x) { return key_of(x + 0.f) >> EMPTY; };
   float ties = 0.f, rest = 0.f;
-  if (cut_k || cut_p) {
-    const bool mass = cut_p && !cut_k;
-    each([&](float x, int) {
-      const float d = below(x);
-      if (d == 0.f) ties += 1.f;
-      else rest += weight(d);
-      if (x > -INFINITY) {
-        const int b = bin_of(d);
-        atomicAdd(&s.hist[0].count[b], 1u);
-        if (mass) add_mass(s.hist[0], b, part_of(d, b));
+  const bool cuts = cut_k || cut_p, mass = cut_p && !cut_k;
+  each([&](const float (&v)[8], int) {
+    float d[8], e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      d[i] = below(v[i]);
+      e[i] = weight(d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ties += d[i] == 0.f ? 1.f : 0.f;
+      rest += d[i] == 0.f ? 0.f : e[i];
+    }
+    if (cuts) {
+      int b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = (int)place(v[i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v[i] > -INFINITY) atomicAdd(&s.hist[0].count[b[i]], 1u);
+      if (mass) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = part_of(d[i], b[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (e[i] > 0.f) add_mass(s.hist[0], b[i], e[i]);
       }
-    });
-  } else {
-    each([&](float x, int) {
-      const float d = below(x);
-      if (d == 0.f) ties += 1.f;
-      else rest += weight(d);
-    });
+    }
+  });
+  {
+    // both sums at once
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ties += __shfl_xor_sync(0xffffffffu, ties, o);
+      rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    }
+    __syncthreads();
+    if (lane == 0) s.red[tid / 32] = ties, s.red[16 + tid / 32] = rest;
+    __syncthreads();
+    if (tid == 0) {
+      ties = rest = 0.f;
+      for (int i = 0; i < CT / 32; ++i) ties += s.red[i], rest += s.red[16 + i];
+      s.ties = ties, s.rest = rest;
+    }
   }
-  ties = block_reduce<CT / 32>(ties, s.red, [](float u, float v) { return u + v; });
-  rest = block_reduce<CT / 32>(rest, s.red, [](float u, float v) { return u + v; });
-  if (tid == 0) s.ties = ties, s.rest = rest;
   cl.sync();
   ties = over_cluster(cl, &s.ties, [](float u, float v) { return u + v; });
   rest = over_cluster(cl, &s.rest, [](float u, float v) { return u + v; });
@@ -399,15 +409,20 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       h ^= 1;
       for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].high[i] = 0, s.hist[h].low[i] = 0;
       __syncthreads();
-      each([&](float x, int) {
-        if (x > -INFINITY) {
-          const float d = below(x);
-          const int b = bin_of(d);
-          if (b < edge || (b == edge && key_of(x + 0.f) >= least)) {
-            atomicAdd(&s.hist[h].count[b], 1u);
-            add_mass(s.hist[h], b, part_of(d, b));
-          }
+      each([&](const float (&v)[8], int) {
+        bool in[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = place(v[i]);
+          in[i] = v[i] > -INFINITY && (f < (float)edge || (f < (float)(edge + 1) && key(v[i]) >= least));
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (in[i]) {
+            const int b = (int)place(v[i]);
+            atomicAdd(&s.hist[h].count[b], 1u);
+            add_mass(s.hist[h], b, part_of(below(v[i]), b));
+          }
       });
       cl.sync();
     }
@@ -424,23 +439,34 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       uint32_t lo = cut == BINS - 1 ? key_of(-INFINITY) + 1 : key_of(value(top - (cut + 1) * wide - slack));
       uint32_t hi = key_of(fminf(top, top - cut * wide + slack));
       if (!(fabsf(top) <= 3.4028235e38f)) lo = key_of(-INFINITY) + 1, hi = key_of(top);
+      lo >>= EMPTY;
+      hi >>= EMPTY;
       if (lo > hi) lo = hi;
       while (more) {
-        const int bits = 32 - __clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;
+        const int bits = 32 - __clz(hi - lo), shift = bits > 9 ? bits - 9 : 0;
         h ^= 1;
         // (find_bin's barriers are behind every CTA's reads of the other histogram only after the
         // cluster's next one: this one was last read a level ago)
         for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].high[i] = 0, s.hist[h].low[i] = 0;
         __syncthreads();
-        each([&](float x, int) {
-          const float d = below(x);
-          if (x > -INFINITY && bin_of(d) == cut) {
-            const uint32_t key = key_of(x + 0.f);
-            if (key >= lo && key <= hi && (cut < kept_edge || key >= kept_least)) {
-              const int b = BINS - 1 - (int)((key - lo) >> shift);      // descending, as the first level
-              atomicAdd(&s.hist[h].count[b], 1u);
-              if (by_mass) add_mass(s.hist[h], b, part_of(d, cut));
-            }
+        each([&](const float (&v)[8], int) {
+          uint32_t in = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float f = place(v[i]);
+            if (v[i] > -INFINITY && f >= (float)cut && f < (float)(cut + 1)) in |= 1u << i;
+          }
+          if (in) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (in >> i & 1u) {
+                const uint32_t q = key(v[i]);
+                if (q >= lo && q <= hi && (cut < kept_edge || q >= kept_least)) {
+                  const int b = BINS - 1 - (int)((q - lo) >> shift);      // descending, as the first level
+                  atomicAdd(&s.hist[h].count[b], 1u);
+                  if (by_mass) add_mass(s.hist[h], b, part_of(below(v[i]), cut));
+                }
+              }
           }
         });
         cl.sync();
@@ -469,24 +495,54 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   float best = -INFINITY;
   int at = -1;
   if (greedy) {
-    each([&](float x, int j) {
-      if (x > best) best = x, at = j;
+    each([&](const float (&v)[8], int j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v[i] > best) best = v[i], at = j + i;
     });
   } else {
-    each([&](float x, int j) {
-      if (!(x > -INFINITY)) return;
-      const float d = below(x);
-      if (edge < BINS) {
-        const int b = bin_of(d);
-        if (b > edge || (b == edge && key_of(x + 0.f) < least)) return;
+    const bool wide = reinterpret_cast<size_t>(noise) % 16 == 0 && a.v % 4 == 0;
+    each([&](const float (&v)[8], int j) {
+      uint32_t in = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bool kept = v[i] > -INFINITY;
+        if (edge < BINS) {
+          const float f = place(v[i]);
+          kept = kept && (f < (float)edge || (f < (float)(edge + 1) && key(v[i]) >= least));
+        }
+        const float d = below(v[i]);
+        if (minp > 0.f) kept = kept && (d == 0.f || -d * inv >= log_minp);
+        in |= (kept ? 1u : 0u) << i;
       }
-      const float z = -d * inv;
-      if (minp > 0.f && d != 0.f && !(z >= log_minp)) return;
-      const float r = __ldg(noise + j);
-      const float l = __logf(r), near = (direct ? shift + z : z) - l;
-      if (near + 1e-4f + 1e-5f * (fabsf(shift) + fabsf(z) + fabsf(l)) < best) return;
-      const float score = (direct ? x / ts : -(d / ts)) - logf(r);
-      if (score > best) best = score, at = j;           // (a thread's indices rise: the lowest on ties)
+      if (!in) return;
+      // all noise first: one trip to memory for the eight
+      float r[8];
+      if (wide && edge == BINS && i0 + j + 8 <= a.v) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(noise + j));
+        const float4 g = __ldg(reinterpret_cast<const float4*>(noise + j + 4));
+        r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
+        r[4] = g.x; r[5] = g.y; r[6] = g.z; r[7] = g.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = in >> i & 1u ? __ldg(noise + j + i) : 1.f;
+      }
+      float near[8];
+      bool maybe = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float z = -below(v[i]) * inv, l = __logf(r[i]);
+        near[i] = (direct ? shift + z : z) - l + (1e-4f + 1e-5f * (fabsf(shift) + fabsf(z) + fabsf(l)));
+        maybe |= (in >> i & 1u) && !(near[i] < best);
+      }
+      if (!maybe) return;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((in >> i & 1u) && !(near[i] < best)) {
+          const float d = below(v[i]);
+          const float score = (direct ? v[i] / ts : -(d / ts)) - logf(r[i]);
+          if (score > best) best = score, at = j + i;     // (a thread's indices rise: the lowest on ties)
+        }
     });
   }
   unsigned long long choice =
