@@ -171,18 +171,21 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
 }
 
 // ------------------------------------------------------------------ a cluster per row
-// A histogram over a CTA's part of the row.  The mass of a bin is in 2^-32 of a unit, the halves
-// of each addend summed apart (a 64-bit atomic in shared memory is a loop): at the first level the
-// unit of bin i is exp(-i / 16), the largest weight in it, at the others 1 at half the digits.
+// A histogram over a CTA's part of the row: how many values a bin has, and by how much their
+// weights fall short of the bin's largest (exp(-bin / 16), less than a sixteenth), in 2^-20 of it:
+// 16 bits a value, so that no sum over 65536 of them overflows.
 struct Hist {
-  uint32_t count[BINS], high[BINS], low[BINS];
+  uint32_t count[BINS], lack[BINS];
 };
+constexpr int LIST = 4096;             // values kept by the first level that a CTA lists
 struct Shared {
   Hist hist[2];                        // of alternate levels: a level clears the next one's
   float top, ties, rest;
   unsigned long long best;
   float red[32];
   unsigned long long red64[32];
+  uint32_t list[LIST];
+  uint32_t listed;
   int bin;
   uint32_t found;                      // the values in it
   unsigned long long left;             // of the target, before that bin
@@ -198,30 +201,35 @@ __device__ __forceinline__ V over_cluster(cg::cluster_group& cl, V* field, F f) 
   return v;
 }
 
-__device__ __forceinline__ void add_mass(Hist& h, int b, float part) {
-  const uint32_t u = (uint32_t)fminf(part * 4294967296.f, 4294967040.f);
-  atomicAdd(&h.high[b], u >> 16);
-  atomicAdd(&h.low[b], u & 0xffffu);
+// Adds a value of weight `part` times its first-level bin's largest (the last bin's weights, below
+// exp(-31), are left out).
+__device__ __forceinline__ void add_to(Hist& h, int b, bool by_mass, float part) {
+  atomicAdd(&h.count[b], 1u);
+  if (by_mass) {
+    const uint32_t lack = (uint32_t)fminf(fmaxf((1.f - part) * 1048576.f + 0.5f, 0.f), 65535.f);
+    if (lack) atomicAdd(&h.lack[b], lack);
+  }
 }
 
 // The cluster's histogram h: the first bin at which the running count (or mass) reaches `left`,
-// the last one if none does.  Thread i has bin i.  Masses are in units of exp(-bin /
-// 16) (`first`) or of `weight`.  Sets s.bin, s.found and s.left.
+// the last one if none does.  Thread i has bin i.  Masses are in
+// units of exp(-bin / 16) (`first`) or of `weight`.  Sets s.bin, s.found and s.left.
 __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, bool first, float p,
                          unsigned long long left, float weight) {
   static_assert(BINS == CT, "a bin a thread");
   const int tid = threadIdx.x, lane = tid % 32, w = tid / 32, n = cl.num_blocks();
   uint32_t count = 0;
-  unsigned long long part = 0;
+  unsigned long long lack = 0;
 #pragma unroll 8
   for (int i = 0; i < n; ++i) {
     const Hist* r = &cl.map_shared_rank(&s, i)->hist[h];
     count += r->count[tid];
-    if (by_mass) part += ((unsigned long long)r->high[tid] << 16) + r->low[tid];
+    if (by_mass) lack += r->lack[tid];
   }
   // in 2^-40 of the largest weight
+  const float unit = !first ? weight : tid == BINS - 1 ? 0.f : expf(-0.0625f * tid);
   const unsigned long long mine =
-      by_mass ? (unsigned long long)((double)part * (256.0 * (first ? expf(-0.0625f * tid) : weight))) : count;
+      by_mass ? (unsigned long long)((double)(((unsigned long long)count << 20) - lack) * (1048576.0 * unit)) : count;
   unsigned long long run = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -323,8 +331,8 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       f(v, 8 * j);
     }
   };
-  for (int i = tid; i < BINS; i += CT) s.hist[0].count[i] = 0, s.hist[0].high[i] = 0, s.hist[0].low[i] = 0;
-  if (tid == 0) s.best = 0;
+  for (int i = tid; i < BINS; i += CT) s.hist[0].count[i] = 0, s.hist[0].lack[i] = 0;
+  if (tid == 0) s.best = 0, s.listed = 0;
   top = block_reduce<CT / 32>(top, s.red, [](float u, float v) { return fmaxf(u, v); });
   if (tid == 0) s.top = top;
   cl.sync();
@@ -342,8 +350,8 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   // the first-level bin of a value, not yet cut to a whole number
   auto place = [&](float x) { return fminf(below(x) * per, (float)(BINS - 1)); };
   auto weight = [&](float d) { return __expf(-d * inv); };
-  // a weight in units of its first-level bin's largest (the last bin's, below exp(-31), is left out)
-  auto part_of = [&](float d, int b) { return b == BINS - 1 ? 0.f : __expf(0.0625f * b - d * inv); };
+  // a weight in units of its first-level bin's largest
+  auto part_of = [&](float d, int b) { return __expf(0.0625f * b - d * inv); };
   // keys: order-preserving, without the bits that a 16-bit type leaves empty
   constexpr int EMPTY = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
   auto key = [&](float x) { return key_of(x + 0.f) >> EMPTY; };
@@ -365,16 +373,13 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       int b[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) b[i] = (int)place(v[i]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (v[i] > -INFINITY) atomicAdd(&s.hist[0].count[b[i]], 1u);
       if (mass) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = part_of(d[i], b[i]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (e[i] > 0.f) add_mass(s.hist[0], b[i], e[i]);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v[i] > -INFINITY) add_to(s.hist[0], b[i], mass, e[i]);
     }
   });
   {
@@ -403,38 +408,65 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   int edge = BINS;
   uint32_t least = 0;
   int h = 0;
-  for (int by_mass = 0; by_mass < 2; ++by_mass) {
-    if (by_mass ? !cut_p : !cut_k) continue;
-    if (by_mass && cut_k) {            // the mass of what k kept
-      h ^= 1;
-      for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].high[i] = 0, s.hist[h].low[i] = 0;
-      __syncthreads();
-      each([&](const float (&v)[8], int) {
-        bool in[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float f = place(v[i]);
-          in[i] = v[i] > -INFINITY && (f < (float)edge || (f < (float)(edge + 1) && key(v[i]) >= least));
-        }
+  bool listing = false;
+  // f(value, index) for what the first level kept, from the list where that holds it all
+  auto visit = [&](auto f) {
+    if (listing) {
+      for (int i = tid; i < (int)s.listed; i += CT) f(to_f32(xs[s.list[i]]), (int)s.list[i]);
+    } else {
+      each([&](const float (&v)[8], int j) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (in[i]) {
-            const int b = (int)place(v[i]);
-            atomicAdd(&s.hist[h].count[b], 1u);
-            add_mass(s.hist[h], b, part_of(below(v[i]), b));
-          }
+          if (v[i] > -INFINITY) f(v[i], j + i);
+      });
+    }
+  };
+  for (int by_mass = 0; by_mass < 2; ++by_mass) {
+    if (by_mass ? !cut_p : !cut_k) continue;
+    const int kept_edge = edge;
+    const uint32_t kept_least = least;
+    auto kept = [&](float x) {
+      const float f = place(x);
+      return f < (float)kept_edge || (f < (float)(kept_edge + 1) && key(x) >= kept_least);
+    };
+    if (by_mass && cut_k) {            // the mass of what k kept
+      h ^= 1;
+      for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].lack[i] = 0;
+      __syncthreads();
+      visit([&](float x, int) {
+        if (kept(x)) {
+          const int b = (int)place(x);
+          add_to(s.hist[h], b, true, part_of(below(x), b));
+        }
       });
       cl.sync();
     }
     find_bin(cl, s, h, by_mass, true, p, (unsigned long long)k, 1.f);
-    int cut = s.bin;
+    const int cut = s.bin;
     uint32_t from = 0;
     unsigned long long left = s.left;
     bool more = s.found > 1 && !(!by_mass && left >= s.found);
-    const int kept_edge = edge;
-    const uint32_t kept_least = least;
+    if (!listing) {
+      // from here on only the values up to this bin matter
+      each([&](const float (&v)[8], int j) {
+        uint32_t in = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) in |= (v[i] > -INFINITY && place(v[i]) < (float)(cut + 1) ? 1u : 0u) << i;
+        if (in) {
+          uint32_t at = atomicAdd(&s.listed, (uint32_t)__popc(in));
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (in >> i & 1u) {
+              if (at < LIST) s.list[at] = (uint32_t)(j + i);
+              ++at;
+            }
+        }
+      });
+      __syncthreads();
+      listing = s.listed <= LIST;
+    }
     if (more) {
-      // the keys that bin `cut` can hold (its bounds, widened by the roundings of bin_of)
+      // the keys that bin `cut` can hold (its bounds, widened by the roundings of place)
       const float wide = 1.f / per, slack = (fabsf(top) + (cut + 1) * wide) * 1e-6f;
       uint32_t lo = cut == BINS - 1 ? key_of(-INFINITY) + 1 : key_of(value(top - (cut + 1) * wide - slack));
       uint32_t hi = key_of(fminf(top, top - cut * wide + slack));
@@ -442,35 +474,23 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       lo >>= EMPTY;
       hi >>= EMPTY;
       if (lo > hi) lo = hi;
+      const float unit = cut == BINS - 1 ? 0.f : expf(-0.0625f * cut);
       while (more) {
         const int bits = 32 - __clz(hi - lo), shift = bits > 9 ? bits - 9 : 0;
         h ^= 1;
-        // (find_bin's barriers are behind every CTA's reads of the other histogram only after the
-        // cluster's next one: this one was last read a level ago)
-        for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].high[i] = 0, s.hist[h].low[i] = 0;
+        // (this histogram was last read before the cluster's last barrier but one)
+        for (int i = tid; i < BINS; i += CT) s.hist[h].count[i] = 0, s.hist[h].lack[i] = 0;
         __syncthreads();
-        each([&](const float (&v)[8], int) {
-          uint32_t in = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float f = place(v[i]);
-            if (v[i] > -INFINITY && f >= (float)cut && f < (float)(cut + 1)) in |= 1u << i;
-          }
-          if (in) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (in >> i & 1u) {
-                const uint32_t q = key(v[i]);
-                if (q >= lo && q <= hi && (cut < kept_edge || q >= kept_least)) {
-                  const int b = BINS - 1 - (int)((q - lo) >> shift);      // descending, as the first level
-                  atomicAdd(&s.hist[h].count[b], 1u);
-                  if (by_mass) add_mass(s.hist[h], b, part_of(below(v[i]), cut));
-                }
-              }
+        visit([&](float x, int) {
+          const float f = place(x);
+          if (f >= (float)cut && f < (float)(cut + 1)) {
+            const uint32_t q = key(x);
+            if (q >= lo && q <= hi && (cut < kept_edge || q >= kept_least))
+              add_to(s.hist[h], BINS - 1 - (int)((q - lo) >> shift), by_mass, part_of(below(x), cut));   // descending
           }
         });
         cl.sync();
-        find_bin(cl, s, h, by_mass, false, p, left, expf(-0.0625f * cut));
+        find_bin(cl, s, h, by_mass, false, p, left, unit);
         const uint32_t b = BINS - 1 - s.bin;
         left = s.left;
         from = lo + (b << shift);
@@ -500,50 +520,75 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       for (int i = 0; i < 8; ++i)
         if (v[i] > best) best = v[i], at = j + i;
     });
+  } else if (listing) {
+    visit([&](float x, int j) {
+      const float f = place(x), d = below(x);
+      if (f > (float)edge && (f >= (float)(edge + 1) || key(x) < least)) return;
+      if (f >= (float)edge && key(x) < least) return;
+      if (minp > 0.f && d != 0.f && !(-d * inv >= log_minp)) return;
+      const float score = (direct ? x / ts : -(d / ts)) - logf(__ldg(noise + j));
+      if (score > best || (score == best && score > -INFINITY && j < at)) best = score, at = j;
+    });
   } else {
-    const bool wide = reinterpret_cast<size_t>(noise) % 16 == 0 && a.v % 4 == 0;
-    each([&](const float (&v)[8], int j) {
+    const bool wide = reinterpret_cast<size_t>(noise) % 16 == 0;
+    float bound = -INFINITY;             // no score of the warp's that counts is below this
+    for (int j0 = 0; j0 < n8; j0 += CT) {
+      // (whole warps: the bound is the warp's)
+      const int j8 = j0 + tid, j = 8 * j8;
+      const bool live = j8 < n8;
+      float v[8];
+      if (live) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 u = reinterpret_cast<const float4*>(xs)[2 * j8], g = reinterpret_cast<const float4*>(xs)[2 * j8 + 1];
+          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+          v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
+        } else {
+          unpack8<T>(reinterpret_cast<const uint4*>(xs)[j8], v);
+        }
+      }
       uint32_t in = 0;
+      float r[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        bool kept = v[i] > -INFINITY;
+        bool ok = live && v[i] > -INFINITY;
         if (edge < BINS) {
           const float f = place(v[i]);
-          kept = kept && (f < (float)edge || (f < (float)(edge + 1) && key(v[i]) >= least));
+          ok = ok && (f < (float)edge || (f < (float)(edge + 1) && key(v[i]) >= least));
         }
         const float d = below(v[i]);
-        if (minp > 0.f) kept = kept && (d == 0.f || -d * inv >= log_minp);
-        in |= (kept ? 1u : 0u) << i;
+        if (minp > 0.f) ok = ok && (d == 0.f || -d * inv >= log_minp);
+        in |= (ok ? 1u : 0u) << i;
+        r[i] = 1.f;
       }
-      if (!in) return;
       // all noise first: one trip to memory for the eight
-      float r[8];
-      if (wide && edge == BINS && i0 + j + 8 <= a.v) {
+      if (wide && in == 255u) {
         const float4 u = __ldg(reinterpret_cast<const float4*>(noise + j));
         const float4 g = __ldg(reinterpret_cast<const float4*>(noise + j + 4));
         r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
         r[4] = g.x; r[5] = g.y; r[6] = g.z; r[7] = g.w;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = in >> i & 1u ? __ldg(noise + j + i) : 1.f;
+        for (int i = 0; i < 8; ++i)
+          if (in >> i & 1u) r[i] = __ldg(noise + j + i);
       }
-      float near[8];
-      bool maybe = false;
+      float high[8], sure = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float z = -below(v[i]) * inv, l = __logf(r[i]);
-        near[i] = (direct ? shift + z : z) - l + (1e-4f + 1e-5f * (fabsf(shift) + fabsf(z) + fabsf(l)));
-        maybe |= (in >> i & 1u) && !(near[i] < best);
+        const float z = -below(v[i]) * inv, l = __logf(r[i]), near = (direct ? shift + z : z) - l;
+        const float off = 1e-4f + 1e-5f * (fabsf(shift) + fabsf(z) + fabsf(l));
+        high[i] = near + off;
+        if (in >> i & 1u) sure = fmaxf(sure, near - off);
       }
-      if (!maybe) return;
+      const uint32_t most = __reduce_max_sync(0xffffffffu, key_of(sure + 0.f));
+      bound = fmaxf(bound, __uint_as_float(most ^ (most >> 31 ? 0x80000000u : 0xffffffffu)));
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if ((in >> i & 1u) && !(near[i] < best)) {
+        if ((in >> i & 1u) && !(high[i] < bound)) {
           const float d = below(v[i]);
           const float score = (direct ? v[i] / ts : -(d / ts)) - logf(r[i]);
           if (score > best) best = score, at = j + i;     // (a thread's indices rise: the lowest on ties)
         }
-    });
+    }
   }
   unsigned long long choice =
       at < 0 ? 0 : ((unsigned long long)key_of(best + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + at));
