@@ -177,14 +177,14 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
 struct Hist {
   uint32_t count[BINS], lack[BINS];
 };
-constexpr int LIST = 4096;             // values kept by the first level that a CTA lists
+constexpr int LIST = 8192;             // values kept by the first level that a CTA lists (by 16-bit index)
 struct Shared {
   Hist hist[2];                        // of alternate levels: a level clears the next one's
   float top, ties, rest;
   unsigned long long best;
   float red[32];
   unsigned long long red64[32];
-  uint32_t list[LIST];
+  unsigned short list[LIST];
   uint32_t listed;
   int bin;
   uint32_t found;                      // the values in it
@@ -203,6 +203,17 @@ __device__ __forceinline__ V over_cluster(cg::cluster_group& cl, V* field, F f) 
 
 // Adds a value of weight `part` times its first-level bin's largest (the last bin's weights, below
 // exp(-31), are left out).
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_of(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void add_to(Hist& h, int b, bool by_mass, float part) {
   atomicAdd(&h.count[b], 1u);
   if (by_mass) {
@@ -278,6 +289,11 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
 
   // ---- this CTA's part of the row
   const int i0 = rank * chunk, n = max(0, min(chunk, a.v - i0));
+  const bool cut_k = !greedy && k > 0 && k < a.v, cut_p = !greedy && p < 1.f, cuts = cut_k || cut_p;
+  const float* noise = a.noise + row * a.noise_ld + i0;
+  if (!greedy && !cuts && !(minp > 0.f)) {              // all of the noise is wanted: into L2 while the row is read
+    for (int j = tid * 32; j < n; j += CT * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + j));
+  }
   const T* src = l + i0;
   float top = -INFINITY;
   constexpr int E = 16 / sizeof(T);
@@ -315,19 +331,24 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     xs[j] = f != f ? none : u;
     top = fmaxf(top, f);
   }
+  top = top + 0.f;
+  const float mine = top;              // the thread's largest
   const int n8 = (n + 7) / 8;
   if (tid < n8 * 8 - n) xs[n + tid] = none;
+  auto values = [&](int j8, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 u = reinterpret_cast<const float4*>(xs)[2 * j8], g = reinterpret_cast<const float4*>(xs)[2 * j8 + 1];
+      v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
+    } else {
+      unpack8<T>(reinterpret_cast<const uint4*>(xs)[j8], v);
+    }
+  };
   // f(eight values, the first one's index in the CTA's part)
   auto each = [&](auto f) {
     for (int j = tid; j < n8; j += CT) {
       float v[8];
-      if constexpr (sizeof(T) == 4) {
-        const float4 u = reinterpret_cast<const float4*>(xs)[2 * j], g = reinterpret_cast<const float4*>(xs)[2 * j + 1];
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-        v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
-      } else {
-        unpack8<T>(reinterpret_cast<const uint4*>(xs)[j], v);
-      }
+      values(j, v);
       f(v, 8 * j);
     }
   };
@@ -344,35 +365,98 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   }
 
   // ---- log sum, and the first histogram
-  const bool cut_k = !greedy && k > 0 && k < a.v, cut_p = !greedy && p < 1.f;
   const float inv = 1.f / ts, per = 16.f * inv;         // bins of 1/16 in z
   auto below = [&](float x) { return x == top ? 0.f : top - x; };
   // the first-level bin of a value, not yet cut to a whole number
   auto place = [&](float x) { return fminf(below(x) * per, (float)(BINS - 1)); };
-  auto weight = [&](float d) { return __expf(-d * inv); };
   // a weight in units of its first-level bin's largest
   auto part_of = [&](float d, int b) { return __expf(0.0625f * b - d * inv); };
   // keys: order-preserving, without the bits that a 16-bit type leaves empty
   constexpr int EMPTY = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
   auto key = [&](float x) { return key_of(x + 0.f) >> EMPTY; };
+  // For a k well below the number of threads, k of the threads' largest values bound the k-th
+  // largest from below: what is under that bound goes into no histogram, and what is not is listed
+  // in the pass that sums the weights.
+  int h = 0, edge = BINS;
+  uint32_t least = 0;
+  bool listing = false;
+  const bool bounded = cut_k && k <= (int)cl.num_blocks() * (CT / 2);
+  const bool by_least = !greedy && !cuts && minp > 0.f;
+  float list_from = INFINITY;
+  if (bounded) {
+    if (mine > -INFINITY) atomicAdd(&s.hist[0].count[(int)place(mine)], 1u);
+    cl.sync();
+    find_bin(cl, s, 0, false, true, p, (unsigned long long)k, 1.f);
+    h = 1;
+    for (int i = tid; i < BINS; i += CT) s.hist[1].count[i] = 0, s.hist[1].lack[i] = 0;
+  }
+  // a value that every value of bins up to `bin` reaches (place's roundings allowed for)
+  auto floor_of = [&](int bin) {
+    if (bin >= BINS - 1 || !(fabsf(top) <= 3.4028235e38f)) return -3.4028235e38f;
+    const float wide = (bin + 1) * (0.0625f * ts);
+    return top - wide - (fabsf(top) + wide) * 1e-6f;
+  };
+  // lists the values from `least` on
+  auto list = [&](const float (&v)[8], int j, float least) {
+    uint32_t in = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) in |= (v[i] >= least ? 1u : 0u) << i;
+    if (in) {
+      uint32_t at = atomicAdd(&s.listed, (uint32_t)__popc(in));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (in >> i & 1u) {
+          if (at < LIST) s.list[at] = (unsigned short)(j + i);
+          ++at;
+        }
+    }
+  };
+  // f(value, index) for what is listed, or for every value where the list did not hold it
+  auto visit = [&](auto f) {
+    if (listing) {
+      for (int i = tid; i < (int)s.listed; i += CT) f(to_f32(xs[s.list[i]]), (int)s.list[i]);
+    } else {
+      each([&](const float (&v)[8], int j) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (v[i] > -INFINITY) f(v[i], j + i);
+      });
+    }
+  };
+  if (bounded) list_from = floor_of(s.bin);
+  if (by_least) {
+    const float deep = fmaxf(-log_minp * ts, 0.f);
+    list_from = fabsf(top) <= 3.4028235e38f ? fmaxf(top - deep - (fabsf(top) + deep) * 1e-5f, -3.4028235e38f)
+                                            : -3.4028235e38f;
+  }
   float ties = 0.f, rest = 0.f;
-  const bool cuts = cut_k || cut_p, mass = cut_p && !cut_k;
-  each([&](const float (&v)[8], int) {
-    float d[8], e[8];
+  const bool mass = cut_p && !cut_k;
+  const float rate = -1.44269504f * inv;         // weights as powers of two
+  if (!cuts || bounded) {
+    each([&](const float (&v)[8], int j) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      d[i] = below(v[i]);
-      e[i] = weight(d[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ties += d[i] == 0.f ? 1.f : 0.f;
-      rest += d[i] == 0.f ? 0.f : e[i];
-    }
-    if (cuts) {
+      for (int i = 0; i < 8; ++i) {
+        const float e = exp2_of(rate * (top - v[i]));
+        if (v[i] == top) ties += 1.f;
+        else rest += e;
+      }
+      if (list_from < INFINITY) list(v, j, list_from);
+    });
+  } else {
+    each([&](const float (&v)[8], int j) {
+      float d[8], e[8];
       int b[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = (int)place(v[i]);
+      for (int i = 0; i < 8; ++i) {
+        d[i] = below(v[i]);
+        e[i] = exp2_of(rate * d[i]);
+        b[i] = (int)place(v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (d[i] == 0.f) ties += 1.f;
+        else rest += e[i];
+      }
       if (mass) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = part_of(d[i], b[i]);
@@ -380,10 +464,10 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (v[i] > -INFINITY) add_to(s.hist[0], b[i], mass, e[i]);
-    }
-  });
+    });
+  }
   {
-    // both sums at once
+    // both sums at once; they are joined over the cluster with the choice
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       ties += __shfl_xor_sync(0xffffffffu, ties, o);
@@ -398,29 +482,14 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       s.ties = ties, s.rest = rest;
     }
   }
-  cl.sync();
-  ties = over_cluster(cl, &s.ties, [](float u, float v) { return u + v; });
-  rest = over_cluster(cl, &s.rest, [](float u, float v) { return u + v; });
-  const float lse = logf(ties) + log1pf(rest / ties);
+  if (bounded || by_least) listing = s.listed <= LIST;
+  if (bounded) {
+    visit([&](float x, int) { add_to(s.hist[1], (int)place(x), false, 0.f); });
+  }
+  if (cuts) cl.sync();
 
   // ---- the cuts: what is kept is every value in a bin before `edge`, and in it the keys from
   // `least` on
-  int edge = BINS;
-  uint32_t least = 0;
-  int h = 0;
-  bool listing = false;
-  // f(value, index) for what the first level kept, from the list where that holds it all
-  auto visit = [&](auto f) {
-    if (listing) {
-      for (int i = tid; i < (int)s.listed; i += CT) f(to_f32(xs[s.list[i]]), (int)s.list[i]);
-    } else {
-      each([&](const float (&v)[8], int j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (v[i] > -INFINITY) f(v[i], j + i);
-      });
-    }
-  };
   for (int by_mass = 0; by_mass < 2; ++by_mass) {
     if (by_mass ? !cut_p : !cut_k) continue;
     const int kept_edge = edge;
@@ -448,20 +517,11 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     bool more = s.found > 1 && !(!by_mass && left >= s.found);
     if (!listing) {
       // from here on only the values up to this bin matter
-      each([&](const float (&v)[8], int j) {
-        uint32_t in = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) in |= (v[i] > -INFINITY && place(v[i]) < (float)(cut + 1) ? 1u : 0u) << i;
-        if (in) {
-          uint32_t at = atomicAdd(&s.listed, (uint32_t)__popc(in));
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (in >> i & 1u) {
-              if (at < LIST) s.list[at] = (uint32_t)(j + i);
-              ++at;
-            }
-        }
-      });
+      __syncthreads();
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+      const float from = floor_of(cut);
+      each([&](const float (&v)[8], int j) { list(v, j, from); });
       __syncthreads();
       listing = s.listed <= LIST;
     }
@@ -506,12 +566,10 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   }
 
   // ---- the choice
-  // The score is l / T - log(noise) where that is in range, z - log(noise) where it is not.  Most
-  // values are far from the best so far: fast arithmetic (off by less than 1e-4 and 1e-5 of its
-  // terms) passes over them.
-  const float* noise = a.noise + row * a.noise_ld + i0;
+  // The score is l / T - log(noise) where that is in range, z - log(noise) where it is not.
   const float shift = top * inv;
   const bool direct = fabsf(top / ts) <= 3.4028235e38f;
+  auto score_of = [&](float x, float r) { return (direct ? x / ts : -(below(x) / ts)) - logf(r); };
   float best = -INFINITY;
   int at = -1;
   if (greedy) {
@@ -520,74 +578,57 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       for (int i = 0; i < 8; ++i)
         if (v[i] > best) best = v[i], at = j + i;
     });
-  } else if (listing) {
+  } else if (cuts || by_least) {
     visit([&](float x, int j) {
       const float f = place(x), d = below(x);
-      if (f > (float)edge && (f >= (float)(edge + 1) || key(x) < least)) return;
-      if (f >= (float)edge && key(x) < least) return;
+      if (f >= (float)edge && (f >= (float)(edge + 1) || key(x) < least)) return;
       if (minp > 0.f && d != 0.f && !(-d * inv >= log_minp)) return;
-      const float score = (direct ? x / ts : -(d / ts)) - logf(__ldg(noise + j));
+      const float score = score_of(x, __ldg(noise + j));
       if (score > best || (score == best && score > -INFINITY && j < at)) best = score, at = j;
     });
   } else {
+    // Every value's noise.  Fast arithmetic (off by less than `off`) passes over all that the best
+    // of the warp so far rules out, which leaves a handful for the division and the logarithm.
     const bool wide = reinterpret_cast<size_t>(noise) % 16 == 0;
+    const float off = 1e-3f + 1e-5f * fabsf(shift);
     float bound = -INFINITY;             // no score of the warp's that counts is below this
-    for (int j0 = 0; j0 < n8; j0 += CT) {
-      // (whole warps: the bound is the warp's)
-      const int j8 = j0 + tid, j = 8 * j8;
-      const bool live = j8 < n8;
-      float v[8];
-      if (live) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 u = reinterpret_cast<const float4*>(xs)[2 * j8], g = reinterpret_cast<const float4*>(xs)[2 * j8 + 1];
-          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-          v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
+    for (int j0 = 0; j0 < n8; j0 += CT) {      // (whole warps)
+      const int j = 8 * (j0 + tid);
+      float v[8], r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = -INFINITY, r[i] = 1.f;
+      if (j < n) {
+        if (wide && j + 8 <= n) {
+          const float4 u = __ldg(reinterpret_cast<const float4*>(noise + j));
+          const float4 q = __ldg(reinterpret_cast<const float4*>(noise + j + 4));
+          r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
+          r[4] = q.x; r[5] = q.y; r[6] = q.z; r[7] = q.w;
         } else {
-          unpack8<T>(reinterpret_cast<const uint4*>(xs)[j8], v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (j + i < n) r[i] = __ldg(noise + j + i);
         }
+        values(j / 8, v);
       }
-      uint32_t in = 0;
-      float r[8];
+      float high[8], sure = -INFINITY, peak = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        bool ok = live && v[i] > -INFINITY;
-        if (edge < BINS) {
-          const float f = place(v[i]);
-          ok = ok && (f < (float)edge || (f < (float)(edge + 1) && key(v[i]) >= least));
-        }
-        const float d = below(v[i]);
-        if (minp > 0.f) ok = ok && (d == 0.f || -d * inv >= log_minp);
-        in |= (ok ? 1u : 0u) << i;
-        r[i] = 1.f;
-      }
-      // all noise first: one trip to memory for the eight
-      if (wide && in == 255u) {
-        const float4 u = __ldg(reinterpret_cast<const float4*>(noise + j));
-        const float4 g = __ldg(reinterpret_cast<const float4*>(noise + j + 4));
-        r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
-        r[4] = g.x; r[5] = g.y; r[6] = g.z; r[7] = g.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (in >> i & 1u) r[i] = __ldg(noise + j + i);
-      }
-      float high[8], sure = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float z = -below(v[i]) * inv, l = __logf(r[i]), near = (direct ? shift + z : z) - l;
-        const float off = 1e-4f + 1e-5f * (fabsf(shift) + fabsf(z) + fabsf(l));
-        high[i] = near + off;
-        if (in >> i & 1u) sure = fmaxf(sure, near - off);
+        const float z = v[i] == top ? 0.f : (v[i] - top) * inv;
+        const float near = fmaf(-0.693147181f, log2_of(r[i]), direct ? z + shift : z), o = fmaf(-1e-6f, z, off);
+        high[i] = near + o;
+        peak = fmaxf(peak, high[i]);
+        sure = fmaxf(sure, near - o);
       }
       const uint32_t most = __reduce_max_sync(0xffffffffu, key_of(sure + 0.f));
       bound = fmaxf(bound, __uint_as_float(most ^ (most >> 31 ? 0x80000000u : 0xffffffffu)));
+      if (!(peak < bound)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if ((in >> i & 1u) && !(high[i] < bound)) {
-          const float d = below(v[i]);
-          const float score = (direct ? v[i] / ts : -(d / ts)) - logf(r[i]);
-          if (score > best) best = score, at = j + i;     // (a thread's indices rise: the lowest on ties)
-        }
+        for (int i = 0; i < 8; ++i)
+          if (v[i] > -INFINITY && !(high[i] < bound)) {
+            const float score = score_of(v[i], r[i]);
+            if (score > best) best = score, at = j + i;     // (a thread's indices rise: the lowest on ties)
+          }
+      }
     }
   }
   unsigned long long choice =
@@ -599,21 +640,34 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   }
   if (lane == 0 && choice) atomicMax(&s.best, choice);
   cl.sync();
-  if (rank == 0 && tid == 0) {
-    const unsigned long long c = over_cluster(
-        cl, &s.best, [](unsigned long long u, unsigned long long v) { return u > v ? u : v; });
-    if (c == 0) {
-      a.tokens[row] = -1, a.logprobs[row] = -INFINITY;
-    } else {
+  if (rank == 0 && tid < 32) {
+    // a lane per CTA, joined in a fixed order
+    unsigned long long c = 0;
+    float all_ties = 0.f, all_rest = 0.f;
+    if (lane < (int)cl.num_blocks()) {
+      const Shared* r = cl.map_shared_rank(&s, lane);
+      c = r->best;
+      all_ties = r->ties;
+      all_rest = r->rest;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const unsigned long long u = __shfl_down_sync(0xffffffffu, c, o);
+      if (u > c) c = u;
+      all_ties += __shfl_down_sync(0xffffffffu, all_ties, o);
+      all_rest += __shfl_down_sync(0xffffffffu, all_rest, o);
+    }
+    if (lane == 0) {
       const int i = (int)(0xffffffffu - (uint32_t)c);
-      a.tokens[row] = i;
-      a.logprobs[row] = scaled(value(to_f32(l[i])), top, ts) - lse;
+      a.tokens[row] = c ? i : -1;
+      a.logprobs[row] =
+          c ? scaled(value(to_f32(l[i])), top, ts) - (logf(all_ties) + log1pf(all_rest / all_ties)) : -INFINITY;
     }
   }
   cl.sync();
 }
 
-constexpr int CHUNK_MAX = 176 * 1024;   // bytes of a row in a CTA (one an SM beyond 80 KB)
+constexpr int CHUNK_MAX = 128 * 1024;   // bytes of a row in a CTA: at most 65536 values (one an SM beyond 80 KB)
 
 template <typename T>
 int run(const SampleArgs& a, cudaStream_t st) {
