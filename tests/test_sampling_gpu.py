@@ -117,6 +117,34 @@ def test_process_parts_alone_and_scalars():
     assert V.process_logits(ld[:0], td[:0]).shape == (0, 700) and V.process_logits(ld[:, :0]).shape == (4, 0)
 
 
+@pytest.mark.parametrize("v", [50000, 262144, 500000, 900001])
+def test_process_large_vocabularies(v):
+    """Counters for a cluster of up to sixteen CTAs, and beyond what one holds."""
+    g = torch.Generator().manual_seed(v)
+    l = torch.randn(2, v, generator=g)
+    tokens = torch.randint(0, v, (2, 3000), generator=g)
+    tokens[:, 500:900] = v - 1
+    ids = torch.randint(0, v, (2, 40), generator=g)
+    values = torch.randn(2, 40, generator=g)
+    ones = np.ones(2)
+    ref, size = process_reference(l, tokens, None, torch.tensor([100, 2000]), 1.7 * ones, 0.3 * ones, 0.01 * ones, ids,
+                                  values, None)
+    out = V.process_logits(l.cuda(), tokens.cuda(), None, torch.tensor([100, 2000]).cuda(), repetition_penalty=1.7,
+                           presence_penalty=0.3, frequency_penalty=0.01, bias_ids=ids.cuda(), bias_values=values.cuda())
+    check_process(out, ref, size, torch.float32)
+
+
+def test_process_many_biases():
+    """More biases in one CTA's range than it lists, with repeats."""
+    g = torch.Generator().manual_seed(11)
+    l = torch.randn(2, 3000, generator=g)
+    ids = torch.randint(0, 2000, (2, 2500), generator=g)
+    values = torch.randn(2, 2500, generator=g)
+    ones = np.ones(2)
+    ref, size = process_reference(l, None, None, None, ones, ones, ones, ids, values, None)
+    check_process(V.process_logits(l.cuda(), bias_ids=ids.cuda(), bias_values=values.cuda()), ref, size, torch.float32)
+
+
 def test_process_equal_bias_ids_the_last_holds():
     l = torch.zeros(2, 64, device="cuda")
     ids = torch.tensor([[3, 5, 3, 3], [7, 7, 8, -1]], device="cuda")
