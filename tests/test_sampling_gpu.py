@@ -119,7 +119,6 @@ def test_process_parts_alone_and_scalars():
 
 @pytest.mark.parametrize("v", [50000, 262144, 500000, 900001])
 def test_process_large_vocabularies(v):
-    """Counters for a cluster of up to sixteen CTAs, and beyond what one holds."""
     g = torch.Generator().manual_seed(v)
     l = torch.randn(2, v, generator=g)
     tokens = torch.randint(0, v, (2, 3000), generator=g)
@@ -131,6 +130,20 @@ def test_process_large_vocabularies(v):
                                   values, None)
     out = V.process_logits(l.cuda(), tokens.cuda(), None, torch.tensor([100, 2000]).cuda(), repetition_penalty=1.7,
                            presence_penalty=0.3, frequency_penalty=0.01, bias_ids=ids.cuda(), bias_values=values.cuda())
+    check_process(out, ref, size, torch.float32)
+
+
+def test_process_very_long_history():
+    """A history beyond the 20 bits of a counter."""
+    n = (1 << 20) + 77
+    tokens = torch.full((1, n), 5)
+    tokens[0, ::3] = 100
+    l = torch.zeros(1, 300)
+    ref, size = process_reference(l, tokens, None, torch.tensor([3]), np.ones(1), 0.25 * np.ones(1),
+                                  2.0 ** -10 * np.ones(1), torch.tensor([[5, 7]]), torch.tensor([[1.0, 2.0]]), None)
+    out = V.process_logits(l.cuda(), tokens.cuda(), None, torch.tensor([3]).cuda(), presence_penalty=0.25,
+                           frequency_penalty=2.0 ** -10, bias_ids=torch.tensor([[5, 7]]).cuda(),
+                           bias_values=torch.tensor([[1.0, 2.0]]).cuda())
     check_process(out, ref, size, torch.float32)
 
 

@@ -278,8 +278,9 @@ __global__ void __launch_bounds__(STAGE_NT) int4_stage_x(const T* __restrict__ x
 
 // The terms of one output that leave_out zeroed, over the group that starts at input k0.
 template <typename T>
-__device__ __noinline__ float left_out(const Int4Args& a, const T* x, long long row, int k0, int group) {
-  const int k1 = min(k0 + group, a.k);
+__device__ __noinline__ float left_out(const T* x, const uint8_t* q, const T* s, const uint8_t* z, int n, int k_all,
+                                       long long row, int k0, int group) {
+  const int k1 = min(k0 + group, k_all);
   float top = 0.f;
   for (int k = k0; k < k1; ++k) {
     const float m = fabsf(to_f32(x[k]));
@@ -294,13 +295,13 @@ __device__ __noinline__ float left_out(const Int4Args& a, const T* x, long long 
     }
   }
   const bool alone = low && high <= group / 16;
-  const long long at = (long long)(k0 / group) * a.n + row;
-  const float zero = a.z ? (float)a.z[at] : 8.f, scale = to_f32(static_cast<const T*>(a.s)[at]);
+  const long long at = (long long)(k0 / group) * n + row;
+  const float zero = z ? (float)z[at] : 8.f, scale = to_f32(s[at]);
   float v = 0.f;
   for (int k = k0; k < k1; ++k) {
     const float xv = to_f32(x[k]);
     if (fabsf(xv) <= FINITE && !(alone && fabsf(xv) >= top * APART)) continue;
-    const uint8_t by = a.q[row * (a.k / 2) + k / 2];
+    const uint8_t by = q[row * (k_all / 2) + k / 2];
     v += xv * (((float)(k & 1 ? by >> 4 : by & 15) - zero) * scale);
   }
   return v;
@@ -731,7 +732,8 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
             const uint32_t mask = t0 + t < toks ? s_masks[w - 12][t0 + t] : 0u;
             for (int g = 0; mask && g < ng; ++g)
               if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
-                acc[t] += left_out<T>(a, x + (m0 + t0 + t) * a.ldx, row, (c0 * GPC + g) * G, G);
+                acc[t] += left_out<T>(x + (m0 + t0 + t) * a.ldx, a.q, static_cast<const T*>(a.s), a.z, a.n, a.k, row,
+                                      (c0 * GPC + g) * G, G);
           }
         }
         if (a.ck > 1) {

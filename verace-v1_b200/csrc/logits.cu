@@ -6,28 +6,27 @@
 //     l <- l + bias[v]                  where the row's list names v
 //     l <- -inf                         where the mask's bit is 0
 //
-// Bound: the bytes of the logits in and out.  A cluster of CTAs takes a row, each CTA a range of
-// the vocabulary with a 32-bit counter per token in shared memory.  The cluster reads the row's
-// history once, a share to each CTA, and counts a token in the counters of the CTA that owns it
-// (distributed shared memory; equal tokens of a warp are added as one, since text repeats a few
-// tokens most).  Then each CTA streams its range, eight values a thread: most have no count, no
-// bias and a full mask, and are copied.  Biased tokens are marked in their counters and looked up
-// in a short list.  Without history and biases there are no counters and no cluster.
+// Bound: the bytes of the logits in and out.  Each CTA takes a range of a row's vocabulary, with a
+// 32-bit counter per token in shared memory, and reads the whole history of the row (from L2 after
+// the first), counting what falls into its range.  (Sharing the history out over a cluster and
+// counting in distributed shared memory was slower: 23 k clocks for 8192 tokens a CTA, remote
+// atomics being the slower ones.)  Then it streams its range, eight values a thread: most have
+// no count, no bias and a full mask, and are copied.  A biased token's counter holds the place of
+// its bias in a short list.
 #include "common.cuh"
-
-#include <cooperative_groups.h>
 
 #include <atomic>
 
 namespace verace {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int NT = 512;
 constexpr int CHUNK = 4096;   // vocabulary entries per CTA of logits_chunks
-constexpr int LIST = 1024;    // biases of a CTA's range held in shared memory
-constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, COUNT = 0x3fffffffu;
+constexpr int LIST = 512;     // biases of a CTA's range held in shared memory
+// A counter: seen in the prompt, biased, the bias's place in the list, the generated count.
+constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, PLACE = 20, COUNT = 0xfffffu;
+constexpr int LENGTH_MAX = 1 << 20;
+constexpr int RANGE = 11264, RANGE_LONG = 24576;   // tokens of a CTA at most (four and two CTAs an SM)
 
 struct LogitsArgs {
   const void* logits;
@@ -56,19 +55,19 @@ __device__ __forceinline__ long long id_at(const void* p, int i64, long long i) 
 }
 
 struct Controls {
-  float r, p, f;
+  float r, inv, p, f;
 };
 __device__ __forceinline__ Controls controls(const LogitsArgs& a, int row) {
-  return {a.rep_rows ? a.rep_rows[row] : a.rep, a.pres_rows ? a.pres_rows[row] : a.pres,
-          a.freq_rows ? a.freq_rows[row] : a.freq};
+  const float r = a.rep_rows ? a.rep_rows[row] : a.rep;
+  return {r, 1.f / r, a.pres_rows ? a.pres_rows[row] : a.pres, a.freq_rows ? a.freq_rows[row] : a.freq};
 }
 __device__ __forceinline__ int history(const LogitsArgs& a, int row) {
   return !a.tokens ? 0 : a.lengths ? max(0, min(a.lengths[row], a.length)) : a.length;
 }
-// A logit of a token with counter c (not 0).
-__device__ __forceinline__ float penalised(float l, uint32_t c, const Controls& k) {
-  if (c & ~BIASED) l = l > 0.f ? l / k.r : l * k.r;
-  if (c & COUNT) l = __fsub_rn(__fsub_rn(l, __fmul_rn(k.f, (float)(c & COUNT))), k.p);
+// A logit of a token seen, `made` of its occurrences being generated.
+__device__ __forceinline__ float penalised(float l, uint32_t made, const Controls& k) {
+  l *= l > 0.f ? k.inv : k.r;
+  if (made) l = __fsub_rn(__fsub_rn(l, __fmul_rn(k.f, (float)made)), k.p);
   return l;
 }
 
@@ -79,83 +78,93 @@ struct Biases {
 };
 
 // The last of the row's biases for a token.
-__device__ __noinline__ float bias_of(const LogitsArgs& a, const Biases& s, int row, int v0, int token) {
-  float value = 0.f;
-  if (s.n <= LIST) {
-    int last = -1;
-    for (int i = 0; i < s.n; ++i)
-      if (s.id[i] == token && s.order[i] > last) last = s.order[i], value = s.value[i];
-  } else {
-    for (int i = a.n_bias - 1; i >= 0; --i)
-      if (id_at(a.bias_ids, a.bias_i64, (long long)row * a.n_bias + i) == v0 + token)
-        return a.bias_values[(long long)row * a.n_bias + i];
-  }
-  return value;
+__device__ __noinline__ float bias_of(const void* ids, int i64, const float* values, long long first, int n, int token) {
+  for (int i = n - 1; i >= 0; --i)
+    if (id_at(ids, i64, first + i) == token) return values[first + i];
+  return 0.f;
 }
 
-// Rows in clusters of `ctas` (COUNTED: with counters; else the CTAs of a row have nothing in
-// common), `range` tokens a CTA.
+// `ctas` CTAs a row, `range` tokens each; COUNTED: with counters.
 template <typename T, typename O, bool COUNTED>
-__global__ void __launch_bounds__(NT, 2) logits_ranges(LogitsArgs a, int ctas, int range) {
+__global__ void __launch_bounds__(NT, 4) logits_ranges(LogitsArgs a, int ctas, int range) {
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ Biases s;
-  const int tid = threadIdx.x, lane = tid % 32, rank = blockIdx.x % ctas, row = blockIdx.x / ctas;
+  const int tid = threadIdx.x, rank = blockIdx.x % ctas, row = blockIdx.x / ctas;
   const int v0 = rank * range, nv = max(0, min(range, a.v - v0));
   const Controls k = controls(a, row);
+  const T* in = static_cast<const T*>(a.logits) + row * a.ld + v0;
+  O* out = static_cast<O*>(a.out) + row * a.out_ld + v0;
+  const uint8_t* mask = a.allowed ? reinterpret_cast<const uint8_t*>(a.allowed + row * a.allowed_ld) + v0 / 8 : nullptr;
   if constexpr (COUNTED) {
-    cg::cluster_group cl = cg::this_cluster();
+    // the range comes into L2 while the history is counted
+    constexpr int LINE = 128 / sizeof(T);
+    for (int i = tid * LINE; i < nv; i += NT * LINE) asm volatile("prefetch.global.L2 [%0];" ::"l"(in + i));
+    if (mask && tid * 1024 < nv) asm volatile("prefetch.global.L2 [%0];" ::"l"(mask + tid * 128));
     for (int i = 4 * tid; i < range; i += 4 * NT) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
     if (tid == 0) s.n = 0;
     const int len = history(a, row), prompt = a.prompt_lengths ? a.prompt_lengths[row] : 0;
-    if (ctas > 1) cl.sync();
-    else __syncthreads();
+    __syncthreads();
     for (int i = tid; i < a.n_bias; i += NT) {
       const long long id = id_at(a.bias_ids, a.bias_i64, (long long)row * a.n_bias + i) - v0;
       if (id >= 0 && id < nv) {
         const int at = atomicAdd(&s.n, 1);
         if (at < LIST) s.id[at] = (int)id, s.order[at] = i, s.value[at] = a.bias_values[(long long)row * a.n_bias + i];
-        atomicOr(&cnt[id], BIASED);
+        else atomicOr(&cnt[id], BIASED);
       }
     }
-    const int share = (len + ctas - 1) / ctas, first = rank * share, last = min(len, first + share);
-    const long long base = row * a.tokens_ld;
-    for (int i0 = first; i0 < last; i0 += 4 * NT) {
-      long long t[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = i0 + e * NT + tid;
-        t[e] = i < last ? id_at(a.tokens, a.tokens_i64, base + i) : -1;
+    auto count = [&](long long token, int i) {
+      const long long t = token - v0;
+      if ((unsigned long long)t < (unsigned long long)nv) {
+        if (i >= prompt) atomicAdd(&cnt[t], 1u);
+        else atomicOr(&cnt[t], PROMPT);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (i0 + e * NT >= last) break;
-        const int i = i0 + e * NT + tid;
-        const bool ok = t[e] >= 0 && t[e] < a.v, made = i >= prompt;
-        const int token = ok ? (int)t[e] : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, ok ? 2 * token + (made ? 1 : 0) : -1);
-        if (ok && lane == __ffs(same) - 1) {
-          const int owner = token / range;
-          uint32_t* c = ctas > 1 ? cl.map_shared_rank(cnt, owner) : cnt;
-          if (made) atomicAdd(c + (token - owner * range), (uint32_t)__popc(same));
-          else atomicOr(c + (token - owner * range), PROMPT);
+    };
+    const long long base = row * a.tokens_ld;
+    int done = 0;
+    if (a.tokens_i64) {
+      const long long* tk = static_cast<const long long*>(a.tokens) + base;
+      if (reinterpret_cast<size_t>(tk) % 16 == 0) {
+        done = len / 2 * 2;
+#pragma unroll 4
+        for (int i = 2 * tid; i < done; i += 2 * NT) {
+          const longlong2 u = __ldg(reinterpret_cast<const longlong2*>(tk + i));
+          count(u.x, i);
+          count(u.y, i + 1);
+        }
+      }
+    } else {
+      const int* tk = static_cast<const int*>(a.tokens) + base;
+      if (reinterpret_cast<size_t>(tk) % 16 == 0) {
+        done = len / 4 * 4;
+#pragma unroll 2
+        for (int i = 4 * tid; i < done; i += 4 * NT) {
+          const int4 u = __ldg(reinterpret_cast<const int4*>(tk + i));
+          count(u.x, i);
+          count(u.y, i + 1);
+          count(u.z, i + 2);
+          count(u.w, i + 3);
         }
       }
     }
-    if (ctas > 1) cl.sync();
-    else __syncthreads();
+#pragma unroll 4
+    for (int i = done + tid; i < len; i += NT) count(id_at(a.tokens, a.tokens_i64, base + i), i);
+    __syncthreads();
+    if (a.n_bias) {
+      // of the list's entries for one token the last in the row's order holds
+      const int listed = min(s.n, LIST);
+      for (int i = tid; i < listed; i += NT) {
+        const int id = s.id[i], order = s.order[i];
+        bool last = true;
+        for (int j = 0; j < listed; ++j) last = last && !(s.id[j] == id && s.order[j] > order);
+        if (last) atomicOr(&cnt[id], BIASED | (uint32_t)i << PLACE);
+      }
+      __syncthreads();
+    }
   }
 
-  const T* in = static_cast<const T*>(a.logits) + row * a.ld + v0;
-  O* out = static_cast<O*>(a.out) + row * a.out_ld + v0;
-  const uint8_t* mask = a.allowed ? reinterpret_cast<const uint8_t*>(a.allowed + row * a.allowed_ld) + v0 / 8 : nullptr;
-  auto one = [&](float l, int j) {
-    if constexpr (COUNTED) {
-      const uint32_t c = cnt[j];
-      if (c) {
-        l = penalised(l, c, k);
-        if (c & BIASED) l += bias_of(a, s, row, v0, j);
-      }
-    }
+  auto one = [&](float l, uint32_t c, int j) {
+    if (c & (PROMPT | COUNT)) l = penalised(l, c & COUNT, k);
+    if (c & BIASED) l += s.n <= LIST ? s.value[c >> PLACE & (LIST - 1)] : bias_of(a.bias_ids, a.bias_i64, a.bias_values, (long long)row * a.n_bias, a.n_bias, v0 + j);
     return l;
   };
   int done = 0;
@@ -179,8 +188,10 @@ __global__ void __launch_bounds__(NT, 2) logits_ranges(LogitsArgs a, int ctas, i
       if constexpr (COUNTED) {
         const uint4 c = *reinterpret_cast<const uint4*>(cnt + j), d = *reinterpret_cast<const uint4*>(cnt + j + 4);
         if (c.x | c.y | c.z | c.w | d.x | d.y | d.z | d.w) {
+          const uint32_t e[8] = {c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) l[i] = one(l[i], j + i);
+          for (int i = 0; i < 8; ++i)
+            if (e[i]) l[i] = one(l[i], e[i], j + i);
         }
       }
       if (bits != 255u) {
@@ -198,14 +209,17 @@ __global__ void __launch_bounds__(NT, 2) logits_ranges(LogitsArgs a, int ctas, i
   }
 #pragma unroll 4
   for (int j = done + tid; j < nv; j += NT) {
-    float l = one(to_f32(in[j]), j);
+    float l = to_f32(in[j]);
+    if constexpr (COUNTED) {
+      if (cnt[j]) l = one(l, cnt[j], j);
+    }
     if (mask && !(__ldg(mask + j / 8) >> (j % 8) & 1u)) l = -INFINITY;
     out[j] = from_f32<O>(l);
   }
 }
 
-// One CTA per CHUNK of a row's vocabulary, each over the whole history: for vocabularies whose
-// counters no cluster holds.
+// The same with a counter and a bias slot of 32 bits each: for histories that the counters above
+// do not hold.
 template <typename T, typename O>
 __global__ void __launch_bounds__(NT) logits_chunks(LogitsArgs a) {
   __shared__ uint32_t cnt[CHUNK];
@@ -232,65 +246,51 @@ __global__ void __launch_bounds__(NT) logits_chunks(LogitsArgs a) {
   O* out = static_cast<O*>(a.out) + row * a.out_ld + v0;
   for (int i = threadIdx.x; i < nv; i += NT) {
     float l = to_f32(in[i]);
-    if (cnt[i]) l = penalised(l, cnt[i], k);
+    if (cnt[i]) l = penalised(l, cnt[i] & ~PROMPT, k);
     if (slot[i]) l += a.bias_values[(long long)row * a.n_bias + slot[i] - 1];
     if (a.allowed && !((a.allowed[row * a.allowed_ld + (v0 + i) / 32] >> (i % 32)) & 1u)) l = -INFINITY;
     out[i] = from_f32<O>(l);
   }
 }
 
-constexpr int RANGE_MAX = 49152;       // counters of a CTA at most (192 KB)
-constexpr int RANGE_HALF = 24576;      // and where two CTAs share an SM
-
 template <typename T, typename O, bool COUNTED>
 int launch_ranges(const LogitsArgs& a, int ctas, int range, cudaStream_t st) {
   auto kern = logits_ranges<T, O, COUNTED>;
-  if (!COUNTED) {
-    kern<<<(unsigned)((long long)a.b * ctas), NT, 0, st>>>(a, ctas, range);
-    return check_launch("logits_process");
+  const size_t smem = COUNTED ? (size_t)range * 4 : 0;
+  if (COUNTED) {
+    static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
+    int dev = 0;
+    VERACE_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+      VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * RANGE_LONG));
+      if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
   }
-  static std::atomic<uint64_t> ready{0};      // devices whose limits are raised
-  int dev = 0;
-  VERACE_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RANGE_MAX * 4));
-    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)a.b * ctas));
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = (size_t)range * 4;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = ctas > 1 ? 1 : 0;
-  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, a, ctas, range));
+  VERACE_REQUIRE((long long)a.b * ctas <= 0x7fffffffLL, VERACE_ERR_UNSUPPORTED, "logits_process: %d rows of %d", a.b,
+                 a.v);
+  kern<<<(unsigned)((long long)a.b * ctas), NT, smem, st>>>(a, ctas, range);
   return check_launch("logits_process");
 }
 
 template <typename T, typename O>
 int run(const LogitsArgs& a, cudaStream_t st) {
   auto range_of = [&](int c) { return ((a.v + c - 1) / c + 31) / 32 * 32; };
+  int c;
   if (!a.tokens && a.n_bias == 0) {
     // 4096 values a CTA, or more where the rows alone fill the device several times over
-    int c = (a.v + 4095) / 4096;
+    c = (a.v + 4095) / 4096;
     if ((long long)a.b * c > 4096) c = (a.v + 16383) / 16384;
     return launch_ranges<T, O, false>(a, c, range_of(c), st);
   }
-  // as few CTAs a row as hold its counters two to an SM, more (of 2048 tokens at least) while the
-  // rows alone leave the device empty
-  int c = 1;
-  while (c < 8 && range_of(c) > RANGE_HALF) c *= 2;
-  if (range_of(c) > RANGE_HALF) c = 16;
-  while (c < 8 && (long long)a.b * c * 2 <= 296 && range_of(2 * c) >= 2048) c *= 2;
-  if (range_of(c) > RANGE_MAX || (long long)a.b * c > 0x7fffffffLL) {
+  if (a.length >= LENGTH_MAX) {
     logits_chunks<T, O><<<dim3((a.v + CHUNK - 1) / CHUNK, a.b), NT, 0, st>>>(a);
     return check_launch("logits_process");
   }
+  // long histories, which every CTA of a row reads: fewer and larger ranges; otherwise more of
+  // them (of 2048 tokens at least) while the rows leave the device empty
+  const int most = a.length > 16384 ? RANGE_LONG : RANGE;
+  c = (a.v + most - 1) / most;
+  while ((long long)a.b * c * 2 <= 296 && range_of(2 * c) >= 2048) c *= 2;
   return launch_ranges<T, O, true>(a, c, range_of(c), st);
 }
 
