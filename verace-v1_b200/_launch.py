@@ -1,16 +1,8 @@
-"""The launch path of the decode step's small calls: the current stream's handle and the
-device guard without the Python objects of ``torch.cuda.stream`` / ``torch.cuda.device``
-(which cost more than these kernels' launches)."""
+"""The launch path of the decode step's small calls, where the host's share of a call is longer
+than the kernel: the current stream's handle without the Python objects of
+``torch.cuda.stream`` (``raw_stream(index)``), and the current device's index (``current()``)
+to skip the device guard where it changes nothing."""
 import torch
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current = torch._C._cuda_getDevice
-
-
-def launch(device: torch.device, entry, *args) -> int:
-    """entry(*args, stream) on `device`'s current stream; returns the entry's status."""
-    index = device.index
-    if index == _current():
-        return entry(*args, _raw_stream(index))
-    with torch.cuda.device(index):
-        return entry(*args, _raw_stream(index))
+raw_stream = torch._C._cuda_getCurrentRawStream
+current = torch._C._cuda_getDevice

@@ -16,11 +16,12 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 
-from ._lib import check, lib
+from ._lib import F32, check, lib
 from .kernels import _DTYPE
-from ._launch import launch
+from ._launch import current, raw_stream
 
 GROUP_SIZES = (32, 64, 128)
+_SIZE = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}
 
 
 def _require_no_grad(x: torch.Tensor, who: str):
@@ -29,19 +30,20 @@ def _require_no_grad(x: torch.Tensor, who: str):
 
 
 def _check_packed(qweight, scales, zeros, bias, k, group_size, dtype):
+    """Checks a packed weight against the inputs' width and dtype; returns its number of rows."""
     if group_size not in GROUP_SIZES:
         raise ValueError(f"group_size {group_size}: expected one of {GROUP_SIZES}")
-    n = qweight.shape[0]
-    groups = -(-k // group_size)
     assert k % 32 == 0, "the input width must be a multiple of 32"
-    assert qweight.dtype == torch.uint8 and qweight.dim() == 2 and qweight.shape[1] * 2 == k, \
+    assert qweight.dtype is torch.uint8 and qweight.dim() == 2 and qweight.shape[1] * 2 == k, \
         "qweight must be uint8 [n, k / 2]"
-    assert scales.dtype == dtype and scales.dim() == 2 and scales.shape[0] == groups and scales.shape[1] == n, \
+    n = qweight.shape[0]
+    shape = (-(-k // group_size), n)
+    assert scales.dtype is dtype and scales.shape == shape, \
         "scales must be [ceil(k / group_size), n] in the activations' dtype"
-    assert zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape), \
+    assert zeros is None or (zeros.dtype is torch.uint8 and zeros.shape == shape), \
         "zeros must be uint8 in the shape of scales"
-    assert bias is None or (bias.dtype == dtype and bias.dim() == 1 and bias.shape[0] == n), \
-        "bias must be [n] in the activations' dtype"
+    assert bias is None or (bias.dtype is dtype and bias.shape == (n,)), "bias must be [n] in the activations' dtype"
+    return n
 
 
 def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
@@ -51,44 +53,64 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     in x's dtype or, with ``out_dtype=torch.float32``, in fp32.  Sums are fp32, the output is
     rounded once.  Any number of rows; meant for the few of a decode step."""
     assert x.is_cuda, "This kernel requires CUDA tensors"
-    _require_no_grad(x, "int4_linear")
+    if x.requires_grad:
+        _require_no_grad(x, "int4_linear")
+    dev = x.device
+    index = dev.index
+    if index != current():
+        with torch.cuda.device(dev):
+            return int4_linear(x, qweight, scales, zeros, bias, group_size=group_size, out_dtype=out_dtype)
     dt = x.dtype
     code = _DTYPE.get(dt)
     if code is None:
         raise ValueError(f"int4_linear: {dt} activations (expected fp32, bf16 or fp16)")
-    odt = dt if out_dtype is None else out_dtype
-    if odt is not dt and odt is not torch.float32:
-        raise ValueError(f"int4_linear: out_dtype {odt} (expected {dt} or torch.float32)")
-    k = x.shape[-1]
-    _check_packed(qweight, scales, zeros, bias, k, group_size, dt)
-    dev = x.device
-    n = qweight.shape[0]
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    m = x2.shape[0]
-    if (m > 1 and x2.stride(0) * x2.element_size() % 16) or (k > 1 and x2.stride(1) != 1) or x2.data_ptr() % 16 \
-            or (m > 1 and x2.stride(0) < k):
+    if out_dtype is None or out_dtype is dt:
+        odt, ocode = dt, code
+    elif out_dtype is torch.float32:
+        odt, ocode = out_dtype, F32
+    else:
+        raise ValueError(f"int4_linear: out_dtype {out_dtype} (expected {dt} or torch.float32)")
+    shape = x.shape
+    k = shape[-1]
+    n = _check_packed(qweight, scales, zeros, bias, k, group_size, dt)
+    flat = len(shape) == 2
+    x2 = x if flat else x.reshape(-1, k)
+    m, ldx = x2.shape[0], k
+    xp = x2.data_ptr()
+    if m > 1:
+        ldx = x2.stride(0)
+    if xp % 16 or (k > 1 and x2.stride(1) != 1) or ldx < k or ldx * _SIZE[dt] % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
-    if not qweight.is_contiguous() or qweight.data_ptr() % 16:
+        xp, ldx = x2.data_ptr(), k
+    qp = qweight.data_ptr()
+    if qp % 16 or not qweight.is_contiguous():
         qweight = qweight.clone(memory_format=torch.contiguous_format)
+        qp = qweight.data_ptr()
     if not scales.is_contiguous():
         scales = scales.contiguous()
-    if zeros is not None and not zeros.is_contiguous():
-        zeros = zeros.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    assert qweight.device == dev and scales.device == dev and (zeros is None or zeros.device == dev) \
-        and (bias is None or bias.device == dev), "all tensors must be on one device"
-    y = torch.empty((m, n), dtype=odt, device=dev)
+    zp = bp = None
+    if zeros is not None:
+        if not zeros.is_contiguous():
+            zeros = zeros.contiguous()
+        zp = zeros.data_ptr()
+    if bias is not None:
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+        bp = bias.data_ptr()
+    assert qweight.device == dev and scales.device == dev and (zp is None or zeros.device == dev) \
+        and (bp is None or bias.device == dev), "all tensors must be on one device"
+    y = x.new_empty((m, n), dtype=odt)
     L = lib()
     nws = L.verace_int4_linear_workspace(m, n, k, group_size, code)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    rc = launch(dev, L.verace_int4_linear, x2.data_ptr(), x2.stride(0) if m > 1 else k, qweight.data_ptr(),
-                scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
-                None if bias is None else bias.data_ptr(), y.data_ptr(), m, n, k, group_size, code, _DTYPE[odt],
-                None if ws is None else ws.data_ptr(), nws)
+    wp = None
+    if nws:
+        ws = x.new_empty(nws, dtype=torch.uint8)
+        wp = ws.data_ptr()
+    rc = L.verace_int4_linear(xp, ldx, qp, scales.data_ptr(), zp, bp, y.data_ptr(), m, n, k, group_size, code, ocode,
+                              wp, nws, raw_stream(index))
     if rc:
         check(rc, "verace_int4_linear")
-    return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
+    return y if flat else y.view(shape[:-1] + (n,))
 
 
 def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool = True
