@@ -17,10 +17,11 @@ Public surface (mirrors the reference package verace_v1 for this path):
     VeraceV1Model                                    (embedding, ACDE over the layers, final
                                                      norm, LM head; incremental decode
                                                      through layer_states)
-    int4_linear, quantize_int4, dequantize_int4, Int4Linear
+    int4_linear, quantize_int4, dequantize_int4, Int4Linear, quantize_model_int4
                                                      (products with 4-bit weights)
     process_logits, sample_logits                    (penalties, biases, grammar masks; the
                                                      choice of a token)
+    generate                                         (the generation loop over VeraceV1Model)
 The kernels live in libverace_b200.so (C ABI: include/verace_b200.h), built by
 build.py; nothing here falls back to CPU or Python arithmetic.
 """
@@ -35,8 +36,9 @@ from .mcmoe import (ManifoldContinuousMoE, SiTUGLU, launch_mcmoe_projection, lau
 from .config import VeraceV1Config
 from .layer import AdaptiveCognitiveDepthEngine, VeraceV1Layer
 from .model import VeraceV1Model
-from .int4 import Int4Linear, dequantize_int4, int4_linear, quantize_int4
+from .int4 import Int4Linear, dequantize_int4, int4_linear, quantize_int4, quantize_model_int4
 from .sampling import process_logits, sample_logits
+from .generate import generate
 
 __all__ = [
     "SSSDAttention", "ContinuousHolographicMemory", "newton_schulz_unitary_retraction",
@@ -47,5 +49,5 @@ __all__ = [
     "ManifoldContinuousMoE", "SiTUGLU", "launch_mcmoe_projection", "launch_mcmoe_triton_projection",
     "launch_mcmoe_route", "situ_glu", "VeraceV1Config", "VeraceV1Layer", "AdaptiveCognitiveDepthEngine",
     "VeraceV1Model", "Int4Linear", "dequantize_int4", "int4_linear", "quantize_int4", "process_logits",
-    "sample_logits",
+    "sample_logits", "quantize_model_int4", "generate",
 ]

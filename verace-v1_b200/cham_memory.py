@@ -37,11 +37,14 @@ class ContinuousHolographicMemory(nn.Module):
         self.w_gamma = nn.Linear(hidden_dim, 1, bias=False)
         self.w_out = nn.Linear(holographic_dim, hidden_dim, bias=False)
         self.norm = nn.RMSNorm(hidden_dim)
+        self.int4_in = None      # the concatenated projection in 4 bits (quantize_model_int4), in w_*'s place
 
     def projection(self, x: torch.Tensor) -> torch.Tensor:
         """The concatenated projection y = x [W_q; W_k; W_v; W_gamma]ᵀ, [b, s, ld] (rows
         q | k | v | gate, zero-padded to a multiple of 8): the GEMM of :meth:`project`
         without its epilogue, as the deferred decode step consumes it."""
+        if self.int4_in is not None:
+            return self.int4_in(x)
         W = concat_weights(self, [self.w_q.weight, self.w_k.weight, self.w_v.weight, self.w_gamma.weight])
         return F.linear(x, W)
 
@@ -50,7 +53,7 @@ class ContinuousHolographicMemory(nn.Module):
         concatenated projection weights, then the fused normalisation/SiLU/gate pass."""
         b, s, _ = x.shape
         D = self.holographic_dim
-        if D % 8:   # widths the fused pass does not tile: the same math as torch ops on the GPU
+        if D % 8 and self.int4_in is None:   # widths the fused pass does not tile: the same math as torch ops on the GPU
             q = F.normalize(self.w_q(x), p=2, dim=-1)
             k = F.normalize(self.w_k(x), p=2, dim=-1)
             v = F.normalize(F.silu(self.w_v(x)), p=2, dim=-1)
@@ -58,8 +61,7 @@ class ContinuousHolographicMemory(nn.Module):
             if active_mask is not None:
                 gamma = gamma * active_mask.reshape(b, s).to(gamma.dtype)
             return q, k, v, gamma
-        W = concat_weights(self, [self.w_q.weight, self.w_k.weight, self.w_v.weight, self.w_gamma.weight])
-        y = F.linear(x, W).reshape(b * s, -1)
+        y = self.projection(x).reshape(b * s, -1)
         q, k, v, gamma = mixer_prologue(y, 1, D, 1, True, active_mask)
         return q.view(b, s, D), k.view(b, s, D), v.view(b, s, D), gamma.view(b, s)
 

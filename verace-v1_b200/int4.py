@@ -194,3 +194,51 @@ class Int4Linear(nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, group_size={self.group_size}, "
                 f"zeros={self.zeros is not None}, bias={self.bias is not None}")
+
+
+def quantize_model_int4(model: nn.Module, group_size: int = 128, symmetric: bool = True,
+                        lm_head: bool = True) -> nn.Module:
+    """Puts the projections of a model's layers (a ``VeraceV1Model``, ``VeraceV1Layer`` or any module
+    that holds the framework's mixers and M-CMoE) into 4 bits, in place: the concatenated input
+    projections of both mixers and the stacked gate / up projection as one weight each, the
+    output projections, the M-CMoE down and sigma projections and, with ``lm_head``, the LM head
+    (the token embedding keeps its own table).  The dense weights are dropped.  Routers, gates of
+    the depth engine, norms and the M-CMoE bases stay as they are; so does a weight whose input
+    width is not a multiple of 32, or a head width that the fused prologue does not tile."""
+    from .cham_memory import ContinuousHolographicMemory
+    from .mcmoe import ManifoldContinuousMoE, SiTUGLU
+    from .sssd_attention import SSSDAttention
+
+    def pack(weights, pad=1):
+        w = torch.cat([x.weight.detach() for x in weights], 0)
+        if pad > 1 and w.shape[0] % pad:
+            w = torch.cat([w, w.new_zeros(-w.shape[0] % pad, w.shape[1])], 0)
+        return Int4Linear.from_weight(w, None, group_size, symmetric)
+
+    def replace(owner, name):
+        lin = getattr(owner, name)
+        if isinstance(lin, nn.Linear) and lin.in_features % 32 == 0:
+            setattr(owner, name, Int4Linear.from_linear(lin, group_size, symmetric))
+
+    for m in list(model.modules()):
+        if isinstance(m, SSSDAttention) and m.int4_in is None and m.hidden_dim % 32 == 0 and m.head_dim % 8 == 0:
+            m.int4_in = pack([m.w_q, m.w_k, m.w_v, m.w_delta], 8)
+            m.w_q = m.w_k = m.w_v = m.w_delta = None
+            m._verace_cat = None
+            replace(m, "w_out")
+        elif isinstance(m, ContinuousHolographicMemory) and m.int4_in is None and m.hidden_dim % 32 == 0 \
+                and m.holographic_dim % 8 == 0:
+            m.int4_in = pack([m.w_q, m.w_k, m.w_v, m.w_gamma], 8)
+            m.w_q = m.w_k = m.w_v = m.w_gamma = None
+            m._verace_cat = None
+            replace(m, "w_out")
+        elif isinstance(m, SiTUGLU) and m.int4_in is None and m.in_features % 32 == 0:
+            m.int4_in = pack([m.w_gate, m.w_up])
+            m.w_gate = m.w_up = None
+            m._stacked = m._stacked_key = None
+        elif isinstance(m, ManifoldContinuousMoE):
+            replace(m, "base_w_down")
+            replace(m, "hyper_sigma")
+    if lm_head and isinstance(getattr(model, "lm_head", None), nn.Linear):
+        replace(model, "lm_head")
+    return model

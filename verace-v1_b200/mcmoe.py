@@ -109,6 +109,7 @@ class SiTUGLU(nn.Module):
         self.beta2 = beta2
         self.w_gate = nn.Linear(in_features, hidden_features, bias=False)
         self.w_up = nn.Linear(in_features, hidden_features, bias=False)
+        self.int4_in = None      # [W_gate; W_up] in 4 bits (quantize_model_int4), in their place
         self._stacked: Optional[torch.Tensor] = None
         self._stacked_key = None
 
@@ -124,7 +125,7 @@ class SiTUGLU(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda or torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("SiTUGLU runs on CUDA inputs for inference (no autograd path)")
-        gu = torch.nn.functional.linear(x, self._gate_up_weight())
+        gu = self.int4_in(x) if self.int4_in is not None else torch.nn.functional.linear(x, self._gate_up_weight())
         hf = self.hidden_features
         return situ_glu(gu[..., :hf], gu[..., hf:], self.beta1, self.beta2)
 

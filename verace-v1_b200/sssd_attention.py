@@ -41,13 +41,14 @@ class SSSDAttention(nn.Module):
         self.w_delta = nn.Linear(hidden_dim, num_heads, bias=False)
         self.head_rmsnorm = nn.RMSNorm(head_dim)
         self.w_out = nn.Linear(num_heads * head_dim, hidden_dim, bias=False)
+        self.int4_in = None      # the concatenated projection in 4 bits (quantize_model_int4), in w_*'s place
 
     def project(self, x: torch.Tensor, active_mask: Optional[torch.Tensor] = None):
         """q, k, v [b, s, h, d] and delta [b, s, h] (sssd_attention.py:116-126): one GEMM
         with the concatenated projection weights, then the fused normalisation/gate pass."""
         b, s, _ = x.shape
         h, d = self.num_heads, self.head_dim
-        if d % 8:   # head widths the fused pass does not tile: the same math as torch ops on the GPU
+        if d % 8 and self.int4_in is None:   # head widths the fused pass does not tile: the same math as torch ops on the GPU
             q = F.normalize(self.w_q(x).view(b, s, h, d), p=2, dim=-1)
             k = F.normalize(self.w_k(x).view(b, s, h, d), p=2, dim=-1)
             v = F.normalize(self.w_v(x).view(b, s, h, d), p=2, dim=-1)
@@ -55,8 +56,11 @@ class SSSDAttention(nn.Module):
             if active_mask is not None:
                 delta = delta * active_mask.reshape(b, s, 1).to(delta.dtype)
             return q, k, v, delta
-        W = concat_weights(self, [self.w_q.weight, self.w_k.weight, self.w_v.weight, self.w_delta.weight])
-        y = F.linear(x, W).reshape(b * s, -1)
+        if self.int4_in is not None:
+            y = self.int4_in(x).reshape(b * s, -1)
+        else:
+            W = concat_weights(self, [self.w_q.weight, self.w_k.weight, self.w_v.weight, self.w_delta.weight])
+            y = F.linear(x, W).reshape(b * s, -1)
         q, k, v, delta = mixer_prologue(y, h, d, h, False, active_mask)
         return q.view(b, s, h, d), k.view(b, s, h, d), v.view(b, s, h, d), delta.view(b, s, h)
 
