@@ -24,12 +24,15 @@
 // there, so those inputs (and infinities and NaN) are left out of the pieces and added one by
 // one as (q - z) x s at the end (rare).
 //
-// One CTA per SM, 128 output rows at a time, 20 warps: one feeds the weights by TMA (128 rows x
-// 256 codes a stage, 128-byte swizzle: a row's thread reads 16 bytes without bank conflicts),
-// one the staged x, two issue the MMAs, eight unpack codes into TMEM (the MMA's A operand; two
-// sets of four take a chunk's halves), eight hold the rows' sums (two sets: half of the tokens
-// each).  Every role is a chain of short dependent steps, hence the two of each.  Few row tiles: k is split over
-// a cluster and the partial sums are joined through distributed shared memory in rank order.
+// One CTA per SM, 128 output rows at a time, 20 warps.  One warp feeds the weights by TMA (128
+// rows x 256 codes a stage, 128-byte swizzle: a row's thread reads 16 bytes without bank
+// conflicts), one the staged x.  The rest are two lines that take every other chunk of 256 inputs,
+// each with four warps that unpack codes into TMEM (the MMA's A operand), one that issues the
+// MMAs, four that hold the rows' sums, and its own places in TMEM.  Every role is a chain of
+// dependent steps of 30 to 100 clocks (a barrier, a shared-memory or TMEM round trip; an MMA takes
+// a warp 33 clocks to issue), 600 to 1000 a chunk; a chunk's weights take 712 clocks of an SM's
+// share of the memory rate, and two lines have twice that.  Few row tiles: k is split over a
+// cluster and the partial sums are joined through distributed shared memory in rank order.
 #include "common.cuh"
 #include "tc.cuh"
 #include "tmap.cuh"
@@ -52,11 +55,9 @@ constexpr uint32_t POLLS = 1u << 16;     // of 64 polls each
 constexpr int NT = 640;                  // threads: 20 warps
 constexpr int ROWS = 128;                // output rows per tile
 constexpr int KC = 256;                  // inputs per chunk
-constexpr int SW = 5;                    // weight stages of one chunk
 constexpr int W_STAGE = ROWS * KC / 2;   // bytes: 128 rows x 256 codes
-constexpr int D_COL = 256;               // first TMEM column of the accumulators
 constexpr int MAX_SB = 32;
-constexpr int B_SMEM = 136 * 1024;
+constexpr int SMEM = 220 * 1024;
 constexpr float FINITE = 3.4028235e38f;
 constexpr float APART = 1.f / 4096.f;
 
@@ -70,11 +71,22 @@ struct Shape {
   static constexpr int P = IS32 ? 5 : std::is_same<T, __half>::value ? 3 : 2;    // pieces
   static constexpr int N = COLS ? (P * MP + 15) / 16 * 16 : MP;                  // MMA columns
   static constexpr int PASSES = COLS ? 1 : P;
-  static constexpr int ND = 128 / N < 2 ? 1 : 2;                                 // pairs of accumulators (one per MMA warp)
-  static constexpr int A_COLS = KC / 4 + 8 * GPC;                                // TMEM columns of a chunk's A
-  static constexpr int NA = 256 / A_COLS;
+  // sums: a line's warps hold all tokens of their chunks, and one line's sums are added to the
+  // other's at the end; for 64 tokens, more than the registers hold, both lines' warps take half
+  // of the tokens of every chunk
+  static constexpr bool HALVES = MP > 32;
+  static constexpr int TB = MP < 16 ? MP : 16;                                   // tokens summed at a time
+  static constexpr int PART = HALVES ? 0 : 2 * MP * ROWS * 4;                    // bytes of sums handed over
+  // TMEM: two accumulators (a pair of groups) per line, the rest for chunks of A, as many per line
+  static constexpr int D_COL = 512 - 4 * N;
+  static constexpr int A_COLS = KC / 4 + 8 * GPC;
+  static constexpr int NA = D_COL / A_COLS >= 4 ? 4 : 2;
+  static_assert(NA * A_COLS <= D_COL, "TMEM");
   // bytes of a chunk's B operands: the passes' [256 / 16][N][16], then per group the zeros' [2][N][16]
   static constexpr int BLK = PASSES * KC * N + GPC * 32 * N;
+  static constexpr int SW = BLK > 44 * 1024 ? 4 : 6;                             // weight stages (even)
+  static constexpr int B_SMEM = SMEM - SW * W_STAGE - PART;                      // bytes for x
+  static_assert(B_SMEM >= 2 * BLK, "x is at least double-buffered");
 };
 
 struct Int4Args {
@@ -364,7 +376,7 @@ __device__ __forceinline__ void pin(float* v) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 struct Bars {
-  uint64_t wfull[SW], wempty[SW], afull[3], aempty[3], dfull[2], dempty[2], bfull[MAX_SB], bempty[MAX_SB], drain;
+  uint64_t wfull[6], wempty[6], afull[4], aempty[4], dfull[2], dempty[2], bfull[MAX_SB], bempty[MAX_SB], xready, drain;
 };
 
 // A place in a ring of barriers, and the parity of the completion awaited there: `phase` for one
@@ -374,6 +386,11 @@ struct Turn {
   uint32_t phase = 0;
   __device__ __forceinline__ void next(int n) {
     if (++slot == n) slot = 0, phase ^= 1;
+  }
+  // every other place of an even ring
+  __device__ __forceinline__ void next2(int n) {
+    slot += 2;
+    if (slot >= n) slot -= n, phase ^= 1;
   }
 };
 
@@ -414,17 +431,18 @@ struct Waiter {
 template <typename T, typename S>
 __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constant__ CUtensorMap wmap, Int4Args a) {
   constexpr int BLK = S::BLK, N = S::N, MP = S::MP, GPC = S::GPC, G = KC / GPC, KB = 8 / GPC;   // KB: k blocks a group
+  constexpr int SW = S::SW, PAIRS = GPC / 2;     // pairs of groups per chunk
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bar;
   __shared__ uint32_t s_slot;
   __shared__ int s_fail;
   __shared__ int s_top[MP];
   __shared__ uint32_t s_mask[MP];
-  __shared__ float s_scale[MP];
-  __shared__ float s_scales[8][MP];            // of the token tile at hand, a copy for each summing warp
-  __shared__ uint32_t s_masks[8][MP];
+  __shared__ float s_factor[8][MP];            // of the token tile at hand, a copy for each summing warp
+  __shared__ uint32_t s_marks[8][MP];
   uint8_t* wst = smem;
   uint8_t* bst = smem + SW * W_STAGE;
+  float* part = reinterpret_cast<float*>(bst + (size_t)a.sb * BLK);   // [2][MP][ROWS]: one line's sums for the other
   const int tid = threadIdx.x, lane = tid % 32, w = __shfl_sync(0xffffffffu, tid / 32, 0);
   const int rank = a.ck > 1 ? blockIdx.x % a.ck : 0;
   const int chunks = (a.k + KC - 1) / KC;
@@ -434,10 +452,11 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
 
   if (w == 1) tc::tmem_alloc(&s_slot, 512);
   if (tid == 0) {
-    for (int i = 0; i < SW; ++i) tc::mbar_init(&bar.wfull[i], 1), tc::mbar_init(&bar.wempty[i], 8);
-    for (int i = 0; i < S::NA; ++i) tc::mbar_init(&bar.afull[i], 8), tc::mbar_init(&bar.aempty[i], 2);
-    for (int i = 0; i < S::ND; ++i) tc::mbar_init(&bar.dfull[i], 2), tc::mbar_init(&bar.dempty[i], 8);
-    for (int i = 0; i < a.sb; ++i) tc::mbar_init(&bar.bfull[i], 1), tc::mbar_init(&bar.bempty[i], 2);
+    for (int i = 0; i < SW; ++i) tc::mbar_init(&bar.wfull[i], 1), tc::mbar_init(&bar.wempty[i], 4);
+    for (int i = 0; i < S::NA; ++i) tc::mbar_init(&bar.afull[i], 4), tc::mbar_init(&bar.aempty[i], 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&bar.dfull[i], 1), tc::mbar_init(&bar.dempty[i], S::HALVES ? 8 : 4);
+    for (int i = 0; i < a.sb; ++i) tc::mbar_init(&bar.bfull[i], 1), tc::mbar_init(&bar.bempty[i], 1);
+    tc::mbar_init(&bar.xready, 8);
     tc::mbar_init(&bar.drain, 2);
     tc::fence_mbar_init();
     s_fail = 0;
@@ -447,7 +466,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
       tc::tma_load_2d(wst + i * W_STAGE, &wmap, (c0 + i) * (KC / 2), unit0 % a.tiles * ROWS, &bar.wfull[i]);
     }
   }
-  if (tid < MP) s_top[tid] = 0, s_mask[tid] = 0, s_scale[tid] = 0.f;
+  if (tid < MP) s_top[tid] = 0, s_mask[tid] = 0;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -457,35 +476,6 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
   if (tid == 0 && s_slot != 0) {
     s_fail = 1;
     atomicExch(&g_int4_status, 1);
-  }
-
-  if (!a.staged && nc > 0) {
-    // every warp stages the CTA's range of x: the tokens' largest inputs, then the pieces
-    constexpr int LANES = 32 / GPC;
-    const T* x = static_cast<const T*>(a.x) + c0 * KC + lane * 8;
-    const int toks = (int)a.m, total = toks * nc;
-    for (int u = w; u < total; u += NT / 32) {
-      const int tok = u / nc, c = u - tok * nc;
-      float v[8];
-      load8(x + (long long)tok * a.ldx + c * KC, (c0 + c) * KC + lane * 8 < a.k, v);
-      bool out;
-      const float most = leave_out<LANES>(v, out);
-      if (out) atomicOr(&s_mask[tok], 1u << ((c * GPC + lane / LANES) / span));
-      const int m = __reduce_max_sync(0xffffffffu, __float_as_int(most));
-      if (lane == 0) atomicMax(&s_top[tok], m);
-    }
-    __syncthreads();
-    for (int u = w; u < total; u += NT / 32) {
-      const int tok = u / nc, c = u - tok * nc;
-      float v[8];
-      load8(x + (long long)tok * a.ldx + c * KC, (c0 + c) * KC + lane * 8 < a.k, v);
-      bool out;
-      leave_out<LANES>(v, out);
-      stage8<T, S>(v, pow2(shift_of(__int_as_float(s_top[tok]))), bst + c * BLK, tok, lane);
-    }
-    if (tid < toks) s_scale[tid] = pow2(-shift_of(__int_as_float(s_top[tid])));
-    tc::fence_proxy_async();
-    __syncthreads();
   }
 
   if (w == 0) {
@@ -519,241 +509,335 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
           tc::bulk_load(bst + tb.slot * BLK, src, BLK, &bar.bfull[tb.slot]);
         }
       }
-      for (int j = it - a.sb < 0 ? 0 : it - a.sb; j < it; ++j)
-        wait(&bar.bfull[j % a.sb], j / a.sb & 1);
+      for (int j = it - a.sb < 0 ? 0 : it - a.sb; j < it; ++j) wait(&bar.bfull[j % a.sb], j / a.sb & 1);
     }
   } else if (w < 4) {
-    // ---- MMAs: two warps, every other group each (an MMA takes a warp 33 clocks to issue, a wait
-    // 100).  The whole warp walks the loop, so that the operands sit in uniform registers.
+    // ---- MMAs.  The whole warp walks the loop, so that the operands sit in uniform registers (33
+    // clocks an MMA; a single lane's loop took 114).
     const bool lead = elect();
-    const int mine = w - 2;
-    Turn ta, tb, td;
+    const int line = w - 2;
+    Turn ta, tb;
+    ta.slot = tb.slot = line;
+    uint32_t dphase = 0;
+    int first = line;
+    if (!a.staged && nc > 0) wait(&bar.xready, 0);
     for (int u = unit0; u < units; u += step) {
-      if (a.resident) tb.slot = 0;
-      const bool new_x = a.staged && !(a.resident && u > unit0);
-      for (int c = 0; c < nc; ++c) {
+      int c = first;
+      for (; c < nc; c += 2) {
+        const int slot = a.resident ? c : tb.slot;
         wait(&bar.afull[ta.slot], ta.phase);
-        if (new_x) wait(&bar.bfull[tb.slot], tb.phase);
+        if (a.staged) wait(&bar.bfull[slot], a.resident ? 0 : tb.phase);
         const uint32_t A = ta.slot * S::A_COLS;
-        const uint64_t B = tc::sdesc(tc::smem_addr(bst + tb.slot * BLK), N * 16, 128);
+        const uint64_t B = tc::sdesc(tc::smem_addr(bst + slot * BLK), N * 16, 128);
 #pragma unroll
-        for (int gj = 0; gj < GPC / 2; ++gj) {
-          wait(&bar.dempty[td.slot], td.phase ^ 1);
+        for (int gj = 0; gj < PAIRS; ++gj, dphase ^= 1) {
+          wait(&bar.dempty[line], dphase ^ 1);
           tc::fence_after_sync();
-          const int gi = 2 * gj + mine;
-          const uint32_t D = D_COL + (2 * td.slot + mine) * N, Ag = A + gi * (8 * KB);
-          const uint64_t Bg = B + (uint64_t)(gi * (KB * 32 * N >> 4));
           if (lead) {
-            constexpr uint32_t first = idesc_f8(N, 0), rest = idesc_f8(N, 1);
+            constexpr uint32_t main0 = idesc_f8(N, 0), rest = idesc_f8(N, 1);
 #pragma unroll
-            for (int p = 0; p < S::PASSES; ++p)
+            for (int gi = 2 * gj; gi < 2 * gj + 2; ++gi) {
+              const uint32_t D = S::D_COL + (2 * line + gi % 2) * N, Ag = A + gi * (8 * KB);
+              const uint64_t Bg = B + (uint64_t)(gi * (KB * 32 * N >> 4));
 #pragma unroll
-              for (int b = 0; b < KB; ++b)
-                mma_f8(D, Ag + 8 * b, Bg + (uint64_t)((p * KC * N + b * 32 * N) >> 4), p > 0 ? rest : first, p + b > 0);
-            mma_f8(D, A + KC / 4 + 8 * gi, B + (uint64_t)((S::PASSES * KC * N >> 4) + gi * (32 * N >> 4)), rest, true);
-            tc::commit(&bar.dfull[td.slot]);
+              for (int p = 0; p < S::PASSES; ++p)
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+                  mma_f8(D, Ag + 8 * b, Bg + (uint64_t)((p * KC * N + b * 32 * N) >> 4), p > 0 ? rest : main0,
+                         p + b > 0);
+              mma_f8(D, A + KC / 4 + 8 * gi, B + (uint64_t)((S::PASSES * KC * N >> 4) + gi * (32 * N >> 4)), rest, true);
+            }
+            tc::commit(&bar.dfull[line]);
           }
-          td.next(S::ND);
         }
         if (lead) {
           tc::commit(&bar.aempty[ta.slot]);
-          if (a.staged && !a.resident) tc::commit(&bar.bempty[tb.slot]);
+          if (a.staged && !a.resident) tc::commit(&bar.bempty[slot]);
         }
-        ta.next(S::NA);
-        if (a.resident) ++tb.slot;
-        else tb.next(a.sb);
+        ta.next2(S::NA);
+        if (!a.resident) tb.next2(a.sb);
       }
+      first = c - nc;
     }
     if (lead) {
       tc::commit(&bar.drain);        // every MMA issued is done before the TMEM goes
       wait(&bar.drain, 0);
     }
   } else if (w < 12) {
-    // ---- unpacking: two sets of four warps, a half of every chunk each; a thread is a row
-    const int half = (w - 4) / 4, r = w % 4 * 32 + lane;
-    const uint32_t at = ((uint32_t)(w % 4 * 32) << 16) + half * 32;
-    constexpr int GH = GPC / 2;        // groups per half
+    // ---- unpacking: a thread is a row
+    const int line = (w - 4) / 4, r = w % 4 * 32 + lane;
+    const uint32_t lanes = (uint32_t)(w % 4 * 32) << 16;
     Turn tw, ta;
-    bool fresh = true;
-    int seen = 0;
-    const int groups = (a.k + G - 1) / G;
+    tw.slot = ta.slot = line;
+    const int groups = (a.k + G - 1) / G - c0 * GPC;         // from this CTA's first
+    // the zeros of the line's next chunk, a chunk ahead (across units)
+    int zu = unit0, ztile = unit0 % a.tiles, zc = line;
+    const uint8_t* zp = nullptr;
+    bool zlive = false;
+    uint8_t zn[GPC];
+    auto zeros_at = [&] {
+      const long long row = (long long)ztile * ROWS + r;
+      zlive = zu < units && row < a.n;
+      zp = a.z + (long long)(c0 + zc) * GPC * a.n + row;
+    };
+    auto load_zeros = [&] {
+      if (zc >= nc) {
+        while (zc >= nc && zu < units) {
+          zc -= nc, zu += step, ztile += step;
+          while (ztile >= a.tiles) ztile -= a.tiles;
+        }
+        zeros_at();
+      }
+#pragma unroll
+      for (int gi = 0; gi < GPC; ++gi)
+        zn[gi] = zlive && zc * GPC + gi < groups ? __ldg(zp + (long long)gi * a.n) : 8;
+      zc += 2;
+      zp += 2LL * GPC * a.n;
+    };
+    if (a.z && nc > 0) {
+      zeros_at();
+      load_zeros();
+    }
+    int first = line, fresh = S::NA / 2;
     for (int u = unit0; u < units; u += step) {
-      const long long row = (long long)(u % a.tiles) * ROWS + r;
-      int g = c0 * GPC + half * GH;
-      const uint8_t* zp = a.z && row < a.n ? a.z + (long long)g * a.n + row : nullptr;
-      uint8_t zn[GH];
-      auto load_zeros = [&](int c) {
-#pragma unroll
-        for (int gi = 0; gi < GH; ++gi) zn[gi] = zp && c < nc && g + gi < groups ? __ldg(zp + (long long)gi * a.n) : 8;
-        g += GPC;
-        if (zp) zp += (long long)GPC * a.n;
-      };
-      if (a.z) load_zeros(0);
-      for (int c = 0; c < nc; ++c) {
+      int c = first;
+      for (; c < nc; c += 2) {
         wait(&bar.wfull[tw.slot], tw.phase);
-        uint4 raw[4];
         const uint8_t* src = wst + tw.slot * W_STAGE + r * (KC / 2);
+        uint4 raw[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + (((half * 4 + j) ^ (r & 7)) * 16));
+        for (int j = 0; j < 8; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + ((j ^ (r & 7)) * 16));
         wait(&bar.aempty[ta.slot], ta.phase ^ 1);
         __syncwarp();
         tc::fence_after_sync();
-        const uint32_t A = at + ta.slot * S::A_COLS;
-        uint32_t code[32];
+        const uint32_t A = lanes + ta.slot * S::A_COLS;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t word[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        for (int h = 0; h < 2; ++h) {
+          uint32_t code[32];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            code[8 * j + 2 * i] = word[i] & 0x0f0f0f0fu;
-            code[8 * j + 2 * i + 1] = (word[i] >> 4) & 0x0f0f0f0fu;
+          for (int j = 0; j < 4; ++j) {
+            const uint4 q = raw[4 * h + j];
+            const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              code[8 * j + 2 * i] = word[i] & 0x0f0f0f0fu;
+              code[8 * j + 2 * i + 1] = (word[i] >> 4) & 0x0f0f0f0fu;
+            }
           }
+          tmem_st32(A + 32 * h, code);
         }
-        tmem_st32(A, code);
-        if (a.z || fresh) {            // without zeros, -8 stays where the first round wrote it
+        if (lane == 0) tc::mbar_arrive(&bar.wempty[tw.slot]);       // (the warp's loads are in registers)
+        if (a.z || fresh > 0) {        // without zeros, -8 stays where the first rounds wrote it
 #pragma unroll
-          for (int gi = 0; gi < GH; ++gi) {
-            uint32_t zc[8];
+          for (int gi = 0; gi < GPC; ++gi) {
+            uint32_t zw[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) zc[j] = a.z ? (0x80u | zn[gi]) * 0x01010101u : 0x88888888u;
-            tmem_st8(A - half * 32 + KC / 4 + 8 * (half * GH + gi), zc);
+            for (int j = 0; j < 8; ++j) zw[j] = a.z ? (0x80u | zn[gi]) * 0x01010101u : 0x88888888u;
+            tmem_st8(A + KC / 4 + 8 * gi, zw);
           }
-          if (a.z) load_zeros(c + 1);
-          if (++seen == S::NA) fresh = false;
+          if (a.z) load_zeros();
+          --fresh;
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) {
-          tc::mbar_arrive(&bar.wempty[tw.slot]);
-          tc::mbar_arrive(&bar.afull[ta.slot]);
-        }
-        tw.next(SW);
-        ta.next(S::NA);
+        if (lane == 0) tc::mbar_arrive(&bar.afull[ta.slot]);
+        tw.next2(SW);
+        ta.next2(S::NA);
       }
+      first = c - nc;
     }
   } else {
-    // ---- sums: two sets of four warps, half of the tokens each; a thread is an output row
-    constexpr int TH = MP / 2;
-    const int set = (w - 12) / 4, t0 = set * TH, r = w % 4 * 32 + lane;
-    const uint32_t at = D_COL + ((uint32_t)(w % 4 * 32) << 16) + t0;
-    const int groups = (a.k + G - 1) / G, ng = nc * GPC;
+    // ---- sums: a thread is an output row
+    const int line = (w - 12) / 4, r = w % 4 * 32 + lane;
+    if (!a.staged && nc > 0) {
+      // first these warps stage the CTA's range of x: the tokens' largest inputs, then the pieces
+      constexpr int LANES = 32 / GPC;
+      const T* x = static_cast<const T*>(a.x) + c0 * KC + lane * 8;
+      const int toks = (int)a.m, total = toks * nc;
+      for (int u = w - 12; u < total; u += 8) {
+        const int tok = u / nc, c = u - tok * nc;
+        float v[8];
+        load8(x + (long long)tok * a.ldx + c * KC, (c0 + c) * KC + lane * 8 < a.k, v);
+        bool out;
+        const float most = leave_out<LANES>(v, out);
+        if (out) atomicOr(&s_mask[tok], 1u << ((c * GPC + lane / LANES) / span));
+        const int m = __reduce_max_sync(0xffffffffu, __float_as_int(most));
+        if (lane == 0) atomicMax(&s_top[tok], m);
+      }
+      tc::named_sync(1, 256);
+      for (int u = w - 12; u < total; u += 8) {
+        const int tok = u / nc, c = u - tok * nc;
+        float v[8];
+        load8(x + (long long)tok * a.ldx + c * KC, (c0 + c) * KC + lane * 8 < a.k, v);
+        bool out;
+        leave_out<LANES>(v, out);
+        stage8<T, S>(v, pow2(shift_of(__int_as_float(s_top[tok]))), bst + c * BLK, tok, lane);
+      }
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.xready);
+    }
     if (a.staged) asm volatile("griddepcontrol.wait;" ::: "memory");
-    Turn td;                            // a pair of groups: one accumulator of each MMA warp
-    for (int u = unit0; u < units; u += step) {
+    constexpr int TH = S::HALVES ? MP / 2 : MP, TB = S::TB;
+    constexpr int STRIDE = S::HALVES ? 1 : 2;      // chunks of the warp
+    const int t0 = S::HALVES ? line * TH : 0;
+    const uint32_t at = S::D_COL + ((uint32_t)(w % 4 * 32) << 16) + t0;
+    const int groups = (a.k + G - 1) / G - c0 * GPC;         // from this CTA's first
+    // the scales of the warp's next two pairs (across units), as loaded: 16-bit ones in words of
+    // their own, since a conversion or a packed pair would wait for the load
+    using Raw = typename std::conditional<S::IS32, uint32_t, unsigned short>::type;
+    int su = unit0, stile = unit0 % a.tiles, sc = S::HALVES ? 0 : line, sg = 0;     // sg: group in the chunk
+    const Raw* sp = nullptr;
+    bool slive = false;
+    auto scales_at = [&] {
+      const long long row = (long long)stile * ROWS + r;
+      slive = su < units && row < a.n;
+      sp = reinterpret_cast<const Raw*>(a.s) + (long long)(c0 + sc) * GPC * a.n + row;
+    };
+    auto load_scales = [&](uint32_t (&to)[2]) {
+      if (sg == GPC) {
+        sg = 0, sc += STRIDE, sp += (long long)(STRIDE - 1) * GPC * a.n;
+        if (sc >= nc) {
+          while (sc >= nc && su < units) {
+            sc -= nc, su += step, stile += step;
+            while (stile >= a.tiles) stile -= a.tiles;
+          }
+          scales_at();
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j, sp += a.n) {
+        to[j] = 0;
+        if (slive && sc * GPC + sg + j < groups) to[j] = __ldg(sp);
+      }
+      sg += 2;
+    };
+    uint32_t s0[2] = {0, 0}, s1[2] = {0, 0};
+    if (nc > 0) {
+      if (sc >= nc) sg = GPC, sc -= STRIDE;        // (the first unit has no chunk of this line)
+      else scales_at();
+      load_scales(s0);
+      load_scales(s1);
+    }
+    int first = S::HALVES ? 0 : line, buf = 0, turn = 0;     // turn: the line of the next chunk (HALVES)
+    uint32_t dphase[2] = {0, 0};
+    long long tile_m = -1;
+    uint32_t any = 0;                   // whether inputs of its tokens were left out
+    for (int u = unit0; u < units; u += step, buf ^= 1) {
       const long long row = (long long)(u % a.tiles) * ROWS + r, m0 = (long long)(u / a.tiles) * MP;
       const int toks = (int)min((long long)MP, a.m - m0);
-      __syncwarp();
-      for (int t = lane; t < toks; t += 32) {
-        s_scales[w - 12][t] = a.staged ? a.ws_scale[m0 + t] : s_scale[t];
-        s_masks[w - 12][t] = a.staged ? a.ws_mask[m0 + t] : s_mask[t];
+      float bv = 0.f;
+      if (a.bias && row < a.n) bv = to_f32(static_cast<const T*>(a.bias)[row]);
+      if (m0 != tile_m) {
+        tile_m = m0;
+        __syncwarp();
+        for (int t = lane; t < toks; t += 32) {
+          s_factor[w - 12][t] = 512.f * (a.staged ? a.ws_scale[m0 + t]
+                                                  : nc > 0 ? pow2(-shift_of(__int_as_float(s_top[t]))) : 0.f);
+          s_marks[w - 12][t] = a.staged ? a.ws_mask[m0 + t] : s_mask[t];
+        }
+        __syncwarp();
+        any = 0;
+        for (int t = t0; t < min(t0 + TH, toks); ++t) any |= s_marks[w - 12][t];
       }
-      __syncwarp();
       float acc[TH];
 #pragma unroll
       for (int t = 0; t < TH; ++t) acc[t] = 0.f;
-      const T* sp = static_cast<const T*>(a.s) + (long long)c0 * GPC * a.n + row;
-      const int have = row < a.n ? min(ng, groups - c0 * GPC) : 0;
-      // the scales of the next four groups, as loaded: 16-bit ones in words of their own, since a
-      // conversion or a packed pair would wait for the load
-      using Raw = typename std::conditional<S::IS32, uint32_t, unsigned short>::type;
-      const Raw* sr = reinterpret_cast<const Raw*>(sp);
-      uint32_t sq[4];
+      int c = first;
+      for (; c < nc; c += STRIDE) {
+        const int from = S::HALVES ? turn : line;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq[i] = i < have ? (uint32_t)__ldg(sr + (long long)i * a.n) : 0u;
-      sr += 4LL * a.n;
-      float bv = 0.f;
-      if (a.bias && row < a.n) bv = to_f32(static_cast<const T*>(a.bias)[row]);
-      for (int g0 = 0; g0 < ng; g0 += 4) {
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          if (g0 + i >= ng) break;          // (ng is even)
-          wait(&bar.dfull[td.slot], td.phase);
+        for (int gj = 0; gj < PAIRS; ++gj) {
+          wait(&bar.dfull[from], S::HALVES ? (from ? dphase[1] : dphase[0]) : dphase[0]);
           __syncwarp();
           tc::fence_after_sync();
-          const uint32_t D = at + 2 * td.slot * N;
+          const uint32_t D = at + 2 * from * N;
           constexpr int NP = S::COLS ? S::P : 1;          // columns of a token
-          // both of the pair at once, where the registers hold them
-          constexpr int ONCE = 2 * NP * TH <= 40 ? 2 : 1;
 #pragma unroll
-          for (int j0 = 0; j0 < 2; j0 += ONCE) {
-            float d[ONCE][NP][TH];
+          for (int j = 0; j < 2; ++j) {
+            float s;
+            if constexpr (S::IS32) s = __uint_as_float(s0[j]);
+            else if constexpr (std::is_same<T, __half>::value) s = __half2float(__ushort_as_half((unsigned short)s0[j]));
+            else s = __uint_as_float(s0[j] << 16);
 #pragma unroll
-            for (int j = 0; j < ONCE; ++j)
+            for (int b = 0; b < TH; b += TB) {
+              float d[NP][TB];
 #pragma unroll
-              for (int p = 0; p < NP; ++p) tmem_ld<TH>(D + (j0 + j) * N + p * MP, d[j][p]);
-            tmem_wait_ld();
-            if (j0 + ONCE == 2) {
-              tc::fence_before_sync();
-              __syncwarp();
-              if (lane == 0) tc::mbar_arrive(&bar.dempty[td.slot]);
-            }
+              for (int p = 0; p < NP; ++p) tmem_ld<TB>(D + j * N + p * MP + b, d[p]);
+              tmem_wait_ld();
+              if (j == 1 && b + TB == TH) {
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bar.dempty[from]);
+              }
 #pragma unroll
-            for (int j = 0; j < ONCE; ++j) {
-              const uint32_t raw = sq[i + j0 + j];
-              float s;
-              if constexpr (S::IS32) s = __uint_as_float(raw);
-              else if constexpr (std::is_same<T, __half>::value) s = __half2float(__ushort_as_half((unsigned short)raw));
-              else s = __uint_as_float(raw << 16);
+              for (int p = 0; p < NP; ++p) pin<TB>(d[p]);
 #pragma unroll
-              for (int p = 0; p < NP; ++p) pin<TH>(d[j][p]);
+              for (int t = 0; t < TB; ++t) {
+                float v = d[NP - 1][t];
 #pragma unroll
-              for (int t = 0; t < TH; ++t) {
-                float v = d[j][NP - 1][t];
-#pragma unroll
-                for (int p = NP - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[j][p][t]);
-                acc[t] = fmaf(s, v, acc[t]);
+                for (int p = NP - 2; p >= 0; --p) v = fmaf(v, 1.f / 32.f, d[p][t]);
+                acc[b + t] = fmaf(s, v, acc[b + t]);
               }
             }
           }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            sq[i + j] = 0;
-            if (g0 + i + j + 4 < have) sq[i + j] = __ldg(sr + (long long)(i + j) * a.n);
-          }
-          td.next(S::ND);
+          s0[0] = s1[0];
+          s0[1] = s1[1];
+          load_scales(s1);
+          if (S::HALVES && from) dphase[1] ^= 1;
+          else dphase[0] ^= 1;
         }
-        sr += 4LL * a.n;
+        turn ^= 1;
+      }
+      first = c - nc;
+      if (!S::HALVES) {
+        // one line's sums go to the other, which writes the tile out; they change places every tile.
+        // (Two buffers: a line writes one again after it has seen the other line's next sums, which
+        // that line has not handed over before reading these.)
+        float* to = part + buf * MP * ROWS + r;
+        if (line != buf) {
+#pragma unroll
+          for (int t = 0; t < TH; ++t) to[t * ROWS] = acc[t];
+          __threadfence_block();
+          asm volatile("bar.arrive %0, 256;" ::"r"(2 + buf) : "memory");
+          continue;
+        }
+        tc::named_sync(2 + buf, 256);
+#pragma unroll
+        for (int t = 0; t < TH; ++t) acc[t] = line ? to[t * ROWS] + acc[t] : acc[t] + to[t * ROWS];
       }
       // the tile's outputs (or this CTA's part of them)
-      {
-        uint32_t any = 0;
+#pragma unroll
+      for (int t = 0; t < TH; ++t) acc[t] *= s_factor[w - 12][t0 + t];      // (what is beyond toks is not stored)
+      if (any && row < a.n) {
+        const T* x = static_cast<const T*>(a.x);
 #pragma unroll
         for (int t = 0; t < TH; ++t) {
-          if (t0 + t < toks) {
-            acc[t] *= 512.f * s_scales[w - 12][t0 + t];
-            any |= s_masks[w - 12][t0 + t];
-          }
+          const uint32_t mask = t0 + t < toks ? s_marks[w - 12][t0 + t] : 0u;
+          for (int g = 0; mask && g < nc * GPC; ++g)
+            if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
+              acc[t] += left_out<T>(x + (m0 + t0 + t) * a.ldx, a.q, static_cast<const T*>(a.s), a.z, a.n, a.k, row,
+                                    (c0 * GPC + g) * G, G);
         }
-        if (any && row < a.n) {
-          const T* x = static_cast<const T*>(a.x);
+      }
+      if (a.ck > 1) {
+        float* red = reinterpret_cast<float*>(wst) + t0 * ROWS + r;   // (all stages are consumed: every sum is in)
 #pragma unroll
-          for (int t = 0; t < TH; ++t) {
-            const uint32_t mask = t0 + t < toks ? s_masks[w - 12][t0 + t] : 0u;
-            for (int g = 0; mask && g < ng; ++g)
-              if ((mask >> (((a.staged ? c0 * GPC : 0) + g) / span) & 1u) && (c0 * GPC + g) * G < a.k)
-                acc[t] += left_out<T>(x + (m0 + t0 + t) * a.ldx, a.q, static_cast<const T*>(a.s), a.z, a.n, a.k, row,
-                                      (c0 * GPC + g) * G, G);
-          }
-        }
-        if (a.ck > 1) {
-          float* red = reinterpret_cast<float*>(wst) + t0 * ROWS + r;   // (all stages are consumed: every sum is in)
+        for (int t = 0; t < TH; ++t)
+          if (t0 + t < toks) red[t * ROWS] = acc[t];
+      } else if (row < a.n) {
+        const long long o = (m0 + t0) * a.n + row;
+        if (a.out_f32) {
+          float* y = static_cast<float*>(a.y) + o;
 #pragma unroll
-          for (int t = 0; t < TH; ++t)
-            if (t0 + t < toks) red[t * ROWS] = acc[t];
-        } else if (row < a.n) {
-          const long long o = (m0 + t0) * a.n + row;
-          if (a.out_f32) {
-            float* y = static_cast<float*>(a.y) + o;
+          for (int t = 0; t < TH; ++t, y += a.n)
+            if (t0 + t < toks) *y = acc[t] + bv;
+        } else {
+          T* y = static_cast<T*>(a.y) + o;
 #pragma unroll
-            for (int t = 0; t < TH; ++t, y += a.n)
-              if (t0 + t < toks) *y = acc[t] + bv;
-          } else {
-            T* y = static_cast<T*>(a.y) + o;
-#pragma unroll
-            for (int t = 0; t < TH; ++t, y += a.n)
-              if (t0 + t < toks) *y = from_f32<T>(acc[t] + bv);
-          }
+          for (int t = 0; t < TH; ++t, y += a.n)
+            if (t0 + t < toks) *y = from_f32<T>(acc[t] + bv);
         }
       }
     }
@@ -812,11 +896,11 @@ Plan plan(long long m, int n, int k) {
   p.ck = 1;
   while (p.ck < 8 && units * p.ck * 2 <= 148 && chunks >= p.ck * 2) p.ck *= 2;
   p.per = (chunks + p.ck - 1) / p.ck;
-  const bool fits = (long long)p.per * S::BLK <= B_SMEM && p.per <= MAX_SB;
-  // every CTA stages x itself while that is at most two rounds of its warps
-  p.staged = !(fits && p.ytiles == 1 && m * p.per <= 2 * NT / 32);
+  const bool fits = (long long)p.per * S::BLK <= S::B_SMEM && p.per <= MAX_SB;
+  // every CTA stages x itself while that is at most five chunks for each of the eight warps that do it
+  p.staged = !(fits && p.ytiles == 1 && m * p.per <= 40);
   p.resident = fits && p.ytiles == 1;
-  p.sb = p.resident ? (p.per > 0 ? p.per : 1) : (B_SMEM / S::BLK < 8 ? B_SMEM / S::BLK : 8);
+  p.sb = p.resident ? (p.per > 0 ? p.per : 1) : (S::B_SMEM / S::BLK < 8 ? S::B_SMEM / S::BLK / 2 * 2 : 8);   // (even)
   p.ws_blocks = align_up((size_t)p.ytiles * chunks * S::BLK, 256);
   p.ws_total = p.staged ? p.ws_blocks + align_up((size_t)p.ytiles * S::MP * 8, 256) + 256 : 0;
   return p;
@@ -860,12 +944,12 @@ int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
     if (rc) return rc;
   }
   auto kern = int4_linear_kernel<T, S>;
-  const int smem = SW * W_STAGE + p.sb * BLK;
+  const int smem = S::SW * W_STAGE + p.sb * BLK + S::PART;
   static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
   int dev = 0;
   VERACE_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SW * W_STAGE + B_SMEM));
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
@@ -911,8 +995,11 @@ auto dispatch(long long m, int group, int dtype, F f) {
   };
   if (dtype == VERACE_F32) {
     if (m <= 4) return by_group(float(), std::integral_constant<int, 4>());
+    // (16 tokens' accumulators and the zeros of 8 groups do not fit TMEM together)
     if (m <= 8) return by_group(float(), std::integral_constant<int, 8>());
-    return by_group(float(), std::integral_constant<int, 16>());
+    if (group == 32) return f(float(), Shape<float, 8, 8>());
+    if (group == 64) return f(float(), Shape<float, 16, 4>());
+    return f(float(), Shape<float, 16, 2>());
   }
   if (dtype == VERACE_BF16) return by_tokens(__nv_bfloat16());
   return by_tokens(__half());
