@@ -19,6 +19,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <cstddef>
 
 namespace verace {
 namespace {
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
 struct Hist {
   uint32_t count[BINS], lack[BINS];
 };
+constexpr int GATHER = 1024;           // listed values of a row that one CTA cuts and chooses from by itself
 constexpr int LIST = 8192;             // values kept by the first level that a CTA lists (by 16-bit index)
 struct Shared {
   Hist hist[2];                        // of alternate levels: a level clears the next one's
@@ -189,6 +191,7 @@ struct Shared {
   int bin;
   uint32_t found;                      // the values in it
   unsigned long long left;             // of the target, before that bin
+  unsigned long long target;           // the mass that the cut by p leaves, absolute
 };
 
 // Every CTA's copy of one field, combined in rank order.
@@ -261,6 +264,7 @@ __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, 
     // a token is kept while the mass strictly above it is below p * total
     left = (unsigned long long)ceil((double)p * (double)total);
     if (left < 1) left = 1;
+    if (tid == 0) s.target = left;
   }
   if ((run >= left && run - mine < left) || (tid == BINS - 1 && run < left)) {
     s.bin = tid;
@@ -483,14 +487,119 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     }
   }
   if (bounded || by_least) listing = s.listed <= LIST;
-  if (bounded) {
-    visit([&](float x, int) { add_to(s.hist[1], (int)place(x), false, 0.f); });
-  }
   if (cuts) cl.sync();
+
+  // A short list, as it mostly is, goes to the first CTA, which compares every value with every
+  // other: kept are those with fewer than k greater ones, and then with less mass above them than
+  // the target.  (No more levels and barriers over the cluster.)
+  const float shift = top * inv;
+  const bool direct = fabsf(top / ts) <= 3.4028235e38f;
+  // the score: l / T - log(noise) where that is in range, z - log(noise) where it is not
+  auto score_of = [&](float x, float r) { return (direct ? x / ts : -(below(x) / ts)) - logf(r); };
+  unsigned long long choice = 0;
+  auto pack = [&](float score, int i) {
+    return ((unsigned long long)key_of(score + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
+  };
+  auto gather = [&] {
+    uint32_t total = 0;
+    const int ranks = cl.num_blocks();
+#pragma unroll 8
+    for (int i = 0; i < ranks; ++i) total += min(*cl.map_shared_rank(&s.listed, i), (uint32_t)(GATHER + 1));
+    if (total > GATHER) return false;
+    if (rank > 0) return true;
+    // (the histograms are read no more; the masses go where this CTA's list was)
+    float* gx = reinterpret_cast<float*>(s.hist);
+    int* gi = reinterpret_cast<int*>(gx + GATHER);
+    unsigned long long* gw = reinterpret_cast<unsigned long long*>(s.list);
+    static_assert(sizeof(s.hist) >= GATHER * 8 && sizeof(s.list) >= GATHER * 8 && offsetof(Shared, list) % 8 == 0,
+                  "gathered values fit");
+    int from = 0;
+    for (int q = 0; q < ranks; ++q) {
+      const Shared* other = cl.map_shared_rank(&s, q);
+      const T* values = cl.map_shared_rank(xs, q);
+      const int count = (int)other->listed;
+      for (int i = tid; i < count; i += CT) {
+        const int j = other->list[i];
+        gx[from + i] = to_f32(values[j]);
+        gi[from + i] = q * chunk + j;
+      }
+      from += count;
+    }
+    __syncthreads();
+    constexpr int EACH = GATHER / CT;
+    float x[EACH];
+    bool in[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = tid + e * CT;
+      in[e] = i < (int)total;
+      x[e] = in[e] ? gx[i] : -INFINITY;
+    }
+    if (cut_k) {
+      int greater[EACH] = {};
+      for (int j = 0; j < (int)total; ++j) {
+        const float y = gx[j];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) greater[e] += y > x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) in[e] = in[e] && greater[e] < k;
+    }
+    if (cut_p) {
+      unsigned long long sum = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const unsigned long long w =
+            in[e] ? (unsigned long long)(expf(-(below(x[e]) / ts)) * 1099511627776.f + 0.5f) : 0ull;
+        if (tid + e * CT < (int)total) gw[tid + e * CT] = w;
+        sum += w;
+      }
+      unsigned long long target = s.target;
+      if (cut_k) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s.red64[tid / 32] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < CT / 32; ++i) sum += s.red64[i];
+        target = (unsigned long long)ceil((double)p * (double)sum);
+        if (target < 1) target = 1;
+      }
+      __syncthreads();
+      unsigned long long above[EACH] = {};
+      for (int j = 0; j < (int)total; ++j) {
+        const float y = gx[j];
+        const unsigned long long w = gw[j];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) above[e] += y > x[e] ? w : 0ull;
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) in[e] = in[e] && above[e] < target;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (!in[e]) continue;
+      const float d = below(x[e]);
+      if (minp > 0.f && d != 0.f && !(-d * inv >= log_minp)) continue;
+      const int i = gi[tid + e * CT];
+      const float score = score_of(x[e], __ldg(noise + i));        // (the first CTA's noise is the row's)
+      if (score > -INFINITY) choice = max(choice, pack(score, i));
+    }
+    return true;
+  };
+  bool chosen = false;
+  if (bounded) {
+    chosen = gather();
+    if (!chosen) {
+      visit([&](float x, int) { add_to(s.hist[1], (int)place(x), false, 0.f); });
+      cl.sync();
+    }
+  }
 
   // ---- the cuts: what is kept is every value in a bin before `edge`, and in it the keys from
   // `least` on
-  for (int by_mass = 0; by_mass < 2; ++by_mass) {
+  for (int by_mass = 0; by_mass < 2 && !chosen; ++by_mass) {
     if (by_mass ? !cut_p : !cut_k) continue;
     const int kept_edge = edge;
     const uint32_t kept_least = least;
@@ -522,8 +631,12 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       __syncthreads();
       const float from = floor_of(cut);
       each([&](const float (&v)[8], int j) { list(v, j, from); });
-      __syncthreads();
+      cl.sync();
       listing = s.listed <= LIST;
+      if (by_mass && !cut_k) {
+        chosen = gather();
+        if (chosen) break;
+      }
     }
     if (more) {
       // the keys that bin `cut` can hold (its bounds, widened by the roundings of place)
@@ -566,13 +679,10 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   }
 
   // ---- the choice
-  // The score is l / T - log(noise) where that is in range, z - log(noise) where it is not.
-  const float shift = top * inv;
-  const bool direct = fabsf(top / ts) <= 3.4028235e38f;
-  auto score_of = [&](float x, float r) { return (direct ? x / ts : -(below(x) / ts)) - logf(r); };
   float best = -INFINITY;
   int at = -1;
-  if (greedy) {
+  if (chosen) {
+  } else if (greedy) {
     each([&](const float (&v)[8], int j) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -631,8 +741,7 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       }
     }
   }
-  unsigned long long choice =
-      at < 0 ? 0 : ((unsigned long long)key_of(best + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + at));
+  if (at >= 0) choice = pack(best, i0 + at);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned long long v = __shfl_xor_sync(0xffffffffu, choice, o);
