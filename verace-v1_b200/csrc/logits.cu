@@ -84,9 +84,10 @@ __device__ __noinline__ float bias_of(const void* ids, int i64, const float* val
   return 0.f;
 }
 
-// `ctas` CTAs a row, `range` tokens each; COUNTED: with counters.
-template <typename T, typename O, bool COUNTED>
-__global__ void __launch_bounds__(NT, 4) logits_ranges(LogitsArgs a, int ctas, int range) {
+// `ctas` CTAs a row, `range` tokens each; COUNTED: with counters; LONG: for long histories, whose
+// time is the latency of reading them: twice the loads in flight, two CTAs an SM instead of four.
+template <typename T, typename O, bool COUNTED, bool LONG>
+__global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, int ctas, int range) {
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ Biases s;
   const int tid = threadIdx.x, rank = blockIdx.x % ctas, row = blockIdx.x / ctas;
@@ -113,8 +114,9 @@ __global__ void __launch_bounds__(NT, 4) logits_ranges(LogitsArgs a, int ctas, i
       }
     }
     auto count = [&](long long token, int i) {
-      const long long t = token - v0;
-      if ((unsigned long long)t < (unsigned long long)nv) {
+      // (in 32-bit halves: this runs for every token of the history)
+      const uint32_t t = (uint32_t)token - (uint32_t)v0;
+      if (t < (uint32_t)nv && (uint32_t)((unsigned long long)token >> 32) == 0u) {
         if (i >= prompt) atomicAdd(&cnt[t], 1u);
         else atomicOr(&cnt[t], PROMPT);
       }
@@ -124,25 +126,42 @@ __global__ void __launch_bounds__(NT, 4) logits_ranges(LogitsArgs a, int ctas, i
     if (a.tokens_i64) {
       const long long* tk = static_cast<const long long*>(a.tokens) + base;
       if (reinterpret_cast<size_t>(tk) % 16 == 0) {
+        constexpr int FLY = LONG ? 8 : 4;
         done = len / 2 * 2;
-#pragma unroll 4
-        for (int i = 2 * tid; i < done; i += 2 * NT) {
-          const longlong2 u = __ldg(reinterpret_cast<const longlong2*>(tk + i));
-          count(u.x, i);
-          count(u.y, i + 1);
+        for (int i = 2 * tid; i < done; i += 2 * NT * FLY) {
+          longlong2 u[FLY];
+#pragma unroll
+          for (int e = 0; e < FLY; ++e) {
+            const int j = i + e * 2 * NT;
+            u[e] = j < done ? __ldg(reinterpret_cast<const longlong2*>(tk + j)) : make_longlong2(-1, -1);
+          }
+#pragma unroll
+          for (int e = 0; e < FLY; ++e) {
+            count(u[e].x, i + e * 2 * NT);
+            count(u[e].y, i + e * 2 * NT + 1);
+          }
         }
       }
     } else {
       const int* tk = static_cast<const int*>(a.tokens) + base;
       if (reinterpret_cast<size_t>(tk) % 16 == 0) {
+        constexpr int FLY = LONG ? 8 : 2;
         done = len / 4 * 4;
-#pragma unroll 2
-        for (int i = 4 * tid; i < done; i += 4 * NT) {
-          const int4 u = __ldg(reinterpret_cast<const int4*>(tk + i));
-          count(u.x, i);
-          count(u.y, i + 1);
-          count(u.z, i + 2);
-          count(u.w, i + 3);
+        for (int i = 4 * tid; i < done; i += 4 * NT * FLY) {
+          int4 u[FLY];
+#pragma unroll
+          for (int e = 0; e < FLY; ++e) {
+            const int j = i + e * 4 * NT;
+            u[e] = j < done ? __ldg(reinterpret_cast<const int4*>(tk + j)) : make_int4(-1, -1, -1, -1);
+          }
+#pragma unroll
+          for (int e = 0; e < FLY; ++e) {
+            const int j = i + e * 4 * NT;
+            count(u[e].x, j);
+            count(u[e].y, j + 1);
+            count(u[e].z, j + 2);
+            count(u[e].w, j + 3);
+          }
         }
       }
     }
@@ -253,9 +272,9 @@ __global__ void __launch_bounds__(NT) logits_chunks(LogitsArgs a) {
   }
 }
 
-template <typename T, typename O, bool COUNTED>
+template <typename T, typename O, bool COUNTED, bool LONG>
 int launch_ranges(const LogitsArgs& a, int ctas, int range, cudaStream_t st) {
-  auto kern = logits_ranges<T, O, COUNTED>;
+  auto kern = logits_ranges<T, O, COUNTED, LONG>;
   const size_t smem = COUNTED ? (size_t)range * 4 : 0;
   if (COUNTED) {
     static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
@@ -280,7 +299,7 @@ int run(const LogitsArgs& a, cudaStream_t st) {
     // 4096 values a CTA, or more where the rows alone fill the device several times over
     c = (a.v + 4095) / 4096;
     if ((long long)a.b * c > 4096) c = (a.v + 16383) / 16384;
-    return launch_ranges<T, O, false>(a, c, range_of(c), st);
+    return launch_ranges<T, O, false, false>(a, c, range_of(c), st);
   }
   if (a.length >= LENGTH_MAX) {
     logits_chunks<T, O><<<dim3((a.v + CHUNK - 1) / CHUNK, a.b), NT, 0, st>>>(a);
@@ -288,10 +307,12 @@ int run(const LogitsArgs& a, cudaStream_t st) {
   }
   // long histories, which every CTA of a row reads: fewer and larger ranges; otherwise more of
   // them (of 2048 tokens at least) while the rows leave the device empty
-  const int most = a.length > 16384 ? RANGE_LONG : RANGE;
+  const bool long_history = a.length > 16384;
+  const int most = long_history ? RANGE_LONG : RANGE;
   c = (a.v + most - 1) / most;
   while ((long long)a.b * c * 2 <= 296 && range_of(2 * c) >= 2048) c *= 2;
-  return launch_ranges<T, O, true>(a, c, range_of(c), st);
+  return long_history ? launch_ranges<T, O, true, true>(a, c, range_of(c), st)
+                      : launch_ranges<T, O, true, false>(a, c, range_of(c), st);
 }
 
 }  // namespace
