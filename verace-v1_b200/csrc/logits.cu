@@ -26,7 +26,7 @@ constexpr int LIST = 512;     // biases of a CTA's range held in shared memory
 // A counter: seen in the prompt, biased, the bias's place in the list, the generated count.
 constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, PLACE = 20, COUNT = 0xfffffu;
 constexpr int LENGTH_MAX = 1 << 20;
-constexpr int RANGE = 11264, RANGE_LONG = 24576;   // tokens of a CTA at most (four and two CTAs an SM)
+constexpr int RANGE = 11264, RANGE_LONG = 24576;   // tokens of a CTA at most
 
 struct LogitsArgs {
   const void* logits;
@@ -85,9 +85,10 @@ __device__ __noinline__ float bias_of(const void* ids, int i64, const float* val
 }
 
 // `ctas` CTAs a row, `range` tokens each; COUNTED: with counters; LONG: for long histories, whose
-// time is the latency of reading them: twice the loads in flight, two CTAs an SM instead of four.
+// time is the pass over them: twice the threads, and twice the loads in flight for each.
 template <typename T, typename O, bool COUNTED, bool LONG>
-__global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, int ctas, int range) {
+__global__ void __launch_bounds__(LONG ? 2 * NT : NT, LONG ? 1 : 4) logits_ranges(LogitsArgs a, int ctas, int range) {
+  constexpr int NTH = LONG ? 2 * NT : NT;
   extern __shared__ __align__(16) uint32_t cnt[];
   __shared__ Biases s;
   const int tid = threadIdx.x, rank = blockIdx.x % ctas, row = blockIdx.x / ctas;
@@ -99,13 +100,13 @@ __global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, 
   if constexpr (COUNTED) {
     // the range comes into L2 while the history is counted
     constexpr int LINE = 128 / sizeof(T);
-    for (int i = tid * LINE; i < nv; i += NT * LINE) asm volatile("prefetch.global.L2 [%0];" ::"l"(in + i));
+    for (int i = tid * LINE; i < nv; i += NTH * LINE) asm volatile("prefetch.global.L2 [%0];" ::"l"(in + i));
     if (mask && tid * 1024 < nv) asm volatile("prefetch.global.L2 [%0];" ::"l"(mask + tid * 128));
-    for (int i = 4 * tid; i < range; i += 4 * NT) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
+    for (int i = 4 * tid; i < range; i += 4 * NTH) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
     if (tid == 0) s.n = 0;
     const int len = history(a, row), prompt = a.prompt_lengths ? a.prompt_lengths[row] : 0;
     __syncthreads();
-    for (int i = tid; i < a.n_bias; i += NT) {
+    for (int i = tid; i < a.n_bias; i += NTH) {
       const long long id = id_at(a.bias_ids, a.bias_i64, (long long)row * a.n_bias + i) - v0;
       if (id >= 0 && id < nv) {
         const int at = atomicAdd(&s.n, 1);
@@ -128,17 +129,17 @@ __global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, 
       if (reinterpret_cast<size_t>(tk) % 16 == 0) {
         constexpr int FLY = LONG ? 8 : 4;
         done = len / 2 * 2;
-        for (int i = 2 * tid; i < done; i += 2 * NT * FLY) {
+        for (int i = 2 * tid; i < done; i += 2 * NTH * FLY) {
           longlong2 u[FLY];
 #pragma unroll
           for (int e = 0; e < FLY; ++e) {
-            const int j = i + e * 2 * NT;
+            const int j = i + e * 2 * NTH;
             u[e] = j < done ? __ldg(reinterpret_cast<const longlong2*>(tk + j)) : make_longlong2(-1, -1);
           }
 #pragma unroll
           for (int e = 0; e < FLY; ++e) {
-            count(u[e].x, i + e * 2 * NT);
-            count(u[e].y, i + e * 2 * NT + 1);
+            count(u[e].x, i + e * 2 * NTH);
+            count(u[e].y, i + e * 2 * NTH + 1);
           }
         }
       }
@@ -147,16 +148,16 @@ __global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, 
       if (reinterpret_cast<size_t>(tk) % 16 == 0) {
         constexpr int FLY = LONG ? 8 : 2;
         done = len / 4 * 4;
-        for (int i = 4 * tid; i < done; i += 4 * NT * FLY) {
+        for (int i = 4 * tid; i < done; i += 4 * NTH * FLY) {
           int4 u[FLY];
 #pragma unroll
           for (int e = 0; e < FLY; ++e) {
-            const int j = i + e * 4 * NT;
+            const int j = i + e * 4 * NTH;
             u[e] = j < done ? __ldg(reinterpret_cast<const int4*>(tk + j)) : make_int4(-1, -1, -1, -1);
           }
 #pragma unroll
           for (int e = 0; e < FLY; ++e) {
-            const int j = i + e * 4 * NT;
+            const int j = i + e * 4 * NTH;
             count(u[e].x, j);
             count(u[e].y, j + 1);
             count(u[e].z, j + 2);
@@ -166,12 +167,12 @@ __global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, 
       }
     }
 #pragma unroll 4
-    for (int i = done + tid; i < len; i += NT) count(id_at(a.tokens, a.tokens_i64, base + i), i);
+    for (int i = done + tid; i < len; i += NTH) count(id_at(a.tokens, a.tokens_i64, base + i), i);
     __syncthreads();
     if (a.n_bias) {
       // of the list's entries for one token the last in the row's order holds
       const int listed = min(s.n, LIST);
-      for (int i = tid; i < listed; i += NT) {
+      for (int i = tid; i < listed; i += NTH) {
         const int id = s.id[i], order = s.order[i];
         bool last = true;
         for (int j = 0; j < listed; ++j) last = last && !(s.id[j] == id && s.order[j] > order);
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, 
   if ((reinterpret_cast<size_t>(in) | reinterpret_cast<size_t>(out)) % 16 == 0) {
     done = nv / 8 * 8;
 #pragma unroll 2
-    for (int j = 8 * tid; j < done; j += 8 * NT) {
+    for (int j = 8 * tid; j < done; j += 8 * NTH) {
       uint4 u[sizeof(T) / 2];
 #pragma unroll
       for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = reinterpret_cast<const uint4*>(in + j)[i];
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(NT, LONG ? 2 : 4) logits_ranges(LogitsArgs a, 
     }
   }
 #pragma unroll 4
-  for (int j = done + tid; j < nv; j += NT) {
+  for (int j = done + tid; j < nv; j += NTH) {
     float l = to_f32(in[j]);
     if constexpr (COUNTED) {
       if (cnt[j]) l = one(l, cnt[j], j);
@@ -287,7 +288,7 @@ int launch_ranges(const LogitsArgs& a, int ctas, int range, cudaStream_t st) {
   }
   VERACE_REQUIRE((long long)a.b * ctas <= 0x7fffffffLL, VERACE_ERR_UNSUPPORTED, "logits_process: %d rows of %d", a.b,
                  a.v);
-  kern<<<(unsigned)((long long)a.b * ctas), NT, smem, st>>>(a, ctas, range);
+  kern<<<(unsigned)((long long)a.b * ctas), LONG ? 2 * NT : NT, smem, st>>>(a, ctas, range);
   return check_launch("logits_process");
 }
 
