@@ -97,6 +97,34 @@ def test_process_matches_formula(b, v, length, dtype):
         check_process(out, ref, size, odt)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,v,length,among,n,pad", [(130, 32776, 601, 32776, 40, 0), (65, 65543, 4000, 6000, 20, 1),
+                                                    (66, 65600, 50, 65600, 700, 8), (130, 32800, 0, 1, 900, 0)])
+def test_process_many_wide_rows(b, v, length, among, n, pad, dtype):
+    """Histories over few or many tokens, biases few or many, of one token or many, in place too."""
+    g = torch.Generator().manual_seed(b + v + length)
+    l = (3 * torch.randn(b, v + pad, generator=g)).to(dtype)[:, :v]
+    tokens = torch.randint(-3, among, (b, max(length, 1)), generator=g)[:, :length]
+    lengths, prompts = torch.randint(0, length + 1, (b,), generator=g), torch.randint(0, length + 1, (b,), generator=g)
+    lengths[:3], prompts[:2] = length, torch.tensor([0, length])
+    r, p, f = 1 + torch.rand(b, generator=g), torch.rand(b, generator=g), 0.3 * torch.rand(b, generator=g) - 0.1
+    ids = torch.randint(-1, min(v, 20000), (b, n), generator=g)
+    ids[1] = 7                                                   # one token, all its biases
+    values = 5 * torch.randn(b, n, generator=g)
+    words = torch.randint(-2 ** 31, 2 ** 31, (b, (v + 31) // 32), generator=g).int()
+    words[2] = 0
+    ref, size = process_reference(l, tokens, lengths, prompts, r.double().numpy(), p.double().numpy(),
+                                  f.double().numpy(), ids, values, words)
+    for i32, odt, place in ((False, torch.float32, False), (True, dtype, False), (False, dtype, True)):
+        cast = (lambda t: t.int()) if i32 else (lambda t: t)
+        ld = torch.empty(b, v + pad, dtype=dtype, device="cuda")[:, :v].copy_(l)
+        out = V.process_logits(ld, cast(tokens).cuda(), lengths.cuda(), prompts.cuda(), repetition_penalty=r.cuda(),
+                               presence_penalty=p.cuda(), frequency_penalty=f.cuda(), bias_ids=cast(ids).cuda(),
+                               bias_values=values.cuda(), allowed=words.cuda(), out_dtype=odt, out=ld if place else None)
+        assert not place or out.data_ptr() == ld.data_ptr()
+        check_process(out, ref, size, odt)
+
+
 def test_process_parts_alone_and_scalars():
     g = torch.Generator().manual_seed(5)
     l = torch.randn(4, 700, generator=g)

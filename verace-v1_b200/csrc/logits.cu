@@ -7,12 +7,17 @@
 //     l <- -inf                         where the mask's bit is 0
 //
 // Bound: the bytes of the logits in and out.  Each CTA takes a range of a row's vocabulary, with a
-// 32-bit counter per token in shared memory, and reads the whole history of the row (from L2 after
-// the first), counting what falls into its range.  (Sharing the history out over a cluster and
-// counting in distributed shared memory was slower: 23 k clocks for 8192 tokens a CTA, remote
-// atomics being the slower ones.)  Then it streams its range, eight values a thread: most have
-// no count, no bias and a full mask, and are copied.  A biased token's counter holds the place of
-// its bias in a short list.
+// counter per token in shared memory, and reads the whole history of the row (from L2 after the
+// first), counting what falls into its range.  (Sharing the history out over a cluster and counting
+// in distributed shared memory was slower: 23 k clocks for 8192 tokens a CTA, remote atomics being
+// the slower ones.)  Then it streams its range, eight values a thread: most have no count, no bias
+// and a full mask, and are copied.
+//
+// Measured on the device: a row of 32000 with 200 tokens of history 3.7 us; 64 rows of 163840, bf16
+// to fp32, 63 MB: mask alone 12.9 us (4.9 TB/s), with 4096 tokens of history 19, with 300 biases too
+// 20.9 (3.0 TB/s; 28 before the listed form: the counting went before the stream, not beside it; what
+// is left is the counting's chain of loads under the stream's, 10 us); 8 rows of 32000 with 65536
+// tokens of history 11.6, in which every CTA of a row reads its history from L2.
 #include "common.cuh"
 
 #include <atomic>
@@ -25,8 +30,9 @@ constexpr int CHUNK = 4096;   // vocabulary entries per CTA of logits_chunks
 constexpr int LIST = 512;     // biases of a CTA's range held in shared memory
 // A counter: seen in the prompt, biased, the bias's place in the list, the generated count.
 constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, PLACE = 20, COUNT = 0xfffffu;
-constexpr int LENGTH_MAX = 1 << 20;
-constexpr int RANGE = 11264, RANGE_LONG = 24576;   // tokens of a CTA at most
+constexpr int LENGTH_MAX = 1 << 20, LENGTH_LISTED = 1 << 14;   // histories below these fit the counters
+constexpr int RANGE = 11264, RANGE_LONG = 24576, RANGE_LISTED = 18432;   // tokens of a CTA at most
+constexpr int TOUCHED = 2048; // touched tokens listed
 
 struct LogitsArgs {
   const void* logits;
@@ -76,6 +82,33 @@ struct Biases {
   int id[LIST], order[LIST];
   float value[LIST];
 };
+
+// Eight values from 16 or 32 bytes, and eight to the output, those left out by the mask as -inf.
+template <typename T>
+__device__ __forceinline__ void values8(const uint4* u, float* l) {
+  if constexpr (sizeof(T) == 4) {
+    l[0] = __uint_as_float(u[0].x); l[1] = __uint_as_float(u[0].y);
+    l[2] = __uint_as_float(u[0].z); l[3] = __uint_as_float(u[0].w);
+    l[4] = __uint_as_float(u[1].x); l[5] = __uint_as_float(u[1].y);
+    l[6] = __uint_as_float(u[1].z); l[7] = __uint_as_float(u[1].w);
+  } else {
+    unpack8<T>(u[0], l);
+  }
+}
+template <typename O>
+__device__ __forceinline__ void store8(O* out, float* l, uint32_t bits) {
+  if (bits != 255u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(bits >> i & 1u)) l[i] = -INFINITY;
+  }
+  if constexpr (sizeof(O) == 4) {
+    reinterpret_cast<float4*>(out)[0] = make_float4(l[0], l[1], l[2], l[3]);
+    reinterpret_cast<float4*>(out)[1] = make_float4(l[4], l[5], l[6], l[7]);
+  } else {
+    *reinterpret_cast<uint4*>(out) = pack8<O>(l);
+  }
+}
 
 // The last of the row's biases for a token.
 __device__ __noinline__ float bias_of(const void* ids, int i64, const float* values, long long first, int n, int token) {
@@ -197,14 +230,7 @@ __global__ void __launch_bounds__(LONG ? 2 * NT : NT, LONG ? 1 : 4) logits_range
       for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = reinterpret_cast<const uint4*>(in + j)[i];
       const uint32_t bits = mask ? __ldg(mask + j / 8) : 255u;
       float l[8];
-      if constexpr (sizeof(T) == 4) {
-        l[0] = __uint_as_float(u[0].x); l[1] = __uint_as_float(u[0].y);
-        l[2] = __uint_as_float(u[0].z); l[3] = __uint_as_float(u[0].w);
-        l[4] = __uint_as_float(u[1].x); l[5] = __uint_as_float(u[1].y);
-        l[6] = __uint_as_float(u[1].z); l[7] = __uint_as_float(u[1].w);
-      } else {
-        unpack8<T>(u[0], l);
-      }
+      values8<T>(u, l);
       if constexpr (COUNTED) {
         const uint4 c = *reinterpret_cast<const uint4*>(cnt + j), d = *reinterpret_cast<const uint4*>(cnt + j + 4);
         if (c.x | c.y | c.z | c.w | d.x | d.y | d.z | d.w) {
@@ -214,17 +240,7 @@ __global__ void __launch_bounds__(LONG ? 2 * NT : NT, LONG ? 1 : 4) logits_range
             if (e[i]) l[i] = one(l[i], e[i], j + i);
         }
       }
-      if (bits != 255u) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (!(bits >> i & 1u)) l[i] = -INFINITY;
-      }
-      if constexpr (sizeof(O) == 4) {
-        reinterpret_cast<float4*>(out + j)[0] = make_float4(l[0], l[1], l[2], l[3]);
-        reinterpret_cast<float4*>(out + j)[1] = make_float4(l[4], l[5], l[6], l[7]);
-      } else {
-        *reinterpret_cast<uint4*>(out + j) = pack8<O>(l);
-      }
+      store8<O>(out + j, l, bits);
     }
   }
 #pragma unroll 4
@@ -235,6 +251,165 @@ __global__ void __launch_bounds__(LONG ? 2 * NT : NT, LONG ? 1 : 4) logits_range
     }
     if (mask && !(__ldg(mask + j / 8) >> (j % 8) & 1u)) l = -INFINITY;
     out[j] = from_f32<O>(l);
+  }
+}
+
+struct Places {      // places in the row's list of biases whose tokens are in the CTA's range, in any order
+  int n;
+  int2 entry[LIST];  // token, place
+};
+
+// The same for many wide rows, in which history and bias touch few tokens.  Half the threads count,
+// list each token at its first time and compute the listed ones' logits; the other half, and then
+// all, stream the range as though nothing touched it; the listed logits are stored last.  (In place
+// too: a value that the mask leaves is stored as it was read.)  The counters are of 16 bits, a pair
+// to a word, so that four CTAs' fit an SM and the rows one wave.
+template <typename T, typename O>
+__global__ void __launch_bounds__(NT, 4) logits_listed(LogitsArgs a, int ctas, int range) {
+  constexpr int CT = NT / 2;
+  constexpr uint32_t SEEN = 0x8000u, NAMED = 0x4000u, MADE = NAMED - 1;
+  extern __shared__ __align__(16) uint32_t cnt[];
+  __shared__ Places s;
+  __shared__ uint16_t list[TOUCHED];
+  __shared__ float value[TOUCHED];
+  __shared__ int touched, next;                                  // tokens listed; the first piece that no warp has
+  const int tid = threadIdx.x, lane = tid % 32, rank = blockIdx.x % ctas, row = blockIdx.x / ctas;
+  const int v0 = rank * range, nv = max(0, min(range, a.v - v0));
+  const T* in = static_cast<const T*>(a.logits) + row * a.ld + v0;
+  O* out = static_cast<O*>(a.out) + row * a.out_ld + v0;
+  const uint8_t* mask = a.allowed ? reinterpret_cast<const uint8_t*>(a.allowed + row * a.allowed_ld) + v0 / 8 : nullptr;
+  const long long first = row * (long long)a.n_bias;
+  auto counter = [&](int j) { return cnt[j / 2] >> 16 * (j & 1) & 0xffffu; };
+  auto bias_at = [&](int j) {
+    const int listed = s.n;
+    if (listed > LIST) return bias_of(a.bias_ids, a.bias_i64, a.bias_values, first, a.n_bias, v0 + j);
+    int place = 0;                                               // the last of equal tokens holds
+    for (int e = 0; e < listed; ++e) {
+      const int2 entry = s.entry[e];
+      if (entry.x == j) place = max(place, entry.y);
+    }
+    return a.bias_values[first + place];
+  };
+  auto final_of = [&](int j, const Controls& k) {
+    const uint32_t c = counter(j);
+    float l = to_f32(in[j]);
+    if (c & (SEEN | MADE)) l = penalised(l, c & MADE, k);
+    return c & NAMED ? l + bias_at(j) : l;
+  };
+  if (tid == 0) s.n = 0, touched = 0, next = 0;
+  __syncthreads();
+
+  if (tid < CT) {
+    auto together = [] { asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory"); };
+    // the first tokens and biases are asked for before all else (within the rows' strides, whatever
+    // the lengths): under the stream's loads each step of such a chain waits for microseconds
+    constexpr int FLY = 4;
+    const long long base = row * a.tokens_ld;
+    const char* tk = static_cast<const char*>(a.tokens) + base * (a.tokens_i64 ? 8 : 4);
+    const int per = a.tokens_i64 ? 2 : 4;                        // tokens in 16 bytes
+    const int fast = a.tokens && reinterpret_cast<size_t>(tk) % 16 == 0 ? a.length / per * per : 0;
+    uint4 u[FLY];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int e = 0; e < FLY; ++e) {
+        const int i = i0 + (e * CT + tid) * per;
+        if (i < fast) u[e] = __ldg(reinterpret_cast<const uint4*>(tk + (long long)i * (16 / per)));
+      }
+    };
+    fetch(0);
+    const long long bias0 = tid < a.n_bias ? id_at(a.bias_ids, a.bias_i64, first + tid) : -1;
+    const int len = history(a, row), prompt = a.prompt_lengths ? a.prompt_lengths[row] : 0;
+    for (int i = 4 * tid; i < range / 2; i += 4 * CT) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
+    together();
+    const Controls k = controls(a, row);
+    auto mark = [&](uint32_t t, uint32_t bits, bool add) {
+      const int at = 16 * (t & 1);
+      const uint32_t old = add ? atomicAdd(cnt + t / 2, bits << at) : atomicOr(cnt + t / 2, bits << at);
+      if (old >> at & 0xffffu) return;
+      const int n = atomicAdd(&touched, 1);                      // the token's first time
+      if (n < TOUCHED) list[n] = (uint16_t)t;
+    };
+    auto count = [&](uint32_t low, uint32_t high, int i) {
+      const uint32_t t = low - (uint32_t)v0;
+      if (t < (uint32_t)nv && high == 0u) mark(t, i >= prompt ? 1u : SEEN, i >= prompt);
+    };
+    for (int i = tid; i < a.n_bias; i += CT) {
+      const long long id = (i == tid ? bias0 : id_at(a.bias_ids, a.bias_i64, first + i)) - v0;
+      if (id >= 0 && id < nv) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < LIST) s.entry[at] = make_int2((int)id, i);
+        mark((uint32_t)id, NAMED, false);
+      }
+    }
+    const int done = min(fast, len / per * per);
+    for (int i0 = 0; i0 < done; i0 += FLY * CT * per) {
+      if (i0 > 0) fetch(i0);
+#pragma unroll
+      for (int e = 0; e < FLY; ++e) {
+        const int i = i0 + (e * CT + tid) * per;
+        if (i < done) {
+          if (a.tokens_i64) {
+            count(u[e].x, u[e].y, i);
+            count(u[e].z, u[e].w, i + 1);
+          } else {                                               // (a negative one's high half is not 0)
+            count(u[e].x, u[e].x >> 31, i);
+            count(u[e].y, u[e].y >> 31, i + 1);
+            count(u[e].z, u[e].z >> 31, i + 2);
+            count(u[e].w, u[e].w >> 31, i + 3);
+          }
+        }
+      }
+    }
+    for (int i = done + tid; i < len; i += CT) {
+      const long long t = id_at(a.tokens, a.tokens_i64, base + i);
+      count((uint32_t)t, (uint32_t)((unsigned long long)t >> 32), i);
+    }
+    together();
+    if (touched <= TOUCHED)
+      for (int i = tid; i < touched; i += CT) value[i] = final_of(list[i], k);
+    __syncwarp();
+  }
+
+  // the range, in pieces of a warp's 512 values
+  const bool wide = (reinterpret_cast<size_t>(in) | reinterpret_cast<size_t>(out)) % 16 == 0;
+  while (true) {
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&next, 1);
+    const int j0 = __shfl_sync(~0u, at, 0) * 512;
+    if (j0 >= nv) break;
+    if (wide && j0 + 512 <= nv) {
+      uint4 u[2][sizeof(T) / 2];
+      uint32_t bits[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = j0 + 8 * (32 * e + lane);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[e][i] = reinterpret_cast<const uint4*>(in + j)[i];
+        bits[e] = mask ? __ldg(mask + j / 8) : 255u;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l[8];
+        values8<T>(u[e], l);
+        store8<O>(out + j0 + 8 * (32 * e + lane), l, bits[e]);
+      }
+    } else {
+      for (int j = j0 + lane; j < min(j0 + 512, nv); j += 32) {
+        const bool kept = !mask || __ldg(mask + j / 8) >> (j % 8) & 1u;
+        out[j] = from_f32<O>(kept ? to_f32(in[j]) : -INFINITY);
+      }
+    }
+  }
+  __syncthreads();
+  auto put = [&](int j, float l) {
+    if (!mask || __ldg(mask + j / 8) >> (j % 8) & 1u) out[j] = from_f32<O>(l);
+  };
+  if (touched <= TOUCHED) {
+    for (int i = tid; i < touched; i += NT) put(list[i], value[i]);
+  } else {                                                       // more than the list holds
+    const Controls k = controls(a, row);
+    for (int j = tid; j < nv; j += NT)
+      if (counter(j)) put(j, final_of(j, k));
   }
 }
 
@@ -273,18 +448,24 @@ __global__ void __launch_bounds__(NT) logits_chunks(LogitsArgs a) {
   }
 }
 
+// Raises a kernel's limit of shared memory, once on each device.
+int raise_limit(const void* kern, std::atomic<uint64_t>& ready, int bytes) {
+  int dev = 0;
+  VERACE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  return VERACE_OK;
+}
+
 template <typename T, typename O, bool COUNTED, bool LONG>
 int launch_ranges(const LogitsArgs& a, int ctas, int range, cudaStream_t st) {
   auto kern = logits_ranges<T, O, COUNTED, LONG>;
   const size_t smem = COUNTED ? (size_t)range * 4 : 0;
   if (COUNTED) {
-    static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
-    int dev = 0;
-    VERACE_CUDA(cudaGetDevice(&dev));
-    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-      VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * RANGE_LONG));
-      if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
+    static std::atomic<uint64_t> ready{0};
+    if (int rc = raise_limit(reinterpret_cast<const void*>(kern), ready, 4 * RANGE_LONG)) return rc;
   }
   VERACE_REQUIRE((long long)a.b * ctas <= 0x7fffffffLL, VERACE_ERR_UNSUPPORTED, "logits_process: %d rows of %d", a.b,
                  a.v);
@@ -305,6 +486,21 @@ int run(const LogitsArgs& a, cudaStream_t st) {
   if (a.length >= LENGTH_MAX) {
     logits_chunks<T, O><<<dim3((a.v + CHUNK - 1) / CHUNK, a.b), NT, 0, st>>>(a);
     return check_launch("logits_process");
+  }
+  // Many wide rows of 16 bits with short histories: listed (256 rows of 32000 with 512 tokens 15.0 us,
+  // by ranges 18.0; 64 of 163840 with 4096 and 300 biases 20.9, by ranges 28; but 64 of 163840 with
+  // 16000 44 against 36, 16 of 163840 with 1024 8.3 against 7.8, and fp32 rows are no faster).
+  if constexpr (sizeof(T) == 2) {
+    if (a.length < LENGTH_LISTED && a.length <= a.v / 16 && (long long)a.b * a.v >= 1LL << 22) {
+      c = (a.v + RANGE_LISTED - 1) / RANGE_LISTED;
+      while ((long long)a.b * c * 2 <= 592 && range_of(2 * c) >= 2048) c *= 2;
+      VERACE_REQUIRE((long long)a.b * c <= 0x7fffffffLL, VERACE_ERR_UNSUPPORTED, "logits_process: %d rows of %d", a.b, a.v);
+      auto kern = logits_listed<T, O>;
+      static std::atomic<uint64_t> ready{0};
+      if (int rc = raise_limit(reinterpret_cast<const void*>(kern), ready, 2 * RANGE_LISTED)) return rc;
+      kern<<<(unsigned)((long long)a.b * c), NT, range_of(c) * 2, st>>>(a, c, range_of(c));
+      return check_launch("logits_process");
+    }
   }
   // long histories, which every CTA of a row reads: fewer and larger ranges; otherwise more of
   // them (of 2048 tokens at least) while the rows leave the device empty
