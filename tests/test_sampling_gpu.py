@@ -254,6 +254,8 @@ def sample_reference(l, noise, t, k, p, minp):
     top = z.max()
     if top == -np.inf:
         return -1, -np.inf, True
+    if top == np.inf:                                            # the infinities share the mass
+        z, top = np.where(z == top, 0.0, -np.inf), 0.0
     with np.errstate(invalid="ignore"):
         w = np.where(z == top, 1.0, np.exp(z - top))
     chosen, clear = [], True
@@ -326,6 +328,21 @@ def test_sample_matches_formula(b, v, dtype):
             (1.0, 1, 1.0, 0.0, 0.0), (0.8, 40, 0.6, 0.05, 0.5), (1.0, 0, 1.0, 0.1, 0.9), (1.0, 1000, 0.5, 0.0, 0.0)]):
         l, noise = draw(b, v, 100 * seed + b + v, masked, dtype)
         check_sample(l, noise if t else None, t, k, p, minp, most_clear=b * v > 100)
+
+
+@pytest.mark.parametrize("v,dtype", [(20501, torch.float32), (20608, torch.float32), (41001, torch.bfloat16)])
+def test_sample_many_rows_too_long_to_hold(v, dtype):
+    """More rows than shared memory holds, values of every kind at the rows' ends among them."""
+    b = 300
+    l, noise = draw(b, v, 11, dtype=dtype)
+    lowest = torch.finfo(dtype).min
+    l[1], l[2], l[3, 100:], l[6], l[7] = -INF, -INF, -INF, 0.0, lowest
+    l[2, v - 1] = lowest
+    l[4, ::7] = float("nan")
+    l[5, 5:9], l[8, v - 1], l[b - 1] = INF, 30.0, lowest
+    for t, k, p, minp in ((0.8, 50, 0.9, 0.0), (1.3, 0, 0.7, 0.0), (1.0, 5000, 1.0, 0.0), (0.7, 0, 1.0, 0.01),
+                          (1.0, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0)):
+        check_sample(l, noise if t else None, t, k, p, minp)
 
 
 def test_sample_per_row_controls():

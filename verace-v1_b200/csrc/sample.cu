@@ -7,13 +7,19 @@
 // the largest logit.  logprob = log softmax(z)[token] over the whole row (T = 0: of l).
 //
 // Two kernels.  sample_cluster: a cluster of CTAs per row, the row read once and kept in shared
-// memory, where the passes after the first run.  The cuts by count (k) and by mass (p) come from
+// memory, where the passes after the first run, or (HELD false) read by each pass, from L2 mostly.  The cuts by count (k) and by mass (p) come from
 // histograms in shared memory, joined over the cluster: first 512 bins linear in z (values
 // near the top spread over many bins; bins of the float's bits would put most of a row into a
 // handful), then within the bin of the cut 512 bins of the values' order-preserving keys, until
 // a bin holds one value or one key: two or three levels for most rows, five at worst.
-// sample_rows: one CTA per row that reads it again for every pass; for rows that no cluster
-// holds.  Mass is summed in 2^-40 fixed point, so that the order of the atomics changes nothing.
+// sample_rows: one CTA per row that reads it again for every pass; for rows of more than 16 x 65536
+// values.  Mass is summed in 2^-40 fixed point, so that the order of the atomics changes nothing.
+//
+// Bound: one read of the row, and of the noise where every value draws.  Measured on the device: one
+// row of 32000 at T = 0 6.1 us (launch and cluster barriers); 64 fp32 rows of 163840 with k = 50,
+// p = 0.9 and min_p 30 us for 42 MB (1.4 TB/s: two passes, the second from L2, then about ten steps
+// between barriers of the cluster; one CTA a row that read it again for every step: 1924); 256 bf16 rows of
+// 32000 without cuts 25 us for 49 MB with the noise (2.0 TB/s: the arithmetic per value).
 #include "common.cuh"
 
 #include <cooperative_groups.h>
@@ -274,7 +280,8 @@ __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, 
   __syncthreads();
 }
 
-template <typename T>
+// HELD: the row is kept in shared memory; else every pass reads it from L2.
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk) {
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ __align__(16) Shared s;
@@ -319,8 +326,8 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       bool nan = f[0] != f[0];
 #pragma unroll
       for (int e = 1; e < E; ++e) most = fmaxf(most, f[e]), nan |= f[e] != f[e];
-      *reinterpret_cast<uint4*>(xs + j) = u;
-      if (nan) {
+      if constexpr (HELD) *reinterpret_cast<uint4*>(xs + j) = u;
+      if (HELD && nan) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (f[e] != f[e]) xs[j + e] = none;
@@ -332,15 +339,34 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   for (int j = done + tid; j < n; j += CT) {
     const T u = src[j];
     const float f = to_f32(u);
-    xs[j] = f != f ? none : u;
+    if constexpr (HELD) xs[j] = f != f ? none : u;
     top = fmaxf(top, f);
   }
   top = top + 0.f;
   const float mine = top;              // the thread's largest
   const int n8 = (n + 7) / 8;
-  if (tid < n8 * 8 - n) xs[n + tid] = none;
+  if (HELD && tid < n8 * 8 - n) xs[n + tid] = none;
   auto values = [&](int j8, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (!HELD) {
+      if (8 * j8 + 8 <= done) {
+        const uint4* u = reinterpret_cast<const uint4*>(src + 8 * j8);
+        const uint4 g = __ldg(u);
+        if constexpr (sizeof(T) == 4) {
+          const uint4 q = __ldg(u + 1);
+          v[0] = __uint_as_float(g.x); v[1] = __uint_as_float(g.y);
+          v[2] = __uint_as_float(g.z); v[3] = __uint_as_float(g.w);
+          v[4] = __uint_as_float(q.x); v[5] = __uint_as_float(q.y);
+          v[6] = __uint_as_float(q.z); v[7] = __uint_as_float(q.w);
+        } else {
+          unpack8<T>(g, v);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 8 * j8 + i < n ? to_f32(src[8 * j8 + i]) : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = fmaxf(v[i], -INFINITY);          // (a NaN's place)
+    } else if constexpr (sizeof(T) == 4) {
       const float4 u = reinterpret_cast<const float4*>(xs)[2 * j8], g = reinterpret_cast<const float4*>(xs)[2 * j8 + 1];
       v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
       v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
@@ -398,7 +424,7 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   auto floor_of = [&](int bin) {
     if (bin >= BINS - 1 || !(fabsf(top) <= 3.4028235e38f)) return -3.4028235e38f;
     const float wide = (bin + 1) * (0.0625f * ts);
-    return top - wide - (fabsf(top) + wide) * 1e-6f;
+    return fmaxf(top - wide - (fabsf(top) + wide) * 1e-6f, -3.4028235e38f);   // (-inf is no value: it fills)
   };
   // lists the values from `least` on
   auto list = [&](const float (&v)[8], int j, float least) {
@@ -418,7 +444,7 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   // f(value, index) for what is listed, or for every value where the list did not hold it
   auto visit = [&](auto f) {
     if (listing) {
-      for (int i = tid; i < (int)s.listed; i += CT) f(to_f32(xs[s.list[i]]), (int)s.list[i]);
+      for (int i = tid; i < (int)s.listed; i += CT) f(to_f32(HELD ? xs[s.list[i]] : src[s.list[i]]), (int)s.list[i]);
     } else {
       each([&](const float (&v)[8], int j) {
 #pragma unroll
@@ -516,7 +542,7 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     int from = 0;
     for (int q = 0; q < ranks; ++q) {
       const Shared* other = cl.map_shared_rank(&s, q);
-      const T* values = cl.map_shared_rank(xs, q);
+      const T* values = HELD ? cl.map_shared_rank(xs, q) : l + q * chunk;
       const int count = (int)other->listed;
       for (int i = tid; i < count; i += CT) {
         const int j = other->list[i];
@@ -776,34 +802,23 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   cl.sync();
 }
 
-constexpr int CHUNK_MAX = 128 * 1024;   // bytes of a row in a CTA: at most 65536 values (one an SM beyond 80 KB)
+constexpr int HELD_MAX = 80 * 1024;     // bytes of a row in a CTA: two CTAs share an SM
 
-template <typename T>
-int run(const SampleArgs& a, cudaStream_t st) {
-  auto chunk_of = [&](int c) { return ((a.v + c - 1) / c + 7) / 8 * 8; };
-  // CTAs per row: as few as two CTAs an SM hold it with, more (of 2048 values at least) while
-  // the rows alone leave the device empty
-  int c = 1;
-  while (c < 16 && (size_t)chunk_of(c) * sizeof(T) > 80 * 1024) c *= 2;
-  while (c < 8 && (long long)a.b * c * 2 <= 296 && chunk_of(2 * c) >= 2048) c *= 2;
-  const size_t bytes = (size_t)chunk_of(c) * sizeof(T);
-  if (bytes > CHUNK_MAX || (long long)a.b * c > 0x7fffffffLL) {
-    sample_rows<T><<<a.b, NT, 0, st>>>(a);
-    return check_launch("sample");
-  }
-  auto kern = sample_cluster<T>;
+template <typename T, bool HELD>
+int launch(const SampleArgs& a, int c, int chunk, cudaStream_t st) {
+  auto kern = sample_cluster<T, HELD>;
   static std::atomic<uint64_t> ready{0};      // devices whose limits are raised
   int dev = 0;
   VERACE_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_MAX));
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD ? HELD_MAX : 0));
     VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.b * c));
   cfg.blockDim = dim3(CT);
-  cfg.dynamicSmemBytes = bytes;
+  cfg.dynamicSmemBytes = HELD ? (size_t)chunk * sizeof(T) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -811,8 +826,33 @@ int run(const SampleArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, a, chunk_of(c)));
+  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, a, chunk));
   return check_launch("sample");
+}
+
+template <typename T>
+int run(const SampleArgs& a, cudaStream_t st) {
+  auto chunk_of = [&](int c) { return ((a.v + c - 1) / c + 7) / 8 * 8; };
+  // CTAs per row: as few as hold it, more (of 2048 values at least) while the rows alone leave
+  // the device empty
+  auto split = [&](int most) {
+    int c = 1;
+    while (c < 16 && chunk_of(c) > most) c *= 2;
+    while (c < 8 && (long long)a.b * c * 2 <= 296 && chunk_of(2 * c) >= 2048) c *= 2;
+    return c;
+  };
+  const int c = split(HELD_MAX / sizeof(T)), free = split(65536);
+  if (chunk_of(free) > 65536 || (long long)a.b * c > 0x7fffffffLL) {
+    sample_rows<T><<<a.b, NT, 0, st>>>(a);
+    return check_launch("sample");
+  }
+  // Held rows take less time for a pass (64 bf16 rows of 163840, 4 CTAs a row either way: 23.1 us
+  // with k and p against 25.2), but large ones more CTAs, which may be more waves (64 fp32 rows of
+  // 163840: 49.9 against 30.2; 256 fp32 rows of 32000: 38.5 against 23.8).
+  auto waves = [&](int c) { return ((long long)a.b * c + 295) / 296; };
+  if (chunk_of(c) * (int)sizeof(T) > HELD_MAX || waves(free) < waves(c))
+    return launch<T, false>(a, free, chunk_of(free), st);
+  return launch<T, true>(a, c, chunk_of(c), st);
 }
 
 }  // namespace
