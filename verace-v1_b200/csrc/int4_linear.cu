@@ -33,6 +33,11 @@
 // a warp 33 clocks to issue), 600 to 1000 a chunk; a chunk's weights take 712 clocks of an SM's
 // share of the memory rate, and two lines have twice that.  Few row tiles: k is split over a
 // cluster and the partial sums are joined through distributed shared memory in rank order.
+//
+// Measured on the device (copies run at 6.55 TB/s): 1 x 163840 x 1024 bf16 21.8 us, 4.0 TB/s;
+// 16 x 65536 x 16384 123 us, 4.5 TB/s (512 tiles over 148 CTAs: 3.46 rounds take the time of 4, which
+// alone is 98 us); 64 x 16384 x 4096 20.5 us, 420 TFLOP/s, 3 us of it the staging of x; 7 x 4096 x
+// 8192 fp16 11.5 us and 1 x 3080 x 1024 6.8 us, of which set-up and joins are 5.
 #include "common.cuh"
 #include "tc.cuh"
 #include "tmap.cuh"
