@@ -17,8 +17,9 @@
 //
 // Bound: one read of the row, and of the noise where every value draws.  Measured on the device: one
 // row of 32000 at T = 0 6.1 us (launch and cluster barriers); 64 fp32 rows of 163840 with k = 50,
-// p = 0.9 and min_p 30 us for 42 MB (1.4 TB/s: two passes, the second from L2, then about ten steps
-// between barriers of the cluster; one CTA a row that read it again for every step: 1924); 256 bf16 rows of
+// p = 0.9 and min_p 26 us for 42 MB (1.6 TB/s: two passes, the second from L2, then about eight steps
+// between barriers of the cluster; one CTA a row that read it again for every step: 1924), with p alone
+// 54; 256 bf16 rows of
 // 32000 without cuts 25 us for 49 MB with the noise (2.0 TB/s: the arithmetic per value).
 #include "common.cuh"
 
@@ -231,6 +232,12 @@ __device__ __forceinline__ void add_to(Hist& h, int b, bool by_mass, float part)
   }
 }
 
+// The mass that a cut by p leaves, of a total.
+__device__ __forceinline__ unsigned long long target_of(float p, double total) {
+  const double target = ceil((double)p * total);
+  return target > 1. ? (unsigned long long)target : 1ull;
+}
+
 // The cluster's histogram h: the first bin at which the running count (or mass) reaches `left`,
 // the last one if none does.  Thread i has bin i.  Masses are in
 // units of exp(-bin / 16) (`first`) or of `weight`.  Sets s.bin, s.found and s.left.
@@ -268,8 +275,7 @@ __device__ void find_bin(cg::cluster_group& cl, Shared& s, int h, bool by_mass, 
   run += before;
   if (by_mass && first) {
     // a token is kept while the mass strictly above it is below p * total
-    left = (unsigned long long)ceil((double)p * (double)total);
-    if (left < 1) left = 1;
+    left = target_of(p, (double)total);
     if (tid == 0) s.target = left;
   }
   if ((run >= left && run - mine < left) || (tid == BINS - 1 && run < left)) {
@@ -515,9 +521,10 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   if (bounded || by_least) listing = s.listed <= LIST;
   if (cuts) cl.sync();
 
-  // A short list, as it mostly is, goes to the first CTA, which compares every value with every
-  // other: kept are those with fewer than k greater ones, and then with less mass above them than
-  // the target.  (No more levels and barriers over the cluster.)
+  // A short list, as it mostly is, goes to the first CTA, which sorts it: the cut by k is the value
+  // at that place, the cut by p the one at which the running mass reaches the target.  (No more
+  // levels and barriers over the cluster.  Comparing every value with every other instead took 60 k
+  // clocks for a list of 1000.)
   const float shift = top * inv;
   const bool direct = fabsf(top / ts) <= 3.4028235e38f;
   // the score: l / T - log(noise) where that is in range, z - log(noise) where it is not
@@ -527,90 +534,76 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     return ((unsigned long long)key_of(score + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
   };
   auto gather = [&] {
-    uint32_t total = 0;
     const int ranks = cl.num_blocks();
-#pragma unroll 8
-    for (int i = 0; i < ranks; ++i) total += min(*cl.map_shared_rank(&s.listed, i), (uint32_t)(GATHER + 1));
-    if (total > GATHER) return false;
+    int total = 0;
+    for (int q = 0; q < ranks; ++q) total += (int)min(*cl.map_shared_rank(&s.listed, q), (uint32_t)(GATHER + 1));
+    if (total < 1 || total > GATHER) return false;
     if (rank > 0) return true;
-    // (the histograms are read no more; the masses go where this CTA's list was)
+    // (the histograms are read no more; the sorted keys go where this CTA's list was)
     float* gx = reinterpret_cast<float*>(s.hist);
     int* gi = reinterpret_cast<int*>(gx + GATHER);
-    unsigned long long* gw = reinterpret_cast<unsigned long long*>(s.list);
-    static_assert(sizeof(s.hist) >= GATHER * 8 && sizeof(s.list) >= GATHER * 8 && offsetof(Shared, list) % 8 == 0,
+    uint32_t* gk = reinterpret_cast<uint32_t*>(s.list);
+    static_assert(sizeof(s.hist) >= GATHER * 8 && sizeof(s.list) >= GATHER * 4 && offsetof(Shared, list) % 4 == 0,
                   "gathered values fit");
-    int from = 0;
-    for (int q = 0; q < ranks; ++q) {
-      const Shared* other = cl.map_shared_rank(&s, q);
-      const T* values = HELD ? cl.map_shared_rank(xs, q) : l + q * chunk;
-      const int count = (int)other->listed;
-      for (int i = tid; i < count; i += CT) {
-        const int j = other->list[i];
-        gx[from + i] = to_f32(values[j]);
-        gi[from + i] = q * chunk + j;
-      }
-      from += count;
+    for (int e = tid; e < total; e += CT) {
+      int q = 0, i = e;                          // which CTA's, and its place there
+      for (int c = (int)*cl.map_shared_rank(&s.listed, 0); i >= c; c = (int)*cl.map_shared_rank(&s.listed, q)) i -= c, ++q;
+      const int at = cl.map_shared_rank(&s, q)->list[i];
+      gx[e] = to_f32(HELD ? cl.map_shared_rank(xs, q)[at] : l[q * chunk + at]);
+      gi[e] = q * chunk + at;
     }
     __syncthreads();
-    constexpr int EACH = GATHER / CT;
-    float x[EACH];
-    bool in[EACH];
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int i = tid + e * CT;
-      in[e] = i < (int)total;
-      x[e] = in[e] ? gx[i] : -INFINITY;
-    }
-    if (cut_k) {
-      int greater[EACH] = {};
-      for (int j = 0; j < (int)total; ++j) {
-        const float y = gx[j];
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) greater[e] += y > x[e];
-      }
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) in[e] = in[e] && greater[e] < k;
-    }
-    if (cut_p) {
-      unsigned long long sum = 0;
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        const unsigned long long w =
-            in[e] ? (unsigned long long)(expf(-(below(x[e]) / ts)) * 1099511627776.f + 0.5f) : 0ull;
-        if (tid + e * CT < (int)total) gw[tid + e * CT] = w;
-        sum += w;
-      }
-      unsigned long long target = s.target;
-      if (cut_k) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s.red64[tid / 32] = sum;
+    int size = 2;
+    while (size < total) size *= 2;
+    for (int e = tid; e < size; e += CT) gk[e] = e < total ? key_of(gx[e] + 0.f) : 0u;
+    // bitonic, descending
+    for (int run = 2; run <= size; run *= 2) {
+      for (int apart = run / 2; apart > 0; apart /= 2) {
         __syncthreads();
-        sum = 0;
-#pragma unroll
-        for (int i = 0; i < CT / 32; ++i) sum += s.red64[i];
-        target = (unsigned long long)ceil((double)p * (double)sum);
-        if (target < 1) target = 1;
+        if (tid < size / 2) {
+          const int i = 2 * tid - (tid & (apart - 1)), j = i + apart;
+          const uint32_t u = gk[i], v = gk[j];
+          if ((u < v) == ((i & run) == 0)) gk[i] = v, gk[j] = u;
+        }
       }
-      __syncthreads();
-      unsigned long long above[EACH] = {};
-      for (int j = 0; j < (int)total; ++j) {
-        const float y = gx[j];
-        const unsigned long long w = gw[j];
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) above[e] += y > x[e] ? w : 0ull;
-      }
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) in[e] = in[e] && above[e] < target;
     }
+    __syncthreads();
+    uint32_t cut = cut_k ? gk[min(k, total) - 1] : 1u;
+    if (cut_p) {
+      static_assert(GATHER == 2 * CT, "two places a thread");
+      unsigned long long w[2], sum;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      if (!in[e]) continue;
-      const float d = below(x[e]);
-      if (minp > 0.f && d != 0.f && !(-d * inv >= log_minp)) continue;
-      const int i = gi[tid + e * CT];
-      const float score = score_of(x[e], __ldg(noise + i));        // (the first CTA's noise is the row's)
-      if (score > -INFINITY) choice = max(choice, pack(score, i));
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t q = 2 * tid + e < size ? gk[2 * tid + e] : 0u;
+        const float x = __uint_as_float(q ^ (q >> 31 ? 0x80000000u : 0xffffffffu));
+        w[e] = q && q >= cut ? (unsigned long long)(expf(-(below(x) / ts)) * 1099511627776.f + 0.5f) : 0ull;
+      }
+      sum = w[0] + w[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (lane == 31) s.red64[tid / 32] = sum;
+      if (tid == 0) s.found = cut;
+      __syncthreads();
+      unsigned long long all = 0;
+      for (int i = 0; i < CT / 32; ++i) {
+        sum += i < tid / 32 ? s.red64[i] : 0;
+        all += s.red64[i];
+      }
+      const unsigned long long target = cut_k ? target_of(p, (double)all) : s.target;
+      // (at one place only)
+      if (sum >= target && sum - w[1] < target) s.found = gk[2 * tid + 1];
+      if (sum - w[1] >= target && sum - w[1] - w[0] < target) s.found = gk[2 * tid];
+      __syncthreads();
+      cut = s.found;
+    }
+    for (int e = tid; e < total; e += CT) {
+      const float x = gx[e], d = below(x);
+      if (key_of(x + 0.f) < cut || (minp > 0.f && d != 0.f && !(-d * inv >= log_minp))) continue;
+      const float score = score_of(x, __ldg(noise + gi[e]));       // (the first CTA's noise is the row's)
+      if (score > -INFINITY) choice = max(choice, pack(score, gi[e]));
     }
     return true;
   };
