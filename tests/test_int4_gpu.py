@@ -68,6 +68,19 @@ def test_matches_formula(m, n, k, group, dtype):
         assert torch.equal(y, V.int4_linear(xd, qd, sd, zd, bd, group_size=group)), "two calls differ"
 
 
+@pytest.mark.parametrize("m,dtype", [(9, torch.bfloat16), (130, torch.float16), (20, torch.float32)])
+def test_last_round_shares_its_inputs(m, dtype):
+    """More row tiles than CTAs and few in the last round, with a long k."""
+    n, k, group = 19400, 7200, 32 if m == 20 else 128
+    x, q, s, z, b = make(m, n, k, group, dtype, True, True, seed=m)
+    x[1, 7000], x[m - 1, 3] = 60000.0, -9000.0                     # far above the rest of their groups
+    rows = torch.cat([torch.arange(0, n - 1600, 97), torch.arange(n - 1600, n)])
+    ref, size = reference(x, q[rows], s[:, rows], z[:, rows], b[rows], group)
+    y = V.int4_linear(*on_gpu(x, q, s, z, b), group_size=group, out_dtype=torch.float32)
+    assert torch.isfinite(y).all()
+    check(y[:, rows.cuda()], ref, size, k, torch.float32)
+
+
 @pytest.mark.parametrize("m", [1, 6, 40])
 def test_many_output_rows_and_long_inputs(m):
     """More rows than a wave of CTAs, and a long k for few rows (the split over k)."""

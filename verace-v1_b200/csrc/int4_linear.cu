@@ -35,8 +35,7 @@
 // cluster and the partial sums are joined through distributed shared memory in rank order.
 //
 // Measured on the device (copies run at 6.55 TB/s): 1 x 163840 x 1024 bf16 21.8 us, 4.0 TB/s;
-// 16 x 65536 x 16384 123 us, 4.5 TB/s (512 tiles over 148 CTAs: 3.46 rounds take the time of 4, which
-// alone is 98 us); 64 x 16384 x 4096 20.5 us, 420 TFLOP/s, 3 us of it the staging of x; 7 x 4096 x
+// 16 x 65536 x 16384 116 to 119 us, 4.7 TB/s (512 tiles over 148 CTAs: three rounds and half a one); 64 x 16384 x 4096 20.5 us, 420 TFLOP/s, 3 us of it the staging of x; 7 x 4096 x
 // 8192 fp16 11.5 us and 1 x 3080 x 1024 6.8 us, of which set-up and joins are 5.
 #include "common.cuh"
 #include "tc.cuh"
@@ -89,7 +88,10 @@ struct Shape {
   static_assert(NA * A_COLS <= D_COL, "TMEM");
   // bytes of a chunk's B operands: the passes' [256 / 16][N][16], then per group the zeros' [2][N][16]
   static constexpr int BLK = PASSES * KC * N + GPC * 32 * N;
-  static constexpr int SW = BLK > 44 * 1024 ? 4 : 6;                             // weight stages (even)
+  // weight stages (even): fewer where x's blocks are large and want the room (64 fp32 tokens of 16384 x
+  // 4096, blocks of 25.6 KB: 44.7 us with 6, 42.0 with 4; 5 of 32001 x 1056 in groups of 32, 24 KB:
+  // 17.9 and 19.6)
+  static constexpr int SW = BLK > 24 * 1024 ? 4 : 6;
   static constexpr int B_SMEM = SMEM - SW * W_STAGE - PART;                      // bytes for x
   static_assert(B_SMEM >= 2 * BLK, "x is at least double-buffered");
 };
@@ -105,6 +107,7 @@ struct Int4Args {
   long long m;
   int n, k, out_f32;
   int tiles, ytiles;   // row tiles and token tiles
+  int first, last;     // the launch's units (a row tile of a token tile)
   int ck, per;         // CTAs that share a tile, each with `per` chunks of k
   int staged;          // x comes from the workspace (else every CTA stages its own)
   int sb;              // chunks of x in shared memory
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
   const int rank = a.ck > 1 ? blockIdx.x % a.ck : 0;
   const int chunks = (a.k + KC - 1) / KC;
   const int c0 = min(rank * a.per, chunks), nc = min(a.per, chunks - c0);
-  const int unit0 = blockIdx.x / a.ck, units = a.tiles * a.ytiles, step = gridDim.x / a.ck;
+  const int unit0 = a.first + blockIdx.x / a.ck, units = a.last, step = gridDim.x / a.ck;
   const int span = ((a.staged ? chunks : a.per) * GPC + 31) / 32;     // groups per bit of a left-out mask
 
   if (w == 1) tc::tmem_alloc(&s_slot, 512);
@@ -888,6 +891,7 @@ int sm_count() {
 // Sizes of a call; the same for the workspace query and the launch.
 struct Plan {
   int tiles, ytiles, ck, per, staged, sb, resident;
+  int rest, rest_ck;   // units of a last round, in a launch of their own
   size_t ws_blocks, ws_total;
 };
 
@@ -902,10 +906,18 @@ Plan plan(long long m, int n, int k) {
   while (p.ck < 8 && units * p.ck * 2 <= 148 && chunks >= p.ck * 2) p.ck *= 2;
   p.per = (chunks + p.ck - 1) / p.ck;
   const bool fits = (long long)p.per * S::BLK <= S::B_SMEM && p.per <= MAX_SB;
-  // every CTA stages x itself while that is at most five chunks for each of the eight warps that do it
+  // Every CTA stages x itself while that is at most five chunks for each of the eight warps that do it.
+  // (There a kernel of its own is 2 us less on the device, 10.6 against 12.5 for 2 x 16384 x 4096, but
+  // its launch takes the host 3 to 4; at 56 chunks, 7 x 4096 x 8192, 11.3 against 16.0.)
   p.staged = !(fits && p.ytiles == 1 && m * p.per <= 40);
   p.resident = fits && p.ytiles == 1;
   p.sb = p.resident ? (p.per > 0 ? p.per : 1) : (S::B_SMEM / S::BLK < 8 ? S::B_SMEM / S::BLK / 2 * 2 : 8);   // (even)
+  // A last round that leaves half of the CTAs idle shares its tiles' k instead, where that saves more
+  // than the second launch costs (16 x 20480 x 16384 fp16, 160 tiles: 94 -> 67 us; 16 x 65536 x 16384, 512
+  // tiles: 120 -> 116).
+  p.rest = units > 148 ? (int)(units % 148) : 0;
+  for (p.rest_ck = 1; p.rest > 0 && p.rest_ck < 8 && p.rest * p.rest_ck * 2 <= 148;) p.rest_ck *= 2;
+  if (!p.staged || p.resident || chunks - chunks / p.rest_ck < 24) p.rest = 0;
   p.ws_blocks = align_up((size_t)p.ytiles * chunks * S::BLK, 256);
   p.ws_total = p.staged ? p.ws_blocks + align_up((size_t)p.ytiles * S::MP * 8, 256) + 256 : 0;
   return p;
@@ -957,29 +969,38 @@ int launch(Int4Args a, void* workspace, size_t ws_bytes, cudaStream_t st) {
     VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  cudaLaunchConfig_t cfg = {};
+  const int sms = sm_count();
+  auto go = [&](int first, int last, int ck, bool dependent) -> int {
+    const int units = last - first;
+    a.first = first, a.last = last;
+    a.ck = ck, a.per = (chunks + ck - 1) / ck;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ck > 1 ? units * ck : units < sms ? units : sms));
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (ck > 1) {
+      attr[na].id = cudaLaunchAttributeClusterDimension;
+      attr[na].val.clusterDim.x = ck;
+      attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+      ++na;
+    }
+    if (dependent) {
+      attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[na].val.programmaticStreamSerializationAllowed = 1;
+      ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, map, a));
+    return check_launch("int4_linear");
+  };
   const int units = p.tiles * p.ytiles;
-  cfg.gridDim = dim3((unsigned)(p.ck > 1 ? units * p.ck : units < sm_count() ? units : sm_count()));
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  int na = 0;
-  if (p.ck > 1) {
-    attr[na].id = cudaLaunchAttributeClusterDimension;
-    attr[na].val.clusterDim.x = p.ck;
-    attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
-    ++na;
-  }
-  if (p.staged) {
-    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[na].val.programmaticStreamSerializationAllowed = 1;
-    ++na;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = na;
-  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, map, a));
-  return check_launch("int4_linear");
+  if (p.rest == 0) return go(0, units, p.ck, p.staged);
+  const int rc = go(0, units - p.rest, 1, p.staged);
+  return rc ? rc : go(units - p.rest, units, p.rest_ck, false);
 }
 
 // Calls f with a problem's type and shape.
