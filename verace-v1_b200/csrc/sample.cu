@@ -839,9 +839,9 @@ int run(const SampleArgs& a, cudaStream_t st) {
     sample_rows<T><<<a.b, NT, 0, st>>>(a);
     return check_launch("sample");
   }
-  // Held rows take less time for a pass (64 bf16 rows of 163840, 4 CTAs a row either way: 23.1 us
-  // with k and p against 25.2), but large ones more CTAs, which may be more waves (64 fp32 rows of
-  // 163840: 49.9 against 30.2; 256 fp32 rows of 32000: 38.5 against 23.8).
+  // Held rows take less time for a pass (64 bf16 rows of 163840, 4 CTAs a row either way: 19.9 us
+  // with k and p against 20.9), but large ones more CTAs, which may be more waves (64 fp32 rows of
+  // 163840: 41.7 against 26.0; 256 fp32 rows of 32000: 32.0 against 20.5).
   auto waves = [&](int c) { return ((long long)a.b * c + 295) / 296; };
   if (chunk_of(c) * (int)sizeof(T) > HELD_MAX || waves(free) < waves(c))
     return launch<T, false>(a, free, chunk_of(free), st);
