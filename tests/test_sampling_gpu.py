@@ -440,6 +440,34 @@ def test_sample_cuts_among_many_equal_values(dtype):
         check_sample(l, noise, t, k, p, minp, most_clear=False)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b", [1, 64])
+def test_sample_rows_crowded_at_one_end(b, dtype):
+    """Rows whose kept tokens lie in one CTA's part, by more than it lists, and not in the others'."""
+    v = 163840
+    l, noise = draw(b, v, 31 + b, dtype=dtype)
+    block = torch.full((b, v), -INF, dtype=dtype)                # a block of tokens allowed, all equal
+    for lo in (0, 60000, v - 20000):
+        block.fill_(-INF)
+        block[:, lo:lo + 20000] = 0.0
+        check_sample(block, noise, 1.0, 50, 1.0, 0.0)
+        block[:, lo:lo + 20000] = l[:, lo:lo + 20000]            # and not equal
+        check_sample(block, noise, 1.0, 1000, 0.9, 0.0)
+    ties = l.clone()
+    ties[:, :10000] = 14.0                                       # equal ones at the top, in front of the rest
+    check_sample(ties, noise, 1.0, 50, 1.0, 0.0)
+    check_sample(ties, noise, 1.0, 50, 0.9, 0.0)
+    ties[:, :v // 2] = 14.0
+    check_sample(ties, noise, 1.0, 1000, 1.0, 0.01)
+    check_sample(ties, noise, 1.0, 0, 0.3, 0.0)
+    padded = (0.1 * l.float()).to(dtype)                         # nearly flat, the vocabulary's end padded
+    padded[:, 150000:] = -INF
+    check_sample(padded, noise, 20.0, 50, 1.0, 0.0)
+    check_sample(padded, noise, 20.0, 50, 0.8, 0.01)
+    check_sample(l, noise, 1.0, 32000, 0.95, 0.0)                # lists of about what a CTA holds
+    check_sample(l, noise, 1.0, 32000, 1.0, 0.0)
+
+
 def test_sample_strides_and_streams():
     l, noise = draw(5, 777, 8, 0.1)
     lw, nw = torch.zeros(5, 800, device="cuda"), torch.ones(5, 779, device="cuda")

@@ -618,6 +618,9 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
 
   // ---- the cuts: what is kept is every value in a bin before `edge`, and in it the keys from
   // `least` on
+  // (`listing` is each CTA's own: one CTA's list may overflow where another's holds, as for a row whose
+  // ties or unmasked tokens all lie in one part.  So no barrier over the cluster and no gather may
+  // depend on it; every other condition here is the same for all of a cluster's CTAs.)
   for (int by_mass = 0; by_mass < 2 && !chosen; ++by_mass) {
     if (by_mass ? !cut_p : !cut_k) continue;
     const int kept_edge = edge;
@@ -650,12 +653,13 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
       __syncthreads();
       const float from = floor_of(cut);
       each([&](const float (&v)[8], int j) { list(v, j, from); });
-      cl.sync();
+      __syncthreads();
       listing = s.listed <= LIST;
-      if (by_mass && !cut_k) {
-        chosen = gather();
-        if (chosen) break;
-      }
+    }
+    if (by_mass && !cut_k) {           // (nothing was listed before: every CTA has just done it)
+      cl.sync();
+      chosen = gather();
+      if (chosen) break;
     }
     if (more) {
       // the keys that bin `cut` can hold (its bounds, widened by the roundings of place)
