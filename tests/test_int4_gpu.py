@@ -91,6 +91,21 @@ def test_many_output_rows_and_long_inputs(m):
         check(y, ref, size, k, torch.float32)
 
 
+@pytest.mark.parametrize("dtype,m", [(torch.bfloat16, 1), (torch.bfloat16, 7), (torch.bfloat16, 32), (torch.float16, 2),
+                                     (torch.float16, 16), (torch.float32, 1), (torch.float32, 5), (torch.float32, 40)])
+@pytest.mark.parametrize("n,k,group", [(300, 1024, 128), (9700, 512, 64), (130, 4096, 32)])
+def test_inputs_of_weight_zero_add_nothing(n, k, group, dtype, m):
+    """Codes equal to their zeros.  (Eight inputs a group: sums below 15 x 8 x 2^8 of the pieces, whose steps are
+    2^-9, are exact.)"""
+    x, q, s, z, b = make(m, n, k, group, dtype, True, False, seed=m + n + k)
+    x[:, torch.arange(k) % group % (group // 8) != 1] = 0
+    q[::2] = (z * 17).t().repeat_interleave(group // 2, 1)[::2]
+    ref, size = reference(x, q, s, z, None, group)
+    y = V.int4_linear(*on_gpu(x, q, s, z), group_size=group, out_dtype=torch.float32)
+    assert (y[:, ::2] == 0).all()
+    check(y, ref, size, k, torch.float32)
+
+
 def test_strides_shapes_and_streams():
     x, q, s, z, b = make(6, 96, 256, 64, torch.bfloat16, True, True, 1)
     ref, size = reference(x, q, s, z, b, 64)

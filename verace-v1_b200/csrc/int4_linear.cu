@@ -16,8 +16,8 @@
 //     MMA after the other into the same columns.
 // Each token is scaled by a power of two, its largest input to [2^7, 2^8); inputs 2^-22 of that
 // and smaller lose digits.  tcgen05.mma adds fp8 products in full fp32 (measured: 2^23 + 1 is
-// exact).  The zeros are one more MMA per group: 32 inputs that hold X = sum of the group's
-// scaled x in 6 e5m2 pieces, against -z.  So D = 2^-9 (sum q x - z X) per group, and a row's
+// exact).  The zeros are one more MMA per group: 32 inputs that hold X = the sum of a column's pieces
+// over the group, in 6 e5m2 pieces, against -z.  So D = 2^-9 (sum q x - z X) per group, and a row's
 // thread adds s D in fp32.  No weight and no input is rounded.
 // What q x and z X lose by cancelling is 2^-24 of the group's largest input.  Where at most a
 // sixteenth of a group is 2^12 above all the rest, that could show in the outputs whose q = z
@@ -180,15 +180,15 @@ __device__ __forceinline__ int shift_of(float top) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Writes the pieces of a lane's eight inputs of a chunk (token row t of the tile; a warp holds the
-// chunk) and, from a group's first lane, X.  A word's codes 0, 2, 4, 6 unpack before 1, 3, 5, 7, and so do x's bytes.
+// chunk) and, from a group's first lanes, X.  A word's codes 0, 2, 4, 6 unpack before 1, 3, 5, 7, and so do x's bytes.
 template <typename T, typename S>
 __device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* block, int t, int lane) {
-  constexpr int LANES = 32 / S::GPC;
-  float sum = 0.f;
+  constexpr int LANES = 32 / S::GPC, NX = S::COLS ? S::P : 1;     // NX: the X of a group
+  float sum[NX];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= scale, sum += v[i];
+  for (int p = 0; p < NX; ++p) sum[p] = 0.f;
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int i = 0; i < 8; ++i) v[i] *= scale;
   constexpr int at[4][2] = {{0, 2}, {4, 6}, {1, 3}, {5, 7}};
   uint8_t* d = block + ((lane / 2) * S::N + t) * 16 + (lane % 2) * 8;
   auto put = [&](int p, const uint32_t (&b)[4]) {
@@ -204,6 +204,7 @@ __device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* bloc
         b[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[at[i][0]], v[at[i][1]]), __NV_SATFINITE, __NV_E4M3);
         const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b[i], __NV_E4M3);
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        sum[p] += f.x + f.y;
         v[at[i][0]] = (v[at[i][0]] - f.x) * 32.f;
         v[at[i][1]] = (v[at[i][1]] - f.y) * 32.f;
       }
@@ -228,27 +229,39 @@ __device__ __forceinline__ void stage8(float (&v)[8], float scale, uint8_t* bloc
           b[i] = __nv_cvt_halfraw2_to_fp8x2(hr, __NV_SATFINITE, __NV_E5M2);
           r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b[i], __NV_E5M2);
         }
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        sum[S::COLS ? p : 0] += f.x + f.y;
         h[i] = __hsub2(h[i], *reinterpret_cast<const __half2*>(&r));
         if (S::COLS) h[i] = __hmul2(h[i], __float2half2_rn(32.f));
       }
       put(p, b);
     }
   }
-  if (lane % LANES == 0) {
-    uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int p = 0; p < 6; ++p) {
-      const uint32_t b = __nv_cvt_float_to_fp8(sum, __NV_SATFINITE, __NV_E5M2);
-      w[p / 4] |= b << (8 * (p % 4));
-      const __half_raw r = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E5M2);
-      sum -= __half2float(*reinterpret_cast<const __half*>(&r));
-    }
-    uint4* z = reinterpret_cast<uint4*>(block + S::PASSES * KC * S::N + (lane / LANES) * 32 * S::N) + t;
-    z[0] = make_uint4(w[0], w[1], 0, 0);
-    z[S::N] = make_uint4(0, 0, 0, 0);
-    if constexpr (S::COLS) {
+  for (int p = 0; p < NX; ++p)
 #pragma unroll
-      for (int p = 1; p < S::P; ++p) z[p * S::MP] = z[S::N + p * S::MP] = make_uint4(0, 0, 0, 0);
+    for (int o = LANES / 2; o > 0; o >>= 1) sum[p] += __shfl_xor_sync(0xffffffffu, sum[p], o);
+  // X of each column in e5m2 pieces, 4 bits each: 24, which hold a column's sum whole (of multiples of
+  // 2^-9 below 2^15), so that code = zero adds nothing
+  uint4* z = reinterpret_cast<uint4*>(block + S::PASSES * KC * S::N + (lane / LANES) * 32 * S::N) + t;
+#pragma unroll
+  for (int p0 = 0; p0 < NX; p0 += LANES) {          // a lane per column
+    float x = sum[p0];
+#pragma unroll
+    for (int p = p0 + 1; p < NX && p < p0 + LANES; ++p)
+      if (lane % LANES == p - p0) x = sum[p];
+    const int p = p0 + lane % LANES;
+    if (p < NX) {
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        const uint32_t b = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E5M2);
+        w[i / 4] |= b << (8 * (i % 4));
+        const __half_raw r = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E5M2);
+        x -= __half2float(*reinterpret_cast<const __half*>(&r));
+      }
+      z[p * S::MP] = make_uint4(w[0], w[1], 0, 0);
+      z[S::N + p * S::MP] = make_uint4(0, 0, 0, 0);
     }
   }
 }
