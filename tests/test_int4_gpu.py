@@ -106,6 +106,28 @@ def test_inputs_of_weight_zero_add_nothing(n, k, group, dtype, m):
     check(y, ref, size, k, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k,group", [(1, 9700, 2304, 32), (3, 200, 16384, 128), (20, 300, 16384, 128), (20, 9700, 16384, 64),
+                                         (40, 300, 16384, 64), (64, 200, 16384, 32)])
+def test_sparse_inputs_count_once(m, n, k, group, dtype):
+    """Few inputs that are not 0: in each group a large one and a small one, within eight inputs throughout
+    every third run of 256, in the next eight throughout another third."""
+    x, q, s, z, b = make(m, n, k, group, dtype, True, False, seed=m + n + k)
+    x.zero_()
+    for i in range(k // group):
+        lo, run = i * group, i * group // 256
+        if run % 3 < 2:
+            x[:, lo + i % 8] = 1.0 + i % 5
+            x[:, lo + (i + 1) % 8 + 8 * (run % 3)] = 1e-4
+    if m > 2:
+        x[1] = 0                                                   # a token of zeros beside the others
+        x[2, group:] = 0
+    rows = torch.arange(0, n, max(1, n // 200))
+    ref, size = reference(x, q[rows], s[:, rows], z[:, rows], None, group)
+    y = V.int4_linear(*on_gpu(x, q, s, z), group_size=group, out_dtype=torch.float32)
+    check(y[:, rows.cuda()], ref, size, k, torch.float32)
+
+
 def test_strides_shapes_and_streams():
     x, q, s, z, b = make(6, 96, 256, 64, torch.bfloat16, True, True, 1)
     ref, size = reference(x, q, s, z, b, 64)

@@ -148,14 +148,15 @@ __device__ __forceinline__ float leave_out(float (&v)[8], bool& out) {
   float top = mine;
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // a lane whose inputs are all far below the largest: perhaps that one stands alone
-  if (__any_sync(0xffffffffu, mine > 0.f && mine < top * APART)) {
-    int high = 0, low = 0;
+  // any input far below the largest: perhaps that one stands alone.  (left_out decides by the same rule,
+  // for every group that shares a bit of the mask: what this leaves in it must not add again.)
+  int low = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      high += fabsf(v[i]) >= top * APART;
-      low |= fabsf(v[i]) < top * APART && v[i] != 0.f;
-    }
+  for (int i = 0; i < 8; ++i) low |= fabsf(v[i]) < top * APART && v[i] != 0.f;
+  if (__any_sync(0xffffffffu, low)) {
+    int high = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) high += fabsf(v[i]) >= top * APART;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
       high += __shfl_xor_sync(0xffffffffu, high, o);
