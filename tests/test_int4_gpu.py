@@ -128,6 +128,28 @@ def test_sparse_inputs_count_once(m, n, k, group, dtype):
     check(y[:, rows.cuda()], ref, size, k, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k,group", [(1, 300, 1024, 128), (9, 200, 4096, 64), (40, 130, 2048, 32)])
+def test_inputs_at_the_ends_of_the_range(m, n, k, group, dtype):
+    """Tokens near the largest and the smallest numbers of the type.  (Below the smallest normal number a
+    product or a sum is off by half of 2^-149 more.)"""
+    for e in (126, 119, 101, 98, -93, -110, -126, -130):
+        x, q, s, z, b = make(m, n, k, group, dtype, True, False, seed=m + n + e)
+        x = (x.double() * 2.0 ** e).clamp(-3.3e38, 3.3e38).to(dtype)
+        ref, size = reference(x, q, s, z, None, group)
+        y = V.int4_linear(*on_gpu(x, q, s, z), group_size=group, out_dtype=torch.float32).cpu().double()
+        fits = size < 3e38
+        assert fits.all() or e > 110
+        bound = k * 2.0 ** -23 * size + 2.0 ** -24 * ref.abs() + k * 2.0 ** -149
+        assert ((y - ref).abs() <= bound)[fits].all(), e
+        if e == 126:                                               # few enough of them to fit
+            x[:, 2:] = 0
+            ref, size = reference(x, q, s, z, None, group)
+            y = V.int4_linear(*on_gpu(x, q, s, z), group_size=group, out_dtype=torch.float32).cpu().double()
+            assert (size < 3e38).sum() > size.numel() // 2
+            assert ((y - ref).abs() <= k * 2.0 ** -23 * size)[size < 3e38].all()
+
+
 def test_strides_shapes_and_streams():
     x, q, s, z, b = make(6, 96, 256, 64, torch.bfloat16, True, True, 1)
     ref, size = reference(x, q, s, z, b, 64)

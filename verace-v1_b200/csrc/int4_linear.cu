@@ -21,8 +21,8 @@
 // thread adds s D in fp32.  No weight and no input is rounded.
 // What q x and z X lose by cancelling is 2^-24 of the group's largest input.  Where at most a
 // sixteenth of a group is 2^12 above all the rest, that could show in the outputs whose q = z
-// there, so those inputs (and infinities and NaN) are left out of the pieces and added one by
-// one as (q - z) x s at the end (rare).
+// there, so those inputs (and what is above 2^100, infinities and NaN) are left out of the pieces and
+// added one by one as (q - z) x s at the end (rare).
 //
 // One CTA per SM, 128 output rows at a time, 20 warps.  One warp feeds the weights by TMA (128
 // rows x 256 codes a stage, 128-byte swizzle: a row's thread reads 16 bytes without bank
@@ -62,7 +62,7 @@ constexpr int KC = 256;                  // inputs per chunk
 constexpr int W_STAGE = ROWS * KC / 2;   // bytes: 128 rows x 256 codes
 constexpr int MAX_SB = 32;
 constexpr int SMEM = 220 * 1024;
-constexpr float FINITE = 3.4028235e38f;
+constexpr float KEPT = 1.2676506e30f;    // 2^100: inputs above it (infinities, NaN) are added one by one
 constexpr float APART = 1.f / 4096.f;
 
 // How a token tile's x is laid out.  MP tokens per tile; COLS: the pieces in columns of their own.
@@ -142,7 +142,7 @@ __device__ __forceinline__ float leave_out(float (&v)[8], bool& out) {
   out = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (!(fabsf(v[i]) <= FINITE)) out = true, v[i] = 0.f;
+    if (!(fabsf(v[i]) <= KEPT)) out = true, v[i] = 0.f;
     mine = fmaxf(mine, fabsf(v[i]));
   }
   float top = mine;
@@ -174,11 +174,14 @@ __device__ __forceinline__ float leave_out(float (&v)[8], bool& out) {
   return mine;
 }
 
-// The exponent that brings `top` to [2^7, 2^8), at most 100.
+// The exponent that brings `top` (at most KEPT) to [2^7, 2^8), or as far as 2^126 does: what is below
+// 2^-119 has no digits that the last piece would miss.  The sums' factor, with the codes' 2^9, stays a
+// normal number at both ends.
 __device__ __forceinline__ int shift_of(float top) {
-  return min(7 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
+  return min(7 - ((int)(__float_as_uint(top) >> 23) - 127), 126);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ float factor_of(int shift) { return pow2(9 - shift); }
 
 // Writes the pieces of a lane's eight inputs of a chunk (token row t of the tile; a warp holds the
 // chunk) and, from a group's first lanes, X.  A word's codes 0, 2, 4, 6 unpack before 1, 3, 5, 7, and so do x's bytes.
@@ -305,7 +308,7 @@ __global__ void __launch_bounds__(STAGE_NT) int4_stage_x(const T* __restrict__ x
     stage8<T, S>(v, pow2(sh), block + (long long)c * S::BLK, (int)(tok % S::MP), lane);
   }
   if (tid == 0) {
-    scales[tok] = pow2(-sh);
+    scales[tok] = factor_of(sh);
     masks[tok] = s_mask;
   }
 }
@@ -318,12 +321,12 @@ __device__ __noinline__ float left_out(const T* x, const uint8_t* q, const T* s,
   float top = 0.f;
   for (int k = k0; k < k1; ++k) {
     const float m = fabsf(to_f32(x[k]));
-    if (m <= FINITE) top = fmaxf(top, m);
+    if (m <= KEPT) top = fmaxf(top, m);
   }
   int high = 0, low = 0;
   for (int k = k0; k < k1; ++k) {
     const float m = fabsf(to_f32(x[k]));
-    if (m <= FINITE) {
+    if (m <= KEPT) {
       high += m >= top * APART;
       low |= m < top * APART && m != 0.f;
     }
@@ -334,7 +337,7 @@ __device__ __noinline__ float left_out(const T* x, const uint8_t* q, const T* s,
   float v = 0.f;
   for (int k = k0; k < k1; ++k) {
     const float xv = to_f32(x[k]);
-    if (fabsf(xv) <= FINITE && !(alone && fabsf(xv) >= top * APART)) continue;
+    if (fabsf(xv) <= KEPT && !(alone && fabsf(xv) >= top * APART)) continue;
     const uint8_t by = q[row * (k_all / 2) + k / 2];
     v += xv * (((float)(k & 1 ? by >> 4 : by & 15) - zero) * scale);
   }
@@ -755,8 +758,8 @@ __global__ void __launch_bounds__(NT, 1) int4_linear_kernel(const __grid_constan
         tile_m = m0;
         __syncwarp();
         for (int t = lane; t < toks; t += 32) {
-          s_factor[w - 12][t] = 512.f * (a.staged ? a.ws_scale[m0 + t]
-                                                  : nc > 0 ? pow2(-shift_of(__int_as_float(s_top[t]))) : 0.f);
+          s_factor[w - 12][t] = a.staged ? a.ws_scale[m0 + t]
+                                         : nc > 0 ? factor_of(shift_of(__int_as_float(s_top[t]))) : 0.f;
           s_marks[w - 12][t] = a.staged ? a.ws_mask[m0 + t] : s_mask[t];
         }
         __syncwarp();
