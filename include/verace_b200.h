@@ -302,7 +302,11 @@ VERACE_API int verace_decode_step(const void* sssd_q, const void* sssd_k, const 
  * bias   : [n] (dtype), or NULL
  * y      : [m, n] (out_dtype: dtype or VERACE_F32), dense
  * k % 32 == 0; group 32, 64 or 128 (the last group of a row may be short).  All sums are
- * fp32; codes, zeros and inputs enter them exactly and each group's sum is scaled once.
+ * fp32; codes and zeros enter them exactly and each group's sum is scaled once.  Inputs enter
+ * exactly down to 2^-13 of their token's largest; smaller ones may be off, by at most the
+ * largest times 2^-22 (bf16, m <= 32), 2^-21 (bf16, m > 32), 2^-26 (fp16, m <= 16), 2^-23
+ * (fp16, m > 16) or 2^-37 (fp32).  (Inputs 2^12 above all but a sixteenth of their group, inputs
+ * above 2^100, infinities and NaN are added one by one and count for no largest.)
  * Workspace: verace_int4_linear_workspace(m, n, k, group, dtype) bytes, 0 for short inputs;
  * calls sharing a workspace must not overlap.
  * ---------------------------------------------------------------------------- */

@@ -150,6 +150,59 @@ def test_inputs_at_the_ends_of_the_range(m, n, k, group, dtype):
             assert ((y - ref).abs() <= k * 2.0 ** -23 * size)[size < 3e38].all()
 
 
+# As stated in the header: y is the product with inputs each off by at most 2^-`bits` of its token's
+# largest.
+LOST = {torch.bfloat16: (32, 22, 21), torch.float16: (16, 26, 23), torch.float32: (1 << 20, 37, 37)}
+
+
+def lost(x, q, s, z, group, m):
+    most, few, many = LOST[x.dtype]
+    _, weights = reference(torch.ones_like(x[:1]), q, s, z, None, group)         # sum |w|
+    return 2.0 ** -(few if m <= most else many) * x.double().abs().amax(1, keepdim=True) * weights
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k,group", [(1, 3080, 1024, 128), (7, 260, 4096, 64), (16, 200, 2048, 32), (24, 200, 2048, 128),
+                                         (33, 130, 1024, 64), (64, 300, 1024, 32), (90, 260, 2048, 128)])
+def test_groups_of_different_magnitude(m, n, k, group, dtype):
+    """A group of ones above the others, and outputs whose weights are 0 there (which then adds exactly 0)."""
+    x, q, s, z, b = make(m, n, k, group, dtype, True, False, seed=m + n + k)
+    i = k // group // 2
+    ones = slice(i * group, (i + 1) * group)
+    q[::2, i * group // 2:(i + 1) * group // 2] = (z[i, ::2] * 17)[:, None]
+    for below in (4, 10, 16, 22):
+        xe = (x.float() * 2.0 ** -below).to(dtype)
+        xe[:, ones] = 1
+        ref, size = reference(xe, q, s, z, None, group)
+        y = V.int4_linear(*on_gpu(xe, q, s, z), group_size=group, out_dtype=torch.float32).cpu().double()
+        bound = k * 2.0 ** -23 * size + lost(xe, q, s, z, group, m)
+        assert ((y - ref).abs() <= bound).all(), below
+
+
+@pytest.mark.parametrize("m", [2, 16, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_inputs_far_below_the_rest_of_their_group(m, dtype):
+    """Half of each group 2^14 above the other half, whose weights alone are not 0."""
+    n, k, group = 200, 512, 64
+    x, q, s, z, b = make(m, n, k, group, dtype, True, False, seed=m)
+    low = torch.arange(k) % 2 == 1
+    x = torch.where(low, (x.float() * 2.0 ** -8).to(dtype), (x.sign() * 64).to(dtype))
+    q = (q & 0xF0) | z.t().repeat_interleave(group // 2, 1)        # code = zero at the even inputs
+    ref, size = reference(x, q, s, z, None, group)
+    y = V.int4_linear(*on_gpu(x, q, s, z), group_size=group, out_dtype=torch.float32).cpu().double()
+    # the sums in the group run over q x and z X, in fp32: 2^-23 of up to twice 15 sum |x|, group terms
+    sums = group * 2.0 ** -23 * 2 * 15 * (x.double().abs().view(m, -1, group).sum(2) @ s.double())
+    assert ((y - ref).abs() <= k * 2.0 ** -23 * size + lost(x, q, s, z, group, m) + sums).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k,group", [(600, 300, 512, 128), (2050, 520, 288, 32), (513, 1160, 1024, 64)])
+def test_prompt_sizes(m, n, k, group, dtype):
+    x, q, s, z, b = make(m, n, k, group, dtype, True, True, seed=m)
+    ref, size = reference(x, q, s, z, b, group)
+    check(V.int4_linear(*on_gpu(x, q, s, z, b), group_size=group), ref, size, k, dtype)
+
+
 def test_strides_shapes_and_streams():
     x, q, s, z, b = make(6, 96, 256, 64, torch.bfloat16, True, True, 1)
     ref, size = reference(x, q, s, z, b, 64)

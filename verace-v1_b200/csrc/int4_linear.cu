@@ -8,18 +8,25 @@
 // at a quarter of the memory rate, bound by instructions.  Here the tensor cores take a code as
 // it is: the bit pattern of an e4m3 number in [0, 15] reads code * 2^-9 (subnormal below 8, the
 // first binade from 8 on, with the same step), so a word of 8 codes becomes 8 operands with one
-// shift and two masks.  x goes in as fp8 pieces that add up to it, exactly:
+// shift and two masks.  x goes in as fp8 pieces that add up to it:
 //   * few tokens: e4m3 pieces, each the rest of the one before times 2^5, in columns of their
 //     own (a 128-row MMA takes 50 clocks for anything up to 64 columns): y = d0 + 2^-5 d1 + ...
 //     bf16's 8 bits are 2 pieces, fp16's 11 are 3, fp32's 24 are 5;
 //   * up to 64 tokens of 16-bit types: an e4m3 piece and one or two e5m2 pieces of the rest, one
 //     MMA after the other into the same columns.
-// Each token is scaled by a power of two, its largest input to [2^7, 2^8); inputs 2^-22 of that
-// and smaller lose digits.  tcgen05.mma adds fp8 products in full fp32 (measured: 2^23 + 1 is
-// exact).  The zeros are one more MMA per group: 32 inputs that hold X = the sum of a column's pieces
-// over the group, in 6 e5m2 pieces, against -z.  So D = 2^-9 (sum q x - z X) per group, and a row's
-// thread adds s D in fp32.  No weight and no input is rounded.
-// What q x and z X lose by cancelling is 2^-24 of the group's largest input.  Where at most a
+// Each token (of a CTA's share of k, where CTAs stage x themselves) is scaled by a power of two, its
+// largest input to [2^7, 2^8).  The pieces hold an input whole down to 2^-14 (bf16), 2^-16 (fp16, up to 16
+// tokens) or 2^-13 (the others) of that largest; a smaller one is off by at most 2^-22 of the largest
+// (bf16; 2^-21 beyond 32 tokens), 2^-26 (fp16; 2^-23 beyond 16 tokens) or 2^-37 (fp32).  The zeros run
+// over the same pieces, so y is the product of these inputs but for fp32 sums.  (A scale for each group
+// as well, one more factor in the sums, would keep more digits where a whole group is far above the rest
+// and has no weight.  It cost 4 to 18 % of every call, 119 to 125-140 us for 16 x 65536 x 16384 in five
+// forms: the summing warps have neither registers nor issue slots left.)
+// tcgen05.mma adds fp8 products in full fp32 (measured: 2^23 + 1 is exact).  The zeros are one
+// more MMA per group: 32 inputs that hold X = the sum of a column's pieces over the group, in 6 e5m2
+// pieces, against -z.  So D = 2^-9 (sum q x - z X) per group, and a row's thread adds s D in fp32.  No
+// weight is rounded.
+// What q x and z X lose by cancelling is 2^-24 of the sums of q |x|.  Where at most a
 // sixteenth of a group is 2^12 above all the rest, that could show in the outputs whose q = z
 // there, so those inputs (and what is above 2^100, infinities and NaN) are left out of the pieces and
 // added one by one as (q - z) x s at the end (rare).

@@ -8,7 +8,7 @@ quarter of bf16's.
 
 Layout, as :func:`quantize_int4` makes it: ``qweight`` uint8 [n, k/2], two codes to a byte
 along k, the even k in the low half; ``scales`` [ceil(k/group), n] in the activations'
-dtype; ``zeros`` uint8 [ceil(k/group), n] or None (8 everywhere).
+dtype; ``zeros`` uint8 [ceil(k/group), n], 0 to 15, or None (8 everywhere).
 W[n, k] = scales[k // group, n] * (code - zero).
 """
 from typing import Optional, Tuple
@@ -51,7 +51,8 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
                 group_size: int = 128, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., k] (fp32, bf16 or fp16) times the 4-bit weight's transpose, plus bias: [..., n]
     in x's dtype or, with ``out_dtype=torch.float32``, in fp32.  Sums are fp32, the output is
-    rounded once.  Any number of rows; meant for the few of a decode step."""
+    rounded once; inputs below 2^-13 of their row's largest may be off by up to 2^-21 of it (bf16;
+    2^-23 fp16, 2^-37 fp32).  Any number of rows; meant for the few of a decode step."""
     assert x.is_cuda, "This kernel requires CUDA tensors"
     if x.requires_grad:
         _require_no_grad(x, "int4_linear")
