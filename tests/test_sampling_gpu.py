@@ -125,6 +125,24 @@ def test_process_many_wide_rows(b, v, length, among, n, pad, dtype):
         check_process(out, ref, size, odt)
 
 
+@pytest.mark.parametrize("b,v,length", [(2, 3000, 900), (130, 32776, 300), (1, 400, (1 << 20) + 5), (2, 5000, 20000)])
+def test_process_repetition_penalty_is_rounded_once(b, v, length):
+    """l / r and l r themselves, not a product with a rounded 1 / r: equal to the last bit, tiny r included."""
+    g = torch.Generator().manual_seed(v)
+    tokens = torch.randint(0, v, (b, length), generator=g)
+    r = 1 + torch.rand(b, generator=g)
+    r[0] = 2e-39                                                   # (its reciprocal is beyond fp32)
+    seen = torch.zeros(b, v, dtype=torch.bool).scatter_(1, tokens, True)
+    for dtype in (torch.float32, torch.bfloat16):
+        l = torch.randn(b, v, generator=g).to(dtype)
+        l[0] = (l[0].float() * 1e-3).to(dtype)
+        x = l.float()
+        want = torch.where(seen, torch.where(x > 0, x / r[:, None], x * r[:, None]), x)
+        out = V.process_logits(l.cuda(), tokens.cuda(), None, torch.full((b,), length).cuda(), repetition_penalty=r.cuda(),
+                               out_dtype=torch.float32)
+        assert torch.isfinite(want).all() and torch.equal(out.cpu(), want)
+
+
 def test_process_parts_alone_and_scalars():
     g = torch.Generator().manual_seed(5)
     l = torch.randn(4, 700, generator=g)

@@ -61,18 +61,18 @@ __device__ __forceinline__ long long id_at(const void* p, int i64, long long i) 
 }
 
 struct Controls {
-  float r, inv, p, f;
+  float r, p, f;
 };
 __device__ __forceinline__ Controls controls(const LogitsArgs& a, int row) {
-  const float r = a.rep_rows ? a.rep_rows[row] : a.rep;
-  return {r, 1.f / r, a.pres_rows ? a.pres_rows[row] : a.pres, a.freq_rows ? a.freq_rows[row] : a.freq};
+  return {a.rep_rows ? a.rep_rows[row] : a.rep, a.pres_rows ? a.pres_rows[row] : a.pres,
+          a.freq_rows ? a.freq_rows[row] : a.freq};
 }
 __device__ __forceinline__ int history(const LogitsArgs& a, int row) {
   return !a.tokens ? 0 : a.lengths ? max(0, min(a.lengths[row], a.length)) : a.length;
 }
 // A logit of a token seen, `made` of its occurrences being generated.
 __device__ __forceinline__ float penalised(float l, uint32_t made, const Controls& k) {
-  l *= l > 0.f ? k.inv : k.r;
+  l = l > 0.f ? l / k.r : l * k.r;       // (the quotient itself: few tokens are touched)
   if (made) l = __fsub_rn(__fsub_rn(l, __fmul_rn(k.f, (float)made)), k.p);
   return l;
 }
