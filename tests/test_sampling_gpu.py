@@ -418,6 +418,31 @@ def test_sample_ties_and_extremes():
     assert V.sample_logits(l[:0].cuda(), temperature=0)[0].shape == (0,)
 
 
+@pytest.mark.parametrize("kw", [{}, {"top_k": 3000}, {"top_p": 0.9999}, {"min_p": 1e-30}])
+@pytest.mark.parametrize("b,v", [(2, 3000), (300, 20608)])
+def test_sample_subnormal_noise(b, v, kw):
+    """-log(noise) of subnormal noise (88 to 103) beside the smallest normal numbers', and of 0 (infinite)."""
+    g = torch.Generator().manual_seed(v)
+    l = 0.1 * torch.randn(b, v, generator=g)
+    noise = 1.2e-38 * (1 + torch.rand(b, v, generator=g))
+    noise[:, ::50] = 2.0 ** -149 * torch.randint(1, 1 << 22, noise[:, ::50].shape, generator=g)
+    l[:, 77], noise[:, 77] = 20.0, 0.5                           # kept, but far from chosen
+    l[1, ::50] -= 30.0                                           # the normal ones win over the subnormal
+    tok, _ = V.sample_logits(l.cuda(), noise.cuda(), **kw)
+    score = l.double() - noise.double().log()
+    if kw.get("top_k", v) < v:
+        score[l < l.sort(dim=1, descending=True).values[:, kw["top_k"] - 1:kw["top_k"]]] = -INF
+    if "min_p" in kw:
+        score[l.double() - l.max(1, keepdim=True).values < np.log(1e-30)] = -INF
+    if "top_p" in kw:
+        score[:, :77], score[:, 78:] = -INF, -INF                # (all but e^-20 of the mass)
+    best = score.max(1).values
+    assert (best - score.gather(1, tok.cpu()[:, None])[:, 0] <= 1e-4).all()
+    noise[0, 1234], l[0, 1234] = 0.0, -10.0
+    if not kw:
+        assert int(V.sample_logits(l.cuda(), noise.cuda())[0][0]) == 1234
+
+
 def test_sample_draws_follow_the_softmax():
     l = torch.tensor([2.0, 1.0, 0.0, -1.0, 3.0, -INF, 0.5, 2.5])
     n = 20000

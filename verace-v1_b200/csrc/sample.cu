@@ -743,11 +743,18 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
         }
         values(j / 8, v);
       }
-      float high[8], sure = -INFINITY, peak = -INFINITY;
+      float high[8], log2_r[8], sure = -INFINITY, peak = -INFINITY, least_r = r[0];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) log2_r[i] = log2_of(r[i]), least_r = fminf(least_r, r[i]);
+      if (least_r < 1.17549435e-38f) {         // (log2_of takes subnormal noise for 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (r[i] < 1.17549435e-38f) log2_r[i] = log2_of(r[i] * 4294967296.f) - 32.f;
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float z = v[i] == top ? 0.f : (v[i] - top) * inv;
-        const float near = fmaf(-0.693147181f, log2_of(r[i]), direct ? z + shift : z), o = fmaf(-1e-6f, z, off);
+        const float near = fmaf(-0.693147181f, log2_r[i], direct ? z + shift : z), o = fmaf(-1e-6f, z, off);
         high[i] = near + o;
         peak = fmaxf(peak, high[i]);
         sure = fmaxf(sure, near - o);
