@@ -443,6 +443,24 @@ def test_sample_subnormal_noise(b, v, kw):
         assert int(V.sample_logits(l.cuda(), noise.cuda())[0][0]) == 1234
 
 
+@pytest.mark.parametrize("b,v", [(3, 1000), (300, 20608), (2, 1100000)])
+def test_sample_infinite_temperatures(b, v):
+    """Rows of infinite T draw evenly from what is not masked: the smallest noise, log p = -log of its count."""
+    l, noise = draw(b, v, v, 0.3)
+    l[1] = -INF
+    l[1, 5:9] = 3e38
+    t = torch.ones(b)
+    t[:2] = INF
+    for kw in ({}, {"top_k": 20}, {"top_p": 0.5}):
+        tok, lp = V.sample_logits(l.cuda(), noise.cuda(), temperature=t.cuda(), **kw)
+        for i in range(2):
+            there = l[i] > -INF
+            if kw:                                                     # (the logits' order, with equal masses)
+                there &= l[i] >= l[i].sort(descending=True).values[19 if "top_k" in kw else (int(there.sum()) - 1) // 2]
+            assert int(tok[i]) == int(torch.where(there, noise[i], INF).argmin())
+            assert abs(float(lp[i]) + np.log(int((l[i] > -INF).sum()))) <= 1e-5
+
+
 def test_sample_draws_follow_the_softmax():
     l = torch.tensor([2.0, 1.0, 0.0, -1.0, 3.0, -INF, 0.5, 2.5])
     n = 20000

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
   const float* noise = a.noise + row * a.noise_ld;
   const float t = a.t_rows ? a.t_rows[row] : a.t;
   const bool greedy = !(t > 0.f);
-  const float ts = greedy ? 1.f : t;
+  const float ts = greedy ? 1.f : fminf(t, 3.4028235e38f);      // (an infinite T: as good as the largest)
   const int k = a.k_rows ? a.k_rows[row] : a.k;
   const float p = a.p_rows ? a.p_rows[row] : a.p;
   const float minp = a.minp_rows ? a.minp_rows[row] : a.minp;
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   const T* l = static_cast<const T*>(a.logits) + row * a.ld;
   const float t = a.t_rows ? a.t_rows[row] : a.t;
   const bool greedy = !(t > 0.f);
-  const float ts = greedy ? 1.f : t;
+  const float ts = greedy ? 1.f : fminf(t, 3.4028235e38f);      // (an infinite T: as good as the largest)
   const int k = a.k_rows ? a.k_rows[row] : a.k;
   const float p = a.p_rows ? a.p_rows[row] : a.p;
   const float minp = a.minp_rows ? a.minp_rows[row] : a.minp;
