@@ -485,6 +485,21 @@ def test_sample_vocabularies_of_any_size():
         check_sample(l, None, 0.0, 0, 1.0, 0.0)
 
 
+def test_sample_masses_of_very_long_rows():
+    """2^24 equal values at the top: their mass alone is 2^64 of the units that shorter rows have."""
+    v, n = (1 << 24) + (1 << 22), 1 << 24
+    l = torch.zeros(1, v, device="cuda")
+    l[:, n:] = -1.0
+    noise = torch.ones(1, v, device="cuda")
+    noise[0, 5], noise[0, v - 9] = 0.5, 1e-6
+    for kw, token in (({"top_p": 0.5}, 5), ({"top_p": 0.999}, v - 9), ({}, v - 9), ({"top_k": 7}, 5)):
+        tok, lp = V.sample_logits(l, noise, **kw)
+        assert int(tok) == token
+        want = (0.0 if token == 5 else -1.0) - np.log(n + (v - n) * np.exp(-1.0))
+        # (4096 fp32 additions a thread, of a tenth of the sum)
+        assert abs(float(lp) - want) <= 4096 * 2.0 ** -24 * 0.1 + 2.0 ** -21 * 20
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_sample_cuts_among_many_equal_values(dtype):
     """Few distinct values, values around zero and of every size: the cut falls into crowded bins."""

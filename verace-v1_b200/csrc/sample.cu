@@ -13,7 +13,9 @@
 // handful), then within the bin of the cut 512 bins of the values' order-preserving keys, until
 // a bin holds one value or one key: two or three levels for most rows, five at worst.
 // sample_rows: one CTA per row that reads it again for every pass; for rows of more than 16 x 65536
-// values.  Mass is summed in 2^-40 fixed point, so that the order of the atomics changes nothing.
+// values.  Mass is summed in whole numbers (2^-40 of the largest weight; in sample_cluster's histograms
+// 2^-20 of the bin's largest, and nothing for the last bin, below exp(-31)), so that the order of the
+// atomics changes nothing.  A cut by p so moves only where it is within about 1e-6 of a value's edge.
 //
 // Bound: one read of the row, and of the noise where every value draws.  Measured on the device: one
 // row of 32000 at T = 0 6.1 us (launch and cluster barriers); 64 fp32 rows of 163840 with k = 50,
@@ -114,6 +116,8 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
   ties = block_reduce(ties, red, [](float x, float y) { return x + y; });
   rest = block_reduce(rest, red, [](float x, float y) { return x + y; });
   const float lse = logf(ties) + log1pf(rest / ties);
+  // the unit of mass: 2^40 to the largest weight, or so many that no sum over the row passes 64 bits
+  const float unit = ldexpf(1.f, min(40, 32 + __clz(a.v)));
 
   // the smallest kept key: every key above key_of(-inf), then by count, then by mass
   uint32_t least = key_of(-INFINITY) + 1;
@@ -130,7 +134,7 @@ __global__ void __launch_bounds__(NT) sample_rows(SampleArgs a) {
           const uint32_t key = key_of(x);
           if (key >= least && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
             atomicAdd(&hist[(key >> shift) & 255],
-                      by_mass ? (unsigned long long)(expf(scaled(x, top, ts)) * 1099511627776.f + 0.5f) : 1ull);
+                      by_mass ? (unsigned long long)(expf(scaled(x, top, ts)) * unit + 0.5f) : 1ull);
         }
         __syncthreads();
         if (tid == 0) {
