@@ -301,7 +301,8 @@ VERACE_API int verace_decode_step(const void* sssd_q, const void* sssd_k, const 
  * zeros  : [ceil(k/group), n] bytes in [0, 15], or NULL (8 everywhere)
  * bias   : [n] (dtype), or NULL
  * y      : [m, n] (out_dtype: dtype or VERACE_F32), dense
- * k % 32 == 0; group 32, 64 or 128 (the last group of a row may be short).  All sums are
+ * m <= 2^20, n <= 2^28, k <= 2^30; k % 32 == 0; group 32, 64 or 128 (the last group of a row
+ * may be short).  All sums are
  * fp32; codes and zeros enter them exactly and each group's sum is scaled once.  Inputs enter
  * exactly down to 2^-13 of their token's largest; smaller ones may be off, by at most the
  * largest times 2^-22 (bf16, m <= 32), 2^-21 (bf16, m > 32), 2^-26 (fp16, m <= 16), 2^-23
@@ -336,6 +337,7 @@ VERACE_API int verace_int4_linear(const void* x, long long ldx, const void* qwei
  *   outside [0, v) are skipped; of entries with the same id the last one holds.
  * allowed: 32-bit words, bit t % 32 of word t / 32 is token t's, row stride allowed_ld words
  *   (0: one row for all), or NULL.
+ * b <= 65535; v, length and n_bias up to 2^30.
  * ---------------------------------------------------------------------------- */
 VERACE_API int verace_logits_process(const void* logits, long long ld, void* out, long long out_ld, int b, int v,
                                      int dtype, int out_dtype, const void* tokens, long long tokens_ld,
@@ -358,7 +360,7 @@ VERACE_API int verace_logits_process(const void* logits, long long ld, void* out
  * A row that leaves no token gives token -1 and logprob -inf.
  * logits [b, v] (dtype), row stride ld; noise [b, v] fp32, row stride noise_ld, read only
  * where a token is kept (NULL only with t_rows NULL and t <= 0); *_rows: [b], or NULL for
- * the scalar; tokens [b] int64, logprobs [b] fp32.
+ * the scalar; tokens [b] int64, logprobs [b] fp32.  v <= 2^30.
  * ---------------------------------------------------------------------------- */
 VERACE_API int verace_sample(const void* logits, long long ld, const float* noise, long long noise_ld, int b, int v,
                              int dtype, const float* t_rows, float t, const int* k_rows, int k,

@@ -143,3 +143,26 @@ def test_sample_rejects_bad_arguments_without_a_device():
     assert call(nld=50) == 1 and "row stride" in _err()
     assert call(tok=None) == 1 and "NULL" in _err()
     assert call(b=0, logits=None) == 0
+
+
+@host_only
+def test_sizes_beyond_32_bit_indices_are_refused_without_a_device():
+    """Sizes at which a device index, a stride past the end, would pass 32 bits."""
+    L = _lib.lib()
+    huge, out = (1 << 30) + 1, ctypes.c_void_p(4096)
+
+    def int4(m, n, k):
+        return L.verace_int4_linear(FAKE, k, FAKE, FAKE, None, None, FAKE, m, n, k, 32, 1, 1, None, 0, None)
+
+    assert int4(1, 8, (1 << 31) - 32) == 2 and "too large" in _err()
+    assert int4((1 << 20) + 1, 8, 64) == 2 and int4(1, (1 << 28) + 1, 64) == 2
+    assert L.verace_int4_linear_workspace(1, 8, (1 << 31) - 32, 32, 1) == 0
+
+    def process(v=100, length=8, biases=0):
+        return L.verace_logits_process(FAKE, v, out, v, 2, v, 0, 0, FAKE, length, 1, length, None, None, None, 1.0, None,
+                                       0.0, None, 0.0, FAKE, FAKE, biases, 0, None, 0, None)
+
+    for kw in ({"v": huge}, {"length": huge}, {"biases": huge}):
+        assert process(**kw) == 2 and "2^30" in _err()
+    assert L.verace_sample(FAKE, huge, FAKE, huge, 2, huge, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, FAKE, FAKE,
+                           None) == 2 and "2^30" in _err()

@@ -1073,7 +1073,7 @@ int int4_read_status(int* status) {
 using namespace verace;
 
 extern "C" size_t verace_int4_linear_workspace(long long m, int n, int k, int group, int dtype) {
-  if (m <= 0 || n <= 0 || k < 0 || k % 32 || (group != 32 && group != 64 && group != 128) || dtype < VERACE_F32 ||
+  if (m <= 0 || n <= 0 || k < 0 || k > 1 << 30 || k % 32 || (group != 32 && group != 64 && group != 128) || dtype < VERACE_F32 ||
       dtype > VERACE_F16)
     return 0;
   return dispatch(m, group, dtype, [&](auto t, auto s) {
@@ -1099,8 +1099,8 @@ extern "C" int verace_int4_linear(const void* x, long long ldx, const void* qwei
   const size_t esz = dtype == VERACE_F32 ? 4 : 2;
   VERACE_REQUIRE((size_t)x % 16 == 0 && ldx * esz % 16 == 0 && (size_t)qweight % 16 == 0, VERACE_ERR_INVALID,
                  "int4_linear: x rows and qweight must be 16-byte aligned");
-  VERACE_REQUIRE(m <= 1LL << 20 && n <= 1 << 28 && (m + 3) / 4 * ((n + ROWS - 1) / ROWS) < 1LL << 30,
-                 VERACE_ERR_UNSUPPORTED, "int4_linear: m %lld, n %d too large", m, n);
+  VERACE_REQUIRE(m <= 1LL << 20 && n <= 1 << 28 && k <= 1 << 30 && (m + 3) / 4 * ((n + ROWS - 1) / ROWS) < 1LL << 30,
+                 VERACE_ERR_UNSUPPORTED, "int4_linear: m %lld, n %d, k %d too large", m, n, k);
   Int4Args a{};
   a.x = x; a.ldx = ldx; a.q = static_cast<const uint8_t*>(qweight); a.s = scales;
   a.z = static_cast<const uint8_t*>(zeros); a.bias = bias; a.y = y; a.m = m; a.n = n; a.k = k;

@@ -530,6 +530,9 @@ extern "C" int verace_logits_process(const void* logits, long long ld, void* out
   VERACE_REQUIRE(out_dtype == dtype || out_dtype == VERACE_F32, VERACE_ERR_INVALID,
                  "logits_process: out_dtype %d (the input's or fp32)", out_dtype);
   VERACE_REQUIRE(b <= 65535, VERACE_ERR_UNSUPPORTED, "logits_process: %d rows (at most 65535)", b);
+  // (indices run a stride past the end in 32 bits)
+  VERACE_REQUIRE(v <= 1 << 30 && length <= 1 << 30 && n_bias <= 1 << 30, VERACE_ERR_UNSUPPORTED,
+                 "logits_process: %d tokens, histories of %d, %d biases (at most 2^30 of each)", v, length, n_bias);
   if (b == 0 || v == 0) return VERACE_OK;
   VERACE_REQUIRE(logits && out, VERACE_ERR_INVALID, "logits_process: NULL pointer");
   VERACE_REQUIRE(ld >= v && out_ld >= v, VERACE_ERR_INVALID, "logits_process: row stride below the vocabulary size");

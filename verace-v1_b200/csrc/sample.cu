@@ -875,6 +875,8 @@ extern "C" int verace_sample(const void* logits, long long ld, const float* nois
   VERACE_REQUIRE(b >= 0 && v >= 0, VERACE_ERR_INVALID, "sample: negative size");
   VERACE_REQUIRE(dtype == VERACE_F32 || dtype == VERACE_BF16 || dtype == VERACE_F16, VERACE_ERR_INVALID,
                  "sample: dtype %d", dtype);
+  // (indices run a stride past the end in 32 bits)
+  VERACE_REQUIRE(v <= 1 << 30, VERACE_ERR_UNSUPPORTED, "sample: %d tokens (at most 2^30)", v);
   if (b == 0) return VERACE_OK;
   VERACE_REQUIRE(v > 0, VERACE_ERR_INVALID, "sample: empty vocabulary");
   VERACE_REQUIRE(logits && tokens && logprobs, VERACE_ERR_INVALID, "sample: NULL pointer");
