@@ -143,6 +143,20 @@ def test_process_repetition_penalty_is_rounded_once(b, v, length):
         assert torch.isfinite(want).all() and torch.equal(out.cpu(), want)
 
 
+def test_process_lengths_beyond_32_bits():
+    g = torch.Generator().manual_seed(21)
+    l, tokens = torch.randn(3, 500, generator=g).cuda(), torch.randint(0, 500, (3, 60), generator=g).cuda()
+    kw = dict(repetition_penalty=1.5, presence_penalty=0.5)
+    for big in (1 << 31, (1 << 32) + 1, (1 << 63) - 1):
+        big = torch.full((3,), big, device="cuda")
+        assert torch.equal(V.process_logits(l, tokens, big, **kw), V.process_logits(l, tokens, **kw))
+        want = V.process_logits(l, tokens, repetition_penalty=1.5)       # all of it the prompt
+        assert not torch.equal(want, l)
+        assert torch.equal(V.process_logits(l, tokens, None, big, **kw), want)
+        want = V.process_logits(l, tokens, repetition_penalty=1.5, presence_penalty=0.5)
+        assert torch.equal(V.process_logits(l, tokens, None, -big, **kw), want)
+
+
 def test_process_parts_alone_and_scalars():
     g = torch.Generator().manual_seed(5)
     l = torch.randn(4, 700, generator=g)
@@ -459,6 +473,16 @@ def test_sample_infinite_temperatures(b, v):
                 there &= l[i] >= l[i].sort(descending=True).values[19 if "top_k" in kw else (int(there.sum()) - 1) // 2]
             assert int(tok[i]) == int(torch.where(there, noise[i], INF).argmin())
             assert abs(float(lp[i]) + np.log(int((l[i] > -INF).sum()))) <= 1e-5
+
+
+def test_sample_top_k_beyond_32_bits():
+    l, noise = draw(4, 3000, 12)
+    want = V.sample_logits(l.cuda(), noise.cuda())
+    assert not torch.equal(want[0].cpu(), l.argmax(1))
+    for k in (1 << 31, (1 << 32) + 1, (1 << 63) - 1, -(1 << 40) + 1):
+        for top_k in (k, torch.full((4,), k, device="cuda")):
+            got = V.sample_logits(l.cuda(), noise.cuda(), top_k=top_k)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 def test_sample_draws_follow_the_softmax():

@@ -19,11 +19,21 @@ PerRow = Union[float, torch.Tensor]
 _INF = float("inf")
 
 
+_INT32 = torch.iinfo(torch.int32)
+
+
+def _int32(value: torch.Tensor) -> torch.Tensor:
+    """value as int32; an int64 one beyond its range (a limit that is meant to hold nothing back) as its end."""
+    if value.dtype is torch.int64:
+        value = value.clamp(_INT32.min, _INT32.max)
+    return value.to(torch.int32)
+
+
 def _per_row(value: torch.Tensor, name: str, b: int, dev, dtype=torch.float32) -> torch.Tensor:
     assert value.dim() == 1 and value.shape[0] == b and value.device == dev, \
         f"{name} must be a number or a [b] tensor on the logits' device"
     if value.dtype is not dtype or not value.is_contiguous():
-        value = value.to(dtype).contiguous()
+        value = (_int32(value) if dtype is torch.int32 else value.to(dtype)).contiguous()
     return value
 
 
@@ -39,7 +49,7 @@ def _lengths(lengths: Optional[torch.Tensor], name: str, b: int, dev):
         return None
     assert lengths.dim() == 1 and lengths.shape[0] == b and lengths.device == dev, \
         f"{name} must be a [b] tensor on the logits' device"
-    return lengths if lengths.dtype is torch.int32 and lengths.is_contiguous() else lengths.to(torch.int32).contiguous()
+    return lengths if lengths.dtype is torch.int32 and lengths.is_contiguous() else _int32(lengths).contiguous()
 
 
 def _dense_rows(x: torch.Tensor, b: int, v: int) -> int:
@@ -214,7 +224,7 @@ def sample_logits(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
         top_k = _per_row(top_k, "top_k", b, dev, torch.int32)
         kp = top_k.data_ptr()
     else:
-        ks = top_k if top_k < v else 0
+        ks = top_k if 0 < top_k < v else 0
     if isinstance(top_p, torch.Tensor):
         top_p = _per_row(top_p, "top_p", b, dev)
         pp = top_p.data_ptr()
