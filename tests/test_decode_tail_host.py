@@ -166,3 +166,17 @@ def test_sizes_beyond_32_bit_indices_are_refused_without_a_device():
         assert process(**kw) == 2 and "2^30" in _err()
     assert L.verace_sample(FAKE, huge, FAKE, huge, 2, huge, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, FAKE, FAKE,
                            None) == 2 and "2^30" in _err()
+
+
+def test_package_imports_on_a_torch_without_cuda(monkeypatch):
+    """Such a torch lacks the two names that the launch path takes a shortcut through."""
+    import importlib
+    from verace_v1_b200 import _launch
+    for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    try:
+        again = importlib.reload(_launch)
+        assert again.current is torch.cuda.current_device and callable(again.raw_stream)
+    finally:
+        monkeypatch.undo()
+        importlib.reload(_launch)
