@@ -73,6 +73,18 @@ def test_quantised_model_matches_its_dequantised_weights():
     assert V.device_status() == 0
 
 
+def test_rows_that_biases_leave_nothing_end():
+    model, ids = make_model(), prompt()
+    everything = torch.arange(100, device="cuda").expand(3, 100).contiguous()
+    values = torch.zeros(3, 100, device="cuda")
+    values[1] = -float("inf")
+    tokens, lp = V.generate(model, ids, 4, bias_ids=everything, bias_values=values)
+    want, want_lp = V.generate(model, ids, 4)
+    assert torch.equal(tokens[[0, 2]], want[[0, 2]])
+    torch.testing.assert_close(lp[[0, 2]], want_lp[[0, 2]], rtol=1e-3, atol=1e-4)
+    assert (tokens[1, 7:] == -1).all() and (lp[1] == 0).all()
+
+
 def test_controls_and_ends_of_rows():
     model, ids = make_model(torch.bfloat16), prompt()
     V.quantize_model_int4(model, group_size=128)

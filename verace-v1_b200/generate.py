@@ -23,9 +23,9 @@ def generate(model: torch.nn.Module, input_ids: torch.Tensor, max_new_tokens: in
     ``max_new_tokens``.  The controls are those of ``process_logits`` (the prompt counts for the
     repetition penalty, not for the other two) and ``sample_logits``; ``allowed`` may be a
     function of the tokens so far, [b, s + i], that returns the step's mask.  A row ends at
-    ``eos_token_id`` or where the mask leaves it nothing: its later tokens are ``eos_token_id`` (-1
-    without one) with log-probability 0, and the loop ends once every row has (a host read a step,
-    only with an eos or a mask)."""
+    ``eos_token_id`` or where the mask or the biases (of -inf) leave it nothing: its tokens from there on
+    are ``eos_token_id`` (-1 without one) with log-probability 0, and the loop ends once every row has (a
+    host read a step, only with an eos or a mask)."""
     if max_new_tokens < 0:
         raise ValueError(f"max_new_tokens {max_new_tokens}: expected at least 0")
     assert input_ids.is_cuda, "This kernel requires CUDA tensors"
@@ -51,7 +51,7 @@ def generate(model: torch.nn.Module, input_ids: torch.Tensor, max_new_tokens: in
                              bias_ids=bias_ids, bias_values=bias_values, allowed=mask, out_dtype=torch.float32)
         noise = torch.empty_like(row).exponential_(generator=generator) if sampled else None
         token, lp = sample_logits(row, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        if ends:
+        if ends or bias_ids is not None:
             done = done | (token < 0)
             token = torch.where(done, end, token)
             lp = torch.where(done, 0.0, lp)
