@@ -20,8 +20,8 @@
 // (bf16; 2^-21 beyond 32 tokens), 2^-26 (fp16; 2^-23 beyond 16 tokens) or 2^-37 (fp32).  The zeros run
 // over the same pieces, so y is the product of these inputs but for fp32 sums.  (A scale for each group
 // as well, one more factor in the sums, would keep more digits where a whole group is far above the rest
-// and has no weight.  It cost 4 to 18 % of every call, 119 to 125-140 us for 16 x 65536 x 16384 in five
-// forms: the summing warps have neither registers nor issue slots left.)
+// and has no weight.  It cost 4 to 20 % of every call, 125 to 147 us against 119 for 16 x 65536 x 16384 in
+// five forms: the summing warps have neither registers nor issue slots left.)
 // tcgen05.mma adds fp8 products in full fp32 (measured: 2^23 + 1 is exact).  The zeros are one
 // more MMA per group: 32 inputs that hold X = the sum of a column's pieces over the group, in 6 e5m2
 // pieces, against -z.  So D = 2^-9 (sum q x - z X) per group, and a row's thread adds s D in fp32.  No
@@ -41,9 +41,10 @@
 // share of the memory rate, and two lines have twice that.  Few row tiles: k is split over a
 // cluster and the partial sums are joined through distributed shared memory in rank order.
 //
-// Measured on the device (copies run at 6.55 TB/s): 1 x 163840 x 1024 bf16 21.8 us, 4.0 TB/s;
-// 16 x 65536 x 16384 116 to 119 us, 4.7 TB/s (512 tiles over 148 CTAs: three rounds and half a one); 64 x 16384 x 4096 20.5 us, 420 TFLOP/s, 3 us of it the staging of x; 7 x 4096 x
-// 8192 fp16 11.5 us and 1 x 3080 x 1024 6.8 us, of which set-up and joins are 5.
+// Measured on the device (copies run at 6.55 TB/s): 1 x 163840 x 1024 bf16 22 to 23 us, 3.9 TB/s;
+// 16 x 65536 x 16384 118 to 122 us, 4.6 TB/s (512 tiles over 148 CTAs: three rounds and half a one);
+// 64 x 16384 x 4096 20.7 us, 415 TFLOP/s, 3 us of it the staging of x; 7 x 4096 x 8192 fp16 12.5 to 13.1 us
+// and 1 x 3080 x 1024 6.7 us, of which set-up and joins are 5.
 #include "common.cuh"
 #include "tc.cuh"
 #include "tmap.cuh"

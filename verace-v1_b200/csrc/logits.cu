@@ -14,10 +14,11 @@
 // and a full mask, and are copied.
 //
 // Measured on the device: a row of 32000 with 200 tokens of history 3.7 us; 64 rows of 163840, bf16
-// to fp32, 63 MB: mask alone 12.9 us (4.9 TB/s), with 4096 tokens of history 19, with 300 biases too
-// 20.9 (3.0 TB/s; 28 before the listed form: the counting went before the stream, not beside it; what
+// to fp32, 63 MB: mask alone 12.9 us (4.9 TB/s), with 4096 tokens of history 19.5, with 300 biases too
+// 22.0 (2.9 TB/s; 28 before the listed form: the counting went before the stream, not beside it; what
 // is left is the counting's chain of loads under the stream's, 10 us); 8 rows of 32000 with 65536
-// tokens of history 11.6, in which every CTA of a row reads its history from L2.
+// tokens of history 12.3, in which every CTA of a row reads its history from L2.  (0.5 to 0.8 us of
+// both last ones are the repetition penalty's division, beside a product with 1 / r.)
 #include "common.cuh"
 
 #include <atomic>

@@ -21,8 +21,8 @@
 // row of 32000 at T = 0 6.1 us (launch and cluster barriers); 64 fp32 rows of 163840 with k = 50,
 // p = 0.9 and min_p 26 us for 42 MB (1.6 TB/s: two passes, the second from L2, then about eight steps
 // between barriers of the cluster; one CTA a row that read it again for every step: 1924), with p alone
-// 54; 256 bf16 rows of
-// 32000 without cuts 25 us for 49 MB with the noise (2.0 TB/s: the arithmetic per value).
+// 54 to 69; 256 bf16 rows of 32000 without cuts 25 us for 49 MB with the noise (2.0 TB/s: three passes with
+// the cluster's barriers between, and the arithmetic per value, about 9 us of it).
 #include "common.cuh"
 
 #include <cooperative_groups.h>
