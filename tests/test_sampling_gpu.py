@@ -432,6 +432,16 @@ def test_sample_ties_and_extremes():
     assert V.sample_logits(l[:0].cuda(), temperature=0)[0].shape == (0,)
 
 
+@pytest.mark.parametrize("b,v", [(40, 3000), (300, 20608), (2, 1100000)])
+@pytest.mark.parametrize("offset", [-6e4, 300.0, 2e5, -3e7])
+def test_sample_logits_far_from_zero(b, v, offset):
+    """z is against the row's largest: what all of a row's logits have in common costs no digits of the noise."""
+    l, noise = draw(b, v, v)
+    l = l + offset
+    for t, k, p, minp in ((0.7, 0, 1.0, 0.0), (0.7, 50, 0.9, 0.0), (1.0, 0, 0.8, 0.01), (1.3, 0, 1.0, 0.05)):
+        check_sample(l, noise, t, k, p, minp, most_clear=b < 300 and v < 1000000)
+
+
 @pytest.mark.parametrize("kw", [{}, {"top_k": 3000}, {"top_p": 0.9999}, {"min_p": 1e-30}])
 @pytest.mark.parametrize("b,v", [(2, 3000), (300, 20608)])
 def test_sample_subnormal_noise(b, v, kw):

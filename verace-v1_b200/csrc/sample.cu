@@ -530,8 +530,8 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
   // levels and barriers over the cluster.  Comparing every value with every other instead took 60 k
   // clocks for a list of 1000.)
   const float shift = top * inv;
-  const bool direct = fabsf(top / ts) <= 3.4028235e38f;
-  // the score: l / T - log(noise) where that is in range, z - log(noise) where it is not
+  // the score: l / T - log(noise) while that loses no more digits than z - log(noise), the latter beyond
+  const bool direct = fabsf(top / ts) <= 64.f;
   auto score_of = [&](float x, float r) { return (direct ? x / ts : -(below(x) / ts)) - logf(r); };
   unsigned long long choice = 0;
   auto pack = [&](float score, int i) {
@@ -727,7 +727,7 @@ __global__ void __launch_bounds__(CT, 2) sample_cluster(SampleArgs a, int chunk)
     // Every value's noise.  Fast arithmetic (off by less than `off`) passes over all that the best
     // of the warp so far rules out, which leaves a handful for the division and the logarithm.
     const bool wide = reinterpret_cast<size_t>(noise) % 16 == 0;
-    const float off = 1e-3f + 1e-5f * fabsf(shift);
+    const float off = direct ? 1e-3f + 1e-5f * fabsf(shift) : 1e-3f;
     float bound = -INFINITY;             // no score of the warp's that counts is below this
     for (int j0 = 0; j0 < n8; j0 += CT) {      // (whole warps)
       const int j = 8 * (j0 + tid);
