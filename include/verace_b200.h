@@ -44,7 +44,7 @@ enum {
   VERACE_ERR_STATE = 6        /* a decode step met a hologram too far from unitary */
 };
 
-enum { VERACE_F32 = 0, VERACE_BF16 = 1, VERACE_F16 = 2 };
+enum { VERACE_F32 = 0, VERACE_BF16 = 1, VERACE_F16 = 2, VERACE_E4M3 = 3 /* 8-bit operands of the dense products only */ };
 
 /* Version of this ABI (major*10000 + minor*100 + patch). */
 VERACE_API int verace_version(void);
@@ -366,6 +366,64 @@ VERACE_API int verace_sample(const void* logits, long long ld, const float* nois
                              int dtype, const float* t_rows, float t, const int* k_rows, int k,
                              const float* p_rows, float p, const float* minp_rows, float minp, long long* tokens,
                              float* logprobs, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * RMS norm with the residual's addition, its output in 8 bits with a scale for each row (beside
+ * verace_add_rmsnorm, whose output is in the activations' type; the reference has no 8-bit path).
+ *   h <- h + y (written to sum, rounded to dtype; with y NULL there is no addition and sum is NULL)
+ *   v = h rsqrt(mean h^2 + eps) weight   (weight NULL: 1; norm 0: v = h, a quantiser of rows)
+ *   a = max(max |v|, 2^-100); scale = a / 448; q = v 448 / a in e4m3 (to nearest even)
+ * h, y, sum, n: [rows, cols] (dtype), dense; q: [rows, cols] bytes; scale: [rows] fp32; n, or NULL: v
+ * rounded to dtype.  sum may be h or y.  v is not rounded to dtype before it is rounded to 8 bits.
+ * 1 <= cols <= 32768.
+ * ---------------------------------------------------------------------------- */
+VERACE_API int verace_rmsnorm_fp8(const void* h, const void* y, void* sum, const void* weight, float eps, int norm,
+                                  void* q, float* scale, void* n, long long rows, int cols, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * Dense products with their epilogues (the reference: torch.nn.Linear products with separate
+ * elementwise steps, verace_v1/modules/mcmoe.py:85-120, activations.py:8-31).
+ *   linear: out = act(x w^T + bias) + residual           act: VERACE_ACT_NONE ... GELU_TANH
+ *   gated:  out = act(g) up(u), g = x w_gate^T, u = x w_up^T    act: VERACE_ACT_RELU ... SITU
+ *           SITU: beta1 tanh(g / beta1) sigmoid(g) beta2 tanh(u / beta2); the others: act(g) u
+ * x: [m, k], rows ldx elements apart; w: [n, k] (w_gate, w_up: [f, k]), rows ldw apart: dtype, 16-byte
+ *   aligned rows unless dtype is fp32.  dtype VERACE_E4M3: x_scale [m], w_scale [n] (gate_scale, up_scale
+ *   [f]) fp32 stand for x_scale[i] x[i][k] and so on; NULL with the other types.
+ * bias: [n] (dtype; with E4M3 out_dtype) or NULL; residual: [m, n] (out_dtype), rows ld_res apart, or NULL.
+ * out: [m, n] (out_dtype: dtype or VERACE_F32; with E4M3 any of the three), dense; may be the residual.
+ * pre (gate and up): NULL, or [m, n] (out_dtype), dense: the sums before the activation (linear: with the
+ *   bias), which the backward call reads.
+ * Backward, from dout [m, n] (out_dtype), dense: dx [m, k], dw [n, k], dbias [n] (dtype, dense; NULL: not
+ *   computed); the residual's gradient is dout.  pre may be NULL with VERACE_ACT_NONE.
+ * Sums are fp32 and outputs are rounded once; in a backward call act'(.) times dout is rounded to dtype
+ * before it is multiplied.  fp32 operands enter as three bf16 parts (24 bits; an infinity gives
+ * NaN).  Sizes up to 2^24.  Workspace: the bytes of the *_workspace query; calls sharing one must not overlap.
+ * ---------------------------------------------------------------------------- */
+enum {
+  VERACE_ACT_NONE = 0, VERACE_ACT_RELU = 1, VERACE_ACT_SILU = 2, VERACE_ACT_GELU = 3,   /* gelu: by erf */
+  VERACE_ACT_GELU_TANH = 4, VERACE_ACT_SITU = 5
+};
+VERACE_API size_t verace_linear_workspace(long long m, int n, int k, int dtype);
+VERACE_API int verace_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
+                             const float* w_scale, const void* bias, const void* residual, long long ld_res, void* out,
+                             void* pre, long long m, int n, int k, int act, int dtype, int out_dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+VERACE_API size_t verace_linear_backward_workspace(long long m, int n, int k, int dtype);
+VERACE_API int verace_linear_backward(const void* dout, const void* x, long long ldx, const void* w, long long ldw,
+                                      const void* pre, void* dx, void* dw, void* dbias, long long m, int n, int k, int act,
+                                      int dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+VERACE_API size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype);
+VERACE_API int verace_gated_linear(const void* x, long long ldx, const float* x_scale, const void* w_gate,
+                                   const void* w_up, long long ldw, const float* gate_scale, const float* up_scale,
+                                   void* out, void* gate, void* up, long long m, int f, int k, int act, float beta1,
+                                   float beta2, int dtype, int out_dtype, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+VERACE_API size_t verace_gated_linear_backward_workspace(long long m, int f, int k, int dtype);
+VERACE_API int verace_gated_linear_backward(const void* dout, const void* x, long long ldx, const void* w_gate,
+                                            const void* w_up, long long ldw, const void* gate, const void* up, void* dx,
+                                            void* dw_gate, void* dw_up, long long m, int f, int k, int act, float beta1,
+                                            float beta2, int dtype, int out_dtype, void* workspace,
+                                            size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,154 @@
+"""RMS norm with the residual's addition and an 8-bit output, against formulas in 64 bits.
+
+Tolerances, derived before any run: the sum h + y is one fp32 addition, rounded to the type: exact.
+With n in 64 bits, the kernel's fp32 norm is within (cols / 32 + 40) 2^-24 + 2^-22 of it (a thread's
+32 squares or cols / 32 of a row, the joins, rsqrt and three products), its scale likewise; an 8-bit value is within half an
+e4m3 step of n / scale: 2^-4 of it, or 2^-10 below 2^-6, plus that error.  ``n`` in the type: one rounding more."""
+import math
+
+import pytest
+import torch
+
+import verace_v1_b200 as V
+from linear_util import HALF, tiny
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def data(rows, cols, dt, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(1000 * rows + cols + seed)
+    h = (torch.randn(rows, cols, device="cuda", generator=g) * (0.2 + 3 * torch.rand(rows, 1, device="cuda", generator=g))).to(dt)
+    y = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
+    norm = torch.nn.RMSNorm(cols, eps=1e-6, device="cuda", dtype=dt).requires_grad_(False)
+    norm.weight.copy_(1 + 0.3 * torch.randn(cols, device="cuda", generator=g))
+    return h, y, norm
+
+
+def check(h, norm, q, scale, n=None):
+    """q, scale (and n) of the rows h, which the norm (None: the quantiser) reads."""
+    x = h.double()
+    rel = 0.0
+    if norm is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + norm.eps).sqrt()
+        if norm.weight is not None:
+            x = x * norm.weight.double()
+        rel = (h.shape[-1] / 32 + 40) * 2.0 ** -24 + 2.0 ** -22
+    top = x.abs().amax(-1, keepdim=True).clamp(min=2.0 ** -100)
+    s = top / 448
+    assert q.dtype is torch.float8_e4m3fn and q.shape == h.shape
+    assert scale.dtype is torch.float32 and scale.shape == h.shape[:-1]
+    assert ((scale.double() - s[..., 0]).abs() <= (rel + 2.0 ** -22) * s[..., 0]).all()
+    v = x / s
+    off = (q.double() - v).abs()
+    assert (off <= torch.maximum(v.abs() * 2.0 ** -4, torch.full_like(v, 2.0 ** -10)) + (2 * rel + 2.0 ** -21) * v.abs()).all()
+    if n is not None:
+        e = HALF[h.dtype]
+        assert ((n.double() - x).abs() <= (rel + e * (1 + rel)) * x.abs() + tiny(h.dtype)).all()
+
+
+SHAPES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 1000), (9, 1024), (4, 1025), (3, 1032), (2, 4096), (3, 4097), (2, 5001),
+          (2, 16384), (1, 16385), (2, 20000), (1, 32768), (700, 256), (333, 4096)]
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("dt", TYPES)
+def test_norm_to_8_bits(rows, cols, dt):
+    h, y, norm = data(rows, cols, dt)
+    check(h, norm, *V.rmsnorm_fp8(h, norm))
+    check(h, norm, *V.rmsnorm_fp8(h, norm, return_norm=True))
+    check(h, None, *V.quantize_fp8(h))
+    want = (h.float() + y.float()).to(dt)
+    into = torch.full_like(h, math.nan)
+    before = h.clone()
+    q, s, n = V.add_rmsnorm_fp8(h, y, norm, out=into, return_norm=True)
+    assert torch.equal(into, want) and torch.equal(h, before)
+    check(want, norm, q, s, n)
+    q2, s2 = V.add_rmsnorm_fp8(h, y, norm)          # in place
+    assert torch.equal(h, want) and torch.equal(s, s2) and torch.equal(q.view(torch.uint8), q2.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_norm_without_weight_and_leading_dimensions(dt):
+    h, _, _ = data(24, 96, dt)
+    norm = torch.nn.RMSNorm(96, elementwise_affine=False, device="cuda")
+    q, s = V.rmsnorm_fp8(h.view(2, 3, 4, 96), norm)
+    assert q.shape == (2, 3, 4, 96) and s.shape == (2, 3, 4)
+    norm.eps = torch.finfo(dt).eps
+    check(h, norm, q.view(24, 96), s.view(24))
+
+
+@pytest.mark.parametrize("cols", [64, 100, 2048, 6000])
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_of_zeros_small_values_and_special_ones(cols, dt):
+    h, _, norm = data(6, cols, dt)
+    h[0] = 0
+    h[1] = 0
+    h[1, cols // 2] = torch.finfo(dt).smallest_normal
+    h[3, 3] = math.nan
+    h[4, 5] = math.inf
+    q, s = V.quantize_fp8(h)
+    assert not q[0].float().any() and abs(float(s[0]) * 448 * 2.0 ** 100 - 1) <= 2.0 ** -23   # (one division in fp32)
+    ok = [0, 1, 2, 5]
+    check(h[ok], None, q.view(torch.uint8)[ok].view(torch.float8_e4m3fn), s[ok])
+    assert s[3].isnan() and q[3].float().isnan().all()          # a NaN takes its row
+    assert s[4].isinf() and q[4].float()[5].isnan()
+    q, s = V.rmsnorm_fp8(h, norm)
+    check(h[ok], norm, q.view(torch.uint8)[ok].view(torch.float8_e4m3fn), s[ok])
+    assert s[3].isnan() and s[4].isnan()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_misaligned_rows_and_aliases(dt):
+    flat = torch.randn(3 * 1024 + 1, device="cuda").to(dt)
+    h = flat[1:].view(3, 1024)
+    a, b = V.quantize_fp8(h), V.quantize_fp8(h.clone())
+    assert torch.equal(a[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(a[1], b[1])
+    t = h.t()                       # not contiguous
+    a, b = V.quantize_fp8(t), V.quantize_fp8(t.contiguous())
+    assert torch.equal(a[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(a[1], b[1])
+    _, _, norm = data(3, 1024, dt)
+    y = torch.randn(3, 1024, device="cuda").to(dt)
+    want = V.add_rmsnorm_fp8(h, y, norm, out=torch.empty_like(y))
+    got = V.add_rmsnorm_fp8(h, y, norm, out=y)      # the sum in y's place
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+    twice = V.add_rmsnorm_fp8(h, h, norm, out=torch.empty_like(y))
+    check((h.float() + h.float()).to(dt), norm, *twice)
+
+
+def test_empty_and_refusals():
+    norm = torch.nn.RMSNorm(64, device="cuda", dtype=torch.bfloat16).requires_grad_(False)
+    q, s = V.rmsnorm_fp8(torch.zeros(0, 64, device="cuda", dtype=torch.bfloat16), norm)
+    assert q.shape == (0, 64) and s.shape == (0,)
+    x = torch.zeros(2, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="match"):
+        V.add_rmsnorm_fp8(x, x[:1], norm)
+    with pytest.raises(AssertionError, match="contiguous"):
+        V.add_rmsnorm_fp8(x, x, norm, out=torch.zeros(64, 2, device="cuda", dtype=torch.bfloat16).t())
+    with pytest.raises(ValueError, match="inputs"):
+        V.quantize_fp8(x.double())
+    with pytest.raises(AssertionError):
+        V.rmsnorm_fp8(x.float(), norm)
+    with pytest.raises(RuntimeError, match="32768"):
+        V.quantize_fp8(torch.zeros(1, 32769, device="cuda"))
+    with pytest.raises(RuntimeError, match="no_grad"):
+        V.quantize_fp8(x.clone().requires_grad_())
+    with pytest.raises(AssertionError):
+        V.quantize_fp8(torch.zeros(3, 0, device="cuda"))
+
+
+def test_captured_and_on_another_stream():
+    h, y, norm = data(33, 2048, torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = V.add_rmsnorm_fp8(h, y, norm, out=torch.empty_like(h))
+    torch.cuda.current_stream().wait_stream(side)
+    into, hh = torch.empty_like(h), h.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = V.add_rmsnorm_fp8(hh, y, norm, out=into)
+    hh.copy_(h)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])

@@ -22,6 +22,10 @@ Public surface (mirrors the reference package verace_v1 for this path):
     process_logits, sample_logits                    (penalties, biases, grammar masks; the
                                                      choice of a token)
     generate                                         (the generation loop over VeraceV1Model)
+    fused_linear, gated_linear                       (dense products with bias, activation, gate and
+                                                     residual in their epilogues; differentiable)
+    rmsnorm_fp8, add_rmsnorm_fp8, quantize_fp8       (rows in 8 bits with scales, which both
+                                                     products take)
 The kernels live in libverace_b200.so (C ABI: include/verace_b200.h), built by
 build.py; nothing here falls back to CPU or Python arithmetic.
 """
@@ -37,6 +41,7 @@ from .config import VeraceV1Config
 from .layer import AdaptiveCognitiveDepthEngine, VeraceV1Layer
 from .model import VeraceV1Model
 from .int4 import Int4Linear, dequantize_int4, int4_linear, quantize_int4, quantize_model_int4
+from .linear import add_rmsnorm_fp8, fused_linear, gated_linear, quantize_fp8, rmsnorm_fp8
 from .sampling import process_logits, sample_logits
 from .generate import generate
 
@@ -49,5 +54,6 @@ __all__ = [
     "ManifoldContinuousMoE", "SiTUGLU", "launch_mcmoe_projection", "launch_mcmoe_triton_projection",
     "launch_mcmoe_route", "situ_glu", "VeraceV1Config", "VeraceV1Layer", "AdaptiveCognitiveDepthEngine",
     "VeraceV1Model", "Int4Linear", "dequantize_int4", "int4_linear", "quantize_int4", "process_logits",
-    "sample_logits", "quantize_model_int4", "generate",
+    "sample_logits", "quantize_model_int4", "generate", "fused_linear", "gated_linear", "rmsnorm_fp8",
+    "add_rmsnorm_fp8", "quantize_fp8",
 ]

@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(HERE, "libverace_b200.so")
 HEADER_PATH = os.path.join(os.path.dirname(HERE), "include", "verace_b200.h")
 
 VERACE_OK = 0
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 
 _c_size = ctypes.c_size_t
 _p = ctypes.c_void_p
@@ -58,6 +58,20 @@ _SIGNATURES = {
                                                                                  ctypes.c_longlong, _p]),
     "verace_sample": (_i, [_p, ctypes.c_longlong, _p, ctypes.c_longlong, _i, _i, _i, _p, ctypes.c_float, _p, _i]
                       + [_p, ctypes.c_float] * 2 + [_p, _p, _p]),
+    "verace_rmsnorm_fp8": (_i, [_p] * 4 + [ctypes.c_float, _i] + [_p] * 3 + [ctypes.c_longlong, _i, _i, _p]),
+    "verace_linear_workspace": (_c_size, [ctypes.c_longlong, _i, _i, _i]),
+    "verace_linear": (_i, [_p, ctypes.c_longlong, _p, _p, ctypes.c_longlong, _p, _p, _p, ctypes.c_longlong, _p, _p,
+                           ctypes.c_longlong] + [_i] * 5 + [_p, _c_size, _p]),
+    "verace_linear_backward_workspace": (_c_size, [ctypes.c_longlong, _i, _i, _i]),
+    "verace_linear_backward": (_i, [_p, _p, ctypes.c_longlong, _p, ctypes.c_longlong, _p, _p, _p, _p, ctypes.c_longlong]
+                               + [_i] * 5 + [_p, _c_size, _p]),
+    "verace_gated_linear_workspace": (_c_size, [ctypes.c_longlong, _i, _i, _i]),
+    "verace_gated_linear": (_i, [_p, ctypes.c_longlong, _p, _p, _p, ctypes.c_longlong] + [_p] * 5
+                            + [ctypes.c_longlong, _i, _i, _i, ctypes.c_float, ctypes.c_float, _i, _i, _p, _c_size, _p]),
+    "verace_gated_linear_backward_workspace": (_c_size, [ctypes.c_longlong, _i, _i, _i]),
+    "verace_gated_linear_backward": (_i, [_p, _p, ctypes.c_longlong, _p, _p, ctypes.c_longlong] + [_p] * 5
+                                     + [ctypes.c_longlong, _i, _i, _i, ctypes.c_float, ctypes.c_float, _i, _i, _p,
+                                        _c_size, _p]),
 }
 
 _lib = None

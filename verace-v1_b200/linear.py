@@ -1,0 +1,357 @@
+"""Dense products of the feed-forward sub-layer with their epilogues in one kernel
+(``verace_linear``, ``verace_gated_linear``), forward and backward, and the RMS norm whose
+output is in 8 bits (``verace_rmsnorm_fp8``), which feeds them.
+
+The reference runs these as separate steps: ``torch.nn.Linear`` products, the SiTU-GLU
+activation (verace_v1/modules/activations.py:8-31), the down projection and the residual's
+addition (verace_v1/modules/mcmoe.py:85-120, backbone.py:96-99).
+
+* ``fused_linear``:  act(x Wᵀ + bias) + residual
+* ``gated_linear``:  act(x Wgᵀ) up(x Wuᵀ); "situ": beta1 tanh(g / beta1) sigmoid(g) beta2 tanh(u / beta2)
+* ``rmsnorm_fp8``, ``add_rmsnorm_fp8``, ``quantize_fp8``: rows as e4m3 values and one fp32 scale each
+
+fp32, bf16 and fp16 operands have gradients; e4m3 operands (with scales) are for inference.
+"""
+import math
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from ._launch import current, raw_stream
+from ._lib import E4M3, F32, check, lib
+from .int4 import _require_no_grad
+from .kernels import _DTYPE, _norm_args
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "situ": 5}
+FP8 = torch.float8_e4m3fn
+_CODE = {**_DTYPE, FP8: E4M3}
+_ALIGN = {torch.float32: 1, torch.bfloat16: 8, torch.float16: 8, FP8: 16}   # values in 16 bytes (fp32 rows: any)
+
+
+def _rows(t: torch.Tensor, m: int, k: int) -> Tuple[torch.Tensor, int]:
+    """t as [m, k] whose rows the kernels can address, and its row stride; copied where it has to be."""
+    if t.dim() != 2:
+        t = t.reshape(m, k)
+    a = _ALIGN[t.dtype]
+    ld = t.stride(0) if m > 1 else -(-k // a) * a
+    if (k > 1 and t.stride(1) != 1) or ld < k or ld % a or (a > 1 and t.data_ptr() % 16):
+        ld = -(-k // a) * a
+        c = torch.empty((m, ld), dtype=t.dtype, device=t.device)
+        if a == 16:     # (copied as bytes)
+            c.view(torch.uint8)[:, :k].copy_(t.view(torch.uint8))
+        else:
+            c[:, :k].copy_(t)
+        t = c
+    return t, ld
+
+
+def _vector(t: Optional[torch.Tensor], n: int, dtype: torch.dtype, device, what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    assert t.dtype is dtype and t.numel() == n and t.device == device, f"{what} must hold {n} values of {dtype} on {device}"
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _checked(who, x, weights, scales, activation, allowed, out_dtype, default):
+    """Checks what both products take; returns (k, out dtype)."""
+    assert x.is_cuda, "This kernel requires CUDA tensors"
+    dt = x.dtype
+    if dt not in _CODE:
+        raise ValueError(f"{who}: {dt} inputs (expected fp32, bf16, fp16 or float8_e4m3fn)")
+    if activation not in allowed:
+        raise ValueError(f"{who}: activation {activation!r} (expected one of {allowed})")
+    assert x.dim() >= 1, "x must have at least one dimension"
+    k = x.shape[-1]
+    for w in weights:
+        assert w.dtype is dt and w.dim() == 2 and w.shape == (weights[0].shape[0], k) and w.device == x.device, \
+            f"{who}: the weights must be [n, {k}] in x's dtype, on its device"
+    eight = dt is FP8
+    if any((s is not None) != eight for s in scales):
+        raise ValueError(f"{who}: scales go with float8_e4m3fn operands, one for x and one for each weight")
+    if out_dtype is None:
+        out_dtype = default if eight else dt
+    if out_dtype not in _DTYPE or not (eight or out_dtype is dt or out_dtype is torch.float32):
+        raise ValueError(f"{who}: out_dtype {out_dtype} for {dt} inputs")
+    return k, out_dtype
+
+
+def _workspace(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------- act(x Wᵀ + bias) + residual
+def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
+    dev = x2.device
+    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    pre = torch.empty_like(y) if want_pre else None
+    L = lib()
+    code = _CODE[x2.dtype]
+    nws = L.verace_linear_workspace(m, n, k, code)
+    ws = _workspace(nws, dev)
+    rc = L.verace_linear(x2.data_ptr(), ldx, _p(sx), w2.data_ptr(), ldw, _p(sw), _p(bias), _p(res), ldr, y.data_ptr(),
+                         _p(pre), m, n, k, act, code, _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index))
+    if rc:
+        check(rc, "verace_linear")
+    return y, pre
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, out_dtype, m, n, k):
+        x2, ldx = _rows(x, m, k)
+        w2, ldw = _rows(weight, n, k)
+        b = _vector(bias, n, x.dtype, x.device, "bias")
+        res, ldr = _residual_rows(residual, m, n)
+        y, pre = _linear(x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
+        ctx.save_for_backward(x2, w2, pre)
+        ctx.sizes = (x.shape, m, n, k, ldx, ldw, act, out_dtype, None if bias is None else bias.shape)
+        return y.view(x.shape[:-1] + (n,))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d):
+        x2, w2, pre = ctx.saved_tensors
+        shape, m, n, k, ldx, ldw, act, out_dtype, bias_shape = ctx.sizes
+        want = ctx.needs_input_grad
+        dev, dt = x2.device, x2.dtype
+        dx = torch.empty((m, k), dtype=dt, device=dev) if want[0] else None
+        dw = torch.empty((n, k), dtype=dt, device=dev) if want[1] else None
+        db = torch.empty(bias_shape, dtype=dt, device=dev) if want[2] else None
+        if want[0] or want[1] or want[2]:
+            d2 = d.contiguous()
+            L = lib()
+            with torch.cuda.device(dev):
+                nws = L.verace_linear_backward_workspace(m, n, k, _DTYPE[dt])
+                ws = _workspace(nws, dev)
+                check(L.verace_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(pre), _p(dx),
+                                               _p(dw), _p(db), m, n, k, act, _DTYPE[dt], _DTYPE[out_dtype], _p(ws), nws,
+                                               raw_stream(dev.index)), "verace_linear_backward")
+        return (None if dx is None else dx.view(shape), dw, db, d if want[3] else None) + (None,) * 5
+
+
+def _residual_rows(residual, m, n):
+    if residual is None:
+        return None, n
+    r = residual if residual.dim() == 2 else residual.reshape(m, n)
+    if (n > 1 and r.stride(1) != 1) or (m > 1 and r.stride(0) < n):
+        r = r.contiguous()
+    return r, r.stride(0) if m > 1 else n
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                 activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+                 x_scale: Optional[torch.Tensor] = None, w_scale: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x weightᵀ + bias) + residual in one kernel: x [..., k], weight [n, k], bias [n] (x's dtype),
+    residual [..., n] (the output's dtype); activation None, "relu", "silu", "gelu" (by erf) or "gelu_tanh".
+    The output has x's dtype or, with ``out_dtype=torch.float32``, fp32; sums are fp32, rounded once.
+
+    With float8_e4m3fn x and weight, ``x_scale`` (one fp32 value a row of x) and ``w_scale`` [n] multiply
+    them; the output is then fp32, bf16 or fp16 (``out_dtype``, else the residual's dtype, else bf16), the bias of
+    the same dtype.  The other types are differentiable in x, weight, bias and residual (once)."""
+    dev = x.device
+    if x.is_cuda and dev.index != current():
+        with torch.cuda.device(dev):
+            return fused_linear(x, weight, bias, activation=activation, residual=residual, x_scale=x_scale,
+                                w_scale=w_scale, out_dtype=out_dtype)
+    default = torch.bfloat16 if residual is None else residual.dtype
+    k, odt = _checked("fused_linear", x, (weight,), (x_scale, w_scale), activation,
+                      (None, "relu", "silu", "gelu", "gelu_tanh"), out_dtype, default)
+    n, lead = weight.shape[0], x.shape[:-1]
+    m = math.prod(lead)
+    assert residual is None or (residual.shape == lead + (n,) and residual.dtype is odt and residual.device == dev), \
+        f"residual must be {tuple(lead) + (n,)} in {odt}, on x's device"
+    act = ACTIVATIONS[activation]
+    eight = x.dtype is FP8
+    bias_dtype = odt if eight else x.dtype
+    assert bias is None or (bias.dtype is bias_dtype and bias.shape == (n,) and bias.device == dev), \
+        f"bias must be [{n}] in {bias_dtype}, on x's device"
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        if eight:
+            raise RuntimeError("fused_linear runs 8-bit operands for inference (no autograd path): "
+                               "call it under torch.no_grad()")
+        return _FusedLinear.apply(x, weight, bias, residual, act, odt, m, n, k)
+    x2, ldx = _rows(x, m, k)
+    w2, ldw = _rows(weight, n, k)
+    sx = sw = None
+    if eight:
+        sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
+        sw = _vector(w_scale, n, torch.float32, dev, "w_scale")
+    res, ldr = _residual_rows(residual, m, n)
+    y, _ = _linear(x2, ldx, sx, w2, ldw, sw, _vector(bias, n, bias_dtype, dev, "bias"), res, ldr, m, n, k, act, odt, False)
+    return y if x.dim() == 2 else y.view(lead + (n,))
+
+
+# ---------------------------------------------------------------------------- act(x Wgᵀ) up(x Wuᵀ)
+def _gate_rows(w_gate, w_up, f, k):
+    g2, ldg = _rows(w_gate, f, k)
+    u2, ldu = _rows(w_up, f, k)
+    if ldg != ldu:      # (two row strides: one of them, or both, become dense)
+        a = _ALIGN[g2.dtype]
+        ld = -(-k // a) * a
+        if ldg != ld:
+            g2, ldg = _rows(w_gate.contiguous(), f, k)
+        if ldu != ld:
+            u2, ldu = _rows(w_up.contiguous(), f, k)
+    return g2, u2, ldg
+
+
+def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
+    dev = x2.device
+    h = torch.empty((m, f), dtype=out_dtype, device=dev)
+    gate, up = (torch.empty_like(h), torch.empty_like(h)) if want_pre else (None, None)
+    L = lib()
+    code = _CODE[x2.dtype]
+    nws = L.verace_gated_linear_workspace(m, f, k, code)
+    ws = _workspace(nws, dev)
+    rc = L.verace_gated_linear(x2.data_ptr(), ldx, _p(sx), g2.data_ptr(), u2.data_ptr(), ldw, _p(sg), _p(su), h.data_ptr(),
+                               _p(gate), _p(up), m, f, k, act, b1, b2, code, _DTYPE[out_dtype], _p(ws), nws,
+                               raw_stream(dev.index))
+    if rc:
+        check(rc, "verace_gated_linear")
+    return h, gate, up
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, act, b1, b2, out_dtype, m, f, k):
+        x2, ldx = _rows(x, m, k)
+        g2, u2, ldw = _gate_rows(w_gate, w_up, f, k)
+        h, gate, up = _gated(x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
+        ctx.save_for_backward(x2, g2, u2, gate, up)
+        ctx.sizes = (x.shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype)
+        return h.view(x.shape[:-1] + (f,))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d):
+        x2, g2, u2, gate, up = ctx.saved_tensors
+        shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype = ctx.sizes
+        want = ctx.needs_input_grad
+        dev, dt = x2.device, x2.dtype
+        dx = torch.empty((m, k), dtype=dt, device=dev) if want[0] else None
+        dg = torch.empty((f, k), dtype=dt, device=dev) if want[1] else None
+        du = torch.empty((f, k), dtype=dt, device=dev) if want[2] else None
+        d2 = d.contiguous()
+        L = lib()
+        with torch.cuda.device(dev):
+            nws = L.verace_gated_linear_backward_workspace(m, f, k, _DTYPE[dt])
+            ws = _workspace(nws, dev)
+            check(L.verace_gated_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, g2.data_ptr(), u2.data_ptr(), ldw,
+                                                 gate.data_ptr(), up.data_ptr(), _p(dx), _p(dg), _p(du), m, f, k, act, b1,
+                                                 b2, _DTYPE[dt], _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index)),
+                  "verace_gated_linear_backward")
+        return (None if dx is None else dx.view(shape), dg, du) + (None,) * 7
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation: str = "situ",
+                 beta1: float = 4.0, beta2: float = 25.0, x_scale: Optional[torch.Tensor] = None,
+                 gate_scale: Optional[torch.Tensor] = None, up_scale: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(g) up(u) with g = x w_gateᵀ and u = x w_upᵀ in one kernel: x [..., k], w_gate and w_up [f, k] ->
+    [..., f].  activation "situ" (``SiTUGLU``: beta1 tanh(g / beta1) sigmoid(g) beta2 tanh(u / beta2)), or "silu",
+    "gelu" (by erf), "gelu_tanh" or "relu" of g, times u.  g and u stay in fp32; the result is rounded once, to
+    x's dtype or, with ``out_dtype=torch.float32``, not at all.
+
+    With float8_e4m3fn operands, ``x_scale`` (one fp32 value a row of x), ``gate_scale`` and ``up_scale`` [f]
+    multiply them, and the output is fp32, bf16 (the default) or fp16.  The other types are differentiable in x, w_gate
+    and w_up (once); the pass keeps g and u, in the output's dtype, for the backward."""
+    dev = x.device
+    if x.is_cuda and dev.index != current():
+        with torch.cuda.device(dev):
+            return gated_linear(x, w_gate, w_up, activation=activation, beta1=beta1, beta2=beta2, x_scale=x_scale,
+                                gate_scale=gate_scale, up_scale=up_scale, out_dtype=out_dtype)
+    k, odt = _checked("gated_linear", x, (w_gate, w_up), (x_scale, gate_scale, up_scale), activation,
+                      ("situ", "silu", "gelu", "gelu_tanh", "relu"), out_dtype, torch.bfloat16)
+    if activation == "situ" and not (beta1 and beta2):
+        raise ValueError(f"gated_linear: beta1 {beta1}, beta2 {beta2} (expected anything but 0)")
+    f, lead = w_gate.shape[0], x.shape[:-1]
+    m = math.prod(lead)
+    act = ACTIVATIONS[activation]
+    eight = x.dtype is FP8
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        if eight:
+            raise RuntimeError("gated_linear runs 8-bit operands for inference (no autograd path): "
+                               "call it under torch.no_grad()")
+        return _GatedLinear.apply(x, w_gate, w_up, act, float(beta1), float(beta2), odt, m, f, k)
+    x2, ldx = _rows(x, m, k)
+    g2, u2, ldw = _gate_rows(w_gate, w_up, f, k)
+    sx = sg = su = None
+    if eight:
+        sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
+        sg = _vector(gate_scale, f, torch.float32, dev, "gate_scale")
+        su = _vector(up_scale, f, torch.float32, dev, "up_scale")
+    h, _, _ = _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, beta1, beta2, odt, False)
+    return h if x.dim() == 2 else h.view(lead + (f,))
+
+
+# ---------------------------------------------------------------------------- rows in 8 bits
+def _to_fp8(who, h, y, sum_out, wp, eps, norm, return_norm):
+    dev = h.device
+    cols = h.shape[-1]
+    rows = h.numel() // cols if cols else 0
+    q = torch.empty(h.shape, dtype=FP8, device=dev)
+    scale = torch.empty(h.shape[:-1], dtype=torch.float32, device=dev)
+    n = torch.empty_like(h) if return_norm else None
+    rc = lib().verace_rmsnorm_fp8(h.data_ptr(), _p(y), _p(sum_out), wp, eps, norm, q.data_ptr(), scale.data_ptr(), _p(n),
+                                  rows, cols, _DTYPE[h.dtype], raw_stream(dev.index))
+    if rc:
+        check(rc, who)
+    return (q, scale, n) if return_norm else (q, scale)
+
+
+def _fp8_input(who, x):
+    assert x.is_cuda, "This kernel requires CUDA tensors"
+    if x.requires_grad:
+        _require_no_grad(x, who)
+    if x.dtype not in _DTYPE:
+        raise ValueError(f"{who}: {x.dtype} inputs (expected fp32, bf16 or fp16)")
+    assert x.dim() >= 1 and x.shape[-1] > 0, f"{who}: rows of at least one value"
+
+
+def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rows of x [..., k] (fp32, bf16 or fp16; k up to 32768) as (float8_e4m3fn [..., k], fp32 scales [...]):
+    scale = max(max |x|, 2^-100) / 448 of the row, values rounded to the nearest."""
+    _fp8_input("quantize_fp8", x)
+    if x.device.index != current():
+        with torch.cuda.device(x.device):
+            return quantize_fp8(x)
+    return _to_fp8("quantize_fp8", x.detach().contiguous(), None, None, None, 0.0, 0, False)
+
+
+def rmsnorm_fp8(x: torch.Tensor, norm: nn.RMSNorm, *, return_norm: bool = False):
+    """``norm`` (a torch.nn.RMSNorm over the last dimension) applied to x, its rows in 8 bits as
+    ``quantize_fp8`` gives them: (q, scale), and with ``return_norm`` the norm's output in x's dtype as well.
+    The values are not rounded to x's dtype before they are rounded to 8 bits."""
+    _fp8_input("rmsnorm_fp8", x)
+    if x.device.index != current():
+        with torch.cuda.device(x.device):
+            return rmsnorm_fp8(x, norm, return_norm=return_norm)
+    x = x.contiguous()
+    w, eps = _norm_args(norm, x)
+    return _to_fp8("rmsnorm_fp8", x, None, None, w or None, eps, 1, return_norm)
+
+
+def add_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, norm: nn.RMSNorm, *, out: Optional[torch.Tensor] = None,
+                    return_norm: bool = False):
+    """A block's residual step ahead of 8-bit products, in one pass: h <- h + y in place (or into ``out``),
+    then ``rmsnorm_fp8`` of the sum: (q, scale), and with ``return_norm`` the norm's output as well."""
+    _fp8_input("add_rmsnorm_fp8", h)
+    if h.device.index != current():
+        with torch.cuda.device(h.device):
+            return add_rmsnorm_fp8(h, y, norm, out=out, return_norm=return_norm)
+    if y.requires_grad:
+        _require_no_grad(y, "add_rmsnorm_fp8")
+    out = h if out is None else out
+    assert y.shape == h.shape and y.dtype is h.dtype and y.device == h.device, "h and y must match"
+    assert out.shape == h.shape and out.dtype is h.dtype and out.device == h.device and out.is_contiguous(), \
+        "the sum goes to a contiguous tensor of h's shape, dtype and device"
+    w, eps = _norm_args(norm, h)
+    return _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, w or None, eps, 1, return_norm)
