@@ -2,156 +2,241 @@
 //     linear:  out = act(x W^T + bias) + residual
 //     gated:   out = act(x Wg^T) up(x Wu^T)
 // fp32, bf16 or fp16, and e4m3 operands with a scale for each row.  Sums are fp32, outputs are
-// rounded once.  Formulas of the activations: linear.cuh.
+// rounded once.  Formulas of the activations: linear.cuh; the products: linear_large.cu.
 //
 // Backward: p = d act'(pre) (gated: dg and du) in one pass over the saved sums, then
-// dx = p W (dg Wg + du Wu), dW = p^T x, and the bias gradient as column sums in a fixed order.
-#include "linear.cuh"
-
-#include <cuda_fp8.h>
+// dx = p W (dg Wg + du Wu) and dW = p^T x.  W, p and x are read there as they are stored; no
+// operand is transposed in memory.  The bias gradient is summed in the pass, in fp32 and in a
+// fixed order (128 rows at a time, then the partial sums).
+//
+// fp32 operands are split into three bf16 parts first (x = h + m + l, 24 bits), and the product
+// runs over the six pairs of parts down to 2^-24 of the largest (hh, hm, mh, hl, mm, lh).
+#include "linear_tc.cuh"
 
 namespace verace {
 namespace {
 
 using namespace lin;
 
+// ------------------------------------------------------------------ operands in memory
 template <typename T>
-__device__ __forceinline__ float val(T x) { return to_f32(x); }
-template <>
-__device__ __forceinline__ float val<__nv_fp8_e4m3>(__nv_fp8_e4m3 x) { return float(x); }
+constexpr bool split_v = sizeof(T) == 4;      // fp32: three bf16 parts
+template <typename T>
+using Part = std::conditional_t<split_v<T>, __nv_bfloat16, T>;
 
-// ------------------------------------------------------------------ simple product
-// out(m, n) = sum over `pairs` and k of a(m, k) b(n, k): 64 x 64 tiles, 4 x 4 a thread, through
-// shared memory.  GATED: b[0] and b[1] give two sums of one row and column.
-struct SimpleArgs {
-  const void *a[2], *b[2];
-  long long sam, sak, sbn, sbk;
-  long long M, N, K;
-  int pairs;
-  Epilogue e;
+// 8 values of a row from column c on (0 beyond the row's end)
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, long long c, long long cols, bool vec, float (&v)[8]) {
+  if (vec) {        // (cols is a multiple of 8)
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(row + c)[0], b = reinterpret_cast<const float4*>(row + c)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      unpack8<T>(*reinterpret_cast<const uint4*>(row + c), v);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
+  }
+}
+// 8 values as an operand of the products: rounded to T, or split into three parts `piece` apart
+template <typename T>
+__device__ __forceinline__ void store_operand(Part<T>* o, long long piece, const float (&v)[8]) {
+  if constexpr (split_v<T>) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = v[j];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint4 w = pack8<__nv_bfloat16>(r);
+      *reinterpret_cast<uint4*>(o + i * piece) = w;
+      float h[8];
+      unpack8<__nv_bfloat16>(w, h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] -= h[j];
+    }
+  } else {
+    *reinterpret_cast<uint4*>(o) = pack8<T>(v);
+  }
+}
+
+// src [rows, cols] fp32 -> three parts [3][rows][ld], ld = cols rounded up to 8
+__global__ void __launch_bounds__(256) split_rows(const float* __restrict__ src, long long ld_src, long long rows,
+                                                  long long cols, bool vec, __nv_bfloat16* __restrict__ dst, long long ld) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long row = i / (ld / 8), c = i % (ld / 8) * 8;
+  if (row >= rows) return;
+  float v[8];
+  load8<float>(src + row * ld_src, c, cols, vec, v);
+  store_operand<float>(dst + row * ld + c, rows * ld, v);
+}
+
+long long padded(long long cols) { return (cols + 7) / 8 * 8; }
+// bytes of an operand that a pass writes
+size_t operand_bytes(long long rows, long long cols, int type) {
+  return align_up((size_t)rows * padded(cols) * (type == VERACE_F32 ? 6 : 2), 256);
+}
+Mat operand_at(void* p, long long rows, long long cols, int type) {
+  const long long ld = padded(cols);
+  return Mat{p, rows, cols, ld, type == VERACE_F32 ? 3 : 1, rows * ld};
+}
+
+// The workspace, taken from its start.
+struct Taker {
+  char* at;
+  explicit Taker(void* ws) : at((char*)align_up((size_t)ws, 256)) {}
+  void* take(size_t bytes) {
+    void* p = at;
+    at += align_up(bytes, 256);
+    return p;
+  }
 };
 
-__device__ __forceinline__ void finish_linear(const Epilogue& e, long long m, long long n, float v) {
-  if (e.row_scale) v *= e.row_scale[m] * e.col_scale[n];
-  if (e.bias) v += load_as(e.bias, n, e.bias_type);
-  if (e.pre) store_as(e.pre, m * e.ld + n, v, e.type);
-  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) { v = act_<decltype(act)::value, decltype(fast)::value>(v); });
-  if (e.residual) v += load_as(e.residual, m * e.ld_res + n, e.type);
-  store_as(e.out, m * e.ld + n, v, e.type);
-}
-__device__ __forceinline__ void finish_gated(const Epilogue& e, long long m, long long n, float g, float u) {
-  if (e.row_scale) {
-    g *= e.row_scale[m] * e.col_scale[n];
-    u *= e.row_scale[m] * e.up_scale[n];
+// An operand of the products from a user's matrix: as it is, or split into parts in the workspace.
+int operand(Mat* out, const void* p, long long ld, long long rows, long long cols, int type, Taker& ws, cudaStream_t st) {
+  if (type != VERACE_F32) {
+    *out = Mat{p, rows, cols, ld, 1, 0};
+    return VERACE_OK;
   }
-  if (e.pre) {
-    store_as(e.pre, m * e.ld + n, g, e.type);
-    store_as(e.pre_up, m * e.ld + n, u, e.type);
-  }
-  float v = 0.f;
-  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
-    v = gate_<decltype(act)::value, decltype(fast)::value>(g, u, e.b1, e.b2, e.r1, e.r2);
-  });
-  store_as(e.out, m * e.ld + n, v, e.type);
+  void* dst = ws.take(operand_bytes(rows, cols, type));
+  *out = operand_at(dst, rows, cols, type);
+  const long long threads = rows * (out->ld / 8);
+  VERACE_REQUIRE((threads + 255) / 256 < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld operand is too large", rows,
+                 cols);
+  const bool vec = cols % 8 == 0 && ld % 4 == 0 && (size_t)p % 16 == 0;
+  split_rows<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>((const float*)p, ld, rows, cols, vec, (__nv_bfloat16*)dst,
+                                                              out->ld);
+  return check_launch("split_rows");
 }
 
-template <typename T, bool GATED>
-__global__ void __launch_bounds__(256) simple_product(SimpleArgs p) {
-  __shared__ float sa[16][65], sb[GATED ? 2 : 1][16][65];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const long long n0 = (long long)blockIdx.x * 64, m0 = (long long)blockIdx.y * 64;
-  float acc[GATED ? 2 : 1][4][4] = {};
-  for (int pair = 0; pair < (GATED ? 1 : p.pairs); ++pair) {
-    const T* a = static_cast<const T*>(p.a[pair]);
-    for (long long k0 = 0; k0 < p.K; k0 += 16) {
-      for (int i = tid; i < 1024; i += 256) {
-        // neighbouring threads along the contiguous direction
-        const int km = p.sak == 1 ? i & 15 : i >> 6, r = p.sak == 1 ? i >> 4 : i & 63;
-        const bool in = m0 + r < p.M && k0 + km < p.K;
-        sa[km][r] = in ? val(a[(m0 + r) * p.sam + (k0 + km) * p.sak]) : 0.f;
-        const int kn = p.sbk == 1 ? i & 15 : i >> 6, c = p.sbk == 1 ? i >> 4 : i & 63;
-        const bool inb = n0 + c < p.N && k0 + kn < p.K;
-#pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-          const T* b = static_cast<const T*>(p.b[GATED ? h : pair]);
-          sb[h][kn][c] = inb ? val(b[(n0 + c) * p.sbn + (k0 + kn) * p.sbk]) : 0.f;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-#pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[h][i][j] = fmaf(sa[k][ty * 4 + i], sb[h][k][tx + 16 * j], acc[h][i][j]);
-      __syncthreads();
-    }
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const long long m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-      if (m >= p.M || n >= p.N) continue;
-      if constexpr (GATED) finish_gated(p.e, m, n, acc[0][i][j], acc[1][i][j]);
-      else finish_linear(p.e, m, n, acc[0][i][j]);
-    }
+// ------------------------------------------------------------------ sums over nothing (k = 0)
+__global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= m * n) return;
+  const long long r = i / n, c = i % n;
+  float v = e.bias ? load_as(e.bias, c, e.bias_type) : 0.f;
+  if (e.pre) store_as(e.pre, r * e.ld + c, v, e.type);
+  if (e.pre_up) store_as(e.pre_up, r * e.ld + c, 0.f, e.type);
+  by_act(e.act, false, [&](auto act, auto fast) { v = act_<decltype(act)::value, false>(v); });
+  if (e.residual) v += load_as(e.residual, r * e.ld_res + c, e.type);
+  store_as(e.out, r * e.ld + c, v, e.type);
 }
 
-template <bool GATED>
-int run_simple(const SimpleArgs& p, int type, cudaStream_t st) {
+// The pairs of parts that make up an fp32 product, the smallest first (other types: one).
+void add_segments(Product& p, int a, int az, int b, int parts, int step) {
+  if (parts == 1) {
+    p.seg[p.segments++] = Segment{(unsigned char)a, (unsigned char)az, (unsigned char)b, 0};
+    return;
+  }
+  constexpr unsigned char A[6] = {2, 1, 0, 1, 0, 0}, B[6] = {0, 1, 2, 0, 1, 0};
+  for (int i = 0; i < 6; ++i)
+    p.seg[p.segments++] = Segment{(unsigned char)a, (unsigned char)(A[i] * step + az), (unsigned char)b, B[i]};
+}
+
+int run_product(Product& p, cudaStream_t st) {
   if (p.M == 0 || p.N == 0) return VERACE_OK;
-  const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64));
-  switch (type) {
-    case VERACE_F32: simple_product<float, GATED><<<grid, 256, 0, st>>>(p); break;
-    case VERACE_BF16: simple_product<__nv_bfloat16, GATED><<<grid, 256, 0, st>>>(p); break;
-    case VERACE_F16: simple_product<__half, GATED><<<grid, 256, 0, st>>>(p); break;
-    default: simple_product<__nv_fp8_e4m3, GATED><<<grid, 256, 0, st>>>(p); break;
+  if (p.K == 0) {
+    for (int z = 0; z < (p.nz > 1 ? p.nz : 1); ++z) {
+      Epilogue e = p.e;
+      if (p.nz > 1) e.out = p.out_z[z];
+      const long long blocks = (p.M * p.N + 255) / 256;
+      VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
+      empty_sum<<<(unsigned)blocks, 256, 0, st>>>(e, p.M, p.N);
+      if (int rc = check_launch("empty_sum")) return rc;
+    }
+    return VERACE_OK;
   }
-  return check_launch("simple_product");
+  if (p.type == VERACE_F32) p.type = VERACE_BF16;   // (the parts' type)
+  return product_large(p, st);
 }
 
 // ------------------------------------------------------------------ backward of the epilogues
-// p = d act'(pre), in the products' type (rounded once: it is an operand of dx and dW).
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) linear_slope(const O* __restrict__ d, const O* __restrict__ pre, T* __restrict__ p,
-                                                    long long total, int act) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const float z = pre ? to_f32(pre[i]) : 0.f;
-  float a, da = 1.f;
-  by_act(act, sizeof(O) == 2, [&](auto c, auto fast) { act_slope_<decltype(c)::value, decltype(fast)::value>(z, a, da); });
-  p[i] = from_f32<T>(to_f32(d[i]) * da);
-}
+// p = d act'(pre) as an operand of the products (rounded to the type of x, or in three parts), and its
+// column sums: a CTA takes 128 rows of 256 columns, a thread every eighth row of 8 columns.
+// Bound: bytes (d and pre read, p written).
+constexpr int CHUNK = 128;
+struct SlopeArgs {
+  const void *d, *pre, *up;
+  void *out;            // p, or dg; null: the sums alone
+  long long piece, second;   // between the parts, and from dg to du
+  float* partial;       // [chunks][n], or null
+  long long m, n, ld;   // ld: of out
+  int act, vec, colblocks;
+  float b1, b2, r1, r2;
+};
 
 template <typename T, typename O>
-__global__ void __launch_bounds__(256) gated_slope(const O* __restrict__ d, const O* __restrict__ gate,
-                                                   const O* __restrict__ up, T* __restrict__ dg, T* __restrict__ du,
-                                                   long long total, int act, float b1, float b2, float r1, float r2) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  float x = 0.f, y = 0.f;
-  by_act(act, sizeof(O) == 2, [&](auto c, auto fast) {
-    gate_slope_<decltype(c)::value, decltype(fast)::value>(to_f32(d[i]), to_f32(gate[i]), to_f32(up[i]), b1, b2, r1, r2, x, y);
-  });
-  dg[i] = from_f32<T>(x);
-  du[i] = from_f32<T>(y);
+__global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
+  __shared__ float part[8][256];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long chunk = blockIdx.x / a.colblocks, c = (blockIdx.x % a.colblocks) * 256LL + lane * 8;
+  const long long end = min(a.m, (chunk + 1) * CHUNK);
+  float sum[8] = {};
+  if (c < a.ld)
+    for (long long r = chunk * CHUNK + w; r < end; r += 8) {
+      float d[8], z[8];
+      load8<O>(static_cast<const O*>(a.d) + r * a.n, c, a.n, a.vec, d);
+      if (a.pre) {
+        load8<O>(static_cast<const O*>(a.pre) + r * a.n, c, a.n, a.vec, z);
+        by_act(a.act, sizeof(O) == 2, [&](auto k, auto fast) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float y, dy;
+            act_slope_<decltype(k)::value, decltype(fast)::value>(z[j], y, dy);
+            d[j] *= dy;
+          }
+        });
+      }
+      if (a.out) store_operand<T>(static_cast<Part<T>*>(a.out) + r * a.ld + c, a.piece, d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += d[j];
+    }
+  if (!a.partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[w][lane * 8 + j] = sum[j];
+  __syncthreads();
+  const long long n = (blockIdx.x % a.colblocks) * 256LL + threadIdx.x;
+  if (n >= a.n) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
+  a.partial[chunk * a.n + n] = s;
 }
 
-// dbias = the column sums of d act'(pre), rows in order
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) bias_sum(const O* __restrict__ d, const O* __restrict__ pre, T* __restrict__ out,
-                                                long long m, long long n, int act) {
+template <typename T>
+__global__ void __launch_bounds__(256) sum_chunks(const float* __restrict__ partial, long long chunks, long long n,
+                                                  T* __restrict__ out) {
   const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
   if (c >= n) return;
   float s = 0.f;
-  for (long long r = 0; r < m; ++r) {
-    const float z = pre ? to_f32(pre[r * n + c]) : 0.f;
-    float a, da = 1.f;
-    by_act(act, sizeof(O) == 2, [&](auto k, auto fast) { act_slope_<decltype(k)::value, decltype(fast)::value>(z, a, da); });
-    s += to_f32(d[r * n + c]) * da;
-  }
+  for (long long i = 0; i < chunks; ++i) s += partial[i * n + c];
   out[c] = from_f32<T>(s);
+}
+
+template <typename T, typename O>
+__global__ void __launch_bounds__(256) gated_slope(SlopeArgs a) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long chunk = blockIdx.x / a.colblocks, c = (blockIdx.x % a.colblocks) * 256LL + lane * 8;
+  const long long end = min(a.m, (chunk + 1) * CHUNK);
+  if (c >= a.ld) return;
+  for (long long r = chunk * CHUNK + w; r < end; r += 8) {
+    float d[8], g[8], u[8];
+    load8<O>(static_cast<const O*>(a.d) + r * a.n, c, a.n, a.vec, d);
+    load8<O>(static_cast<const O*>(a.pre) + r * a.n, c, a.n, a.vec, g);
+    load8<O>(static_cast<const O*>(a.up) + r * a.n, c, a.n, a.vec, u);
+    by_act(a.act, sizeof(O) == 2, [&](auto k, auto fast) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float x, y;
+        gate_slope_<decltype(k)::value, decltype(fast)::value>(d[j], g[j], u[j], a.b1, a.b2, a.r1, a.r2, x, y);
+        g[j] = x;
+        u[j] = y;
+      }
+    });
+    Part<T>* o = static_cast<Part<T>*>(a.out) + r * a.ld + c;
+    store_operand<T>(o, a.piece, g);
+    store_operand<T>(o + a.second, a.piece, u);
+  }
 }
 
 // ------------------------------------------------------------------ checks
@@ -179,6 +264,12 @@ int check_rows(const char* who, const char* name, const void* p, long long ld, l
   return VERACE_OK;
 }
 
+int check_workspace(const char* who, size_t need, const void* ws, size_t given) {
+  VERACE_REQUIRE(need == 0 || (ws && given >= need), VERACE_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given",
+                 who, need, ws ? given : (size_t)0);
+  return VERACE_OK;
+}
+
 // Calls f(T(), O()) for the products' type and the outputs' of a differentiable call.
 template <typename F>
 int by_types(int dtype, int out_dtype, F f) {
@@ -193,13 +284,25 @@ Epilogue plain_out(void* out, long long ld, int type) {
   return e;
 }
 
+long long chunks_of(long long m) { return (m + CHUNK - 1) / CHUNK; }
+
+int slope_grid(const SlopeArgs& a, unsigned* grid) {
+  const long long blocks = chunks_of(a.m) * a.colblocks;
+  VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", a.m, a.n);
+  *grid = (unsigned)blocks;
+  return VERACE_OK;
+}
+
 }  // namespace
 }  // namespace verace
 
 using namespace verace;
 using namespace verace::lin;
 
-extern "C" size_t verace_linear_workspace(long long m, int n, int k, int dtype) { return 0; }
+extern "C" size_t verace_linear_workspace(long long m, int n, int k, int dtype) {
+  if (m <= 0 || n <= 0 || k <= 0 || dtype != VERACE_F32) return 0;
+  return operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype) + 256;
+}
 
 extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
                              const float* w_scale, const void* bias, const void* residual, long long ld_res, void* out,
@@ -214,19 +317,26 @@ extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale,
   VERACE_REQUIRE(out && (dtype == VERACE_E4M3) == (x_scale != nullptr) && (dtype == VERACE_E4M3) == (w_scale != nullptr),
                  VERACE_ERR_INVALID, "%s: NULL out, or scales that do not go with the type", who);
   VERACE_REQUIRE(!residual || ld_res >= n, VERACE_ERR_INVALID, "%s: row stride %lld of the residual < %d", who, ld_res, n);
-  SimpleArgs p{};
-  p.a[0] = x; p.b[0] = w; p.sam = ldx; p.sak = 1; p.sbn = ldw; p.sbk = 1;
-  p.M = m; p.N = n; p.K = k; p.pairs = 1;
+  if ((rc = check_workspace(who, verace_linear_workspace(m, n, k, dtype), workspace, workspace_bytes))) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  Taker ws(workspace);
+  Product p{};
+  p.type = dtype; p.M = m; p.N = n; p.K = k; p.nz = 1;
   p.e = plain_out(out, n, out_dtype);
   p.e.row_scale = x_scale; p.e.col_scale = w_scale; p.e.bias = bias; p.e.residual = residual; p.e.ld_res = ld_res;
   p.e.pre = pre; p.e.act = act;
   p.e.bias_type = dtype == VERACE_E4M3 ? out_dtype : dtype;
-  return run_simple<false>(p, dtype, (cudaStream_t)stream);
+  if (k > 0 && ((rc = operand(&p.a[0], x, ldx, m, k, dtype, ws, st)) || (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st))))
+    return rc;
+  add_segments(p, 0, 0, 0, dtype == VERACE_F32 ? 3 : 1, 1);
+  return run_product(p, st);
 }
 
 extern "C" size_t verace_linear_backward_workspace(long long m, int n, int k, int dtype) {
   if (m <= 0 || n <= 0) return 0;
-  return align_up((size_t)m * n * size_of(dtype), 256) + 256;
+  size_t s = operand_bytes(m, n, dtype) + align_up((size_t)chunks_of(m) * n * 4, 256) + 256;
+  if (dtype == VERACE_F32 && k > 0) s += operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype);
+  return s;
 }
 
 extern "C" int verace_linear_backward(const void* dout, const void* x, long long ldx, const void* w, long long ldw,
@@ -236,43 +346,70 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
   int rc;
   if ((rc = check_sizes(who, m, n, k)) || (rc = check_types(who, dtype, out_dtype, false))) return rc;
   VERACE_REQUIRE(act >= VERACE_ACT_NONE && act <= VERACE_ACT_GELU_TANH, VERACE_ERR_INVALID, "%s: activation %d", who, act);
-  VERACE_REQUIRE(m == 0 || n == 0 || (dout && (pre || act == VERACE_ACT_NONE)), VERACE_ERR_INVALID, "%s: NULL pointer", who);
-  if (m > 0 && n > 0 && k > 0 && ((rc = check_rows(who, "x", x, ldx, k, dtype)) || (rc = check_rows(who, "w", w, ldw, k, dtype)))) return rc;
-  const size_t need = verace_linear_backward_workspace(m, n, k, dtype);
-  VERACE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VERACE_ERR_WORKSPACE,
-                 "%s: workspace of %zu bytes required, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  const bool any = m > 0 && n > 0;
+  VERACE_REQUIRE(!any || (dout && (pre || act == VERACE_ACT_NONE)), VERACE_ERR_INVALID, "%s: NULL pointer", who);
+  if (any && k > 0 && ((dw && (rc = check_rows(who, "x", x, ldx, k, dtype))) || (dx && (rc = check_rows(who, "w", w, ldw, k, dtype)))))
+    return rc;
+  if ((rc = check_workspace(who, verace_linear_backward_workspace(m, n, k, dtype), workspace, workspace_bytes))) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   return by_types(dtype, out_dtype, [&](auto t, auto o) -> int {
     using T = decltype(t);
     using O = decltype(o);
-    T* p = reinterpret_cast<T*>(align_up((size_t)workspace, 256));
-    const O* z = act == VERACE_ACT_NONE ? nullptr : (const O*)pre;
     int rc;
-    if (m > 0 && n > 0) {
-      linear_slope<T, O><<<(unsigned)((m * n + 255) / 256), 256, 0, st>>>((const O*)dout, z, p, m * n, act);
-      if ((rc = check_launch("linear_slope"))) return rc;
+    Taker ws(workspace);
+    Mat p{nullptr, m, n, padded(n), 1, 0};
+    SlopeArgs s{};
+    s.d = dout; s.pre = act == VERACE_ACT_NONE ? nullptr : pre; s.act = act;
+    s.m = m; s.n = n; s.ld = padded(n);
+    s.vec = n % 8 == 0 && ((size_t)dout | (size_t)s.pre) % 16 == 0;
+    s.colblocks = (int)((s.ld + 255) / 256);
+    if (any) {
+      if (!split_v<T> && std::is_same<T, O>::value && !s.pre && s.vec) {
+        p = Mat{dout, m, n, n, 1, 0};                   // d is p, and an operand as it is
+      } else if ((dx || dw) && k > 0) {
+        s.out = ws.take(operand_bytes(m, n, dtype));
+        p = operand_at(s.out, m, n, dtype);
+        s.piece = p.piece;
+      }
+      if (dbias) s.partial = (float*)ws.take((size_t)chunks_of(m) * n * 4);
+      if (s.out || s.partial) {
+        unsigned grid;
+        if ((rc = slope_grid(s, &grid))) return rc;
+        linear_slope<T, O><<<grid, 256, 0, st>>>(s);
+        if ((rc = check_launch("linear_slope"))) return rc;
+      }
     }
     if (dbias && n > 0) {
-      bias_sum<T, O><<<(n + 255) / 256, 256, 0, st>>>((const O*)dout, z, (T*)dbias, m, n, act);
-      if ((rc = check_launch("bias_sum"))) return rc;
+      sum_chunks<T><<<(n + 255) / 256, 256, 0, st>>>(s.partial, any ? chunks_of(m) : 0, n, (T*)dbias);
+      if ((rc = check_launch("sum_chunks"))) return rc;
     }
-    SimpleArgs a{};
-    a.pairs = 1;
-    if (dx) {
-      a.a[0] = p; a.sam = n; a.sak = 1; a.b[0] = w; a.sbn = 1; a.sbk = ldw;
-      a.M = m; a.N = k; a.K = n; a.e = plain_out(dx, k, dtype);
-      if ((rc = run_simple<false>(a, dtype, st))) return rc;
+    const int parts = split_v<T> ? 3 : 1;
+    if (dx && k > 0) {
+      Product d{};
+      d.type = dtype; d.M = m; d.N = k; d.K = n; d.nz = 1; d.b_mn = true;
+      d.e = plain_out(dx, k, dtype);
+      d.a[0] = p;
+      if (any && (rc = operand(&d.b[0], w, ldw, n, k, dtype, ws, st))) return rc;
+      add_segments(d, 0, 0, 0, parts, 1);
+      if ((rc = run_product(d, st))) return rc;
     }
-    if (dw) {
-      a.a[0] = p; a.sam = 1; a.sak = n; a.b[0] = x; a.sbn = 1; a.sbk = ldx;
-      a.M = n; a.N = k; a.K = m; a.e = plain_out(dw, k, dtype);
-      if ((rc = run_simple<false>(a, dtype, st))) return rc;
+    if (dw && k > 0) {
+      Product d{};
+      d.type = dtype; d.M = n; d.N = k; d.K = m; d.nz = 1; d.a_mn = d.b_mn = true;
+      d.e = plain_out(dw, k, dtype);
+      d.a[0] = p;
+      if (any && (rc = operand(&d.b[0], x, ldx, m, k, dtype, ws, st))) return rc;
+      add_segments(d, 0, 0, 0, parts, 1);
+      if ((rc = run_product(d, st))) return rc;
     }
     return VERACE_OK;
   });
 }
 
-extern "C" size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype) { return 0; }
+extern "C" size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype) {
+  if (m <= 0 || f <= 0 || k <= 0 || dtype != VERACE_F32) return 0;
+  return operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype) + 256;
+}
 
 extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_scale, const void* w_gate, const void* w_up,
                                    long long ldw, const float* gate_scale, const float* up_scale, void* out, void* gate,
@@ -291,19 +428,28 @@ extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_
   VERACE_REQUIRE(out && (gate != nullptr) == (up != nullptr) && eight == (x_scale != nullptr) &&
                      eight == (gate_scale != nullptr) && eight == (up_scale != nullptr),
                  VERACE_ERR_INVALID, "%s: NULL out, one of gate and up, or scales that do not go with the type", who);
-  SimpleArgs p{};
-  p.a[0] = x; p.b[0] = w_gate; p.b[1] = w_up; p.sam = ldx; p.sak = 1; p.sbn = ldw; p.sbk = 1;
-  p.M = m; p.N = f; p.K = k; p.pairs = 1;
+  if ((rc = check_workspace(who, verace_gated_linear_workspace(m, f, k, dtype), workspace, workspace_bytes))) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  Taker ws(workspace);
+  Product p{};
+  p.type = dtype; p.M = m; p.N = f; p.K = k; p.nz = 1; p.gated = true;
   p.e = plain_out(out, f, out_dtype);
   p.e.row_scale = x_scale; p.e.col_scale = gate_scale; p.e.up_scale = up_scale;
   p.e.pre = gate; p.e.pre_up = up; p.e.act = act;
   p.e.b1 = beta1; p.e.b2 = beta2; p.e.r1 = 1.f / beta1; p.e.r2 = 1.f / beta2;
-  return run_simple<true>(p, dtype, (cudaStream_t)stream);
+  if (k > 0 && ((rc = operand(&p.a[0], x, ldx, m, k, dtype, ws, st)) ||
+                (rc = operand(&p.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
+                (rc = operand(&p.b[1], w_up, ldw, f, k, dtype, ws, st))))
+    return rc;
+  add_segments(p, 0, 0, 0, dtype == VERACE_F32 ? 3 : 1, 1);
+  return run_product(p, st);
 }
 
 extern "C" size_t verace_gated_linear_backward_workspace(long long m, int f, int k, int dtype) {
   if (m <= 0 || f <= 0) return 0;
-  return 2 * align_up((size_t)m * f * size_of(dtype), 256) + 256;
+  size_t s = 2 * operand_bytes(m, f, dtype) + 256;
+  if (dtype == VERACE_F32 && k > 0) s += operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype);
+  return s;
 }
 
 extern "C" int verace_gated_linear_backward(const void* dout, const void* x, long long ldx, const void* w_gate,
@@ -316,42 +462,68 @@ extern "C" int verace_gated_linear_backward(const void* dout, const void* x, lon
   if ((rc = check_sizes(who, m, f, k)) || (rc = check_types(who, dtype, out_dtype, false))) return rc;
   VERACE_REQUIRE(act >= VERACE_ACT_RELU && act <= VERACE_ACT_SITU, VERACE_ERR_INVALID, "%s: activation %d", who, act);
   VERACE_REQUIRE(act != VERACE_ACT_SITU || (beta1 != 0.f && beta2 != 0.f), VERACE_ERR_INVALID, "%s: beta of 0", who);
-  VERACE_REQUIRE(m == 0 || f == 0 || (dout && gate && up), VERACE_ERR_INVALID, "%s: NULL pointer", who);
-  if (m > 0 && f > 0 && k > 0 &&
-      ((rc = check_rows(who, "x", x, ldx, k, dtype)) || (rc = check_rows(who, "w_gate", w_gate, ldw, k, dtype)) ||
-       (rc = check_rows(who, "w_up", w_up, ldw, k, dtype))))
+  const bool any = m > 0 && f > 0;
+  VERACE_REQUIRE(!any || (dout && gate && up), VERACE_ERR_INVALID, "%s: NULL pointer", who);
+  if (any && k > 0 &&
+      (((dw_gate || dw_up) && (rc = check_rows(who, "x", x, ldx, k, dtype))) ||
+       (dx && ((rc = check_rows(who, "w_gate", w_gate, ldw, k, dtype)) || (rc = check_rows(who, "w_up", w_up, ldw, k, dtype))))))
     return rc;
-  const size_t need = verace_gated_linear_backward_workspace(m, f, k, dtype);
-  VERACE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), VERACE_ERR_WORKSPACE,
-                 "%s: workspace of %zu bytes required, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  if ((rc = check_workspace(who, verace_gated_linear_backward_workspace(m, f, k, dtype), workspace, workspace_bytes))) return rc;
+  if (k == 0) return VERACE_OK;   // (the gradients are empty)
   cudaStream_t st = (cudaStream_t)stream;
   return by_types(dtype, out_dtype, [&](auto t, auto o) -> int {
     using T = decltype(t);
     using O = decltype(o);
-    T* dg = reinterpret_cast<T*>(align_up((size_t)workspace, 256));
-    T* du = reinterpret_cast<T*>(align_up((size_t)(dg + m * f), 256));
     int rc;
-    if (m > 0 && f > 0) {
-      gated_slope<T, O><<<(unsigned)((m * f + 255) / 256), 256, 0, st>>>((const O*)dout, (const O*)gate, (const O*)up, dg, du,
-                                                                      m * f, act, beta1, beta2, 1.f / beta1, 1.f / beta2);
+    Taker ws(workspace);
+    // [part][gate, up][m][f]
+    Mat p{nullptr, m, f, padded(f), 1, 0};
+    if (any) {
+      const long long one = m * padded(f), parts = split_v<T> ? 3 : 1;
+      void* out = ws.take(2 * operand_bytes(m, f, dtype));
+      p = Mat{out, m, f, padded(f), (int)(2 * parts), one};
+      SlopeArgs s{};
+      s.d = dout; s.pre = gate; s.up = up; s.out = out; s.piece = 2 * one; s.second = one;
+      s.m = m; s.n = f; s.ld = padded(f); s.act = act;
+      s.vec = f % 8 == 0 && ((size_t)dout | (size_t)gate | (size_t)up) % 16 == 0;
+      s.colblocks = (int)((s.ld + 255) / 256);
+      s.b1 = beta1; s.b2 = beta2; s.r1 = 1.f / beta1; s.r2 = 1.f / beta2;
+      unsigned grid;
+      if ((rc = slope_grid(s, &grid))) return rc;
+      gated_slope<T, O><<<grid, 256, 0, st>>>(s);
       if ((rc = check_launch("gated_slope"))) return rc;
     }
-    SimpleArgs a{};
-    a.pairs = 2;
+    const int parts = split_v<T> ? 3 : 1;
     if (dx) {
-      a.a[0] = dg; a.a[1] = du; a.sam = f; a.sak = 1; a.b[0] = w_gate; a.b[1] = w_up; a.sbn = 1; a.sbk = ldw;
-      a.M = m; a.N = k; a.K = f; a.e = plain_out(dx, k, dtype);
-      if ((rc = run_simple<false>(a, dtype, st))) return rc;
+      Product d{};
+      d.type = dtype; d.M = m; d.N = k; d.K = f; d.nz = 1; d.b_mn = true;
+      d.e = plain_out(dx, k, dtype);
+      d.a[0] = p;
+      if (any && ((rc = operand(&d.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
+                  (rc = operand(&d.b[1], w_up, ldw, f, k, dtype, ws, st))))
+        return rc;
+      // both products' pairs of parts, the smallest of both first
+      add_segments(d, 0, 0, 0, parts, 2);
+      add_segments(d, 0, 1, 1, parts, 2);
+      if (parts == 3) {
+        Segment s[12];
+        for (int i = 0; i < 12; ++i) s[i] = d.seg[i % 2 * 6 + i / 2];
+        for (int i = 0; i < 12; ++i) d.seg[i] = s[i];
+      }
+      if ((rc = run_product(d, st))) return rc;
     }
-    a.pairs = 1;
-    a.sam = 1; a.sak = f; a.b[0] = x; a.sbn = 1; a.sbk = ldx;
-    a.M = f; a.N = k; a.K = m;
-    for (int h = 0; h < 2; ++h) {
-      void* out = h ? dw_up : dw_gate;
-      if (!out) continue;
-      a.a[0] = h ? du : dg;
-      a.e = plain_out(out, k, dtype);
-      if ((rc = run_simple<false>(a, dtype, st))) return rc;
+    if (dw_gate || dw_up) {
+      Product d{};
+      d.type = dtype; d.M = f; d.N = k; d.K = m; d.a_mn = d.b_mn = true;
+      d.nz = dw_gate && dw_up ? 2 : 1;
+      d.out_z[0] = dw_gate; d.out_z[1] = dw_up;
+      d.e = plain_out(dw_gate ? dw_gate : dw_up, k, dtype);
+      d.a[0] = p;
+      if (any && (rc = operand(&d.b[0], x, ldx, m, k, dtype, ws, st))) return rc;
+      // (with two outputs a part's piece is 2 part + output)
+      if (d.nz == 2) add_segments(d, 0, 0, 0, parts, 1);
+      else add_segments(d, 0, dw_gate ? 0 : 1, 0, parts, 2);
+      if ((rc = run_product(d, st))) return rc;
     }
     return VERACE_OK;
   });

@@ -1,0 +1,570 @@
+// Products of many rows on the tensor cores (the engine behind linear.cu):
+//     out(m, n) = epilogue(sum_k A(m, k) B(n, k))
+// A pair of CTAs on neighbouring SMs computes a tile of 256 x BN: each holds 128 rows of A and
+// half of B's rows in shared memory, and one tcgen05.mma.cta_group::2 a step of 32 bytes of K
+// reads both, 128 rows x BN columns of fp32 sums landing in each CTA's TMEM.  (A single CTA's
+// 128 x 256 tile would read 12 KB of shared memory for what the pair does with 8 KB a CTA.)
+//
+// Warps: 0 feeds stages of 128 bytes of K by TMA (128-byte swizzle; operands stored with K
+// outermost come as boxes of 64 x 64 and go to the MMA as MN-major), 1 issues the MMAs (in the pair's
+// first CTA), 4 to 11 are the epilogue.  Two sets of sums in TMEM: a tile's epilogue runs under
+// the next one's products.  Persistent: a pair takes every 74th tile, eight rows of tiles
+// beside each other so that the running tiles share their operands in L2.
+//
+// Gated products put 64 or 128 rows of each weight into one tile (the first CTA of the pair loads the
+// gate's, the second the up projection's), so both sums of an output lie in one TMEM row and the product is formed in
+// registers.  fp32 operands come as three bf16 parts and run over six pairs of them, the smallest first, into
+// one fp32 sum; a sum of two products (the input gradient of a gated block) is two runs over K.
+//
+// Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
+// applies scales, bias and activation, and the warp turns the rounded values over in shared memory so
+// that a store is 128 neighbouring bytes; residuals come in the same way.
+#include "linear_tc.cuh"
+#include "tc.cuh"
+#include "tmap.cuh"
+
+#include <atomic>
+
+namespace verace {
+
+__device__ int g_linear_status = 0;   // non-zero after a bounded wait gave up
+
+namespace {
+
+using namespace lin;
+
+constexpr int NT = 384, EPI_WARPS = 8;
+constexpr uint32_t POLLS = 1u << 22;
+constexpr int TURN = 32 * 33 * 4;      // a warp's place to turn 32 rows of 32 words over
+
+template <int BN>
+struct Shape {
+  static constexpr int STAGE = 16384 + BN * 64;              // A: 128 rows x 128 bytes; B: BN / 2 rows
+  static constexpr int STAGES = BN == 256 ? 6 : 8;
+  static constexpr int TURNS = STAGE * STAGES, BARS = TURNS + EPI_WARPS * TURN, SMEM = BARS + 256 + 1024;
+};
+
+struct Maps {
+  CUtensorMap a[2], b[2];
+};
+
+struct Args {
+  long long M, N;
+  int kblocks, segments;
+  Segment seg[MAX_SEGMENTS];
+  int nz, tiles_m, tiles_n, tiles;
+  uint32_t idesc;
+  void* out_z[2];
+  Epilogue e;
+};
+
+__device__ __forceinline__ uint32_t in_cta0(const void* p) {   // the address of p's place in the pair's first CTA
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc::smem_addr(p)));
+  return a;
+}
+__device__ __forceinline__ uint32_t cta_in_pair() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// a box into this CTA's shared memory, its bytes counted on the first CTA's barrier
+__device__ __forceinline__ void load_box(void* smem, const CUtensorMap* map, int x, int y, int z, uint32_t bar0) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(tc::smem_addr(smem)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar0)
+      : "memory");
+}
+template <bool F8>
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (F8)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate));
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate));
+}
+// arrive on `bar` in both CTAs once the MMAs issued so far are done
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   tc::smem_addr(bar)),
+               "h"((unsigned short)3)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// 16 columns of this thread's TMEM row, without waiting for them
+__device__ __forceinline__ void tmem_ld16_async(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+// waits for the loads; the registers pass through so that nothing reads them earlier
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
+// ------------------------------------------------------------------ the epilogue's stores and loads
+// A warp's 32 rows of 32 words, the word `lane` of row r at turn[33 r + lane]: for 16-bit types 64
+// columns, two to a word.
+struct Block {
+  uint32_t* turn;
+  long long m0, n0, M, N;   // first row and column; ends
+};
+
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, int type) {
+  return type == VERACE_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
+}
+__device__ __forceinline__ float2 unpack_pair(uint32_t w, int type) {
+  return type == VERACE_BF16 ? unpack2<__nv_bfloat16>(w) : unpack2<__half>(w);
+}
+
+// the block to `p` (rows `ld` values apart, values of `size` bytes)
+__device__ __forceinline__ void write_block(const Block& b, void* p, long long ld, bool wide, int lane) {
+  __syncwarp();
+  const int rows = (int)min(32LL, b.M - b.m0);
+  if (wide) {                                  // fp32
+    const long long n = b.n0 + lane;
+    float* o = static_cast<float*>(p) + b.m0 * ld + n;
+    if (n < b.N)
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, o += ld) *o = __uint_as_float(b.turn[33 * r + lane]);
+  } else {
+    const long long n = b.n0 + 2 * lane;
+    unsigned short* o = static_cast<unsigned short*>(p) + b.m0 * ld + n;
+    if (((ld & 1) | ((size_t)p & 3)) == 0 && n + 1 < b.N) {
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, o += ld) *reinterpret_cast<uint32_t*>(o) = b.turn[33 * r + lane];
+    } else if (n < b.N) {
+      for (int r = 0; r < rows; ++r, o += ld) {
+        const uint32_t w = b.turn[33 * r + lane];
+        o[0] = (unsigned short)w;
+        if (n + 1 < b.N) o[1] = (unsigned short)(w >> 16);
+      }
+    }
+  }
+  __syncwarp();
+}
+// and from `p`
+__device__ __forceinline__ void read_block(const Block& b, const void* p, long long ld, bool wide, int lane) {
+  const int rows = (int)min(32LL, b.M - b.m0);
+  if (wide) {
+    const long long n = b.n0 + lane;
+    const float* o = static_cast<const float*>(p) + b.m0 * ld + n;
+    if (n < b.N)
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, o += ld) b.turn[33 * r + lane] = __float_as_uint(*o);
+  } else {
+    const long long n = b.n0 + 2 * lane;
+    const unsigned short* o = static_cast<const unsigned short*>(p) + b.m0 * ld + n;
+    if (((ld & 1) | ((size_t)p & 3)) == 0 && n + 1 < b.N) {
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, o += ld) b.turn[33 * r + lane] = *reinterpret_cast<const uint32_t*>(o);
+    } else if (n < b.N) {
+      for (int r = 0; r < rows; ++r, o += ld)
+        b.turn[33 * r + lane] = o[0] | (n + 1 < b.N ? (uint32_t)o[1] << 16 : 0u);
+    }
+  }
+  __syncwarp();
+}
+
+// 16 values into the thread's own row of the block, from column c on
+__device__ __forceinline__ void put16(const Block& b, int c, const float (&v)[16], int type, int lane) {
+  uint32_t* t = b.turn + 33 * lane;
+  if (type == VERACE_F32) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[c + j] = __float_as_uint(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[c / 2 + j] = pack_pair(v[2 * j], v[2 * j + 1], type);
+  }
+}
+__device__ __forceinline__ void add16(const Block& b, int c, float (&v)[16], int type, int lane) {
+  const uint32_t* t = b.turn + 33 * lane;
+  if (type == VERACE_F32) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(t[c + j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = unpack_pair(t[c / 2 + j], type);
+      v[2 * j] += f.x;
+      v[2 * j + 1] += f.y;
+    }
+  }
+}
+
+// 16 sums of one row, columns n0 ...: what the epilogue asks for before the activation
+__device__ __forceinline__ void scaled16(const Epilogue& e, const uint32_t (&r)[16], float (&v)[16], float rs,
+                                         const float* col_scale, const void* bias, long long n0, long long N) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+  if (col_scale) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= rs * (n0 + j < N ? col_scale[n0 + j] : 0.f);
+  }
+  if (bias) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += n0 + j < N ? load_as(bias, n0 + j, e.bias_type) : 0.f;
+  }
+}
+
+// One block of `width` columns from TMEM column `col` (the second sums at `col_up`) on.
+template <bool GATED>
+__device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b, uint32_t tmem, int col, int col_up,
+                                               void* out, int lane) {
+  const bool wide = e.type == VERACE_F32;
+  const int width = wide ? 32 : 64;
+  const long long m = b.m0 + lane;
+  const float rs = e.row_scale && m < b.M ? e.row_scale[m] : 0.f;
+  if constexpr (!GATED) {
+    // saved sums go out in a pass of their own: the block's place is one
+    if (e.pre) {
+      for (int c = 0; c < width; c += 16) {
+        uint32_t r[16];
+        tmem_ld16_async(tmem + col + c, r);
+        tmem_wait(r);
+        float v[16];
+        scaled16(e, r, v, rs, e.col_scale, e.bias, b.n0 + c, b.N);
+        put16(b, c, v, e.type, lane);
+      }
+      write_block(b, e.pre, e.ld, wide, lane);
+    }
+    if (e.residual) read_block(b, e.residual, e.ld_res, wide, lane);
+    for (int c = 0; c < width; c += 16) {
+      uint32_t r[16];
+      tmem_ld16_async(tmem + col + c, r);
+      tmem_wait(r);
+      float v[16];
+      scaled16(e, r, v, rs, e.col_scale, e.bias, b.n0 + c, b.N);
+      by_act(e.act, !wide, [&](auto act, auto fast) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = act_<decltype(act)::value, decltype(fast)::value>(v[j]);
+      });
+      if (e.residual) add16(b, c, v, e.type, lane);
+      put16(b, c, v, e.type, lane);
+    }
+  } else {
+    if (e.pre) {
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        for (int c = 0; c < width; c += 16) {
+          uint32_t r[16];
+          tmem_ld16_async(tmem + (h ? col_up : col) + c, r);
+          tmem_wait(r);
+          float v[16];
+          scaled16(e, r, v, rs, h ? e.up_scale : e.col_scale, nullptr, b.n0 + c, b.N);
+          put16(b, c, v, e.type, lane);
+        }
+        write_block(b, h ? e.pre_up : e.pre, e.ld, wide, lane);
+      }
+    }
+    for (int c = 0; c < width; c += 16) {
+      uint32_t r[16], s[16];
+      tmem_ld16_async(tmem + col + c, r);
+      tmem_ld16_async(tmem + col_up + c, s);
+      tmem_wait(r);
+      tmem_wait(s);
+      float g[16], u[16];
+      scaled16(e, r, g, rs, e.col_scale, nullptr, b.n0 + c, b.N);
+      scaled16(e, s, u, rs, e.up_scale, nullptr, b.n0 + c, b.N);
+      by_act(e.act, !wide, [&](auto act, auto fast) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
+      });
+      put16(b, c, g, e.type, lane);
+    }
+  }
+  write_block(b, out, e.ld, wide, lane);
+}
+
+// tile t -> (z, row, column) of tiles: groups of eight rows, column by column
+struct Place {
+  int z, m, n;
+};
+__device__ __forceinline__ Place place(const Args& p, int t) {
+  Place o;
+  const int each = p.tiles_m * p.tiles_n;
+  o.z = t / each;
+  t -= o.z * each;
+  const int group = t / (8 * p.tiles_n), first = 8 * group, high = min(8, p.tiles_m - first);
+  t -= group * 8 * p.tiles_n;
+  o.n = t / high;
+  o.m = first + t - o.n * high;
+  return o;
+}
+
+template <bool F8, bool AMN, bool BMN, bool GATED, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
+large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
+  using S = Shape<BN>;
+  constexpr int KB = F8 ? 128 : 64;            // values of K in a stage
+  constexpr int HB = BN / 2;                   // rows of B in a CTA
+  constexpr int TN = GATED ? HB : BN;          // output columns of a tile
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(((size_t)raw + 1023) & ~(size_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::BARS);
+  uint64_t* empty = full + S::STAGES;
+  uint64_t* acc_full = empty + S::STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* fail = reinterpret_cast<volatile int*>(slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cta_in_pair();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(slot)), "r"(2 * BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S::STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&acc_full[i], 1);
+      tc::mbar_init(&acc_empty[i], 2 * EPI_WARPS);
+    }
+    *fail = 0;
+    tc::fence_mbar_init();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = *slot;
+  const int steps = p.segments * p.kblocks;
+
+  if (warp == 0) {
+    if (lane == 0) {   // ---- operands
+      int i = 0, flying = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < p.tiles && ok; t += pairs) {
+        const Place at = place(p, t);
+        const int m0 = at.m * 256 + (int)rank * 128;
+        const int n0 = GATED ? at.n * HB : at.n * BN + (int)rank * HB;
+        for (int s = 0; s < p.segments && ok; ++s) {
+          const Segment g = p.seg[s];
+          const CUtensorMap* ma = &maps.a[g.a];
+          const CUtensorMap* mb = &maps.b[GATED ? rank : g.b];
+          const int az = g.az * p.nz + at.z;
+          for (int kb = 0; kb < p.kblocks; ++kb) {
+            if (*fail || !tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
+              ok = false;
+              break;
+            }
+            if (rank == 0) tc::mbar_expect_tx(&full[i], 2 * S::STAGE);
+            const uint32_t bar = in_cta0(&full[i]);
+            unsigned char* a = sm + i * S::STAGE;
+            unsigned char* b = a + 16384;
+            if constexpr (AMN) {
+              load_box(a, ma, m0, kb * KB, az, bar);
+              load_box(a + 8192, ma, m0 + 64, kb * KB, az, bar);
+            } else {
+              load_box(a, ma, kb * KB, m0, az, bar);
+            }
+            if constexpr (BMN) {
+#pragma unroll
+              for (int h = 0; h < HB / 64; ++h) load_box(b + h * 8192, mb, n0 + 64 * h, kb * KB, g.bz, bar);
+            } else {
+              load_box(b, mb, kb * KB, n0, g.bz, bar);
+            }
+            if (++i == S::STAGES) i = 0, phase ^= 1;
+            flying = min(flying + 1, S::STAGES);
+          }
+        }
+      }
+      if (!ok) {
+        *fail = 1;
+        atomicExch(&g_linear_status, 1);
+      }
+      // copies in flight land before the CTA may end (the first CTA's barriers count both CTAs'; the
+      // second one stays for the first at the cluster's barrier below)
+      if (rank == 0)
+        while (flying-- > 0) {
+          if (i == 0) i = S::STAGES, phase ^= 1;
+          tc::mbar_wait(&full[--i], phase, POLLS);
+        }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {   // ---- MMAs of the pair
+      int i = 0, n = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < p.tiles && ok; t += pairs, ++n) {
+        const int b = n & 1, use = n >> 1;
+        if (*fail || !tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        const uint32_t d = tmem + b * BN;
+        for (int s = 0; s < steps; ++s) {
+          if (*fail || !tc::mbar_wait(&full[i], phase, POLLS)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+          const uint32_t a = tc::smem_addr(sm + i * S::STAGE), bb = a + 16384;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
+            const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
+            const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
+            mma_pair<F8>(d, da, db, p.idesc, s > 0 || k > 0 ? 1u : 0u);
+          }
+          commit_pair(&empty[i]);
+          if (++i == S::STAGES) i = 0, phase ^= 1;
+        }
+        commit_pair(&acc_full[b]);   // (also after a failure: every MMA issued completes)
+        if (!ok) tc::mbar_wait(&acc_full[b], use & 1, POLLS);
+      }
+      if (!ok) {
+        *fail = 1;
+        atomicExch(&g_linear_status, 1);
+      }
+    }
+  } else if (warp >= 4) {   // ---- epilogue: TMEM lanes 32 (warp % 4) ..., one half of the columns
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int width = p.e.type == VERACE_F32 ? 32 : 64, per = max(TN / 2, width);
+    Block b;
+    b.turn = reinterpret_cast<uint32_t*>(sm + S::TURNS + (warp - 4) * TURN);
+    b.M = p.M;
+    b.N = p.N;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
+    int n = 0;
+    for (int t = pair; t < p.tiles; t += pairs, ++n) {
+      const Place at = place(p, t);
+      const int buf = n & 1, use = n >> 1;
+      if (*fail || !tc::mbar_wait(&acc_full[buf], use & 1, POLLS)) {
+        *fail = 1;
+        if (lane == 0) atomicExch(&g_linear_status, 1);
+        break;
+      }
+      tc::fence_after_sync();
+      b.m0 = at.m * 256LL + rank * 128 + 32 * quarter;
+      void* out = p.nz > 1 ? p.out_z[at.z] : p.e.out;
+      // (every warp reads its blocks even outside of the output: tcgen05.ld is the warp's as a whole)
+      for (int c = half * per; c < min(TN, (half + 1) * per); c += width) {
+        b.n0 = (long long)at.n * TN + c;
+        if (b.n0 < p.N && b.m0 < p.M) epilogue_block<GATED>(p.e, b, lanes + buf * BN, c, c + HB, out, lane);
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_at(in_cta0(&acc_empty[buf]));
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc::fence_after_sync();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+}
+
+// ------------------------------------------------------------------ host
+// boxes of 128 bytes x `rows`
+int operand_map(CUtensorMap* map, const Mat& m, int type, int rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tmap_encoder();
+  VERACE_REQUIRE(enc, VERACE_ERR_CUDA, "linear: the driver has no cuTensorMapEncodeTiled");
+  const size_t es = size_of(type);
+  const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.pieces};
+  const cuuint64_t strides[2] = {m.ld * es, (m.pieces > 1 ? m.piece : m.ld) * es};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)rows, 1}, el[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = type == VERACE_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : type == VERACE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = enc(map, dt, 3, const_cast<void*>(m.p), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  VERACE_REQUIRE(r == CUDA_SUCCESS, VERACE_ERR_CUDA, "linear: tensor map of %lld x %lld (stride %lld) refused (%d)", m.rows,
+                 m.cols, m.ld, (int)r);
+  return VERACE_OK;
+}
+
+template <bool F8, bool AMN, bool BMN, bool GATED, int BN>
+int launch(const Product& p, cudaStream_t st) {
+  using S = Shape<BN>;
+  constexpr int TN = GATED ? BN / 2 : BN;
+  Maps maps;
+  int rc;
+  for (int i = 0; i < 2; ++i) {
+    const Mat& a = p.a[p.a[i].p ? i : 0];
+    const Mat& b = p.b[p.b[i].p ? i : 0];
+    if ((rc = operand_map(&maps.a[i], a, p.type, AMN ? 64 : 128)) || (rc = operand_map(&maps.b[i], b, p.type, BMN ? 64 : BN / 2)))
+      return rc;
+  }
+  Args a{};
+  a.M = p.M; a.N = p.N;
+  a.kblocks = (int)((p.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
+  a.segments = p.segments;
+  for (int i = 0; i < p.segments; ++i) a.seg[i] = p.seg[i];
+  a.nz = p.nz;
+  a.tiles_m = (int)((p.M + 255) / 256);
+  a.tiles_n = (int)((p.N + TN - 1) / TN);
+  const long long tiles = (long long)a.tiles_m * a.tiles_n * p.nz;
+  VERACE_REQUIRE(tiles < 1LL << 30, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
+  a.tiles = (int)tiles;
+  a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
+            (uint32_t)AMN << 15 | (uint32_t)BMN << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+  a.out_z[0] = p.out_z[0]; a.out_z[1] = p.out_z[1];
+  a.e = p.e;
+  auto kern = large_product<F8, AMN, BMN, GATED, BN>;
+  int dev = 0;
+  VERACE_CUDA(cudaGetDevice(&dev));
+  static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  const int pairs = tiles < 74 ? (int)tiles : 74;
+  kern<<<2 * pairs, NT, S::SMEM, st>>>(maps, a);
+  return check_launch("large_product");
+}
+
+template <int BN>
+int by_kind(const Product& p, cudaStream_t st) {
+  if (p.type == VERACE_E4M3)
+    return p.gated ? launch<true, false, false, true, BN>(p, st) : launch<true, false, false, false, BN>(p, st);
+  if (p.gated) return launch<false, false, false, true, BN>(p, st);
+  if (p.a_mn) return launch<false, true, true, false, BN>(p, st);
+  return p.b_mn ? launch<false, false, true, false, BN>(p, st) : launch<false, false, false, false, BN>(p, st);
+}
+
+}  // namespace
+
+namespace lin {
+
+int product_large(const Product& p, cudaStream_t st) {
+  const long long wide = (p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256) * ((p.M + 255) / 256) * p.nz;
+  return wide >= 74 ? by_kind<256>(p, st) : by_kind<128>(p, st);
+}
+
+}  // namespace lin
+
+int linear_read_status(int* status) {
+  int h = 0;
+  VERACE_CUDA(cudaMemcpyFromSymbol(&h, g_linear_status, sizeof(int)));
+  if (h) {
+    const int zero = 0;
+    VERACE_CUDA(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
+  }
+  *status = h;
+  return VERACE_OK;
+}
+
+}  // namespace verace
