@@ -47,6 +47,7 @@ int sssd_tc_read_status(int* status);
 int decode_read_status(unsigned int* status);
 int mcmoe_read_status(int* status);
 int linear_read_status(int* status);
+int linear_few_read_status(int* status);
 int int4_read_status(int* status);
 
 namespace {
@@ -796,6 +797,9 @@ extern "C" int verace_device_status(void* stream) {
   if (rc) return rc;
   status |= status2;
   rc = linear_read_status(&status2);
+  if (rc) return rc;
+  status |= status2;
+  rc = linear_few_read_status(&status2);
   if (rc) return rc;
   status |= status2;
   unsigned int dstat = 0;   // bit 0: a hologram far from unitary; bit 1: a decode wait gave up

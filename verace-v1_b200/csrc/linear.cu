@@ -122,6 +122,8 @@ __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long l
   store_as(e.out, r * e.ld + c, v, e.type);
 }
 
+constexpr long long FEW = 256;
+
 // The pairs of parts that make up an fp32 product, the smallest first (other types: one).
 void add_segments(Product& p, int a, int az, int b, int parts, int step) {
   if (parts == 1) {
@@ -131,6 +133,11 @@ void add_segments(Product& p, int a, int az, int b, int parts, int step) {
   constexpr unsigned char A[6] = {2, 1, 0, 1, 0, 0}, B[6] = {0, 1, 2, 0, 1, 0};
   for (int i = 0; i < 6; ++i)
     p.seg[p.segments++] = Segment{(unsigned char)a, (unsigned char)(A[i] * step + az), (unsigned char)b, B[i]};
+}
+
+// Whether a product goes to the engine that streams the weights past its rows.
+bool few_rows(const Product& p, bool parts) {
+  return !p.a_mn && p.M <= FEW;
 }
 
 int run_product(Product& p, cudaStream_t st) {
@@ -146,8 +153,9 @@ int run_product(Product& p, cudaStream_t st) {
     }
     return VERACE_OK;
   }
-  if (p.type == VERACE_F32) p.type = VERACE_BF16;   // (the parts' type)
-  return product_large(p, st);
+  const bool parts = p.type == VERACE_F32;
+  if (parts) p.type = VERACE_BF16;
+  return few_rows(p, parts) ? product_few(p, st) : product_large(p, st);
 }
 
 // ------------------------------------------------------------------ backward of the epilogues

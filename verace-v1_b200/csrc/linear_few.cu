@@ -1,0 +1,405 @@
+// Products of few rows (tokens) on the tensor cores, the other engine behind linear.cu:
+//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 256
+// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 256 columns, so
+// a weight crosses shared memory once and no row of the MMA is idle; a CTA streams its 128 rows (gated:
+// 128 of each weight, two sums side by side in TMEM) by TMA in stages of 128 bytes of K.  Two
+// CTAs share an SM where shared memory allows, so that one's set-up and epilogue run under the other's
+// stream.  Few tiles: K is split over a cluster of up to 8 CTAs, whose partial sums are joined through
+// distributed shared memory in rank order.
+//
+// Warps: 0 feeds the stages, 1 issues the MMAs, 2 to 5 read the sums (all join them): a thread holds a weight row, so
+// neighbouring threads store neighbouring outputs of a token.  The input gradient of few tokens
+// (a_mn: weights stored [K][N], read as MN-major) runs here too, for a gated block over both weights.
+#include "linear_tc.cuh"
+
+#include <cooperative_groups.h>
+
+#include <atomic>
+
+namespace verace {
+
+__device__ int g_linear_few_status = 0;   // non-zero after a bounded wait gave up
+
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace lin;
+
+constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8, MAX_TOKENS = 256;
+// shared memory for stages of a CTA that has an SM to itself, and of one that shares it (228 KB an SM,
+// less 1 KB a CTA that the system takes, 1 KB of barriers and 1 KB to align the stages)
+constexpr int ROOM = 225 * 1024, HALF_ROOM = 111 * 1024;
+constexpr uint32_t POLLS = 1u << 22;
+
+struct Maps {
+  CUtensorMap w[2], x;
+};
+
+struct Args {
+  long long M, N;       // tokens, outputs
+  int mp;               // tokens of a tile, rounded up to 16
+  int stages, stage;    // and a stage's bytes
+  int kblocks, steps, per, ck, tiles_n;
+  int cols;             // of TMEM
+  int round;            // tokens whose partial sums a CTA holds at a time (ck > 1)
+  int segments;
+  Segment seg[MAX_SEGMENTS];
+  uint32_t idesc;
+  Epilogue e;
+};
+
+template <bool F8>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (F8)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate));
+  else
+    tc::mma_bf16(d, a, b, idesc, accumulate);   // (kind::f16; the descriptor names the type)
+}
+
+// four neighbouring values of a row, `n` of them inside of it
+__device__ __forceinline__ void load4(const void* p, long long i, int n, int type, float (&v)[4]) {
+  const size_t at = (size_t)p + i * (type == VERACE_F32 ? 4 : 2);
+  if (n == 4 && type != VERACE_F32 && (at & 7) == 0) {
+    const uint2 w = *reinterpret_cast<const uint2*>(at);
+    const float2 a = unpack_pair(w.x, type), b = unpack_pair(w.y, type);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? load_as(p, i + j, type) : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(void* p, long long i, int n, int type, const float (&v)[4]) {
+  const size_t at = (size_t)p + i * (type == VERACE_F32 ? 4 : 2);
+  if (n == 4 && type != VERACE_F32 && (at & 7) == 0) {
+    *reinterpret_cast<uint2*>(at) = make_uint2(pack_pair(v[0], v[1], type), pack_pair(v[2], v[3], type));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) store_as(p, i + j, v[j], type);
+  }
+}
+
+// four outputs of row m from their sums (u: the up projection's)
+template <bool GATED>
+__device__ __forceinline__ void finish4(const Epilogue& e, long long m, long long c, long long N, float (&g)[4], float (&u)[4]) {
+  const int n = (int)min(4LL, N - c);
+  float res[4] = {};
+  if (!GATED && e.residual) load4(e.residual, m * e.ld_res + c, n, e.type, res);
+  if (e.col_scale) {
+    const float rs = e.row_scale[m];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) {
+        g[j] *= rs * e.col_scale[c + j];
+        if (GATED) u[j] *= rs * e.up_scale[c + j];
+      }
+  }
+  if (!GATED && e.bias) {
+    float b[4];
+    load4(e.bias, c, n, e.bias_type, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] += b[j];
+  }
+  if (e.pre) {
+    store4(e.pre, m * e.ld + c, n, e.type, g);
+    if (GATED) store4(e.pre_up, m * e.ld + c, n, e.type, u);
+  }
+  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (GATED) g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
+      else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
+    }
+  });
+  if (!GATED && e.residual) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] += res[j];
+  }
+  store4(e.out, m * e.ld + c, n, e.type, g);
+}
+
+template <bool F8, bool WMN, bool GATED>
+__global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
+  constexpr int KB = F8 ? 128 : 64, WB = GATED ? 2 * ROWS * 128 : ROWS * 128;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(((size_t)raw + 1023) & ~(size_t)1023);
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], done;
+  __shared__ uint32_t slot;
+  __shared__ volatile int fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int unit = blockIdx.x / p.ck, rank = blockIdx.x - unit * p.ck;
+  const int tile_m = unit / p.tiles_n, tile_n = unit - tile_m * p.tiles_n;
+  const int n0 = tile_n * ROWS;
+  const long long m0 = (long long)tile_m * p.mp;
+  const int first = rank * p.per, last = min(p.steps, first + p.per);
+  if (warp == 1) tc::tmem_alloc(&slot, p.cols);
+  if (tid == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    tc::mbar_init(&done, 1);
+    fail = 0;
+    tc::fence_mbar_init();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = slot;
+
+  if (warp == 0) {
+    if (lane == 0) {   // ---- weights and tokens
+      int i = 0, flying = 0, seg = first / p.kblocks, kb = first - seg * p.kblocks;
+      uint32_t phase = 0;
+      for (int s = first; s < last; ++s) {
+        if (fail || !tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {
+          fail = 1;
+          atomicExch(&g_linear_few_status, 1);
+          break;
+        }
+        const Segment g = p.seg[seg];
+        unsigned char* w = sm + i * p.stage;
+        tc::mbar_expect_tx(&full[i], p.stage);
+        if constexpr (WMN) {
+          tc::tma_load_3d(w, &maps.w[g.b], n0, kb * KB, g.bz, &full[i]);
+          tc::tma_load_3d(w + 8192, &maps.w[g.b], n0 + 64, kb * KB, g.bz, &full[i]);
+        } else {
+          tc::tma_load_3d(w, &maps.w[GATED ? 0 : g.b], kb * KB, n0, g.bz, &full[i]);
+          if (GATED) tc::tma_load_3d(w + ROWS * 128, &maps.w[1], kb * KB, n0, g.bz, &full[i]);
+        }
+        tc::tma_load_3d(w + WB, &maps.x, kb * KB, (int)m0, g.az, &full[i]);
+        if (++kb == p.kblocks) kb = 0, ++seg;
+        if (++i == p.stages) i = 0, phase ^= 1;
+        flying = min(flying + 1, p.stages);
+      }
+      while (flying-- > 0) {   // copies in flight land before the CTA may end
+        if (i == 0) i = p.stages, phase ^= 1;
+        tc::mbar_wait(&full[--i], phase, POLLS);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {   // ---- MMAs
+      int i = 0;
+      uint32_t phase = 0;
+      for (int s = first; s < last; ++s) {
+        if (fail || !tc::mbar_wait(&full[i], phase, POLLS)) {
+          fail = 1;
+          atomicExch(&g_linear_few_status, 1);
+          break;
+        }
+        tc::fence_after_sync();
+        const uint32_t w = tc::smem_addr(sm + i * p.stage), x = w + WB;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint64_t dx = tc::sdesc_sw128(x + k * 32, 16, 1024);
+          const uint64_t dw = WMN ? tc::sdesc_sw128(w + k * 2048, 8192, 1024) : tc::sdesc_sw128(w + k * 32, 16, 1024);
+          const uint32_t more = s > first || k > 0;
+          mma<F8>(tmem, dw, dx, p.idesc, more);
+          if (GATED) mma<F8>(tmem + p.mp, tc::sdesc_sw128(w + ROWS * 128 + k * 32, 16, 1024), dx, p.idesc, more);
+        }
+        tc::commit(&empty[i]);
+        if (++i == p.stages) i = 0, phase ^= 1;
+      }
+      tc::commit(&done);
+      tc::mbar_wait(&done, 0, POLLS);   // (every MMA issued completes before the CTA may end)
+    }
+  }
+  __syncwarp();
+  // ---- the sums
+  const int tokens = (int)min((long long)p.mp, p.M - m0);
+  const int quarter = warp & 3;
+  const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
+  const int n = n0 + 32 * quarter + lane;
+  bool ok = true;
+  if (warp >= 2 && warp < 6) {
+    ok = tc::mbar_wait(&done, 0, POLLS) && !fail;
+    if (!ok && lane == 0) atomicExch(&g_linear_few_status, 1);
+    tc::fence_after_sync();
+  }
+  if (p.ck == 1) {
+    if (warp >= 2 && warp < 6 && ok) {
+      const Epilogue& e = p.e;
+      const bool in = n < p.N;
+      const float cs = e.col_scale && in ? e.col_scale[n] : 1.f, us = GATED && e.up_scale && in ? e.up_scale[n] : 1.f;
+      const float bias = !GATED && e.bias && in ? load_as(e.bias, n, e.bias_type) : 0.f;
+      for (int t = 0; t < tokens; t += 16) {
+        uint32_t r[16], s[16];
+        tmem_ld16_async(mine + t, r);
+        if (GATED) tmem_ld16_async(mine + p.mp + t, s);
+        float res[16];
+        if (!GATED && e.residual) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            res[j] = in && t + j < tokens ? load_as(e.residual, (m0 + t + j) * e.ld_res + n, e.type) : 0.f;
+        }
+        tmem_wait(r);
+        if (GATED) tmem_wait(s);
+        float g[16], u[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float rs = e.row_scale && t + j < tokens ? e.row_scale[m0 + t + j] : 1.f;
+          g[j] = __uint_as_float(r[j]);
+          if (e.col_scale) g[j] *= rs * cs;
+          g[j] += bias;
+          if (GATED) {
+            u[j] = __uint_as_float(s[j]);
+            if (e.col_scale) u[j] *= rs * us;
+          }
+        }
+        if (e.pre && in) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (t + j < tokens) {
+              store_as(e.pre, (m0 + t + j) * e.ld + n, g[j], e.type);
+              if (GATED) store_as(e.pre_up, (m0 + t + j) * e.ld + n, u[j], e.type);
+            }
+        }
+        by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if constexpr (GATED) g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
+            else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
+          }
+        });
+        if (in) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (t + j < tokens) store_as(e.out, (m0 + t + j) * e.ld + n, !GATED && e.residual ? g[j] + res[j] : g[j], e.type);
+        }
+      }
+    }
+  } else {
+    // every CTA's sums of `round` tokens in its shared memory (the stages' place), [token][128]
+    cg::cluster_group cl = cg::this_cluster();
+    float* part = reinterpret_cast<float*>(sm);
+    for (int t0 = 0; t0 < tokens; t0 += p.round) {
+      if (warp >= 2 && warp < 6) {
+        for (int t = 0; t < p.round && t0 + t < tokens; t += 16)
+#pragma unroll
+          for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+            uint32_t r[16];
+            tmem_ld16_async(mine + h * p.mp + t0 + t, r);
+            tmem_wait(r);
+            float* o = part + (h * p.round + t) * ROWS + 32 * quarter + lane;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j * ROWS] = ok && first < last ? __uint_as_float(r[j]) : 0.f;
+          }
+      }
+      cl.sync();
+      const int total = min(p.round, tokens - t0) * (ROWS / 4);
+#pragma unroll 2
+      for (int i = rank * NT + tid; i < total; i += p.ck * NT) {
+        float g[4] = {}, u[4] = {};
+#pragma unroll 4
+        for (int c = 0; c < p.ck; ++c) {
+          const float4* o = reinterpret_cast<const float4*>(cl.map_shared_rank(part, c));
+          const float4 a = o[i];
+          g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+          if (GATED) {
+            const float4 b = o[p.round * (ROWS / 4) + i];
+            u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+          }
+        }
+        const long long c = n0 + i % (ROWS / 4) * 4;
+        if (c < p.N) finish4<GATED>(p.e, m0 + t0 + i / (ROWS / 4), c, p.N, g, u);
+      }
+      cl.sync();
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tc::tmem_dealloc(tmem, p.cols);
+}
+
+// ------------------------------------------------------------------ host
+template <bool F8, bool WMN, bool GATED>
+int launch(const Product& p, cudaStream_t st) {
+  Maps maps;
+  Args a{};
+  int rc;
+  a.M = p.M; a.N = p.N;
+  const int tiles_m = (int)((p.M + MAX_TOKENS - 1) / MAX_TOKENS);
+  a.mp = (int)(((p.M + tiles_m - 1) / tiles_m + 15) / 16 * 16);
+  // A (x) in boxes of the tile's tokens, B (the weights) as the MMA's rows
+  if ((rc = operand_map(&maps.x, p.a[0], p.type, a.mp))) return rc;
+  for (int i = 0; i < 2; ++i)
+    if ((rc = operand_map(&maps.w[i], p.b[p.b[i].p ? i : 0], p.type, WMN ? 64 : ROWS))) return rc;
+  a.kblocks = (int)((p.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
+  a.segments = p.segments;
+  for (int i = 0; i < p.segments; ++i) a.seg[i] = p.seg[i];
+  a.steps = a.kblocks * p.segments;
+  a.tiles_n = (int)((p.N + ROWS - 1) / ROWS);
+  const long long units = (long long)a.tiles_n * tiles_m;
+  VERACE_REQUIRE(units < 1LL << 27, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
+  a.ck = 1;
+  while (a.ck < 8 && units * a.ck * 2 <= 148 && a.steps >= a.ck * 4) a.ck *= 2;
+  a.per = (a.steps + a.ck - 1) / a.ck;
+  a.stage = ROWS * 128 * (GATED ? 2 : 1) + a.mp * 128;
+  // two CTAs an SM, unless that leaves a CTA fewer than three stages
+  int room = HALF_ROOM;
+  if (room / a.stage < 3) room = ROOM;
+  a.stages = room / a.stage < MAX_STAGES ? room / a.stage : MAX_STAGES;
+  if (a.stages > a.per) a.stages = a.per;
+  const int want = a.mp * (GATED ? 2 : 1);
+  a.cols = 32;
+  while (a.cols < want) a.cols *= 2;
+  const int token = ROWS * 4 * (GATED ? 2 : 1);
+  int smem = a.stages * a.stage;
+  a.round = a.mp;
+  if (a.ck > 1) {
+    if (smem < a.mp * token) smem = a.mp * token < room ? a.mp * token : room;   // (a short K: few stages)
+    if (a.round * token > smem) a.round = smem / token / 16 * 16;
+  }
+  smem += 1024;
+  a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
+            (uint32_t)WMN << 15 | (uint32_t)(a.mp >> 3) << 17 | (uint32_t)(ROWS >> 4) << 24;
+  a.e = p.e;
+  auto kern = few_product<F8, WMN, GATED>;
+  int dev = 0;
+  VERACE_CUDA(cudaGetDevice(&dev));
+  static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ROOM + 1024));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * a.ck));
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.ck;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.ck > 1 ? 1 : 0;
+  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, maps, a));
+  return check_launch("few_product");
+}
+
+}  // namespace
+
+namespace lin {
+
+int product_few(const Product& p, cudaStream_t st) {
+  if (p.type == VERACE_E4M3) return p.gated ? launch<true, false, true>(p, st) : launch<true, false, false>(p, st);
+  if (p.gated) return launch<false, false, true>(p, st);
+  return p.b_mn ? launch<false, true, false>(p, st) : launch<false, false, false>(p, st);
+}
+
+}  // namespace lin
+
+int linear_few_read_status(int* status) {
+  int h = 0;
+  VERACE_CUDA(cudaMemcpyFromSymbol(&h, g_linear_few_status, sizeof(int)));
+  if (h) {
+    const int zero = 0;
+    VERACE_CUDA(cudaMemcpyToSymbol(g_linear_few_status, &zero, sizeof(int)));
+  }
+  *status = h;
+  return VERACE_OK;
+}
+
+}  // namespace verace

@@ -20,8 +20,6 @@
 // applies scales, bias and activation, and the warp turns the rounded values over in shared memory so
 // that a store is 128 neighbouring bytes; residuals come in the same way.
 #include "linear_tc.cuh"
-#include "tc.cuh"
-#include "tmap.cuh"
 
 #include <atomic>
 
@@ -100,21 +98,6 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// 16 columns of this thread's TMEM row, without waiting for them
-__device__ __forceinline__ void tmem_ld16_async(uint32_t addr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-}
-// waits for the loads; the registers pass through so that nothing reads them earlier
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-}
-
 // ------------------------------------------------------------------ the epilogue's stores and loads
 // A warp's 32 rows of 32 words, the word `lane` of row r at turn[33 r + lane]: for 16-bit types 64
 // columns, two to a word.
@@ -122,13 +105,6 @@ struct Block {
   uint32_t* turn;
   long long m0, n0, M, N;   // first row and column; ends
 };
-
-__device__ __forceinline__ uint32_t pack_pair(float a, float b, int type) {
-  return type == VERACE_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
-}
-__device__ __forceinline__ float2 unpack_pair(uint32_t w, int type) {
-  return type == VERACE_BF16 ? unpack2<__nv_bfloat16>(w) : unpack2<__half>(w);
-}
 
 // the block to `p` (rows `ld` values apart, values of `size` bytes)
 __device__ __forceinline__ void write_block(const Block& b, void* p, long long ld, bool wide, int lane) {
@@ -478,24 +454,6 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
 }
 
 // ------------------------------------------------------------------ host
-// boxes of 128 bytes x `rows`
-int operand_map(CUtensorMap* map, const Mat& m, int type, int rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc = tmap_encoder();
-  VERACE_REQUIRE(enc, VERACE_ERR_CUDA, "linear: the driver has no cuTensorMapEncodeTiled");
-  const size_t es = size_of(type);
-  const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.pieces};
-  const cuuint64_t strides[2] = {m.ld * es, (m.pieces > 1 ? m.piece : m.ld) * es};
-  const cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)rows, 1}, el[3] = {1, 1, 1};
-  const CUtensorMapDataType dt = type == VERACE_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                 : type == VERACE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUresult r = enc(map, dt, 3, const_cast<void*>(m.p), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  VERACE_REQUIRE(r == CUDA_SUCCESS, VERACE_ERR_CUDA, "linear: tensor map of %lld x %lld (stride %lld) refused (%d)", m.rows,
-                 m.cols, m.ld, (int)r);
-  return VERACE_OK;
-}
-
 template <bool F8, bool AMN, bool BMN, bool GATED, int BN>
 int launch(const Product& p, cudaStream_t st) {
   using S = Shape<BN>;
@@ -548,6 +506,23 @@ int by_kind(const Product& p, cudaStream_t st) {
 }  // namespace
 
 namespace lin {
+
+int operand_map(CUtensorMap* map, const Mat& m, int type, int rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tmap_encoder();
+  VERACE_REQUIRE(enc, VERACE_ERR_CUDA, "linear: the driver has no cuTensorMapEncodeTiled");
+  const size_t es = size_of(type);
+  const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.pieces};
+  const cuuint64_t strides[2] = {m.ld * es, (m.pieces > 1 ? m.piece : m.ld) * es};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)rows, 1}, el[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = type == VERACE_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : type == VERACE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = enc(map, dt, 3, const_cast<void*>(m.p), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  VERACE_REQUIRE(r == CUDA_SUCCESS, VERACE_ERR_CUDA, "linear: tensor map of %lld x %lld (stride %lld) refused (%d)", m.rows,
+                 m.cols, m.ld, (int)r);
+  return VERACE_OK;
+}
 
 int product_large(const Product& p, cudaStream_t st) {
   const long long wide = (p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256) * ((p.M + 255) / 256) * p.nz;

@@ -2,6 +2,8 @@
 #pragma once
 
 #include "linear.cuh"
+#include "tc.cuh"
+#include "tmap.cuh"
 
 namespace verace {
 namespace lin {
@@ -36,7 +38,35 @@ struct Product {
   Epilogue e;
 };
 
-int product_large(const Product& p, cudaStream_t st);
+int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
+int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: few rows of A
+
+// The tensor map of an operand: boxes of 128 bytes x `rows`.
+int operand_map(CUtensorMap* map, const Mat& m, int type, int rows);
+
+// ------------------------------------------------------------------ device parts of both engines
+// two 16-bit values of a runtime type in a word, and back
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, int type) {
+  return type == VERACE_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
+}
+__device__ __forceinline__ float2 unpack_pair(uint32_t w, int type) {
+  return type == VERACE_BF16 ? unpack2<__nv_bfloat16>(w) : unpack2<__half>(w);
+}
+
+// 16 columns of this thread's TMEM row, without waiting for them
+__device__ __forceinline__ void tmem_ld16_async(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+// waits for the loads; the registers pass through so that nothing reads them earlier
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
 
 }  // namespace lin
 }  // namespace verace
