@@ -391,7 +391,7 @@ VERACE_API int verace_rmsnorm_fp8(const void* h, const void* y, void* sum, const
  *   [f]) fp32 stand for x_scale[i] x[i][k] and so on; NULL with the other types.
  * bias: [n] (dtype; with E4M3 out_dtype) or NULL; residual: [m, n] (out_dtype), rows ld_res apart, or NULL.
  * out: [m, n] (out_dtype: dtype or VERACE_F32; with E4M3 any of the three), dense; may be the residual.
- * pre (gate and up): NULL, or [m, n] (out_dtype), dense: the sums before the activation (linear: with the
+ * pre (gate and up): NULL, or [m, n] fp32, dense: the sums before the activation (linear: with the
  *   bias), which the backward call reads.
  * Backward, from dout [m, n] (out_dtype), dense: dx [m, k], dw [n, k], dbias [n] (dtype, dense; NULL: not
  *   computed); the residual's gradient is dout.  pre may be NULL with VERACE_ACT_NONE.
@@ -406,21 +406,21 @@ enum {
 VERACE_API size_t verace_linear_workspace(long long m, int n, int k, int dtype);
 VERACE_API int verace_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
                              const float* w_scale, const void* bias, const void* residual, long long ld_res, void* out,
-                             void* pre, long long m, int n, int k, int act, int dtype, int out_dtype, void* workspace,
+                             float* pre, long long m, int n, int k, int act, int dtype, int out_dtype, void* workspace,
                              size_t workspace_bytes, void* stream);
 VERACE_API size_t verace_linear_backward_workspace(long long m, int n, int k, int dtype);
 VERACE_API int verace_linear_backward(const void* dout, const void* x, long long ldx, const void* w, long long ldw,
-                                      const void* pre, void* dx, void* dw, void* dbias, long long m, int n, int k, int act,
+                                      const float* pre, void* dx, void* dw, void* dbias, long long m, int n, int k, int act,
                                       int dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 VERACE_API size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype);
 VERACE_API int verace_gated_linear(const void* x, long long ldx, const float* x_scale, const void* w_gate,
                                    const void* w_up, long long ldw, const float* gate_scale, const float* up_scale,
-                                   void* out, void* gate, void* up, long long m, int f, int k, int act, float beta1,
+                                   void* out, float* gate, float* up, long long m, int f, int k, int act, float beta1,
                                    float beta2, int dtype, int out_dtype, void* workspace, size_t workspace_bytes,
                                    void* stream);
 VERACE_API size_t verace_gated_linear_backward_workspace(long long m, int f, int k, int dtype);
 VERACE_API int verace_gated_linear_backward(const void* dout, const void* x, long long ldx, const void* w_gate,
-                                            const void* w_up, long long ldw, const void* gate, const void* up, void* dx,
+                                            const void* w_up, long long ldw, const float* gate, const float* up, void* dx,
                                             void* dw_gate, void* dw_up, long long m, int f, int k, int act, float beta1,
                                             float beta2, int dtype, int out_dtype, void* workspace,
                                             size_t workspace_bytes, void* stream);

@@ -12,7 +12,7 @@ import math
 
 import torch
 
-F64 = torch.float64
+F64, F32 = torch.float64, torch.float32
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 B1, B2 = 4.0, 25.0
 
@@ -79,13 +79,13 @@ def slopes64(f, z):
 
 
 def gated_backward64(x, wg, wu, act, d, odt):
-    """[(gradient, tolerance)] of x, w_gate, w_up: the saved sums are rounded to odt, dg and du to x's
-    type; both enter the products as they are."""
-    dt, e, es = x.dtype, HALF[x.dtype], HALF[odt]
+    """[(gradient, tolerance)] of x, w_gate, w_up: the sums are kept in fp32, dg and du are rounded to x's
+    type before they enter the products."""
+    dt, e, es = x.dtype, HALF[x.dtype], HALF[F32]
     x, wg, wu, d = (t.to(F64) for t in (x, wg, wu, d))
     g, tg = product64(x, wg)
     u, tu = product64(x, wu)
-    tg, tu = tg + es * g.abs() + tiny(odt), tu + es * u.abs() + tiny(odt)
+    tg, tu = tg + es * g.abs(), tu + es * u.abs()
     a, b = act64(act, g), up64(act, u)
     da, db = slopes64(lambda z: act64(act, z), g), slopes64(lambda z: up64(act, z), u)
     dg, du = d * da * b, d * a * db
@@ -107,12 +107,12 @@ def gated_backward64(x, wg, wu, act, d, odt):
 
 def linear_backward64(x, w, bias, act, d, odt):
     """[(gradient, tolerance)] of x, w, bias."""
-    dt, e, es = x.dtype, HALF[x.dtype], HALF[odt]
+    dt, e, es = x.dtype, HALF[x.dtype], HALF[F32]
     x, w, d = (t.to(F64) for t in (x, w, d))
     z, tz = product64(x, w)
     if bias is not None:
         z = z + bias.to(F64)
-    tz = 2 * tz + es * z.abs() + tiny(odt)
+    tz = 2 * tz + es * z.abs()
     p = d * slopes64(lambda v: act64(act, v), z)
     soft = 0.0 if act in (None, "relu") else 1.2
     tp = d.abs() * (soft * tz + (0.0 if act in (None, "relu") else 8 * act_error(odt))) + e * p.abs() + tiny(dt)

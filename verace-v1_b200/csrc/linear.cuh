@@ -128,9 +128,10 @@ inline size_t size_of(int type) { return type == VERACE_F32 ? 4 : type == VERACE
 struct Epilogue {
   const float *row_scale, *col_scale, *up_scale;   // of 8-bit operands, or null
   const void *bias, *residual;                     // or null
-  void *out, *pre, *pre_up;                        // pre: the sums before the activation, for a backward pass
+  void* out;
+  float *pre, *pre_up;                             // the sums before the activation in fp32, for a backward pass, or null
   long long ld, ld_res;                            // row strides of out and pre, and of the residual
-  int bias_type, type, act;                        // type: of out, pre and the residual
+  int bias_type, type, act;                        // type: of out and the residual
   float b1, b2, r1, r2;                            // r = 1 / b
 };
 

@@ -103,8 +103,8 @@ __device__ __forceinline__ void finish4(const Epilogue& e, long long m, long lon
     for (int j = 0; j < 4; ++j) g[j] += b[j];
   }
   if (e.pre) {
-    store4(e.pre, m * e.ld + c, n, e.type, g);
-    if (GATED) store4(e.pre_up, m * e.ld + c, n, e.type, u);
+    store4(e.pre, m * e.ld + c, n, VERACE_F32, g);
+    if (GATED) store4(e.pre_up, m * e.ld + c, n, VERACE_F32, u);
   }
   by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
 #pragma unroll
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], done;
   __shared__ uint32_t slot;
   __shared__ volatile int fail;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int unit = blockIdx.x / p.ck, rank = blockIdx.x - unit * p.ck;
   const int tile_m = unit / p.tiles_n, tile_n = unit - tile_m * p.tiles_n;
   const int n0 = tile_n * ROWS;
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
       int i = 0, flying = 0, seg = first / p.kblocks, kb = first - seg * p.kblocks;
       uint32_t phase = 0;
       for (int s = first; s < last; ++s) {
-        if (fail || !tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {
+        if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {
           fail = 1;
           atomicExch(&g_linear_few_status, 1);
           break;
@@ -179,18 +179,19 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
         tc::mbar_wait(&full[--i], phase, POLLS);
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0) {   // ---- MMAs
-      int i = 0;
-      uint32_t phase = 0;
-      for (int s = first; s < last; ++s) {
-        if (fail || !tc::mbar_wait(&full[i], phase, POLLS)) {
-          fail = 1;
-          atomicExch(&g_linear_few_status, 1);
-          break;
-        }
-        tc::fence_after_sync();
-        const uint32_t w = tc::smem_addr(sm + i * p.stage), x = w + WB;
+  } else if (warp == 1) {   // ---- MMAs (the whole warp walks the loop: the operands sit in uniform registers)
+    const bool lead = elect();
+    int i = 0;
+    uint32_t phase = 0;
+    for (int s = first; s < last; ++s) {
+      if (!tc::mbar_wait(&full[i], phase, POLLS)) {
+        fail = 1;
+        if (lane == 0) atomicExch(&g_linear_few_status, 1);
+        break;
+      }
+      tc::fence_after_sync();
+      const uint32_t w = tc::smem_addr(sm + i * p.stage), x = w + WB;
+      if (lead) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint64_t dx = tc::sdesc_sw128(x + k * 32, 16, 1024);
@@ -200,11 +201,13 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
           if (GATED) mma<F8>(tmem + p.mp, tc::sdesc_sw128(w + ROWS * 128 + k * 32, 16, 1024), dx, p.idesc, more);
         }
         tc::commit(&empty[i]);
-        if (++i == p.stages) i = 0, phase ^= 1;
       }
-      tc::commit(&done);
-      tc::mbar_wait(&done, 0, POLLS);   // (every MMA issued completes before the CTA may end)
+      __syncwarp();
+      if (++i == p.stages) i = 0, phase ^= 1;
     }
+    if (lead) tc::commit(&done);
+    __syncwarp();
+    tc::mbar_wait(&done, 0, POLLS);   // (every MMA issued completes before the CTA may end)
   }
   __syncwarp();
   // ---- the sums
@@ -226,8 +229,8 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
       const float bias = !GATED && e.bias && in ? load_as(e.bias, n, e.bias_type) : 0.f;
       for (int t = 0; t < tokens; t += 16) {
         uint32_t r[16], s[16];
-        tmem_ld16_async(mine + t, r);
-        if (GATED) tmem_ld16_async(mine + p.mp + t, s);
+        tmem_ld_async(mine + t, r);
+        if (GATED) tmem_ld_async(mine + p.mp + t, s);
         float res[16];
         if (!GATED && e.residual) {
 #pragma unroll
@@ -252,8 +255,8 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (t + j < tokens) {
-              store_as(e.pre, (m0 + t + j) * e.ld + n, g[j], e.type);
-              if (GATED) store_as(e.pre_up, (m0 + t + j) * e.ld + n, u[j], e.type);
+              e.pre[(m0 + t + j) * e.ld + n] = g[j];
+              if (GATED) e.pre_up[(m0 + t + j) * e.ld + n] = u[j];
             }
         }
         by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
 #pragma unroll
           for (int h = 0; h < (GATED ? 2 : 1); ++h) {
             uint32_t r[16];
-            tmem_ld16_async(mine + h * p.mp + t0 + t, r);
+            tmem_ld_async(mine + h * p.mp + t0 + t, r);
             tmem_wait(r);
             float* o = part + (h * p.round + t) * ROWS + 32 * quarter + lane;
 #pragma unroll

@@ -98,174 +98,6 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// ------------------------------------------------------------------ the epilogue's stores and loads
-// A warp's 32 rows of 32 words, the word `lane` of row r at turn[33 r + lane]: for 16-bit types 64
-// columns, two to a word.
-struct Block {
-  uint32_t* turn;
-  long long m0, n0, M, N;   // first row and column; ends
-};
-
-// the block to `p` (rows `ld` values apart, values of `size` bytes)
-__device__ __forceinline__ void write_block(const Block& b, void* p, long long ld, bool wide, int lane) {
-  __syncwarp();
-  const int rows = (int)min(32LL, b.M - b.m0);
-  if (wide) {                                  // fp32
-    const long long n = b.n0 + lane;
-    float* o = static_cast<float*>(p) + b.m0 * ld + n;
-    if (n < b.N)
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r, o += ld) *o = __uint_as_float(b.turn[33 * r + lane]);
-  } else {
-    const long long n = b.n0 + 2 * lane;
-    unsigned short* o = static_cast<unsigned short*>(p) + b.m0 * ld + n;
-    if (((ld & 1) | ((size_t)p & 3)) == 0 && n + 1 < b.N) {
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r, o += ld) *reinterpret_cast<uint32_t*>(o) = b.turn[33 * r + lane];
-    } else if (n < b.N) {
-      for (int r = 0; r < rows; ++r, o += ld) {
-        const uint32_t w = b.turn[33 * r + lane];
-        o[0] = (unsigned short)w;
-        if (n + 1 < b.N) o[1] = (unsigned short)(w >> 16);
-      }
-    }
-  }
-  __syncwarp();
-}
-// and from `p`
-__device__ __forceinline__ void read_block(const Block& b, const void* p, long long ld, bool wide, int lane) {
-  const int rows = (int)min(32LL, b.M - b.m0);
-  if (wide) {
-    const long long n = b.n0 + lane;
-    const float* o = static_cast<const float*>(p) + b.m0 * ld + n;
-    if (n < b.N)
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r, o += ld) b.turn[33 * r + lane] = __float_as_uint(*o);
-  } else {
-    const long long n = b.n0 + 2 * lane;
-    const unsigned short* o = static_cast<const unsigned short*>(p) + b.m0 * ld + n;
-    if (((ld & 1) | ((size_t)p & 3)) == 0 && n + 1 < b.N) {
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r, o += ld) b.turn[33 * r + lane] = *reinterpret_cast<const uint32_t*>(o);
-    } else if (n < b.N) {
-      for (int r = 0; r < rows; ++r, o += ld)
-        b.turn[33 * r + lane] = o[0] | (n + 1 < b.N ? (uint32_t)o[1] << 16 : 0u);
-    }
-  }
-  __syncwarp();
-}
-
-// 16 values into the thread's own row of the block, from column c on
-__device__ __forceinline__ void put16(const Block& b, int c, const float (&v)[16], int type, int lane) {
-  uint32_t* t = b.turn + 33 * lane;
-  if (type == VERACE_F32) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) t[c + j] = __float_as_uint(v[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[c / 2 + j] = pack_pair(v[2 * j], v[2 * j + 1], type);
-  }
-}
-__device__ __forceinline__ void add16(const Block& b, int c, float (&v)[16], int type, int lane) {
-  const uint32_t* t = b.turn + 33 * lane;
-  if (type == VERACE_F32) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(t[c + j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 f = unpack_pair(t[c / 2 + j], type);
-      v[2 * j] += f.x;
-      v[2 * j + 1] += f.y;
-    }
-  }
-}
-
-// 16 sums of one row, columns n0 ...: what the epilogue asks for before the activation
-__device__ __forceinline__ void scaled16(const Epilogue& e, const uint32_t (&r)[16], float (&v)[16], float rs,
-                                         const float* col_scale, const void* bias, long long n0, long long N) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-  if (col_scale) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= rs * (n0 + j < N ? col_scale[n0 + j] : 0.f);
-  }
-  if (bias) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] += n0 + j < N ? load_as(bias, n0 + j, e.bias_type) : 0.f;
-  }
-}
-
-// One block of `width` columns from TMEM column `col` (the second sums at `col_up`) on.
-template <bool GATED>
-__device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b, uint32_t tmem, int col, int col_up,
-                                               void* out, int lane) {
-  const bool wide = e.type == VERACE_F32;
-  const int width = wide ? 32 : 64;
-  const long long m = b.m0 + lane;
-  const float rs = e.row_scale && m < b.M ? e.row_scale[m] : 0.f;
-  if constexpr (!GATED) {
-    // saved sums go out in a pass of their own: the block's place is one
-    if (e.pre) {
-      for (int c = 0; c < width; c += 16) {
-        uint32_t r[16];
-        tmem_ld16_async(tmem + col + c, r);
-        tmem_wait(r);
-        float v[16];
-        scaled16(e, r, v, rs, e.col_scale, e.bias, b.n0 + c, b.N);
-        put16(b, c, v, e.type, lane);
-      }
-      write_block(b, e.pre, e.ld, wide, lane);
-    }
-    if (e.residual) read_block(b, e.residual, e.ld_res, wide, lane);
-    for (int c = 0; c < width; c += 16) {
-      uint32_t r[16];
-      tmem_ld16_async(tmem + col + c, r);
-      tmem_wait(r);
-      float v[16];
-      scaled16(e, r, v, rs, e.col_scale, e.bias, b.n0 + c, b.N);
-      by_act(e.act, !wide, [&](auto act, auto fast) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = act_<decltype(act)::value, decltype(fast)::value>(v[j]);
-      });
-      if (e.residual) add16(b, c, v, e.type, lane);
-      put16(b, c, v, e.type, lane);
-    }
-  } else {
-    if (e.pre) {
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        for (int c = 0; c < width; c += 16) {
-          uint32_t r[16];
-          tmem_ld16_async(tmem + (h ? col_up : col) + c, r);
-          tmem_wait(r);
-          float v[16];
-          scaled16(e, r, v, rs, h ? e.up_scale : e.col_scale, nullptr, b.n0 + c, b.N);
-          put16(b, c, v, e.type, lane);
-        }
-        write_block(b, h ? e.pre_up : e.pre, e.ld, wide, lane);
-      }
-    }
-    for (int c = 0; c < width; c += 16) {
-      uint32_t r[16], s[16];
-      tmem_ld16_async(tmem + col + c, r);
-      tmem_ld16_async(tmem + col_up + c, s);
-      tmem_wait(r);
-      tmem_wait(s);
-      float g[16], u[16];
-      scaled16(e, r, g, rs, e.col_scale, nullptr, b.n0 + c, b.N);
-      scaled16(e, s, u, rs, e.up_scale, nullptr, b.n0 + c, b.N);
-      by_act(e.act, !wide, [&](auto act, auto fast) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
-      });
-      put16(b, c, g, e.type, lane);
-    }
-  }
-  write_block(b, out, e.ld, wide, lane);
-}
-
 // tile t -> (z, row, column) of tiles: groups of eight rows, column by column
 struct Place {
   int z, m, n;
@@ -282,13 +114,240 @@ __device__ __forceinline__ Place place(const Args& p, int t) {
   return o;
 }
 
+// ------------------------------------------------------------------ the epilogue
+// A warp's block: 32 rows of 32 words, the word `lane` of row r at turn[33 r + lane]: 32 columns of fp32, or
+// 64 of 16-bit types, two to a word.
+struct Block {
+  uint32_t* turn;
+  long long m0, n0, M, N;   // first row and column; ends
+};
+
+// Where a warp reads or writes a block: row by row, a word (or its two halves) a lane.
+struct Rows {
+  char* at;           // the lane's word in the first row
+  long long step;     // bytes of a row
+  int rows;           // rows inside
+  int part;           // 0: no column of the lane inside, 1: its first half, 2: two halves, 3: a word
+};
+template <bool WIDE>
+__device__ __forceinline__ Rows rows_of(const Block& b, const void* p, long long ld, int lane) {
+  constexpr int SIZE = WIDE ? 4 : 2, PER = WIDE ? 1 : 2;
+  const long long n = b.n0 + PER * lane;
+  Rows r;
+  r.at = (char*)p + (b.m0 * ld + n) * SIZE;
+  r.step = ld * SIZE;
+  r.rows = (int)min(32LL, b.M - b.m0);
+  if (WIDE) r.part = n < b.N ? 3 : 0;
+  else r.part = n >= b.N ? 0 : n + 1 == b.N ? 1 : ((r.step | (size_t)r.at) & 3) == 0 ? 3 : 2;
+  return r;
+}
+// the block to p
+template <bool WIDE>
+__device__ __forceinline__ void write_block(const Block& b, void* p, long long ld, int lane) {
+  __syncwarp();
+  Rows r = rows_of<WIDE>(b, p, ld, lane);
+  const uint32_t* t = b.turn + lane;
+  if (r.part == 3 && r.rows == 32) {
+#pragma unroll 16
+    for (int i = 0; i < 32; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = t[33 * i];
+  } else if (r.part) {
+    for (int i = 0; i < r.rows; ++i, r.at += r.step) {
+      const uint32_t w = t[33 * i];
+      if (r.part == 3) {
+        *reinterpret_cast<uint32_t*>(r.at) = w;
+      } else {
+        reinterpret_cast<unsigned short*>(r.at)[0] = (unsigned short)w;
+        if (r.part == 2) reinterpret_cast<unsigned short*>(r.at)[1] = (unsigned short)(w >> 16);
+      }
+    }
+  }
+  __syncwarp();
+}
+// the words of a block of p, all loads in flight together
+template <bool WIDE>
+__device__ __forceinline__ void read_words(const Block& b, const void* p, long long ld, int lane, uint32_t (&w)[32]) {
+  const Rows r = rows_of<WIDE>(b, p, ld, lane);
+  if (r.part == 3) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] = i < r.rows ? *reinterpret_cast<const uint32_t*>(r.at + i * r.step) : 0u;
+  } else if (r.part) {
+    const int second = r.part == 2 ? 1 : 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      w[i] = i < r.rows ? reinterpret_cast<const unsigned short*>(r.at + i * r.step)[0] : 0u;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (second && i < r.rows) w[i] |= (uint32_t)reinterpret_cast<const unsigned short*>(r.at + i * r.step)[1] << 16;
+  }
+}
+// U values into the thread's own row of the block, from column c on
+template <bool WIDE, int U>
+__device__ __forceinline__ void put(const Block& b, int c, const float (&v)[U], int type, int lane) {
+  uint32_t* t = b.turn + 33 * lane;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) t[c + j] = __float_as_uint(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < U / 2; ++j) t[c / 2 + j] = pack_pair(v[2 * j], v[2 * j + 1], type);
+  }
+}
+template <bool WIDE, int U>
+__device__ __forceinline__ void add(const Block& b, int c, float (&v)[U], int type, int lane) {
+  const uint32_t* t = b.turn + 33 * lane;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] += __uint_as_float(t[c + j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < U / 2; ++j) {
+      const float2 f = unpack_pair(t[c / 2 + j], type);
+      v[2 * j] += f.x;
+      v[2 * j + 1] += f.y;
+    }
+  }
+}
+// U sums of a row from column n0 on, with scales and bias
+template <int U>
+__device__ __forceinline__ void scaled(const Epilogue& e, const uint32_t (&r)[U], float (&v)[U], float rs,
+                                       const float* col_scale, const void* bias, long long n0, long long N) {
+#pragma unroll
+  for (int j = 0; j < U; ++j) v[j] = __uint_as_float(r[j]);
+  if (col_scale) {
+    float s[U];
+    column_values(col_scale, VERACE_F32, n0, N, s);
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] *= rs * s[j];
+  }
+  if (bias) {
+    float s[U];
+    column_values(bias, e.bias_type, n0, N, s);
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] += s[j];
+  }
+}
+
+// The saved sums of `width` columns, in fp32: 32 columns at a time.
+__device__ __forceinline__ void save_sums(const Epilogue& e, Block b, uint32_t tmem, int width, float rs, const float* col_scale,
+                                          const void* bias, void* out, int lane) {
+  for (int c = 0; c < width && b.n0 < b.N; c += 32, b.n0 += 32) {
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      uint32_t r[16];
+      tmem_ld_async(tmem + c + h, r);
+      tmem_wait(r);
+      float v[16];
+      scaled(e, r, v, rs, col_scale, bias, b.n0 + h, b.N);
+      put<true>(b, h, v, VERACE_F32, lane);
+    }
+    write_block<true>(b, out, e.ld, lane);
+  }
+}
+
+// One block from TMEM address `tmem` (the second sums at `tmem_up`) on, its residual in `res`; the sums of
+// the next columns are on their way while one lot is worked on.  `loaded` is called once the
+// block's sums are in registers.
+template <bool GATED, bool WIDE, typename F>
+__device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b, uint32_t tmem, uint32_t tmem_up,
+                                               const uint32_t (&res)[32], void* out, int lane, F&& loaded) {
+  constexpr int WIDTH = WIDE ? 32 : 64, U = 16, LOTS = WIDTH / U;
+  const long long m = b.m0 + lane;
+  const float rs = e.row_scale && m < b.M ? e.row_scale[m] : 0.f;
+  if (e.pre) {
+    save_sums(e, b, tmem, WIDTH, rs, e.col_scale, GATED ? nullptr : e.bias, e.pre, lane);
+    if (GATED) save_sums(e, b, tmem_up, WIDTH, rs, e.up_scale, nullptr, e.pre_up, lane);
+  }
+  uint32_t r[2][U], s[2][U];
+  tmem_ld_async(tmem, r[0]);
+  if constexpr (GATED) tmem_ld_async(tmem_up, s[0]);
+  if (!GATED && e.residual) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) b.turn[33 * i + lane] = res[i];
+    __syncwarp();
+  }
+#pragma unroll
+  for (int l = 0; l < LOTS; ++l) {
+    tmem_wait(r[l & 1]);
+    if constexpr (GATED) tmem_wait(s[l & 1]);
+    if (l + 1 < LOTS) {
+      tmem_ld_async(tmem + (l + 1) * U, r[(l + 1) & 1]);
+      if constexpr (GATED) tmem_ld_async(tmem_up + (l + 1) * U, s[(l + 1) & 1]);
+    } else {
+      loaded();
+    }
+    float v[U];
+    scaled(e, r[l & 1], v, rs, e.col_scale, GATED ? nullptr : e.bias, b.n0 + l * U, b.N);
+    if constexpr (GATED) {
+      float u[U];
+      scaled(e, s[l & 1], u, rs, e.up_scale, nullptr, b.n0 + l * U, b.N);
+      by_act(e.act, !WIDE, [&](auto act, auto fast) {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          v[j] = gate_<decltype(act)::value, decltype(fast)::value>(v[j], u[j], e.b1, e.b2, e.r1, e.r2);
+      });
+    } else {
+      by_act(e.act, !WIDE, [&](auto act, auto fast) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = act_<decltype(act)::value, decltype(fast)::value>(v[j]);
+      });
+      if (e.residual) add<WIDE>(b, l * U, v, e.type, lane);
+    }
+    put<WIDE>(b, l * U, v, e.type, lane);
+  }
+  write_block<WIDE>(b, out, e.ld, lane);
+}
+
+// A warp's part of every tile of the pair: TMEM lanes 32 (warp % 4) ..., one half of the columns.
+template <bool GATED, bool WIDE, int BN, typename Wait, typename Free>
+__device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t* turn, uint32_t tmem, int pair, int pairs, int rank,
+                                               int warp, int lane, Wait&& wait, Free&& release) {
+  constexpr int HB = BN / 2, TN = GATED ? HB : BN, WIDTH = WIDE ? 32 : 64, PER = TN / 2 > WIDTH ? TN / 2 : WIDTH;
+  const int half = (warp - 4) >> 2, first = half * PER, last = min(TN, first + PER);
+  const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  Block b;
+  b.turn = turn;
+  b.M = p.M;
+  b.N = p.N;
+  int n = 0;
+  for (int t = pair; t < p.tiles; t += pairs, ++n) {
+    const Place at = place(p, t);
+    b.m0 = at.m * 256LL + rank * 128 + 32 * (warp & 3);
+    b.n0 = (long long)at.n * TN + first;
+    void* out = p.nz > 1 ? p.out_z[at.z] : p.e.out;
+    uint32_t res[32];
+    if (!GATED && p.e.residual && b.m0 < b.M && b.n0 < b.N && first < last)   // on its way while the products run
+      read_words<WIDE>(b, p.e.residual, p.e.ld_res, lane, res);
+    if (!wait(n)) break;
+    const uint32_t sums = lanes + (n & 1) * BN;
+    bool held = true;
+    for (int c = first; c < last; c += WIDTH) {
+      b.n0 = (long long)at.n * TN + c;
+      if (b.m0 >= b.M || b.n0 >= b.N) break;
+      uint32_t next[32];
+      Block after = b;
+      after.n0 += WIDTH;
+      const bool more = c + WIDTH < last && after.n0 < b.N;
+      if (!GATED && p.e.residual && more) read_words<WIDE>(after, p.e.residual, p.e.ld_res, lane, next);
+      epilogue_block<GATED, WIDE>(p.e, b, sums + c, sums + HB + c, res, out, lane, [&] {
+        if (!more) {
+          release(n);
+          held = false;
+        }
+      });
+      if (!GATED && p.e.residual)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) res[i] = next[i];
+    }
+    if (held) release(n);
+  }
+}
+
 template <bool F8, bool AMN, bool BMN, bool GATED, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
 large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
   using S = Shape<BN>;
   constexpr int KB = F8 ? 128 : 64;            // values of K in a stage
   constexpr int HB = BN / 2;                   // rows of B in a CTA
-  constexpr int TN = GATED ? HB : BN;          // output columns of a tile
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((size_t)raw + 1023) & ~(size_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::BARS);
@@ -297,7 +356,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* fail = reinterpret_cast<volatile int*>(slot + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t rank = cta_in_pair();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
@@ -340,7 +399,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
           const CUtensorMap* mb = &maps.b[GATED ? rank : g.b];
           const int az = g.az * p.nz + at.z;
           for (int kb = 0; kb < p.kblocks; ++kb) {
-            if (*fail || !tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
+            if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
               ok = false;
               break;
             }
@@ -378,72 +437,67 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
         }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {   // ---- MMAs of the pair
+    if (rank == 0) {   // ---- MMAs of the pair.  The whole warp walks the loop, so that the operands sit in uniform registers:
+      // by one thread's own loop a step of four MMAs took 657 clocks, the MMAs themselves take 512
+      const bool lead = elect();
       int i = 0, n = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < p.tiles && ok; t += pairs, ++n) {
         const int b = n & 1, use = n >> 1;
-        if (*fail || !tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
+        if (!tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
           ok = false;
           break;
         }
         tc::fence_after_sync();
         const uint32_t d = tmem + b * BN;
         for (int s = 0; s < steps; ++s) {
-          if (*fail || !tc::mbar_wait(&full[i], phase, POLLS)) {
+          if (!tc::mbar_wait(&full[i], phase, POLLS)) {
             ok = false;
             break;
           }
           tc::fence_after_sync();
           const uint32_t a = tc::smem_addr(sm + i * S::STAGE), bb = a + 16384;
+          if (lead) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
-            const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
-            const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
-            mma_pair<F8>(d, da, db, p.idesc, s > 0 || k > 0 ? 1u : 0u);
+            for (int k = 0; k < 4; ++k) {
+              // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
+              const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
+              const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
+              mma_pair<F8>(d, da, db, p.idesc, s > 0 || k > 0 ? 1u : 0u);
+            }
+            commit_pair(&empty[i]);
           }
-          commit_pair(&empty[i]);
+          __syncwarp();
           if (++i == S::STAGES) i = 0, phase ^= 1;
         }
-        commit_pair(&acc_full[b]);   // (also after a failure: every MMA issued completes)
+        if (lead) commit_pair(&acc_full[b]);   // (also after a failure: every MMA issued completes)
+        __syncwarp();
         if (!ok) tc::mbar_wait(&acc_full[b], use & 1, POLLS);
       }
       if (!ok) {
         *fail = 1;
-        atomicExch(&g_linear_status, 1);
+        if (lane == 0) atomicExch(&g_linear_status, 1);
       }
     }
-  } else if (warp >= 4) {   // ---- epilogue: TMEM lanes 32 (warp % 4) ..., one half of the columns
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const int width = p.e.type == VERACE_F32 ? 32 : 64, per = max(TN / 2, width);
-    Block b;
-    b.turn = reinterpret_cast<uint32_t*>(sm + S::TURNS + (warp - 4) * TURN);
-    b.M = p.M;
-    b.N = p.N;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
-    int n = 0;
-    for (int t = pair; t < p.tiles; t += pairs, ++n) {
-      const Place at = place(p, t);
-      const int buf = n & 1, use = n >> 1;
-      if (*fail || !tc::mbar_wait(&acc_full[buf], use & 1, POLLS)) {
+  } else if (warp >= 4) {   // ---- epilogue
+    uint32_t* turn = reinterpret_cast<uint32_t*>(sm + S::TURNS + (warp - 4) * TURN);
+    auto wait = [&](int n) {
+      if (!tc::mbar_wait(&acc_full[n & 1], (n >> 1) & 1, POLLS)) {
         *fail = 1;
         if (lane == 0) atomicExch(&g_linear_status, 1);
-        break;
+        return false;
       }
       tc::fence_after_sync();
-      b.m0 = at.m * 256LL + rank * 128 + 32 * quarter;
-      void* out = p.nz > 1 ? p.out_z[at.z] : p.e.out;
-      // (every warp reads its blocks even outside of the output: tcgen05.ld is the warp's as a whole)
-      for (int c = half * per; c < min(TN, (half + 1) * per); c += width) {
-        b.n0 = (long long)at.n * TN + c;
-        if (b.n0 < p.N && b.m0 < p.M) epilogue_block<GATED>(p.e, b, lanes + buf * BN, c, c + HB, out, lane);
-      }
+      return *fail == 0;
+    };
+    auto release = [&](int n) {
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) arrive_at(in_cta0(&acc_empty[buf]));
-    }
+      if (lane == 0) arrive_at(in_cta0(&acc_empty[n & 1]));
+    };
+    if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else epilogue_tiles<GATED, false, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
   }
   tc::fence_before_sync();
   __syncthreads();

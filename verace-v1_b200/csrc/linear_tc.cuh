@@ -45,6 +45,11 @@ int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: few ro
 int operand_map(CUtensorMap* map, const Mat& m, int type, int rows);
 
 // ------------------------------------------------------------------ device parts of both engines
+__device__ __forceinline__ bool elect() {   // one lane of a converged warp
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // two 16-bit values of a runtime type in a word, and back
 __device__ __forceinline__ uint32_t pack_pair(float a, float b, int type) {
   return type == VERACE_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
@@ -54,7 +59,7 @@ __device__ __forceinline__ float2 unpack_pair(uint32_t w, int type) {
 }
 
 // 16 columns of this thread's TMEM row, without waiting for them
-__device__ __forceinline__ void tmem_ld16_async(uint32_t addr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_async(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
@@ -66,6 +71,42 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                  "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
+// U values from column n0 on of a vector of N, the same ones for every lane (0 beyond the end)
+template <int U>
+__device__ __forceinline__ void column_values(const void* p, int type, long long n0, long long N, float (&v)[U]) {
+  const char* at = static_cast<const char*>(p) + n0 * (type == VERACE_F32 ? 4 : 2);
+  if (n0 + U <= N && ((size_t)at & 15) == 0) {
+    if (type == VERACE_F32) {
+#pragma unroll
+      for (int j = 0; j < U / 4; ++j) {
+        const float4 f = reinterpret_cast<const float4*>(at)[j];
+        v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < U / 8; ++j) {
+        const uint4 w = reinterpret_cast<const uint4*>(at)[j];
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack_pair(x[i], type);
+          v[8 * j + 2 * i] = f.x;
+          v[8 * j + 2 * i + 1] = f.y;
+        }
+      }
+    }
+  } else if (type == VERACE_F32) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] = n0 + j < N ? reinterpret_cast<const float*>(at)[j] : 0.f;
+  } else {
+    uint32_t w[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) w[j] = n0 + j < N ? reinterpret_cast<const unsigned short*>(at)[j] : 0u;
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] = unpack_pair(w[j], type).x;
+  }
 }
 
 }  // namespace lin

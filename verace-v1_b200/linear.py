@@ -89,7 +89,7 @@ def _p(t: Optional[torch.Tensor]):
 def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
     dev = x2.device
     y = torch.empty((m, n), dtype=out_dtype, device=dev)
-    pre = torch.empty_like(y) if want_pre else None
+    pre = torch.empty((m, n), dtype=torch.float32, device=dev) if want_pre else None
     L = lib()
     code = _CODE[x2.dtype]
     nws = L.verace_linear_workspace(m, n, k, code)
@@ -206,7 +206,7 @@ def _gate_rows(w_gate, w_up, f, k):
 def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
     dev = x2.device
     h = torch.empty((m, f), dtype=out_dtype, device=dev)
-    gate, up = (torch.empty_like(h), torch.empty_like(h)) if want_pre else (None, None)
+    gate, up = torch.empty((2, m, f), dtype=torch.float32, device=dev) if want_pre else (None, None)
     L = lib()
     code = _CODE[x2.dtype]
     nws = L.verace_gated_linear_workspace(m, f, k, code)
@@ -262,7 +262,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
 
     With float8_e4m3fn operands, ``x_scale`` (one fp32 value a row of x), ``gate_scale`` and ``up_scale`` [f]
     multiply them, and the output is fp32, bf16 (the default) or fp16.  The other types are differentiable in x, w_gate
-    and w_up (once); the pass keeps g and u, in the output's dtype, for the backward."""
+    and w_up (once); the pass keeps g and u, in fp32, for the backward."""
     dev = x.device
     if x.is_cuda and dev.index != current():
         with torch.cuda.device(dev):
