@@ -81,6 +81,35 @@ __device__ __forceinline__ void store4(void* p, long long i, int n, int type, co
   }
 }
 
+// one value of each of 16 rows `ld` apart (of `n` rows; 0 beyond), the loads in flight together
+__device__ __forceinline__ void load_rows16(const void* p, long long i, long long ld, int n, int type, float (&v)[16]) {
+  if (type == VERACE_F32) {
+    const float* f = static_cast<const float*>(p) + i;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = j < n ? f[j * ld] : 0.f;
+  } else {
+    const unsigned short* f = static_cast<const unsigned short*>(p) + i;
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = j < n ? f[j * ld] : 0u;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = unpack_pair(w[j], type).x;
+  }
+}
+__device__ __forceinline__ void store_rows16(void* p, long long i, long long ld, int n, int type, const float (&v)[16]) {
+  if (type == VERACE_F32) {
+    float* f = static_cast<float*>(p) + i;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) f[j * ld] = v[j];
+  } else {
+    unsigned short* f = static_cast<unsigned short*>(p) + i;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) f[j * ld] = (unsigned short)pack_pair(v[j], 0.f, type);
+  }
+}
+
 // four outputs of row m from their sums (u: the up projection's)
 template <bool GATED>
 __device__ __forceinline__ void finish4(const Epilogue& e, long long m, long long c, long long N, float (&g)[4], float (&u)[4]) {
@@ -135,6 +164,8 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
   const long long m0 = (long long)tile_m * p.mp;
   const int first = rank * p.per, last = min(p.steps, first + p.per);
   if (warp == 1) tc::tmem_alloc(&slot, p.cols);
+  if (warp == 2 && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 2 ? &maps.x : &maps.w[lane]) : "memory");
   if (tid == 0) {
     for (int i = 0; i < p.stages; ++i) {
       tc::mbar_init(&full[i], 1);
@@ -231,12 +262,9 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
         uint32_t r[16], s[16];
         tmem_ld_async(mine + t, r);
         if (GATED) tmem_ld_async(mine + p.mp + t, s);
-        float res[16];
-        if (!GATED && e.residual) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            res[j] = in && t + j < tokens ? load_as(e.residual, (m0 + t + j) * e.ld_res + n, e.type) : 0.f;
-        }
+        const int rows = in ? min(16, tokens - t) : 0;
+        float res[16] = {};
+        if (!GATED && e.residual) load_rows16(e.residual, (m0 + t) * e.ld_res + n, e.ld_res, rows, e.type, res);
         tmem_wait(r);
         if (GATED) tmem_wait(s);
         float g[16], u[16];
@@ -251,13 +279,9 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
             if (e.col_scale) u[j] *= rs * us;
           }
         }
-        if (e.pre && in) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (t + j < tokens) {
-              e.pre[(m0 + t + j) * e.ld + n] = g[j];
-              if (GATED) e.pre_up[(m0 + t + j) * e.ld + n] = u[j];
-            }
+        if (e.pre) {
+          store_rows16(e.pre, (m0 + t) * e.ld + n, e.ld, rows, VERACE_F32, g);
+          if (GATED) store_rows16(e.pre_up, (m0 + t) * e.ld + n, e.ld, rows, VERACE_F32, u);
         }
         by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
 #pragma unroll
@@ -266,11 +290,9 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
             else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
           }
         });
-        if (in) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (t + j < tokens) store_as(e.out, (m0 + t + j) * e.ld + n, !GATED && e.residual ? g[j] + res[j] : g[j], e.type);
-        }
+        for (int j = 0; j < 16; ++j) g[j] += res[j];
+        store_rows16(e.out, (m0 + t) * e.ld + n, e.ld, rows, e.type, g);
       }
     }
   } else {
