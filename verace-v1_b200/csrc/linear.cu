@@ -137,9 +137,15 @@ void add_segments(Product& p, int a, int az, int b, int parts, int step) {
     p.seg[p.segments++] = Segment{(unsigned char)a, (unsigned char)(A[i] * step + az), (unsigned char)b, B[i]};
 }
 
-// Whether a product goes to the engine that streams the weights past its rows.
-bool few_rows(const Product& p, bool parts) {
-  return !p.a_mn && p.M <= FEW;
+// Whether a forward product goes to the engine of dot products.  In fp32 that saves splitting the weights
+// (8 x 4096 x 4096: 23 us against 59; 16 tokens 38 against 59, 32 tokens 68 against 61).  In 16 and 8 bits the tensor cores
+// win where the weights' bytes count (1 x 1024 x 163840 bf16 58 us against 60, 4 x 4096 x 4096 12.3
+// against 13.5), the dot products where the launch does (1 x 1024 x 2048 bf16 3.1 us against 7.1, gated 4.2 M
+// weights 5.5 against 7.9; 1 x 4096 x 4096 8.7 against 12.3; 4 tokens of gated 4.2 M 5.4 against 8.8).
+bool by_dots(long long m, long long n, long long k, int type, int weights) {
+  if (k == 0 || n > 65535LL * 8) return false;
+  if (type == VERACE_F32) return m <= 16;
+  return m <= 4 && n * k * weights <= (m == 1 ? 24LL << 20 : 6LL << 20);
 }
 
 int run_product(Product& p, cudaStream_t st) {
@@ -155,9 +161,12 @@ int run_product(Product& p, cudaStream_t st) {
     }
     return VERACE_OK;
   }
-  const bool parts = p.type == VERACE_F32;
-  if (parts) p.type = VERACE_BF16;
-  return few_rows(p, parts) ? product_few(p, st) : product_large(p, st);
+  if (p.type == VERACE_F32) {
+    p.type = VERACE_BF16;
+    p.parts = true;
+    return product_large(p, st);
+  }
+  return !p.a_mn && p.M <= FEW ? product_few(p, st) : product_large(p, st);
 }
 
 // ------------------------------------------------------------------ backward of the epilogues
@@ -311,7 +320,7 @@ using namespace verace;
 using namespace verace::lin;
 
 extern "C" size_t verace_linear_workspace(long long m, int n, int k, int dtype) {
-  if (m <= 0 || n <= 0 || k <= 0 || dtype != VERACE_F32) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || dtype != VERACE_F32 || by_dots(m, n, k, dtype, 1)) return 0;
   return operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype) + 256;
 }
 
@@ -337,6 +346,11 @@ extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale,
   p.e.row_scale = x_scale; p.e.col_scale = w_scale; p.e.bias = bias; p.e.residual = residual; p.e.ld_res = ld_res;
   p.e.pre = pre; p.e.act = act;
   p.e.bias_type = dtype == VERACE_E4M3 ? out_dtype : dtype;
+  if (by_dots(m, n, k, dtype, 1)) {
+    p.a[0] = Mat{x, m, k, ldx, 1, 0};
+    p.b[0] = Mat{w, n, k, ldw, 1, 0};
+    return product_dot(p, st);
+  }
   if (k > 0 && ((rc = operand(&p.a[0], x, ldx, m, k, dtype, ws, st)) || (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st))))
     return rc;
   add_segments(p, 0, 0, 0, dtype == VERACE_F32 ? 3 : 1, 1);
@@ -418,7 +432,7 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
 }
 
 extern "C" size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype) {
-  if (m <= 0 || f <= 0 || k <= 0 || dtype != VERACE_F32) return 0;
+  if (m <= 0 || f <= 0 || k <= 0 || dtype != VERACE_F32 || by_dots(m, f, k, dtype, 2)) return 0;
   return operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype) + 256;
 }
 
@@ -448,6 +462,12 @@ extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_
   p.e.row_scale = x_scale; p.e.col_scale = gate_scale; p.e.up_scale = up_scale;
   p.e.pre = gate; p.e.pre_up = up; p.e.act = act;
   p.e.b1 = beta1; p.e.b2 = beta2; p.e.r1 = 1.f / beta1; p.e.r2 = 1.f / beta2;
+  if (by_dots(m, f, k, dtype, 2)) {
+    p.a[0] = Mat{x, m, k, ldx, 1, 0};
+    p.b[0] = Mat{w_gate, f, k, ldw, 1, 0};
+    p.b[1] = Mat{w_up, f, k, ldw, 1, 0};
+    return product_dot(p, st);
+  }
   if (k > 0 && ((rc = operand(&p.a[0], x, ldx, m, k, dtype, ws, st)) ||
                 (rc = operand(&p.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
                 (rc = operand(&p.b[1], w_up, ldw, f, k, dtype, ws, st))))

@@ -13,8 +13,12 @@
 //
 // Gated products put 64 or 128 rows of each weight into one tile (the first CTA of the pair loads the
 // gate's, the second the up projection's), so both sums of an output lie in one TMEM row and the product is formed in
-// registers.  fp32 operands come as three bf16 parts and run over six pairs of them, the smallest first, into
-// one fp32 sum; a sum of two products (the input gradient of a gated block) is two runs over K.
+// registers.  A sum of two products (the input gradient of a gated block) is two runs over K.
+//
+// fp32 operands come as three bf16 parts and run over six pairs of them, the smallest first.  The tensor core cuts
+// its sums to fp32 after every step instead of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the
+// result); so after every 128 values of K (CHUNK stages of each pair) the epilogue's warps add the sums to a third
+// set in TMEM, rounding, while the next 128 run into the other set.
 //
 // Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
 // applies scales, bias and activation, and the warp turns the rounded values over in shared memory so
@@ -34,6 +38,8 @@ using namespace lin;
 constexpr int NT = 384, EPI_WARPS = 8;
 constexpr uint32_t POLLS = 1u << 22;
 constexpr int TURN = 32 * 33 * 4;      // a warp's place to turn 32 rows of 32 words over
+
+constexpr int CHUNK = 2;
 
 template <int BN>
 struct Shape {
@@ -317,8 +323,9 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t* turn, ui
     uint32_t res[32];
     if (!GATED && p.e.residual && b.m0 < b.M && b.n0 < b.N && first < last)   // on its way while the products run
       read_words<WIDE>(b, p.e.residual, p.e.ld_res, lane, res);
-    if (!wait(n)) break;
-    const uint32_t sums = lanes + (n & 1) * BN;
+    const int set = wait(n);
+    if (set < 0) break;
+    const uint32_t sums = lanes + set;
     bool held = true;
     for (int c = first; c < last; c += WIDTH) {
       b.n0 = (long long)at.n * TN + c;
@@ -342,12 +349,14 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t* turn, ui
   }
 }
 
-template <bool F8, bool AMN, bool BMN, bool GATED, int BN>
+template <bool F8, bool AMN, bool BMN, bool GATED, int BN, bool PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
 large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
   using S = Shape<BN>;
   constexpr int KB = F8 ? 128 : 64;            // values of K in a stage
   constexpr int HB = BN / 2;                   // rows of B in a CTA
+  constexpr int COLS = PARTS || BN == 256 ? 512 : 256;   // of TMEM: two sets of sums, of parts a third
+  static_assert(!PARTS || BN == 128, "three sets of sums");
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((size_t)raw + 1023) & ~(size_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::BARS);
@@ -361,7 +370,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(slot)), "r"(2 * BN)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(slot)), "r"(COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -382,7 +391,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = *slot;
-  const int steps = p.segments * p.kblocks;
+  const int chunk = PARTS ? CHUNK : p.kblocks, chunks = PARTS ? (p.kblocks + CHUNK - 1) / CHUNK : 1;
 
   if (warp == 0) {
     if (lane == 0) {   // ---- operands
@@ -393,12 +402,13 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
         const Place at = place(p, t);
         const int m0 = at.m * 256 + (int)rank * 128;
         const int n0 = GATED ? at.n * HB : at.n * BN + (int)rank * HB;
-        for (int s = 0; s < p.segments && ok; ++s) {
+        for (int u = 0; u < p.segments * chunks && ok; ++u) {   // (chunk by chunk, in each all segments)
+          const int s = PARTS ? u % p.segments : u, k0 = PARTS ? u / p.segments * chunk : 0;
           const Segment g = p.seg[s];
           const CUtensorMap* ma = &maps.a[g.a];
           const CUtensorMap* mb = &maps.b[GATED ? rank : g.b];
           const int az = g.az * p.nz + at.z;
-          for (int kb = 0; kb < p.kblocks; ++kb) {
+          for (int kb = k0; kb < min(k0 + chunk, p.kblocks); ++kb) {
             if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
               ok = false;
               break;
@@ -443,8 +453,10 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       int i = 0, n = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; t < p.tiles && ok; t += pairs, ++n) {
+      const int mine = (p.tiles - pair + pairs - 1) / pairs * chunks;   // sets of sums to fill
+      for (; n < mine && ok; ++n) {
         const int b = n & 1, use = n >> 1;
+        const int steps = p.segments * (PARTS ? min(chunk, p.kblocks - n % chunks * chunk) : p.kblocks);
         if (!tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
           ok = false;
           break;
@@ -482,7 +494,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
     }
   } else if (warp >= 4) {   // ---- epilogue
     uint32_t* turn = reinterpret_cast<uint32_t*>(sm + S::TURNS + (warp - 4) * TURN);
-    auto wait = [&](int n) {
+    auto filled = [&](int n) {
       if (!tc::mbar_wait(&acc_full[n & 1], (n >> 1) & 1, POLLS)) {
         *fail = 1;
         if (lane == 0) atomicExch(&g_linear_status, 1);
@@ -491,12 +503,43 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       tc::fence_after_sync();
       return *fail == 0;
     };
-    auto release = [&](int n) {
+    auto free = [&](int n) {
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) arrive_at(in_cta0(&acc_empty[n & 1]));
     };
-    if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    // tile n's sums: the TMEM column of their set, or -1
+    auto wait = [&](int n) {
+      if constexpr (!PARTS) return filled(n) ? (n & 1) * BN : -1;
+      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+      for (int c = 0; c < chunks; ++c) {
+        const int set = n * chunks + c;
+        if (!filled(set)) return -1;
+        for (int h = 0; h < BN / 2; h += 16) {   // the warp's half of the columns (gated: of both sums)
+          const int col = GATED ? (h >= HB / 2 ? HB / 2 + h : h) + (warp >= 8 ? HB / 2 : 0) : h + (warp >= 8 ? HB : 0);
+          uint32_t r[16], s[16];
+          tmem_ld_async(lanes + (set & 1) * BN + col, r);
+          if (c > 0) {
+            tmem_ld_async(lanes + 2 * BN + col, s);
+            tmem_wait(r);
+            tmem_wait(s);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(s[j]));
+          } else {
+            tmem_wait(r);
+          }
+          tmem_st(lanes + 2 * BN + col, r);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        free(set);
+      }
+      return 2 * BN;
+    };
+    auto release = [&](int n) {
+      if (!PARTS) free(n);
+    };
+    if (PARTS) epilogue_tiles<GATED, true, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
     else epilogue_tiles<GATED, false, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
   }
   tc::fence_before_sync();
@@ -504,11 +547,11 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   cluster_sync();
   tc::fence_after_sync();
   if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
 }
 
 // ------------------------------------------------------------------ host
-template <bool F8, bool AMN, bool BMN, bool GATED, int BN>
+template <bool F8, bool AMN, bool BMN, bool GATED, int BN, bool PARTS = false>
 int launch(const Product& p, cudaStream_t st) {
   using S = Shape<BN>;
   constexpr int TN = GATED ? BN / 2 : BN;
@@ -535,7 +578,7 @@ int launch(const Product& p, cudaStream_t st) {
             (uint32_t)AMN << 15 | (uint32_t)BMN << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
   a.out_z[0] = p.out_z[0]; a.out_z[1] = p.out_z[1];
   a.e = p.e;
-  auto kern = large_product<F8, AMN, BMN, GATED, BN>;
+  auto kern = large_product<F8, AMN, BMN, GATED, BN, PARTS>;
   int dev = 0;
   VERACE_CUDA(cudaGetDevice(&dev));
   static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
@@ -550,6 +593,11 @@ int launch(const Product& p, cudaStream_t st) {
 
 template <int BN>
 int by_kind(const Product& p, cudaStream_t st) {
+  if constexpr (BN == 128) {
+    if (p.parts && p.gated) return launch<false, false, false, true, BN, true>(p, st);
+    if (p.parts && p.a_mn) return launch<false, true, true, false, BN, true>(p, st);
+    if (p.parts) return p.b_mn ? launch<false, false, true, false, BN, true>(p, st) : launch<false, false, false, false, BN, true>(p, st);
+  }
   if (p.type == VERACE_E4M3)
     return p.gated ? launch<true, false, false, true, BN>(p, st) : launch<true, false, false, false, BN>(p, st);
   if (p.gated) return launch<false, false, false, true, BN>(p, st);
@@ -580,7 +628,7 @@ int operand_map(CUtensorMap* map, const Mat& m, int type, int rows) {
 
 int product_large(const Product& p, cudaStream_t st) {
   const long long wide = (p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256) * ((p.M + 255) / 256) * p.nz;
-  return wide >= 74 ? by_kind<256>(p, st) : by_kind<128>(p, st);
+  return wide >= 74 && !p.parts ? by_kind<256>(p, st) : by_kind<128>(p, st);
 }
 
 }  // namespace lin

@@ -28,6 +28,7 @@ constexpr int MAX_SEGMENTS = 12;
 // z runs over nz outputs, each of A's piece z (nz > 1: one segment, or pieces az * nz + z).
 struct Product {
   int type;             // VERACE_BF16, VERACE_F16 or VERACE_E4M3
+  bool parts;           // the operands are the parts of fp32 matrices
   long long M, N, K;
   Mat a[2], b[2];
   bool a_mn, b_mn, gated;
@@ -39,7 +40,8 @@ struct Product {
 };
 
 int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
-int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: few rows of A
+int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to 256 rows of A
+int product_dot(const Product& p, cudaStream_t st);     // linear_dot.cu: a few rows of A, fp32 operands as they are
 
 // The tensor map of an operand: boxes of 128 bytes x `rows`.
 int operand_map(CUtensorMap* map, const Mat& m, int type, int rows);
@@ -65,6 +67,13 @@ __device__ __forceinline__ void tmem_ld_async(uint32_t addr, uint32_t (&r)[16]) 
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[16]) {   // (tcgen05.wait::st is the caller's)
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 // waits for the loads; the registers pass through so that nothing reads them earlier
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
