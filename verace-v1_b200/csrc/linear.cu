@@ -9,11 +9,13 @@
 // gated, 3.0e-3 of the gradients' norm against 2.3e-3; 4 bytes a sum instead of 2), then
 // dx = p W (dg Wg + du Wu) and dW = p^T x.  W, p and x are read there as they are stored; no
 // operand is transposed in memory.  The bias gradient is summed in the pass, in fp32 and in a
-// fixed order (128 rows at a time, then the partial sums).
+// fixed order (32 rows at a time, then the partial sums).
 //
 // fp32 operands are split into three bf16 parts first (x = h + m + l, 24 bits), and the product
-// runs over the six pairs of parts down to 2^-24 of the largest (hh, hm, mh, hl, mm, lh).
+// takes the six pairs of parts down to 2^-24 of the largest (hh, hm, mh, hl, mm, lh).
 #include "linear_tc.cuh"
+
+#include <algorithm>
 
 namespace verace {
 namespace {
@@ -124,18 +126,8 @@ __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long l
   store_as(e.out, r * e.ld + c, v, e.type);
 }
 
-constexpr long long FEW = 256;
 
-// The pairs of parts that make up an fp32 product, the smallest first (other types: one).
-void add_segments(Product& p, int a, int az, int b, int parts, int step) {
-  if (parts == 1) {
-    p.seg[p.segments++] = Segment{(unsigned char)a, (unsigned char)az, (unsigned char)b, 0};
-    return;
-  }
-  constexpr unsigned char A[6] = {2, 1, 0, 1, 0, 0}, B[6] = {0, 1, 2, 0, 1, 0};
-  for (int i = 0; i < 6; ++i)
-    p.seg[p.segments++] = Segment{(unsigned char)a, (unsigned char)(A[i] * step + az), (unsigned char)b, B[i]};
-}
+constexpr long long FEW = 256;
 
 // Whether a forward product goes to the engine of dot products.  In fp32 that saves splitting the weights
 // (8 x 4096 x 4096: 23 us against 59; 16 tokens 38 against 59, 32 tokens 68 against 61).  In 16 and 8 bits the tensor cores
@@ -146,6 +138,15 @@ bool by_dots(long long m, long long n, long long k, int type, int weights) {
   if (k == 0 || n > 65535LL * 8) return false;
   if (type == VERACE_F32) return m <= 16;
   return m <= 4 && n * k * weights <= (m == 1 ? 24LL << 20 : 6LL << 20);
+}
+
+// Whether a product of operands in memory goes to the engine that streams the weights past its rows.
+bool by_few(long long M, int type, bool a_mn) { return !a_mn && type != VERACE_F32 && M <= FEW; }
+
+// Workspace of a product's partial sums.
+size_t partial_bytes(long long M, long long N, long long K, int sums, int nz, bool gated, int type, bool a_mn) {
+  const bool parts = type == VERACE_F32;
+  return by_few(M, type, a_mn) ? 0 : split_bytes(M, N, K, sums, nz, gated, parts ? VERACE_BF16 : type, parts);
 }
 
 int run_product(Product& p, cudaStream_t st) {
@@ -161,19 +162,17 @@ int run_product(Product& p, cudaStream_t st) {
     }
     return VERACE_OK;
   }
-  if (p.type == VERACE_F32) {
-    p.type = VERACE_BF16;
-    p.parts = true;
-    return product_large(p, st);
-  }
-  return !p.a_mn && p.M <= FEW ? product_few(p, st) : product_large(p, st);
+  const bool few = by_few(p.M, p.type, p.a_mn);
+  p.parts = p.type == VERACE_F32;
+  if (p.parts) p.type = VERACE_BF16;
+  return few ? product_few(p, st) : product_large(p, st);
 }
 
 // ------------------------------------------------------------------ backward of the epilogues
 // p = d act'(pre) as an operand of the products (rounded to the type of x, or in three parts), and its
-// column sums: a CTA takes 128 rows of 256 columns, a thread every eighth row of 8 columns.
+// column sums: a CTA takes 32 rows (gated: 16) of 256 columns, a thread every eighth row of 8 columns.
 // Bound: bytes (d and pre read, p written).
-constexpr int CHUNK = 128;
+constexpr int CHUNK = 32, GATED_CHUNK = 16;
 struct SlopeArgs {
   const void* d;
   const float *pre, *up;
@@ -223,13 +222,22 @@ __global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
   a.partial[chunk * a.n + n] = s;
 }
 
+// the sums of the chunks, always in the same order: 32 columns a CTA, eight runs of chunks each
 template <typename T>
 __global__ void __launch_bounds__(256) sum_chunks(const float* __restrict__ partial, long long chunks, long long n,
                                                   T* __restrict__ out) {
-  const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long c = (long long)blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (long long i = 0; i < chunks; ++i) s += partial[i * n + c];
+  if (c < n)
+#pragma unroll 8
+    for (long long i = w; i < chunks; i += 8) s += partial[i * n + c];
+  part[w][lane] = s;
+  __syncthreads();
+  if (w > 0 || c >= n) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += part[i][lane];
   out[c] = from_f32<T>(s);
 }
 
@@ -237,9 +245,9 @@ template <typename T, typename O>
 __global__ void __launch_bounds__(256) gated_slope(SlopeArgs a) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const long long chunk = blockIdx.x / a.colblocks, c = (blockIdx.x % a.colblocks) * 256LL + lane * 8;
-  const long long end = min(a.m, (chunk + 1) * CHUNK);
+  const long long end = min(a.m, (chunk + 1) * GATED_CHUNK);
   if (c >= a.ld) return;
-  for (long long r = chunk * CHUNK + w; r < end; r += 8) {
+  for (long long r = chunk * GATED_CHUNK + w; r < end; r += 8) {
     float d[8], g[8], u[8];
     load8<O>(static_cast<const O*>(a.d) + r * a.n, c, a.n, a.vec, d);
     load8<float>(a.pre + r * a.n, c, a.n, a.vec, g);
@@ -306,8 +314,8 @@ Epilogue plain_out(void* out, long long ld, int type) {
 
 long long chunks_of(long long m) { return (m + CHUNK - 1) / CHUNK; }
 
-int slope_grid(const SlopeArgs& a, unsigned* grid) {
-  const long long blocks = chunks_of(a.m) * a.colblocks;
+int slope_grid(const SlopeArgs& a, int rows, unsigned* grid) {
+  const long long blocks = (a.m + rows - 1) / rows * a.colblocks;
   VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", a.m, a.n);
   *grid = (unsigned)blocks;
   return VERACE_OK;
@@ -320,8 +328,10 @@ using namespace verace;
 using namespace verace::lin;
 
 extern "C" size_t verace_linear_workspace(long long m, int n, int k, int dtype) {
-  if (m <= 0 || n <= 0 || k <= 0 || dtype != VERACE_F32 || by_dots(m, n, k, dtype, 1)) return 0;
-  return operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype) + 256;
+  if (m <= 0 || n <= 0 || k <= 0 || by_dots(m, n, k, dtype, 1)) return 0;
+  const size_t split = dtype == VERACE_F32 ? operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype) : 0;
+  const size_t part = partial_bytes(m, n, k, 1, 1, false, dtype, false);
+  return split + part ? split + part + 256 : 0;
 }
 
 extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
@@ -347,19 +357,22 @@ extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale,
   p.e.pre = pre; p.e.act = act;
   p.e.bias_type = dtype == VERACE_E4M3 ? out_dtype : dtype;
   if (by_dots(m, n, k, dtype, 1)) {
-    p.a[0] = Mat{x, m, k, ldx, 1, 0};
+    p.a = Mat{x, m, k, ldx, 1, 0};
     p.b[0] = Mat{w, n, k, ldw, 1, 0};
     return product_dot(p, st);
   }
-  if (k > 0 && ((rc = operand(&p.a[0], x, ldx, m, k, dtype, ws, st)) || (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st))))
+  if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) || (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st))))
     return rc;
-  add_segments(p, 0, 0, 0, dtype == VERACE_F32 ? 3 : 1, 1);
+  p.segments = p.a_step = 1;
+  p.ws = ws.at;
   return run_product(p, st);
 }
 
 extern "C" size_t verace_linear_backward_workspace(long long m, int n, int k, int dtype) {
   if (m <= 0 || n <= 0) return 0;
   size_t s = operand_bytes(m, n, dtype) + align_up((size_t)chunks_of(m) * n * 4, 256) + 256;
+  // (dx and dw follow each other: one place for the partial sums of either)
+  s += std::max(partial_bytes(m, k, n, 1, 1, false, dtype, false), partial_bytes(n, k, m, 1, 1, false, dtype, true));
   if (dtype == VERACE_F32 && k > 0) s += operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype);
   return s;
 }
@@ -399,32 +412,33 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
       if (dbias) s.partial = (float*)ws.take((size_t)chunks_of(m) * n * 4);
       if (s.out || s.partial) {
         unsigned grid;
-        if ((rc = slope_grid(s, &grid))) return rc;
+        if ((rc = slope_grid(s, CHUNK, &grid))) return rc;
         linear_slope<T, O><<<grid, 256, 0, st>>>(s);
         if ((rc = check_launch("linear_slope"))) return rc;
       }
     }
     if (dbias && n > 0) {
-      sum_chunks<T><<<(n + 255) / 256, 256, 0, st>>>(s.partial, any ? chunks_of(m) : 0, n, (T*)dbias);
+      sum_chunks<T><<<(n + 31) / 32, 256, 0, st>>>(s.partial, any ? chunks_of(m) : 0, n, (T*)dbias);
       if ((rc = check_launch("sum_chunks"))) return rc;
     }
-    const int parts = split_v<T> ? 3 : 1;
     if (dx && k > 0) {
       Product d{};
       d.type = dtype; d.M = m; d.N = k; d.K = n; d.nz = 1; d.b_mn = true;
       d.e = plain_out(dx, k, dtype);
-      d.a[0] = p;
+      d.a = p;
       if (any && (rc = operand(&d.b[0], w, ldw, n, k, dtype, ws, st))) return rc;
-      add_segments(d, 0, 0, 0, parts, 1);
+      d.segments = d.a_step = 1;
+      d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
     }
     if (dw && k > 0) {
       Product d{};
       d.type = dtype; d.M = n; d.N = k; d.K = m; d.nz = 1; d.a_mn = d.b_mn = true;
       d.e = plain_out(dw, k, dtype);
-      d.a[0] = p;
+      d.a = p;
       if (any && (rc = operand(&d.b[0], x, ldx, m, k, dtype, ws, st))) return rc;
-      add_segments(d, 0, 0, 0, parts, 1);
+      d.segments = d.a_step = 1;
+      d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
     }
     return VERACE_OK;
@@ -432,8 +446,10 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
 }
 
 extern "C" size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype) {
-  if (m <= 0 || f <= 0 || k <= 0 || dtype != VERACE_F32 || by_dots(m, f, k, dtype, 2)) return 0;
-  return operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype) + 256;
+  if (m <= 0 || f <= 0 || k <= 0 || by_dots(m, f, k, dtype, 2)) return 0;
+  const size_t split = dtype == VERACE_F32 ? operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype) : 0;
+  const size_t part = partial_bytes(m, f, k, 1, 1, true, dtype, false);
+  return split + part ? split + part + 256 : 0;
 }
 
 extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_scale, const void* w_gate, const void* w_up,
@@ -463,22 +479,26 @@ extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_
   p.e.pre = gate; p.e.pre_up = up; p.e.act = act;
   p.e.b1 = beta1; p.e.b2 = beta2; p.e.r1 = 1.f / beta1; p.e.r2 = 1.f / beta2;
   if (by_dots(m, f, k, dtype, 2)) {
-    p.a[0] = Mat{x, m, k, ldx, 1, 0};
+    p.a = Mat{x, m, k, ldx, 1, 0};
     p.b[0] = Mat{w_gate, f, k, ldw, 1, 0};
     p.b[1] = Mat{w_up, f, k, ldw, 1, 0};
     return product_dot(p, st);
   }
-  if (k > 0 && ((rc = operand(&p.a[0], x, ldx, m, k, dtype, ws, st)) ||
+  if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) ||
                 (rc = operand(&p.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
                 (rc = operand(&p.b[1], w_up, ldw, f, k, dtype, ws, st))))
     return rc;
-  add_segments(p, 0, 0, 0, dtype == VERACE_F32 ? 3 : 1, 1);
+  p.segments = p.a_step = 1;
+  p.ws = ws.at;
   return run_product(p, st);
 }
 
 extern "C" size_t verace_gated_linear_backward_workspace(long long m, int f, int k, int dtype) {
   if (m <= 0 || f <= 0) return 0;
   size_t s = 2 * operand_bytes(m, f, dtype) + 256;
+  // (dx and the weights' gradients follow each other: one place for the partial sums of either)
+  s += std::max(partial_bytes(m, k, f, 2, 1, false, dtype, false),
+                std::max(partial_bytes(f, k, m, 1, 1, false, dtype, true), partial_bytes(f, k, m, 1, 2, false, dtype, true)));
   if (dtype == VERACE_F32 && k > 0) s += operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype);
   return s;
 }
@@ -520,27 +540,20 @@ extern "C" int verace_gated_linear_backward(const void* dout, const void* x, lon
       s.colblocks = (int)((s.ld + 255) / 256);
       s.b1 = beta1; s.b2 = beta2; s.r1 = 1.f / beta1; s.r2 = 1.f / beta2;
       unsigned grid;
-      if ((rc = slope_grid(s, &grid))) return rc;
+      if ((rc = slope_grid(s, GATED_CHUNK, &grid))) return rc;
       gated_slope<T, O><<<grid, 256, 0, st>>>(s);
       if ((rc = check_launch("gated_slope"))) return rc;
     }
-    const int parts = split_v<T> ? 3 : 1;
     if (dx) {
       Product d{};
       d.type = dtype; d.M = m; d.N = k; d.K = f; d.nz = 1; d.b_mn = true;
       d.e = plain_out(dx, k, dtype);
-      d.a[0] = p;
+      d.a = p;
       if (any && ((rc = operand(&d.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
                   (rc = operand(&d.b[1], w_up, ldw, f, k, dtype, ws, st))))
         return rc;
-      // both products' pairs of parts, the smallest of both first
-      add_segments(d, 0, 0, 0, parts, 2);
-      add_segments(d, 0, 1, 1, parts, 2);
-      if (parts == 3) {
-        Segment s[12];
-        for (int i = 0; i < 12; ++i) s[i] = d.seg[i % 2 * 6 + i / 2];
-        for (int i = 0; i < 12; ++i) d.seg[i] = s[i];
-      }
+      d.segments = d.a_step = 2;
+      d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
     }
     if (dw_gate || dw_up) {
@@ -549,11 +562,12 @@ extern "C" int verace_gated_linear_backward(const void* dout, const void* x, lon
       d.nz = dw_gate && dw_up ? 2 : 1;
       d.out_z[0] = dw_gate; d.out_z[1] = dw_up;
       d.e = plain_out(dw_gate ? dw_gate : dw_up, k, dtype);
-      d.a[0] = p;
+      d.a = p;
       if (any && (rc = operand(&d.b[0], x, ldx, m, k, dtype, ws, st))) return rc;
-      // (with two outputs a part's piece is 2 part + output)
-      if (d.nz == 2) add_segments(d, 0, 0, 0, parts, 1);
-      else add_segments(d, 0, dw_gate ? 0 : 1, 0, parts, 2);
+      d.segments = 1;
+      d.a_step = 2;
+      d.a_first = dw_gate ? 0 : 1;
+      d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
     }
     return VERACE_OK;

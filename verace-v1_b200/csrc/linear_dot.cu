@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(32 * WARPS) dot_product(const __grid_constant_
 template <typename T, int MT, int RG, bool GATED, bool VEC>
 int launch(const Product& p, cudaStream_t st) {
   Args a{};
-  a.x = p.a[0].p; a.w = p.b[0].p; a.w_up = p.b[1].p;
-  a.ldx = p.a[0].ld; a.ldw = p.b[0].ld;
+  a.x = p.a.p; a.w = p.b[0].p; a.w_up = p.b[1].p;
+  a.ldx = p.a.ld; a.ldw = p.b[0].ld;
   a.M = p.M; a.N = p.N; a.K = p.K;
   a.e = p.e;
   a.groups = (p.N + RG - 1) / RG;
@@ -207,7 +207,7 @@ namespace lin {
 // x and W stored [M][K] and [N][K], one segment; p.type may be VERACE_F32 here.
 int product_dot(const Product& p, cudaStream_t st) {
   if (p.type == VERACE_F32) {
-    const bool vec = (((size_t)p.a[0].p | (size_t)p.b[0].p | (size_t)p.b[1].p) % 16 | (p.a[0].ld | p.b[0].ld) % 4) == 0;
+    const bool vec = (((size_t)p.a.p | (size_t)p.b[0].p | (size_t)p.b[1].p) % 16 | (p.a.ld | p.b[0].ld) % 4) == 0;
     if (p.M == 1) return vec ? by_gate<float, 1, 2>(p, st) : by_gate<float, 1, 2, false>(p, st);
     if (p.M <= 4) return vec ? by_gate<float, 4, 4>(p, st) : by_gate<float, 4, 4, false>(p, st);
     return vec ? by_gate<float, 8, 4>(p, st) : by_gate<float, 8, 4, false>(p, st);

@@ -42,8 +42,7 @@ struct Args {
   int kblocks, steps, per, ck, tiles_n;
   int cols;             // of TMEM
   int round;            // tokens whose partial sums a CTA holds at a time (ck > 1)
-  int segments;
-  Segment seg[MAX_SEGMENTS];
+  int a_first;
   uint32_t idesc;
   Epilogue e;
 };
@@ -56,29 +55,6 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
                  "r"(accumulate));
   else
     tc::mma_bf16(d, a, b, idesc, accumulate);   // (kind::f16; the descriptor names the type)
-}
-
-// four neighbouring values of a row, `n` of them inside of it
-__device__ __forceinline__ void load4(const void* p, long long i, int n, int type, float (&v)[4]) {
-  const size_t at = (size_t)p + i * (type == VERACE_F32 ? 4 : 2);
-  if (n == 4 && type != VERACE_F32 && (at & 7) == 0) {
-    const uint2 w = *reinterpret_cast<const uint2*>(at);
-    const float2 a = unpack_pair(w.x, type), b = unpack_pair(w.y, type);
-    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = j < n ? load_as(p, i + j, type) : 0.f;
-  }
-}
-__device__ __forceinline__ void store4(void* p, long long i, int n, int type, const float (&v)[4]) {
-  const size_t at = (size_t)p + i * (type == VERACE_F32 ? 4 : 2);
-  if (n == 4 && type != VERACE_F32 && (at & 7) == 0) {
-    *reinterpret_cast<uint2*>(at) = make_uint2(pack_pair(v[0], v[1], type), pack_pair(v[2], v[3], type));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) store_as(p, i + j, v[j], type);
-  }
 }
 
 // one value of each of 16 rows `ld` apart (of `n` rows; 0 beyond), the loads in flight together
@@ -108,45 +84,6 @@ __device__ __forceinline__ void store_rows16(void* p, long long i, long long ld,
     for (int j = 0; j < 16; ++j)
       if (j < n) f[j * ld] = (unsigned short)pack_pair(v[j], 0.f, type);
   }
-}
-
-// four outputs of row m from their sums (u: the up projection's)
-template <bool GATED>
-__device__ __forceinline__ void finish4(const Epilogue& e, long long m, long long c, long long N, float (&g)[4], float (&u)[4]) {
-  const int n = (int)min(4LL, N - c);
-  float res[4] = {};
-  if (!GATED && e.residual) load4(e.residual, m * e.ld_res + c, n, e.type, res);
-  if (e.col_scale) {
-    const float rs = e.row_scale[m];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) {
-        g[j] *= rs * e.col_scale[c + j];
-        if (GATED) u[j] *= rs * e.up_scale[c + j];
-      }
-  }
-  if (!GATED && e.bias) {
-    float b[4];
-    load4(e.bias, c, n, e.bias_type, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] += b[j];
-  }
-  if (e.pre) {
-    store4(e.pre, m * e.ld + c, n, VERACE_F32, g);
-    if (GATED) store4(e.pre_up, m * e.ld + c, n, VERACE_F32, u);
-  }
-  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (GATED) g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
-      else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
-    }
-  });
-  if (!GATED && e.residual) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] += res[j];
-  }
-  store4(e.out, m * e.ld + c, n, e.type, g);
 }
 
 template <bool F8, bool WMN, bool GATED>
@@ -190,17 +127,16 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
           atomicExch(&g_linear_few_status, 1);
           break;
         }
-        const Segment g = p.seg[seg];
         unsigned char* w = sm + i * p.stage;
         tc::mbar_expect_tx(&full[i], p.stage);
         if constexpr (WMN) {
-          tc::tma_load_3d(w, &maps.w[g.b], n0, kb * KB, g.bz, &full[i]);
-          tc::tma_load_3d(w + 8192, &maps.w[g.b], n0 + 64, kb * KB, g.bz, &full[i]);
+          tc::tma_load_3d(w, &maps.w[seg], n0, kb * KB, 0, &full[i]);
+          tc::tma_load_3d(w + 8192, &maps.w[seg], n0 + 64, kb * KB, 0, &full[i]);
         } else {
-          tc::tma_load_3d(w, &maps.w[GATED ? 0 : g.b], kb * KB, n0, g.bz, &full[i]);
-          if (GATED) tc::tma_load_3d(w + ROWS * 128, &maps.w[1], kb * KB, n0, g.bz, &full[i]);
+          tc::tma_load_3d(w, &maps.w[0], kb * KB, n0, 0, &full[i]);
+          if (GATED) tc::tma_load_3d(w + ROWS * 128, &maps.w[1], kb * KB, n0, 0, &full[i]);
         }
-        tc::tma_load_3d(w + WB, &maps.x, kb * KB, (int)m0, g.az, &full[i]);
+        tc::tma_load_3d(w + WB, &maps.x, kb * KB, (int)m0, p.a_first + seg, &full[i]);
         if (++kb == p.kblocks) kb = 0, ++seg;
         if (++i == p.stages) i = 0, phase ^= 1;
         flying = min(flying + 1, p.stages);
@@ -348,12 +284,11 @@ int launch(const Product& p, cudaStream_t st) {
   const int tiles_m = (int)((p.M + MAX_TOKENS - 1) / MAX_TOKENS);
   a.mp = (int)(((p.M + tiles_m - 1) / tiles_m + 15) / 16 * 16);
   // A (x) in boxes of the tile's tokens, B (the weights) as the MMA's rows
-  if ((rc = operand_map(&maps.x, p.a[0], p.type, a.mp))) return rc;
+  if ((rc = operand_map(&maps.x, p.a, p.type, a.mp))) return rc;
   for (int i = 0; i < 2; ++i)
     if ((rc = operand_map(&maps.w[i], p.b[p.b[i].p ? i : 0], p.type, WMN ? 64 : ROWS))) return rc;
   a.kblocks = (int)((p.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
-  a.segments = p.segments;
-  for (int i = 0; i < p.segments; ++i) a.seg[i] = p.seg[i];
+  a.a_first = p.a_first;
   a.steps = a.kblocks * p.segments;
   a.tiles_n = (int)((p.N + ROWS - 1) / ROWS);
   const long long units = (long long)a.tiles_n * tiles_m;

@@ -15,10 +15,10 @@
 // gate's, the second the up projection's), so both sums of an output lie in one TMEM row and the product is formed in
 // registers.  A sum of two products (the input gradient of a gated block) is two runs over K.
 //
-// fp32 operands come as three bf16 parts and run over six pairs of them, the smallest first.  The tensor core cuts
-// its sums to fp32 after every step instead of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the
-// result); so after every 128 values of K (CHUNK stages of each pair) the epilogue's warps add the sums to a third
-// set in TMEM, rounding, while the next 128 run into the other set.
+// fp32 operands come as three bf16 parts, three stages for 64 values of K (a stage holds one part of A and of B), and
+// the MMAs take six pairs of them, the smallest first.  The tensor core cuts its sums to fp32 after every step instead
+// of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the result); so after every 128 values of K
+// (CHUNK) the epilogue's warps add the sums to a third set in TMEM, rounding, while the next 128 run into the other set.
 //
 // Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
 // applies scales, bias and activation, and the warp turns the rounded values over in shared memory so
@@ -49,14 +49,15 @@ struct Shape {
 };
 
 struct Maps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a, b[2];
 };
 
 struct Args {
   long long M, N;
-  int kblocks, segments;
-  Segment seg[MAX_SEGMENTS];
+  int kblocks, segments, a_first, a_step;
   int nz, tiles_m, tiles_n, tiles;
+  int splits, per;      // of K: `per` stages (of every segment) each; the sums of split i go to the i-th partial outputs
+  long long partial;    // values from one split's outputs to the next
   uint32_t idesc;
   void* out_z[2];
   Epilogue e;
@@ -104,15 +105,17 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// tile t -> (z, row, column) of tiles: groups of eight rows, column by column
+// tile t -> (split of K, output, row, column) of tiles: groups of eight rows, column by column
 struct Place {
-  int z, m, n;
+  int split, z, m, n;
 };
 __device__ __forceinline__ Place place(const Args& p, int t) {
   Place o;
   const int each = p.tiles_m * p.tiles_n;
   o.z = t / each;
   t -= o.z * each;
+  o.split = o.z / p.nz;
+  o.z -= o.split * p.nz;
   const int group = t / (8 * p.tiles_n), first = 8 * group, high = min(8, p.tiles_m - first);
   t -= group * 8 * p.tiles_n;
   o.n = t / high;
@@ -133,7 +136,7 @@ struct Rows {
   char* at;           // the lane's word in the first row
   long long step;     // bytes of a row
   int rows;           // rows inside
-  int part;           // 0: no column of the lane inside, 1: its first half, 2: two halves, 3: a word
+  int part;           // 0: no column of the lane inside, 3: a whole word in every row, else 1: its first half alone, 2: both
 };
 template <bool WIDE>
 __device__ __forceinline__ Rows rows_of(const Block& b, const void* p, long long ld, int lane) {
@@ -156,14 +159,23 @@ __device__ __forceinline__ void write_block(const Block& b, void* p, long long l
   if (r.part == 3 && r.rows == 32) {
 #pragma unroll 16
     for (int i = 0; i < 32; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = t[33 * i];
-  } else if (r.part) {
-    for (int i = 0; i < r.rows; ++i, r.at += r.step) {
+  } else if (r.part == 3) {
+    for (int i = 0; i < r.rows; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = t[33 * i];
+  } else if (!WIDE && r.part) {
+    // rows off 4-byte borders (an odd row stride), or a last word cut in two: where the row's words lie between two
+    // words of the block, a lane stores the column before its own and its first
+    const int left = (int)min(64LL, b.N - b.n0) - 2 * lane;   // columns from the lane's on
+#pragma unroll 8
+    for (int i = 0; i < r.rows; ++i) {
       const uint32_t w = t[33 * i];
-      if (r.part == 3) {
-        *reinterpret_cast<uint32_t*>(r.at) = w;
+      unsigned short* o = reinterpret_cast<unsigned short*>(r.at + i * r.step);
+      if (((size_t)o & 3) == 0) {
+        if (left > 1) *reinterpret_cast<uint32_t*>(o) = w;
+        else o[0] = (unsigned short)w;
       } else {
-        reinterpret_cast<unsigned short*>(r.at)[0] = (unsigned short)w;
-        if (r.part == 2) reinterpret_cast<unsigned short*>(r.at)[1] = (unsigned short)(w >> 16);
+        if (lane == 0) o[0] = (unsigned short)w;
+        else *reinterpret_cast<uint32_t*>(o - 1) = t[33 * i - 1] >> 16 | w << 16;
+        if (left > 1 && (lane == 31 || left == 2)) o[1] = (unsigned short)(w >> 16);
       }
     }
   }
@@ -263,6 +275,10 @@ __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b
     save_sums(e, b, tmem, WIDTH, rs, e.col_scale, GATED ? nullptr : e.bias, e.pre, lane);
     if (GATED) save_sums(e, b, tmem_up, WIDTH, rs, e.up_scale, nullptr, e.pre_up, lane);
   }
+  if (GATED && out == nullptr) {   // (partial sums: the two above are all)
+    loaded();
+    return;
+  }
   uint32_t r[2][U], s[2][U];
   tmem_ld_async(tmem, r[0]);
   if constexpr (GATED) tmem_ld_async(tmem_up, s[0]);
@@ -319,7 +335,17 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t* turn, ui
     const Place at = place(p, t);
     b.m0 = at.m * 256LL + rank * 128 + 32 * (warp & 3);
     b.n0 = (long long)at.n * TN + first;
-    void* out = p.nz > 1 ? p.out_z[at.z] : p.e.out;
+    Epilogue e = p.e;
+    void* out = p.nz > 1 ? p.out_z[at.z] : e.out;
+    if (p.splits > 1) {
+      const long long first_of = (at.split * p.nz + at.z) * p.partial;
+      if (GATED) {
+        e.pre += first_of;
+        e.pre_up += first_of;
+      } else {
+        out = static_cast<float*>(e.out) + first_of;
+      }
+    }
     uint32_t res[32];
     if (!GATED && p.e.residual && b.m0 < b.M && b.n0 < b.N && first < last)   // on its way while the products run
       read_words<WIDE>(b, p.e.residual, p.e.ld_res, lane, res);
@@ -335,7 +361,7 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t* turn, ui
       after.n0 += WIDTH;
       const bool more = c + WIDTH < last && after.n0 < b.N;
       if (!GATED && p.e.residual && more) read_words<WIDE>(after, p.e.residual, p.e.ld_res, lane, next);
-      epilogue_block<GATED, WIDE>(p.e, b, sums + c, sums + HB + c, res, out, lane, [&] {
+      epilogue_block<GATED, WIDE>(e, b, sums + c, sums + HB + c, res, out, lane, [&] {
         if (!more) {
           release(n);
           held = false;
@@ -391,7 +417,8 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = *slot;
-  const int chunk = PARTS ? CHUNK : p.kblocks, chunks = PARTS ? (p.kblocks + CHUNK - 1) / CHUNK : 1;
+  // a tile's stages of K: in one lot, of parts `chunk` by `chunk` (PARTS: as many for every split, the last one's may be empty)
+  const int chunk = PARTS ? CHUNK : p.per, chunks = PARTS ? (p.per + CHUNK - 1) / CHUNK : 1;
 
   if (warp == 0) {
     if (lane == 0) {   // ---- operands
@@ -404,11 +431,11 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
         const int n0 = GATED ? at.n * HB : at.n * BN + (int)rank * HB;
         for (int u = 0; u < p.segments * chunks && ok; ++u) {   // (chunk by chunk, in each all segments)
           const int s = PARTS ? u % p.segments : u, k0 = PARTS ? u / p.segments * chunk : 0;
-          const Segment g = p.seg[s];
-          const CUtensorMap* ma = &maps.a[g.a];
-          const CUtensorMap* mb = &maps.b[GATED ? rank : g.b];
-          const int az = g.az * p.nz + at.z;
-          for (int kb = k0; kb < min(k0 + chunk, p.kblocks); ++kb) {
+          const CUtensorMap* mb = &maps.b[GATED ? rank : s];
+          const int end = min(min(k0 + chunk, p.per) + at.split * p.per, p.kblocks);
+          constexpr int EACH = PARTS ? 3 : 1;
+          for (int q = (k0 + at.split * p.per) * EACH; q < end * EACH; ++q) {
+            const int kb = q / EACH, part = q % EACH, az = part * p.a_step + p.a_first + s + at.z;
             if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
               ok = false;
               break;
@@ -418,16 +445,16 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
             unsigned char* a = sm + i * S::STAGE;
             unsigned char* b = a + 16384;
             if constexpr (AMN) {
-              load_box(a, ma, m0, kb * KB, az, bar);
-              load_box(a + 8192, ma, m0 + 64, kb * KB, az, bar);
+              load_box(a, &maps.a, m0, kb * KB, az, bar);
+              load_box(a + 8192, &maps.a, m0 + 64, kb * KB, az, bar);
             } else {
-              load_box(a, ma, kb * KB, m0, az, bar);
+              load_box(a, &maps.a, kb * KB, m0, az, bar);
             }
             if constexpr (BMN) {
 #pragma unroll
-              for (int h = 0; h < HB / 64; ++h) load_box(b + h * 8192, mb, n0 + 64 * h, kb * KB, g.bz, bar);
+              for (int h = 0; h < HB / 64; ++h) load_box(b + h * 8192, mb, n0 + 64 * h, kb * KB, part, bar);
             } else {
-              load_box(b, mb, kb * KB, n0, g.bz, bar);
+              load_box(b, mb, kb * KB, n0, part, bar);
             }
             if (++i == S::STAGES) i = 0, phase ^= 1;
             flying = min(flying + 1, S::STAGES);
@@ -454,9 +481,21 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       uint32_t phase = 0;
       bool ok = true;
       const int mine = (p.tiles - pair + pairs - 1) / pairs * chunks;   // sets of sums to fill
+      // four MMAs: 128 bytes of K of stage ia's A and stage ib's B
+      auto step = [&](uint32_t d, int ia, int ib, bool more) {
+        const uint32_t a = tc::smem_addr(sm + ia * S::STAGE), bb = tc::smem_addr(sm + ib * S::STAGE) + 16384;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
+          const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
+          const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
+          mma_pair<F8>(d, da, db, p.idesc, more || k > 0 ? 1u : 0u);
+        }
+      };
       for (; n < mine && ok; ++n) {
         const int b = n & 1, use = n >> 1;
-        const int steps = p.segments * (PARTS ? min(chunk, p.kblocks - n % chunks * chunk) : p.kblocks);
+        const int base = place(p, pair + n / chunks * pairs).split * p.per + n % chunks * chunk;
+        const int steps = p.segments * (min(min(base + chunk, base - n % chunks * chunk + p.per), p.kblocks) - base);
         if (!tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
           ok = false;
           break;
@@ -464,24 +503,40 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
         tc::fence_after_sync();
         const uint32_t d = tmem + b * BN;
         for (int s = 0; s < steps; ++s) {
-          if (!tc::mbar_wait(&full[i], phase, POLLS)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after_sync();
-          const uint32_t a = tc::smem_addr(sm + i * S::STAGE), bb = a + 16384;
-          if (lead) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
-              const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
-              const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
-              mma_pair<F8>(d, da, db, p.idesc, s > 0 || k > 0 ? 1u : 0u);
+          if constexpr (!PARTS) {
+            if (!tc::mbar_wait(&full[i], phase, POLLS)) {
+              ok = false;
+              break;
             }
-            commit_pair(&empty[i]);
+            tc::fence_after_sync();
+            if (lead) {
+              step(d, i, i, s > 0);
+              commit_pair(&empty[i]);
+            }
+            __syncwarp();
+            if (++i == S::STAGES) i = 0, phase ^= 1;
+          } else {
+            int at[3];
+            for (int j = 0; j < 3 && ok; ++j) {
+              at[j] = i;
+              ok = tc::mbar_wait(&full[i], phase, POLLS);
+              if (++i == S::STAGES) i = 0, phase ^= 1;
+            }
+            if (!ok) break;
+            tc::fence_after_sync();
+            if (lead) {   // parts: 0 the high one
+              step(d, at[2], at[0], s > 0);
+              step(d, at[1], at[1], true);
+              step(d, at[0], at[2], true);
+              commit_pair(&empty[at[2]]);
+              step(d, at[1], at[0], true);
+              step(d, at[0], at[1], true);
+              commit_pair(&empty[at[1]]);
+              step(d, at[0], at[0], true);
+              commit_pair(&empty[at[0]]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          if (++i == S::STAGES) i = 0, phase ^= 1;
         }
         if (lead) commit_pair(&acc_full[b]);   // (also after a failure: every MMA issued completes)
         __syncwarp();
@@ -512,9 +567,14 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
     auto wait = [&](int n) {
       if constexpr (!PARTS) return filled(n) ? (n & 1) * BN : -1;
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+      const int base = place(p, pair + n * pairs).split * p.per;
       for (int c = 0; c < chunks; ++c) {
         const int set = n * chunks + c;
         if (!filled(set)) return -1;
+        if (base + c * CHUNK >= p.kblocks) {   // (a last split's missing stages)
+          free(set);
+          continue;
+        }
         for (int h = 0; h < BN / 2; h += 16) {   // the warp's half of the columns (gated: of both sums)
           const int col = GATED ? (h >= HB / 2 ? HB / 2 + h : h) + (warp >= 8 ? HB / 2 : 0) : h + (warp >= 8 ? HB : 0);
           uint32_t r[16], s[16];
@@ -552,32 +612,42 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
 
 // ------------------------------------------------------------------ host
 template <bool F8, bool AMN, bool BMN, bool GATED, int BN, bool PARTS = false>
-int launch(const Product& p, cudaStream_t st) {
+int launch(const Product& p, int splits, cudaStream_t st) {
   using S = Shape<BN>;
   constexpr int TN = GATED ? BN / 2 : BN;
   Maps maps;
   int rc;
-  for (int i = 0; i < 2; ++i) {
-    const Mat& a = p.a[p.a[i].p ? i : 0];
-    const Mat& b = p.b[p.b[i].p ? i : 0];
-    if ((rc = operand_map(&maps.a[i], a, p.type, AMN ? 64 : 128)) || (rc = operand_map(&maps.b[i], b, p.type, BMN ? 64 : BN / 2)))
-      return rc;
-  }
+  if ((rc = operand_map(&maps.a, p.a, p.type, AMN ? 64 : 128))) return rc;
+  for (int i = 0; i < 2; ++i)
+    if ((rc = operand_map(&maps.b[i], p.b[p.b[i].p ? i : 0], p.type, BMN ? 64 : BN / 2))) return rc;
   Args a{};
   a.M = p.M; a.N = p.N;
   a.kblocks = (int)((p.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
-  a.segments = p.segments;
-  for (int i = 0; i < p.segments; ++i) a.seg[i] = p.seg[i];
+  a.segments = p.segments; a.a_first = p.a_first; a.a_step = p.a_step;
   a.nz = p.nz;
   a.tiles_m = (int)((p.M + 255) / 256);
   a.tiles_n = (int)((p.N + TN - 1) / TN);
-  const long long tiles = (long long)a.tiles_m * a.tiles_n * p.nz;
+  a.splits = splits;
+  a.per = (a.kblocks + splits - 1) / splits;
+  a.partial = p.M * p.N;
+  const long long tiles = (long long)a.tiles_m * a.tiles_n * p.nz * splits;
   VERACE_REQUIRE(tiles < 1LL << 30, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
   a.tiles = (int)tiles;
   a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
             (uint32_t)AMN << 15 | (uint32_t)BMN << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
   a.out_z[0] = p.out_z[0]; a.out_z[1] = p.out_z[1];
   a.e = p.e;
+  if (splits > 1) {
+    Epilogue e{};
+    e.ld = p.N; e.type = VERACE_F32; e.act = VERACE_ACT_NONE;
+    if (GATED) {
+      e.pre = static_cast<float*>(p.ws);
+      e.pre_up = e.pre + splits * a.partial;
+    } else {
+      e.out = p.ws;
+    }
+    a.e = e;
+  }
   auto kern = large_product<F8, AMN, BMN, GATED, BN, PARTS>;
   int dev = 0;
   VERACE_CUDA(cudaGetDevice(&dev));
@@ -592,17 +662,67 @@ int launch(const Product& p, cudaStream_t st) {
 }
 
 template <int BN>
-int by_kind(const Product& p, cudaStream_t st) {
+int by_kind(const Product& p, int s, cudaStream_t st) {
   if constexpr (BN == 128) {
-    if (p.parts && p.gated) return launch<false, false, false, true, BN, true>(p, st);
-    if (p.parts && p.a_mn) return launch<false, true, true, false, BN, true>(p, st);
-    if (p.parts) return p.b_mn ? launch<false, false, true, false, BN, true>(p, st) : launch<false, false, false, false, BN, true>(p, st);
+    if (p.parts && p.gated) return launch<false, false, false, true, BN, true>(p, s, st);
+    if (p.parts && p.a_mn) return launch<false, true, true, false, BN, true>(p, s, st);
+    if (p.parts) return p.b_mn ? launch<false, false, true, false, BN, true>(p, s, st) : launch<false, false, false, false, BN, true>(p, s, st);
   }
   if (p.type == VERACE_E4M3)
-    return p.gated ? launch<true, false, false, true, BN>(p, st) : launch<true, false, false, false, BN>(p, st);
-  if (p.gated) return launch<false, false, false, true, BN>(p, st);
-  if (p.a_mn) return launch<false, true, true, false, BN>(p, st);
-  return p.b_mn ? launch<false, false, true, false, BN>(p, st) : launch<false, false, false, false, BN>(p, st);
+    return p.gated ? launch<true, false, false, true, BN>(p, s, st) : launch<true, false, false, false, BN>(p, s, st);
+  if (p.gated) return launch<false, false, false, true, BN>(p, s, st);
+  if (p.a_mn) return launch<false, true, true, false, BN>(p, s, st);
+  return p.b_mn ? launch<false, false, true, false, BN>(p, s, st) : launch<false, false, false, false, BN>(p, s, st);
+}
+
+// ------------------------------------------------------------------ split K
+// The outputs from the partial sums, added in order; four columns a thread.
+template <bool GATED>
+__global__ void __launch_bounds__(256) join_splits(const float* __restrict__ part, int splits, long long partial, long long up,
+                                                   Epilogue e, long long M, long long N, long long quads) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long m = i / quads, c = i % quads * 4;
+  if (m >= M) return;
+  const int n = (int)min(4LL, N - c);
+  float g[4] = {}, u[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    float v[4];
+    load4(part, s * partial + m * N + c, n, VERACE_F32, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] += v[j];
+    if (GATED) {
+      load4(part, up + s * partial + m * N + c, n, VERACE_F32, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] += v[j];
+    }
+  }
+  finish4<GATED>(e, m, c, N, g, u);
+}
+
+// How a product is cut: columns of a tile, and splits of K.  A pair's time in clocks: a step of four
+// MMAs takes 512 (BN 256) or 400 (BN 128, bound by the 24 KB that each CTA loads for it), one of parts 1600, an epilogue about 40 a column (under the next tile's products but for
+// the last), the first operands 6000; partial sums are written and read at about 2 KB a clock, and joining them takes another launch (5000).
+struct Cut {
+  int bn, splits;
+};
+Cut cut(long long M, long long N, long long K, int segments, int nz, bool gated, int type, bool parts) {
+  const long long kblocks = (K + (type == VERACE_E4M3 ? 127 : 63)) / (type == VERACE_E4M3 ? 128 : 64);
+  Cut best{parts ? 128 : 256, 1};
+  double least = 0;
+  for (int bn = parts ? 128 : 256; bn >= 128; bn /= 2) {
+    const int tn = gated ? bn / 2 : bn;
+    const long long tiles = (M + 255) / 256 * ((N + tn - 1) / tn) * nz;
+    for (int s = 1; s <= 16 && (s == 1 || (s * tiles <= 74 && kblocks >= 8 * s)); ++s) {
+      const long long stages = (kblocks + s - 1) / s;
+      if ((s - 1) * stages >= kblocks) continue;      // (a split would be empty)
+      const double per = (double)stages * segments * (parts ? 1600 : bn == 256 ? 512 : 400), epi = 40. * bn;
+      double t = (double)((tiles * s + 73) / 74) * (per > epi ? per : epi) + epi + 6000;
+      if (s > 1) t += 5000 + (double)M * N * nz * (gated ? 8 : 4) * 2 * s / 2048;
+      if (least == 0 || t < least) least = t, best = Cut{bn, s};
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -626,9 +746,28 @@ int operand_map(CUtensorMap* map, const Mat& m, int type, int rows) {
   return VERACE_OK;
 }
 
+size_t split_bytes(long long M, long long N, long long K, int segments, int nz, bool gated, int type, bool parts) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const int s = cut(M, N, K, segments, nz, gated, type, parts).splits;
+  return s > 1 ? align_up((size_t)M * N * nz * s * (gated ? 8 : 4), 256) : 0;
+}
+
 int product_large(const Product& p, cudaStream_t st) {
-  const long long wide = (p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256) * ((p.M + 255) / 256) * p.nz;
-  return wide >= 74 && !p.parts ? by_kind<256>(p, st) : by_kind<128>(p, st);
+  const Cut c = cut(p.M, p.N, p.K, p.segments, p.nz, p.gated, p.type, p.parts);
+  int rc = c.bn == 256 ? by_kind<256>(p, c.splits, st) : by_kind<128>(p, c.splits, st);
+  if (rc || c.splits == 1) return rc;
+  const long long quads = (p.N + 3) / 4, blocks = (p.M * quads + 255) / 256, one = p.M * p.N;
+  for (int z = 0; z < p.nz; ++z) {
+    Epilogue e = p.e;
+    if (p.nz > 1) e.out = p.out_z[z];
+    const float* part = static_cast<const float*>(p.ws) + z * one;
+    if (p.gated)
+      join_splits<true><<<(unsigned)blocks, 256, 0, st>>>(part, c.splits, one, c.splits * one, e, p.M, p.N, quads);
+    else
+      join_splits<false><<<(unsigned)blocks, 256, 0, st>>>(part, c.splits, p.nz * one, 0, e, p.M, p.N, quads);
+    if ((rc = check_launch("join_splits"))) return rc;
+  }
+  return VERACE_OK;
 }
 
 }  // namespace lin

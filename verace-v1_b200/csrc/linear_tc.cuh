@@ -16,28 +16,24 @@ struct Mat {
   long long piece;
 };
 
-// One run over K: which A and B, and which piece of each.
-struct Segment {
-  unsigned char a, az, b, bz;
-};
-constexpr int MAX_SEGMENTS = 12;
-
-// out[z](m, n) = epilogue(sum over segments and k of A(m, k) B(n, k)).
+// out[z](m, n) = epilogue(sum over s < segments and k of A_s(m, k) B_s(n, k)).
+// A_s is a's matrix a_first + s + z (the parts of an fp32 matrix `a_step` further each); B_s is b[s].
 // A and B are stored [M][K] and [N][K], or [K][M] and [K][N] where a_mn, b_mn are set (16-bit types).
-// gated: b[0] and b[1] give the two sums of a row and column (N: columns of each).
-// z runs over nz outputs, each of A's piece z (nz > 1: one segment, or pieces az * nz + z).
+// gated: one segment, b[0] and b[1] give the two sums of a row and column (N: columns of each).
 struct Product {
   int type;             // VERACE_BF16, VERACE_F16 or VERACE_E4M3
   bool parts;           // the operands are the parts of fp32 matrices
   long long M, N, K;
-  Mat a[2], b[2];
+  Mat a, b[2];
   bool a_mn, b_mn, gated;
-  int segments;
-  Segment seg[MAX_SEGMENTS];
-  int nz;
-  void* out_z[2];       // the outputs where nz is 2
+  int segments, a_first, a_step;
+  int nz;               // outputs: 1 or 2
+  void* out_z[2];       // where nz is 2
   Epilogue e;
+  void* ws;             // split_bytes(...) bytes, for partial sums where K is split
 };
+// What product_large may take for partial sums (M x N outputs each, nz of them).
+size_t split_bytes(long long M, long long N, long long K, int segments, int nz, bool gated, int type, bool parts);
 
 int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
 int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to 256 rows of A
@@ -116,6 +112,73 @@ __device__ __forceinline__ void column_values(const void* p, int type, long long
 #pragma unroll
     for (int j = 0; j < U; ++j) v[j] = unpack_pair(w[j], type).x;
   }
+}
+
+// four neighbouring values of a row, `n` of them inside of it
+__device__ __forceinline__ void load4(const void* p, long long i, int n, int type, float (&v)[4]) {
+  const size_t at = (size_t)p + i * (type == VERACE_F32 ? 4 : 2);
+  if (n == 4 && type != VERACE_F32 && (at & 7) == 0) {
+    const uint2 w = *reinterpret_cast<const uint2*>(at);
+    const float2 a = unpack_pair(w.x, type), b = unpack_pair(w.y, type);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  } else if (n == 4 && type == VERACE_F32 && (at & 15) == 0) {
+    const float4 f = *reinterpret_cast<const float4*>(at);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? load_as(p, i + j, type) : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(void* p, long long i, int n, int type, const float (&v)[4]) {
+  const size_t at = (size_t)p + i * (type == VERACE_F32 ? 4 : 2);
+  if (n == 4 && type != VERACE_F32 && (at & 7) == 0) {
+    *reinterpret_cast<uint2*>(at) = make_uint2(pack_pair(v[0], v[1], type), pack_pair(v[2], v[3], type));
+  } else if (n == 4 && type == VERACE_F32 && (at & 15) == 0) {
+    *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) store_as(p, i + j, v[j], type);
+  }
+}
+
+// four outputs of row m from their sums (u: the up projection's)
+template <bool GATED>
+__device__ __forceinline__ void finish4(const Epilogue& e, long long m, long long c, long long N, float (&g)[4], float (&u)[4]) {
+  const int n = (int)min(4LL, N - c);
+  float res[4] = {};
+  if (!GATED && e.residual) load4(e.residual, m * e.ld_res + c, n, e.type, res);
+  if (e.col_scale) {
+    const float rs = e.row_scale[m];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) {
+        g[j] *= rs * e.col_scale[c + j];
+        if (GATED) u[j] *= rs * e.up_scale[c + j];
+      }
+  }
+  if (!GATED && e.bias) {
+    float b[4];
+    load4(e.bias, c, n, e.bias_type, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] += b[j];
+  }
+  if (e.pre) {
+    store4(e.pre, m * e.ld + c, n, VERACE_F32, g);
+    if (GATED) store4(e.pre_up, m * e.ld + c, n, VERACE_F32, u);
+  }
+  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (GATED) g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
+      else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
+    }
+  });
+  if (!GATED && e.residual) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] += res[j];
+  }
+  store4(e.out, m * e.ld + c, n, e.type, g);
 }
 
 }  // namespace lin
