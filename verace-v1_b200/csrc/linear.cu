@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long l
   float v = e.bias ? load_as(e.bias, c, e.bias_type) : 0.f;
   if (e.pre) e.pre[r * e.ld + c] = v;
   if (e.pre_up) e.pre_up[r * e.ld + c] = 0.f;
-  by_act(e.act, false, [&](auto act, auto fast) { v = act_<decltype(act)::value, false>(v); });
+  by_act(e.act, [&](auto act) { v = act_<decltype(act)::value, false>(v); });
   if (e.residual) v += load_as(e.residual, r * e.ld_res + c, e.type);
   store_as(e.out, r * e.ld + c, v, e.type);
 }
@@ -197,11 +197,11 @@ __global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
       load8<O>(static_cast<const O*>(a.d) + r * a.n, c, a.n, a.vec, d);
       if (a.pre) {
         load8<float>(a.pre + r * a.n, c, a.n, a.vec, z);
-        by_act(a.act, sizeof(O) == 2, [&](auto k, auto fast) {
+        by_act(a.act, [&](auto k) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             float y, dy;
-            act_slope_<decltype(k)::value, decltype(fast)::value>(z[j], y, dy);
+            act_slope_<decltype(k)::value, sizeof(O) == 2>(z[j], y, dy);
             d[j] *= dy;
           }
         });
@@ -252,11 +252,11 @@ __global__ void __launch_bounds__(256) gated_slope(SlopeArgs a) {
     load8<O>(static_cast<const O*>(a.d) + r * a.n, c, a.n, a.vec, d);
     load8<float>(a.pre + r * a.n, c, a.n, a.vec, g);
     load8<float>(a.up + r * a.n, c, a.n, a.vec, u);
-    by_act(a.act, sizeof(O) == 2, [&](auto k, auto fast) {
+    by_act(a.act, [&](auto k) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float x, y;
-        gate_slope_<decltype(k)::value, decltype(fast)::value>(d[j], g[j], u[j], a.b1, a.b2, a.r1, a.r2, x, y);
+        gate_slope_<decltype(k)::value, sizeof(O) == 2>(d[j], g[j], u[j], a.b1, a.b2, a.r1, a.r2, x, y);
         g[j] = x;
         u[j] = y;
       }

@@ -15,23 +15,34 @@ namespace lin {
 // FAST serves outputs of 16 bits: exponentials and reciprocals by the approximate instructions, a
 // few units of 2^-23 off, against the output's half step of 2^-9 or 2^-12.  fp32 outputs take
 // the CUDA functions.
+__device__ __forceinline__ float ex2_(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float LOG2E = 1.4426950408889634f;
 template <bool FAST>
 __device__ __forceinline__ float exp_(float x) {
-  return FAST ? __expf(x) : expf(x);
+  return FAST ? ex2_(x * LOG2E) : expf(x);
 }
 template <bool FAST>
 __device__ __forceinline__ float sigmoid_(float x) {
-  return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
+  return FAST ? rcp_(1.f + ex2_(x * -LOG2E)) : 1.f / (1.f + expf(-x));
 }
-// tanh x = 1 - 2 / (1 + e^2x), which cancels near 0; there its odd Taylor series up to x^9 (the first
-// term left out is 1382/155925 x^11: 3e-9 relative at 1/4).
+// tanh x = 1 - 2 / (1 + e^2x), which cancels near 0; there its odd Taylor series up to x^7 (the first
+// term left out is 62/2835 x^9: 6e-8 relative at 1/5).
 template <bool FAST>
 __device__ __forceinline__ float tanh_(float x) {
   if (!FAST) return tanhf(x);
   const float q = x * x;
-  const float s = x * fmaf(q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-  const float t = 1.f - __fdividef(2.f, 1.f + __expf(2.f * x));
-  return q < 0.0625f ? s : t;
+  const float s = x * fmaf(q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float t = fmaf(-2.f, rcp_(1.f + ex2_(x * (2.f * LOG2E))), 1.f);
+  return q < 0.04f ? s : t;
 }
 
 constexpr float SQRT_HALF = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
@@ -91,24 +102,29 @@ __device__ __forceinline__ void gate_slope_(float d, float g, float u, float b1,
   }
 }
 
-// Calls f(std::integral_constant<int, ACT>, std::bool_constant<FAST>) for a runtime activation.
+// Calls f(std::integral_constant<int, ACT>) for a runtime activation.
 template <typename F>
-__host__ __device__ __forceinline__ void by_act(int act, bool fast, F&& f) {
-#define VERACE_BY_ACT(A)                                                       \
-  case A:                                                                      \
-    if (fast) f(std::integral_constant<int, A>(), std::true_type());           \
-    else f(std::integral_constant<int, A>(), std::false_type());               \
-    break
+__device__ __forceinline__ void by_act(int act, F&& f) {
   switch (act) {
-    VERACE_BY_ACT(VERACE_ACT_RELU);
-    VERACE_BY_ACT(VERACE_ACT_SILU);
-    VERACE_BY_ACT(VERACE_ACT_GELU);
-    VERACE_BY_ACT(VERACE_ACT_GELU_TANH);
-    VERACE_BY_ACT(VERACE_ACT_SITU);
-    default:
-      f(std::integral_constant<int, VERACE_ACT_NONE>(), std::false_type());
+    case VERACE_ACT_RELU: f(std::integral_constant<int, VERACE_ACT_RELU>()); break;
+    case VERACE_ACT_SILU: f(std::integral_constant<int, VERACE_ACT_SILU>()); break;
+    case VERACE_ACT_GELU: f(std::integral_constant<int, VERACE_ACT_GELU>()); break;
+    case VERACE_ACT_GELU_TANH: f(std::integral_constant<int, VERACE_ACT_GELU_TANH>()); break;
+    case VERACE_ACT_SITU: f(std::integral_constant<int, VERACE_ACT_SITU>()); break;
+    default: f(std::integral_constant<int, VERACE_ACT_NONE>());
   }
-#undef VERACE_BY_ACT
+}
+// v <- act(v), or act(v) up(u): U values, FAST with the output's type
+template <bool GATED, bool FAST, int U, typename E>
+__device__ __forceinline__ void activate(const E& e, float (&v)[U], const float (&u)[U]) {
+  if (!GATED && e.act == VERACE_ACT_NONE) return;
+  by_act(e.act, [&](auto act) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if constexpr (GATED) v[j] = gate_<decltype(act)::value, FAST>(v[j], u[j], e.b1, e.b2, e.r1, e.r2);
+      else v[j] = act_<decltype(act)::value, FAST>(v[j]);
+    }
+  });
 }
 
 // ------------------------------------------------------------------ values by a runtime type

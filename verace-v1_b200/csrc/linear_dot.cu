@@ -80,10 +80,10 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long m, long long
     e.pre[m * e.ld + n] = g;
     if (GATED) e.pre_up[m * e.ld + n] = u;
   }
-  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
-    if constexpr (GATED) g = gate_<decltype(act)::value, decltype(fast)::value>(g, u, e.b1, e.b2, e.r1, e.r2);
-    else g = act_<decltype(act)::value, decltype(fast)::value>(g);
-  });
+  float v[1] = {g}, w[1] = {u};
+  if (e.type == VERACE_F32) activate<GATED, false>(e, v, w);
+  else activate<GATED, true>(e, v, w);
+  g = v[0];
   if (!GATED && e.residual) g += load_as(e.residual, m * e.ld_res + n, e.type);
   store_as(e.out, m * e.ld + n, g, e.type);
 }

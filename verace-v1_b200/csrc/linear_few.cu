@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
         if (!GATED && e.residual) load_rows16(e.residual, (m0 + t) * e.ld_res + n, e.ld_res, rows, e.type, res);
         tmem_wait(r);
         if (GATED) tmem_wait(s);
-        float g[16], u[16];
+        float g[16], u[16] = {};
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float rs = e.row_scale && t + j < tokens ? e.row_scale[m0 + t + j] : 1.f;
@@ -219,13 +219,8 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
           store_rows16(e.pre, (m0 + t) * e.ld + n, e.ld, rows, VERACE_F32, g);
           if (GATED) store_rows16(e.pre_up, (m0 + t) * e.ld + n, e.ld, rows, VERACE_F32, u);
         }
-        by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if constexpr (GATED) g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
-            else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
-          }
-        });
+        if (e.type == VERACE_F32) activate<GATED, false>(e, g, u);
+        else activate<GATED, true>(e, g, u);
 #pragma unroll
         for (int j = 0; j < 16; ++j) g[j] += res[j];
         store_rows16(e.out, (m0 + t) * e.ld + n, e.ld, rows, e.type, g);

@@ -102,8 +102,10 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
                "h"((unsigned short)3)
                : "memory");
 }
+// (What it hands over is TMEM, ordered by the tcgen05 fences; a release over the cluster would wait for the
+// warp's stores.)
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // tile t -> (split of K, output, row, column) of tiles: groups of eight rows, column by column
 struct Place {
@@ -127,9 +129,19 @@ __device__ __forceinline__ Place place(const Args& p, int t) {
 // A warp's block: 32 rows of 32 words, the word `lane` of row r at turn[33 r + lane]: 32 columns of fp32, or
 // 64 of 16-bit types, two to a word.
 struct Block {
-  uint32_t* turn;
+  uint32_t turn;            // its address in shared memory
   long long m0, n0, M, N;   // first row and column; ends
 };
+
+// (by their address: through pointers these would be generic accesses)
+__device__ __forceinline__ uint32_t word(const Block& b, int i) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(b.turn + 4 * i) : "memory");
+  return v;
+}
+__device__ __forceinline__ void set_word(const Block& b, int i, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(b.turn + 4 * i), "r"(v) : "memory");
+}
 
 // Where a warp reads or writes a block: row by row, a word (or its two halves) a lane.
 struct Rows {
@@ -155,26 +167,31 @@ template <bool WIDE>
 __device__ __forceinline__ void write_block(const Block& b, void* p, long long ld, int lane) {
   __syncwarp();
   Rows r = rows_of<WIDE>(b, p, ld, lane);
-  const uint32_t* t = b.turn + lane;
   if (r.part == 3 && r.rows == 32) {
-#pragma unroll 16
-    for (int i = 0; i < 32; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = t[33 * i];
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = word(b, 33 * (h + i) + lane);
+#pragma unroll
+      for (int i = 0; i < 16; ++i, r.at += r.step) *reinterpret_cast<uint32_t*>(r.at) = w[i];
+    }
   } else if (r.part == 3) {
-    for (int i = 0; i < r.rows; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = t[33 * i];
+    for (int i = 0; i < r.rows; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = word(b, 33 * i + lane);
   } else if (!WIDE && r.part) {
     // rows off 4-byte borders (an odd row stride), or a last word cut in two: where the row's words lie between two
     // words of the block, a lane stores the column before its own and its first
     const int left = (int)min(64LL, b.N - b.n0) - 2 * lane;   // columns from the lane's on
 #pragma unroll 8
     for (int i = 0; i < r.rows; ++i) {
-      const uint32_t w = t[33 * i];
+      const uint32_t w = word(b, 33 * i + lane);
       unsigned short* o = reinterpret_cast<unsigned short*>(r.at + i * r.step);
       if (((size_t)o & 3) == 0) {
         if (left > 1) *reinterpret_cast<uint32_t*>(o) = w;
         else o[0] = (unsigned short)w;
       } else {
         if (lane == 0) o[0] = (unsigned short)w;
-        else *reinterpret_cast<uint32_t*>(o - 1) = t[33 * i - 1] >> 16 | w << 16;
+        else *reinterpret_cast<uint32_t*>(o - 1) = word(b, 33 * i + lane - 1) >> 16 | w << 16;
         if (left > 1 && (lane == 31 || left == 2)) o[1] = (unsigned short)(w >> 16);
       }
     }
@@ -201,25 +218,28 @@ __device__ __forceinline__ void read_words(const Block& b, const void* p, long l
 // U values into the thread's own row of the block, from column c on
 template <bool WIDE, int U>
 __device__ __forceinline__ void put(const Block& b, int c, const float (&v)[U], int type, int lane) {
-  uint32_t* t = b.turn + 33 * lane;
+  const int t = 33 * lane;
   if constexpr (WIDE) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) t[c + j] = __float_as_uint(v[j]);
+    for (int j = 0; j < U; ++j) set_word(b, t + c + j, __float_as_uint(v[j]));
+  } else if (type == VERACE_BF16) {
+#pragma unroll
+    for (int j = 0; j < U / 2; ++j) set_word(b, t + c / 2 + j, pack_pair(v[2 * j], v[2 * j + 1], VERACE_BF16));
   } else {
 #pragma unroll
-    for (int j = 0; j < U / 2; ++j) t[c / 2 + j] = pack_pair(v[2 * j], v[2 * j + 1], type);
+    for (int j = 0; j < U / 2; ++j) set_word(b, t + c / 2 + j, pack_pair(v[2 * j], v[2 * j + 1], VERACE_F16));
   }
 }
 template <bool WIDE, int U>
 __device__ __forceinline__ void add(const Block& b, int c, float (&v)[U], int type, int lane) {
-  const uint32_t* t = b.turn + 33 * lane;
+  const int t = 33 * lane;
   if constexpr (WIDE) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) v[j] += __uint_as_float(t[c + j]);
+    for (int j = 0; j < U; ++j) v[j] += __uint_as_float(word(b, t + c + j));
   } else {
 #pragma unroll
     for (int j = 0; j < U / 2; ++j) {
-      const float2 f = unpack_pair(t[c / 2 + j], type);
+      const float2 f = unpack_pair(word(b, t + c / 2 + j), type);
       v[2 * j] += f.x;
       v[2 * j + 1] += f.y;
     }
@@ -279,41 +299,29 @@ __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b
     loaded();
     return;
   }
-  uint32_t r[2][U], s[2][U];
-  tmem_ld_async(tmem, r[0]);
-  if constexpr (GATED) tmem_ld_async(tmem_up, s[0]);
+  uint32_t r[U], s[U];
+  tmem_ld_async(tmem, r);
+  if constexpr (GATED) tmem_ld_async(tmem_up, s);
   if (!GATED && e.residual) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) b.turn[33 * i + lane] = res[i];
+    for (int i = 0; i < 32; ++i) set_word(b, 33 * i + lane, res[i]);
     __syncwarp();
   }
-#pragma unroll
+#pragma unroll 1
   for (int l = 0; l < LOTS; ++l) {
-    tmem_wait(r[l & 1]);
-    if constexpr (GATED) tmem_wait(s[l & 1]);
+    float v[U], u[U] = {};
+    tmem_wait(r);
+    if constexpr (GATED) tmem_wait(s);
+    scaled(e, r, v, rs, e.col_scale, GATED ? nullptr : e.bias, b.n0 + l * U, b.N);
+    if constexpr (GATED) scaled(e, s, u, rs, e.up_scale, nullptr, b.n0 + l * U, b.N);
     if (l + 1 < LOTS) {
-      tmem_ld_async(tmem + (l + 1) * U, r[(l + 1) & 1]);
-      if constexpr (GATED) tmem_ld_async(tmem_up + (l + 1) * U, s[(l + 1) & 1]);
+      tmem_ld_async(tmem + (l + 1) * U, r);
+      if constexpr (GATED) tmem_ld_async(tmem_up + (l + 1) * U, s);
     } else {
       loaded();
     }
-    float v[U];
-    scaled(e, r[l & 1], v, rs, e.col_scale, GATED ? nullptr : e.bias, b.n0 + l * U, b.N);
-    if constexpr (GATED) {
-      float u[U];
-      scaled(e, s[l & 1], u, rs, e.up_scale, nullptr, b.n0 + l * U, b.N);
-      by_act(e.act, !WIDE, [&](auto act, auto fast) {
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-          v[j] = gate_<decltype(act)::value, decltype(fast)::value>(v[j], u[j], e.b1, e.b2, e.r1, e.r2);
-      });
-    } else {
-      by_act(e.act, !WIDE, [&](auto act, auto fast) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = act_<decltype(act)::value, decltype(fast)::value>(v[j]);
-      });
-      if (e.residual) add<WIDE>(b, l * U, v, e.type, lane);
-    }
+    activate<GATED, !WIDE>(e, v, u);
+    if (!GATED && e.residual) add<WIDE>(b, l * U, v, e.type, lane);
     put<WIDE>(b, l * U, v, e.type, lane);
   }
   write_block<WIDE>(b, out, e.ld, lane);
@@ -321,7 +329,7 @@ __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b
 
 // A warp's part of every tile of the pair: TMEM lanes 32 (warp % 4) ..., one half of the columns.
 template <bool GATED, bool WIDE, int BN, typename Wait, typename Free>
-__device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t* turn, uint32_t tmem, int pair, int pairs, int rank,
+__device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t turn, uint32_t tmem, int pair, int pairs, int rank,
                                                int warp, int lane, Wait&& wait, Free&& release) {
   constexpr int HB = BN / 2, TN = GATED ? HB : BN, WIDTH = WIDE ? 32 : 64, PER = TN / 2 > WIDTH ? TN / 2 : WIDTH;
   const int half = (warp - 4) >> 2, first = half * PER, last = min(TN, first + PER);
@@ -548,7 +556,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       }
     }
   } else if (warp >= 4) {   // ---- epilogue
-    uint32_t* turn = reinterpret_cast<uint32_t*>(sm + S::TURNS + (warp - 4) * TURN);
+    const uint32_t turn = tc::smem_addr(sm + S::TURNS + (warp - 4) * TURN);
     auto filled = [&](int n) {
       if (!tc::mbar_wait(&acc_full[n & 1], (n >> 1) & 1, POLLS)) {
         *fail = 1;

@@ -49,8 +49,11 @@ __device__ __forceinline__ bool elect() {   // one lane of a converged warp
   return p != 0;
 }
 // two 16-bit values of a runtime type in a word, and back
-__device__ __forceinline__ uint32_t pack_pair(float a, float b, int type) {
-  return type == VERACE_BF16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, int type) {   // (one packed conversion: the single ones share the
+  uint32_t w;                                                                    // unit of the exponentials)
+  if (type == VERACE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+  return w;
 }
 __device__ __forceinline__ float2 unpack_pair(uint32_t w, int type) {
   return type == VERACE_BF16 ? unpack2<__nv_bfloat16>(w) : unpack2<__half>(w);
@@ -167,13 +170,8 @@ __device__ __forceinline__ void finish4(const Epilogue& e, long long m, long lon
     store4(e.pre, m * e.ld + c, n, VERACE_F32, g);
     if (GATED) store4(e.pre_up, m * e.ld + c, n, VERACE_F32, u);
   }
-  by_act(e.act, e.type != VERACE_F32, [&](auto act, auto fast) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (GATED) g[j] = gate_<decltype(act)::value, decltype(fast)::value>(g[j], u[j], e.b1, e.b2, e.r1, e.r2);
-      else g[j] = act_<decltype(act)::value, decltype(fast)::value>(g[j]);
-    }
-  });
+  if (e.type == VERACE_F32) activate<GATED, false>(e, g, u);
+  else activate<GATED, true>(e, g, u);
   if (!GATED && e.residual) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] += res[j];
