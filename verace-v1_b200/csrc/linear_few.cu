@@ -7,8 +7,8 @@
 // stream.  Few tiles: K is split over a cluster of up to 8 CTAs, whose partial sums are joined through
 // distributed shared memory in rank order.
 //
-// Warps: 0 feeds the stages, 1 issues the MMAs, 2 to 5 read the sums (all join them): a thread holds a weight row, so
-// neighbouring threads store neighbouring outputs of a token.  The input gradient of few tokens
+// Warps: 0 feeds the stages, 1 issues the MMAs; then all eight read the sums, two a quarter of TMEM: a thread holds a weight
+// row, so neighbouring threads store neighbouring outputs of a token.  The input gradient of few tokens
 // (a_mn: weights stored [K][N], read as MN-major) runs here too, for a gated block over both weights.
 #include "linear_tc.cuh"
 
@@ -62,12 +62,12 @@ __device__ __forceinline__ void load_rows16(const void* p, long long i, long lon
   if (type == VERACE_F32) {
     const float* f = static_cast<const float*>(p) + i;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = j < n ? f[j * ld] : 0.f;
+    for (int j = 0; j < 16; ++j, f += ld) v[j] = j < n ? *f : 0.f;
   } else {
     const unsigned short* f = static_cast<const unsigned short*>(p) + i;
     uint32_t w[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) w[j] = j < n ? f[j * ld] : 0u;
+    for (int j = 0; j < 16; ++j, f += ld) w[j] = j < n ? *f : 0u;
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = unpack_pair(w[j], type).x;
   }
@@ -76,18 +76,26 @@ __device__ __forceinline__ void store_rows16(void* p, long long i, long long ld,
   if (type == VERACE_F32) {
     float* f = static_cast<float*>(p) + i;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) f[j * ld] = v[j];
+    for (int j = 0; j < 16; ++j, f += ld)
+      if (j < n) *f = v[j];
   } else {
     unsigned short* f = static_cast<unsigned short*>(p) + i;
+    uint32_t w[8];
+    if (type == VERACE_BF16) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) f[j * ld] = (unsigned short)pack_pair(v[j], 0.f, type);
+      for (int j = 0; j < 8; ++j) w[j] = pack_pair(v[2 * j], v[2 * j + 1], VERACE_BF16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = pack_pair(v[2 * j], v[2 * j + 1], VERACE_F16);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j, f += ld)
+      if (j < n) *f = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
   }
 }
 
 template <bool F8, bool WMN, bool GATED>
-__global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
   constexpr int KB = F8 ? 128 : 64, WB = GATED ? 2 * ROWS * 128 : ROWS * 128;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((size_t)raw + 1023) & ~(size_t)1023);
@@ -174,7 +182,6 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
     }
     if (lead) tc::commit(&done);
     __syncwarp();
-    tc::mbar_wait(&done, 0, POLLS);   // (every MMA issued completes before the CTA may end)
   }
   __syncwarp();
   // ---- the sums
@@ -182,19 +189,17 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
   const int quarter = warp & 3;
   const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
   const int n = n0 + 32 * quarter + lane;
-  bool ok = true;
-  if (warp >= 2 && warp < 6) {
-    ok = tc::mbar_wait(&done, 0, POLLS) && !fail;
-    if (!ok && lane == 0) atomicExch(&g_linear_few_status, 1);
-    tc::fence_after_sync();
-  }
+  const bool ok = tc::mbar_wait(&done, 0, POLLS) && !fail;
+  if (!ok && lane == 0) atomicExch(&g_linear_few_status, 1);
+  tc::fence_after_sync();
   if (p.ck == 1) {
-    if (warp >= 2 && warp < 6 && ok) {
+    if (ok) {
       const Epilogue& e = p.e;
       const bool in = n < p.N;
       const float cs = e.col_scale && in ? e.col_scale[n] : 1.f, us = GATED && e.up_scale && in ? e.up_scale[n] : 1.f;
       const float bias = !GATED && e.bias && in ? load_as(e.bias, n, e.bias_type) : 0.f;
-      for (int t = 0; t < tokens; t += 16) {
+#pragma unroll 1
+      for (int t = 16 * (warp >> 2); t < tokens; t += 32) {
         uint32_t r[16], s[16];
         tmem_ld_async(mine + t, r);
         if (GATED) tmem_ld_async(mine + p.mp + t, s);
@@ -231,18 +236,16 @@ __global__ void __launch_bounds__(NT) few_product(const __grid_constant__ Maps m
     cg::cluster_group cl = cg::this_cluster();
     float* part = reinterpret_cast<float*>(sm);
     for (int t0 = 0; t0 < tokens; t0 += p.round) {
-      if (warp >= 2 && warp < 6) {
-        for (int t = 0; t < p.round && t0 + t < tokens; t += 16)
+      for (int t = 16 * (warp >> 2); t < p.round && t0 + t < tokens; t += 32)
 #pragma unroll
-          for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-            uint32_t r[16];
-            tmem_ld_async(mine + h * p.mp + t0 + t, r);
-            tmem_wait(r);
-            float* o = part + (h * p.round + t) * ROWS + 32 * quarter + lane;
+        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+          uint32_t r[16];
+          tmem_ld_async(mine + h * p.mp + t0 + t, r);
+          tmem_wait(r);
+          float* o = part + (h * p.round + t) * ROWS + 32 * quarter + lane;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j * ROWS] = ok && first < last ? __uint_as_float(r[j]) : 0.f;
-          }
-      }
+          for (int j = 0; j < 16; ++j) o[j * ROWS] = ok && first < last ? __uint_as_float(r[j]) : 0.f;
+        }
       cl.sync();
       const int total = min(p.round, tokens - t0) * (ROWS / 4);
 #pragma unroll 2

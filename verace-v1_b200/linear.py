@@ -24,7 +24,8 @@ from ._lib import E4M3, F32, check, lib
 from .int4 import _require_no_grad
 from .kernels import _DTYPE, _norm_args
 
-ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "situ": 5}
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+_GATES = {"situ": 5, "silu": 2, "gelu": 3, "gelu_tanh": 4, "relu": 1}
 FP8 = torch.float8_e4m3fn
 _CODE = {**_DTYPE, FP8: E4M3}
 _ALIGN = {torch.float32: 1, torch.bfloat16: 8, torch.float16: 8, FP8: 16}   # values in 16 bytes (fp32 rows: any)
@@ -32,9 +33,11 @@ _ALIGN = {torch.float32: 1, torch.bfloat16: 8, torch.float16: 8, FP8: 16}   # va
 
 def _rows(t: torch.Tensor, m: int, k: int) -> Tuple[torch.Tensor, int]:
     """t as [m, k] whose rows the kernels can address, and its row stride; copied where it has to be."""
+    a = _ALIGN[t.dtype]
+    if k % a == 0 and t.is_contiguous() and (a == 1 or t.data_ptr() % 16 == 0):
+        return t, k
     if t.dim() != 2:
         t = t.reshape(m, k)
-    a = _ALIGN[t.dtype]
     ld = t.stride(0) if m > 1 else -(-k // a) * a
     if (k > 1 and t.stride(1) != 1) or ld < k or ld % a or (a > 1 and t.data_ptr() % 16):
         ld = -(-k // a) * a
@@ -54,27 +57,32 @@ def _vector(t: Optional[torch.Tensor], n: int, dtype: torch.dtype, device, what:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _checked(who, x, weights, scales, activation, allowed, out_dtype, default):
-    """Checks what both products take; returns (k, out dtype)."""
-    assert x.is_cuda, "This kernel requires CUDA tensors"
+def _checked(who, x, weight, scales, want, activation, allowed, out_dtype, default):
+    """Checks what both products take (``scales`` of ``want`` are given); returns (activation, k, n, out dtype)."""
     dt = x.dtype
+    act = allowed.get(activation)
+    shape, (n, k) = x.shape, weight.shape
     if dt not in _CODE:
         raise ValueError(f"{who}: {dt} inputs (expected fp32, bf16, fp16 or float8_e4m3fn)")
-    if activation not in allowed:
-        raise ValueError(f"{who}: activation {activation!r} (expected one of {allowed})")
-    assert x.dim() >= 1, "x must have at least one dimension"
-    k = x.shape[-1]
-    for w in weights:
-        assert w.dtype is dt and w.dim() == 2 and w.shape == (weights[0].shape[0], k) and w.device == x.device, \
-            f"{who}: the weights must be [n, {k}] in x's dtype, on its device"
-    eight = dt is FP8
-    if any((s is not None) != eight for s in scales):
-        raise ValueError(f"{who}: scales go with float8_e4m3fn operands, one for x and one for each weight")
+    if act is None:
+        raise ValueError(f"{who}: activation {activation!r} (expected one of {tuple(allowed)})")
+    assert len(shape) >= 1, "x must have at least one dimension"
+    assert weight.dtype is dt and shape[-1] == k and weight.device == x.device, \
+        f"{who}: the weights must be [n, {shape[-1]}] in x's dtype, on its device"
+    if dt is FP8:
+        if scales != want:
+            raise ValueError(f"{who}: float8_e4m3fn operands need their scales, one for x and one for each weight")
+        out_dtype = default if out_dtype is None else out_dtype
+        if out_dtype not in _DTYPE:
+            raise ValueError(f"{who}: out_dtype {out_dtype} for {dt} inputs")
+        return act, k, n, out_dtype
+    if scales:
+        raise ValueError(f"{who}: scales go with float8_e4m3fn operands")
     if out_dtype is None:
-        out_dtype = default if eight else dt
-    if out_dtype not in _DTYPE or not (eight or out_dtype is dt or out_dtype is torch.float32):
+        out_dtype = dt
+    elif out_dtype is not dt and out_dtype is not torch.float32:
         raise ValueError(f"{who}: out_dtype {out_dtype} for {dt} inputs")
-    return k, out_dtype
+    return act, k, n, out_dtype
 
 
 def _workspace(nbytes: int, device):
@@ -88,7 +96,7 @@ def _p(t: Optional[torch.Tensor]):
 # ---------------------------------------------------------------------------- act(x Wᵀ + bias) + residual
 def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
     dev = x2.device
-    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=dev)
     pre = torch.empty((m, n), dtype=torch.float32, device=dev) if want_pre else None
     L = lib()
     code = _CODE[x2.dtype]
@@ -156,24 +164,31 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     them; the output is then fp32, bf16 or fp16 (``out_dtype``, else the residual's dtype, else bf16), the bias of
     the same dtype.  The other types are differentiable in x, weight, bias and residual (once)."""
     dev = x.device
-    if x.is_cuda and dev.index != current():
+    if dev.index is None or dev.index != current():
+        assert x.is_cuda, "This kernel requires CUDA tensors"
         with torch.cuda.device(dev):
             return fused_linear(x, weight, bias, activation=activation, residual=residual, x_scale=x_scale,
                                 w_scale=w_scale, out_dtype=out_dtype)
-    default = torch.bfloat16 if residual is None else residual.dtype
-    k, odt = _checked("fused_linear", x, (weight,), (x_scale, w_scale), activation,
-                      (None, "relu", "silu", "gelu", "gelu_tanh"), out_dtype, default)
-    n, lead = weight.shape[0], x.shape[:-1]
-    m = math.prod(lead)
-    assert residual is None or (residual.shape == lead + (n,) and residual.dtype is odt and residual.device == dev), \
-        f"residual must be {tuple(lead) + (n,)} in {odt}, on x's device"
-    act = ACTIVATIONS[activation]
+    act, k, n, odt = _checked("fused_linear", x, weight, (x_scale is not None) + (w_scale is not None), 2, activation,
+                              _ACTIVATIONS, out_dtype, torch.bfloat16 if residual is None else residual.dtype)
+    lead = x.shape[:-1]
+    flat = len(lead) == 1
+    m = lead[0] if flat else math.prod(lead)
     eight = x.dtype is FP8
-    bias_dtype = odt if eight else x.dtype
-    assert bias is None or (bias.dtype is bias_dtype and bias.shape == (n,) and bias.device == dev), \
-        f"bias must be [{n}] in {bias_dtype}, on x's device"
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+    b = bias
+    if bias is not None:
+        bias_dtype = odt if eight else x.dtype
+        assert bias.dtype is bias_dtype and bias.shape == (n,) and bias.device == dev, \
+            f"bias must be [{n}] in {bias_dtype}, on x's device"
+        grad = grad or bias.requires_grad and torch.is_grad_enabled()
+        if not bias.is_contiguous():
+            b = bias.contiguous()
+    if residual is not None:
+        assert residual.shape == lead + (n,) and residual.dtype is odt and residual.device == dev, \
+            f"residual must be {tuple(lead) + (n,)} in {odt}, on x's device"
+        grad = grad or residual.requires_grad and torch.is_grad_enabled()
+    if grad:
         if eight:
             raise RuntimeError("fused_linear runs 8-bit operands for inference (no autograd path): "
                                "call it under torch.no_grad()")
@@ -185,8 +200,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
         sw = _vector(w_scale, n, torch.float32, dev, "w_scale")
     res, ldr = _residual_rows(residual, m, n)
-    y, _ = _linear(x2, ldx, sx, w2, ldw, sw, _vector(bias, n, bias_dtype, dev, "bias"), res, ldr, m, n, k, act, odt, False)
-    return y if x.dim() == 2 else y.view(lead + (n,))
+    y, _ = _linear(x2, ldx, sx, w2, ldw, sw, b, res, ldr, m, n, k, act, odt, False)
+    return y if flat else y.view(lead + (n,))
 
 
 # ---------------------------------------------------------------------------- act(x Wgᵀ) up(x Wuᵀ)
@@ -205,7 +220,7 @@ def _gate_rows(w_gate, w_up, f, k):
 
 def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
     dev = x2.device
-    h = torch.empty((m, f), dtype=out_dtype, device=dev)
+    h = torch.empty_strided((m, f), (f, 1), dtype=out_dtype, device=dev)
     gate, up = torch.empty((2, m, f), dtype=torch.float32, device=dev) if want_pre else (None, None)
     L = lib()
     code = _CODE[x2.dtype]
@@ -264,17 +279,20 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     multiply them, and the output is fp32, bf16 (the default) or fp16.  The other types are differentiable in x, w_gate
     and w_up (once); the pass keeps g and u, in fp32, for the backward."""
     dev = x.device
-    if x.is_cuda and dev.index != current():
+    if dev.index is None or dev.index != current():
+        assert x.is_cuda, "This kernel requires CUDA tensors"
         with torch.cuda.device(dev):
             return gated_linear(x, w_gate, w_up, activation=activation, beta1=beta1, beta2=beta2, x_scale=x_scale,
                                 gate_scale=gate_scale, up_scale=up_scale, out_dtype=out_dtype)
-    k, odt = _checked("gated_linear", x, (w_gate, w_up), (x_scale, gate_scale, up_scale), activation,
-                      ("situ", "silu", "gelu", "gelu_tanh", "relu"), out_dtype, torch.bfloat16)
-    if activation == "situ" and not (beta1 and beta2):
+    act, k, f, odt = _checked("gated_linear", x, w_gate, (x_scale is not None) + (gate_scale is not None)
+                              + (up_scale is not None), 3, activation, _GATES, out_dtype, torch.bfloat16)
+    assert w_up.shape == w_gate.shape and w_up.dtype is w_gate.dtype and w_up.device == dev, \
+        "gated_linear: the weights must be two of one shape and dtype, on x's device"
+    if act == 5 and not (beta1 and beta2):
         raise ValueError(f"gated_linear: beta1 {beta1}, beta2 {beta2} (expected anything but 0)")
-    f, lead = w_gate.shape[0], x.shape[:-1]
-    m = math.prod(lead)
-    act = ACTIVATIONS[activation]
+    lead = x.shape[:-1]
+    flat = len(lead) == 1
+    m = lead[0] if flat else math.prod(lead)
     eight = x.dtype is FP8
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         if eight:
@@ -289,69 +307,75 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
         sg = _vector(gate_scale, f, torch.float32, dev, "gate_scale")
         su = _vector(up_scale, f, torch.float32, dev, "up_scale")
     h, _, _ = _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, beta1, beta2, odt, False)
-    return h if x.dim() == 2 else h.view(lead + (f,))
+    return h if flat else h.view(lead + (f,))
 
 
 # ---------------------------------------------------------------------------- rows in 8 bits
-def _to_fp8(who, h, y, sum_out, wp, eps, norm, return_norm):
-    dev = h.device
-    cols = h.shape[-1]
-    rows = h.numel() // cols if cols else 0
-    q = torch.empty(h.shape, dtype=FP8, device=dev)
-    scale = torch.empty(h.shape[:-1], dtype=torch.float32, device=dev)
+def _to_fp8(who, h, y, sum_out, norm, return_norm):
+    """The rows of h (of h + y, which goes to sum_out) in 8 bits; norm None: as they are.  All contiguous."""
+    dt, shape = h.dtype, h.shape
+    code = _DTYPE.get(dt)
+    if code is None:
+        raise ValueError(f"{who}: {dt} inputs (expected fp32, bf16 or fp16)")
+    assert len(shape) >= 1 and shape[-1] > 0, f"{who}: rows of at least one value"
+    if h.requires_grad:
+        _require_no_grad(h, who)
+    dev, cols = h.device, shape[-1]
+    w, eps = (None, 0.0) if norm is None else _norm_args(norm, h)
+    q = torch.empty_like(h, dtype=FP8)
+    if len(shape) == 2:
+        scale = torch.empty_strided(shape[:1], (1,), dtype=torch.float32, device=dev)
+    else:
+        scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
     n = torch.empty_like(h) if return_norm else None
-    rc = lib().verace_rmsnorm_fp8(h.data_ptr(), _p(y), _p(sum_out), wp, eps, norm, q.data_ptr(), scale.data_ptr(), _p(n),
-                                  rows, cols, _DTYPE[h.dtype], raw_stream(dev.index))
+    rc = lib().verace_rmsnorm_fp8(h.data_ptr(), None if y is None else y.data_ptr(),
+                                  None if y is None else sum_out.data_ptr(), w or None, eps, 0 if norm is None else 1,
+                                  q.data_ptr(), scale.data_ptr(), None if n is None else n.data_ptr(), h.numel() // cols,
+                                  cols, code, raw_stream(dev.index))
     if rc:
         check(rc, who)
     return (q, scale, n) if return_norm else (q, scale)
 
 
-def _fp8_input(who, x):
-    assert x.is_cuda, "This kernel requires CUDA tensors"
-    if x.requires_grad:
-        _require_no_grad(x, who)
-    if x.dtype not in _DTYPE:
-        raise ValueError(f"{who}: {x.dtype} inputs (expected fp32, bf16 or fp16)")
-    assert x.dim() >= 1 and x.shape[-1] > 0, f"{who}: rows of at least one value"
-
-
 def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """The rows of x [..., k] (fp32, bf16 or fp16; k up to 32768) as (float8_e4m3fn [..., k], fp32 scales [...]):
     scale = max(max |x|, 2^-100) / 448 of the row, values rounded to the nearest."""
-    _fp8_input("quantize_fp8", x)
-    if x.device.index != current():
+    dev = x.device
+    if dev.index is None or dev.index != current():
+        assert x.is_cuda, "This kernel requires CUDA tensors"
         with torch.cuda.device(x.device):
             return quantize_fp8(x)
-    return _to_fp8("quantize_fp8", x.detach().contiguous(), None, None, None, 0.0, 0, False)
+    return _to_fp8("quantize_fp8", x.contiguous(), None, None, None, False)
 
 
 def rmsnorm_fp8(x: torch.Tensor, norm: nn.RMSNorm, *, return_norm: bool = False):
     """``norm`` (a torch.nn.RMSNorm over the last dimension) applied to x, its rows in 8 bits as
     ``quantize_fp8`` gives them: (q, scale), and with ``return_norm`` the norm's output in x's dtype as well.
     The values are not rounded to x's dtype before they are rounded to 8 bits."""
-    _fp8_input("rmsnorm_fp8", x)
-    if x.device.index != current():
+    dev = x.device
+    if dev.index is None or dev.index != current():
+        assert x.is_cuda, "This kernel requires CUDA tensors"
         with torch.cuda.device(x.device):
             return rmsnorm_fp8(x, norm, return_norm=return_norm)
-    x = x.contiguous()
-    w, eps = _norm_args(norm, x)
-    return _to_fp8("rmsnorm_fp8", x, None, None, w or None, eps, 1, return_norm)
+    return _to_fp8("rmsnorm_fp8", x.contiguous(), None, None, norm, return_norm)
 
 
 def add_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, norm: nn.RMSNorm, *, out: Optional[torch.Tensor] = None,
                     return_norm: bool = False):
     """A block's residual step ahead of 8-bit products, in one pass: h <- h + y in place (or into ``out``),
     then ``rmsnorm_fp8`` of the sum: (q, scale), and with ``return_norm`` the norm's output as well."""
-    _fp8_input("add_rmsnorm_fp8", h)
-    if h.device.index != current():
-        with torch.cuda.device(h.device):
+    dev = h.device
+    if dev.index is None or dev.index != current():
+        assert h.is_cuda, "This kernel requires CUDA tensors"
+        with torch.cuda.device(dev):
             return add_rmsnorm_fp8(h, y, norm, out=out, return_norm=return_norm)
     if y.requires_grad:
         _require_no_grad(y, "add_rmsnorm_fp8")
-    out = h if out is None else out
-    assert y.shape == h.shape and y.dtype is h.dtype and y.device == h.device, "h and y must match"
-    assert out.shape == h.shape and out.dtype is h.dtype and out.device == h.device and out.is_contiguous(), \
-        "the sum goes to a contiguous tensor of h's shape, dtype and device"
-    w, eps = _norm_args(norm, h)
-    return _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, w or None, eps, 1, return_norm)
+    assert y.shape == h.shape and y.dtype is h.dtype and y.device == dev, "h and y must match"
+    if out is None:
+        out = h
+    elif out is not h:
+        assert out.shape == h.shape and out.dtype is h.dtype and out.device == dev, \
+            "the sum goes to a tensor of h's shape, dtype and device"
+    assert out.is_contiguous(), "the sum goes to a contiguous tensor"
+    return _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, norm, return_norm)
