@@ -375,7 +375,7 @@ VERACE_API int verace_sample(const void* logits, long long ld, const float* nois
  *   a = max(max |v|, 2^-100); scale = a / 448; q = v 448 / a in e4m3 (to nearest even)
  * h, y, sum, n: [rows, cols] (dtype), dense; q: [rows, cols] bytes; scale: [rows] fp32; n, or NULL: v
  * rounded to dtype.  sum may be h or y.  v is not rounded to dtype before it is rounded to 8 bits.
- * 1 <= cols <= 32768.
+ * 1 <= cols <= 32761, or 32768 with 16-byte aligned tensors.
  * ---------------------------------------------------------------------------- */
 VERACE_API int verace_rmsnorm_fp8(const void* h, const void* y, void* sum, const void* weight, float eps, int norm,
                                   void* q, float* scale, void* n, long long rows, int cols, int dtype, void* stream);

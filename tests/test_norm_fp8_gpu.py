@@ -116,6 +116,39 @@ def test_misaligned_rows_and_aliases(dt):
     check((h.float() + h.float()).to(dt), norm, *twice)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cols", [13, 1017, 1018, 4090, 5001, 32761])
+def test_rows_anywhere_in_a_word(dt, cols):
+    """Every tensor off the others' alignment; nothing is written beside the outputs."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+
+    def at(offset, *shape):
+        flat = torch.randn(5 * cols + 16, device="cuda", generator=g).to(dt)
+        return flat, flat[offset:offset + 5 * cols].view(5, cols)
+    _, h = at(1, 5, cols)
+    _, y = at(2, 5, cols)
+    whole, into = at(3, 5, cols)
+    before = whole.clone()
+    norm = torch.nn.RMSNorm(cols, eps=1e-6, device="cuda", dtype=dt).requires_grad_(False)
+    norm.weight = torch.nn.Parameter(at(5, 5, cols)[1][0], requires_grad=False)
+    q, s, n = V.add_rmsnorm_fp8(h, y, norm, out=into, return_norm=True)
+    want = (h.float() + y.float()).to(dt)
+    assert torch.equal(into, want)
+    check(want, norm, q, s, n)
+    whole[3:3 + 5 * cols] = before[3:3 + 5 * cols]
+    assert torch.equal(whole, before)
+    # the 8-bit output in an odd place, through the C entry point
+    flat = torch.full((5 * cols + 16,), 7, device="cuda", dtype=torch.uint8)
+    s2 = torch.empty(5, device="cuda")
+    rc = V._lib.lib().verace_rmsnorm_fp8(want.data_ptr(), None, None, norm.weight.data_ptr(), 1e-6, 1, flat.data_ptr() + 3,
+                                         s2.data_ptr(), None, 5, cols, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dt],
+                                         torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    # (against the formula: the order of a row's squares follows its words, and want starts at another place than h)
+    check(want, norm, flat[3:3 + 5 * cols].clone().view(torch.float8_e4m3fn).view(5, cols), s2)
+    assert (flat[:3] == 7).all() and (flat[3 + 5 * cols:] == 7).all()
+
+
 def test_empty_and_refusals():
     norm = torch.nn.RMSNorm(64, device="cuda", dtype=torch.bfloat16).requires_grad_(False)
     q, s = V.rmsnorm_fp8(torch.zeros(0, 64, device="cuda", dtype=torch.bfloat16), norm)
@@ -131,6 +164,10 @@ def test_empty_and_refusals():
         V.rmsnorm_fp8(x.float(), norm)
     with pytest.raises(RuntimeError, match="32768"):
         V.quantize_fp8(torch.zeros(1, 32769, device="cuda"))
+    with pytest.raises(RuntimeError, match="32761"):
+        V.quantize_fp8(torch.zeros(1, 32762, device="cuda"))
+    with pytest.raises(RuntimeError, match="32761"):
+        V.quantize_fp8(torch.zeros(32769, device="cuda")[1:].view(1, 32768))
     with pytest.raises(RuntimeError, match="no_grad"):
         V.quantize_fp8(x.clone().requires_grad_())
     with pytest.raises(AssertionError):

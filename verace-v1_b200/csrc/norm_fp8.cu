@@ -6,11 +6,13 @@
 // 2^-100 keeps 448 / a finite; a row of zeros gives zeros.  A NaN or infinity in a row makes its
 // scale NaN or leaves NaN in its place, as in torch.
 //
-// Bound: bytes (7 a value with the residual in 16 bits).  A row stays in the registers of its
-// group of threads: a warp for up to 1024 values, 128, 512 or 1024 threads beyond, 32 values a
-// thread; two reductions (squares, then magnitudes) by shuffles and, above a warp, one exchange
-// through shared memory each.  Rows of a width that is no multiple of 8, or not 16-byte aligned,
-// are read value by value, neighbouring threads at neighbouring places.
+// Bound: bytes (7 a value with the residual in 16 bits; 16384 x 4096 bf16 with the residual 71.7 us, 6.55 TB/s, the
+// rate of a copy).  A row stays in the registers of its group of threads: a warp for up to 1024 values, 128 to
+// 1024 threads beyond, 32 values a thread, all loads of a row in flight before its first store; two
+// reductions (squares, then magnitudes) by shuffles and, above a warp, one exchange through shared memory each.
+// Rows whose width is no multiple of 8 start anywhere in a 16-byte word: their words are those of the whole
+// tensor, the first and last one masked, so that all but the norm's weights is read and written a word
+// at a time all the same (1111 x 5001 fp32: 14.7 us, value by value 19.9).
 #include "common.cuh"
 
 #include <cuda_fp8.h>
@@ -34,22 +36,35 @@ struct NormArgs {
   float eps;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    unpack8<T>(*reinterpret_cast<const uint4*>(p), x);
+// VEC neighbouring values (16 bytes, or 32 of fp32), as loaded
+template <typename T, int VEC>
+struct Lot {
+  static constexpr int WORDS = VEC * (int)sizeof(T) / 16;
+  uint4 w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* x) {
+  __device__ __forceinline__ void values(float (&v)[VEC]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) {
+        v[4 * i] = __uint_as_float(w[i].x); v[4 * i + 1] = __uint_as_float(w[i].y);
+        v[4 * i + 2] = __uint_as_float(w[i].z); v[4 * i + 3] = __uint_as_float(w[i].w);
+      }
+    } else {
+      unpack8<T>(w[0], v);
+    }
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
   if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   } else {
-    *reinterpret_cast<uint4*>(p) = pack8<T>(x);
+    *reinterpret_cast<uint4*>(p) = pack8<T>(v);
   }
 }
 template <typename T>
@@ -57,45 +72,73 @@ __device__ __forceinline__ float rounded(float x) {
   return to_f32(from_f32<T>(x));
 }
 
-// A group of G threads holds a row of up to 32 G values: VEC (8 or 1) neighbouring ones at VEC (g + G i).
-template <typename T, int G, int VEC>
+// A group of G threads holds a row of up to 32 G values: VEC neighbouring ones from column VEC (g + G i) on, less
+// `shift`, the row's place in its first word, where rows are not WHOLE words.
+template <typename T, int G, bool WHOLE, bool ADD>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a) {
-  constexpr int NT = G < 128 ? 128 : G, NV = 32 / VEC, W = G / 32;
+  constexpr int NT = G < 128 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G / 32;
   __shared__ float part[2][W > 1 ? W : 1];
   const int g = threadIdx.x % G;
   const long long row = (long long)blockIdx.x * (NT / G) + threadIdx.x / G;
   if (G < 128 && row >= a.rows) return;   // (whole warps; larger groups are one row a CTA)
   const long long off = row * a.cols;
   const T* h = static_cast<const T*>(a.h) + off;
-  const T* y = a.y ? static_cast<const T*>(a.y) + off : nullptr;
   const T* w = static_cast<const T*>(a.w);
-  float v[NV][VEC];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = VEC * (g + G * i);
-    if (c < a.cols) {
-      if constexpr (VEC == 8) load8<T>(h + c, v[i]);
-      else v[i][0] = to_f32(h[c]);
+  const int shift = WHOLE ? 0 : (int)(((size_t)h & 15) / sizeof(T));
+  auto column = [&](int i) { return VEC * (g + G * i) - shift; };
+  auto any = [&](int i) { return VEC * G * i < a.cols + shift && column(i) < a.cols; };
+  auto in = [&](int c) { return WHOLE || (c >= 0 && c < a.cols); };
+  // whether a vector of p may be moved as one: inside of the row, and p's words where h's are
+  auto as_one = [&](const T* p, int c) {
+    return WHOLE || (c >= 0 && c + VEC <= a.cols && ((size_t)(p + off + c) & 15) == 0);
+  };
+  auto put = [&](void* to, int c, const float (&v)[VEC]) {
+    T* p = static_cast<T*>(to);
+    if (as_one(p, c)) {
+      store<T, VEC>(p + off + c, v);
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+      for (int j = 0; j < VEC; ++j)
+        if (in(c + j)) p[off + c + j] = from_f32<T>(v[j]);
     }
-  }
-  if (y) {
-    T* sum = static_cast<T*>(a.sum) + off;
+  };
+  float v[NV][VEC];
+  {
+    // h and y on their way together, before the first store (sum may be either)
+    Lot<T, VEC> lh[NV], ly[ADD ? NV : 1];
+    const T* y = static_cast<const T*>(a.y);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (any(i)) {
+        lh[i].load(h + column(i));
+        if constexpr (ADD) {
+          if (as_one(y, column(i))) {
+            ly[i].load(y + off + column(i));
+          } else {
+            float t[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) t[j] = in(column(i) + j) ? to_f32(y[off + column(i) + j]) : 0.f;
+            store<T, VEC>(reinterpret_cast<T*>(ly[i].w), t);
+          }
+        }
+      }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = VEC * (g + G * i);
-      if (c < a.cols) {
-        if constexpr (VEC == 8) {
-          float t[8];
-          load8<T>(y + c, t);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = rounded<T>(v[i][j] + t[j]);
-          store8<T>(sum + c, v[i]);
-        } else {
-          v[i][0] = rounded<T>(v[i][0] + to_f32(y[c]));
-          sum[c] = from_f32<T>(v[i][0]);
+      for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+      if (any(i)) {
+        lh[i].values(v[i]);
+        if constexpr (!WHOLE) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (!in(column(i) + j)) v[i][j] = 0.f;
+        }
+        if constexpr (ADD) {
+          float t[VEC];
+          ly[i].values(t);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[i][j] = rounded<T>(v[i][j] + (in(column(i) + j) ? t[j] : 0.f));
+          put(a.sum, column(i), v[i]);
         }
       }
     }
@@ -117,24 +160,29 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
     }
     const float rs = rsqrtf(ss / (float)a.cols + a.eps);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = VEC * (g + G * i);
-      if (c < a.cols) {
+    for (int i = 0; i < NV; ++i)
+      if (any(i)) {
         float t[VEC];
         if (w) {
-          if constexpr (VEC == 8) load8<T>(w + c, t);
-          else t[0] = to_f32(w[c]);
+          if constexpr (WHOLE) {
+            Lot<T, VEC> lw;
+            lw.load(w + column(i));
+            lw.values(t);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) t[j] = in(column(i) + j) ? to_f32(w[column(i) + j]) : 0.f;
+          }
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[i][j] = w ? v[i][j] * rs * t[j] : v[i][j] * rs;
       }
-    }
   }
   float top = 0x1p-100f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) top = max_nan(top, fabsf(v[i][j]));
+    for (int j = 0; j < VEC; ++j)
+      if (in(column(i) + j)) top = max_nan(top, fabsf(v[i][j]));   // (0 rs is NaN where rs is infinite)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if constexpr (W > 1) {
@@ -145,44 +193,51 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
   }
   const float inv = 448.f / top;
   if (g == 0) a.scale[row] = top / 448.f;
-  uint8_t* q = a.q + off;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = VEC * (g + G * i);
-    if (c < a.cols) {
-      if constexpr (VEC == 8) {
-        uint32_t o[2];
+  for (int i = 0; i < NV; ++i)
+    if (any(i)) {
+      const int c = column(i);
+      uint32_t o[VEC / 4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i][4 * j] * inv, v[i][4 * j + 1] * inv),
-                                                       __NV_SATFINITE, __NV_E4M3);
-          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i][4 * j + 2] * inv, v[i][4 * j + 3] * inv),
-                                                       __NV_SATFINITE, __NV_E4M3);
-          o[j] = lo | hi << 16;
-        }
-        *reinterpret_cast<uint2*>(q + c) = make_uint2(o[0], o[1]);
-        if (a.n) store8<T>(static_cast<T*>(a.n) + off + c, v[i]);
-      } else {
-        q[c] = __nv_cvt_float_to_fp8(v[i][0] * inv, __NV_SATFINITE, __NV_E4M3);
-        if (a.n) static_cast<T*>(a.n)[off + c] = from_f32<T>(v[i][0]);
+      for (int j = 0; j < VEC / 4; ++j) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i][4 * j] * inv, v[i][4 * j + 1] * inv), __NV_SATFINITE,
+                                                     __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i][4 * j + 2] * inv, v[i][4 * j + 3] * inv),
+                                                     __NV_SATFINITE, __NV_E4M3);
+        o[j] = lo | hi << 16;
       }
+      uint8_t* q = a.q + off + c;
+      if (WHOLE || (c >= 0 && c + VEC <= a.cols && (size_t)q % VEC == 0)) {
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q) = make_uint2(o[0], o[1]);
+        else *reinterpret_cast<uint32_t*>(q) = o[0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (in(c + j)) q[j] = (uint8_t)(o[j / 4] >> (8 * (j & 3)));
+      }
+      if (a.n) put(a.n, c, v[i]);
     }
-  }
 }
 
-template <typename T, int VEC>
+template <typename T, bool WHOLE, bool ADD>
 int launch(const NormArgs& a, cudaStream_t st) {
-  if (a.cols <= 1024) norm_fp8_kernel<T, 32, VEC><<<(unsigned)((a.rows + 3) / 4), 128, 0, st>>>(a);
-  else if (a.cols <= 4096) norm_fp8_kernel<T, 128, VEC><<<(unsigned)a.rows, 128, 0, st>>>(a);
-  else if (a.cols <= 16384) norm_fp8_kernel<T, 512, VEC><<<(unsigned)a.rows, 512, 0, st>>>(a);
-  else norm_fp8_kernel<T, 1024, VEC><<<(unsigned)a.rows, 1024, 0, st>>>(a);
+  const int cols = a.cols + (WHOLE ? 0 : 7);   // (a row may start in the middle of a word)
+  if (cols <= 1024) norm_fp8_kernel<T, 32, WHOLE, ADD><<<(unsigned)((a.rows + 3) / 4), 128, 0, st>>>(a);
+  else if (cols <= 4096) norm_fp8_kernel<T, 128, WHOLE, ADD><<<(unsigned)a.rows, 128, 0, st>>>(a);
+  else if (cols <= 8192) norm_fp8_kernel<T, 256, WHOLE, ADD><<<(unsigned)a.rows, 256, 0, st>>>(a);
+  else if (cols <= 16384) norm_fp8_kernel<T, 512, WHOLE, ADD><<<(unsigned)a.rows, 512, 0, st>>>(a);
+  else norm_fp8_kernel<T, 1024, WHOLE, ADD><<<(unsigned)a.rows, 1024, 0, st>>>(a);
   return check_launch("norm_fp8_kernel");
 }
 
 template <typename T>
 int launch(const NormArgs& a, cudaStream_t st) {
   const size_t all = (size_t)a.h | (size_t)a.y | (size_t)a.w | (size_t)a.sum | (size_t)a.n;
-  return a.cols % 8 == 0 && all % 16 == 0 && (size_t)a.q % 8 == 0 ? launch<T, 8>(a, st) : launch<T, 1>(a, st);
+  const bool whole = a.cols % 8 == 0 && all % 16 == 0 && (size_t)a.q % 8 == 0;
+  VERACE_REQUIRE(whole || a.cols <= 32761, VERACE_ERR_UNSUPPORTED,
+                 "verace_rmsnorm_fp8: rows of %d columns that are not whole 16-byte words (at most 32761)", a.cols);
+  if (a.y) return whole ? launch<T, true, true>(a, st) : launch<T, false, true>(a, st);
+  return whole ? launch<T, true, false>(a, st) : launch<T, false, false>(a, st);
 }
 
 }  // namespace

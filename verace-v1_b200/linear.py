@@ -338,7 +338,7 @@ def _to_fp8(who, h, y, sum_out, norm, return_norm):
 
 
 def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The rows of x [..., k] (fp32, bf16 or fp16; k up to 32768) as (float8_e4m3fn [..., k], fp32 scales [...]):
+    """The rows of x [..., k] (fp32, bf16 or fp16; k up to 32761, or 32768) as (float8_e4m3fn [..., k], fp32 scales [...]):
     scale = max(max |x|, 2^-100) / 448 of the row, values rounded to the nearest."""
     dev = x.device
     if dev.index is None or dev.index != current():
