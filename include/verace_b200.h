@@ -386,8 +386,9 @@ VERACE_API int verace_rmsnorm_fp8(const void* h, const void* y, void* sum, const
  *   linear: out = act(x w^T + bias) + residual           act: VERACE_ACT_NONE ... GELU_TANH
  *   gated:  out = act(g) up(u), g = x w_gate^T, u = x w_up^T    act: VERACE_ACT_RELU ... SITU
  *           SITU: beta1 tanh(g / beta1) sigmoid(g) beta2 tanh(u / beta2); the others: act(g) u
- * x: [m, k], rows ldx elements apart; w: [n, k] (w_gate, w_up: [f, k]), rows ldw apart: dtype, 16-byte
- *   aligned rows unless dtype is fp32.  dtype VERACE_E4M3: x_scale [m], w_scale [n] (gate_scale, up_scale
+ * x: [m, k], rows ldx elements apart; w: [n, k] (w_gate, w_up: [f, k]), rows ldw apart: dtype.  Rows of a
+ *   multiple of 16 bytes must be 16-byte aligned unless dtype is fp32 (others may start anywhere; they are copied).
+ *   dtype VERACE_E4M3: x_scale [m], w_scale [n] (gate_scale, up_scale
  *   [f]) fp32 stand for x_scale[i] x[i][k] and so on; NULL with the other types.
  * bias: [n] (dtype; with E4M3 out_dtype) or NULL; residual: [m, n] (out_dtype), rows ld_res apart, or NULL.
  * out: [m, n] (out_dtype: dtype or VERACE_F32; with E4M3 any of the three), dense; may be the residual.

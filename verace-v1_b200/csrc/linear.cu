@@ -75,10 +75,38 @@ __global__ void __launch_bounds__(256) split_rows(const float* __restrict__ src,
   store_operand<float>(dst + row * ld + c, rows * ld, v);
 }
 
-long long padded(long long cols) { return (cols + 7) / 8 * 8; }
+// src: rows of `bytes` bytes, ld_src apart, starting anywhere -> dst: rows ld apart (a multiple of 16), zeros behind
+// them; 16 bytes a thread, read as the aligned words around them.
+__global__ void __launch_bounds__(256) align_rows(const char* __restrict__ src, long long ld_src, long long rows, long long bytes,
+                                                  char* __restrict__ dst, long long ld) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long row = i / (ld / 16), c = i % (ld / 16) * 16;
+  if (row >= rows) return;
+  const char* s = src + row * ld_src + c;
+  const int off = (int)((size_t)s & 3), left = (int)min(16LL, bytes - c);    // (left > 0: ld is bytes rounded up)
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(s - off);
+  uint32_t x[5];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) x[j] = 4 * j < off + left ? w[j] : 0u;
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    o[j] = __funnelshift_r(x[j], x[j + 1], 8 * off);
+    const int valid = left - 4 * j;
+    if (valid < 4) o[j] = valid <= 0 ? 0u : o[j] & ((1u << (8 * valid)) - 1u);
+  }
+  *reinterpret_cast<uint4*>(dst + row * ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+long long padded(long long cols, int type = VERACE_BF16) { return type == VERACE_E4M3 ? (cols + 15) / 16 * 16 : (cols + 7) / 8 * 8; }
 // bytes of an operand that a pass writes
 size_t operand_bytes(long long rows, long long cols, int type) {
-  return align_up((size_t)rows * padded(cols) * (type == VERACE_F32 ? 6 : 2), 256);
+  return align_up((size_t)rows * padded(cols, type) * (type == VERACE_F32 ? 6 : size_of(type)), 256);
+}
+// bytes of an operand made of a user's matrix: its parts, or its rows at 16-byte borders where their width is no
+// multiple of 16 bytes
+size_t copy_bytes(long long rows, long long cols, int type) {
+  return type == VERACE_F32 || cols * size_of(type) % 16 ? operand_bytes(rows, cols, type) : 0;
 }
 Mat operand_at(void* p, long long rows, long long cols, int type) {
   const long long ld = padded(cols);
@@ -96,11 +124,20 @@ struct Taker {
   }
 };
 
-// An operand of the products from a user's matrix: as it is, or split into parts in the workspace.
+bool aligned_rows(const void* p, long long ld, int type) { return (size_t)p % 16 == 0 && ld * size_of(type) % 16 == 0; }
+
+// An operand of the products from a user's matrix: as it is, split into parts or copied in the workspace.
 int operand(Mat* out, const void* p, long long ld, long long rows, long long cols, int type, Taker& ws, cudaStream_t st) {
   if (type != VERACE_F32) {
     *out = Mat{p, rows, cols, ld, 1, 0};
-    return VERACE_OK;
+    if (aligned_rows(p, ld, type)) return VERACE_OK;
+    const long long es = size_of(type);
+    out->ld = padded(cols, type);
+    out->p = ws.take(rows * out->ld * es);
+    const long long blocks = (rows * (out->ld * es / 16) + 255) / 256;
+    VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld operand is too large", rows, cols);
+    align_rows<<<(unsigned)blocks, 256, 0, st>>>((const char*)p, ld * es, rows, cols * es, (char*)out->p, out->ld * es);
+    return check_launch("align_rows");
   }
   void* dst = ws.take(operand_bytes(rows, cols, type));
   *out = operand_at(dst, rows, cols, type);
@@ -287,7 +324,7 @@ int check_types(const char* who, int dtype, int out_dtype, bool eight) {
 int check_rows(const char* who, const char* name, const void* p, long long ld, long long cols, int dtype) {
   VERACE_REQUIRE(p, VERACE_ERR_INVALID, "%s: NULL %s", who, name);
   VERACE_REQUIRE(ld >= cols, VERACE_ERR_INVALID, "%s: row stride %lld of %s < %lld", who, ld, name, cols);
-  VERACE_REQUIRE(dtype == VERACE_F32 || ((size_t)p % 16 == 0 && ld * size_of(dtype) % 16 == 0), VERACE_ERR_INVALID,
+  VERACE_REQUIRE(dtype == VERACE_F32 || cols * size_of(dtype) % 16 || aligned_rows(p, ld, dtype), VERACE_ERR_INVALID,
                  "%s: the rows of %s must be 16-byte aligned", who, name);
   return VERACE_OK;
 }
@@ -328,10 +365,12 @@ using namespace verace;
 using namespace verace::lin;
 
 extern "C" size_t verace_linear_workspace(long long m, int n, int k, int dtype) {
-  if (m <= 0 || n <= 0 || k <= 0 || by_dots(m, n, k, dtype, 1)) return 0;
-  const size_t split = dtype == VERACE_F32 ? operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype) : 0;
-  const size_t part = partial_bytes(m, n, k, 1, 1, false, dtype, false);
-  return split + part ? split + part + 256 : 0;
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const bool dots = by_dots(m, n, k, dtype, 1);
+  if (dots && dtype == VERACE_F32) return 0;
+  const size_t copies = copy_bytes(m, k, dtype) + copy_bytes(n, k, dtype);
+  const size_t part = dots ? 0 : partial_bytes(m, n, k, 1, 1, false, dtype, false);
+  return copies + part ? copies + part + 256 : 0;
 }
 
 extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw,
@@ -356,13 +395,15 @@ extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale,
   p.e.row_scale = x_scale; p.e.col_scale = w_scale; p.e.bias = bias; p.e.residual = residual; p.e.ld_res = ld_res;
   p.e.pre = pre; p.e.act = act;
   p.e.bias_type = dtype == VERACE_E4M3 ? out_dtype : dtype;
-  if (by_dots(m, n, k, dtype, 1)) {
+  const bool dots = by_dots(m, n, k, dtype, 1);
+  if (dots && dtype == VERACE_F32) {
     p.a = Mat{x, m, k, ldx, 1, 0};
     p.b[0] = Mat{w, n, k, ldw, 1, 0};
-    return product_dot(p, st);
-  }
-  if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) || (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st))))
+  } else if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) ||
+                       (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st)))) {
     return rc;
+  }
+  if (dots) return product_dot(p, st);
   p.segments = p.a_step = 1;
   p.ws = ws.at;
   return run_product(p, st);
@@ -373,7 +414,7 @@ extern "C" size_t verace_linear_backward_workspace(long long m, int n, int k, in
   size_t s = operand_bytes(m, n, dtype) + align_up((size_t)chunks_of(m) * n * 4, 256) + 256;
   // (dx and dw follow each other: one place for the partial sums of either)
   s += std::max(partial_bytes(m, k, n, 1, 1, false, dtype, false), partial_bytes(n, k, m, 1, 1, false, dtype, true));
-  if (dtype == VERACE_F32 && k > 0) s += operand_bytes(m, k, dtype) + operand_bytes(n, k, dtype);
+  if (k > 0) s += copy_bytes(m, k, dtype) + copy_bytes(n, k, dtype);
   return s;
 }
 
@@ -446,10 +487,12 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
 }
 
 extern "C" size_t verace_gated_linear_workspace(long long m, int f, int k, int dtype) {
-  if (m <= 0 || f <= 0 || k <= 0 || by_dots(m, f, k, dtype, 2)) return 0;
-  const size_t split = dtype == VERACE_F32 ? operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype) : 0;
-  const size_t part = partial_bytes(m, f, k, 1, 1, true, dtype, false);
-  return split + part ? split + part + 256 : 0;
+  if (m <= 0 || f <= 0 || k <= 0) return 0;
+  const bool dots = by_dots(m, f, k, dtype, 2);
+  if (dots && dtype == VERACE_F32) return 0;
+  const size_t copies = copy_bytes(m, k, dtype) + 2 * copy_bytes(f, k, dtype);
+  const size_t part = dots ? 0 : partial_bytes(m, f, k, 1, 1, true, dtype, false);
+  return copies + part ? copies + part + 256 : 0;
 }
 
 extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_scale, const void* w_gate, const void* w_up,
@@ -478,16 +521,17 @@ extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_
   p.e.row_scale = x_scale; p.e.col_scale = gate_scale; p.e.up_scale = up_scale;
   p.e.pre = gate; p.e.pre_up = up; p.e.act = act;
   p.e.b1 = beta1; p.e.b2 = beta2; p.e.r1 = 1.f / beta1; p.e.r2 = 1.f / beta2;
-  if (by_dots(m, f, k, dtype, 2)) {
+  const bool dots = by_dots(m, f, k, dtype, 2);
+  if (dots && dtype == VERACE_F32) {
     p.a = Mat{x, m, k, ldx, 1, 0};
     p.b[0] = Mat{w_gate, f, k, ldw, 1, 0};
     p.b[1] = Mat{w_up, f, k, ldw, 1, 0};
-    return product_dot(p, st);
-  }
-  if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) ||
-                (rc = operand(&p.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
-                (rc = operand(&p.b[1], w_up, ldw, f, k, dtype, ws, st))))
+  } else if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) ||
+                       (rc = operand(&p.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
+                       (rc = operand(&p.b[1], w_up, ldw, f, k, dtype, ws, st)))) {
     return rc;
+  }
+  if (dots) return product_dot(p, st);
   p.segments = p.a_step = 1;
   p.ws = ws.at;
   return run_product(p, st);
@@ -499,7 +543,7 @@ extern "C" size_t verace_gated_linear_backward_workspace(long long m, int f, int
   // (dx and the weights' gradients follow each other: one place for the partial sums of either)
   s += std::max(partial_bytes(m, k, f, 2, 1, false, dtype, false),
                 std::max(partial_bytes(f, k, m, 1, 1, false, dtype, true), partial_bytes(f, k, m, 1, 2, false, dtype, true)));
-  if (dtype == VERACE_F32 && k > 0) s += operand_bytes(m, k, dtype) + 2 * operand_bytes(f, k, dtype);
+  if (k > 0) s += copy_bytes(m, k, dtype) + 2 * copy_bytes(f, k, dtype);
   return s;
 }
 

@@ -32,21 +32,20 @@ _ALIGN = {torch.float32: 1, torch.bfloat16: 8, torch.float16: 8, FP8: 16}   # va
 
 
 def _rows(t: torch.Tensor, m: int, k: int) -> Tuple[torch.Tensor, int]:
-    """t as [m, k] whose rows the kernels can address, and its row stride; copied where it has to be."""
+    """t as [m, k] whose rows the kernels can address, and its row stride; copied where it has to be.  (Rows
+    that are not whole 16-byte words may start anywhere.)"""
     a = _ALIGN[t.dtype]
-    if k % a == 0 and t.is_contiguous() and (a == 1 or t.data_ptr() % 16 == 0):
+    if t.is_contiguous() and (k % a or a == 1 or t.data_ptr() % 16 == 0):
         return t, k
     if t.dim() != 2:
         t = t.reshape(m, k)
-    ld = t.stride(0) if m > 1 else -(-k // a) * a
-    if (k > 1 and t.stride(1) != 1) or ld < k or ld % a or (a > 1 and t.data_ptr() % 16):
-        ld = -(-k // a) * a
-        c = torch.empty((m, ld), dtype=t.dtype, device=t.device)
+    ld = t.stride(0) if m > 1 else k
+    if (k > 1 and t.stride(1) != 1) or ld < k or (k % a == 0 and (ld % a or (a > 1 and t.data_ptr() % 16))):
         if a == 16:     # (copied as bytes)
-            c.view(torch.uint8)[:, :k].copy_(t.view(torch.uint8))
+            t = t.view(torch.uint8).clone(memory_format=torch.contiguous_format).view(FP8)
         else:
-            c[:, :k].copy_(t)
-        t = c
+            t = t.clone(memory_format=torch.contiguous_format)
+        ld = k
     return t, ld
 
 
@@ -208,12 +207,10 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
 def _gate_rows(w_gate, w_up, f, k):
     g2, ldg = _rows(w_gate, f, k)
     u2, ldu = _rows(w_up, f, k)
-    if ldg != ldu:      # (two row strides: one of them, or both, become dense)
-        a = _ALIGN[g2.dtype]
-        ld = -(-k // a) * a
-        if ldg != ld:
+    if ldg != ldu:      # (two row strides: the one that is not dense, or both, become so)
+        if ldg != k:
             g2, ldg = _rows(w_gate.contiguous(), f, k)
-        if ldu != ld:
+        if ldu != k:
             u2, ldu = _rows(w_up.contiguous(), f, k)
     return g2, u2, ldg
 
