@@ -17,8 +17,8 @@
 //
 // fp32 operands come as three bf16 parts, three stages for 64 values of K (a stage holds one part of A and of B), and
 // the MMAs take six pairs of them, the smallest first.  The tensor core cuts its sums to fp32 after every step instead
-// of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the result); so after every 128 values of K
-// (CHUNK) the epilogue's warps add the sums to a third set in TMEM, rounding, while the next 128 run into the other set.
+// of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the result); so after every 64 values of K
+// the epilogue's warps add the sums to a third set in TMEM, rounding, while the next 64 run into the other set.
 //
 // Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
 // applies scales, bias and activation, and the warp turns the rounded values over in shared memory so
@@ -38,8 +38,6 @@ using namespace lin;
 constexpr int NT = 384, EPI_WARPS = 8;
 constexpr uint32_t POLLS = 1u << 22;
 constexpr int TURN = 32 * 33 * 4;      // a warp's place to turn 32 rows of 32 words over
-
-constexpr int CHUNK = 2;
 
 template <int BN>
 struct Shape {
@@ -425,8 +423,9 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = *slot;
-  // a tile's stages of K: in one lot, of parts `chunk` by `chunk` (PARTS: as many for every split, the last one's may be empty)
-  const int chunk = PARTS ? CHUNK : p.per, chunks = PARTS ? (p.per + CHUNK - 1) / CHUNK : 1;
+  // sets of sums that make up a tile: one; of parts one for 64 values of K of a segment (as many for every split of K,
+  // the last one's may be empty)
+  const int sets = PARTS ? p.per * p.segments : 1;
 
   if (warp == 0) {
     if (lane == 0) {   // ---- operands
@@ -437,13 +436,14 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
         const Place at = place(p, t);
         const int m0 = at.m * 256 + (int)rank * 128;
         const int n0 = GATED ? at.n * HB : at.n * BN + (int)rank * HB;
-        for (int u = 0; u < p.segments * chunks && ok; ++u) {   // (chunk by chunk, in each all segments)
-          const int s = PARTS ? u % p.segments : u, k0 = PARTS ? u / p.segments * chunk : 0;
-          const CUtensorMap* mb = &maps.b[GATED ? rank : s];
-          const int end = min(min(k0 + chunk, p.per) + at.split * p.per, p.kblocks);
-          constexpr int EACH = PARTS ? 3 : 1;
-          for (int q = (k0 + at.split * p.per) * EACH; q < end * EACH; ++q) {
-            const int kb = q / EACH, part = q % EACH, az = part * p.a_step + p.a_first + s + at.z;
+        const int k0 = at.split * p.per, k1 = min(k0 + p.per, p.kblocks);
+        // (segment by segment; of parts 64 values of K of every segment, then the next)
+        const int outer = PARTS ? k1 - k0 : p.segments, inner = PARTS ? 3 * p.segments : k1 - k0;
+        for (int u = 0; u < outer && ok; ++u) {
+          for (int v = 0; v < inner; ++v) {
+            const int s = PARTS ? v / 3 : u, kb = k0 + (PARTS ? u : v), part = PARTS ? v % 3 : 0;
+            const CUtensorMap* mb = &maps.b[GATED ? rank : s];
+            const int az = part * p.a_step + p.a_first + s + at.z;
             if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
               ok = false;
               break;
@@ -488,7 +488,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       int i = 0, n = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const int mine = (p.tiles - pair + pairs - 1) / pairs * chunks;   // sets of sums to fill
+      const int mine = (p.tiles - pair + pairs - 1) / pairs * sets;   // sets to fill
       // four MMAs: 128 bytes of K of stage ia's A and stage ib's B
       auto step = [&](uint32_t d, int ia, int ib, bool more) {
         const uint32_t a = tc::smem_addr(sm + ia * S::STAGE), bb = tc::smem_addr(sm + ib * S::STAGE) + 16384;
@@ -502,8 +502,8 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       };
       for (; n < mine && ok; ++n) {
         const int b = n & 1, use = n >> 1;
-        const int base = place(p, pair + n / chunks * pairs).split * p.per + n % chunks * chunk;
-        const int steps = p.segments * (min(min(base + chunk, base - n % chunks * chunk + p.per), p.kblocks) - base);
+        const int k0 = place(p, pair + n / sets * pairs).split * p.per;
+        const int steps = PARTS ? k0 + n % sets / p.segments < p.kblocks : p.segments * (min(k0 + p.per, p.kblocks) - k0);
         if (!tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
           ok = false;
           break;
@@ -533,7 +533,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
             if (!ok) break;
             tc::fence_after_sync();
             if (lead) {   // parts: 0 the high one
-              step(d, at[2], at[0], s > 0);
+              step(d, at[2], at[0], false);
               step(d, at[1], at[1], true);
               step(d, at[0], at[2], true);
               commit_pair(&empty[at[2]]);
@@ -575,30 +575,37 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
     auto wait = [&](int n) {
       if constexpr (!PARTS) return filled(n) ? (n & 1) * BN : -1;
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-      const int base = place(p, pair + n * pairs).split * p.per;
-      for (int c = 0; c < chunks; ++c) {
-        const int set = n * chunks + c;
+      const int k0 = place(p, pair + n * pairs).split * p.per;
+      for (int c = 0; c < sets; ++c) {
+        const int set = n * sets + c;
         if (!filled(set)) return -1;
-        if (base + c * CHUNK >= p.kblocks) {   // (a last split's missing stages)
-          free(set);
-          continue;
-        }
-        for (int h = 0; h < BN / 2; h += 16) {   // the warp's half of the columns (gated: of both sums)
-          const int col = GATED ? (h >= HB / 2 ? HB / 2 + h : h) + (warp >= 8 ? HB / 2 : 0) : h + (warp >= 8 ? HB : 0);
-          uint32_t r[16], s[16];
-          tmem_ld_async(lanes + (set & 1) * BN + col, r);
-          if (c > 0) {
-            tmem_ld_async(lanes + 2 * BN + col, s);
+        if (k0 + c / p.segments < p.kblocks) {
+#pragma unroll 1
+          for (int h = 0; h < BN / 2; h += 32) {   // the warp's half of the columns (gated: of both sums)
+            const int col = GATED ? (h >= HB / 2 ? HB / 2 + h : h) + (warp >= 8 ? HB / 2 : 0) : h + (warp >= 8 ? HB : 0);
+            uint32_t r[16], s[16], r1[16], s1[16];
+            tmem_ld_async(lanes + (set & 1) * BN + col, r);
+            tmem_ld_async(lanes + (set & 1) * BN + col + 16, r1);
+            if (c > 0) {
+              tmem_ld_async(lanes + 2 * BN + col, s);
+              tmem_ld_async(lanes + 2 * BN + col + 16, s1);
+              tmem_wait(s);
+              tmem_wait(s1);
+            }
             tmem_wait(r);
-            tmem_wait(s);
+            tmem_wait(r1);
+            if (c > 0) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(s[j]));
-          } else {
-            tmem_wait(r);
+              for (int j = 0; j < 16; ++j) {
+                r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(s[j]));
+                r1[j] = __float_as_uint(__uint_as_float(r1[j]) + __uint_as_float(s1[j]));
+              }
+            }
+            tmem_st(lanes + 2 * BN + col, r);
+            tmem_st(lanes + 2 * BN + col + 16, r1);
           }
-          tmem_st(lanes + 2 * BN + col, r);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         free(set);
       }
       return 2 * BN;

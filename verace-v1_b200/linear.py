@@ -12,6 +12,7 @@ addition (verace_v1/modules/mcmoe.py:85-120, backbone.py:96-99).
 
 fp32, bf16 and fp16 operands have gradients; e4m3 operands (with scales) are for inference.
 """
+import contextlib
 import math
 from typing import Optional, Tuple
 
@@ -88,6 +89,14 @@ def _workspace(nbytes: int, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+_NOTHING = contextlib.nullcontext()
+
+
+def _on(dev):
+    """The device as the current one (a context; nothing to do where it is)."""
+    return _NOTHING if dev.index == current() else torch.cuda.device(dev)
+
+
 def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -133,9 +142,9 @@ class _FusedLinear(torch.autograd.Function):
         if want[0] or want[1] or want[2]:
             d2 = d.contiguous()
             L = lib()
-            with torch.cuda.device(dev):
-                nws = L.verace_linear_backward_workspace(m, n, k, _DTYPE[dt])
-                ws = _workspace(nws, dev)
+            nws = L.verace_linear_backward_workspace(m, n, k, _DTYPE[dt])
+            ws = _workspace(nws, dev)
+            with _on(dev):
                 check(L.verace_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(pre), _p(dx),
                                                _p(dw), _p(db), m, n, k, act, _DTYPE[dt], _DTYPE[out_dtype], _p(ws), nws,
                                                raw_stream(dev.index)), "verace_linear_backward")
@@ -253,9 +262,9 @@ class _GatedLinear(torch.autograd.Function):
         du = torch.empty((f, k), dtype=dt, device=dev) if want[2] else None
         d2 = d.contiguous()
         L = lib()
-        with torch.cuda.device(dev):
-            nws = L.verace_gated_linear_backward_workspace(m, f, k, _DTYPE[dt])
-            ws = _workspace(nws, dev)
+        nws = L.verace_gated_linear_backward_workspace(m, f, k, _DTYPE[dt])
+        ws = _workspace(nws, dev)
+        with _on(dev):
             check(L.verace_gated_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, g2.data_ptr(), u2.data_ptr(), ldw,
                                                  gate.data_ptr(), up.data_ptr(), _p(dx), _p(dg), _p(du), m, f, k, act, b1,
                                                  b2, _DTYPE[dt], _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index)),
