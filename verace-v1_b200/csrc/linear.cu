@@ -67,6 +67,7 @@ __device__ __forceinline__ void store_operand(Part<T>* o, long long piece, const
 // src [rows, cols] fp32 -> three parts [3][rows][ld], ld = cols rounded up to 8
 __global__ void __launch_bounds__(256) split_rows(const float* __restrict__ src, long long ld_src, long long rows,
                                                   long long cols, bool vec, __nv_bfloat16* __restrict__ dst, long long ld) {
+  depend();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long row = i / (ld / 8), c = i % (ld / 8) * 8;
   if (row >= rows) return;
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(256) split_rows(const float* __restrict__ src,
 // them; 16 bytes a thread, read as the aligned words around them.
 __global__ void __launch_bounds__(256) align_rows(const char* __restrict__ src, long long ld_src, long long rows, long long bytes,
                                                   char* __restrict__ dst, long long ld) {
+  depend();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long row = i / (ld / 16), c = i % (ld / 16) * 16;
   if (row >= rows) return;
@@ -136,8 +138,8 @@ int operand(Mat* out, const void* p, long long ld, long long rows, long long col
     out->p = ws.take(rows * out->ld * es);
     const long long blocks = (rows * (out->ld * es / 16) + 255) / 256;
     VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld operand is too large", rows, cols);
-    align_rows<<<(unsigned)blocks, 256, 0, st>>>((const char*)p, ld * es, rows, cols * es, (char*)out->p, out->ld * es);
-    return check_launch("align_rows");
+    return launch_after("align_rows", align_rows, dim3((unsigned)blocks), 256, 0, st, 1, (const char*)p, ld * es, rows, cols * es,
+                        (char*)out->p, out->ld * es);
   }
   void* dst = ws.take(operand_bytes(rows, cols, type));
   *out = operand_at(dst, rows, cols, type);
@@ -145,13 +147,13 @@ int operand(Mat* out, const void* p, long long ld, long long rows, long long col
   VERACE_REQUIRE((threads + 255) / 256 < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld operand is too large", rows,
                  cols);
   const bool vec = cols % 8 == 0 && ld % 4 == 0 && (size_t)p % 16 == 0;
-  split_rows<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>((const float*)p, ld, rows, cols, vec, (__nv_bfloat16*)dst,
-                                                              out->ld);
-  return check_launch("split_rows");
+  return launch_after("split_rows", split_rows, dim3((unsigned)((threads + 255) / 256)), 256, 0, st, 1, (const float*)p, ld, rows,
+                      cols, vec, (__nv_bfloat16*)dst, out->ld);
 }
 
 // ------------------------------------------------------------------ sums over nothing (k = 0)
 __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long long n) {
+  depend();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= m * n) return;
   const long long r = i / n, c = i % n;
@@ -164,7 +166,10 @@ __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long l
 }
 
 
-constexpr long long FEW = 256;
+// Tokens up to which weights are streamed past them (linear_few.cu).  bf16: 48 x 4096 x 8192 17.6 us against 19.8 for
+// tiles of 256 rows, 96 x 8192 x 4096 21.0 against 25.4, 128 x 4096 x 32000 50.0 against 56.7; 128 x 1024 x 4096 9.2 against 8.8,
+// 176 x 4096 x 8192 23.4 against 20.2, 256 x 4096 x 32000 76.9 against 59.8.
+constexpr long long FEW = 112;
 
 // Whether a forward product goes to the engine of dot products.  In fp32 that saves splitting the weights
 // (8 x 4096 x 4096: 23 us against 59; 16 tokens 38 against 59, 32 tokens 68 against 61).  In 16 and 8 bits the tensor cores
@@ -194,8 +199,7 @@ int run_product(Product& p, cudaStream_t st) {
       if (p.nz > 1) e.out = p.out_z[z];
       const long long blocks = (p.M * p.N + 255) / 256;
       VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
-      empty_sum<<<(unsigned)blocks, 256, 0, st>>>(e, p.M, p.N);
-      if (int rc = check_launch("empty_sum")) return rc;
+      if (int rc = launch_after("empty_sum", empty_sum, dim3((unsigned)blocks), 256, 0, st, 1, e, p.M, p.N)) return rc;
     }
     return VERACE_OK;
   }
@@ -223,6 +227,7 @@ struct SlopeArgs {
 
 template <typename T, typename O>
 __global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
+  depend();
   __shared__ float part[8][256];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const long long chunk = blockIdx.x / a.colblocks, c = (blockIdx.x % a.colblocks) * 256LL + lane * 8;
@@ -263,6 +268,7 @@ __global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(256) sum_chunks(const float* __restrict__ partial, long long chunks, long long n,
                                                   T* __restrict__ out) {
+  depend();
   __shared__ float part[8][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const long long c = (long long)blockIdx.x * 32 + lane;
@@ -280,6 +286,7 @@ __global__ void __launch_bounds__(256) sum_chunks(const float* __restrict__ part
 
 template <typename T, typename O>
 __global__ void __launch_bounds__(256) gated_slope(SlopeArgs a) {
+  depend();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const long long chunk = blockIdx.x / a.colblocks, c = (blockIdx.x % a.colblocks) * 256LL + lane * 8;
   const long long end = min(a.m, (chunk + 1) * GATED_CHUNK);
@@ -454,13 +461,13 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
       if (s.out || s.partial) {
         unsigned grid;
         if ((rc = slope_grid(s, CHUNK, &grid))) return rc;
-        linear_slope<T, O><<<grid, 256, 0, st>>>(s);
-        if ((rc = check_launch("linear_slope"))) return rc;
+        if ((rc = launch_after("linear_slope", linear_slope<T, O>, dim3(grid), 256, 0, st, 1, s))) return rc;
       }
     }
     if (dbias && n > 0) {
-      sum_chunks<T><<<(n + 31) / 32, 256, 0, st>>>(s.partial, any ? chunks_of(m) : 0, n, (T*)dbias);
-      if ((rc = check_launch("sum_chunks"))) return rc;
+      if ((rc = launch_after("sum_chunks", sum_chunks<T>, dim3((n + 31) / 32), 256, 0, st, 1, (const float*)s.partial,
+                             any ? chunks_of(m) : 0LL, (long long)n, (T*)dbias)))
+        return rc;
     }
     if (dx && k > 0) {
       Product d{};
@@ -585,8 +592,7 @@ extern "C" int verace_gated_linear_backward(const void* dout, const void* x, lon
       s.b1 = beta1; s.b2 = beta2; s.r1 = 1.f / beta1; s.r2 = 1.f / beta2;
       unsigned grid;
       if ((rc = slope_grid(s, GATED_CHUNK, &grid))) return rc;
-      gated_slope<T, O><<<grid, 256, 0, st>>>(s);
-      if ((rc = check_launch("gated_slope"))) return rc;
+      if ((rc = launch_after("gated_slope", gated_slope<T, O>, dim3(grid), 256, 0, st, 1, s))) return rc;
     }
     if (dx) {
       Product d{};

@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(32 * WARPS) dot_product(const __grid_constant_
   const long long group = (long long)blockIdx.y * (WARPS / p.share) + warp / p.share;
   const long long m0 = (long long)blockIdx.x * MT, n0 = group * RG;
   float acc[H][MT][RG] = {};
+  depend();
   if (group < p.groups) {
     const T* x[MT];
     const T* w[H][RG];
@@ -186,8 +187,8 @@ int launch(const Product& p, cudaStream_t st) {
   const long long blocks = (a.groups * a.share + WARPS - 1) / WARPS;
   VERACE_REQUIRE(tokens < 1LL << 31 && blocks <= 65535, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M,
                  p.N);
-  dot_product<T, MT, RG, GATED, VEC><<<dim3((unsigned)tokens, (unsigned)blocks), 32 * WARPS, 0, st>>>(a);
-  return check_launch("dot_product");
+  return launch_after("dot_product", dot_product<T, MT, RG, GATED, VEC>, dim3((unsigned)tokens, (unsigned)blocks), 32 * WARPS, 0,
+                      st, 1, a);
 }
 
 template <typename T, int MT, int RG, bool VEC = true>

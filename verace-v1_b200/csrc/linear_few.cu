@@ -1,6 +1,6 @@
 // Products of few rows (tokens) on the tensor cores, the other engine behind linear.cu:
-//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 256
-// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 256 columns, so
+//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 128
+// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 128 columns, so
 // a weight crosses shared memory once and no row of the MMA is idle; a CTA streams its 128 rows (gated:
 // 128 of each weight, two sums side by side in TMEM) by TMA in stages of 128 bytes of K.  Two
 // CTAs share an SM where shared memory allows, so that one's set-up and epilogue run under the other's
@@ -25,7 +25,7 @@ namespace {
 namespace cg = cooperative_groups;
 using namespace lin;
 
-constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8, MAX_TOKENS = 256;
+constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8;
 // shared memory for stages of a CTA that has an SM to itself, and of one that shares it (228 KB an SM,
 // less 1 KB a CTA that the system takes, 1 KB of barriers and 1 KB to align the stages)
 constexpr int ROOM = 225 * 1024, HALF_ROOM = 111 * 1024;
@@ -37,7 +37,7 @@ struct Maps {
 
 struct Args {
   long long M, N;       // tokens, outputs
-  int mp;               // tokens of a tile, rounded up to 16
+  int mp;               // tokens, rounded up to 16
   int stages, stage;    // and a stage's bytes
   int kblocks, steps, per, ck, tiles_n;
   int cols;             // of TMEM
@@ -103,10 +103,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   __shared__ uint32_t slot;
   __shared__ volatile int fail;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int unit = blockIdx.x / p.ck, rank = blockIdx.x - unit * p.ck;
-  const int tile_m = unit / p.tiles_n, tile_n = unit - tile_m * p.tiles_n;
-  const int n0 = tile_n * ROWS;
-  const long long m0 = (long long)tile_m * p.mp;
+  const int tile_n = blockIdx.x / p.ck, rank = blockIdx.x - tile_n * p.ck, n0 = tile_n * ROWS;
   const int first = rank * p.per, last = min(p.steps, first + p.per);
   if (warp == 1) tc::tmem_alloc(&slot, p.cols);
   if (warp == 2 && lane < 3)
@@ -123,6 +120,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  depend();
   const uint32_t tmem = slot;
 
   if (warp == 0) {
@@ -144,7 +142,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
           tc::tma_load_3d(w, &maps.w[0], kb * KB, n0, 0, &full[i]);
           if (GATED) tc::tma_load_3d(w + ROWS * 128, &maps.w[1], kb * KB, n0, 0, &full[i]);
         }
-        tc::tma_load_3d(w + WB, &maps.x, kb * KB, (int)m0, p.a_first + seg, &full[i]);
+        tc::tma_load_3d(w + WB, &maps.x, kb * KB, 0, p.a_first + seg, &full[i]);
         if (++kb == p.kblocks) kb = 0, ++seg;
         if (++i == p.stages) i = 0, phase ^= 1;
         flying = min(flying + 1, p.stages);
@@ -185,7 +183,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   }
   __syncwarp();
   // ---- the sums
-  const int tokens = (int)min((long long)p.mp, p.M - m0);
+  const int tokens = (int)p.M;
   const int quarter = warp & 3;
   const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
   const int n = n0 + 32 * quarter + lane;
@@ -205,13 +203,13 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
         if (GATED) tmem_ld_async(mine + p.mp + t, s);
         const int rows = in ? min(16, tokens - t) : 0;
         float res[16] = {};
-        if (!GATED && e.residual) load_rows16(e.residual, (m0 + t) * e.ld_res + n, e.ld_res, rows, e.type, res);
+        if (!GATED && e.residual) load_rows16(e.residual, (long long)t * e.ld_res + n, e.ld_res, rows, e.type, res);
         tmem_wait(r);
         if (GATED) tmem_wait(s);
         float g[16], u[16] = {};
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float rs = e.row_scale && t + j < tokens ? e.row_scale[m0 + t + j] : 1.f;
+          const float rs = e.row_scale && t + j < tokens ? e.row_scale[t + j] : 1.f;
           g[j] = __uint_as_float(r[j]);
           if (e.col_scale) g[j] *= rs * cs;
           g[j] += bias;
@@ -221,14 +219,14 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
           }
         }
         if (e.pre) {
-          store_rows16(e.pre, (m0 + t) * e.ld + n, e.ld, rows, VERACE_F32, g);
-          if (GATED) store_rows16(e.pre_up, (m0 + t) * e.ld + n, e.ld, rows, VERACE_F32, u);
+          store_rows16(e.pre, (long long)t * e.ld + n, e.ld, rows, VERACE_F32, g);
+          if (GATED) store_rows16(e.pre_up, (long long)t * e.ld + n, e.ld, rows, VERACE_F32, u);
         }
         if (e.type == VERACE_F32) activate<GATED, false>(e, g, u);
         else activate<GATED, true>(e, g, u);
 #pragma unroll
         for (int j = 0; j < 16; ++j) g[j] += res[j];
-        store_rows16(e.out, (m0 + t) * e.ld + n, e.ld, rows, e.type, g);
+        store_rows16(e.out, (long long)t * e.ld + n, e.ld, rows, e.type, g);
       }
     }
   } else {
@@ -262,7 +260,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
           }
         }
         const long long c = n0 + i % (ROWS / 4) * 4;
-        if (c < p.N) finish4<GATED>(p.e, m0 + t0 + i / (ROWS / 4), c, p.N, g, u);
+        if (c < p.N) finish4<GATED>(p.e, t0 + i / (ROWS / 4), c, p.N, g, u);
       }
       cl.sync();
     }
@@ -279,9 +277,8 @@ int launch(const Product& p, cudaStream_t st) {
   Args a{};
   int rc;
   a.M = p.M; a.N = p.N;
-  const int tiles_m = (int)((p.M + MAX_TOKENS - 1) / MAX_TOKENS);
-  a.mp = (int)(((p.M + tiles_m - 1) / tiles_m + 15) / 16 * 16);
-  // A (x) in boxes of the tile's tokens, B (the weights) as the MMA's rows
+  a.mp = (int)((p.M + 15) / 16 * 16);
+  // A (x) in one box of all tokens, B (the weights) as the MMA's rows
   if ((rc = operand_map(&maps.x, p.a, p.type, a.mp))) return rc;
   for (int i = 0; i < 2; ++i)
     if ((rc = operand_map(&maps.w[i], p.b[p.b[i].p ? i : 0], p.type, WMN ? 64 : ROWS))) return rc;
@@ -289,10 +286,8 @@ int launch(const Product& p, cudaStream_t st) {
   a.a_first = p.a_first;
   a.steps = a.kblocks * p.segments;
   a.tiles_n = (int)((p.N + ROWS - 1) / ROWS);
-  const long long units = (long long)a.tiles_n * tiles_m;
-  VERACE_REQUIRE(units < 1LL << 27, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
   a.ck = 1;
-  while (a.ck < 8 && units * a.ck * 2 <= 148 && a.steps >= a.ck * 4) a.ck *= 2;
+  while (a.ck < 8 && a.tiles_n * a.ck * 2 <= 148 && a.steps >= a.ck * 4) a.ck *= 2;
   a.per = (a.steps + a.ck - 1) / a.ck;
   a.stage = ROWS * 128 * (GATED ? 2 : 1) + a.mp * 128;
   // two CTAs an SM, unless that leaves a CTA fewer than three stages
@@ -322,19 +317,7 @@ int launch(const Product& p, cudaStream_t st) {
     VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ROOM + 1024));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * a.ck));
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.ck;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.ck > 1 ? 1 : 0;
-  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kern, maps, a));
-  return check_launch("few_product");
+  return launch_after("few_product", kern, dim3(a.tiles_n * a.ck), NT, smem, st, a.ck, maps, a);
 }
 
 }  // namespace

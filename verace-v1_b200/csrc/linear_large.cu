@@ -382,7 +382,7 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t turn, uin
 }
 
 template <bool F8, bool AMN, bool BMN, bool GATED, int BN, bool PARTS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
+__global__ void __launch_bounds__(NT, 1)
 large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
   using S = Shape<BN>;
   constexpr int KB = F8 ? 128 : 64;            // values of K in a stage
@@ -422,6 +422,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   __syncthreads();
   cluster_sync();
   tc::fence_after_sync();
+  depend();
   const uint32_t tmem = *slot;
   // sets of sums that make up a tile: one; of parts one for 64 values of K of a segment (as many for every split of K,
   // the last one's may be empty)
@@ -672,8 +673,7 @@ int launch(const Product& p, int splits, cudaStream_t st) {
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   const int pairs = tiles < 74 ? (int)tiles : 74;
-  kern<<<2 * pairs, NT, S::SMEM, st>>>(maps, a);
-  return check_launch("large_product");
+  return launch_after("large_product", kern, dim3(2 * pairs), NT, S::SMEM, st, 2, maps, a);
 }
 
 template <int BN>
@@ -695,6 +695,7 @@ int by_kind(const Product& p, int s, cudaStream_t st) {
 template <bool GATED>
 __global__ void __launch_bounds__(256) join_splits(const float* __restrict__ part, int splits, long long partial, long long up,
                                                    Epilogue e, long long M, long long N, long long quads) {
+  depend();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long m = i / quads, c = i % quads * 4;
   if (m >= M) return;
@@ -776,11 +777,11 @@ int product_large(const Product& p, cudaStream_t st) {
     Epilogue e = p.e;
     if (p.nz > 1) e.out = p.out_z[z];
     const float* part = static_cast<const float*>(p.ws) + z * one;
-    if (p.gated)
-      join_splits<true><<<(unsigned)blocks, 256, 0, st>>>(part, c.splits, one, c.splits * one, e, p.M, p.N, quads);
-    else
-      join_splits<false><<<(unsigned)blocks, 256, 0, st>>>(part, c.splits, p.nz * one, 0, e, p.M, p.N, quads);
-    if ((rc = check_launch("join_splits"))) return rc;
+    rc = p.gated ? launch_after("join_splits", join_splits<true>, dim3((unsigned)blocks), 256, 0, st, 1, part, c.splits, one,
+                                c.splits * one, e, (long long)p.M, (long long)p.N, quads)
+                 : launch_after("join_splits", join_splits<false>, dim3((unsigned)blocks), 256, 0, st, 1, part, c.splits,
+                                p.nz * one, 0LL, e, (long long)p.M, (long long)p.N, quads);
+    if (rc) return rc;
   }
   return VERACE_OK;
 }

@@ -39,6 +39,33 @@ int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
 int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to 256 rows of A
 int product_dot(const Product& p, cudaStream_t st);     // linear_dot.cu: a few rows of A, fp32 operands as they are
 
+// ------------------------------------------------------------------ launches
+// Every kernel here is launched as a programmatic dependent of the one before it on the stream: it may be
+// resident, and set itself up, while that one ends, waits for it (depend()) before its first access to global
+// memory, and only then lets its own dependents in, so that whatever came before is complete for
+// them too (chains of small products: 1.5 to 2 us a launch).
+template <typename K, typename... A>
+int launch_after(const char* what, K kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  VERACE_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return check_launch(what);
+}
+__device__ __forceinline__ void depend() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // The tensor map of an operand: boxes of 128 bytes x `rows`.
 int operand_map(CUtensorMap* map, const Mat& m, int type, int rows);
 

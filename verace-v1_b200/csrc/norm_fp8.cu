@@ -13,7 +13,7 @@
 // Rows whose width is no multiple of 8 start anywhere in a 16-byte word: their words are those of the whole
 // tensor, the first and last one masked, so that all but the norm's weights is read and written a word
 // at a time all the same (1111 x 5001 fp32: 14.7 us, value by value 19.9).
-#include "common.cuh"
+#include "linear_tc.cuh"
 
 #include <cuda_fp8.h>
 
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
   __shared__ float part[2][W > 1 ? W : 1];
   const int g = threadIdx.x % G;
   const long long row = (long long)blockIdx.x * (NT / G) + threadIdx.x / G;
+  lin::depend();
   if (G < 128 && row >= a.rows) return;   // (whole warps; larger groups are one row a CTA)
   const long long off = row * a.cols;
   const T* h = static_cast<const T*>(a.h) + off;
@@ -222,12 +223,14 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
 template <typename T, bool WHOLE, bool ADD>
 int launch(const NormArgs& a, cudaStream_t st) {
   const int cols = a.cols + (WHOLE ? 0 : 7);   // (a row may start in the middle of a word)
-  if (cols <= 1024) norm_fp8_kernel<T, 32, WHOLE, ADD><<<(unsigned)((a.rows + 3) / 4), 128, 0, st>>>(a);
-  else if (cols <= 4096) norm_fp8_kernel<T, 128, WHOLE, ADD><<<(unsigned)a.rows, 128, 0, st>>>(a);
-  else if (cols <= 8192) norm_fp8_kernel<T, 256, WHOLE, ADD><<<(unsigned)a.rows, 256, 0, st>>>(a);
-  else if (cols <= 16384) norm_fp8_kernel<T, 512, WHOLE, ADD><<<(unsigned)a.rows, 512, 0, st>>>(a);
-  else norm_fp8_kernel<T, 1024, WHOLE, ADD><<<(unsigned)a.rows, 1024, 0, st>>>(a);
-  return check_launch("norm_fp8_kernel");
+  auto go = [&](auto kernel, long long blocks, int threads) {
+    return lin::launch_after("norm_fp8_kernel", kernel, dim3((unsigned)blocks), threads, 0, st, 1, a);
+  };
+  if (cols <= 1024) return go(norm_fp8_kernel<T, 32, WHOLE, ADD>, (a.rows + 3) / 4, 128);
+  if (cols <= 4096) return go(norm_fp8_kernel<T, 128, WHOLE, ADD>, a.rows, 128);
+  if (cols <= 8192) return go(norm_fp8_kernel<T, 256, WHOLE, ADD>, a.rows, 256);
+  if (cols <= 16384) return go(norm_fp8_kernel<T, 512, WHOLE, ADD>, a.rows, 512);
+  return go(norm_fp8_kernel<T, 1024, WHOLE, ADD>, a.rows, 1024);
 }
 
 template <typename T>
