@@ -21,8 +21,9 @@
 // the epilogue's warps add the sums to a third set in TMEM, rounding, while the next 64 run into the other set.
 //
 // Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
-// applies scales, bias and activation, and the warp turns the rounded values over in shared memory so
-// that a store is 128 neighbouring bytes; residuals come in the same way.
+// applies scales, bias and activation and puts the rounded values into the warp's block of shared memory, from where
+// TMA stores them; rows that are not 16-byte aligned are stored word by word, the warp along a row.  Residuals come
+// into the block that way too, fetched while the products run.
 #include "linear_tc.cuh"
 
 #include <atomic>
@@ -37,7 +38,7 @@ using namespace lin;
 
 constexpr int NT = 384, EPI_WARPS = 8;
 constexpr uint32_t POLLS = 1u << 22;
-constexpr int TURN = 32 * 33 * 4;      // a warp's place to turn 32 rows of 32 words over
+constexpr int TURN = 4096;             // a warp's block of the output: 32 rows of 128 bytes
 
 template <int BN>
 struct Shape {
@@ -47,13 +48,14 @@ struct Shape {
 };
 
 struct Maps {
-  CUtensorMap a, b[2];
+  CUtensorMap a, b[2], out[2], pre[2];
 };
 
 struct Args {
   long long M, N;
   int kblocks, segments, a_first, a_step;
   int nz, tiles_m, tiles_n, tiles;
+  int by_tma, pre_by_tma;   // whether the rows of the outputs and of the saved sums are 16-byte aligned
   int splits, per;      // of K: `per` stages (of every segment) each; the sums of split i go to the i-th partial outputs
   long long partial;    // values from one split's outputs to the next
   uint32_t idesc;
@@ -124,21 +126,49 @@ __device__ __forceinline__ Place place(const Args& p, int t) {
 }
 
 // ------------------------------------------------------------------ the epilogue
-// A warp's block: 32 rows of 32 words, the word `lane` of row r at turn[33 r + lane]: 32 columns of fp32, or
-// 64 of 16-bit types, two to a word.
+// A warp's block: 32 rows of 128 bytes (32 columns of fp32, or 64 of 16-bit types) in shared memory, the 16-byte
+// pieces of a row exchanged as TMA's 128-byte swizzle has them, which also keeps both a thread's walk along its own
+// row and the warp's walk along one row free of bank conflicts.
 struct Block {
   uint32_t turn;            // its address in shared memory
   long long m0, n0, M, N;   // first row and column; ends
 };
+// Where a block goes: by TMA through a map, or to rows in memory `ld` values apart.
+struct Target {
+  const CUtensorMap* map;
+  int z;
+  void* p;
+  long long ld;
+};
 
+__device__ __forceinline__ uint32_t piece_at(const Block& b, int row, int piece) {   // the address of 16 bytes of a row
+  return b.turn + row * 128 + ((piece ^ (row & 7)) << 4);
+}
 // (by their address: through pointers these would be generic accesses)
-__device__ __forceinline__ uint32_t word(const Block& b, int i) {
+__device__ __forceinline__ uint32_t word(const Block& b, int row, int i) {
   uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(b.turn + 4 * i) : "memory");
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(piece_at(b, row, i >> 2) + 4 * (i & 3)) : "memory");
   return v;
 }
-__device__ __forceinline__ void set_word(const Block& b, int i, uint32_t v) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(b.turn + 4 * i), "r"(v) : "memory");
+__device__ __forceinline__ void set_word(const Block& b, int row, int i, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(piece_at(b, row, i >> 2) + 4 * (i & 3)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint4 get_piece(const Block& b, int row, int piece) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(piece_at(b, row, piece))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void set_piece(const Block& b, int row, int piece, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(b, row, piece)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+// the block's last copy to memory has left it
+__device__ __forceinline__ void reclaim(int lane) {
+  if (lane == 0) tc::bulk_wait_read<0>();
+  __syncwarp();
 }
 
 // Where a warp reads or writes a block: row by row, a word (or its two halves) a lane.
@@ -160,36 +190,47 @@ __device__ __forceinline__ Rows rows_of(const Block& b, const void* p, long long
   else r.part = n >= b.N ? 0 : n + 1 == b.N ? 1 : ((r.step | (size_t)r.at) & 3) == 0 ? 3 : 2;
   return r;
 }
-// the block to p
+// the block to memory
 template <bool WIDE>
-__device__ __forceinline__ void write_block(const Block& b, void* p, long long ld, int lane) {
+__device__ __forceinline__ void write_block(const Block& b, const Target& to, int lane) {
+  if (to.map) {
+    tc::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(to.map),
+                   "r"((int)b.n0), "r"((int)b.m0), "r"(to.z), "r"(b.turn)
+                   : "memory");
+      tc::bulk_commit();
+    }
+    return;
+  }
   __syncwarp();
-  Rows r = rows_of<WIDE>(b, p, ld, lane);
+  Rows r = rows_of<WIDE>(b, to.p, to.ld, lane);
   if (r.part == 3 && r.rows == 32) {
 #pragma unroll
     for (int h = 0; h < 32; h += 16) {
       uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = word(b, 33 * (h + i) + lane);
+      for (int i = 0; i < 16; ++i) w[i] = word(b, h + i, lane);
 #pragma unroll
       for (int i = 0; i < 16; ++i, r.at += r.step) *reinterpret_cast<uint32_t*>(r.at) = w[i];
     }
   } else if (r.part == 3) {
-    for (int i = 0; i < r.rows; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = word(b, 33 * i + lane);
+    for (int i = 0; i < r.rows; ++i) *reinterpret_cast<uint32_t*>(r.at + i * r.step) = word(b, i, lane);
   } else if (!WIDE && r.part) {
     // rows off 4-byte borders (an odd row stride), or a last word cut in two: where the row's words lie between two
     // words of the block, a lane stores the column before its own and its first
     const int left = (int)min(64LL, b.N - b.n0) - 2 * lane;   // columns from the lane's on
 #pragma unroll 8
     for (int i = 0; i < r.rows; ++i) {
-      const uint32_t w = word(b, 33 * i + lane);
+      const uint32_t w = word(b, i, lane);
       unsigned short* o = reinterpret_cast<unsigned short*>(r.at + i * r.step);
       if (((size_t)o & 3) == 0) {
         if (left > 1) *reinterpret_cast<uint32_t*>(o) = w;
         else o[0] = (unsigned short)w;
       } else {
         if (lane == 0) o[0] = (unsigned short)w;
-        else *reinterpret_cast<uint32_t*>(o - 1) = word(b, 33 * i + lane - 1) >> 16 | w << 16;
+        else *reinterpret_cast<uint32_t*>(o - 1) = word(b, i, lane - 1) >> 16 | w << 16;
         if (left > 1 && (lane == 31 || left == 2)) o[1] = (unsigned short)(w >> 16);
       }
     }
@@ -216,30 +257,39 @@ __device__ __forceinline__ void read_words(const Block& b, const void* p, long l
 // U values into the thread's own row of the block, from column c on
 template <bool WIDE, int U>
 __device__ __forceinline__ void put(const Block& b, int c, const float (&v)[U], int type, int lane) {
-  const int t = 33 * lane;
   if constexpr (WIDE) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) set_word(b, t + c + j, __float_as_uint(v[j]));
-  } else if (type == VERACE_BF16) {
-#pragma unroll
-    for (int j = 0; j < U / 2; ++j) set_word(b, t + c / 2 + j, pack_pair(v[2 * j], v[2 * j + 1], VERACE_BF16));
+    for (int j = 0; j < U / 4; ++j)
+      set_piece(b, lane, c / 4 + j, make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                               __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
   } else {
+    uint32_t w[U / 2];
+    if (type == VERACE_BF16) {
 #pragma unroll
-    for (int j = 0; j < U / 2; ++j) set_word(b, t + c / 2 + j, pack_pair(v[2 * j], v[2 * j + 1], VERACE_F16));
+      for (int j = 0; j < U / 2; ++j) w[j] = pack_pair(v[2 * j], v[2 * j + 1], VERACE_BF16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < U / 2; ++j) w[j] = pack_pair(v[2 * j], v[2 * j + 1], VERACE_F16);
+    }
+#pragma unroll
+    for (int j = 0; j < U / 8; ++j) set_piece(b, lane, c / 8 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
   }
 }
 template <bool WIDE, int U>
 __device__ __forceinline__ void add(const Block& b, int c, float (&v)[U], int type, int lane) {
-  const int t = 33 * lane;
-  if constexpr (WIDE) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) v[j] += __uint_as_float(word(b, t + c + j));
-  } else {
+  for (int j = 0; j < U / (WIDE ? 4 : 8); ++j) {
+    const uint4 w = get_piece(b, lane, c / (WIDE ? 4 : 8) + j);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int j = 0; j < U / 2; ++j) {
-      const float2 f = unpack_pair(word(b, t + c / 2 + j), type);
-      v[2 * j] += f.x;
-      v[2 * j + 1] += f.y;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (WIDE) {
+        v[4 * j + i] += __uint_as_float(x[i]);
+      } else {
+        const float2 f = unpack_pair(x[i], type);
+        v[8 * j + 2 * i] += f.x;
+        v[8 * j + 2 * i + 1] += f.y;
+      }
     }
   }
 }
@@ -265,8 +315,9 @@ __device__ __forceinline__ void scaled(const Epilogue& e, const uint32_t (&r)[U]
 
 // The saved sums of `width` columns, in fp32: 32 columns at a time.
 __device__ __forceinline__ void save_sums(const Epilogue& e, Block b, uint32_t tmem, int width, float rs, const float* col_scale,
-                                          const void* bias, void* out, int lane) {
+                                          const void* bias, const Target& to, int lane) {
   for (int c = 0; c < width && b.n0 < b.N; c += 32, b.n0 += 32) {
+    reclaim(lane);
 #pragma unroll
     for (int h = 0; h < 32; h += 16) {
       uint32_t r[16];
@@ -276,7 +327,7 @@ __device__ __forceinline__ void save_sums(const Epilogue& e, Block b, uint32_t t
       scaled(e, r, v, rs, col_scale, bias, b.n0 + h, b.N);
       put<true>(b, h, v, VERACE_F32, lane);
     }
-    write_block<true>(b, out, e.ld, lane);
+    write_block<true>(b, to, lane);
   }
 }
 
@@ -285,24 +336,26 @@ __device__ __forceinline__ void save_sums(const Epilogue& e, Block b, uint32_t t
 // block's sums are in registers.
 template <bool GATED, bool WIDE, typename F>
 __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b, uint32_t tmem, uint32_t tmem_up,
-                                               const uint32_t (&res)[32], void* out, int lane, F&& loaded) {
+                                               const uint32_t (&res)[32], const Target& out, const Target& pre,
+                                               const Target& pre_up, int lane, F&& loaded) {
   constexpr int WIDTH = WIDE ? 32 : 64, U = 16, LOTS = WIDTH / U;
   const long long m = b.m0 + lane;
   const float rs = e.row_scale && m < b.M ? e.row_scale[m] : 0.f;
   if (e.pre) {
-    save_sums(e, b, tmem, WIDTH, rs, e.col_scale, GATED ? nullptr : e.bias, e.pre, lane);
-    if (GATED) save_sums(e, b, tmem_up, WIDTH, rs, e.up_scale, nullptr, e.pre_up, lane);
+    save_sums(e, b, tmem, WIDTH, rs, e.col_scale, GATED ? nullptr : e.bias, pre, lane);
+    if (GATED) save_sums(e, b, tmem_up, WIDTH, rs, e.up_scale, nullptr, pre_up, lane);
   }
-  if (GATED && out == nullptr) {   // (partial sums: the two above are all)
+  if (GATED && out.p == nullptr) {   // (partial sums: the two above are all)
     loaded();
     return;
   }
   uint32_t r[U], s[U];
   tmem_ld_async(tmem, r);
   if constexpr (GATED) tmem_ld_async(tmem_up, s);
+  reclaim(lane);
   if (!GATED && e.residual) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) set_word(b, 33 * i + lane, res[i]);
+    for (int i = 0; i < 32; ++i) set_word(b, i, lane, res[i]);
     __syncwarp();
   }
 #pragma unroll 1
@@ -322,12 +375,12 @@ __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b
     if (!GATED && e.residual) add<WIDE>(b, l * U, v, e.type, lane);
     put<WIDE>(b, l * U, v, e.type, lane);
   }
-  write_block<WIDE>(b, out, e.ld, lane);
+  write_block<WIDE>(b, out, lane);
 }
 
 // A warp's part of every tile of the pair: TMEM lanes 32 (warp % 4) ..., one half of the columns.
 template <bool GATED, bool WIDE, int BN, typename Wait, typename Free>
-__device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t turn, uint32_t tmem, int pair, int pairs, int rank,
+__device__ __forceinline__ void epilogue_tiles(const Args& p, const Maps& maps, uint32_t turn, uint32_t tmem, int pair, int pairs, int rank,
                                                int warp, int lane, Wait&& wait, Free&& release) {
   constexpr int HB = BN / 2, TN = GATED ? HB : BN, WIDTH = WIDE ? 32 : 64, PER = TN / 2 > WIDTH ? TN / 2 : WIDTH;
   const int half = (warp - 4) >> 2, first = half * PER, last = min(TN, first + PER);
@@ -341,17 +394,13 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t turn, uin
     const Place at = place(p, t);
     b.m0 = at.m * 256LL + rank * 128 + 32 * (warp & 3);
     b.n0 = (long long)at.n * TN + first;
-    Epilogue e = p.e;
-    void* out = p.nz > 1 ? p.out_z[at.z] : e.out;
-    if (p.splits > 1) {
-      const long long first_of = (at.split * p.nz + at.z) * p.partial;
-      if (GATED) {
-        e.pre += first_of;
-        e.pre_up += first_of;
-      } else {
-        out = static_cast<float*>(e.out) + first_of;
-      }
-    }
+    // the tile's outputs: of split i the i-th of the partial ones
+    const long long first_of = p.splits > 1 ? (at.split * p.nz + at.z) * p.partial : 0;
+    const int slot = p.splits > 1 ? 0 : at.z, z = p.splits > 1 ? at.split * p.nz + at.z : 0;
+    Target out{p.by_tma ? &maps.out[slot] : nullptr, z, p.nz > 1 && p.splits == 1 ? p.out_z[at.z] : p.e.out, p.e.ld};
+    Target pre{p.pre_by_tma ? &maps.pre[0] : nullptr, z, p.e.pre ? p.e.pre + first_of : nullptr, p.e.ld};
+    Target pre_up{p.pre_by_tma ? &maps.pre[1] : nullptr, z, p.e.pre_up ? p.e.pre_up + first_of : nullptr, p.e.ld};
+    if (!GATED && p.splits > 1) out.p = static_cast<float*>(p.e.out) + first_of;
     uint32_t res[32];
     if (!GATED && p.e.residual && b.m0 < b.M && b.n0 < b.N && first < last)   // on its way while the products run
       read_words<WIDE>(b, p.e.residual, p.e.ld_res, lane, res);
@@ -367,7 +416,7 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t turn, uin
       after.n0 += WIDTH;
       const bool more = c + WIDTH < last && after.n0 < b.N;
       if (!GATED && p.e.residual && more) read_words<WIDE>(after, p.e.residual, p.e.ld_res, lane, next);
-      epilogue_block<GATED, WIDE>(e, b, sums + c, sums + HB + c, res, out, lane, [&] {
+      epilogue_block<GATED, WIDE>(p.e, b, sums + c, sums + HB + c, res, out, pre, pre_up, lane, [&] {
         if (!more) {
           release(n);
           held = false;
@@ -379,6 +428,7 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, uint32_t turn, uin
     }
     if (held) release(n);
   }
+  if (lane == 0) tc::bulk_wait<0>();   // (the stores are done before the CTA ends)
 }
 
 template <bool F8, bool AMN, bool BMN, bool GATED, int BN, bool PARTS>
@@ -614,9 +664,9 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
     auto release = [&](int n) {
       if (!PARTS) free(n);
     };
-    if (PARTS) epilogue_tiles<GATED, true, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
-    else if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
-    else epilogue_tiles<GATED, false, BN>(p, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    if (PARTS) epilogue_tiles<GATED, true, BN>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else epilogue_tiles<GATED, false, BN>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -638,21 +688,8 @@ int launch(const Product& p, int splits, cudaStream_t st) {
     if ((rc = operand_map(&maps.b[i], p.b[p.b[i].p ? i : 0], p.type, BMN ? 64 : BN / 2))) return rc;
   Args a{};
   a.M = p.M; a.N = p.N;
-  a.kblocks = (int)((p.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
-  a.segments = p.segments; a.a_first = p.a_first; a.a_step = p.a_step;
-  a.nz = p.nz;
-  a.tiles_m = (int)((p.M + 255) / 256);
-  a.tiles_n = (int)((p.N + TN - 1) / TN);
-  a.splits = splits;
-  a.per = (a.kblocks + splits - 1) / splits;
-  a.partial = p.M * p.N;
-  const long long tiles = (long long)a.tiles_m * a.tiles_n * p.nz * splits;
-  VERACE_REQUIRE(tiles < 1LL << 30, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
-  a.tiles = (int)tiles;
-  a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
-            (uint32_t)AMN << 15 | (uint32_t)BMN << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
-  a.out_z[0] = p.out_z[0]; a.out_z[1] = p.out_z[1];
   a.e = p.e;
+  a.partial = p.M * p.N;
   if (splits > 1) {
     Epilogue e{};
     e.ld = p.N; e.type = VERACE_F32; e.act = VERACE_ACT_NONE;
@@ -664,6 +701,30 @@ int launch(const Product& p, int splits, cudaStream_t st) {
     }
     a.e = e;
   }
+  // the outputs' maps (of splits: one, over all partial outputs)
+  const int outs = splits > 1 ? 1 : p.nz, planes = splits > 1 ? splits * p.nz : 1;
+  void* const out[2] = {outs > 1 ? p.out_z[0] : a.e.out, outs > 1 ? p.out_z[1] : nullptr};
+  auto aligned = [&](const void* q, int type) { return q && (size_t)q % 16 == 0 && a.e.ld * size_of(type) % 16 == 0; };
+  a.by_tma = aligned(out[0], a.e.type) && (outs == 1 || aligned(out[1], a.e.type));
+  a.pre_by_tma = aligned(a.e.pre, VERACE_F32) && (!GATED || aligned(a.e.pre_up, VERACE_F32));
+  for (int i = 0; i < outs && a.by_tma; ++i)
+    if ((rc = operand_map(&maps.out[i], Mat{out[i], p.M, p.N, a.e.ld, planes, a.partial}, a.e.type, 32))) return rc;
+  for (int i = 0; i < (GATED ? 2 : 1) && a.pre_by_tma; ++i)
+    if ((rc = operand_map(&maps.pre[i], Mat{i ? a.e.pre_up : a.e.pre, p.M, p.N, a.e.ld, planes, a.partial}, VERACE_F32, 32)))
+      return rc;
+  a.kblocks = (int)((p.K + (F8 ? 127 : 63)) / (F8 ? 128 : 64));
+  a.segments = p.segments; a.a_first = p.a_first; a.a_step = p.a_step;
+  a.nz = p.nz;
+  a.tiles_m = (int)((p.M + 255) / 256);
+  a.tiles_n = (int)((p.N + TN - 1) / TN);
+  a.splits = splits;
+  a.per = (a.kblocks + splits - 1) / splits;
+  const long long tiles = (long long)a.tiles_m * a.tiles_n * p.nz * splits;
+  VERACE_REQUIRE(tiles < 1LL << 30, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld outputs are too many", p.M, p.N);
+  a.tiles = (int)tiles;
+  a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
+            (uint32_t)AMN << 15 | (uint32_t)BMN << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+  a.out_z[0] = p.out_z[0]; a.out_z[1] = p.out_z[1];
   auto kern = large_product<F8, AMN, BMN, GATED, BN, PARTS>;
   int dev = 0;
   VERACE_CUDA(cudaGetDevice(&dev));
@@ -752,7 +813,8 @@ int operand_map(CUtensorMap* map, const Mat& m, int type, int rows) {
   const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.pieces};
   const cuuint64_t strides[2] = {m.ld * es, (m.pieces > 1 ? m.piece : m.ld) * es};
   const cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)rows, 1}, el[3] = {1, 1, 1};
-  const CUtensorMapDataType dt = type == VERACE_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+  const CUtensorMapDataType dt = type == VERACE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : type == VERACE_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : type == VERACE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUresult r = enc(map, dt, 3, const_cast<void*>(m.p), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
