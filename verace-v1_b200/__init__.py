@@ -26,6 +26,8 @@ Public surface (mirrors the reference package verace_v1 for this path):
                                                      residual in their epilogues; differentiable)
     rmsnorm_fp8, add_rmsnorm_fp8, quantize_fp8       (rows in 8 bits with scales, which both
                                                      products take)
+    Fp8Linear, Fp8GatedLinear, quantize_model_fp8    (the feed-forward sub-layers and the LM head in
+                                                     8 bits)
 The kernels live in libverace_b200.so (C ABI: include/verace_b200.h), built by
 build.py; nothing here falls back to CPU or Python arithmetic.
 """
@@ -41,7 +43,8 @@ from .config import VeraceV1Config
 from .layer import AdaptiveCognitiveDepthEngine, VeraceV1Layer
 from .model import VeraceV1Model
 from .int4 import Int4Linear, dequantize_int4, int4_linear, quantize_int4, quantize_model_int4
-from .linear import add_rmsnorm_fp8, fused_linear, gated_linear, quantize_fp8, rmsnorm_fp8
+from .linear import (Fp8GatedLinear, Fp8Linear, add_rmsnorm_fp8, fused_linear, gated_linear, quantize_fp8,
+                     quantize_model_fp8, rmsnorm_fp8)
 from .sampling import process_logits, sample_logits
 from .generate import generate
 
@@ -55,5 +58,5 @@ __all__ = [
     "launch_mcmoe_route", "situ_glu", "VeraceV1Config", "VeraceV1Layer", "AdaptiveCognitiveDepthEngine",
     "VeraceV1Model", "Int4Linear", "dequantize_int4", "int4_linear", "quantize_int4", "process_logits",
     "sample_logits", "quantize_model_int4", "generate", "fused_linear", "gated_linear", "rmsnorm_fp8",
-    "add_rmsnorm_fp8", "quantize_fp8",
+    "add_rmsnorm_fp8", "quantize_fp8", "Fp8Linear", "Fp8GatedLinear", "quantize_model_fp8",
 ]

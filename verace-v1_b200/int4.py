@@ -233,7 +233,7 @@ def quantize_model_int4(model: nn.Module, group_size: int = 128, symmetric: bool
             m.w_q = m.w_k = m.w_v = m.w_gamma = None
             m._verace_cat = None
             replace(m, "w_out")
-        elif isinstance(m, SiTUGLU) and m.int4_in is None and m.in_features % 32 == 0:
+        elif isinstance(m, SiTUGLU) and m.int4_in is None and m.fp8_in is None and m.in_features % 32 == 0:
             m.int4_in = pack([m.w_gate, m.w_up])
             m.w_gate = m.w_up = None
             m._stacked = m._stacked_key = None

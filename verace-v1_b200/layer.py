@@ -30,6 +30,7 @@ import torch.nn as nn
 
 from .cham_memory import ContinuousHolographicMemory
 from .kernels import add_rmsnorm, apply_rmsnorm, fused_norm_supported
+from .linear import add_rmsnorm_fp8
 from .mcmoe import ManifoldContinuousMoE
 from .sssd_attention import SSSDAttention
 
@@ -82,8 +83,12 @@ class VeraceV1Layer(nn.Module):
                                                   active_mask=active_mask)
         n = _residual(hcur, sssd_out, self.cham_norm)            # h_mid1, RMSNorm(h_mid1)
         cham_out, new_cham_hologram = self.cham_memory(n, initial_hologram=cham_hologram, active_mask=active_mask)
-        n = _residual(hcur, cham_out, self.mcmoe_norm)           # h_mid2, RMSNorm(h_mid2)
-        _residual(hcur, self.mcmoe(n), None)                     # h_out
+        if self.mcmoe.base_situ_glu.fp8_in is not None and cham_out.dtype == hcur.dtype == self.mcmoe_norm.weight.dtype:
+            q, scale, n = add_rmsnorm_fp8(hcur, cham_out, self.mcmoe_norm, return_norm=True)   # the same, and its rows in 8 bits
+            _residual(hcur, self.mcmoe(n, (q, scale)), None)
+        else:
+            n = _residual(hcur, cham_out, self.mcmoe_norm)       # h_mid2, RMSNorm(h_mid2)
+            _residual(hcur, self.mcmoe(n), None)                 # h_out
         return hcur, block_residual, new_sssd_state, new_cham_hologram
 
 

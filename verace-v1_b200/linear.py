@@ -385,3 +385,93 @@ def add_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, norm: nn.RMSNorm, *, out: 
             "the sum goes to a tensor of h's shape, dtype and device"
     assert out.is_contiguous(), "the sum goes to a contiguous tensor"
     return _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, norm, return_norm)
+
+
+# ---------------------------------------------------------------------------- modules with 8-bit weights
+Rows8 = Tuple[torch.Tensor, torch.Tensor]     # e4m3 rows and their scales
+
+
+def _rows8(x) -> Rows8:
+    return x if isinstance(x, tuple) else quantize_fp8(x)
+
+
+class Fp8Linear(nn.Module):
+    """A linear layer with e4m3 weights (buffers ``weight``, ``scales``, ``bias``) in place of a
+    ``torch.nn.Linear``.  Its input is a tensor, whose rows it quantises, or rows in 8 bits as
+    ``rmsnorm_fp8`` gives them: (values, scales).  The output has ``dtype``."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, dtype: torch.dtype = torch.bfloat16,
+                 device=None):
+        super().__init__()
+        self.in_features, self.out_features, self.dtype = in_features, out_features, dtype
+        self.register_buffer("weight", torch.zeros(out_features, in_features, dtype=FP8, device=device))
+        self.register_buffer("scales", torch.zeros(out_features, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=dtype, device=device) if bias else None)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "Fp8Linear":
+        m = cls(linear.in_features, linear.out_features, linear.bias is not None, linear.weight.dtype, device="meta")
+        m.weight, m.scales = quantize_fp8(linear.weight.detach())
+        m.bias = None if linear.bias is None else linear.bias.detach().clone()
+        return m
+
+    def forward(self, x, residual: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
+        q, s = _rows8(x)
+        return fused_linear(q, self.weight, self.bias, activation=activation, residual=residual, x_scale=s,
+                            w_scale=self.scales, out_dtype=self.dtype)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+class Fp8GatedLinear(nn.Module):
+    """The gate and up projections of a gated block with e4m3 weights and the gate in their product's epilogue
+    (buffers ``w_gate``, ``w_up``, ``gate_scales``, ``up_scales``); its input is as ``Fp8Linear``'s."""
+
+    def __init__(self, in_features: int, hidden_features: int, activation: str = "situ", beta1: float = 4.0,
+                 beta2: float = 25.0, dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        self.in_features, self.hidden_features, self.dtype = in_features, hidden_features, dtype
+        self.activation, self.beta1, self.beta2 = activation, beta1, beta2
+        for w, s in (("w_gate", "gate_scales"), ("w_up", "up_scales")):
+            self.register_buffer(w, torch.zeros(hidden_features, in_features, dtype=FP8, device=device))
+            self.register_buffer(s, torch.zeros(hidden_features, device=device))
+
+    @classmethod
+    def from_weights(cls, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "situ", beta1: float = 4.0,
+                     beta2: float = 25.0) -> "Fp8GatedLinear":
+        f, k = w_gate.shape
+        m = cls(k, f, activation, beta1, beta2, w_gate.dtype, device="meta")
+        m.w_gate, m.gate_scales = quantize_fp8(w_gate.detach())
+        m.w_up, m.up_scales = quantize_fp8(w_up.detach())
+        return m
+
+    def forward(self, x) -> torch.Tensor:
+        q, s = _rows8(x)
+        return gated_linear(q, self.w_gate, self.w_up, activation=self.activation, beta1=self.beta1, beta2=self.beta2,
+                            x_scale=s, gate_scale=self.gate_scales, up_scale=self.up_scales, out_dtype=self.dtype)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, hidden_features={self.hidden_features}, activation={self.activation}"
+
+
+def quantize_model_fp8(model: nn.Module, lm_head: bool = True) -> nn.Module:
+    """Puts the feed-forward sub-layers of a model (a ``VeraceV1Model``, ``VeraceV1Layer`` or any module that
+    holds the framework's M-CMoE) into 8 bits, in place, and with ``lm_head`` the LM head (the token embedding
+    keeps its own table): the gate and up projections with the gate in their epilogue, the down projection with the
+    manifold's part in its epilogue; inside a layer the norm before the sub-layer writes the rows in 8 bits along
+    with the residual's addition.  The model must be on a CUDA device; the dense weights are dropped.  Routers, the
+    sigma projection, norms, bases and the mixers stay as they are, and so does what ``quantize_model_int4`` has
+    put into 4 bits."""
+    from .mcmoe import ManifoldContinuousMoE, SiTUGLU
+
+    for m in list(model.modules()):
+        if isinstance(m, SiTUGLU) and m.fp8_in is None and m.int4_in is None:
+            m.fp8_in = Fp8GatedLinear.from_weights(m.w_gate.weight, m.w_up.weight, "situ", m.beta1, m.beta2)
+            m.w_gate = m.w_up = None
+            m._stacked = m._stacked_key = None
+        elif isinstance(m, ManifoldContinuousMoE) and isinstance(m.base_w_down, nn.Linear):
+            m.base_w_down = Fp8Linear.from_linear(m.base_w_down)
+    if lm_head and isinstance(getattr(model, "lm_head", None), nn.Linear):
+        model.lm_head = Fp8Linear.from_linear(model.lm_head)
+    return model

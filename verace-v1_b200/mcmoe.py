@@ -15,6 +15,10 @@ signature.  The forward pass runs as:
   the hyper-network's sigmoid folded into the epilogue for bf16; a direct fp32 kernel
   otherwise), from the hyper-network's pre-activation;
 * ``base + RMSNorm(manifold)`` in one pass (``verace_add_rmsnorm``).
+
+After ``quantize_model_fp8`` the base FFN runs in 8 bits: both projections and the activation in one
+kernel (``verace_gated_linear``), the down projection with RMSNorm(manifold) as its epilogue's
+residual (``verace_linear``).
 """
 from typing import Optional, Tuple
 
@@ -22,7 +26,8 @@ import torch
 import torch.nn as nn
 
 from ._lib import check, lib
-from .kernels import _DTYPE, _stream, _workspace, add_rmsnorm, fused_norm_supported
+from .kernels import _DTYPE, _stream, _workspace, add_rmsnorm, apply_rmsnorm, fused_norm_supported
+from .linear import Fp8Linear
 
 
 def launch_mcmoe_route(logits: torch.Tensor, k: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -110,6 +115,7 @@ class SiTUGLU(nn.Module):
         self.w_gate = nn.Linear(in_features, hidden_features, bias=False)
         self.w_up = nn.Linear(in_features, hidden_features, bias=False)
         self.int4_in = None      # [W_gate; W_up] in 4 bits (quantize_model_int4), in their place
+        self.fp8_in = None       # both in 8 bits with the gate in their epilogue (quantize_model_fp8)
         self._stacked: Optional[torch.Tensor] = None
         self._stacked_key = None
 
@@ -125,6 +131,8 @@ class SiTUGLU(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda or torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("SiTUGLU runs on CUDA inputs for inference (no autograd path)")
+        if self.fp8_in is not None:
+            return self.fp8_in(x)
         gu = self.int4_in(x) if self.int4_in is not None else torch.nn.functional.linear(x, self._gate_up_weight())
         hf = self.hidden_features
         return situ_glu(gu[..., :hf], gu[..., hf:], self.beta1, self.beta2)
@@ -148,18 +156,27 @@ class ManifoldContinuousMoE(nn.Module):
         self.hyper_sigma = nn.Linear(hidden_dim, num_components * rank, bias=False)
         self.norm = nn.RMSNorm(hidden_dim)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """x: [batch, seq_len, hidden_dim] -> [batch, seq_len, hidden_dim]"""
+    def forward(self, x: torch.Tensor, x8: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+        """x: [batch, seq_len, hidden_dim] -> [batch, seq_len, hidden_dim].  ``x8``: x's rows in 8 bits with
+        their scales (as ``rmsnorm_fp8`` gives them), for a base block in 8 bits (``quantize_model_fp8``)."""
         if not x.is_cuda or torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("ManifoldContinuousMoE runs on CUDA inputs for inference (no autograd path)")
         b, s, d = x.shape
         x_flat = x.reshape(b * s, d).contiguous()
-        base_out = self.base_w_down(self.base_situ_glu(x_flat)).contiguous()
+        fp8 = self.base_situ_glu.fp8_in
+        if fp8 is not None:
+            base_in = fp8(x_flat if x8 is None else (x8[0].view(b * s, d), x8[1].reshape(b * s)))
+        else:
+            base_in = self.base_situ_glu(x_flat)
+        down8 = isinstance(self.base_w_down, Fp8Linear)
+        base_out = None if down8 else self.base_w_down(base_in).contiguous()
         k_val = min(self.top_k_components, self.num_components)
         idx, w = launch_mcmoe_route(self.router(x_flat), k_val)
         sig_pre = self.hyper_sigma(x_flat)
         manifold = launch_mcmoe_projection(x_flat, self.u_basis, self.v_basis, idx, w, sig_pre, sigma_is_logits=True)
-        if fused_norm_supported(base_out) and self.norm.weight.dtype == base_out.dtype:
+        if down8:                # the manifold's part is the down projection's residual
+            y = self.base_w_down(base_in, residual=apply_rmsnorm(self.norm, manifold))
+        elif fused_norm_supported(base_out) and self.norm.weight.dtype == base_out.dtype:
             add_rmsnorm(base_out, manifold, y_norm=self.norm)   # base_out <- base_out + norm(manifold)
             y = base_out
         else:
