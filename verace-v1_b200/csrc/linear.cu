@@ -166,11 +166,6 @@ __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long l
 }
 
 
-// Tokens up to which weights are streamed past them (linear_few.cu).  bf16: 48 x 4096 x 8192 17.6 us against 19.8 for
-// tiles of 256 rows, 96 x 8192 x 4096 21.0 against 25.4, 128 x 4096 x 32000 50.0 against 56.7; 128 x 1024 x 4096 9.2 against 8.8,
-// 176 x 4096 x 8192 23.4 against 20.2, 256 x 4096 x 32000 76.9 against 59.8.
-constexpr long long FEW = 112;
-
 // Whether a forward product goes to the engine of dot products.  In fp32 that saves splitting the weights
 // (8 x 4096 x 4096: 23 us against 59; 16 tokens 38 against 59, 32 tokens 68 against 61).  In 16 and 8 bits the tensor cores
 // win where the weights' bytes count (1 x 1024 x 163840 bf16 58 us against 60, 4 x 4096 x 4096 12.3

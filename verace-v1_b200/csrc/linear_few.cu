@@ -1,6 +1,6 @@
 // Products of few rows (tokens) on the tensor cores, the other engine behind linear.cu:
-//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 128
-// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 128 columns, so
+//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 96
+// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 96 columns, so
 // a weight crosses shared memory once and no row of the MMA is idle; a CTA streams its 128 rows (gated:
 // 128 of each weight, two sums side by side in TMEM) by TMA in stages of 128 bytes of K.  Two
 // CTAs share an SM where shared memory allows, so that one's set-up and epilogue run under the other's
@@ -26,7 +26,7 @@ namespace cg = cooperative_groups;
 using namespace lin;
 
 constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8;
-// shared memory for stages of a CTA that has an SM to itself, and of one that shares it (228 KB an SM,
+// shared memory for stages, or for the sums of up to FEW tokens, of a CTA that has an SM to itself, and of one that shares it (228 KB an SM,
 // less 1 KB a CTA that the system takes, 1 KB of barriers and 1 KB to align the stages)
 constexpr int ROOM = 225 * 1024, HALF_ROOM = 111 * 1024;
 constexpr uint32_t POLLS = 1u << 22;
@@ -41,7 +41,6 @@ struct Args {
   int stages, stage;    // and a stage's bytes
   int kblocks, steps, per, ck, tiles_n;
   int cols;             // of TMEM
-  int round;            // tokens whose partial sums a CTA holds at a time (ck > 1)
   int a_first;
   uint32_t idesc;
   Epilogue e;
@@ -230,44 +229,46 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
       }
     }
   } else {
-    // every CTA's sums of `round` tokens in its shared memory (the stages' place), [token][128]
-    cg::cluster_group cl = cg::this_cluster();
+    // every CTA's sums in its shared memory (the stages' place), [token][128].  TMEM is given back before the CTA
+    // waits for the others of its cluster: one that held it there could wait for a CTA that waits for TMEM
     float* part = reinterpret_cast<float*>(sm);
-    for (int t0 = 0; t0 < tokens; t0 += p.round) {
-      for (int t = 16 * (warp >> 2); t < p.round && t0 + t < tokens; t += 32)
+    for (int t = 16 * (warp >> 2); t < tokens; t += 32)
 #pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-          uint32_t r[16];
-          tmem_ld_async(mine + h * p.mp + t0 + t, r);
-          tmem_wait(r);
-          float* o = part + (h * p.round + t) * ROWS + 32 * quarter + lane;
+      for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+        uint32_t r[16];
+        tmem_ld_async(mine + h * p.mp + t, r);
+        tmem_wait(r);
+        float* o = part + (h * p.mp + t) * ROWS + 32 * quarter + lane;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j * ROWS] = ok && first < last ? __uint_as_float(r[j]) : 0.f;
-        }
-      cl.sync();
-      const int total = min(p.round, tokens - t0) * (ROWS / 4);
-#pragma unroll 2
-      for (int i = rank * NT + tid; i < total; i += p.ck * NT) {
-        float g[4] = {}, u[4] = {};
-#pragma unroll 4
-        for (int c = 0; c < p.ck; ++c) {
-          const float4* o = reinterpret_cast<const float4*>(cl.map_shared_rank(part, c));
-          const float4 a = o[i];
-          g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
-          if (GATED) {
-            const float4 b = o[p.round * (ROWS / 4) + i];
-            u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
-          }
-        }
-        const long long c = n0 + i % (ROWS / 4) * 4;
-        if (c < p.N) finish4<GATED>(p.e, t0 + i / (ROWS / 4), c, p.N, g, u);
+        for (int j = 0; j < 16; ++j) o[j * ROWS] = ok && first < last ? __uint_as_float(r[j]) : 0.f;
       }
-      cl.sync();
-    }
   }
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 1) tc::tmem_dealloc(tmem, p.cols);
+  if (p.ck > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    const float* part = reinterpret_cast<const float*>(sm);
+    cl.sync();
+    const int total = tokens * (ROWS / 4);
+#pragma unroll 2
+    for (int i = rank * NT + tid; i < total; i += p.ck * NT) {
+      float g[4] = {}, u[4] = {};
+#pragma unroll 4
+      for (int c = 0; c < p.ck; ++c) {
+        const float4* o = reinterpret_cast<const float4*>(cl.map_shared_rank(part, c));
+        const float4 a = o[i];
+        g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+        if (GATED) {
+          const float4 b = o[p.mp * (ROWS / 4) + i];
+          u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+        }
+      }
+      const long long c = n0 + i % (ROWS / 4) * 4;
+      if (c < p.N) finish4<GATED>(p.e, i / (ROWS / 4), c, p.N, g, u);
+    }
+    cl.sync();   // (the others may still read this CTA's sums)
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -277,6 +278,7 @@ int launch(const Product& p, cudaStream_t st) {
   Args a{};
   int rc;
   a.M = p.M; a.N = p.N;
+  static_assert(FEW % 16 == 0 && FEW * ROWS * 4 * 2 <= HALF_ROOM, "a cluster's sums fit beside another CTA's");
   a.mp = (int)((p.M + 15) / 16 * 16);
   // A (x) in one box of all tokens, B (the weights) as the MMA's rows
   if ((rc = operand_map(&maps.x, p.a, p.type, a.mp))) return rc;
@@ -298,13 +300,9 @@ int launch(const Product& p, cudaStream_t st) {
   const int want = a.mp * (GATED ? 2 : 1);
   a.cols = 32;
   while (a.cols < want) a.cols *= 2;
-  const int token = ROWS * 4 * (GATED ? 2 : 1);
   int smem = a.stages * a.stage;
-  a.round = a.mp;
-  if (a.ck > 1) {
-    if (smem < a.mp * token) smem = a.mp * token < room ? a.mp * token : room;   // (a short K: few stages)
-    if (a.round * token > smem) a.round = smem / token / 16 * 16;
-  }
+  const int sums = a.mp * ROWS * 4 * (GATED ? 2 : 1);
+  if (a.ck > 1 && smem < sums) smem = sums;
   smem += 1024;
   a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
             (uint32_t)WMN << 15 | (uint32_t)(a.mp >> 3) << 17 | (uint32_t)(ROWS >> 4) << 24;

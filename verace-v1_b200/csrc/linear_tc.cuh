@@ -35,8 +35,13 @@ struct Product {
 // What product_large may take for partial sums (M x N outputs each, nz of them).
 size_t split_bytes(long long M, long long N, long long K, int segments, int nz, bool gated, int type, bool parts);
 
+// Tokens up to which weights are streamed past them (linear_few.cu).  bf16: 48 x 4096 x 8192 17.6 us against 19.8 for
+// tiles of 256 rows, 96 x 8192 x 4096 21.0 against 25.4, 128 x 4096 x 32000 50.0 against 56.7; 128 x 1024 x 4096 9.2 against 8.8,
+// 176 x 4096 x 8192 23.4 against 20.2, 256 x 4096 x 32000 76.9 against 59.8.
+constexpr int FEW = 96;
+
 int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
-int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to 256 rows of A
+int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to FEW rows of A
 int product_dot(const Product& p, cudaStream_t st);     // linear_dot.cu: a few rows of A, fp32 operands as they are
 
 // ------------------------------------------------------------------ launches
