@@ -456,6 +456,8 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  if (warp == 2 && lane < 5)   // (the tensor maps on their way: a, b, b, out, out)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a + lane) : "memory");
   if (tid == 0) {
     for (int i = 0; i < S::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);

@@ -86,7 +86,7 @@ def _checked(who, x, weight, scales, want, activation, allowed, out_dtype, defau
 
 
 def _workspace(nbytes: int, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device) if nbytes else None
 
 
 _NOTHING = contextlib.nullcontext()
@@ -105,7 +105,7 @@ def _p(t: Optional[torch.Tensor]):
 def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
     dev = x2.device
     y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=dev)
-    pre = torch.empty((m, n), dtype=torch.float32, device=dev) if want_pre else None
+    pre = torch.empty_strided((m, n), (n, 1), dtype=torch.float32, device=dev) if want_pre else None
     L = lib()
     code = _CODE[x2.dtype]
     nws = L.verace_linear_workspace(m, n, k, code)
@@ -117,38 +117,54 @@ def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, w
     return y, pre
 
 
+def _fused_linear_backward(ctx, d):
+    x2, w2, pre = ctx.saved_tensors
+    shape, m, n, k, ldx, ldw, act, out_dtype = ctx.sizes
+    want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
+    dx = dw = db = None
+    if want_x or want_w or want_b:
+        dev, dt = x2.device, x2.dtype
+        if want_x:
+            dx = torch.empty_strided((m, k), (k, 1), dtype=dt, device=dev)
+        if want_w:
+            dw = torch.empty_strided((n, k), (k, 1), dtype=dt, device=dev)
+        if want_b:
+            db = torch.empty_strided((n,), (1,), dtype=dt, device=dev)
+        d2 = d.contiguous()
+        L = lib()
+        code = _DTYPE[dt]
+        nws = L.verace_linear_backward_workspace(m, n, k, code)
+        ws = _workspace(nws, dev)
+        with _on(dev):
+            rc = L.verace_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(pre), _p(dx), _p(dw),
+                                          _p(db), m, n, k, act, code, _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index))
+            if rc:
+                check(rc, "verace_linear_backward")
+        if dx is not None and len(shape) != 2:
+            dx = dx.view(shape)
+    return dx, dw, db, d if want_r else None, None, None, None, None, None
+
+
+_fused_linear_backward_once = once_differentiable(_fused_linear_backward)
+
+
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, out_dtype, m, n, k):
         x2, ldx = _rows(x, m, k)
         w2, ldw = _rows(weight, n, k)
-        b = _vector(bias, n, x.dtype, x.device, "bias")
+        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         res, ldr = _residual_rows(residual, m, n)
         y, pre = _linear(x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
         ctx.save_for_backward(x2, w2, pre)
-        ctx.sizes = (x.shape, m, n, k, ldx, ldw, act, out_dtype, None if bias is None else bias.shape)
-        return y.view(x.shape[:-1] + (n,))
+        shape = x.shape
+        ctx.sizes = (shape, m, n, k, ldx, ldw, act, out_dtype)
+        return y if len(shape) == 2 else y.view(shape[:-1] + (n,))
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d):
-        x2, w2, pre = ctx.saved_tensors
-        shape, m, n, k, ldx, ldw, act, out_dtype, bias_shape = ctx.sizes
-        want = ctx.needs_input_grad
-        dev, dt = x2.device, x2.dtype
-        dx = torch.empty((m, k), dtype=dt, device=dev) if want[0] else None
-        dw = torch.empty((n, k), dtype=dt, device=dev) if want[1] else None
-        db = torch.empty(bias_shape, dtype=dt, device=dev) if want[2] else None
-        if want[0] or want[1] or want[2]:
-            d2 = d.contiguous()
-            L = lib()
-            nws = L.verace_linear_backward_workspace(m, n, k, _DTYPE[dt])
-            ws = _workspace(nws, dev)
-            with _on(dev):
-                check(L.verace_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(pre), _p(dx),
-                                               _p(dw), _p(db), m, n, k, act, _DTYPE[dt], _DTYPE[out_dtype], _p(ws), nws,
-                                               raw_stream(dev.index)), "verace_linear_backward")
-        return (None if dx is None else dx.view(shape), dw, db, d if want[3] else None) + (None,) * 5
+        # (where no graph is asked for, without the wrapper that refuses the second derivative: 6 us)
+        return (_fused_linear_backward_once if torch.is_grad_enabled() else _fused_linear_backward)(ctx, d)
 
 
 def _residual_rows(residual, m, n):
@@ -227,7 +243,10 @@ def _gate_rows(w_gate, w_up, f, k):
 def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
     dev = x2.device
     h = torch.empty_strided((m, f), (f, 1), dtype=out_dtype, device=dev)
-    gate, up = torch.empty((2, m, f), dtype=torch.float32, device=dev) if want_pre else (None, None)
+    gate = up = None
+    if want_pre:
+        gate = torch.empty_strided((m, f), (f, 1), dtype=torch.float32, device=dev)
+        up = torch.empty_strided((m, f), (f, 1), dtype=torch.float32, device=dev)
     L = lib()
     code = _CODE[x2.dtype]
     nws = L.verace_gated_linear_workspace(m, f, k, code)
@@ -240,6 +259,33 @@ def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, wa
     return h, gate, up
 
 
+def _gated_linear_backward(ctx, d):
+    x2, g2, u2, gate, up = ctx.saved_tensors
+    shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype = ctx.sizes
+    want_x, want_g, want_u = ctx.needs_input_grad[:3]
+    dev, dt = x2.device, x2.dtype
+    dx = torch.empty_strided((m, k), (k, 1), dtype=dt, device=dev) if want_x else None
+    dg = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_g else None
+    du = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_u else None
+    d2 = d.contiguous()
+    L = lib()
+    code = _DTYPE[dt]
+    nws = L.verace_gated_linear_backward_workspace(m, f, k, code)
+    ws = _workspace(nws, dev)
+    with _on(dev):
+        rc = L.verace_gated_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, g2.data_ptr(), u2.data_ptr(), ldw,
+                                            gate.data_ptr(), up.data_ptr(), _p(dx), _p(dg), _p(du), m, f, k, act, b1, b2, code,
+                                            _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index))
+        if rc:
+            check(rc, "verace_gated_linear_backward")
+    if dx is not None and len(shape) != 2:
+        dx = dx.view(shape)
+    return dx, dg, du, None, None, None, None, None, None, None
+
+
+_gated_linear_backward_once = once_differentiable(_gated_linear_backward)
+
+
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act, b1, b2, out_dtype, m, f, k):
@@ -247,29 +293,13 @@ class _GatedLinear(torch.autograd.Function):
         g2, u2, ldw = _gate_rows(w_gate, w_up, f, k)
         h, gate, up = _gated(x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
         ctx.save_for_backward(x2, g2, u2, gate, up)
-        ctx.sizes = (x.shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype)
-        return h.view(x.shape[:-1] + (f,))
+        shape = x.shape
+        ctx.sizes = (shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype)
+        return h if len(shape) == 2 else h.view(shape[:-1] + (f,))
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d):
-        x2, g2, u2, gate, up = ctx.saved_tensors
-        shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype = ctx.sizes
-        want = ctx.needs_input_grad
-        dev, dt = x2.device, x2.dtype
-        dx = torch.empty((m, k), dtype=dt, device=dev) if want[0] else None
-        dg = torch.empty((f, k), dtype=dt, device=dev) if want[1] else None
-        du = torch.empty((f, k), dtype=dt, device=dev) if want[2] else None
-        d2 = d.contiguous()
-        L = lib()
-        nws = L.verace_gated_linear_backward_workspace(m, f, k, _DTYPE[dt])
-        ws = _workspace(nws, dev)
-        with _on(dev):
-            check(L.verace_gated_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, g2.data_ptr(), u2.data_ptr(), ldw,
-                                                 gate.data_ptr(), up.data_ptr(), _p(dx), _p(dg), _p(du), m, f, k, act, b1,
-                                                 b2, _DTYPE[dt], _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index)),
-                  "verace_gated_linear_backward")
-        return (None if dx is None else dx.view(shape), dg, du) + (None,) * 7
+        return (_gated_linear_backward_once if torch.is_grad_enabled() else _gated_linear_backward)(ctx, d)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation: str = "situ",
