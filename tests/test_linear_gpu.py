@@ -384,6 +384,90 @@ def test_feed_forward_sub_layer(m):
     assert_within(out, linear64(dequantised(qa, sa), dequantised(wd, sd), None, None, h, BF16))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,k,n", [(300, 9000, 100), (260, 4100, 33), (97, 20000, 64)])
+def test_long_sums_over_few_tiles(m, k, n, dt):
+    """K is split over many tiles' worth of CTAs, forward and (K the tokens) in the weights' gradients."""
+    g = gen(m, k, n, 20)
+    x, wg, wu = randn(g, m, k, dt=dt), weight(g, n, k, dt), weight(g, n, k, dt)
+    b, r = randn(g, n, dt=dt), randn(g, m, n, dt=dt)
+    assert_within(V.fused_linear(x, wg, b, activation="silu", residual=r), linear64(x, wg, b, "silu", r, dt), "linear")
+    assert_within(V.gated_linear(x, wg, wu), gated64(x, wg, wu, "situ", dt), "gated")
+    # tokens and widths change places
+    xt, w1, w2, d = randn(g, k, 40, dt=dt), weight(g, n, 40, dt), weight(g, n, 40, dt), randn(g, k, n, dt=dt)
+    leaves = [v.requires_grad_() for v in (xt, w1, w2)]
+    got = torch.autograd.grad(V.gated_linear(*leaves, activation="silu"), leaves, d)
+    for name, a, c in zip(("dx", "dw_gate", "dw_up"), got, gated_backward64(*(v.detach() for v in leaves), "silu", d, dt)):
+        assert_within(a, c, name)
+    only = w2.detach().requires_grad_()         # one of the weights alone
+    one = torch.autograd.grad(V.gated_linear(xt.detach(), w1.detach(), only, activation="silu"), only, d)[0]
+    assert_within(one, gated_backward64(xt.detach(), w1.detach(), only.detach(), "silu", d, dt)[2], "dw_up alone")
+    got = torch.autograd.grad(V.fused_linear(xt, w1), (xt, w1), d)
+    for name, a, c in zip(("dx", "dw"), got, linear_backward64(xt.detach(), w1.detach(), None, None, d, dt)):
+        assert_within(a, c, name)
+
+
+def test_long_sums_in_8_bits():
+    g = gen(21)
+    (x, sx), (wg, sg), (wu, su) = (fp8_rows(t) for t in (randn(g, 300, 9008), weight(g, 100, 9008), weight(g, 100, 9008)))
+    x64, g64, u64 = dequantised(x, sx), dequantised(wg, sg), dequantised(wu, su)
+    b = randn(g, 100, dt=F16)
+    assert_within(V.fused_linear(x, wg, b, activation="gelu", x_scale=sx, w_scale=sg, out_dtype=F16),
+                  linear64(x64, g64, b, "gelu", None, F16))
+    assert_within(V.gated_linear(x, wg, wu, x_scale=sx, gate_scale=sg, up_scale=su), gated64(x64, g64, u64, "situ", BF16))
+
+
+@pytest.mark.parametrize("m", [1, 3, 50, 300])
+@pytest.mark.parametrize("n", [64, 101])
+def test_out_may_be_the_residual(m, n):
+    """The C entry point with the output in the residual's place, in each engine."""
+    g = gen(m, n, 22)
+    for dt, code in ((F32, 0), (BF16, 1)):
+        x, w, r = randn(g, m, 96, dt=dt), weight(g, n, 96, dt), randn(g, m, n, dt=dt)
+        want = V.fused_linear(x, w, residual=r)
+        L = V._lib.lib()
+        nws = L.verace_linear_workspace(m, n, 96, code)
+        ws = torch.empty(max(nws, 1), dtype=torch.uint8, device="cuda")
+        rc = L.verace_linear(x.data_ptr(), 96, None, w.data_ptr(), 96, None, None, r.data_ptr(), n, r.data_ptr(), None, m, n, 96,
+                             0, code, code, ws.data_ptr(), nws, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(r, want)
+
+
+@pytest.mark.parametrize("m", [1, 2, 40, 300])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_chains_of_calls_wait_for_each_other(m, dt):
+    """Kernels that become resident before the one ahead of them ends: a chain without a wait on the host gives the bits
+    of the same chain with one after every call.  The framework's other early launches (rmsnorm, int4) are among them."""
+    g = gen(m, 23)
+    k, f = 128, 256
+    norm = torch.nn.RMSNorm(k, eps=1e-6, device="cuda", dtype=dt).requires_grad_(False)
+    wg, wu, wd, w4 = weight(g, f, k, dt), weight(g, f, k, dt), weight(g, k, f, dt), weight(g, k, k, dt)
+    q8, s8 = V.quantize_fp8(weight(g, k, k))
+    q4, s4, _ = V.quantize_int4(w4)
+    first = randn(g, m, k, dt=dt)
+
+    def chain(wait):
+        h, out = first.clone(), []
+        for _ in range(12):
+            n = V.rmsnorm(h, norm)
+            wait()
+            a = V.gated_linear(n, wg, wu)
+            wait()
+            h = V.fused_linear(a, wd, residual=h)
+            wait()
+            q, s = V.add_rmsnorm_fp8(h, n, norm)
+            wait()
+            y = V.fused_linear(q, q8, x_scale=s, w_scale=s8, out_dtype=dt)
+            wait()
+            h = V.add_rmsnorm(h, y, out_norm=norm) + V.int4_linear(y, q4, s4)
+            wait()
+            out.append(h)
+        return out
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), want))
+
+
 def test_refusals():
     g = gen(19)
     x, w = randn(g, 4, 64, dt=BF16), weight(g, 32, 64, BF16)

@@ -165,16 +165,17 @@ __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long l
   store_as(e.out, r * e.ld + c, v, e.type);
 }
 
-
 // Whether a forward product goes to the engine of dot products.  In fp32 that saves splitting the weights
-// (8 x 4096 x 4096: 23 us against 59; 16 tokens 38 against 59, 32 tokens 68 against 61).  In 16 and 8 bits the tensor cores
-// win where the weights' bytes count (1 x 1024 x 163840 bf16 58 us against 60, 4 x 4096 x 4096 12.3
-// against 13.5), the dot products where the launch does (1 x 1024 x 2048 bf16 3.1 us against 7.1, gated 4.2 M
-// weights 5.5 against 7.9; 1 x 4096 x 4096 8.7 against 12.3; 4 tokens of gated 4.2 M 5.4 against 8.8).
+// (8 x 4096 x 4096: 23 us against 71, 24 tokens 63 against 72; gated 16 tokens 111 against 135, 24 tokens 162 against
+// 135).  In 16 and 8 bits the tensor cores win where the weights' bytes count, the dot products where the launch does
+// (us, dot products against the others, in chains of calls; bf16: 1 x 1024 x 1024 2.5 and 4.4, 1 x 4096 x 4096 8.4 and
+// 9.6, 1 x 8192 x 4096 13.8 and 14.7; gated 1 x 1024 x 4096 5.7 and 6.3, 1 x 2048 x 4096 8.8 and 8.2; 4 x 1024 x 4096 4.9
+// and 5.6, 4 x 2048 x 4096 8.6 and 6.8; e4m3: 1 x 2048 x 4096 5.9 and 6.1, 1 x 4096 x 4096 8.7 and 7.4).
 bool by_dots(long long m, long long n, long long k, int type, int weights) {
   if (k == 0 || n > 65535LL * 8) return false;
-  if (type == VERACE_F32) return m <= 16;
-  return m <= 4 && n * k * weights <= (m == 1 ? 24LL << 20 : 6LL << 20);
+  if (type == VERACE_F32) return m <= (weights == 1 ? 24 : 16);
+  const long long most = m > 4 ? 0 : m > 1 ? 5 : weights == 1 && type != VERACE_E4M3 ? 32 : 10;   // millions of weights
+  return n * k * weights <= most << 20;
 }
 
 // Whether a product of operands in memory goes to the engine that streams the weights past its rows.
@@ -207,7 +208,7 @@ int run_product(Product& p, cudaStream_t st) {
 // ------------------------------------------------------------------ backward of the epilogues
 // p = d act'(pre) as an operand of the products (rounded to the type of x, or in three parts), and its
 // column sums: a CTA takes 32 rows (gated: 16) of 256 columns, a thread every eighth row of 8 columns.
-// Bound: bytes (d and pre read, p written).
+// Bound: bytes (d and pre read, p written): gated 4096 x 8192 bf16 90 us for 470 MB, 5.2 TB/s.
 constexpr int CHUNK = 32, GATED_CHUNK = 16;
 struct SlopeArgs {
   const void* d;

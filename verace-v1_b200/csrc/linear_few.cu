@@ -10,6 +10,9 @@
 // Warps: 0 feeds the stages, 1 issues the MMAs; then all eight read the sums, two a quarter of TMEM: a thread holds a weight
 // row, so neighbouring threads store neighbouring outputs of a token.  The input gradient of few tokens
 // (a_mn: weights stored [K][N], read as MN-major) runs here too, for a gated block over both weights.
+//
+// Measured in chains of calls: 7 x 8192 x 4096 fp16 15.3 us (4.4 TB/s, 5 us of it set-up, first loads and the join),
+// 32 x 1024 x 163840 bf16 66 us (5.1 TB/s), gated 64 x 4096 x 2 x 8192 e4m3 19.7 us (3.4 TB/s).
 #include "linear_tc.cuh"
 
 #include <cooperative_groups.h>
@@ -29,7 +32,7 @@ constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8;
 // shared memory for stages, or for the sums of up to FEW tokens, of a CTA that has an SM to itself, and of one that shares it (228 KB an SM,
 // less 1 KB a CTA that the system takes, 1 KB of barriers and 1 KB to align the stages)
 constexpr int ROOM = 225 * 1024, HALF_ROOM = 111 * 1024;
-constexpr uint32_t POLLS = 1u << 22;
+constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum may run over 2^24 values: 0.1 s)
 
 struct Maps {
   CUtensorMap w[2], x;
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   const int quarter = warp & 3;
   const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
   const int n = n0 + 32 * quarter + lane;
-  const bool ok = tc::mbar_wait(&done, 0, POLLS) && !fail;
+  const bool ok = tc::mbar_wait(&done, 0, SUM_POLLS) && !fail;
   if (!ok && lane == 0) atomicExch(&g_linear_few_status, 1);
   tc::fence_after_sync();
   if (p.ck == 1) {
@@ -250,23 +253,41 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
     cg::cluster_group cl = cg::this_cluster();
     const float* part = reinterpret_cast<const float*>(sm);
     cl.sync();
-    const int total = tokens * (ROWS / 4);
-#pragma unroll 2
-    for (int i = rank * NT + tid; i < total; i += p.ck * NT) {
-      float g[4] = {}, u[4] = {};
-#pragma unroll 4
-      for (int c = 0; c < p.ck; ++c) {
-        const float4* o = reinterpret_cast<const float4*>(cl.map_shared_rank(part, c));
-        const float4 a = o[i];
-        g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
-        if (GATED) {
-          const float4 b = o[p.mp * (ROWS / 4) + i];
-          u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+    // (eight vectors of every sum on their way together)
+    auto join = [&](auto ck) {
+      constexpr int CK = decltype(ck)::value, U = 8 / CK, H = GATED ? 2 : 1;
+      const float4* o[CK];
+#pragma unroll
+      for (int c = 0; c < CK; ++c) o[c] = reinterpret_cast<const float4*>(cl.map_shared_rank(part, c));
+      const int total = tokens * (ROWS / 4), stride = CK * NT;
+      for (int i0 = rank * NT + tid; i0 < total; i0 += U * stride) {
+        float4 v[U][H][CK];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+          if (i0 + k * stride < total)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+              for (int c = 0; c < CK; ++c) v[k][h][c] = o[c][h * p.mp * (ROWS / 4) + i0 + k * stride];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int i = i0 + k * stride;
+          const long long c0 = n0 + i % (ROWS / 4) * 4;
+          if (i >= total || c0 >= p.N) continue;
+          float s[2][4] = {};
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int c = 0; c < CK; ++c) {
+              s[h][0] += v[k][h][c].x; s[h][1] += v[k][h][c].y; s[h][2] += v[k][h][c].z; s[h][3] += v[k][h][c].w;
+            }
+          finish4<GATED>(p.e, i / (ROWS / 4), c0, p.N, s[0], s[1]);
         }
       }
-      const long long c = n0 + i % (ROWS / 4) * 4;
-      if (c < p.N) finish4<GATED>(p.e, i / (ROWS / 4), c, p.N, g, u);
-    }
+    };
+    if (p.ck == 2) join(std::integral_constant<int, 2>());
+    else if (p.ck == 4) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, 8>());
     cl.sync();   // (the others may still read this CTA's sums)
   }
 }
@@ -292,9 +313,12 @@ int launch(const Product& p, cudaStream_t st) {
   while (a.ck < 8 && a.tiles_n * a.ck * 2 <= 148 && a.steps >= a.ck * 4) a.ck *= 2;
   a.per = (a.steps + a.ck - 1) / a.ck;
   a.stage = ROWS * 128 * (GATED ? 2 : 1) + a.mp * 128;
-  // two CTAs an SM, unless that leaves a CTA fewer than three stages
+  // Two CTAs an SM while that leaves a CTA three stages (gated, 64 x 4096 x 32000: 91 us either way, 48 of it for 8 bits
+  // against 52); of a split K five, as there is a CTA for every SM at most (64 x 8192 x 4096: 17.7 us with three, 16.4 alone on
+  // the SM with seven); clusters of eight always, which the SMs of a GPC hold only twice otherwise (32 x 16384 x 2048 16.2 us
+  // against 26.2).
   int room = HALF_ROOM;
-  if (room / a.stage < 3) room = ROOM;
+  if (a.ck < 8 && room / a.stage < (a.ck > 1 ? 5 : 3)) room = ROOM;
   a.stages = room / a.stage < MAX_STAGES ? room / a.stage : MAX_STAGES;
   if (a.stages > a.per) a.stages = a.per;
   const int want = a.mp * (GATED ? 2 : 1);
