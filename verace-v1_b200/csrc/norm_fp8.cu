@@ -7,8 +7,8 @@
 // scale NaN or leaves NaN in its place, as in torch.
 //
 // Bound: bytes (7 a value with the residual in 16 bits; 16384 x 4096 bf16 with the residual 71.7 us, 6.55 TB/s, the
-// rate of a copy).  A row stays in the registers of its group of threads: a warp for up to 1024 values, 128 to
-// 1024 threads beyond, 32 values a thread, all loads of a row in flight before its first store; two
+// rate of a copy).  A row stays in the registers of its group of 8 to 1024 threads, 32 values a thread (8 for up to 256
+// values: 56541 x 70 bf16 with the residual 19.0 us, with a warp a row 50), all loads of a row in flight before its first store; two
 // reductions (squares, then magnitudes) by shuffles and, above a warp, one exchange through shared memory each.
 // Rows whose width is no multiple of 8 start anywhere in a 16-byte word: their words are those of the whole
 // tensor, the first and last one masked, so that all but the norm's weights is read and written a word
@@ -76,22 +76,25 @@ __device__ __forceinline__ float rounded(float x) {
 // `shift`, the row's place in its first word, where rows are not WHOLE words.
 template <typename T, int G, bool WHOLE, bool ADD>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a) {
-  constexpr int NT = G < 128 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G / 32;
-  __shared__ float part[2][W > 1 ? W : 1];
-  const int g = threadIdx.x % G;
-  const long long row = (long long)blockIdx.x * (NT / G) + threadIdx.x / G;
+  constexpr int NT = G < 128 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G > 32 ? G / 32 : 1;
+  __shared__ float part[2][NT / G][W > 1 ? W : 1];
+  const int g = threadIdx.x % G, mine = threadIdx.x / G;
+  long long row = (long long)blockIdx.x * (NT / G) + mine;
   lin::depend();
-  if (G < 128 && row >= a.rows) return;   // (whole warps; larger groups are one row a CTA)
+  // a group behind the last row goes along with the others' reductions: a row of no columns
+  const bool act = NT == G || row < a.rows;
+  const int cols = act ? a.cols : 0;
+  if (!act) row = 0;
   const long long off = row * a.cols;
   const T* h = static_cast<const T*>(a.h) + off;
   const T* w = static_cast<const T*>(a.w);
   const int shift = WHOLE ? 0 : (int)(((size_t)h & 15) / sizeof(T));
   auto column = [&](int i) { return VEC * (g + G * i) - shift; };
-  auto any = [&](int i) { return VEC * G * i < a.cols + shift && column(i) < a.cols; };
-  auto in = [&](int c) { return WHOLE || (c >= 0 && c < a.cols); };
+  auto any = [&](int i) { return VEC * G * i < cols + shift && column(i) < cols; };
+  auto in = [&](int c) { return WHOLE || (c >= 0 && c < cols); };
   // whether a vector of p may be moved as one: inside of the row, and p's words where h's are
   auto as_one = [&](const T* p, int c) {
-    return WHOLE || (c >= 0 && c + VEC <= a.cols && ((size_t)(p + off + c) & 15) == 0);
+    return WHOLE || (c >= 0 && c + VEC <= cols && ((size_t)(p + off + c) & 15) == 0);
   };
   auto put = [&](void* to, int c, const float (&v)[VEC]) {
     T* p = static_cast<T*>(to);
@@ -151,13 +154,13 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) ss = fmaf(v[i][j], v[i][j], ss);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    for (int o = G < 32 ? G / 2 : 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if constexpr (W > 1) {
-      if (g % 32 == 0) part[0][g / 32] = ss;
+      if (g % 32 == 0) part[0][mine][g / 32] = ss;
       __syncthreads();
       ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) ss += part[0][i];
+      for (int i = 0; i < W; ++i) ss += part[0][mine][i];
     }
     const float rs = rsqrtf(ss / (float)a.cols + a.eps);
 #pragma unroll
@@ -185,15 +188,15 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
     for (int j = 0; j < VEC; ++j)
       if (in(column(i) + j)) top = max_nan(top, fabsf(v[i][j]));   // (0 rs is NaN where rs is infinite)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = G < 32 ? G / 2 : 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if constexpr (W > 1) {
-    if (g % 32 == 0) part[1][g / 32] = top;
+    if (g % 32 == 0) part[1][mine][g / 32] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < W; ++i) top = max_nan(top, part[1][i]);
+    for (int i = 0; i < W; ++i) top = max_nan(top, part[1][mine][i]);
   }
   const float inv = 448.f / top;
-  if (g == 0) a.scale[row] = top / 448.f;
+  if (g == 0 && act) a.scale[row] = top / 448.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (any(i)) {
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
         o[j] = lo | hi << 16;
       }
       uint8_t* q = a.q + off + c;
-      if (WHOLE || (c >= 0 && c + VEC <= a.cols && (size_t)q % VEC == 0)) {
+      if (WHOLE || (c >= 0 && c + VEC <= cols && (size_t)q % VEC == 0)) {
         if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q) = make_uint2(o[0], o[1]);
         else *reinterpret_cast<uint32_t*>(q) = o[0];
       } else {
@@ -226,7 +229,10 @@ int launch(const NormArgs& a, cudaStream_t st) {
   auto go = [&](auto kernel, long long blocks, int threads) {
     return lin::launch_after("norm_fp8_kernel", kernel, dim3((unsigned)blocks), threads, 0, st, 1, a);
   };
+  if (cols <= 256) return go(norm_fp8_kernel<T, 8, WHOLE, ADD>, (a.rows + 15) / 16, 128);
+  if (cols <= 512) return go(norm_fp8_kernel<T, 16, WHOLE, ADD>, (a.rows + 7) / 8, 128);
   if (cols <= 1024) return go(norm_fp8_kernel<T, 32, WHOLE, ADD>, (a.rows + 3) / 4, 128);
+  if (cols <= 2048) return go(norm_fp8_kernel<T, 64, WHOLE, ADD>, (a.rows + 1) / 2, 128);
   if (cols <= 4096) return go(norm_fp8_kernel<T, 128, WHOLE, ADD>, a.rows, 128);
   if (cols <= 8192) return go(norm_fp8_kernel<T, 256, WHOLE, ADD>, a.rows, 256);
   if (cols <= 16384) return go(norm_fp8_kernel<T, 512, WHOLE, ADD>, a.rows, 512);
