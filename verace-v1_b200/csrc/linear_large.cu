@@ -18,7 +18,7 @@
 // fp32 operands come as three bf16 parts, three stages for 64 values of K (a stage holds one part of A and of B), and
 // the MMAs take six pairs of them, the smallest first.  The tensor core cuts its sums to fp32 after every step instead
 // of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the result); so after every 64 values of K
-// the epilogue's warps add the sums to a third set in TMEM, rounding, while the next 64 run into the other set.
+// the epilogue's warps add them up in registers, rounding, while the next 64 run into the other set.
 //
 // Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
 // applies scales, bias and activation and puts the rounded values into the warp's block of shared memory, from where
@@ -42,6 +42,10 @@ using namespace lin;
 
 constexpr int NT = 384, EPI_WARPS = 8;
 constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum may run over 2^24 values: 0.1 s)
+// 256 columns of parts: four warps give up registers for the epilogue's eight.  What the block was launched with has to cover
+// both shares, or the increase would wait for ever; the host checks the kernel's count before it launches one.
+constexpr int SPLIT_REGISTERS = 168;
+static_assert(128 * 72 + 256 * 216 <= NT * SPLIT_REGISTERS, "the shares' sum");
 constexpr int TURN = 4096;             // a warp's block of the output: 32 rows of 128 bytes
 
 template <int BN>
@@ -317,64 +321,101 @@ __device__ __forceinline__ void scaled(const Epilogue& e, const uint32_t (&r)[U]
   }
 }
 
-// The saved sums of `width` columns, in fp32: 32 columns at a time.
-__device__ __forceinline__ void save_sums(const Epilogue& e, Block b, uint32_t tmem, int width, float rs, const float* col_scale,
-                                          const void* bias, const Target& to, int lane) {
+// Where a block takes its sums from, 16 columns a lot: r, and of gated products the second sums s.
+// TMEM: the next lot is on its way (ask) while one is worked on (have).
+template <bool GATED>
+struct TmemSums {
+  uint32_t at, up;
+  __device__ __forceinline__ void ask(int lot, uint32_t (&r)[16], uint32_t (&s)[16]) const {
+    tmem_ld_async(at + 16 * lot, r);
+    if constexpr (GATED) tmem_ld_async(up + 16 * lot, s);
+  }
+  __device__ __forceinline__ void have(uint32_t (&r)[16], uint32_t (&s)[16]) const {
+    tmem_wait(r);
+    if constexpr (GATED) tmem_wait(s);
+  }
+};
+// local memory (parts): the warp's half of the tile's columns, of gated products half of each sum's; from lot `first` on
+template <bool GATED, int N>
+struct HeldSums {
+  const float* sum;
+  int first;
+  __device__ __forceinline__ void ask(int lot, uint32_t (&r)[16], uint32_t (&s)[16]) const {
+    const float4* f = reinterpret_cast<const float4*>(sum + 16 * (first + lot));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 a = f[j];
+      r[4 * j] = __float_as_uint(a.x); r[4 * j + 1] = __float_as_uint(a.y);
+      r[4 * j + 2] = __float_as_uint(a.z); r[4 * j + 3] = __float_as_uint(a.w);
+      if constexpr (GATED) {
+        const float4 b = f[N / 8 + j];
+        s[4 * j] = __float_as_uint(b.x); s[4 * j + 1] = __float_as_uint(b.y);
+        s[4 * j + 2] = __float_as_uint(b.z); s[4 * j + 3] = __float_as_uint(b.w);
+      }
+    }
+  }
+  __device__ __forceinline__ void have(uint32_t (&)[16], uint32_t (&)[16]) const {}
+};
+
+// The saved sums of `width` columns, in fp32: 32 columns at a time.  UP: the second sums.
+template <bool UP, typename Sums>
+__device__ __forceinline__ void save_sums(const Epilogue& e, Block b, const Sums& sums, int width, float rs,
+                                          const float* col_scale, const void* bias, const Target& to, int lane) {
+#pragma unroll 1
   for (int c = 0; c < width && b.n0 < b.N; c += 32, b.n0 += 32) {
     reclaim(lane);
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < 32; h += 16) {
-      uint32_t r[16];
-      tmem_ld_async(tmem + c + h, r);
-      tmem_wait(r);
+      uint32_t r[16], s[16];
+      sums.ask((c + h) / 16, r, s);
+      sums.have(r, s);
       float v[16];
-      scaled(e, r, v, rs, col_scale, bias, b.n0 + h, b.N);
+      scaled(e, UP ? s : r, v, rs, col_scale, bias, b.n0 + h, b.N);
       put<true>(b, h, v, VERACE_F32, lane);
     }
     write_block<true>(b, to, lane);
   }
 }
 
-// One block from TMEM address `tmem` (the second sums at `tmem_up`) on, its residual in `res`; the sums of
-// the next columns are on their way while one lot is worked on.  `loaded` is called once the
-// block's sums are in registers.
-template <bool GATED, bool WIDE, typename F>
-__device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b, uint32_t tmem, uint32_t tmem_up,
-                                               const uint32_t (&res)[32], const Target& out, const Target& pre,
+// One block, its residual in `res` (AHEAD) or read here.  `loaded` is called once the block's sums are in registers.
+template <bool GATED, bool WIDE, bool AHEAD, typename Sums, typename F>
+__device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b, const Sums& sums,
+                                               const uint32_t (&res)[AHEAD ? 32 : 1], const Target& out, const Target& pre,
                                                const Target& pre_up, int lane, F&& loaded) {
   constexpr int WIDTH = WIDE ? 32 : 64, U = 16, LOTS = WIDTH / U;
   const long long m = b.m0 + lane;
   const float rs = e.row_scale && m < b.M ? e.row_scale[m] : 0.f;
   if (e.pre) {
-    save_sums(e, b, tmem, WIDTH, rs, e.col_scale, GATED ? nullptr : e.bias, pre, lane);
-    if (GATED) save_sums(e, b, tmem_up, WIDTH, rs, e.up_scale, nullptr, pre_up, lane);
+    save_sums<false>(e, b, sums, WIDTH, rs, e.col_scale, GATED ? nullptr : e.bias, pre, lane);
+    if (GATED) save_sums<true>(e, b, sums, WIDTH, rs, e.up_scale, nullptr, pre_up, lane);
   }
   if (GATED && out.p == nullptr) {   // (partial sums: the two above are all)
     loaded();
     return;
   }
   uint32_t r[U], s[U];
-  tmem_ld_async(tmem, r);
-  if constexpr (GATED) tmem_ld_async(tmem_up, s);
+  sums.ask(0, r, s);
   reclaim(lane);
   if (!GATED && e.residual) {
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) set_word(b, i, lane, res[i]);
+      for (int i = 0; i < 32; ++i) set_word(b, i, lane, res[i]);
+    } else {
+      uint32_t w[32];
+      read_words<WIDE>(b, e.residual, e.ld_res, lane, w);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) set_word(b, i, lane, w[i]);
+    }
     __syncwarp();
   }
 #pragma unroll 1
   for (int l = 0; l < LOTS; ++l) {
     float v[U], u[U] = {};
-    tmem_wait(r);
-    if constexpr (GATED) tmem_wait(s);
+    sums.have(r, s);
     scaled(e, r, v, rs, e.col_scale, GATED ? nullptr : e.bias, b.n0 + l * U, b.N);
     if constexpr (GATED) scaled(e, s, u, rs, e.up_scale, nullptr, b.n0 + l * U, b.N);
-    if (l + 1 < LOTS) {
-      tmem_ld_async(tmem + (l + 1) * U, r);
-      if constexpr (GATED) tmem_ld_async(tmem_up + (l + 1) * U, s);
-    } else {
-      loaded();
-    }
+    if (l + 1 < LOTS) sums.ask(l + 1, r, s);
+    else loaded();
     activate<GATED, !WIDE>(e, v, u);
     if (!GATED && e.residual) add<WIDE>(b, l * U, v, e.type, lane);
     put<WIDE>(b, l * U, v, e.type, lane);
@@ -383,7 +424,7 @@ __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b
 }
 
 // A warp's part of every tile of the pair: TMEM lanes 32 (warp % 4) ..., one half of the columns.
-template <bool GATED, bool WIDE, int BN, typename Wait, typename Free>
+template <bool GATED, bool WIDE, int BN, bool PARTS, typename Wait, typename Free>
 __device__ __forceinline__ void epilogue_tiles(const Args& p, const Maps& maps, uint32_t turn, uint32_t tmem, int pair, int pairs, int rank,
                                                int warp, int lane, Wait&& wait, Free&& release) {
   constexpr int HB = BN / 2, TN = GATED ? HB : BN, WIDTH = WIDE ? 32 : 64, PER = TN / 2 > WIDTH ? TN / 2 : WIDTH;
@@ -405,30 +446,39 @@ __device__ __forceinline__ void epilogue_tiles(const Args& p, const Maps& maps, 
     Target pre{p.pre_by_tma ? &maps.pre[0] : nullptr, z, p.e.pre ? p.e.pre + first_of : nullptr, p.e.ld};
     Target pre_up{p.pre_by_tma ? &maps.pre[1] : nullptr, z, p.e.pre_up ? p.e.pre_up + first_of : nullptr, p.e.ld};
     if (!GATED && p.splits > 1) out.p = static_cast<float*>(p.e.out) + first_of;
-    uint32_t res[32];
-    if (!GATED && p.e.residual && b.m0 < b.M && b.n0 < b.N && first < last)   // on its way while the products run
-      read_words<WIDE>(b, p.e.residual, p.e.ld_res, lane, res);
-    const int set = wait(n);
+    constexpr bool AHEAD = !PARTS;   // residuals on their way while the products run (parts' sums leave no registers for them)
+    uint32_t res[AHEAD ? 32 : 1];
+    if constexpr (AHEAD)
+      if (!GATED && p.e.residual && b.m0 < b.M && b.n0 < b.N && first < last)
+        read_words<WIDE>(b, p.e.residual, p.e.ld_res, lane, res);
+    __align__(16) float held_sums[PARTS ? BN / 2 : 4];
+    const int set = wait(n, held_sums);
     if (set < 0) break;
     const uint32_t sums = lanes + set;
     bool held = true;
     for (int c = first; c < last; c += WIDTH) {
       b.n0 = (long long)at.n * TN + c;
       if (b.m0 >= b.M || b.n0 >= b.N) break;
-      uint32_t next[32];
       Block after = b;
       after.n0 += WIDTH;
       const bool more = c + WIDTH < last && after.n0 < b.N;
-      if (!GATED && p.e.residual && more) read_words<WIDE>(after, p.e.residual, p.e.ld_res, lane, next);
-      epilogue_block<GATED, WIDE>(p.e, b, sums + c, sums + HB + c, res, out, pre, pre_up, lane, [&] {
+      auto loaded = [&] {
         if (!more) {
           release(n);
           held = false;
         }
-      });
-      if (!GATED && p.e.residual)
+      };
+      if constexpr (PARTS) {
+        epilogue_block<GATED, WIDE, false>(p.e, b, HeldSums<GATED, BN / 2>{held_sums, (c - first) / 16}, res, out, pre, pre_up,
+                                           lane, loaded);
+      } else {
+        uint32_t next[32];
+        if (!GATED && p.e.residual && more) read_words<WIDE>(after, p.e.residual, p.e.ld_res, lane, next);
+        epilogue_block<GATED, WIDE, true>(p.e, b, TmemSums<GATED>{sums + c, sums + HB + c}, res, out, pre, pre_up, lane, loaded);
+        if (!GATED && p.e.residual)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) res[i] = next[i];
+          for (int i = 0; i < 32; ++i) res[i] = next[i];
+      }
     }
     if (held) release(n);
   }
@@ -441,8 +491,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   using S = Shape<BN>;
   constexpr int KB = F8 ? 128 : 64;            // values of K in a stage
   constexpr int HB = BN / 2;                   // rows of B in a CTA
-  constexpr int COLS = PARTS || BN == 256 ? 512 : 256;   // of TMEM: two sets of sums, of parts a third
-  static_assert(!PARTS || BN == 128, "three sets of sums");
+  constexpr int COLS = 2 * BN;                 // of TMEM: two sets of sums
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((size_t)raw + 1023) & ~(size_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::BARS);
@@ -484,6 +533,8 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   // the last one's may be empty)
   const int sets = PARTS ? p.per * p.segments : 1;
 
+  if (warp < 4) {
+  if constexpr (PARTS && BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");   // (see SPLIT_REGISTERS)
   if (warp == 0) {
     if (lane == 0) {   // ---- operands
       int i = 0, flying = 0;
@@ -612,7 +663,9 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
         if (lane == 0) atomicExch(&g_linear_status, 1);
       }
     }
-  } else if (warp >= 4) {   // ---- epilogue
+  }
+  } else {   // ---- epilogue
+    if constexpr (PARTS && BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const uint32_t turn = tc::smem_addr(sm + S::TURNS + (warp - 4) * TURN);
     auto filled = [&](int n) {
       if (!tc::mbar_wait(&acc_full[n & 1], (n >> 1) & 1, SUM_POLLS)) {
@@ -628,51 +681,50 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       __syncwarp();
       if (lane == 0) arrive_at(in_cta0(&acc_empty[n & 1]));
     };
-    // tile n's sums: the TMEM column of their set, or -1
-    auto wait = [&](int n) {
-      if constexpr (!PARTS) return filled(n) ? (n & 1) * BN : -1;
-      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-      const int k0 = place(p, pair + n * pairs).split * p.per;
-      for (int c = 0; c < sets; ++c) {
-        const int set = n * sets + c;
-        if (!filled(set)) return -1;
-        if (k0 + c / p.segments < p.kblocks) {
+    // tile n's sums: the TMEM column of their set, or -1; of parts in `sum`, the warp's half of the columns (gated: of
+    // both sums)
+    auto wait = [&](int n, auto& sum) {
+      if constexpr (!PARTS) {
+        return filled(n) ? (n & 1) * BN : -1;
+      } else {
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const int k0 = place(p, pair + n * pairs).split * p.per;
+        auto col = [&](int h) {
+          return GATED ? (h >= HB / 2 ? HB / 2 + h : h) + (warp >= 8 ? HB / 2 : 0) : h + (warp >= 8 ? HB : 0);
+        };
+        float acc[HB] = {};   // (in registers: no index but constants; `sum`, which the epilogue walks, is in local memory)
 #pragma unroll 1
-          for (int h = 0; h < BN / 2; h += 32) {   // the warp's half of the columns (gated: of both sums)
-            const int col = GATED ? (h >= HB / 2 ? HB / 2 + h : h) + (warp >= 8 ? HB / 2 : 0) : h + (warp >= 8 ? HB : 0);
-            uint32_t r[16], s[16], r1[16], s1[16];
-            tmem_ld_async(lanes + (set & 1) * BN + col, r);
-            tmem_ld_async(lanes + (set & 1) * BN + col + 16, r1);
-            if (c > 0) {
-              tmem_ld_async(lanes + 2 * BN + col, s);
-              tmem_ld_async(lanes + 2 * BN + col + 16, s1);
+        for (int c = 0; c < sets; ++c) {
+          const int set = n * sets + c;
+          if (!filled(set)) return -1;
+          if (k0 + c / p.segments < p.kblocks) {   // (a last split's missing stages)
+#pragma unroll
+            for (int h = 0; h < HB; h += 32) {
+              uint32_t r[16], s[16];
+              tmem_ld_async(lanes + (set & 1) * BN + col(h), r);
+              tmem_ld_async(lanes + (set & 1) * BN + col(h + 16), s);
+              tmem_wait(r);
               tmem_wait(s);
-              tmem_wait(s1);
-            }
-            tmem_wait(r);
-            tmem_wait(r1);
-            if (c > 0) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(s[j]));
-                r1[j] = __float_as_uint(__uint_as_float(r1[j]) + __uint_as_float(s1[j]));
+                acc[h + j] += __uint_as_float(r[j]);
+                acc[h + 16 + j] += __uint_as_float(s[j]);
               }
             }
-            tmem_st(lanes + 2 * BN + col, r);
-            tmem_st(lanes + 2 * BN + col + 16, r1);
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          free(set);
         }
-        free(set);
+#pragma unroll
+        for (int i = 0; i < HB; ++i) sum[i] = acc[i];
+        return 0;
       }
-      return 2 * BN;
     };
     auto release = [&](int n) {
       if (!PARTS) free(n);
     };
-    if (PARTS) epilogue_tiles<GATED, true, BN>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
-    else if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
-    else epilogue_tiles<GATED, false, BN>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    if constexpr (PARTS) epilogue_tiles<GATED, true, BN, true>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN, false>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else epilogue_tiles<GATED, false, BN, false>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -736,6 +788,12 @@ int launch(const Product& p, int splits, cudaStream_t st) {
   VERACE_CUDA(cudaGetDevice(&dev));
   static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
   if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (PARTS && BN == 256) {
+      cudaFuncAttributes fa;
+      VERACE_CUDA(cudaFuncGetAttributes(&fa, kern));
+      VERACE_REQUIRE(fa.numRegs == SPLIT_REGISTERS, VERACE_ERR_UNSUPPORTED, "linear: %d registers where %d are shared out",
+                     fa.numRegs, SPLIT_REGISTERS);
+    }
     VERACE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
@@ -745,11 +803,9 @@ int launch(const Product& p, int splits, cudaStream_t st) {
 
 template <int BN>
 int by_kind(const Product& p, int s, cudaStream_t st) {
-  if constexpr (BN == 128) {
-    if (p.parts && p.gated) return launch<false, false, false, true, BN, true>(p, s, st);
-    if (p.parts && p.a_mn) return launch<false, true, true, false, BN, true>(p, s, st);
-    if (p.parts) return p.b_mn ? launch<false, false, true, false, BN, true>(p, s, st) : launch<false, false, false, false, BN, true>(p, s, st);
-  }
+  if (p.parts && p.gated) return launch<false, false, false, true, BN, true>(p, s, st);
+  if (p.parts && p.a_mn) return launch<false, true, true, false, BN, true>(p, s, st);
+  if (p.parts) return p.b_mn ? launch<false, false, true, false, BN, true>(p, s, st) : launch<false, false, false, false, BN, true>(p, s, st);
   if (p.type == VERACE_E4M3)
     return p.gated ? launch<true, false, false, true, BN>(p, s, st) : launch<true, false, false, false, BN>(p, s, st);
   if (p.gated) return launch<false, false, false, true, BN>(p, s, st);
@@ -784,22 +840,23 @@ __global__ void __launch_bounds__(256) join_splits(const float* __restrict__ par
 }
 
 // How a product is cut: columns of a tile, and splits of K.  A pair's time in clocks: a step of four
-// MMAs takes 512 (BN 256) or 400 (BN 128, bound by the 24 KB that each CTA loads for it), one of parts 1600, an epilogue about 40 a column (under the next tile's products but for
+// MMAs takes 512 (BN 256) or 400 (BN 128, bound by
+// shared memory: 8 KB for 64 clocks of an MMA), 64 values of parts 3200 or 2900, an epilogue about 40 a column (under the next tile's products but for
 // the last), the first operands 6000; partial sums are written and read at about 2 KB a clock, and joining them takes another launch (5000).
 struct Cut {
   int bn, splits;
 };
 Cut cut(long long M, long long N, long long K, int segments, int nz, bool gated, int type, bool parts) {
   const long long kblocks = (K + (type == VERACE_E4M3 ? 127 : 63)) / (type == VERACE_E4M3 ? 128 : 64);
-  Cut best{parts ? 128 : 256, 1};
+  Cut best{256, 1};
   double least = 0;
-  for (int bn = parts ? 128 : 256; bn >= 128; bn /= 2) {
+  for (int bn = 256; bn >= 128; bn /= 2) {
     const int tn = gated ? bn / 2 : bn;
     const long long tiles = (M + 255) / 256 * ((N + tn - 1) / tn) * nz;
     for (int s = 1; s <= 16 && (s == 1 || (s * tiles <= 74 && kblocks >= 8 * s)); ++s) {
       const long long stages = (kblocks + s - 1) / s;
       if ((s - 1) * stages >= kblocks) continue;      // (a split would be empty)
-      const double per = (double)stages * segments * (parts ? 1600 : bn == 256 ? 512 : 400), epi = 40. * bn;
+      const double per = (double)stages * segments * (parts ? bn == 256 ? 3200 : 2900 : bn == 256 ? 512 : 400), epi = 40. * bn;
       double t = (double)((tiles * s + 73) / 74) * (per > epi ? per : epi) + epi + 6000;
       if (s > 1) t += 5000 + (double)M * N * nz * (gated ? 8 : 4) * 2 * s / 2048;
       if (least == 0 || t < least) least = t, best = Cut{bn, s};
