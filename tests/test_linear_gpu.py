@@ -347,6 +347,47 @@ def test_captured_in_a_graph(m, dt):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_captured_between_streams_and_copies(m):
+    """In a graph behind a copy, a join of two streams and kernels of torch's own."""
+    g = gen(m, 24)
+    x, w, w2 = randn(g, m, 128, dt=BF16), weight(g, 128, 128, BF16), weight(g, 128, 128, BF16)
+    norm = torch.nn.RMSNorm(128, eps=1e-6, device="cuda", dtype=BF16).requires_grad_(False)
+    into, side = torch.empty_like(x), torch.cuda.Stream()
+
+    def work():
+        into.copy_(x)
+        a = V.fused_linear(into, w)
+        here, there = torch.cuda.Event(), torch.cuda.Event()
+        here.record()
+        with torch.cuda.stream(side):
+            side.wait_event(here)
+            b = V.gated_linear(a, w, w2)
+            there.record()
+        c = V.fused_linear(a, w2, activation="silu")
+        torch.cuda.current_stream().wait_event(there)
+        q, s = V.add_rmsnorm_fp8(c, b, norm)
+        y = V.fused_linear(c + b, w, residual=b)
+        return a, b, c, y, q.view(torch.uint8), s
+    first = torch.cuda.Stream()
+    first.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(first):
+        work()
+    torch.cuda.current_stream().wait_stream(first)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    x.copy_(randn(g, m, 128, dt=BF16))
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    kept = [t.clone() for t in got]
+    want = work()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(kept, want))
+
+
 def test_rows_behind_the_output_stay():
     """Nothing is written outside of the output: its allocation's neighbours keep their values."""
     g = gen(17)
@@ -487,6 +528,8 @@ def test_refusals():
         V.fused_linear(x, w.float())
     with pytest.raises(AssertionError, match="weights"):
         V.fused_linear(x, w.cpu())
+    with pytest.raises(AssertionError, match="two dimensions"):
+        V.gated_linear(x, w[0], w[0])
     with pytest.raises(ValueError, match="scales"):
         V.fused_linear(q, wq, x_scale=s)
     with pytest.raises(ValueError, match="scales"):

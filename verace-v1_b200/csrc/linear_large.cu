@@ -25,9 +25,9 @@
 // TMA stores them; rows that are not 16-byte aligned are stored word by word, the warp along a row.  Residuals come
 // into the block that way too, fetched while the products run.
 //
-// Measured on the device: gated 8192 x 4096 x 2 x 8192 bf16 699 us (1.57 PFLOP/s, the tensor pipe 96 % active; a second of
-// such calls runs into the power limit, 800 us), 8192 x 8192 x 4096 e4m3 191 us (2.9 PFLOP/s; bound by what the CTAs load,
-// 32 KB each for 256 clocks of MMAs), 8192 x 1024 x 4096 bf16 48 us (1.42), 4096^3 fp32 676 us (203 TFLOP/s).
+// Measured on the device: gated 8192 x 4096 x 2 x 8192 bf16 690 us (1.59 PFLOP/s, the tensor pipe 96 % active; a second of
+// such calls runs into the power limit, 800 us), 8192 x 8192 x 4096 e4m3 188 us (2.9 PFLOP/s; bound by what the CTAs load,
+// 32 KB each for 256 clocks of MMAs), 8192 x 1024 x 4096 bf16 48 us (1.42), 4096^3 fp32 607 us (226 TFLOP/s).
 #include "linear_tc.cuh"
 
 #include <atomic>
@@ -534,136 +534,136 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
   const int sets = PARTS ? p.per * p.segments : 1;
 
   if (warp < 4) {
-  if constexpr (PARTS && BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");   // (see SPLIT_REGISTERS)
-  if (warp == 0) {
-    if (lane == 0) {   // ---- operands
-      int i = 0, flying = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = pair; t < p.tiles && ok; t += pairs) {
-        const Place at = place(p, t);
-        const int m0 = at.m * 256 + (int)rank * 128;
-        const int n0 = GATED ? at.n * HB : at.n * BN + (int)rank * HB;
-        const int k0 = at.split * p.per, k1 = min(k0 + p.per, p.kblocks);
-        // (segment by segment; of parts 64 values of K of every segment, then the next)
-        const int outer = PARTS ? k1 - k0 : p.segments, inner = PARTS ? 3 * p.segments : k1 - k0;
-        for (int u = 0; u < outer && ok; ++u) {
-          for (int v = 0; v < inner; ++v) {
-            const int s = PARTS ? v / 3 : u, kb = k0 + (PARTS ? u : v), part = PARTS ? v % 3 : 0;
-            const CUtensorMap* mb = &maps.b[GATED ? rank : s];
-            const int az = part * p.a_step + p.a_first + s + at.z;
-            if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
-              ok = false;
-              break;
-            }
-            if (rank == 0) tc::mbar_expect_tx(&full[i], 2 * S::STAGE);
-            const uint32_t bar = in_cta0(&full[i]);
-            unsigned char* a = sm + i * S::STAGE;
-            unsigned char* b = a + 16384;
-            if constexpr (AMN) {
-              load_box(a, &maps.a, m0, kb * KB, az, bar);
-              load_box(a + 8192, &maps.a, m0 + 64, kb * KB, az, bar);
-            } else {
-              load_box(a, &maps.a, kb * KB, m0, az, bar);
-            }
-            if constexpr (BMN) {
+    if constexpr (PARTS && BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");   // (see SPLIT_REGISTERS)
+    if (warp == 0) {
+      if (lane == 0) {   // ---- operands
+        int i = 0, flying = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = pair; t < p.tiles && ok; t += pairs) {
+          const Place at = place(p, t);
+          const int m0 = at.m * 256 + (int)rank * 128;
+          const int n0 = GATED ? at.n * HB : at.n * BN + (int)rank * HB;
+          const int k0 = at.split * p.per, k1 = min(k0 + p.per, p.kblocks);
+          // (segment by segment; of parts 64 values of K of every segment, then the next)
+          const int outer = PARTS ? k1 - k0 : p.segments, inner = PARTS ? 3 * p.segments : k1 - k0;
+          for (int u = 0; u < outer && ok; ++u) {
+            for (int v = 0; v < inner; ++v) {
+              const int s = PARTS ? v / 3 : u, kb = k0 + (PARTS ? u : v), part = PARTS ? v % 3 : 0;
+              const CUtensorMap* mb = &maps.b[GATED ? rank : s];
+              const int az = part * p.a_step + p.a_first + s + at.z;
+              if (!tc::mbar_wait(&empty[i], phase ^ 1, POLLS)) {   // (a fresh barrier lets the first round through)
+                ok = false;
+                break;
+              }
+              if (rank == 0) tc::mbar_expect_tx(&full[i], 2 * S::STAGE);
+              const uint32_t bar = in_cta0(&full[i]);
+              unsigned char* a = sm + i * S::STAGE;
+              unsigned char* b = a + 16384;
+              if constexpr (AMN) {
+                load_box(a, &maps.a, m0, kb * KB, az, bar);
+                load_box(a + 8192, &maps.a, m0 + 64, kb * KB, az, bar);
+              } else {
+                load_box(a, &maps.a, kb * KB, m0, az, bar);
+              }
+              if constexpr (BMN) {
 #pragma unroll
-              for (int h = 0; h < HB / 64; ++h) load_box(b + h * 8192, mb, n0 + 64 * h, kb * KB, part, bar);
-            } else {
-              load_box(b, mb, kb * KB, n0, part, bar);
-            }
-            if (++i == S::STAGES) i = 0, phase ^= 1;
-            flying = min(flying + 1, S::STAGES);
-          }
-        }
-      }
-      if (!ok) {
-        *fail = 1;
-        atomicExch(&g_linear_status, 1);
-      }
-      // copies in flight land before the CTA may end (the first CTA's barriers count both CTAs'; the
-      // second one stays for the first at the cluster's barrier below)
-      if (rank == 0)
-        while (flying-- > 0) {
-          if (i == 0) i = S::STAGES, phase ^= 1;
-          tc::mbar_wait(&full[--i], phase, POLLS);
-        }
-    }
-  } else if (warp == 1) {
-    if (rank == 0) {   // ---- MMAs of the pair.  The whole warp walks the loop, so that the operands sit in uniform registers:
-      // by one thread's own loop a step of four MMAs took 657 clocks, the MMAs themselves take 512
-      const bool lead = elect();
-      int i = 0, n = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const int mine = (p.tiles - pair + pairs - 1) / pairs * sets;   // sets to fill
-      // four MMAs: 128 bytes of K of stage ia's A and stage ib's B
-      auto step = [&](uint32_t d, int ia, int ib, bool more) {
-        const uint32_t a = tc::smem_addr(sm + ia * S::STAGE), bb = tc::smem_addr(sm + ib * S::STAGE) + 16384;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
-          const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
-          const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
-          mma_pair<F8>(d, da, db, p.idesc, more || k > 0 ? 1u : 0u);
-        }
-      };
-      for (; n < mine && ok; ++n) {
-        const int b = n & 1, use = n >> 1;
-        const int k0 = place(p, pair + n / sets * pairs).split * p.per;
-        const int steps = PARTS ? k0 + n % sets / p.segments < p.kblocks : p.segments * (min(k0 + p.per, p.kblocks) - k0);
-        if (!tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
-          ok = false;
-          break;
-        }
-        tc::fence_after_sync();
-        const uint32_t d = tmem + b * BN;
-        for (int s = 0; s < steps; ++s) {
-          if constexpr (!PARTS) {
-            if (!tc::mbar_wait(&full[i], phase, POLLS)) {
-              ok = false;
-              break;
-            }
-            tc::fence_after_sync();
-            if (lead) {
-              step(d, i, i, s > 0);
-              commit_pair(&empty[i]);
-            }
-            __syncwarp();
-            if (++i == S::STAGES) i = 0, phase ^= 1;
-          } else {
-            int at[3];
-            for (int j = 0; j < 3 && ok; ++j) {
-              at[j] = i;
-              ok = tc::mbar_wait(&full[i], phase, POLLS);
+                for (int h = 0; h < HB / 64; ++h) load_box(b + h * 8192, mb, n0 + 64 * h, kb * KB, part, bar);
+              } else {
+                load_box(b, mb, kb * KB, n0, part, bar);
+              }
               if (++i == S::STAGES) i = 0, phase ^= 1;
+              flying = min(flying + 1, S::STAGES);
             }
-            if (!ok) break;
-            tc::fence_after_sync();
-            if (lead) {   // parts: 0 the high one
-              step(d, at[2], at[0], false);
-              step(d, at[1], at[1], true);
-              step(d, at[0], at[2], true);
-              commit_pair(&empty[at[2]]);
-              step(d, at[1], at[0], true);
-              step(d, at[0], at[1], true);
-              commit_pair(&empty[at[1]]);
-              step(d, at[0], at[0], true);
-              commit_pair(&empty[at[0]]);
-            }
-            __syncwarp();
           }
         }
-        if (lead) commit_pair(&acc_full[b]);   // (also after a failure: every MMA issued completes)
-        __syncwarp();
-        if (!ok) tc::mbar_wait(&acc_full[b], use & 1, POLLS);
+        if (!ok) {
+          *fail = 1;
+          atomicExch(&g_linear_status, 1);
+        }
+        // copies in flight land before the CTA may end (the first CTA's barriers count both CTAs'; the
+        // second one stays for the first at the cluster's barrier below)
+        if (rank == 0)
+          while (flying-- > 0) {
+            if (i == 0) i = S::STAGES, phase ^= 1;
+            tc::mbar_wait(&full[--i], phase, POLLS);
+          }
       }
-      if (!ok) {
-        *fail = 1;
-        if (lane == 0) atomicExch(&g_linear_status, 1);
+    } else if (warp == 1) {
+      if (rank == 0) {   // ---- MMAs of the pair.  The whole warp walks the loop, so that the operands sit in uniform registers:
+        // by one thread's own loop a step of four MMAs took 657 clocks, the MMAs themselves take 512
+        const bool lead = elect();
+        int i = 0, n = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const int mine = (p.tiles - pair + pairs - 1) / pairs * sets;   // sets to fill
+        // four MMAs: 128 bytes of K of stage ia's A and stage ib's B
+        auto step = [&](uint32_t d, int ia, int ib, bool more) {
+          const uint32_t a = tc::smem_addr(sm + ia * S::STAGE), bb = tc::smem_addr(sm + ib * S::STAGE) + 16384;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
+            const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
+            const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
+            mma_pair<F8>(d, da, db, p.idesc, more || k > 0 ? 1u : 0u);
+          }
+        };
+        for (; n < mine && ok; ++n) {
+          const int b = n & 1, use = n >> 1;
+          const int k0 = place(p, pair + n / sets * pairs).split * p.per;
+          const int steps = PARTS ? k0 + n % sets / p.segments < p.kblocks : p.segments * (min(k0 + p.per, p.kblocks) - k0);
+          if (!tc::mbar_wait(&acc_empty[b], (use & 1) ^ 1, POLLS)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+          const uint32_t d = tmem + b * BN;
+          for (int s = 0; s < steps; ++s) {
+            if constexpr (!PARTS) {
+              if (!tc::mbar_wait(&full[i], phase, POLLS)) {
+                ok = false;
+                break;
+              }
+              tc::fence_after_sync();
+              if (lead) {
+                step(d, i, i, s > 0);
+                commit_pair(&empty[i]);
+              }
+              __syncwarp();
+              if (++i == S::STAGES) i = 0, phase ^= 1;
+            } else {
+              int at[3];
+              for (int j = 0; j < 3 && ok; ++j) {
+                at[j] = i;
+                ok = tc::mbar_wait(&full[i], phase, POLLS);
+                if (++i == S::STAGES) i = 0, phase ^= 1;
+              }
+              if (!ok) break;
+              tc::fence_after_sync();
+              if (lead) {   // parts: 0 the high one
+                step(d, at[2], at[0], false);
+                step(d, at[1], at[1], true);
+                step(d, at[0], at[2], true);
+                commit_pair(&empty[at[2]]);
+                step(d, at[1], at[0], true);
+                step(d, at[0], at[1], true);
+                commit_pair(&empty[at[1]]);
+                step(d, at[0], at[0], true);
+                commit_pair(&empty[at[0]]);
+              }
+              __syncwarp();
+            }
+          }
+          if (lead) commit_pair(&acc_full[b]);   // (also after a failure: every MMA issued completes)
+          __syncwarp();
+          if (!ok) tc::mbar_wait(&acc_full[b], use & 1, POLLS);
+        }
+        if (!ok) {
+          *fail = 1;
+          if (lane == 0) atomicExch(&g_linear_status, 1);
+        }
       }
     }
-  }
   } else {   // ---- epilogue
     if constexpr (PARTS && BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const uint32_t turn = tc::smem_addr(sm + S::TURNS + (warp - 4) * TURN);
@@ -839,10 +839,10 @@ __global__ void __launch_bounds__(256) join_splits(const float* __restrict__ par
   finish4<GATED>(e, m, c, N, g, u);
 }
 
-// How a product is cut: columns of a tile, and splits of K.  A pair's time in clocks: a step of four
-// MMAs takes 512 (BN 256) or 400 (BN 128, bound by
-// shared memory: 8 KB for 64 clocks of an MMA), 64 values of parts 3200 or 2900, an epilogue about 40 a column (under the next tile's products but for
-// the last), the first operands 6000; partial sums are written and read at about 2 KB a clock, and joining them takes another launch (5000).
+// How a product is cut: columns of a tile, and splits of K.  A pair's time in clocks: a step of four MMAs takes 512
+// (BN 256) or 400 (BN 128, bound by shared memory: 8 KB for 64 clocks of an MMA), 64 values of parts 3200 or
+// 2900, an epilogue about 40 a column (under the next tile's products but for the last), the first operands
+// 6000; partial sums are written and read at about 2 KB a clock, and joining them takes another launch (5000).
 struct Cut {
   int bn, splits;
 };

@@ -61,6 +61,7 @@ def _checked(who, x, weight, scales, want, activation, allowed, out_dtype, defau
     """Checks what both products take (``scales`` of ``want`` are given); returns (activation, k, n, out dtype)."""
     dt = x.dtype
     act = allowed.get(activation)
+    assert weight.dim() == 2, f"{who}: the weights must have two dimensions"
     shape, (n, k) = x.shape, weight.shape
     if dt not in _CODE:
         raise ValueError(f"{who}: {dt} inputs (expected fp32, bf16, fp16 or float8_e4m3fn)")
