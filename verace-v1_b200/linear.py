@@ -13,6 +13,7 @@ addition (verace_v1/modules/mcmoe.py:85-120, backbone.py:96-99).
 fp32, bf16 and fp16 operands have gradients; e4m3 operands (with scales) are for inference.
 """
 import contextlib
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -86,6 +87,12 @@ def _checked(who, x, weight, scales, want, activation, allowed, out_dtype, defau
     return act, k, n, out_dtype
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, m: int, n: int, k: int, code: int) -> int:
+    """What the workspace query says, which depends on the sizes and the type alone."""
+    return getattr(lib(), query)(m, n, k, code)
+
+
 def _workspace(nbytes: int, device):
     return torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device) if nbytes else None
 
@@ -109,7 +116,7 @@ def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, w
     pre = torch.empty_strided((m, n), (n, 1), dtype=torch.float32, device=dev) if want_pre else None
     L = lib()
     code = _CODE[x2.dtype]
-    nws = L.verace_linear_workspace(m, n, k, code)
+    nws = _workspace_bytes("verace_linear_workspace", m, n, k, code)
     ws = _workspace(nws, dev)
     rc = L.verace_linear(x2.data_ptr(), ldx, _p(sx), w2.data_ptr(), ldw, _p(sw), _p(bias), _p(res), ldr, y.data_ptr(),
                          _p(pre), m, n, k, act, code, _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index))
@@ -134,7 +141,7 @@ def _fused_linear_backward(ctx, d):
         d2 = d.contiguous()
         L = lib()
         code = _DTYPE[dt]
-        nws = L.verace_linear_backward_workspace(m, n, k, code)
+        nws = _workspace_bytes("verace_linear_backward_workspace", m, n, k, code)
         ws = _workspace(nws, dev)
         with _on(dev):
             rc = L.verace_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(pre), _p(dx), _p(dw),
@@ -250,7 +257,7 @@ def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, wa
         up = torch.empty_strided((m, f), (f, 1), dtype=torch.float32, device=dev)
     L = lib()
     code = _CODE[x2.dtype]
-    nws = L.verace_gated_linear_workspace(m, f, k, code)
+    nws = _workspace_bytes("verace_gated_linear_workspace", m, f, k, code)
     ws = _workspace(nws, dev)
     rc = L.verace_gated_linear(x2.data_ptr(), ldx, _p(sx), g2.data_ptr(), u2.data_ptr(), ldw, _p(sg), _p(su), h.data_ptr(),
                                _p(gate), _p(up), m, f, k, act, b1, b2, code, _DTYPE[out_dtype], _p(ws), nws,
@@ -271,7 +278,7 @@ def _gated_linear_backward(ctx, d):
     d2 = d.contiguous()
     L = lib()
     code = _DTYPE[dt]
-    nws = L.verace_gated_linear_backward_workspace(m, f, k, code)
+    nws = _workspace_bytes("verace_gated_linear_backward_workspace", m, f, k, code)
     ws = _workspace(nws, dev)
     with _on(dev):
         rc = L.verace_gated_linear_backward(d2.data_ptr(), x2.data_ptr(), ldx, g2.data_ptr(), u2.data_ptr(), ldw,
