@@ -11,8 +11,9 @@
 // row, so neighbouring threads store neighbouring outputs of a token.  The input gradient of few tokens
 // (a_mn: weights stored [K][N], read as MN-major) runs here too, for a gated block over both weights.
 //
-// Measured in chains of calls: 7 x 8192 x 4096 fp16 15.3 us (4.4 TB/s, 5 us of it set-up, first loads and the join),
-// 32 x 1024 x 163840 bf16 66 us (5.1 TB/s), gated 64 x 4096 x 2 x 8192 e4m3 19.7 us (3.4 TB/s).
+// Measured in chains of calls: 7 x 8192 x 4096 fp16 15.0 us (4.5 TB/s, 5 us of it set-up, first loads and the join),
+// 16 x 1024 x 163840 bf16 63 us (5.3 TB/s), gated 64 x 4096 x 2 x 8192 e4m3 17.3 us (3.9 TB/s: the stream ends at 11.4,
+// the sums are joined at 13, the gates and outputs take to 15.5, the next call begins 1.9 later).
 #include "linear_tc.cuh"
 
 #include <cooperative_groups.h>
@@ -29,9 +30,9 @@ namespace cg = cooperative_groups;
 using namespace lin;
 
 constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8;
-// shared memory for stages, or for the sums of up to FEW tokens, of a CTA that has an SM to itself, and of one that shares it (228 KB an SM,
-// less 1 KB a CTA that the system takes, 1 KB of barriers and 1 KB to align the stages)
-constexpr int ROOM = 225 * 1024, HALF_ROOM = 111 * 1024;
+// shared memory for stages, or for the sums of up to FEW tokens, of a CTA that has an SM to itself, and of one that
+// shares it (228 KB an SM, less 1 KB a CTA that the system takes, 2 KB of barriers and scales and 1 KB to align the stages)
+constexpr int ROOM = 224 * 1024, HALF_ROOM = 110 * 1024;
 constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum may run over 2^24 values: 0.1 s)
 
 struct Maps {
@@ -104,6 +105,7 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], done;
   __shared__ uint32_t slot;
   __shared__ volatile int fail;
+  __shared__ __align__(16) float row_scale[FEW], col_scale[ROWS], col_add[ROWS];   // (col_add: up_scale, or the bias)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int tile_n = blockIdx.x / p.ck, rank = blockIdx.x - tile_n * p.ck, n0 = tile_n * ROWS;
   const int first = rank * p.per, last = min(p.steps, first + p.per);
@@ -184,20 +186,38 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
     __syncwarp();
   }
   __syncwarp();
-  // ---- the sums
+  // ---- the sums.  What the epilogue reads beside them is fetched while the products run (read after them it took 2 us):
+  // scales and bias go to shared memory, the residual to L2.
   const int tokens = (int)p.M;
+  const bool joins = p.ck > 1;
+  const Epilogue& e = p.e;
+  if (warp >= 2) {
+    for (int i = tid - 64; i < ROWS; i += NT - 64) {
+      if (e.row_scale && i < tokens) row_scale[i] = e.row_scale[i];
+      if (n0 + i < p.N) {
+        if (e.col_scale) col_scale[i] = e.col_scale[n0 + i];
+        if (GATED && e.col_scale) col_add[i] = e.up_scale[n0 + i];
+        if (!GATED && e.bias) col_add[i] = load_as(e.bias, n0 + i, e.bias_type);
+      }
+    }
+    if (!GATED && e.residual)
+      for (int i = tid - 64; i < 4 * tokens; i += NT - 64) {
+        const int c = n0 + 32 * (i & 3);
+        if (c < p.N)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"((size_t)e.residual + ((i >> 2) * e.ld_res + c) * (e.type == VERACE_F32 ? 4 : 2)));
+      }
+  }
   const int quarter = warp & 3;
   const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
-  const int n = n0 + 32 * quarter + lane;
+  if (!joins) __syncthreads();   // (the scales; of a split K the barrier behind the sums)
   const bool ok = tc::mbar_wait(&done, 0, SUM_POLLS) && !fail;
   if (!ok && lane == 0) atomicExch(&g_linear_few_status, 1);
   tc::fence_after_sync();
-  if (p.ck == 1) {
+  if (!joins) {
     if (ok) {
-      const Epilogue& e = p.e;
+      const int c = 32 * quarter + lane, n = n0 + c;
       const bool in = n < p.N;
-      const float cs = e.col_scale && in ? e.col_scale[n] : 1.f, us = GATED && e.up_scale && in ? e.up_scale[n] : 1.f;
-      const float bias = !GATED && e.bias && in ? load_as(e.bias, n, e.bias_type) : 0.f;
+      const float cs = col_scale[c], ca = col_add[c];   // (read where they are set alone)
 #pragma unroll 1
       for (int t = 16 * (warp >> 2); t < tokens; t += 32) {
         uint32_t r[16], s[16];
@@ -211,13 +231,13 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
         float g[16], u[16] = {};
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float rs = e.row_scale && t + j < tokens ? e.row_scale[t + j] : 1.f;
+          const float rs = e.row_scale && t + j < tokens ? row_scale[t + j] : 1.f;
           g[j] = __uint_as_float(r[j]);
           if (e.col_scale) g[j] *= rs * cs;
-          g[j] += bias;
+          if (!GATED && e.bias) g[j] += ca;
           if (GATED) {
             u[j] = __uint_as_float(s[j]);
-            if (e.col_scale) u[j] *= rs * us;
+            if (e.col_scale) u[j] *= rs * ca;
           }
         }
         if (e.pre) {
@@ -249,40 +269,51 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 1) tc::tmem_dealloc(tmem, p.cols);
-  if (p.ck > 1) {
+  if (joins) {
     cg::cluster_group cl = cg::this_cluster();
     const float* part = reinterpret_cast<const float*>(sm);
-    cl.sync();
-    // (eight vectors of every sum on their way together)
+    auto met = cl.barrier_arrive();
+    // a thread joins four columns of every 8 ck'th token
+    const int col = 4 * lane, quad = (int)max(0LL, min(4LL, p.N - n0 - col)), joiner = rank * NT + tid,
+              total = quad ? tokens * (ROWS / 4) : 0;
+    const long long c0 = n0 + col;
+    float res[4] = {};
+    auto residual = [&](int i) {
+      if (!GATED && e.residual && i < total) load4(e.residual, (long long)(i / (ROWS / 4)) * e.ld_res + c0, quad, e.type, res);
+    };
+    residual(joiner);
+    cl.barrier_wait(std::move(met));
+    // (the next vectors on their way while one is finished; one body for all of them: unrolled, it took 3.7 us for 64
+    // gated tokens where it takes 2.2, most of it instructions on their way)
     auto join = [&](auto ck) {
-      constexpr int CK = decltype(ck)::value, U = 8 / CK, H = GATED ? 2 : 1;
+      constexpr int CK = decltype(ck)::value, H = GATED ? 2 : 1;
       const float4* o[CK];
 #pragma unroll
       for (int c = 0; c < CK; ++c) o[c] = reinterpret_cast<const float4*>(cl.map_shared_rank(part, c));
-      const int total = tokens * (ROWS / 4), stride = CK * NT;
-      for (int i0 = rank * NT + tid; i0 < total; i0 += U * stride) {
-        float4 v[U][H][CK];
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-          if (i0 + k * stride < total)
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-              for (int c = 0; c < CK; ++c) v[k][h][c] = o[c][h * p.mp * (ROWS / 4) + i0 + k * stride];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int i = i0 + k * stride;
-          const long long c0 = n0 + i % (ROWS / 4) * 4;
-          if (i >= total || c0 >= p.N) continue;
-          float s[2][4] = {};
+      float4 v[H][CK];
+      auto load = [&](int i) {
+        if (i < total)
 #pragma unroll
           for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int c = 0; c < CK; ++c) {
-              s[h][0] += v[k][h][c].x; s[h][1] += v[k][h][c].y; s[h][2] += v[k][h][c].z; s[h][3] += v[k][h][c].w;
-            }
-          finish4<GATED>(p.e, i / (ROWS / 4), c0, p.N, s[0], s[1]);
-        }
+            for (int c = 0; c < CK; ++c) v[h][c] = o[c][h * p.mp * (ROWS / 4) + i];
+      };
+      load(joiner);
+#pragma unroll 1
+      for (int i = joiner; i < total; i += CK * NT) {
+        float s[2][4] = {}, r[4];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int c = 0; c < CK; ++c) {
+            s[h][0] += v[h][c].x; s[h][1] += v[h][c].y; s[h][2] += v[h][c].z; s[h][3] += v[h][c].w;
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = res[j];
+        load(i + CK * NT);
+        residual(i + CK * NT);
+        const int t = i / (ROWS / 4);
+        finish4<GATED>(e, t, c0, quad, col_scale + col, col_add + col, row_scale[t], r, s[0], s[1]);
       }
     };
     if (p.ck == 2) join(std::integral_constant<int, 2>());

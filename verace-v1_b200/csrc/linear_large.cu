@@ -823,7 +823,14 @@ __global__ void __launch_bounds__(256) join_splits(const float* __restrict__ par
   const long long m = i / quads, c = i % quads * 4;
   if (m >= M) return;
   const int n = (int)min(4LL, N - c);
-  float g[4] = {}, u[4] = {};
+  float g[4] = {}, u[4] = {}, res[4] = {}, scale[4], add[4], row_scale = 1.f;   // (all on their way together)
+  if (e.col_scale) {
+    row_scale = e.row_scale[m];
+    load4(e.col_scale, c, n, VERACE_F32, scale);
+    if (GATED) load4(e.up_scale, c, n, VERACE_F32, add);
+  }
+  if (!GATED && e.bias) load4(e.bias, c, n, e.bias_type, add);
+  if (!GATED && e.residual) load4(e.residual, m * e.ld_res + c, n, e.type, res);
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     float v[4];
@@ -836,7 +843,7 @@ __global__ void __launch_bounds__(256) join_splits(const float* __restrict__ par
       for (int j = 0; j < 4; ++j) u[j] += v[j];
     }
   }
-  finish4<GATED>(e, m, c, N, g, u);
+  finish4<GATED>(e, m, c, n, scale, add, row_scale, res, g, u);
 }
 
 // How a product is cut: columns of a tile, and splits of K.  A pair's time in clocks: a step of four MMAs takes 512

@@ -177,26 +177,22 @@ __device__ __forceinline__ void store4(void* p, long long i, int n, int type, co
   }
 }
 
-// four outputs of row m from their sums (u: the up projection's)
+// four outputs (n of them inside of the row) of row m from their sums (u: the up projection's), the columns' scales, their
+// bias (a gated product's: the up projection's scales), the row's scale and the residual, each read where e has it
 template <bool GATED>
-__device__ __forceinline__ void finish4(const Epilogue& e, long long m, long long c, long long N, float (&g)[4], float (&u)[4]) {
-  const int n = (int)min(4LL, N - c);
-  float res[4] = {};
-  if (!GATED && e.residual) load4(e.residual, m * e.ld_res + c, n, e.type, res);
+__device__ __forceinline__ void finish4(const Epilogue& e, long long m, long long c, int n, const float* col_scale,
+                                        const float* col_add, float row_scale, const float (&res)[4], float (&g)[4],
+                                        float (&u)[4]) {
   if (e.col_scale) {
-    const float rs = e.row_scale[m];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) {
-        g[j] *= rs * e.col_scale[c + j];
-        if (GATED) u[j] *= rs * e.up_scale[c + j];
-      }
+    for (int j = 0; j < 4; ++j) {
+      g[j] *= row_scale * col_scale[j];
+      if (GATED) u[j] *= row_scale * col_add[j];
+    }
   }
   if (!GATED && e.bias) {
-    float b[4];
-    load4(e.bias, c, n, e.bias_type, b);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] += b[j];
+    for (int j = 0; j < 4; ++j) g[j] += col_add[j];
   }
   if (e.pre) {
     store4(e.pre, m * e.ld + c, n, VERACE_F32, g);
