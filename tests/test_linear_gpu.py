@@ -27,10 +27,11 @@ def weight(g, n, k, dt=F32, gain=1.0):
     return (gain * torch.randn(n, k, device="cuda", generator=g) / math.sqrt(max(k, 1))).to(dt)
 
 
-# m around the few-token limits and the tiles' borders; k and n that no tile or vector divides
+# m around the few-token limits (160; 112 of small gated weights) and the tiles' borders; k and n that no tile or vector divides
 SIZES = [(1, 64, 128), (1, 1024, 2048), (2, 72, 129), (7, 1000, 255), (8, 1, 1), (16, 65, 257), (17, 513, 64),
          (33, 100, 1001), (64, 4096, 512), (65, 256, 300), (127, 640, 128), (128, 128, 130), (129, 200, 520),
-         (255, 71, 256), (257, 1024, 777), (300, 320, 1024), (1000, 129, 640)]
+         (255, 71, 256), (257, 1024, 777), (300, 320, 1024), (1000, 129, 640), (97, 130, 100), (113, 1030, 200),
+         (145, 1000, 640), (150, 4100, 1100), (160, 8192, 1000), (161, 8192, 1000)]
 
 
 @pytest.mark.parametrize("m,k,n", SIZES)

@@ -1,6 +1,6 @@
 // Products of few rows (tokens) on the tensor cores, the other engine behind linear.cu:
-//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 96
-// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 96 columns, so
+//     out(m, n) = epilogue(sum_k x(m, k) W(n, k)),  m up to 160
+// Bound: the weights' bytes.  W's rows are the MMA's 128 rows and the tokens its 16 to 160 columns, so
 // a weight crosses shared memory once and no row of the MMA is idle; a CTA streams its 128 rows (gated:
 // 128 of each weight, two sums side by side in TMEM) by TMA in stages of 128 bytes of K.  Two
 // CTAs share an SM where shared memory allows, so that one's set-up and epilogue run under the other's
@@ -192,9 +192,9 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
   const bool joins = p.ck > 1;
   const Epilogue& e = p.e;
   if (warp >= 2) {
-    for (int i = tid - 64; i < ROWS; i += NT - 64) {
+    for (int i = tid - 64; i < (FEW > ROWS ? FEW : ROWS); i += NT - 64) {
       if (e.row_scale && i < tokens) row_scale[i] = e.row_scale[i];
-      if (n0 + i < p.N) {
+      if (i < ROWS && n0 + i < p.N) {
         if (e.col_scale) col_scale[i] = e.col_scale[n0 + i];
         if (GATED && e.col_scale) col_add[i] = e.up_scale[n0 + i];
         if (!GATED && e.bias) col_add[i] = load_as(e.bias, n0 + i, e.bias_type);
@@ -330,7 +330,7 @@ int launch(const Product& p, cudaStream_t st) {
   Args a{};
   int rc;
   a.M = p.M; a.N = p.N;
-  static_assert(FEW % 16 == 0 && FEW * ROWS * 4 * 2 <= HALF_ROOM, "a cluster's sums fit beside another CTA's");
+  static_assert(FEW % 16 == 0 && FEW * ROWS * 4 * 2 <= ROOM && 2 * FEW <= 512, "a CTA's sums fit in shared memory and TMEM");
   a.mp = (int)((p.M + 15) / 16 * 16);
   // A (x) in one box of all tokens, B (the weights) as the MMA's rows
   if ((rc = operand_map(&maps.x, p.a, p.type, a.mp))) return rc;
@@ -344,20 +344,20 @@ int launch(const Product& p, cudaStream_t st) {
   while (a.ck < 8 && a.tiles_n * a.ck * 2 <= 148 && a.steps >= a.ck * 4) a.ck *= 2;
   a.per = (a.steps + a.ck - 1) / a.ck;
   a.stage = ROWS * 128 * (GATED ? 2 : 1) + a.mp * 128;
-  // Two CTAs an SM while that leaves a CTA three stages (gated, 64 x 4096 x 32000: 91 us either way, 48 of it for 8 bits
-  // against 52); of a split K five, as there is a CTA for every SM at most (64 x 8192 x 4096: 17.7 us with three, 16.4 alone on
-  // the SM with seven); clusters of eight always, which the SMs of a GPC hold only twice otherwise (32 x 16384 x 2048 16.2 us
-  // against 26.2).
+  // Two CTAs an SM while that leaves a CTA three stages (gated, 64 x 4096 x 32000: 89 us against 90, 48 of it for 8 bits
+  // against 50); of a split K five, as there is a CTA for every SM at most (64 x 8192 x 4096: 17.4 us with four, 15.8 alone
+  // on the SM with eight); clusters of eight always, which the SMs of a GPC hold only twice otherwise (32 x 16384 x 2048
+  // 16.6 us against 26.1), unless their sums need more.
+  const int sums = a.ck > 1 ? a.mp * ROWS * 4 * (GATED ? 2 : 1) : 0;
   int room = HALF_ROOM;
-  if (a.ck < 8 && room / a.stage < (a.ck > 1 ? 5 : 3)) room = ROOM;
+  if (sums > room || (a.ck < 8 && room / a.stage < (a.ck > 1 ? 5 : 3))) room = ROOM;
   a.stages = room / a.stage < MAX_STAGES ? room / a.stage : MAX_STAGES;
   if (a.stages > a.per) a.stages = a.per;
   const int want = a.mp * (GATED ? 2 : 1);
   a.cols = 32;
   while (a.cols < want) a.cols *= 2;
   int smem = a.stages * a.stage;
-  const int sums = a.mp * ROWS * 4 * (GATED ? 2 : 1);
-  if (a.ck > 1 && smem < sums) smem = sums;
+  if (smem < sums) smem = sums;
   smem += 1024;
   a.idesc = (1u << 4) | (uint32_t)(p.type == VERACE_BF16) << 7 | (uint32_t)(p.type == VERACE_BF16) << 10 |
             (uint32_t)WMN << 15 | (uint32_t)(a.mp >> 3) << 17 | (uint32_t)(ROWS >> 4) << 24;

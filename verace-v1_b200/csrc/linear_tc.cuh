@@ -35,10 +35,8 @@ struct Product {
 // What product_large may take for partial sums (M x N outputs each, nz of them).
 size_t split_bytes(long long M, long long N, long long K, int segments, int nz, bool gated, int type, bool parts);
 
-// Tokens up to which weights are streamed past them (linear_few.cu).  bf16, against tiles of 256 rows: 32 x 4096 x 8192
-// 16.1 us and 19.0, 96 x 8192 x 4096 17.6 and 23.3, 96 x 4096 x 32000 48.5 and 54.8, gated 96 x 4096 x 8192 30.9 and 34.4; 96 x
-// 1024 x 4096 7.8 and 7.8, gated 11.1 and 10.4.
-constexpr int FEW = 96;
+// Tokens up to which weights may be streamed past them (linear_few.cu).
+constexpr int FEW = 160;
 
 int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
 int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to FEW rows of A
