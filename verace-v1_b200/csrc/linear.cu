@@ -64,28 +64,28 @@ __device__ __forceinline__ void store_operand(Part<T>* o, long long piece, const
   }
 }
 
-// src [rows, cols] fp32 -> three parts [3][rows][ld], ld = cols rounded up to 8
-__global__ void __launch_bounds__(256) split_rows(const float* __restrict__ src, long long ld_src, long long rows,
-                                                  long long cols, bool vec, __nv_bfloat16* __restrict__ dst, long long ld) {
-  depend();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / (ld / 8), c = i % (ld / 8) * 8;
-  if (row >= rows) return;
+// Matrices that the products cannot read as they lie, up to three in one launch (one after the other they took 2 to 3 us
+// more each), 8 values or 16 bytes a thread.
+struct Copy {
+  const char* src;
+  char* dst;
+  long long ld_src, ld, rows, width;   // in values of fp32 parts, else in bytes
+  unsigned blocks;
+  bool vec;                            // (fp32) whole aligned words
+};
+struct Copies {
+  Copy m[3];
+};
+// fp32 rows -> three bf16 parts [3][rows][ld], ld = width rounded up to 8
+__device__ __forceinline__ void split_row(const Copy& a, long long row, long long c) {
   float v[8];
-  load8<float>(src + row * ld_src, c, cols, vec, v);
-  store_operand<float>(dst + row * ld + c, rows * ld, v);
+  load8<float>(reinterpret_cast<const float*>(a.src) + row * a.ld_src, c, a.width, a.vec, v);
+  store_operand<float>(reinterpret_cast<__nv_bfloat16*>(a.dst) + row * a.ld + c, a.rows * a.ld, v);
 }
-
-// src: rows of `bytes` bytes, ld_src apart, starting anywhere -> dst: rows ld apart (a multiple of 16), zeros behind
-// them; 16 bytes a thread, read as the aligned words around them.
-__global__ void __launch_bounds__(256) align_rows(const char* __restrict__ src, long long ld_src, long long rows, long long bytes,
-                                                  char* __restrict__ dst, long long ld) {
-  depend();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / (ld / 16), c = i % (ld / 16) * 16;
-  if (row >= rows) return;
-  const char* s = src + row * ld_src + c;
-  const int off = (int)((size_t)s & 3), left = (int)min(16LL, bytes - c);    // (left > 0: ld is bytes rounded up)
+// rows that start anywhere -> rows ld apart (a multiple of 16), zeros behind them; read as the aligned words around them
+__device__ __forceinline__ void align_row(const Copy& a, long long row, long long c) {
+  const char* s = a.src + row * a.ld_src + c;
+  const int off = (int)((size_t)s & 3), left = (int)min(16LL, a.width - c);    // (left > 0: ld is width rounded up)
   const uint32_t* w = reinterpret_cast<const uint32_t*>(s - off);
   uint32_t x[5];
 #pragma unroll
@@ -97,10 +97,30 @@ __global__ void __launch_bounds__(256) align_rows(const char* __restrict__ src, 
     const int valid = left - 4 * j;
     if (valid < 4) o[j] = valid <= 0 ? 0u : o[j] & ((1u << (8 * valid)) - 1u);
   }
-  *reinterpret_cast<uint4*>(dst + row * ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
+  *reinterpret_cast<uint4*>(a.dst + row * a.ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) copy_rows(const __grid_constant__ Copies all) {
+  constexpr int U = SPLIT ? 8 : 16;
+  depend();
+  unsigned block = blockIdx.x;
+  int z = 0;
+  while (z < 2 && block >= all.m[z].blocks) block -= all.m[z++].blocks;
+  const Copy& a = all.m[z];
+  const unsigned per_row = (unsigned)(a.ld / U);
+  // (a division of 64 bits once in a matrix of 2^36 bytes alone)
+  const unsigned long long first = (unsigned long long)block * 256;
+  const unsigned long long row0 = first >> 32 ? first / per_row : (unsigned)first / per_row;
+  const unsigned at = (unsigned)(first - row0 * per_row) + threadIdx.x;
+  const long long row = (long long)row0 + at / per_row;
+  if (row >= a.rows) return;
+  if constexpr (SPLIT) split_row(a, row, (long long)(at % per_row) * U);
+  else align_row(a, row, (long long)(at % per_row) * U);
 }
 
-long long padded(long long cols, int type = VERACE_BF16) { return type == VERACE_E4M3 ? (cols + 15) / 16 * 16 : (cols + 7) / 8 * 8; }
+long long padded(long long cols, int type = VERACE_BF16) {
+  return type == VERACE_E4M3 ? (cols + 15) / 16 * 16 : (cols + 7) / 8 * 8;
+}
 // bytes of an operand that a pass writes
 size_t operand_bytes(long long rows, long long cols, int type) {
   return align_up((size_t)rows * padded(cols, type) * (type == VERACE_F32 ? 6 : size_of(type)), 256);
@@ -128,28 +148,34 @@ struct Taker {
 
 bool aligned_rows(const void* p, long long ld, int type) { return (size_t)p % 16 == 0 && ld * size_of(type) % 16 == 0; }
 
-// An operand of the products from a user's matrix: as it is, split into parts or copied in the workspace.
-int operand(Mat* out, const void* p, long long ld, long long rows, long long cols, int type, Taker& ws, cudaStream_t st) {
-  if (type != VERACE_F32) {
-    *out = Mat{p, rows, cols, ld, 1, 0};
-    if (aligned_rows(p, ld, type)) return VERACE_OK;
-    const long long es = size_of(type);
-    out->ld = padded(cols, type);
-    out->p = ws.take(rows * out->ld * es);
-    const long long blocks = (rows * (out->ld * es / 16) + 255) / 256;
-    VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld operand is too large", rows, cols);
-    return launch_after("align_rows", align_rows, dim3((unsigned)blocks), 256, 0, st, 1, (const char*)p, ld * es, rows, cols * es,
-                        (char*)out->p, out->ld * es);
+// Operands of the products from a user's matrices: as they are, split into parts or copied in the workspace.
+struct Operands {
+  int type;
+  Taker& ws;
+  Copies all = {};
+  int n = 0;
+  long long blocks = 0;
+  void add(Mat* out, const void* p, long long ld, long long rows, long long cols) {
+    const bool split = type == VERACE_F32;
+    if (!split && aligned_rows(p, ld, type)) {
+      *out = Mat{p, rows, cols, ld, 1, 0};
+      return;
+    }
+    const long long es = split ? 1 : size_of(type);
+    void* dst = ws.take(operand_bytes(rows, cols, type));
+    *out = split ? operand_at(dst, rows, cols, type) : Mat{dst, rows, cols, padded(cols, type), 1, 0};
+    const long long mine = (rows * (out->ld * es / (split ? 8 : 16)) + 255) / 256;
+    blocks += mine;
+    all.m[n++] = Copy{(const char*)p, (char*)dst, ld * es, out->ld * es, rows, cols * es, (unsigned)mine,
+                      cols % 8 == 0 && ld % 4 == 0 && (size_t)p % 16 == 0};
   }
-  void* dst = ws.take(operand_bytes(rows, cols, type));
-  *out = operand_at(dst, rows, cols, type);
-  const long long threads = rows * (out->ld / 8);
-  VERACE_REQUIRE((threads + 255) / 256 < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: %lld x %lld operand is too large", rows,
-                 cols);
-  const bool vec = cols % 8 == 0 && ld % 4 == 0 && (size_t)p % 16 == 0;
-  return launch_after("split_rows", split_rows, dim3((unsigned)((threads + 255) / 256)), 256, 0, st, 1, (const float*)p, ld, rows,
-                      cols, vec, (__nv_bfloat16*)dst, out->ld);
-}
+  int make(cudaStream_t st) {
+    if (n == 0) return VERACE_OK;
+    VERACE_REQUIRE(blocks < 1LL << 31, VERACE_ERR_UNSUPPORTED, "linear: operands of %lld bytes are too large", blocks * 4096);
+    return launch_after("copy_rows", type == VERACE_F32 ? copy_rows<true> : copy_rows<false>, dim3((unsigned)blocks), 256, 0, st,
+                        1, all);
+  }
+};
 
 // ------------------------------------------------------------------ sums over nothing (k = 0)
 __global__ void __launch_bounds__(256) empty_sum(Epilogue e, long long m, long long n) {
@@ -408,9 +434,11 @@ extern "C" int verace_linear(const void* x, long long ldx, const float* x_scale,
   if (dots && dtype == VERACE_F32) {
     p.a = Mat{x, m, k, ldx, 1, 0};
     p.b[0] = Mat{w, n, k, ldw, 1, 0};
-  } else if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) ||
-                       (rc = operand(&p.b[0], w, ldw, n, k, dtype, ws, st)))) {
-    return rc;
+  } else if (k > 0) {
+    Operands o{dtype, ws};
+    o.add(&p.a, x, ldx, m, k);
+    o.add(&p.b[0], w, ldw, n, k);
+    if ((rc = o.make(st))) return rc;
   }
   if (dots) return product_dot(p, st);
   p.segments = p.a_step = 1;
@@ -436,7 +464,8 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
   VERACE_REQUIRE(act >= VERACE_ACT_NONE && act <= VERACE_ACT_GELU_TANH, VERACE_ERR_INVALID, "%s: activation %d", who, act);
   const bool any = m > 0 && n > 0;
   VERACE_REQUIRE(!any || (dout && (pre || act == VERACE_ACT_NONE)), VERACE_ERR_INVALID, "%s: NULL pointer", who);
-  if (any && k > 0 && ((dw && (rc = check_rows(who, "x", x, ldx, k, dtype))) || (dx && (rc = check_rows(who, "w", w, ldw, k, dtype)))))
+  if (any && k > 0 &&
+      ((dw && (rc = check_rows(who, "x", x, ldx, k, dtype))) || (dx && (rc = check_rows(who, "w", w, ldw, k, dtype)))))
     return rc;
   if ((rc = check_workspace(who, verace_linear_backward_workspace(m, n, k, dtype), workspace, workspace_bytes))) return rc;
   cudaStream_t st = (cudaStream_t)stream;
@@ -471,12 +500,19 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
                              any ? chunks_of(m) : 0LL, (long long)n, (T*)dbias)))
         return rc;
     }
+    Mat xm{}, wm{};
+    if (any && k > 0) {
+      Operands made{dtype, ws};
+      if (dx) made.add(&wm, w, ldw, n, k);
+      if (dw) made.add(&xm, x, ldx, m, k);
+      if ((rc = made.make(st))) return rc;
+    }
     if (dx && k > 0) {
       Product d{};
       d.type = dtype; d.M = m; d.N = k; d.K = n; d.nz = 1; d.b_mn = true;
       d.e = plain_out(dx, k, dtype);
       d.a = p;
-      if (any && (rc = operand(&d.b[0], w, ldw, n, k, dtype, ws, st))) return rc;
+      d.b[0] = wm;
       d.segments = d.a_step = 1;
       d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
@@ -486,7 +522,7 @@ extern "C" int verace_linear_backward(const void* dout, const void* x, long long
       d.type = dtype; d.M = n; d.N = k; d.K = m; d.nz = 1; d.a_mn = d.b_mn = true;
       d.e = plain_out(dw, k, dtype);
       d.a = p;
-      if (any && (rc = operand(&d.b[0], x, ldx, m, k, dtype, ws, st))) return rc;
+      d.b[0] = xm;
       d.segments = d.a_step = 1;
       d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
@@ -535,10 +571,12 @@ extern "C" int verace_gated_linear(const void* x, long long ldx, const float* x_
     p.a = Mat{x, m, k, ldx, 1, 0};
     p.b[0] = Mat{w_gate, f, k, ldw, 1, 0};
     p.b[1] = Mat{w_up, f, k, ldw, 1, 0};
-  } else if (k > 0 && ((rc = operand(&p.a, x, ldx, m, k, dtype, ws, st)) ||
-                       (rc = operand(&p.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
-                       (rc = operand(&p.b[1], w_up, ldw, f, k, dtype, ws, st)))) {
-    return rc;
+  } else if (k > 0) {
+    Operands o{dtype, ws};
+    o.add(&p.a, x, ldx, m, k);
+    o.add(&p.b[0], w_gate, ldw, f, k);
+    o.add(&p.b[1], w_up, ldw, f, k);
+    if ((rc = o.make(st))) return rc;
   }
   if (dots) return product_dot(p, st);
   p.segments = p.a_step = 1;
@@ -596,14 +634,21 @@ extern "C" int verace_gated_linear_backward(const void* dout, const void* x, lon
       if ((rc = slope_grid(s, GATED_CHUNK, &grid))) return rc;
       if ((rc = launch_after("gated_slope", gated_slope<T, O>, dim3(grid), 256, 0, st, 1, s))) return rc;
     }
+    Mat xm{}, gm{}, um{};
+    if (any) {
+      Operands made{dtype, ws};
+      if (dx) made.add(&gm, w_gate, ldw, f, k);
+      if (dx) made.add(&um, w_up, ldw, f, k);
+      if (dw_gate || dw_up) made.add(&xm, x, ldx, m, k);
+      if ((rc = made.make(st))) return rc;
+    }
     if (dx) {
       Product d{};
       d.type = dtype; d.M = m; d.N = k; d.K = f; d.nz = 1; d.b_mn = true;
       d.e = plain_out(dx, k, dtype);
       d.a = p;
-      if (any && ((rc = operand(&d.b[0], w_gate, ldw, f, k, dtype, ws, st)) ||
-                  (rc = operand(&d.b[1], w_up, ldw, f, k, dtype, ws, st))))
-        return rc;
+      d.b[0] = gm;
+      d.b[1] = um;
       d.segments = d.a_step = 2;
       d.ws = ws.at;
       if ((rc = run_product(d, st))) return rc;
@@ -615,7 +660,7 @@ extern "C" int verace_gated_linear_backward(const void* dout, const void* x, lon
       d.out_z[0] = dw_gate; d.out_z[1] = dw_up;
       d.e = plain_out(dw_gate ? dw_gate : dw_up, k, dtype);
       d.a = p;
-      if (any && (rc = operand(&d.b[0], x, ldx, m, k, dtype, ws, st))) return rc;
+      d.b[0] = xm;
       d.segments = 1;
       d.a_step = 2;
       d.a_first = dw_gate ? 0 : 1;
