@@ -313,7 +313,31 @@ def test_repeatable_and_out_is_not_shared(m):
         assert all(torch.equal(a, b) for a, b in zip(o, want))
 
 
-@pytest.mark.parametrize("m", [2, 200])
+def test_engines_side_by_side_on_streams():
+    """Products of every engine and of the largest claims on an SM's memory, on four streams at once: their bits alone."""
+    g = gen(26)
+    x, wg, wu = randn(g, 160, 1024, dt=BF16), weight(g, 4224, 1024, BF16), weight(g, 4224, 1024, BF16)
+    (x8, sx), (w8, sg), (u8, su) = (fp8_rows(t) for t in (randn(g, 150, 4096), weight(g, 1100, 4096), weight(g, 1100, 4096)))
+    small, w7, r7 = randn(g, 7, 2048, dt=F16), weight(g, 512, 2048, F16), randn(g, 7, 512, dt=F16)
+    big, wb = randn(g, 600, 512, dt=BF16), weight(g, 1000, 512, BF16)
+    one, w1 = randn(g, 1, 256, dt=F32), weight(g, 512, 256, F32)
+    calls = [lambda: V.gated_linear(x, wg, wu), lambda: V.fused_linear(small, w7, residual=r7), lambda: V.fused_linear(big, wb),
+             lambda: V.fused_linear(one, w1), lambda: V.fused_linear(x, wg, activation="silu"),
+             lambda: V.gated_linear(x8, w8, u8, x_scale=sx, gate_scale=sg, up_scale=su)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams, out = [torch.cuda.Stream() for _ in range(4)], []
+    for i in range(10):
+        for s, st in enumerate(streams):
+            for j in range(len(calls)):
+                which = (i + s + j) % len(calls)
+                with torch.cuda.stream(st):
+                    out.append((which, calls[which]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in out)
+
+
+@pytest.mark.parametrize("m", [2, 120, 200])
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_captured_in_a_graph(m, dt):
     """Forward and backward captured once and replayed on new values; two graphs do not disturb each other."""
@@ -475,7 +499,7 @@ def test_out_may_be_the_residual(m, n):
         assert rc == 0 and torch.equal(r, want)
 
 
-@pytest.mark.parametrize("m", [1, 2, 40, 300])
+@pytest.mark.parametrize("m", [1, 2, 40, 130, 300])
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_chains_of_calls_wait_for_each_other(m, dt):
     """Kernels that become resident before the one ahead of them ends: a chain without a wait on the host gives the bits
