@@ -72,11 +72,35 @@ __device__ __forceinline__ float rounded(float x) {
   return to_f32(from_f32<T>(x));
 }
 
-// A group of G threads holds a row of up to 32 G values: VEC neighbouring ones from column VEC (g + G i) on, less
-// `shift`, the row's place in its first word, where rows are not WHOLE words.
+// The VEC values (16 bytes) from column c of a row of `cols` on, wherever it starts: the aligned words around them, those
+// that hold a value of the row.  Values outside of the row are whatever lies there.
+template <typename T, int VEC>
+__device__ __forceinline__ void unaligned(const T* p, int c, int cols, float (&v)[VEC]) {
+  static_assert(VEC * sizeof(T) == 16, "a word");
+  const int off = (int)((size_t)(p + c) & 15), first = c - off / (int)sizeof(T);
+  const uint4* w = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p + c) - off);
+  uint4 a = make_uint4(0, 0, 0, 0), b = a;
+  if (first + VEC > 0 && first < cols) a = w[0];
+  if (off && first + 2 * VEC > 0 && first + VEC < cols) b = w[1];
+  uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 6; ++j) x[j] = off & 8 ? x[j + 2] : x[j];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) x[j] = off & 4 ? x[j + 1] : x[j];
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = off & 2 ? __funnelshift_r(x[j], x[j + 1], 16) : x[j];
+  }
+  Lot<T, VEC> l;
+  l.w[0] = make_uint4(x[0], x[1], x[2], x[3]);
+  l.values(v);
+}
+
+// A group of G threads (of a block of 128, or a block) holds a row of up to 32 G values: VEC neighbouring ones from column
+// VEC (g + G i) on, less `shift`, the row's place in its first word, where rows are not WHOLE words.
 template <typename T, int G, bool WHOLE, bool ADD>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a) {
-  constexpr int NT = G < 128 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G > 32 ? G / 32 : 1;
+__global__ void __launch_bounds__(G < 96 ? 128 : G) norm_fp8_kernel(NormArgs a) {
+  constexpr int NT = G < 96 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G > 32 ? G / 32 : 1;
   __shared__ float part[2][NT / G][W > 1 ? W : 1];
   const int g = threadIdx.x % G, mine = threadIdx.x / G;
   long long row = (long long)blockIdx.x * (NT / G) + mine;
@@ -92,9 +116,10 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
   auto column = [&](int i) { return VEC * (g + G * i) - shift; };
   auto any = [&](int i) { return VEC * G * i < cols + shift && column(i) < cols; };
   auto in = [&](int c) { return WHOLE || (c >= 0 && c < cols); };
+  auto inner = [&](int c) { return WHOLE || (c >= 0 && c + VEC <= cols); };   // all but the first and the last vector
   // whether a vector of p may be moved as one: inside of the row, and p's words where h's are
   auto as_one = [&](const T* p, int c) {
-    return WHOLE || (c >= 0 && c + VEC <= cols && ((size_t)(p + off + c) & 15) == 0);
+    return WHOLE || (inner(c) && ((size_t)(p + off + c) & 15) == 0);
   };
   auto put = [&](void* to, int c, const float (&v)[VEC]) {
     T* p = static_cast<T*>(to);
@@ -116,12 +141,11 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
       if (any(i)) {
         lh[i].load(h + column(i));
         if constexpr (ADD) {
-          if (as_one(y, column(i))) {
+          if constexpr (WHOLE) {
             ly[i].load(y + off + column(i));
           } else {
             float t[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) t[j] = in(column(i) + j) ? to_f32(y[off + column(i) + j]) : 0.f;
+            unaligned<T, VEC>(y + off, column(i), cols, t);
             store<T, VEC>(reinterpret_cast<T*>(ly[i].w), t);
           }
         }
@@ -132,7 +156,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
       for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
       if (any(i)) {
         lh[i].values(v[i]);
-        if constexpr (!WHOLE) {
+        if (!inner(column(i))) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
             if (!in(column(i) + j)) v[i][j] = 0.f;
@@ -173,8 +197,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
             lw.load(w + column(i));
             lw.values(t);
           } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) t[j] = in(column(i) + j) ? to_f32(w[column(i) + j]) : 0.f;
+            unaligned<T, VEC>(w, column(i), cols, t);
           }
         }
 #pragma unroll
@@ -183,10 +206,17 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
   }
   float top = 0x1p-100f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    if (!any(i)) continue;
+    if (inner(column(i))) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (in(column(i) + j)) top = max_nan(top, fabsf(v[i][j]));   // (0 rs is NaN where rs is infinite)
+      for (int j = 0; j < VEC; ++j) top = max_nan(top, fabsf(v[i][j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (in(column(i) + j)) top = max_nan(top, fabsf(v[i][j]));
+    }
+  }
 #pragma unroll
   for (int o = G < 32 ? G / 2 : 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if constexpr (W > 1) {
@@ -211,7 +241,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
         o[j] = lo | hi << 16;
       }
       uint8_t* q = a.q + off + c;
-      if (WHOLE || (c >= 0 && c + VEC <= cols && (size_t)q % VEC == 0)) {
+      if (WHOLE || (inner(c) && (size_t)q % VEC == 0)) {
         if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q) = make_uint2(o[0], o[1]);
         else *reinterpret_cast<uint32_t*>(q) = o[0];
       } else {
@@ -226,17 +256,18 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a)
 template <typename T, bool WHOLE, bool ADD>
 int launch(const NormArgs& a, cudaStream_t st) {
   const int cols = a.cols + (WHOLE ? 0 : 7);   // (a row may start in the middle of a word)
-  auto go = [&](auto kernel, long long blocks, int threads) {
-    return lin::launch_after("norm_fp8_kernel", kernel, dim3((unsigned)blocks), threads, 0, st, 1, a);
+  auto go = [&](auto group) {
+    constexpr int G = decltype(group)::value, NT = G < 96 ? 128 : G;
+    return lin::launch_after("norm_fp8_kernel", norm_fp8_kernel<T, G, WHOLE, ADD>, dim3((unsigned)((a.rows + NT / G - 1) / (NT / G))),
+                             NT, 0, st, 1, a);
   };
-  if (cols <= 256) return go(norm_fp8_kernel<T, 8, WHOLE, ADD>, (a.rows + 15) / 16, 128);
-  if (cols <= 512) return go(norm_fp8_kernel<T, 16, WHOLE, ADD>, (a.rows + 7) / 8, 128);
-  if (cols <= 1024) return go(norm_fp8_kernel<T, 32, WHOLE, ADD>, (a.rows + 3) / 4, 128);
-  if (cols <= 2048) return go(norm_fp8_kernel<T, 64, WHOLE, ADD>, (a.rows + 1) / 2, 128);
-  if (cols <= 4096) return go(norm_fp8_kernel<T, 128, WHOLE, ADD>, a.rows, 128);
-  if (cols <= 8192) return go(norm_fp8_kernel<T, 256, WHOLE, ADD>, a.rows, 256);
-  if (cols <= 16384) return go(norm_fp8_kernel<T, 512, WHOLE, ADD>, a.rows, 512);
-  return go(norm_fp8_kernel<T, 1024, WHOLE, ADD>, a.rows, 1024);
+#define VERACE_GROUP(G) \
+  if (cols <= 32 * G) return go(std::integral_constant<int, G>())
+  VERACE_GROUP(8); VERACE_GROUP(16); VERACE_GROUP(32); VERACE_GROUP(64); VERACE_GROUP(96); VERACE_GROUP(128);
+  VERACE_GROUP(160); VERACE_GROUP(192); VERACE_GROUP(224); VERACE_GROUP(256); VERACE_GROUP(320); VERACE_GROUP(384);
+  VERACE_GROUP(512); VERACE_GROUP(640); VERACE_GROUP(768);
+#undef VERACE_GROUP
+  return go(std::integral_constant<int, 1024>());
 }
 
 template <typename T>
