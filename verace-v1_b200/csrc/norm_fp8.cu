@@ -6,13 +6,15 @@
 // 2^-100 keeps 448 / a finite; a row of zeros gives zeros.  A NaN or infinity in a row makes its
 // scale NaN or leaves NaN in its place, as in torch.
 //
-// Bound: bytes (7 a value with the residual in 16 bits; 16384 x 4096 bf16 with the residual 71.7 us, 6.55 TB/s, the
+// Bound: bytes (7 a value with the residual in 16 bits; 16384 x 4096 bf16 with the residual 71.5 us, 6.55 TB/s, the
 // rate of a copy).  A row stays in the registers of its group of 8 to 1024 threads, 32 values a thread (8 for up to 256
-// values: 56541 x 70 bf16 with the residual 19.0 us, with a warp a row 50), all loads of a row in flight before its first store; two
-// reductions (squares, then magnitudes) by shuffles and, above a warp, one exchange through shared memory each.
+// values: 56541 x 70 bf16 with the residual 19.0 us, with a warp a row 50), all loads of a row in flight before its first
+// store; two reductions (squares, then magnitudes) by shuffles and, above a warp, one exchange through shared memory each.
+// A group has the warps that a row fills (16384 x 5120 bf16: 51 us; with 256 threads instead of 160, 67).
 // Rows whose width is no multiple of 8 start anywhere in a 16-byte word: their words are those of the whole
-// tensor, the first and last one masked, so that all but the norm's weights is read and written a word
-// at a time all the same (1111 x 5001 fp32: 14.7 us, value by value 19.9).
+// tensor, the first and last one masked, so that all is read and written a word at a time all the same; the weights,
+// which start at another place in their words, are shifted there (8888 x 5001 bf16: 42 us, with weights read value by
+// value and 256 threads 70; whole words, 8888 x 5000, take 30).
 #include "linear_tc.cuh"
 
 #include <cuda_fp8.h>
