@@ -48,7 +48,8 @@ def check(h, norm, q, scale, n=None):
 
 
 SHAPES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 1000), (9, 1024), (4, 1025), (3, 1032), (2, 4096), (3, 4097), (2, 5001),
-          (2, 16384), (1, 16385), (2, 20000), (1, 32768), (700, 256), (333, 4096)]
+          (2, 16384), (1, 16385), (2, 20000), (1, 32768), (700, 256), (333, 4096),
+          (3, 5120), (2, 5121), (2, 6143), (3, 7168), (2, 8185), (2, 10240), (2, 12281), (1, 20473), (1, 24576)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
@@ -189,3 +190,29 @@ def test_captured_and_on_another_stream():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cols", [5, 259, 1003, 5120])
+def test_every_place_in_a_word(cols, dt):
+    """h, y, the sum and the weights each start anywhere in a 16-byte word, with NaN before and behind them."""
+    rows, word = 3, 16 // dt.itemsize
+    h0, y0, norm0 = data(rows, cols, dt, 7)
+    want = (h0.float() + y0.float()).to(dt)
+
+    def at(t, off):
+        base = torch.full((t.numel() + 2 * word,), math.nan, device="cuda", dtype=dt)
+        view = base[off:off + t.numel()].view(t.shape)
+        view.copy_(t)
+        return base, view
+    for i in range(word):
+        for j, k in ((0, i), (i, 0), (3 * i % word, 5 * i % word), (i + 1 - i % 2 if i + 1 < word else 0, i)):
+            (_, h), (_, y), (_, w) = at(h0, i), at(y0, j), at(norm0.weight.detach(), k)
+            into, out = at(torch.zeros_like(h0), (i + j) % word)
+            norm = torch.nn.RMSNorm(cols, eps=1e-6, device="cuda", dtype=dt)
+            norm.weight = torch.nn.Parameter(w, requires_grad=False)
+            assert norm.weight.data_ptr() == w.data_ptr()
+            check(h0, norm0, *V.rmsnorm_fp8(h, norm))
+            q, s, n = V.add_rmsnorm_fp8(h, y, norm, out=out, return_norm=True)
+            assert torch.equal(out, want) and int(into.isnan().sum()) == 2 * word
+            check(want, norm0, q, s, n)

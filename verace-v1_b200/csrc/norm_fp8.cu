@@ -101,8 +101,8 @@ __device__ __forceinline__ void unaligned(const T* p, int c, int cols, float (&v
 // A group of G threads (of a block of 128, or a block) holds a row of up to 32 G values: VEC neighbouring ones from column
 // VEC (g + G i) on, less `shift`, the row's place in its first word, where rows are not WHOLE words.
 template <typename T, int G, bool WHOLE, bool ADD>
-__global__ void __launch_bounds__(G < 96 ? 128 : G) norm_fp8_kernel(NormArgs a) {
-  constexpr int NT = G < 96 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G > 32 ? G / 32 : 1;
+__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fp8_kernel(NormArgs a) {
+  constexpr int NT = G < 128 ? 128 : G, VEC = WHOLE ? 8 : 16 / (int)sizeof(T), NV = 32 / VEC, W = G > 32 ? G / 32 : 1;
   __shared__ float part[2][NT / G][W > 1 ? W : 1];
   const int g = threadIdx.x % G, mine = threadIdx.x / G;
   long long row = (long long)blockIdx.x * (NT / G) + mine;
@@ -259,13 +259,13 @@ template <typename T, bool WHOLE, bool ADD>
 int launch(const NormArgs& a, cudaStream_t st) {
   const int cols = a.cols + (WHOLE ? 0 : 7);   // (a row may start in the middle of a word)
   auto go = [&](auto group) {
-    constexpr int G = decltype(group)::value, NT = G < 96 ? 128 : G;
+    constexpr int G = decltype(group)::value, NT = G < 128 ? 128 : G;
     return lin::launch_after("norm_fp8_kernel", norm_fp8_kernel<T, G, WHOLE, ADD>, dim3((unsigned)((a.rows + NT / G - 1) / (NT / G))),
                              NT, 0, st, 1, a);
   };
 #define VERACE_GROUP(G) \
   if (cols <= 32 * G) return go(std::integral_constant<int, G>())
-  VERACE_GROUP(8); VERACE_GROUP(16); VERACE_GROUP(32); VERACE_GROUP(64); VERACE_GROUP(96); VERACE_GROUP(128);
+  VERACE_GROUP(8); VERACE_GROUP(16); VERACE_GROUP(32); VERACE_GROUP(64); VERACE_GROUP(128);
   VERACE_GROUP(160); VERACE_GROUP(192); VERACE_GROUP(224); VERACE_GROUP(256); VERACE_GROUP(320); VERACE_GROUP(384);
   VERACE_GROUP(512); VERACE_GROUP(640); VERACE_GROUP(768);
 #undef VERACE_GROUP
