@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
     if (!GATED && e.residual)
       for (int i = tid - 64; i < 4 * tokens; i += NT - 64) {
         const int c = n0 + 32 * (i & 3);
-        if (c < p.N)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"((size_t)e.residual + ((i >> 2) * e.ld_res + c) * (e.type == VERACE_F32 ? 4 : 2)));
+        const size_t at = (size_t)e.residual + ((i >> 2) * e.ld_res + c) * (e.type == VERACE_F32 ? 4 : 2);
+        if (c < p.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
       }
   }
   const int quarter = warp & 3;

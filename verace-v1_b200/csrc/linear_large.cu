@@ -425,8 +425,8 @@ __device__ __forceinline__ void epilogue_block(const Epilogue& e, const Block& b
 
 // A warp's part of every tile of the pair: TMEM lanes 32 (warp % 4) ..., one half of the columns.
 template <bool GATED, bool WIDE, int BN, bool PARTS, typename Wait, typename Free>
-__device__ __forceinline__ void epilogue_tiles(const Args& p, const Maps& maps, uint32_t turn, uint32_t tmem, int pair, int pairs, int rank,
-                                               int warp, int lane, Wait&& wait, Free&& release) {
+__device__ __forceinline__ void epilogue_tiles(const Args& p, const Maps& maps, uint32_t turn, uint32_t tmem, int pair, int pairs,
+                                               int rank, int warp, int lane, Wait&& wait, Free&& release) {
   constexpr int HB = BN / 2, TN = GATED ? HB : BN, WIDTH = WIDE ? 32 : 64, PER = TN / 2 > WIDTH ? TN / 2 : WIDTH;
   const int half = (warp - 4) >> 2, first = half * PER, last = min(TN, first + PER);
   const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
@@ -723,7 +723,8 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       if (!PARTS) free(n);
     };
     if constexpr (PARTS) epilogue_tiles<GATED, true, BN, true>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
-    else if (p.e.type == VERACE_F32) epilogue_tiles<GATED, true, BN, false>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
+    else if (p.e.type == VERACE_F32)
+      epilogue_tiles<GATED, true, BN, false>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
     else epilogue_tiles<GATED, false, BN, false>(p, maps, turn, tmem, pair, pairs, rank, warp, lane, wait, release);
   }
   tc::fence_before_sync();
@@ -805,7 +806,8 @@ template <int BN>
 int by_kind(const Product& p, int s, cudaStream_t st) {
   if (p.parts && p.gated) return launch<false, false, false, true, BN, true>(p, s, st);
   if (p.parts && p.a_mn) return launch<false, true, true, false, BN, true>(p, s, st);
-  if (p.parts) return p.b_mn ? launch<false, false, true, false, BN, true>(p, s, st) : launch<false, false, false, false, BN, true>(p, s, st);
+  if (p.parts)
+    return p.b_mn ? launch<false, false, true, false, BN, true>(p, s, st) : launch<false, false, false, false, BN, true>(p, s, st);
   if (p.type == VERACE_E4M3)
     return p.gated ? launch<true, false, false, true, BN>(p, s, st) : launch<true, false, false, false, BN>(p, s, st);
   if (p.gated) return launch<false, false, false, true, BN>(p, s, st);

@@ -260,8 +260,8 @@ int launch(const NormArgs& a, cudaStream_t st) {
   const int cols = a.cols + (WHOLE ? 0 : 7);   // (a row may start in the middle of a word)
   auto go = [&](auto group) {
     constexpr int G = decltype(group)::value, NT = G < 128 ? 128 : G;
-    return lin::launch_after("norm_fp8_kernel", norm_fp8_kernel<T, G, WHOLE, ADD>, dim3((unsigned)((a.rows + NT / G - 1) / (NT / G))),
-                             NT, 0, st, 1, a);
+    const dim3 grid((unsigned)((a.rows + NT / G - 1) / (NT / G)));
+    return lin::launch_after("norm_fp8_kernel", norm_fp8_kernel<T, G, WHOLE, ADD>, grid, NT, 0, st, 1, a);
   };
 #define VERACE_GROUP(G) \
   if (cols <= 32 * G) return go(std::integral_constant<int, G>())
