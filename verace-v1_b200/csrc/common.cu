@@ -29,17 +29,32 @@ int check_launch(const char* what) {
   return VERACE_OK;
 }
 
+static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+// The driver's entry point wants a current context, which a thread has from its first call of the runtime that needs one.
+// Neither cudaGetDevice nor a block out of torch's cache is such a call, so a thread's first product may come here without
+// (autograd's own thread, a server's worker): the current device's context is bound then, and the map asked for again.
+static CUresult CUDAAPI encode_here(CUtensorMap* map, CUtensorMapDataType type, cuuint32_t rank, void* base,
+                                    const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                                    const cuuint32_t* steps, CUtensorMapInterleave interleave, CUtensorMapSwizzle swizzle,
+                                    CUtensorMapL2promotion promotion, CUtensorMapFloatOOBfill fill) {
+  CUresult r = g_encode(map, type, rank, base, dims, strides, box, steps, interleave, swizzle, promotion, fill);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = g_encode(map, type, rank, base, dims, strides, box, steps, interleave, swizzle, promotion, fill);
+  return r;
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult qr;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
         qr == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
-  return fn;
+  return g_encode ? encode_here : nullptr;
 }
 
 }  // namespace verace

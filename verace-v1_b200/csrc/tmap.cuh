@@ -6,7 +6,7 @@
 
 namespace verace {
 
-// nullptr when the driver does not provide the entry point.
+// The entry point (with a context bound first, on a thread that has none); nullptr when the driver does not provide it.
 PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder();
 
 }  // namespace verace
