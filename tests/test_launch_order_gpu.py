@@ -1,0 +1,74 @@
+"""Kernels that become resident before the one ahead of them ends: what that one writes last, and nothing runs in between,
+is read as it wrote it.  Each chain is held to the same chain with a wait on the host after every call."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import verace_v1_b200 as V
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dt=F32):
+    return torch.randn(*shape, device="cuda", generator=g).to(dt)
+
+
+def unit(g, *shape, dt):
+    return F.normalize(randn(g, *shape), dim=-1).to(dt)
+
+
+def both(chain):
+    """What the chain gives with a wait after every call, and without (three times)."""
+    want = chain(torch.cuda.synchronize)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = chain(lambda: None)
+        torch.cuda.synchronize()
+        assert len(got) == len(want)
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("b", [1, 3, 64])
+def test_sssd_steps_behind_one_another(b, dt):
+    """Steps on one state, their inputs all there beforehand."""
+    g = gen(b)
+    steps, h, d = 12, 8, 128
+    q, k, v = (unit(g, steps, b, h, d, dt=dt) for _ in range(3))
+    dl = 0.1 * torch.rand(steps, b, h, device="cuda", generator=g)
+    start = torch.eye(d, device="cuda").expand(b, h, d, d).contiguous()
+
+    def chain(wait):
+        psi, out = start.clone(), []
+        wait()
+        for t in range(steps):
+            out.append(V.launch_decode_step((q[t], k[t], v[t], dl[t], psi), None)[0])
+            wait()
+        return out + [psi]
+    both(chain)
+
+
+@pytest.mark.parametrize("rows", [128, 8 * 128])
+def test_sssd_state_from_a_product(rows):
+    """A first state that a product writes, straight before the step."""
+    g = gen(7)
+    b, h = rows // 128, 1
+    x, w = randn(g, rows, 2048, dt=BF16), randn(g, 128, 2048, dt=BF16)
+    q, k, v = (unit(g, b, h, 128, dt=BF16) for _ in range(3))
+    dl = 0.1 * torch.rand(b, h, device="cuda", generator=g)
+
+    def chain(wait):
+        out = []
+        for i in range(4):
+            psi = V.fused_linear(x, w, out_dtype=F32).view(b, h, 128, 128)
+            wait()
+            out += [V.launch_decode_step((q, k, v, dl, psi), None)[0], psi]
+            wait()
+        return out
+    both(chain)
