@@ -72,3 +72,35 @@ def test_sssd_state_from_a_product(rows):
             wait()
         return out
     both(chain)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [64, 128, 1024, 2048])
+@pytest.mark.parametrize("maker", ["linear", "gated", "norm"])
+def test_norm_weight_from_the_call_before(n, dt, maker):
+    """An adaptive norm: its weight is what the call straight before it writes."""
+    g = gen(n)
+    k = 4096
+    c, w, u = randn(g, 4, 1, k, dt=dt), randn(g, n, k, dt=dt) / 64, randn(g, n, k, dt=dt) / 64
+    x = randn(g, 300, n, dt=dt)
+    plain = torch.nn.RMSNorm(n, device="cuda", dtype=dt).requires_grad_(False)
+    h, y = randn(g, 4, 1, n, dt=dt), randn(g, 4, 1, n, dt=dt)
+
+    def chain(wait):
+        out, sums = [], torch.zeros(4, 1, n, device="cuda", dtype=dt)
+        norm = torch.nn.RMSNorm(n, device="cuda", dtype=dt).requires_grad_(False)
+        wait()
+        for i in range(4):
+            if maker == "linear":
+                made = V.fused_linear(c[i], w)
+            elif maker == "gated":
+                made = V.gated_linear(c[i], w, u)
+            else:
+                V.add_rmsnorm_fp8(h[i], y[i], plain, out=sums[i])
+                made = sums[i]
+            norm.weight = torch.nn.Parameter(made[0], requires_grad=False)
+            wait()
+            out.append(V.rmsnorm(x, norm))
+            wait()
+        return out
+    both(chain)

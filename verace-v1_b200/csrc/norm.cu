@@ -11,6 +11,9 @@
 // vector loads, fp32 sums by segmented shuffles.  For rows of up to 1024 the weights are
 // loaded together with the rows, so a small launch (a decode step's 64 rows) waits for
 // one round trip to memory before its reductions instead of one per weight vector.
+// rmsnorm is launched early (as a programmatic dependent): nothing is loaded there ahead of
+// the wait, since the kernel before it may write the weights as well as the rows, and nothing
+// through the read-only path, since that one is still writing while this one is resident.
 #include "common.cuh"
 
 namespace verace {
@@ -70,7 +73,7 @@ struct Raw8 {
 template <typename T>
 __device__ __forceinline__ void ldraw(const T* p, Raw8<T>& r) {
 #pragma unroll
-  for (int k = 0; k < (int)(sizeof(T) / 2); ++k) r.u[k] = __ldg(reinterpret_cast<const uint4*>(p) + k);
+  for (int k = 0; k < (int)(sizeof(T) / 2); ++k) r.u[k] = reinterpret_cast<const uint4*>(p)[k];
 }
 
 template <typename T>
@@ -94,7 +97,7 @@ constexpr bool prefetch_w() { return V <= 4; }
 
 // the lane's weight chunks (when prefetch_w<V>() and w is given)
 template <typename T, int L, int V>
-__device__ __forceinline__ void load_w(const T* __restrict__ w, int sl, int nc, Raw8<T> (&wr)[V]) {
+__device__ __forceinline__ void load_w(const T* w, int sl, int nc, Raw8<T> (&wr)[V]) {
   if constexpr (prefetch_w<V>()) {
     if (w) {
 #pragma unroll
@@ -107,7 +110,7 @@ __device__ __forceinline__ void load_w(const T* __restrict__ w, int sl, int nc, 
 // x[V][8] <- RMSNorm(x) (with weight w when given; its chunks in wr when prefetched),
 // rounded as torch does
 template <typename T, int L, int V>
-__device__ __forceinline__ void rms_apply(float (&x)[V][8], const T* __restrict__ w, const Raw8<T> (&wr)[V], int sl,
+__device__ __forceinline__ void rms_apply(float (&x)[V][8], const T* w, const Raw8<T> (&wr)[V], int sl,
                                           int nc, int cols, float eps) {
   float ss = 0.f;
 #pragma unroll
@@ -137,18 +140,20 @@ __device__ __forceinline__ void rms_apply(float (&x)[V][8], const T* __restrict_
 
 template <typename T, int L, int V>
 __global__ void __launch_bounds__(NT)
-rmsnorm_kernel(const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ y, long long rows, int cols,
-               float eps) {
+rmsnorm_kernel(const T* x, const T* w, T* y, long long rows, int cols, float eps) {
   const int lane = threadIdx.x & 31;
   const long long row = ((long long)blockIdx.x * NT + threadIdx.x) / L;
   const int sl = lane % L, nc = cols / 8;
   const bool act = row < rows;
   const T* xr = x + (act ? row : 0) * cols;
+  // the weights on their way to the L2, which holds no stale values
+  if (w)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (sl + L * i < nc) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + 8 * (sl + L * i)));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Raw8<T> wr[V];
   load_w<T, L, V>(w, sl, nc, wr);
-  // launched as a programmatic dependent of the kernel before it (the SSSD decode step ahead
-  // of its per-head norm triggers early): the weights above need nothing from it, x does
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   float v[V][8];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
