@@ -104,3 +104,40 @@ def test_norm_weight_from_the_call_before(n, dt, maker):
             wait()
         return out
     both(chain)
+
+
+@pytest.mark.parametrize("b,D,P", [(1, 128, 4), (4, 256, 8)])
+@pytest.mark.parametrize("projected", [False, True])
+def test_hologram_planes_from_the_call_before(b, D, P, projected):
+    """The deferred hologram step straight behind what writes its planes: a product, and a flush."""
+    g = gen(b + D)
+    x, w = randn(g, b * D, 1024, dt=BF16), randn(g, D, 1024, dt=BF16) / 32
+    q, k, v = (unit(g, b, D, dt=BF16) for _ in range(3))
+    gamma = 0.1 * torch.rand(b, device="cuda", generator=g)
+    rows = randn(g, b, 3 * D + 8, dt=BF16)
+    empty = V.pending_storage(b, D, P)
+    hi = torch.zeros(b, D, D, device="cuda")
+
+    def chain(wait):
+        pending, im, out = empty.clone(), hi.clone(), []
+        wait()
+
+        def step(re):
+            if projected:
+                out.append(V.launch_decode_cham_lazy_projected(rows, re, im, pending, P))
+            else:
+                out.append(V.launch_decode_cham_lazy(q, k, v, gamma, re, im, pending, P))
+            wait()
+        for i in range(3):
+            re = V.fused_linear(x, w, out_dtype=F32).view(b, D, D)
+            wait()
+            step(re)
+            step(re)
+            V.decode.flush_pending(re, im, pending, P)
+            wait()
+            step(re)
+            V.decode.flush_pending(re, im, pending, P)
+            wait()
+            out.append(re)
+        return out + [im, pending]
+    both(chain)

@@ -708,10 +708,11 @@ __global__ void __launch_bounds__(DT) lazy_pre_kernel(LazyArgs A) {
   const int item = blockIdx.x / P, j = blockIdx.x % P;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   // launched as a programmatic dependent of the projection epilogue (k, v, q) or, PROJ, of
-  // the projection itself; the stripe kernel that follows may start its hologram loads
-  // once every CTA here has started
-  asm volatile("griddepcontrol.launch_dependents;");
+  // the projection itself.  The stripe kernel that follows starts its hologram loads as soon
+  // as it runs: it is let in behind the wait, so that whatever was before this kernel, which
+  // may have written the planes (a flush, a product), is complete for it too.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   const int p = A.pcount[item];
   if (j == 0 && tid == 0) A.pcold[item] = p;
   const bool dots = p < P && j < p;   // (a folding step needs none of them)
