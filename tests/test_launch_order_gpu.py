@@ -141,3 +141,27 @@ def test_hologram_planes_from_the_call_before(b, D, P, projected):
             out.append(re)
         return out + [im, pending]
     both(chain)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(300, 9000, 100), (200, 4096, 64)])
+def test_partial_sums_in_chains(m, k, n, dt):
+    """Sums split over K and the bias gradient's chunks, whose joins are resident while the parts are written, in workspaces
+    that the calls hand on to each other."""
+    g = gen(m)
+    w, u, b = randn(g, n, k, dt=dt) / 64, randn(g, n, k, dt=dt) / 64, randn(g, n, dt=dt)
+    x = [randn(g, m, k, dt=dt) for _ in range(4)]
+    d = [randn(g, m, n, dt=dt) for _ in range(4)]
+
+    def chain(wait):
+        out = []
+        for i in range(4):
+            out += [V.fused_linear(x[i], w, b, activation="silu", residual=d[i]), V.gated_linear(x[i], w, u)]
+            wait()
+            leaves = [t.detach().requires_grad_() for t in (x[i], w, b)]
+            y = V.fused_linear(*leaves, activation="gelu")
+            wait()
+            out += torch.autograd.grad(y, leaves, d[i])
+            wait()
+        return out
+    both(chain)

@@ -292,10 +292,10 @@ __global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
   a.partial[chunk * a.n + n] = s;
 }
 
-// the sums of the chunks, always in the same order: 32 columns a CTA, eight runs of chunks each
+// the sums of the chunks, always in the same order: 32 columns a CTA, eight runs of chunks each.  (`partial` is still being
+// written while this kernel is resident: no restricted pointer.)
 template <typename T>
-__global__ void __launch_bounds__(256) sum_chunks(const float* __restrict__ partial, long long chunks, long long n,
-                                                  T* __restrict__ out) {
+__global__ void __launch_bounds__(256) sum_chunks(const float* partial, long long chunks, long long n, T* out) {
   depend();
   __shared__ float part[8][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;

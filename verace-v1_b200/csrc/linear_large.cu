@@ -816,9 +816,10 @@ int by_kind(const Product& p, int s, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ split K
-// The outputs from the partial sums, added in order; four columns a thread.
+// The outputs from the partial sums, added in order; four columns a thread.  (`part` is no restricted pointer: the kernel
+// before this one still writes there while this one is resident, so these are no loads of constant memory.)
 template <bool GATED>
-__global__ void __launch_bounds__(256) join_splits(const float* __restrict__ part, int splits, long long partial, long long up,
+__global__ void __launch_bounds__(256) join_splits(const float* part, int splits, long long partial, long long up,
                                                    Epilogue e, long long M, long long N, long long quads) {
   depend();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
