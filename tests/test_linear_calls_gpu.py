@@ -71,3 +71,54 @@ def test_first_backward_of_a_process(wants):
     """Autograd's own thread, whose first call is a product of operands as they lie (no bias, no activation)."""
     r = subprocess.run([sys.executable, "-c", FIRST % wants], cwd=HERE, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
+
+
+def in_place_calls(x, norm):
+    """(name, call) of what writes x through its pointer."""
+    y = torch.ones_like(x)
+    yield "add_rmsnorm_fp8", lambda: V.add_rmsnorm_fp8(x, y, norm)
+    yield "add_rmsnorm_fp8 out", lambda: V.add_rmsnorm_fp8(y, y, norm, out=x)
+    yield "add_rmsnorm", lambda: V.add_rmsnorm(x, y, out_norm=norm)
+    rows, ids = x.view(-1, x.shape[-1]), torch.zeros(x.numel() // x.shape[-1], 1, dtype=torch.int64, device="cuda")
+    yield "process_logits", lambda: V.process_logits(rows, ids, presence_penalty=0.5, out=rows)
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("shape", [(6, 64), (2, 3, 64)])
+def test_writing_what_a_backward_has_saved_is_refused(which, shape):
+    """As behind torch's own in-place operations: an input that trainable weights have read may not change before the
+    backward pass has."""
+    g = gen(3)
+    norm = torch.nn.RMSNorm(64, device="cuda", dtype=BF16).requires_grad_(False)
+    for gated in (False, True):
+        x, w, u = randn(g, *shape, dt=BF16), randn(g, 96, 64, dt=BF16).requires_grad_(), randn(g, 96, 64, dt=BF16)
+        y = V.gated_linear(x, w, u) if gated else V.fused_linear(x, w)
+        name, call = list(in_place_calls(x, norm))[which]
+        call()
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.sum().backward()
+        y = V.gated_linear(x, w, u) if gated else V.fused_linear(x, w)      # (and one without a write between is not)
+        y.sum().backward()
+        assert w.grad.isfinite().all()
+
+
+def test_states_of_a_decode_step_count_their_versions():
+    g = gen(4)
+    q, k, v = (randn(g, 2, 1, 128, dt=BF16) for _ in range(3))
+    psi, gate = torch.eye(128, device="cuda").expand(2, 1, 128, 128).contiguous(), torch.rand(2, 1, device="cuda", generator=g)
+    re, im, pending = psi.view(2, 128, 128).clone(), torch.zeros(2, 128, 128, device="cuda"), V.pending_storage(2, 128, 4)
+    was = [t._version for t in (psi, re, im, pending)]
+    V.launch_decode_step((q, k, v, gate, psi), (q.view(2, 128), k.view(2, 128), v.view(2, 128), gate.view(2), re, im))
+    assert psi._version > was[0] and re._version > was[1] and im._version > was[2]
+    was = [t._version for t in (re, im, pending)]
+    V.launch_decode_cham_lazy(q.view(2, 128), k.view(2, 128), v.view(2, 128), gate.view(2), re, im, pending, 4)
+    assert all(t._version > v for t, v in zip((re, im, pending), was))
+    was = [t._version for t in (re, im, pending)]
+    V.flush_pending(re, im, pending, 4)
+    assert all(t._version > v for t, v in zip((re, im, pending), was))
+    with torch.inference_mode():        # (tensors without a version are written all the same)
+        h = torch.ones(2, 64, device="cuda", dtype=BF16)
+        V.add_rmsnorm_fp8(h, h, torch.nn.RMSNorm(64, device="cuda", dtype=BF16))
+        assert (h == 2).all()
+    V.add_rmsnorm_fp8(h, h, torch.nn.RMSNorm(64, device="cuda", dtype=BF16).requires_grad_(False))
+    assert (h == 4).all()

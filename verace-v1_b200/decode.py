@@ -34,6 +34,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
+from ._launch import wrote
 from ._lib import BF16, F16, F32, check, lib
 
 _DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -123,6 +124,7 @@ def launch_decode_step(sssd: Optional[Sequence[torch.Tensor]],
                                   workspace.data_ptr(), workspace.numel(),
                                   torch.cuda.current_stream(dev).cuda_stream)
     check(rc, "verace_decode_step")
+    wrote([t for state in (sssd and sssd[4:], cham and cham[4:]) for t in state or ()])
     return sout, cout
 
 
@@ -171,6 +173,7 @@ def launch_decode_cham_lazy(q, k, v, gamma, H_real, H_imag, pending: torch.Tenso
                                            out.data_ptr(), b, D, _DTYPE[dt], workspace.data_ptr(),
                                            workspace.numel(), torch.cuda.current_stream(q.device).cuda_stream)
     check(rc, "verace_decode_cham_lazy")
+    wrote((H_real, H_imag, pending))
     return out
 
 
@@ -199,6 +202,7 @@ def launch_decode_cham_lazy_projected(y: torch.Tensor, H_real, H_imag, pending: 
                                                      _DTYPE[y.dtype], workspace.data_ptr(), workspace.numel(),
                                                      torch.cuda.current_stream(y.device).cuda_stream)
     check(rc, "verace_decode_cham_lazy_projected")
+    wrote((H_real, H_imag, pending))
     return out
 
 
@@ -209,6 +213,7 @@ def flush_pending(H_real: torch.Tensor, H_imag: torch.Tensor, pending: torch.Ten
         rc = lib().verace_decode_cham_flush(H_real.data_ptr(), H_imag.data_ptr(), pending.data_ptr(), P, b, D,
                                             torch.cuda.current_stream(H_real.device).cuda_stream)
     check(rc, "verace_decode_cham_flush")
+    wrote((H_real, H_imag, pending))
 
 
 def device_status(device=None) -> int:

@@ -18,6 +18,7 @@ from typing import Optional, Tuple
 
 import torch
 
+from ._launch import wrote
 from ._lib import BF16, F16, F32, check, lib
 
 _DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -287,6 +288,7 @@ def add_rmsnorm(h: torch.Tensor, y: torch.Tensor, y_norm: Optional[torch.nn.Modu
         rc = lib().verace_add_rmsnorm(h.data_ptr(), y.data_ptr(), 1 if y_norm is not None else 0, wy, ey, wn, en,
                                       _ptr(n), h.numel() // cols, cols, _DTYPE[h.dtype], _stream(h.device))
     check(rc, "verace_add_rmsnorm")
+    wrote(h)
     return n
 
 

@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from ._launch import current, raw_stream
+from ._launch import current, raw_stream, wrote
 from ._lib import E4M3, F32, check, lib
 from .int4 import _require_no_grad
 from .kernels import _DTYPE, _norm_args
@@ -422,7 +422,9 @@ def add_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, norm: nn.RMSNorm, *, out: 
         assert out.shape == h.shape and out.dtype is h.dtype and out.device == dev, \
             "the sum goes to a tensor of h's shape, dtype and device"
     assert out.is_contiguous(), "the sum goes to a contiguous tensor"
-    return _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, norm, return_norm)
+    made = _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, norm, return_norm)
+    wrote(out)
+    return made
 
 
 # ---------------------------------------------------------------------------- modules with 8-bit weights

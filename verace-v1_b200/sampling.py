@@ -11,7 +11,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._lib import F32, check, lib
-from ._launch import current, raw_stream
+from ._launch import current, raw_stream, wrote
 from .int4 import _require_no_grad
 from .kernels import _DTYPE
 
@@ -103,7 +103,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     if not ld:
         assert out is not logits, "in-place processing needs dense rows"
         logits, ld = logits.contiguous(), max(v, 1)
-    if out is None:
+    given = out is not None
+    if not given:
         if out_dtype is None or out_dtype is dt:
             out, ocode = logits.new_empty((b, v)), code
         elif out_dtype is torch.float32:
@@ -180,6 +181,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
                                      qp, rp, rs, pp, ps, fp, fs, ip, vp, nb, b64, ap, ald, raw_stream(index))
     if rc:
         check(rc, "verace_logits_process")
+    if given:
+        wrote(out)
     return out
 
 
