@@ -397,8 +397,8 @@ VERACE_API int verace_rmsnorm_fp8(const void* h, const void* y, void* sum, const
  * Backward, from dout [m, n] (out_dtype), dense: dx [m, k], dw [n, k], dbias [n] (dtype, dense; NULL: not
  *   computed); the residual's gradient is dout.  pre may be NULL with VERACE_ACT_NONE.
  * Sums are fp32 and outputs are rounded once; in a backward call act'(.) times dout is rounded to dtype
- * before it is multiplied.  fp32 operands enter as three bf16 parts (24 bits; an infinity gives
- * NaN).  Sizes up to 2^24.  Workspace: the bytes of the *_workspace query; calls sharing one must not overlap.
+ * before it is multiplied.  fp32 operands enter as three bf16 parts (24 bits of every finite value; an infinity gives
+ * NaN in every output that it enters), but for up to 24 rows of x (gated: 16), which take them as they are.  Sizes up to 2^24.  Workspace: the bytes of the *_workspace query; calls sharing one must not overlap.
  * ---------------------------------------------------------------------------- */
 enum {
   VERACE_ACT_NONE = 0, VERACE_ACT_RELU = 1, VERACE_ACT_SILU = 2, VERACE_ACT_GELU = 3,   /* gelu: by erf */

@@ -11,8 +11,10 @@
 // operand is transposed in memory.  The bias gradient is summed in the pass, in fp32 and in a
 // fixed order (32 rows at a time, then the partial sums).
 //
-// fp32 operands are split into three bf16 parts first (x = h + m + l, 24 bits), and the product
-// takes the six pairs of parts down to 2^-24 of the largest (hh, hm, mh, hl, mm, lh).
+// fp32 operands are split into three bf16 parts first (x = h + 2^-8 m + 2^-16 l, 24 bits; the powers of two keep the
+// lower parts of small values inside of bf16's range), and the product takes the six pairs of parts down to 2^-24 of the
+// largest (hh, hm, mh, hl, mm, lh).  Exact for every finite value: one that rounds to more than bf16's largest has that
+// as its part, and the rest in the next ones.  An infinity's second part is NaN, and so is every output that it enters.
 #include "linear_tc.cuh"
 
 #include <algorithm>
@@ -43,21 +45,24 @@ __device__ __forceinline__ void load8(const T* row, long long c, long long cols,
     for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
   }
 }
+constexpr float BF16_MOST = 0x1.fep127f;
 // 8 values as an operand of the products: rounded to T, or split into three parts `piece` apart
 template <typename T>
 __device__ __forceinline__ void store_operand(Part<T>* o, long long piece, const float (&v)[8]) {
   if constexpr (split_v<T>) {
-    float r[8];
+    float r[8], h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = v[j];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const uint4 w = pack8<__nv_bfloat16>(r);
+      // (an infinity stays one)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = fabsf(r[j]) > BF16_MOST && fabsf(r[j]) < INFINITY ? copysignf(BF16_MOST, r[j]) : r[j];
+      const uint4 w = pack8<__nv_bfloat16>(h);
       *reinterpret_cast<uint4*>(o + i * piece) = w;
-      float h[8];
       unpack8<__nv_bfloat16>(w, h);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] -= h[j];
+      for (int j = 0; j < 8; ++j) r[j] = (r[j] - h[j]) * 256.f;
     }
   } else {
     *reinterpret_cast<uint4*>(o) = pack8<T>(v);

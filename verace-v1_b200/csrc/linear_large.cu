@@ -16,7 +16,8 @@
 // registers.  A sum of two products (the input gradient of a gated block) is two runs over K.
 //
 // fp32 operands come as three bf16 parts, three stages for 64 values of K (a stage holds one part of A and of B), and
-// the MMAs take six pairs of them, the smallest first.  The tensor core cuts its sums to fp32 after every step instead
+// the MMAs take six pairs of them, the smallest first: the pairs of one order lie 2^8 above the next, by which the sums so
+// far are brought down as the next order begins.  The tensor core cuts its sums to fp32 after every step instead
 // of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the result); so after every 64 values of K
 // the epilogue's warps add them up in registers, rounding, while the next 64 run into the other set.
 //
@@ -92,16 +93,21 @@ __device__ __forceinline__ void load_box(void* smem, const CUtensorMap* map, int
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar0)
       : "memory");
 }
-template <bool F8>
+// (SHIFT: the sums so far are multiplied by 2^-SHIFT)
+template <bool F8, int SHIFT = 0>
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if constexpr (F8)
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
                  "r"(accumulate));
-  else
+  else if constexpr (SHIFT == 0)
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
                  "r"(accumulate));
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %5;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate), "n"(SHIFT));
 }
 // arrive on `bar` in both CTAs once the MMAs issued so far are done
 __device__ __forceinline__ void commit_pair(uint64_t* bar) {
@@ -593,19 +599,22 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
       if (rank == 0) {   // ---- MMAs of the pair.  The whole warp walks the loop, so that the operands sit in uniform registers:
         // by one thread's own loop a step of four MMAs took 657 clocks, the MMAs themselves take 512
         const bool lead = elect();
+        constexpr std::integral_constant<int, 0> NONE;
+        constexpr std::integral_constant<int, PARTS ? 8 : 0> PART;
         int i = 0, n = 0;
         uint32_t phase = 0;
         bool ok = true;
         const int mine = (p.tiles - pair + pairs - 1) / pairs * sets;   // sets to fill
         // four MMAs: 128 bytes of K of stage ia's A and stage ib's B
-        auto step = [&](uint32_t d, int ia, int ib, bool more) {
+        auto step = [&](uint32_t d, int ia, int ib, bool more, auto shift) {
           const uint32_t a = tc::smem_addr(sm + ia * S::STAGE), bb = tc::smem_addr(sm + ib * S::STAGE) + 16384;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             // K-major: 32 bytes along the rows; MN-major: 16 rows of 128 bytes
             const uint64_t da = AMN ? tc::sdesc_sw128(a + k * 2048, 8192, 1024) : tc::sdesc_sw128(a + k * 32, 16, 1024);
             const uint64_t db = BMN ? tc::sdesc_sw128(bb + k * 2048, 8192, 1024) : tc::sdesc_sw128(bb + k * 32, 16, 1024);
-            mma_pair<F8>(d, da, db, p.idesc, more || k > 0 ? 1u : 0u);
+            if (k == 0) mma_pair<F8, decltype(shift)::value>(d, da, db, p.idesc, more ? 1u : 0u);
+            else mma_pair<F8>(d, da, db, p.idesc, 1u);
           }
         };
         for (; n < mine && ok; ++n) {
@@ -626,7 +635,7 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
               }
               tc::fence_after_sync();
               if (lead) {
-                step(d, i, i, s > 0);
+                step(d, i, i, s > 0, NONE);
                 commit_pair(&empty[i]);
               }
               __syncwarp();
@@ -640,15 +649,15 @@ large_product(const __grid_constant__ Maps maps, const __grid_constant__ Args p)
               }
               if (!ok) break;
               tc::fence_after_sync();
-              if (lead) {   // parts: 0 the high one
-                step(d, at[2], at[0], false);
-                step(d, at[1], at[1], true);
-                step(d, at[0], at[2], true);
+              if (lead) {   // parts: 0 the high one, 1 and 2 times 2^8 and 2^16
+                step(d, at[2], at[0], false, NONE);
+                step(d, at[1], at[1], true, NONE);
+                step(d, at[0], at[2], true, NONE);
                 commit_pair(&empty[at[2]]);
-                step(d, at[1], at[0], true);
-                step(d, at[0], at[1], true);
+                step(d, at[1], at[0], true, PART);
+                step(d, at[0], at[1], true, NONE);
                 commit_pair(&empty[at[1]]);
-                step(d, at[0], at[0], true);
+                step(d, at[0], at[0], true, PART);
                 commit_pair(&empty[at[0]]);
               }
               __syncwarp();

@@ -190,7 +190,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
                  out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """act(x weightᵀ + bias) + residual in one kernel: x [..., k], weight [n, k], bias [n] (x's dtype),
     residual [..., n] (the output's dtype); activation None, "relu", "silu", "gelu" (by erf) or "gelu_tanh".
-    The output has x's dtype or, with ``out_dtype=torch.float32``, fp32; sums are fp32, rounded once.
+    The output has x's dtype or, with ``out_dtype=torch.float32``, fp32; sums are fp32, rounded once.  fp32 operands keep
+    their 24 bits; an infinity in them gives NaN (that of the formula with up to 24 rows of x).
 
     With float8_e4m3fn x and weight, ``x_scale`` (one fp32 value a row of x) and ``w_scale`` [n] multiply
     them; the output is then fp32, bf16 or fp16 (``out_dtype``, else the residual's dtype, else bf16), the bias of
