@@ -88,7 +88,7 @@ def test_sums_of_small_and_large_values(scale):
     want = x.to(F64) @ w.to(F64).t()
     assert off(V.fused_linear(x, w), want) < 1e-6
     assert off(V.fused_linear(w, x), want.t()) < 1e-6
-    a, b = x.requires_grad_(), w.requires_grad_()
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
     d = randn(g, 300, 130) * 2.0 ** -6
     dx, dw = torch.autograd.grad(V.fused_linear(a, b), (a, b), d)
     assert off(dw, d.to(F64).t() @ x.to(F64)) < 1e-6 and off(dx, d.to(F64) @ w.to(F64)) < 1e-6
@@ -116,3 +116,109 @@ def test_an_infinity_in_fp32():
         y = V.fused_linear(x[keep], u)
         assert torch.equal(y[:, [i for i in range(96) if i != 5]], V.fused_linear(x[keep], w)[:, [i for i in range(96) if i != 5]])
         assert y[:, 5].isnan().all() if len(keep) > 24 else torch.equal(y[:, 5], math.inf * x[keep][:, 11].sign())
+
+
+# ---------------------------------------------------------------------------- errors in the 2-norm
+LONG = [1001, 9000, 20000]
+
+
+@pytest.mark.parametrize("k", LONG)
+@pytest.mark.parametrize("m", [1, 8, 24, 30, 300])
+def test_fp32_operands_keep_their_bits(m, k):
+    """Two parts instead of three are 3.4e-6 off, any one of the six pairs left out at least 2.4e-6 (on CPU, these values)."""
+    g = gen(k)
+    x, w, u, b = randn(g, m, k), randn(g, 100, k), randn(g, 100, k), randn(g, 100)
+    s, t = x.to(F64) @ w.to(F64).t(), x.to(F64) @ u.to(F64).t()
+    assert off(V.fused_linear(x, w), s) < 1e-6
+    r = randn(g, m, 100)
+    assert off(V.fused_linear(x, w, b, activation="relu", residual=r), torch.relu(s + b) + r) < 1e-6
+    # (a product of two sums: their errors side by side)
+    assert off(V.gated_linear(x, w, u, activation="relu"), torch.relu(s) * t) < 1.5e-6
+
+
+@pytest.mark.parametrize("m,k,n", [(1001, 60, 300), (200, 60, 9000), (20000, 40, 64), (64, 300, 20000)])
+def test_fp32_gradients_keep_their_bits(m, k, n):
+    """dx sums over n, dw and the bias over m.  (Gated: dg and du are products of four fp32 values, each sum 2e-7 off.)"""
+    g = gen(m)
+    x, w, u, b = (t.requires_grad_() for t in (randn(g, m, k), randn(g, n, k) / k ** 0.5, randn(g, n, k) / k ** 0.5, randn(g, n)))
+    d = randn(g, m, n)
+    x64, w64, u64, d64 = (t.detach().to(F64) for t in (x, w, u, d))
+    dx, dw, db = torch.autograd.grad(V.fused_linear(x, w, b), (x, w, b), d)
+    assert off(dx, d64 @ w64) < 1e-6 and off(dw, d64.t() @ x64) < 1e-6 and off(db, d64.sum(0)) < 1e-6
+    dx, dw, du = torch.autograd.grad(V.gated_linear(x, w, u, activation="relu"), (x, w, u), d)
+    a, up = x64 @ w64.t(), x64 @ u64.t()
+    pg, pu = torch.where(V.fused_linear(x, w).detach() > 0, d64 * up, 0.0), d64 * torch.relu(a)
+    assert off(dx, pg @ w64 + pu @ u64) < 1.5e-6 and off(dw, pg.t() @ x64) < 1.5e-6 and off(du, pu.t() @ x64) < 1.5e-6
+
+
+@pytest.mark.parametrize("k", LONG)
+@pytest.mark.parametrize("m", [3, 30, 150, 300])
+@pytest.mark.parametrize("dt", [BF16, F16, torch.float8_e4m3fn])
+def test_16_and_8_bit_operands_summed_in_fp32(m, k, dt):
+    g = gen(m + k)
+    bound = k / 24 * 2.0 ** -23 + 2e-7
+    if dt is torch.float8_e4m3fn:
+        (x, sx), (w, sw) = fp8_rows(randn(g, m, k)), fp8_rows(randn(g, 100, k))
+        got, want = V.fused_linear(x, w, x_scale=sx, w_scale=sw, out_dtype=F32), dequantised(x, sx) @ dequantised(w, sw).t()
+    else:
+        x, w = randn(g, m, k, dt=dt), randn(g, 100, k, dt=dt)
+        got, want = V.fused_linear(x, w, out_dtype=F32), x.to(F64) @ w.to(F64).t()
+        a = V.gated_linear(x, w, w, activation="silu", out_dtype=F32)
+        # (16 more 2^-24 for the exponential; act'(z) z <= 1.1 act(z) but where act is small)
+        assert off(a, act64("silu", want) * want) < 2.5 * bound + 1e-6
+    assert off(got, want) < bound
+
+
+# ---------------------------------------------------------------------------- sums that are exact
+def whole(g, most, *shape, dt=F32):
+    return torch.randint(-most, most + 1, shape, device="cuda", generator=g).to(F32).to(dt)
+
+
+def exact_operands(g, dt, m, n, k):
+    """Whole numbers, every partial sum of whose products is one below 2^24 (fp32: x of two parts)."""
+    if dt is F32:
+        return whole(g, 511, m, k), whole(g, 1, n, k)
+    if dt is torch.float8_e4m3fn:
+        return whole(g, 8, m, k, dt=dt), whole(g, 8, n, k, dt=dt)
+    return whole(g, 16, m, k, dt=dt), whole(g, 16, n, k, dt=dt)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("m", [1, 3, 20, 40, 150, 300])
+@pytest.mark.parametrize("k", [64, 257, 9008, 20000])
+def test_whole_numbers_come_out_exactly(dt, m, k):
+    """One stage, split or part of the sum lost or counted twice shows."""
+    for n in (70, 300):
+        g = gen(m + n + k)
+        x, w = exact_operands(g, dt, m, n, k)
+        ones = torch.ones(max(m, n), device="cuda")
+        scales = {"x_scale": ones[:m], "w_scale": ones[:n]} if dt is torch.float8_e4m3fn else {}
+        want = x.to(F64) @ w.to(F64).t()
+        assert torch.equal(V.fused_linear(x, w, out_dtype=F32, **scales).to(F64), want)
+        first = x.to(F32)
+        first[:, 0] = 1
+        u = torch.zeros(n, k, device="cuda")
+        u[:, 0] = 1                                  # the up projection gives 1
+        x, u = first.to(dt), u.to(dt)
+        want = torch.relu(x.to(F64) @ w.to(F64).t())
+        scales = {"x_scale": ones[:m], "gate_scale": ones[:n], "up_scale": ones[:n]} if scales else {}
+        assert torch.equal(V.gated_linear(x, w, u, activation="relu", out_dtype=F32, **scales).to(F64), want)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(3, 70, 257), (150, 70, 9008), (300, 130, 1000), (20000, 70, 64), (9000, 33, 131)])
+def test_whole_gradients_come_out_exactly(dt, m, k, n):
+    g = gen(m + k + n)
+    x, w = exact_operands(g, dt, m, n, k)
+    b, d = torch.zeros(n, device="cuda", dtype=dt), whole(g, 1, m, n, dt=dt)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(V.fused_linear(*leaves), leaves, d)
+    d64, x64, w64 = (t.detach().to(F64) for t in (d, x, w))
+    assert torch.equal(dx, (d64 @ w64).to(dt)) and torch.equal(dw, (d64.t() @ x64).to(dt)) and torch.equal(db, d64.sum(0).to(dt))
+    u = torch.zeros(n, k, device="cuda", dtype=dt)
+    u[:, 0] = 1
+    with torch.no_grad():
+        x[:, 0] = 1
+    dw, = torch.autograd.grad(V.gated_linear(x, w, u, activation="relu"), w, d)
+    live = (x.detach().to(F64) @ w64.t() > 0).to(F64)
+    assert torch.equal(dw, ((d64 * live).t() @ x.detach().to(F64)).to(dt))
