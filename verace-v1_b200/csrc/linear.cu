@@ -214,14 +214,15 @@ bool by_dots(long long m, long long n, long long k, int type, int weights) {
 // 52.7 and 59.8, 160 x 1024 x 4096 8.4 and 8.2, but 200 x 4096 x 32000 63.1 and 60.4; gated 128 x 4096 x 8192 30.9 and 33.8,
 // 160 x 4096 x 32000 106 and 114, of small weights 112 x 1024 x 4096 10.5 and 10.5, 128 x 4096 x 1024 13.4 and 12.4; e4m3:
 // 160 x 4096 x 8192 13.8 and 14.7, gated 19.7 and 23.1).
-bool by_few(long long M, long long N, long long K, bool gated, int type, bool a_mn) {
-  return !a_mn && type != VERACE_F32 && M <= (gated && N * K <= 4 << 20 ? 112 : FEW);
+bool by_few(long long M, long long N, long long K, int segments, bool gated, int type, bool a_mn) {
+  return !a_mn && type != VERACE_F32 && M <= (gated && N * K <= 4 << 20 ? 112 : FEW) &&
+         K * segments <= run_of(type) * few_splits(N, K, segments, type);
 }
 
 // Workspace of a product's partial sums.
 size_t partial_bytes(long long M, long long N, long long K, int sums, int nz, bool gated, int type, bool a_mn) {
   const bool parts = type == VERACE_F32;
-  return by_few(M, N, K, gated, type, a_mn) ? 0 : split_bytes(M, N, K, sums, nz, gated, parts ? VERACE_BF16 : type, parts);
+  return by_few(M, N, K, sums, gated, type, a_mn) ? 0 : split_bytes(M, N, K, sums, nz, gated, parts ? VERACE_BF16 : type, parts);
 }
 
 int run_product(Product& p, cudaStream_t st) {
@@ -236,7 +237,7 @@ int run_product(Product& p, cudaStream_t st) {
     }
     return VERACE_OK;
   }
-  const bool few = by_few(p.M, p.N, p.K, p.gated, p.type, p.a_mn);
+  const bool few = by_few(p.M, p.N, p.K, p.segments, p.gated, p.type, p.a_mn);
   p.parts = p.type == VERACE_F32;
   if (p.parts) p.type = VERACE_BF16;
   return few ? product_few(p, st) : product_large(p, st);

@@ -33,7 +33,7 @@ constexpr int NT = 256, ROWS = 128, MAX_STAGES = 8;
 // shared memory for stages, or for the sums of up to FEW tokens, of a CTA that has an SM to itself, and of one that
 // shares it (228 KB an SM, less 1 KB a CTA that the system takes, 2 KB of barriers and scales and 1 KB to align the stages)
 constexpr int ROOM = 224 * 1024, HALF_ROOM = 110 * 1024;
-constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum may run over 2^24 values: 0.1 s)
+constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum runs over up to run_of(type) values)
 
 struct Maps {
   CUtensorMap w[2], x;
@@ -340,8 +340,7 @@ int launch(const Product& p, cudaStream_t st) {
   a.a_first = p.a_first;
   a.steps = a.kblocks * p.segments;
   a.tiles_n = (int)((p.N + ROWS - 1) / ROWS);
-  a.ck = 1;
-  while (a.ck < 8 && a.tiles_n * a.ck * 2 <= 148 && a.steps >= a.ck * 4) a.ck *= 2;
+  a.ck = few_splits(p.N, p.K, p.segments, p.type);
   a.per = (a.steps + a.ck - 1) / a.ck;
   a.stage = ROWS * 128 * (GATED ? 2 : 1) + a.mp * 128;
   // Two CTAs an SM while that leaves a CTA three stages (gated, 64 x 4096 x 32000: 89 us against 90, 48 of it for 8 bits

@@ -19,7 +19,8 @@
 // the MMAs take six pairs of them, the smallest first: the pairs of one order lie 2^8 above the next, by which the sums so
 // far are brought down as the next order begins.  The tensor core cuts its sums to fp32 after every step instead
 // of rounding them, which over a whole K adds up (K = 1001: 6e-6 of the result); so after every 64 values of K
-// the epilogue's warps add them up in registers, rounding, while the next 64 run into the other set.
+// the epilogue's warps add them up in registers, rounding, while the next 64 run into the other set.  Sums of 16- and
+// 8-bit operands stay there for up to run_of(type) values (linear_tc.cuh); K beyond that is split.
 //
 // Epilogue: a thread holds a row of the tile (as TMEM gives it), 64 columns at a time (32 of fp32),
 // applies scales, bias and activation and puts the rounded values into the warp's block of shared memory, from where
@@ -42,7 +43,7 @@ namespace {
 using namespace lin;
 
 constexpr int NT = 384, EPI_WARPS = 8;
-constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum may run over 2^24 values: 0.1 s)
+constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum runs over up to run_of(type) values)
 // 256 columns of parts: four warps give up registers for the epilogue's eight.  What the block was launched with has to cover
 // both shares, or the increase would wait for ever; the host checks the kernel's count before it launches one.
 constexpr int SPLIT_REGISTERS = 168;
@@ -869,10 +870,11 @@ Cut cut(long long M, long long N, long long K, int segments, int nz, bool gated,
   const long long kblocks = (K + (type == VERACE_E4M3 ? 127 : 63)) / (type == VERACE_E4M3 ? 128 : 64);
   Cut best{256, 1};
   double least = 0;
+  const int runs = parts ? 1 : (int)((K * segments + run_of(type) - 1) / run_of(type));   // (64 values of parts are a sum of their own)
   for (int bn = 256; bn >= 128; bn /= 2) {
     const int tn = gated ? bn / 2 : bn;
     const long long tiles = (M + 255) / 256 * ((N + tn - 1) / tn) * nz;
-    for (int s = 1; s <= 16 && (s == 1 || (s * tiles <= 74 && kblocks >= 8 * s)); ++s) {
+    for (int s = runs; s == runs || (s <= 16 && s * tiles <= 74 && kblocks >= 8 * s); ++s) {
       const long long stages = (kblocks + s - 1) / s;
       if ((s - 1) * stages >= kblocks) continue;      // (a split would be empty)
       const double per = (double)stages * segments * (parts ? bn == 256 ? 3200 : 2900 : bn == 256 ? 512 : 400), epi = 40. * bn;

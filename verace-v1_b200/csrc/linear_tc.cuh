@@ -38,6 +38,22 @@ size_t split_bytes(long long M, long long N, long long K, int segments, int nz, 
 // Tokens up to which weights may be streamed past them (linear_few.cu).
 constexpr int FEW = 160;
 
+// Values of K that a sum of 16- or 8-bit operands may run over in the tensor core, which cuts every product to the last place
+// of the running sum (and two bits more) instead of rounding the sum.  Where all terms have one sign that takes 6.4e-9 of the
+// sum a term (fp16; bf16 5e-9 to 6.2e-9, e4m3 up to 1.2e-9; 2048 x 2048 outputs, K = 2^12 ... 2^18): 2.1e-4 of it at 2^15 and
+// 8e-4 at 2^17, less than half of fp16's and of bf16's half step.  Longer sums are split, and the splits' sums added with
+// rounding.  (8 bytes an output and split: 2 to 3 % of the product's time.)
+inline long long run_of(int type) { return type == VERACE_F16 ? 1 << 15 : 1 << 17; }
+
+// CTAs of a cluster that share K in linear_few.cu.
+inline int few_splits(long long N, long long K, int segments, int type) {
+  const int step = type == VERACE_E4M3 ? 128 : 64;
+  const long long tiles = (N + 127) / 128, steps = (K + step - 1) / step * segments;
+  int ck = 1;
+  while (ck < 8 && tiles * ck * 2 <= 148 && steps >= ck * 4) ck *= 2;
+  return ck;
+}
+
 int product_large(const Product& p, cudaStream_t st);   // linear_large.cu
 int product_few(const Product& p, cudaStream_t st);     // linear_few.cu: up to FEW rows of A
 int product_dot(const Product& p, cudaStream_t st);     // linear_dot.cu: a few rows of A, fp32 operands as they are
