@@ -122,3 +122,33 @@ def test_states_of_a_decode_step_count_their_versions():
         assert (h == 2).all()
     V.add_rmsnorm_fp8(h, h, torch.nn.RMSNorm(64, device="cuda", dtype=BF16).requires_grad_(False))
     assert (h == 4).all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("m", [20, 300])
+def test_relu_selects_its_gradient(dt, m):
+    """0 at a unit that is off, whatever the gradient is there; the gradient itself where the sum is NaN."""
+    g = gen(m)
+    x, w, u, d = randn(g, m, 64, dt=dt), randn(g, 96, 64, dt=dt), randn(g, 96, 64, dt=dt), randn(g, m, 96, dt=dt)
+    z = x.double() @ w.double().t()
+    sure = z.abs() > 0.01
+    d = torch.where(sure, d, torch.zeros_like(d))
+    off = (z < 0) & sure
+    clean = torch.autograd.grad(V.fused_linear(*(t := [x.clone().requires_grad_(), w.clone().requires_grad_()]), activation="relu"), t, d)
+    bad = d.clone()
+    bad[off & (torch.rand(m, 96, device="cuda", generator=g) < 0.2)] = float("inf")
+    bad[off & (torch.rand(m, 96, device="cuda", generator=g) < 0.2)] = float("nan")
+    got = torch.autograd.grad(V.fused_linear(*t, activation="relu"), t, bad)
+    assert all(torch.equal(a, b) for a, b in zip(got, clean)) and all(a.isfinite().all() for a in got)
+    # the gate's gradient likewise (the up projection's is d relu(g): NaN of an infinite d, as torch's product is)
+    t = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+    got, = torch.autograd.grad(V.gated_linear(t[0], t[1], u, activation="relu"), t[1], bad)
+    want, = torch.autograd.grad(V.gated_linear(t[0], t[1], u, activation="relu"), t[1], d)
+    assert torch.equal(got, want) and got.isfinite().all()
+    # a row of NaN sums: the weights as they are in x's gradient
+    x2 = x.clone()
+    x2[3, 5] = float("nan")
+    t = [x2.requires_grad_(), w]
+    got, = torch.autograd.grad(V.fused_linear(*t, activation="relu"), t[0], d)
+    plain, = torch.autograd.grad(V.fused_linear(*t), t[0], d)
+    assert torch.equal(got[3], plain[3]) and torch.equal(got[[i for i in range(m) if i != 3]], clean[0][[i for i in range(m) if i != 3]])

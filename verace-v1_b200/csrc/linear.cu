@@ -275,11 +275,7 @@ __global__ void __launch_bounds__(256) linear_slope(SlopeArgs a) {
         load8<float>(a.pre + r * a.n, c, a.n, a.vec, z);
         by_act(a.act, [&](auto k) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float y, dy;
-            act_slope_<decltype(k)::value, sizeof(O) == 2>(z[j], y, dy);
-            d[j] *= dy;
-          }
+          for (int j = 0; j < 8; ++j) d[j] = back_<decltype(k)::value, sizeof(O) == 2>(d[j], z[j]);
         });
       }
       if (a.out) store_operand<T>(static_cast<Part<T>*>(a.out) + r * a.ld + c, a.piece, d);

@@ -57,13 +57,10 @@ __device__ __forceinline__ float act_(float z) {
   if (ACT == VERACE_ACT_GELU_TANH) return 0.5f * z * (1.f + tanh_<FAST>(GT0 * fmaf(GT1 * z * z, z, z)));
   return z;
 }
-// act(z) and act'(z)
+// act(z) and act'(z), but for relu
 template <int ACT, bool FAST>
 __device__ __forceinline__ void act_slope_(float z, float& a, float& da) {
-  if (ACT == VERACE_ACT_RELU) {
-    a = z < 0.f ? 0.f : z;
-    da = z > 0.f ? 1.f : 0.f;
-  } else if (ACT == VERACE_ACT_SILU) {
+  if (ACT == VERACE_ACT_SILU) {
     const float p = sigmoid_<FAST>(z);
     a = z * p;
     da = p * (1.f + z * (1.f - p));
@@ -80,6 +77,15 @@ __device__ __forceinline__ void act_slope_(float z, float& a, float& da) {
     da = 1.f;
   }
 }
+// the gradient of z from d, the gradient of act(z).  (relu selects, as torch does: 0 where z <= 0, even of an infinite d,
+// and d where z is NaN)
+template <int ACT, bool FAST>
+__device__ __forceinline__ float back_(float d, float z) {
+  if (ACT == VERACE_ACT_RELU) return z <= 0.f ? 0.f : d;
+  float a, da;
+  act_slope_<ACT, FAST>(z, a, da);
+  return d * da;
+}
 // act(g) up(u)
 template <int ACT, bool FAST>
 __device__ __forceinline__ float gate_(float g, float u, float b1, float b2, float r1, float r2) {
@@ -94,6 +100,9 @@ __device__ __forceinline__ void gate_slope_(float d, float g, float u, float b1,
     const float tg = tanh_<FAST>(g * r1), tu = tanh_<FAST>(u * r2), p = sigmoid_<FAST>(g);
     dg = d * (b2 * tu) * ((1.f - tg * tg) * p + b1 * tg * p * (1.f - p));
     du = d * (b1 * tg * p) * (1.f - tu * tu);
+  } else if (ACT == VERACE_ACT_RELU) {
+    dg = back_<ACT, FAST>(d * u, g);
+    du = d * act_<ACT, FAST>(g);
   } else {
     float a, da;
     act_slope_<ACT, FAST>(g, a, da);
