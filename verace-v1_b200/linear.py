@@ -30,6 +30,7 @@ _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _GATES = {"situ": 5, "silu": 2, "gelu": 3, "gelu_tanh": 4, "relu": 1}
 FP8 = torch.float8_e4m3fn
 _CODE = {**_DTYPE, FP8: E4M3}
+_MOST = 1 << 24      # rows and columns of any operand (the C entry points', whose widths are 32-bit)
 _ALIGN = {torch.float32: 1, torch.bfloat16: 8, torch.float16: 8, FP8: 16}   # values in 16 bytes (fp32 rows: any)
 
 
@@ -71,6 +72,8 @@ def _checked(who, x, weight, scales, want, activation, allowed, out_dtype, defau
     assert len(shape) >= 1, "x must have at least one dimension"
     assert weight.dtype is dt and shape[-1] == k and weight.device == x.device, \
         f"{who}: the weights must be [n, {shape[-1]}] in x's dtype, on its device"
+    if n > _MOST or k > _MOST:
+        raise ValueError(f"{who}: weights of {n} x {k} (at most {_MOST} rows and columns)")
     if dt is FP8:
         if scales != want:
             raise ValueError(f"{who}: float8_e4m3fn operands need their scales, one for x and one for each weight")
@@ -363,6 +366,8 @@ def _to_fp8(who, h, y, sum_out, norm, return_norm):
     if code is None:
         raise ValueError(f"{who}: {dt} inputs (expected fp32, bf16 or fp16)")
     assert len(shape) >= 1 and shape[-1] > 0, f"{who}: rows of at least one value"
+    if shape[-1] > _MOST:
+        raise ValueError(f"{who}: rows of {shape[-1]} columns (at most 32768)")
     if h.requires_grad:
         _require_no_grad(h, who)
     dev, cols = h.device, shape[-1]
