@@ -152,3 +152,35 @@ def test_relu_selects_its_gradient(dt, m):
     got, = torch.autograd.grad(V.fused_linear(*t, activation="relu"), t[0], d)
     plain, = torch.autograd.grad(V.fused_linear(*t), t[0], d)
     assert torch.equal(got[3], plain[3]) and torch.equal(got[[i for i in range(m) if i != 3]], clean[0][[i for i in range(m) if i != 3]])
+
+
+def test_derivatives_that_nobody_would_get_are_refused():
+    """Scales that require a gradient, and forward-mode tangents of any operand."""
+    import torch.autograd.forward_ad as ad
+    g = gen(6)
+    x, w, b, r = randn(g, 5, 64, dt=BF16), randn(g, 32, 64, dt=BF16), randn(g, 32, dt=BF16), randn(g, 5, 32, dt=BF16)
+    (q, s), (wq, ws) = V.quantize_fp8(x), V.quantize_fp8(w)
+    for i in range(2):
+        sc = [s.clone(), ws.clone()]
+        sc[i].requires_grad_()
+        with pytest.raises(RuntimeError, match="no_grad"):
+            V.fused_linear(q, wq, x_scale=sc[0], w_scale=sc[1])
+        with torch.no_grad():
+            V.fused_linear(q, wq, x_scale=sc[0], w_scale=sc[1])
+    for i in range(3):
+        sc = [s.clone(), ws.clone(), ws.clone()]
+        sc[i].requires_grad_()
+        with pytest.raises(RuntimeError, match="no_grad"):
+            V.gated_linear(q, wq, wq, x_scale=sc[0], gate_scale=sc[1], up_scale=sc[2])
+    norm = torch.nn.RMSNorm(64, device="cuda", dtype=BF16).requires_grad_(False)
+    with ad.dual_level():
+        def dual(t):
+            return ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: V.fused_linear(dual(x), w), lambda: V.fused_linear(x, dual(w)), lambda: V.fused_linear(x, w, dual(b)),
+                     lambda: V.fused_linear(x, w, residual=dual(r)), lambda: V.gated_linear(dual(x), w, w),
+                     lambda: V.gated_linear(x, w, dual(w)), lambda: V.quantize_fp8(dual(x)), lambda: V.rmsnorm_fp8(dual(x), norm),
+                     lambda: V.fused_linear(q, wq, x_scale=dual(s), w_scale=ws),
+                     lambda: V.add_rmsnorm_fp8(x.clone(), dual(x), norm)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        V.fused_linear(x, w)            # (no operand with a tangent)

@@ -19,6 +19,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._launch import current, raw_stream, wrote
@@ -98,6 +99,13 @@ def _workspace_bytes(query: str, m: int, n: int, k: int, code: int) -> int:
 
 def _workspace(nbytes: int, device):
     return torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _no_tangents(who, *tensors):
+    """Refuses dual numbers, whose tangents a kernel would drop (called inside of a dual level alone)."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{who} has no forward-mode derivative")
 
 
 _NOTHING = contextlib.nullcontext()
@@ -224,6 +232,10 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         assert residual.shape == lead + (n,) and residual.dtype is odt and residual.device == dev, \
             f"residual must be {tuple(lead) + (n,)} in {odt}, on x's device"
         grad = grad or residual.requires_grad and torch.is_grad_enabled()
+    if forward_ad._current_level >= 0:
+        _no_tangents("fused_linear", x, weight, bias, residual, x_scale, w_scale)
+    if eight and (x_scale.requires_grad or w_scale.requires_grad):
+        grad = torch.is_grad_enabled()
     if grad:
         if eight:
             raise RuntimeError("fused_linear runs 8-bit operands for inference (no autograd path): "
@@ -342,7 +354,10 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     flat = len(lead) == 1
     m = lead[0] if flat else math.prod(lead)
     eight = x.dtype is FP8
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+    if forward_ad._current_level >= 0:
+        _no_tangents("gated_linear", x, w_gate, w_up, x_scale, gate_scale, up_scale)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or eight and (x_scale.requires_grad or gate_scale.requires_grad or up_scale.requires_grad)):
         if eight:
             raise RuntimeError("gated_linear runs 8-bit operands for inference (no autograd path): "
                                "call it under torch.no_grad()")
@@ -370,6 +385,8 @@ def _to_fp8(who, h, y, sum_out, norm, return_norm):
         raise ValueError(f"{who}: rows of {shape[-1]} columns (at most 32768)")
     if h.requires_grad:
         _require_no_grad(h, who)
+    if forward_ad._current_level >= 0:
+        _no_tangents(who, h, y, None if norm is None else norm.weight)
     dev, cols = h.device, shape[-1]
     w, eps = (None, 0.0) if norm is None else _norm_args(norm, h)
     q = torch.empty_like(h, dtype=FP8)
