@@ -271,3 +271,26 @@ def test_long_gradients_of_one_sign(dt):
     dx, = torch.autograd.grad(V.fused_linear(x, w), x, d)
     want = product_in_64(d, w.t())
     assert bool(((dx.to(F64) - want).abs() <= (lost + half) * want).all()), off(dx, want)
+
+
+# ---------------------------------------------------------------------------- scales whose product leaves fp32's range
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 64), (3, 4096, 64), (40, 4096, 2000), (40, 4096, 20000), (300, 4096, 200), (300, 9008, 70)])
+@pytest.mark.parametrize("rows,cols", [(1e-25, 1e-20), (1e-20, 1e-25), (1e30, 1e20), (1e20, 1e30), (1e-30, 1e30), (1e30, 1e-30),
+                                       (2.0 ** -109, 1e4)])
+def test_scales_far_from_1(m, k, n, rows, cols):
+    """Sums of up to 8e8, and of 0 in every other row: the result is fp32's where it has one, to the sum's and two
+    multiplications' rounding."""
+    g = gen(m + n)
+    x, w = (torch.randint(1, 9, s, device="cuda", generator=g).float() * 56 for s in ((m, k), (n, k)))
+    x[1::2] = 0
+    x, w = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+    sx, sw = torch.full((m,), rows, device="cuda"), torch.full((n,), cols, device="cuda")
+    want = dequantised(x, sx) @ dequantised(w, sw).t()
+    y = V.fused_linear(x, w, x_scale=sx, w_scale=sw, out_dtype=F32)
+    one = torch.ones_like(sw) / sx[0]
+    h = V.gated_linear(x, w, w, activation="relu", x_scale=sx, gate_scale=sw, up_scale=one, out_dtype=F32)
+    sums = x.to(F64) @ w.to(F64).t()
+    for got, exact in ((y, want), (h, want * sums)):
+        over = exact > MOST
+        assert bool((got[over] == math.inf).all()) and bool((got[~over].to(F64) - exact[~over]).abs().le(
+            4e-6 * exact[~over].abs() + 2.0 ** -126).all())

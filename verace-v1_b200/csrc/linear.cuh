@@ -136,6 +136,13 @@ __device__ __forceinline__ void activate(const E& e, float (&v)[U], const float 
   });
 }
 
+// a sum of 8-bit products times the scales of its row and column, the smaller one first: then nothing on the way leaves
+// fp32's range that the result does not (their product may: 1e20 by 1e20 times a sum of 0, 1e-25 by 1e-20 times one of 1e9)
+__device__ __forceinline__ float scaled_by(float v, float row, float col) {
+  const bool first = fabsf(row) < fabsf(col);
+  return v * (first ? row : col) * (first ? col : row);
+}
+
 // ------------------------------------------------------------------ values by a runtime type
 __device__ __forceinline__ float load_as(const void* p, long long i, int type) {
   if (type == VERACE_F32) return static_cast<const float*>(p)[i];

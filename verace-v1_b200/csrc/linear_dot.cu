@@ -73,8 +73,8 @@ template <bool GATED>
 __device__ __forceinline__ void finish(const Epilogue& e, long long m, long long n, float g, float u) {
   if (e.col_scale) {
     const float rs = e.row_scale[m];
-    g *= rs * e.col_scale[n];
-    if (GATED) u *= rs * e.up_scale[n];
+    g = scaled_by(g, rs, e.col_scale[n]);
+    if (GATED) u = scaled_by(u, rs, e.up_scale[n]);
   }
   if (!GATED && e.bias) g += load_as(e.bias, n, e.bias_type);
   if (e.pre) {

@@ -233,11 +233,11 @@ __global__ void __launch_bounds__(NT, 2) few_product(const __grid_constant__ Map
         for (int j = 0; j < 16; ++j) {
           const float rs = e.row_scale && t + j < tokens ? row_scale[t + j] : 1.f;
           g[j] = __uint_as_float(r[j]);
-          if (e.col_scale) g[j] *= rs * cs;
+          if (e.col_scale) g[j] = scaled_by(g[j], rs, cs);
           if (!GATED && e.bias) g[j] += ca;
           if (GATED) {
             u[j] = __uint_as_float(s[j]);
-            if (e.col_scale) u[j] *= rs * ca;
+            if (e.col_scale) u[j] = scaled_by(u[j], rs, ca);
           }
         }
         if (e.pre) {

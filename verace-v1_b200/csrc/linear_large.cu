@@ -318,7 +318,7 @@ __device__ __forceinline__ void scaled(const Epilogue& e, const uint32_t (&r)[U]
     float s[U];
     column_values(col_scale, VERACE_F32, n0, N, s);
 #pragma unroll
-    for (int j = 0; j < U; ++j) v[j] *= rs * s[j];
+    for (int j = 0; j < U; ++j) v[j] = scaled_by(v[j], rs, s[j]);
   }
   if (bias) {
     float s[U];

@@ -200,8 +200,8 @@ __device__ __forceinline__ void finish4(const Epilogue& e, long long m, long lon
   if (e.col_scale) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      g[j] *= row_scale * col_scale[j];
-      if (GATED) u[j] *= row_scale * col_add[j];
+      g[j] = scaled_by(g[j], row_scale, col_scale[j]);
+      if (GATED) u[j] = scaled_by(u[j], row_scale, col_add[j]);
     }
   }
   if (!GATED && e.bias) {
