@@ -184,3 +184,26 @@ def test_derivatives_that_nobody_would_get_are_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
         V.fused_linear(x, w)            # (no operand with a tangent)
+
+
+def test_a_quantised_model_in_another_type():
+    """model.half() behind quantize_model_fp8: the same 8-bit weights, fp16 in and out."""
+    from test_fp8_model_gpu import make_model
+    model = V.quantize_model_fp8(make_model(BF16))
+    moe = model.layers[0].mcmoe
+    up, down = moe.base_situ_glu.fp8_in.w_up.clone().view(torch.uint8), moe.base_w_down.scales.clone()
+    model.half()
+    assert torch.equal(moe.base_situ_glu.fp8_in.w_up.view(torch.uint8), up) and torch.equal(moe.base_w_down.scales, down)
+    ids = torch.randint(0, 101, (2, 5), generator=torch.Generator().manual_seed(1)).cuda()
+    tokens, lp = V.generate(model, ids, 3)
+    assert tokens.shape == (2, 8) and lp.isfinite().all()
+    with torch.no_grad():
+        logits, _, _ = model(ids, return_layer_states=True)
+        x = randn(gen(8), 1, 4, 128, dt=F16)
+        q, s = V.quantize_fp8(x)
+        f = moe.base_situ_glu.fp8_in
+        assert torch.equal(f(x), V.gated_linear(q, f.w_gate, f.w_up, x_scale=s, gate_scale=f.gate_scales, up_scale=f.up_scales,
+                                                out_dtype=F16))
+    assert logits.dtype is F16 and logits.isfinite().all()
+    model.float()
+    assert V.generate(model, ids, 2)[1].isfinite().all() and model.lm_head.dtype is F32

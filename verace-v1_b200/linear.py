@@ -458,10 +458,32 @@ def _rows8(x) -> Rows8:
     return x if isinstance(x, tuple) else quantize_fp8(x)
 
 
-class Fp8Linear(nn.Module):
+class _Fp8Module(nn.Module):
+    """A module with e4m3 weights.  ``to``, ``half`` and the like change the type of its outputs (``dtype``) and bias; the
+    8-bit values and their fp32 scales keep theirs and move between devices with it (torch counts 8-bit values as
+    floating point and would cast them)."""
+    _packed: Tuple[str, ...] = ()
+
+    def _apply(self, fn, recurse: bool = True):
+        held = {name: self._buffers[name] for name in self._packed}
+        device = held[self._packed[0]].device
+        self._buffers.update(dict.fromkeys(held))
+        try:
+            super()._apply(fn, recurse)
+            for name, t in held.items():
+                bits = fn(t.view(torch.uint8 if t.dtype is FP8 else torch.int32))
+                held[name] = bits.view(t.dtype) if not bits.is_floating_point() else t.to(bits.device)
+            self.dtype = fn(torch.empty(0, dtype=self.dtype, device=device)).dtype
+        finally:
+            self._buffers.update(held)
+        return self
+
+
+class Fp8Linear(_Fp8Module):
     """A linear layer with e4m3 weights (buffers ``weight``, ``scales``, ``bias``) in place of a
     ``torch.nn.Linear``.  Its input is a tensor, whose rows it quantises, or rows in 8 bits as
     ``rmsnorm_fp8`` gives them: (values, scales).  The output has ``dtype``."""
+    _packed = ("weight", "scales")
 
     def __init__(self, in_features: int, out_features: int, bias: bool = False, dtype: torch.dtype = torch.bfloat16,
                  device=None):
@@ -487,9 +509,10 @@ class Fp8Linear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
-class Fp8GatedLinear(nn.Module):
+class Fp8GatedLinear(_Fp8Module):
     """The gate and up projections of a gated block with e4m3 weights and the gate in their product's epilogue
     (buffers ``w_gate``, ``w_up``, ``gate_scales``, ``up_scales``); its input is as ``Fp8Linear``'s."""
+    _packed = ("w_gate", "w_up", "gate_scales", "up_scales")
 
     def __init__(self, in_features: int, hidden_features: int, activation: str = "situ", beta1: float = 4.0,
                  beta2: float = 25.0, dtype: torch.dtype = torch.bfloat16, device=None):
