@@ -207,3 +207,21 @@ def test_a_quantised_model_in_another_type():
     assert logits.dtype is F16 and logits.isfinite().all()
     model.float()
     assert V.generate(model, ids, 2)[1].isfinite().all() and model.lm_head.dtype is F32
+
+
+@pytest.mark.parametrize("handed_on", [False, True])
+def test_hooks_of_the_base_block_see_its_8_bit_calls(handed_on):
+    from test_fp8_model_gpu import make_model
+    moe = V.quantize_model_fp8(make_model(BF16)).layers[1].mcmoe
+    x = randn(gen(9), 2, 3, 128, dt=BF16)
+    x8 = V.quantize_fp8(x) if handed_on else None
+    with torch.no_grad():
+        want = moe(x, x8)
+        seen = []
+        handles = [moe.base_situ_glu.register_forward_pre_hook(lambda m, a: seen.append(len(a))),
+                   moe.base_situ_glu.register_forward_hook(lambda m, a, out: out * 0)]
+        without = moe(x, x8)
+        assert seen == [2 if handed_on else 1] and not torch.equal(without, want)
+        for h in handles:
+            h.remove()
+        assert torch.equal(moe(x, x8), want)

@@ -128,11 +128,12 @@ class SiTUGLU(nn.Module):
             self._stacked_key = key
         return self._stacked
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, x8: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+        """``x8``: x's rows in 8 bits with their scales, for a block in 8 bits (which quantises x without them)."""
         if not x.is_cuda or torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("SiTUGLU runs on CUDA inputs for inference (no autograd path)")
         if self.fp8_in is not None:
-            return self.fp8_in(x)
+            return self.fp8_in(x if x8 is None else x8)
         gu = self.int4_in(x) if self.int4_in is not None else torch.nn.functional.linear(x, self._gate_up_weight())
         hf = self.hidden_features
         return situ_glu(gu[..., :hf], gu[..., hf:], self.beta1, self.beta2)
@@ -163,11 +164,10 @@ class ManifoldContinuousMoE(nn.Module):
             raise RuntimeError("ManifoldContinuousMoE runs on CUDA inputs for inference (no autograd path)")
         b, s, d = x.shape
         x_flat = x.reshape(b * s, d).contiguous()
-        fp8 = self.base_situ_glu.fp8_in
-        if fp8 is not None:
-            base_in = fp8(x_flat if x8 is None else (x8[0].view(b * s, d), x8[1].reshape(b * s)))
-        else:
+        if x8 is None:
             base_in = self.base_situ_glu(x_flat)
+        else:
+            base_in = self.base_situ_glu(x_flat, (x8[0].view(b * s, d), x8[1].reshape(b * s)))
         down8 = isinstance(self.base_w_down, Fp8Linear)
         base_out = None if down8 else self.base_w_down(base_in).contiguous()
         k_val = min(self.top_k_components, self.num_components)
