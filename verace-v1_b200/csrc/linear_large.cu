@@ -45,7 +45,7 @@ using namespace lin;
 constexpr int NT = 384, EPI_WARPS = 8;
 constexpr uint32_t POLLS = 1u << 22, SUM_POLLS = 1u << 26;   // (a sum runs over up to run_of(type) values)
 // 256 columns of parts: four warps give up registers for the epilogue's eight.  What the block was launched with has to cover
-// both shares, or the increase would wait for ever; the host checks the kernel's count before it launches one.
+// both shares, or the increase would wait for ever; the host checks the kernels' count before it chooses them (wide_parts).
 constexpr int SPLIT_REGISTERS = 168;
 static_assert(128 * 72 + 256 * 216 <= NT * SPLIT_REGISTERS, "the shares' sum");
 constexpr int TURN = 4096;             // a warp's block of the output: 32 rows of 128 bytes
@@ -799,7 +799,7 @@ int launch(const Product& p, int splits, cudaStream_t st) {
   VERACE_CUDA(cudaGetDevice(&dev));
   static std::atomic<uint64_t> ready{0};      // devices whose limit is raised
   if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (PARTS && BN == 256) {
+    if (PARTS && BN == 256) {     // (where wide_parts could not ask)
       cudaFuncAttributes fa;
       VERACE_CUDA(cudaFuncGetAttributes(&fa, kern));
       VERACE_REQUIRE(fa.numRegs == SPLIT_REGISTERS, VERACE_ERR_UNSUPPORTED, "linear: %d registers where %d are shared out",
@@ -859,6 +859,30 @@ __global__ void __launch_bounds__(256) join_splits(const float* part, int splits
   finish4<GATED>(e, m, c, n, scale, add, row_scale, res, g, u);
 }
 
+// Whether the compiler gave the kernels of 256 columns of parts the registers that their warps share out among them; where
+// it did not, products of parts run in tiles of 128 columns, which share none out.  (On a machine without a device, where
+// nothing is launched, they are taken to be right.)
+bool wide_parts() {
+  static std::atomic<int> known{0};     // 0: not yet, 1: yes, 2: no
+  int k = known.load(std::memory_order_relaxed);
+  if (k == 0) {
+    const void* kernels[] = {
+        (const void*)large_product<false, false, false, true, 256, true>, (const void*)large_product<false, true, true, false, 256, true>,
+        (const void*)large_product<false, false, true, false, 256, true>, (const void*)large_product<false, false, false, false, 256, true>};
+    k = 1;
+    for (const void* f : kernels) {
+      cudaFuncAttributes a;
+      if (cudaFuncGetAttributes(&a, f) != cudaSuccess) {
+        cudaGetLastError();
+        return true;
+      }
+      if (a.numRegs != SPLIT_REGISTERS) k = 2;
+    }
+    known.store(k, std::memory_order_relaxed);
+  }
+  return k == 1;
+}
+
 // How a product is cut: columns of a tile, and splits of K.  A pair's time in clocks: a step of four MMAs takes 512
 // (BN 256) or 400 (BN 128, bound by shared memory: 8 KB for 64 clocks of an MMA), 64 values of parts 3200 or
 // 2900, an epilogue about 40 a column (under the next tile's products but for the last), the first operands
@@ -871,7 +895,7 @@ Cut cut(long long M, long long N, long long K, int segments, int nz, bool gated,
   Cut best{256, 1};
   double least = 0;
   const int runs = parts ? 1 : (int)((K * segments + run_of(type) - 1) / run_of(type));   // (64 values of parts are a sum of their own)
-  for (int bn = 256; bn >= 128; bn /= 2) {
+  for (int bn = parts && !wide_parts() ? 128 : 256; bn >= 128; bn /= 2) {
     const int tn = gated ? bn / 2 : bn;
     const long long tiles = (M + 255) / 256 * ((N + tn - 1) / tn) * nz;
     for (int s = runs; s == runs || (s <= 16 && s * tiles <= 74 && kblocks >= 8 * s); ++s) {
