@@ -12,9 +12,10 @@ namespace verace {
 namespace lin {
 
 // ------------------------------------------------------------------ activations
-// FAST serves outputs of 16 bits: exponentials and reciprocals by the approximate instructions, a
-// few units of 2^-23 off, against the output's half step of 2^-9 or 2^-12.  fp32 outputs take
-// the CUDA functions.
+// FAST serves outputs of 16 bits: exponentials and reciprocals by the approximate instructions, against the output's half
+// step of 2^-9 or 2^-12.  exp(x) is about (2 + |x|) 2^-23 off (x log2 e is rounded before the instruction takes it: 2^-17 at
+// 80), tanh a few 2^-22; what would be below 2^-126 on the way is 0 (sigmoid below -87.3, and with it SiLU, which is less
+// than 1.2e-36 there).  fp32 outputs take the CUDA functions.
 __device__ __forceinline__ float ex2_(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
