@@ -225,3 +225,17 @@ def test_hooks_of_the_base_block_see_its_8_bit_calls(handed_on):
         for h in handles:
             h.remove()
         assert torch.equal(moe(x, x8), want)
+
+
+def test_a_model_that_cannot_go_into_8_bits_stays_as_it_is():
+    from test_fp8_model_gpu import make_model
+    for spoil in (lambda m: setattr(m.layers[2].mcmoe, "base_w_down", torch.nn.Linear(40000, 128, bias=False, device="cuda")),
+                  lambda m: m.layers[1].mcmoe.base_w_down.cpu(), lambda m: m.lm_head.double()):
+        model = make_model(BF16)
+        spoil(model)
+        with pytest.raises((ValueError, AssertionError)):
+            V.quantize_model_fp8(model)
+        for layer in model.layers:
+            assert layer.mcmoe.base_situ_glu.w_gate is not None and layer.mcmoe.base_situ_glu.fp8_in is None
+            assert isinstance(layer.mcmoe.base_w_down, torch.nn.Linear)
+        assert isinstance(model.lm_head, torch.nn.Linear)

@@ -541,6 +541,16 @@ class Fp8GatedLinear(_Fp8Module):
         return f"in_features={self.in_features}, hidden_features={self.hidden_features}, activation={self.activation}"
 
 
+def _check_weights(*weights: torch.Tensor):
+    """Refuses weights that ``quantize_fp8`` does not take."""
+    for w in weights:
+        assert w.is_cuda, "This kernel requires CUDA tensors"
+        if w.dtype not in _DTYPE:
+            raise ValueError(f"quantize_model_fp8: {w.dtype} weights (expected fp32, bf16 or fp16)")
+        if w.shape[1] > 32761 and w.shape[1] != 32768:
+            raise ValueError(f"quantize_model_fp8: weights of {w.shape[1]} inputs (at most 32761, or 32768)")
+
+
 def quantize_model_fp8(model: nn.Module, lm_head: bool = True) -> nn.Module:
     """Puts the feed-forward sub-layers of a model (a ``VeraceV1Model``, ``VeraceV1Layer`` or any module that
     holds the framework's M-CMoE) into 8 bits, in place, and with ``lm_head`` the LM head (the token embedding
@@ -548,16 +558,25 @@ def quantize_model_fp8(model: nn.Module, lm_head: bool = True) -> nn.Module:
     manifold's part in its epilogue; inside a layer the norm before the sub-layer writes the rows in 8 bits along
     with the residual's addition.  The model must be on a CUDA device; the dense weights are dropped.  Routers, the
     sigma projection, norms, bases and the mixers stay as they are, and so does what ``quantize_model_int4`` has
-    put into 4 bits."""
+    put into 4 bits.  A model that cannot go into 8 bits as a whole is refused as it is."""
     from .mcmoe import ManifoldContinuousMoE, SiTUGLU
 
-    for m in list(model.modules()):
+    modules = list(model.modules())
+    lm_head = lm_head and isinstance(getattr(model, "lm_head", None), nn.Linear)
+    for m in modules:
+        if isinstance(m, SiTUGLU) and m.fp8_in is None and m.int4_in is None:
+            _check_weights(m.w_gate.weight, m.w_up.weight)
+        elif isinstance(m, ManifoldContinuousMoE) and isinstance(m.base_w_down, nn.Linear):
+            _check_weights(m.base_w_down.weight)
+    if lm_head:
+        _check_weights(model.lm_head.weight)
+    for m in modules:
         if isinstance(m, SiTUGLU) and m.fp8_in is None and m.int4_in is None:
             m.fp8_in = Fp8GatedLinear.from_weights(m.w_gate.weight, m.w_up.weight, "situ", m.beta1, m.beta2)
             m.w_gate = m.w_up = None
             m._stacked = m._stacked_key = None
         elif isinstance(m, ManifoldContinuousMoE) and isinstance(m.base_w_down, nn.Linear):
             m.base_w_down = Fp8Linear.from_linear(m.base_w_down)
-    if lm_head and isinstance(getattr(model, "lm_head", None), nn.Linear):
+    if lm_head:
         model.lm_head = Fp8Linear.from_linear(model.lm_head)
     return model
