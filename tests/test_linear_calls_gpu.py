@@ -239,3 +239,15 @@ def test_a_model_that_cannot_go_into_8_bits_stays_as_it_is():
             assert layer.mcmoe.base_situ_glu.w_gate is not None and layer.mcmoe.base_situ_glu.fp8_in is None
             assert isinstance(layer.mcmoe.base_w_down, torch.nn.Linear)
         assert isinstance(model.lm_head, torch.nn.Linear)
+
+
+def test_a_sum_is_not_written_over_a_leaf():
+    norm = torch.nn.RMSNorm(64, device="cuda", dtype=BF16).requires_grad_(False)
+    h, y = torch.ones(3, 64, device="cuda", dtype=BF16), torch.ones(3, 64, device="cuda", dtype=BF16)
+    out = torch.zeros(3, 64, device="cuda", dtype=BF16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        V.add_rmsnorm_fp8(h, y, norm, out=out)
+    assert not out.any()
+    with torch.no_grad():
+        V.add_rmsnorm_fp8(h, y, norm, out=out)
+    assert (out == 2).all()

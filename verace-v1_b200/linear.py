@@ -444,6 +444,8 @@ def add_rmsnorm_fp8(h: torch.Tensor, y: torch.Tensor, norm: nn.RMSNorm, *, out: 
     elif out is not h:
         assert out.shape == h.shape and out.dtype is h.dtype and out.device == dev, \
             "the sum goes to a tensor of h's shape, dtype and device"
+        if out.requires_grad:
+            _require_no_grad(out, "add_rmsnorm_fp8")
     assert out.is_contiguous(), "the sum goes to a contiguous tensor"
     made = _to_fp8("add_rmsnorm_fp8", h.contiguous(), y.contiguous(), out, norm, return_norm)
     wrote(out)
