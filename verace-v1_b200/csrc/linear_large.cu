@@ -27,9 +27,10 @@
 // TMA stores them; rows that are not 16-byte aligned are stored word by word, the warp along a row.  Residuals come
 // into the block that way too, fetched while the products run.
 //
-// Measured on the device: gated 8192 x 4096 x 2 x 8192 bf16 690 us (1.59 PFLOP/s, the tensor pipe 96 % active; a second of
-// such calls runs into the power limit, 800 us), 8192 x 8192 x 4096 e4m3 188 us (2.9 PFLOP/s; bound by what the CTAs load,
-// 32 KB each for 256 clocks of MMAs), 8192 x 1024 x 4096 bf16 48 us (1.42), 4096^3 fp32 607 us (226 TFLOP/s).
+// Measured on the device: gated 8192 x 4096 x 2 x 8192 bf16 690 to 708 us (1.55 to 1.59 PFLOP/s, the tensor pipe 96 % active;
+// a second of such calls runs into the power limit, 805 to 821 us), 8192 x 8192 x 4096 e4m3 188 to 194 us (2.8 to 2.9 PFLOP/s;
+// bound by what the CTAs load, 32 KB each for 256 clocks of MMAs; in long runs 230), 8192 x 1024 x 4096 bf16 48 us (1.42),
+// 4096^3 fp32 603 us (228 TFLOP/s).
 #include "linear_tc.cuh"
 
 #include <atomic>
