@@ -919,7 +919,8 @@ lazy_cham_kernel(LazyArgs A, const __grid_constant__ CUtensorMap tm_r, const __g
     if (tid == 0) atomicOr(&g_decode_status, 2u);   // (reported as a pass that did not run)
     return;
   }
-  // The hologram stages depend on no earlier kernel of this step: they are requested
+  // The hologram stages depend on no earlier kernel of this step, and what wrote them before
+  // it was complete when lazy_pre_kernel let this kernel in: they are requested
   // before griddepcontrol.wait, which (this kernel being launched as a programmatic
   // dependent of lazy_pre_kernel) returns once lazy_pre_kernel and, through it, the
   // projection epilogue are complete and their writes visible.
