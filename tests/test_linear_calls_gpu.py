@@ -251,3 +251,35 @@ def test_a_sum_is_not_written_over_a_leaf():
     with torch.no_grad():
         V.add_rmsnorm_fp8(h, y, norm, out=out)
     assert (out == 2).all()
+
+
+def back_and_forth(t):
+    """A saved tensor, as a hook may keep it: another tensor of the same values, dense."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def columns_first(t):
+    """Dense along the other dimension."""
+    return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("m", [4, 130, 300])
+@pytest.mark.parametrize("hooks", [(back_and_forth, back_and_forth), (columns_first, lambda t: t), "cpu"])
+def test_what_was_saved_comes_back_in_another_layout(dt, m, hooks):
+    """Operands inside of wider tensors, whose saved rows come back dense, or transposed, behind hooks."""
+    g = gen(m)
+    wide, ww, d = randn(g, m, 200, dt=dt), randn(g, 96, 300, dt=dt), randn(g, m, 96, dt=dt)
+
+    def grads():
+        x, w, u = (t.detach().requires_grad_() for t in (wide[:, 8:136], ww[:, 16:144], ww[:, 160:288]))
+        y, h = V.fused_linear(x, w, activation="silu"), V.gated_linear(x, w, u)
+        return torch.autograd.grad(y, (x, w), d) + torch.autograd.grad(h, (x, w, u), d)
+    want = grads()
+    if hooks == "cpu":
+        with torch.autograd.graph.save_on_cpu():
+            got = grads()
+    else:
+        with torch.autograd.graph.saved_tensors_hooks(*hooks):
+            got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

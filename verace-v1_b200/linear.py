@@ -138,10 +138,14 @@ def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, w
 
 def _fused_linear_backward(ctx, d):
     x2, w2, pre = ctx.saved_tensors
-    shape, m, n, k, ldx, ldw, act, out_dtype = ctx.sizes
+    shape, m, n, k, act, out_dtype = ctx.sizes
     want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
     dx = dw = db = None
     if want_x or want_w or want_b:
+        # (what was saved may come back in another layout: hooks move it to the host and back, for one)
+        (x2, ldx), (w2, ldw) = _rows(x2, m, k), _rows(w2, n, k)
+        if pre is not None:
+            pre = pre.contiguous()
         dev, dt = x2.device, x2.dtype
         if want_x:
             dx = torch.empty_strided((m, k), (k, 1), dtype=dt, device=dev)
@@ -177,7 +181,7 @@ class _FusedLinear(torch.autograd.Function):
         y, pre = _linear(x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
         ctx.save_for_backward(x2, w2, pre)
         shape = x.shape
-        ctx.sizes = (shape, m, n, k, ldx, ldw, act, out_dtype)
+        ctx.sizes = (shape, m, n, k, act, out_dtype)
         return y if len(shape) == 2 else y.view(shape[:-1] + (n,))
 
     @staticmethod
@@ -285,8 +289,10 @@ def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, wa
 
 def _gated_linear_backward(ctx, d):
     x2, g2, u2, gate, up = ctx.saved_tensors
-    shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype = ctx.sizes
+    shape, m, f, k, act, b1, b2, out_dtype = ctx.sizes
     want_x, want_g, want_u = ctx.needs_input_grad[:3]
+    (x2, ldx), (g2, u2, ldw) = _rows(x2, m, k), _gate_rows(g2, u2, f, k)     # (as in _fused_linear_backward)
+    gate, up = gate.contiguous(), up.contiguous()
     dev, dt = x2.device, x2.dtype
     dx = torch.empty_strided((m, k), (k, 1), dtype=dt, device=dev) if want_x else None
     dg = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_g else None
@@ -318,7 +324,7 @@ class _GatedLinear(torch.autograd.Function):
         h, gate, up = _gated(x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
         ctx.save_for_backward(x2, g2, u2, gate, up)
         shape = x.shape
-        ctx.sizes = (shape, m, f, k, ldx, ldw, act, b1, b2, out_dtype)
+        ctx.sizes = (shape, m, f, k, act, b1, b2, out_dtype)
         return h if len(shape) == 2 else h.view(shape[:-1] + (f,))
 
     @staticmethod
