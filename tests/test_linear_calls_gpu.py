@@ -283,3 +283,20 @@ def test_what_was_saved_comes_back_in_another_layout(dt, m, hooks):
         with torch.autograd.graph.saved_tensors_hooks(*hooks):
             got = grads()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("shape", [(64,), (6, 64), (2, 3, 64), (2, 1, 3, 64), (0, 3, 64)])
+def test_outputs_may_be_changed_in_place(shape):
+    """As torch.nn.functional.linear's may, in any number of dimensions."""
+    g = gen(11)
+    x, w, r = randn(g, *shape), randn(g, 96, 64), randn(g, *shape[:-1], 96)
+    for call in (lambda a, b: V.fused_linear(a, b), lambda a, b: V.gated_linear(a, b, w)):
+        got = [t.clone().requires_grad_() for t in (x, w)]
+        want = [t.clone().requires_grad_() for t in (x, w)]
+        y = call(*got)
+        assert y.shape == shape[:-1] + (96,)
+        y.mul_(r)
+        y += 1
+        y.sum().backward()
+        (call(*want) * r + 1).sum().backward()
+        assert all(torch.equal(a.grad, b.grad) and a.grad.shape == b.shape for a, b in zip(got, want))

@@ -108,6 +108,14 @@ def _no_tangents(who, *tensors):
             raise RuntimeError(f"{who} has no forward-mode derivative")
 
 
+def _output(lead, m, n, dtype, device):
+    """Rows of n values in x's leading dimensions.  (Made in that shape: a view made inside of an autograd function may not
+    be changed in place.)"""
+    if len(lead) == 1:
+        return torch.empty_strided((m, n), (n, 1), dtype=dtype, device=device)
+    return torch.empty(tuple(lead) + (n,), dtype=dtype, device=device)
+
+
 _NOTHING = contextlib.nullcontext()
 
 
@@ -121,9 +129,9 @@ def _p(t: Optional[torch.Tensor]):
 
 
 # ---------------------------------------------------------------------------- act(x Wᵀ + bias) + residual
-def _linear(x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
+def _linear(lead, x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
     dev = x2.device
-    y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=dev)
+    y = _output(lead, m, n, out_dtype, dev)
     pre = torch.empty_strided((m, n), (n, 1), dtype=torch.float32, device=dev) if want_pre else None
     L = lib()
     code = _CODE[x2.dtype]
@@ -148,7 +156,7 @@ def _fused_linear_backward(ctx, d):
             pre = pre.contiguous()
         dev, dt = x2.device, x2.dtype
         if want_x:
-            dx = torch.empty_strided((m, k), (k, 1), dtype=dt, device=dev)
+            dx = _output(shape[:-1], m, k, dt, dev)
         if want_w:
             dw = torch.empty_strided((n, k), (k, 1), dtype=dt, device=dev)
         if want_b:
@@ -163,8 +171,6 @@ def _fused_linear_backward(ctx, d):
                                           _p(db), m, n, k, act, code, _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index))
             if rc:
                 check(rc, "verace_linear_backward")
-        if dx is not None and len(shape) != 2:
-            dx = dx.view(shape)
     return dx, dw, db, d if want_r else None, None, None, None, None, None
 
 
@@ -178,11 +184,10 @@ class _FusedLinear(torch.autograd.Function):
         w2, ldw = _rows(weight, n, k)
         b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         res, ldr = _residual_rows(residual, m, n)
-        y, pre = _linear(x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
+        y, pre = _linear(x.shape[:-1], x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
         ctx.save_for_backward(x2, w2, pre)
-        shape = x.shape
-        ctx.sizes = (shape, m, n, k, act, out_dtype)
-        return y if len(shape) == 2 else y.view(shape[:-1] + (n,))
+        ctx.sizes = (x.shape, m, n, k, act, out_dtype)
+        return y
 
     @staticmethod
     def backward(ctx, d):
@@ -220,8 +225,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     act, k, n, odt = _checked("fused_linear", x, weight, (x_scale is not None) + (w_scale is not None), 2, activation,
                               _ACTIVATIONS, out_dtype, torch.bfloat16 if residual is None else residual.dtype)
     lead = x.shape[:-1]
-    flat = len(lead) == 1
-    m = lead[0] if flat else math.prod(lead)
+    m = lead[0] if len(lead) == 1 else math.prod(lead)
     eight = x.dtype is FP8
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
     b = bias
@@ -252,8 +256,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
         sw = _vector(w_scale, n, torch.float32, dev, "w_scale")
     res, ldr = _residual_rows(residual, m, n)
-    y, _ = _linear(x2, ldx, sx, w2, ldw, sw, b, res, ldr, m, n, k, act, odt, False)
-    return y if flat else y.view(lead + (n,))
+    return _linear(lead, x2, ldx, sx, w2, ldw, sw, b, res, ldr, m, n, k, act, odt, False)[0]
 
 
 # ---------------------------------------------------------------------------- act(x Wgᵀ) up(x Wuᵀ)
@@ -268,9 +271,9 @@ def _gate_rows(w_gate, w_up, f, k):
     return g2, u2, ldg
 
 
-def _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
+def _gated(lead, x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
     dev = x2.device
-    h = torch.empty_strided((m, f), (f, 1), dtype=out_dtype, device=dev)
+    h = _output(lead, m, f, out_dtype, dev)
     gate = up = None
     if want_pre:
         gate = torch.empty_strided((m, f), (f, 1), dtype=torch.float32, device=dev)
@@ -294,7 +297,7 @@ def _gated_linear_backward(ctx, d):
     (x2, ldx), (g2, u2, ldw) = _rows(x2, m, k), _gate_rows(g2, u2, f, k)     # (as in _fused_linear_backward)
     gate, up = gate.contiguous(), up.contiguous()
     dev, dt = x2.device, x2.dtype
-    dx = torch.empty_strided((m, k), (k, 1), dtype=dt, device=dev) if want_x else None
+    dx = _output(shape[:-1], m, k, dt, dev) if want_x else None
     dg = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_g else None
     du = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_u else None
     d2 = d.contiguous()
@@ -308,8 +311,6 @@ def _gated_linear_backward(ctx, d):
                                             _DTYPE[out_dtype], _p(ws), nws, raw_stream(dev.index))
         if rc:
             check(rc, "verace_gated_linear_backward")
-    if dx is not None and len(shape) != 2:
-        dx = dx.view(shape)
     return dx, dg, du, None, None, None, None, None, None, None
 
 
@@ -321,11 +322,10 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, act, b1, b2, out_dtype, m, f, k):
         x2, ldx = _rows(x, m, k)
         g2, u2, ldw = _gate_rows(w_gate, w_up, f, k)
-        h, gate, up = _gated(x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
+        h, gate, up = _gated(x.shape[:-1], x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
         ctx.save_for_backward(x2, g2, u2, gate, up)
-        shape = x.shape
-        ctx.sizes = (shape, m, f, k, act, b1, b2, out_dtype)
-        return h if len(shape) == 2 else h.view(shape[:-1] + (f,))
+        ctx.sizes = (x.shape, m, f, k, act, b1, b2, out_dtype)
+        return h
 
     @staticmethod
     def backward(ctx, d):
@@ -357,8 +357,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     if act == 5 and not (beta1 and beta2):
         raise ValueError(f"gated_linear: beta1 {beta1}, beta2 {beta2} (expected anything but 0)")
     lead = x.shape[:-1]
-    flat = len(lead) == 1
-    m = lead[0] if flat else math.prod(lead)
+    m = lead[0] if len(lead) == 1 else math.prod(lead)
     eight = x.dtype is FP8
     if forward_ad._current_level >= 0:
         _no_tangents("gated_linear", x, w_gate, w_up, x_scale, gate_scale, up_scale)
@@ -375,8 +374,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
         sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
         sg = _vector(gate_scale, f, torch.float32, dev, "gate_scale")
         su = _vector(up_scale, f, torch.float32, dev, "up_scale")
-    h, _, _ = _gated(x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, beta1, beta2, odt, False)
-    return h if flat else h.view(lead + (f,))
+    return _gated(lead, x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, beta1, beta2, odt, False)[0]
 
 
 # ---------------------------------------------------------------------------- rows in 8 bits
