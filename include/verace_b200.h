@@ -241,7 +241,7 @@ VERACE_API int verace_decode_cham_lazy_projected(const void* y, long long ld, fl
  * SSSDAttention's per-head RMSNorm, sssd_attention.py:177-182; CHAM's output RMSNorm,
  * cham_memory.py:241).  RMSNorm as torch.nn.RMSNorm: x * rsqrt(mean(x^2) + eps) in fp32,
  * rounded to the dtype, then times the weight (rounded); no weight when weight is NULL.
- * Rows of `cols` contiguous elements; cols % 8 == 0, cols <= 2048.
+ * Rows of `cols` contiguous elements; cols % 8 == 0, cols <= 2048; 16-byte aligned tensors.
  * verace_rmsnorm:     y = RMSNorm(x)                   (x and y may alias)
  * verace_add_rmsnorm: h <- h + (norm_y ? RMSNorm(y; y_weight, y_eps) : y), in place;
  *                     then n = RMSNorm(h; n_weight, n_eps) when n is not NULL.

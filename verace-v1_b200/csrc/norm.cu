@@ -399,6 +399,8 @@ extern "C" int verace_rmsnorm(const void* x, const void* weight, void* y, long l
   if (int rc = check_shape("verace_rmsnorm", rows, cols, dtype)) return rc;
   if (rows == 0) return VERACE_OK;
   VERACE_REQUIRE(x && y, VERACE_ERR_INVALID, "verace_rmsnorm: NULL pointer");
+  VERACE_REQUIRE((((uintptr_t)x | (uintptr_t)weight | (uintptr_t)y) & 15) == 0, VERACE_ERR_INVALID,
+                 "verace_rmsnorm: x, weight and y must be 16-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case VERACE_F32: return launch_rmsnorm<float>(x, weight, y, rows, cols, eps, st);
@@ -413,6 +415,8 @@ extern "C" int verace_add_rmsnorm(void* h, const void* y, int norm_y, const void
   if (int rc = check_shape("verace_add_rmsnorm", rows, cols, dtype)) return rc;
   if (rows == 0) return VERACE_OK;
   VERACE_REQUIRE(h && y, VERACE_ERR_INVALID, "verace_add_rmsnorm: NULL pointer");
+  VERACE_REQUIRE((((uintptr_t)h | (uintptr_t)y | (uintptr_t)y_weight | (uintptr_t)n_weight | (uintptr_t)n) & 15) == 0,
+                 VERACE_ERR_INVALID, "verace_add_rmsnorm: h, y, n and the weights must be 16-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case VERACE_F32:

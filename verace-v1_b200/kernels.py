@@ -253,6 +253,20 @@ def _norm_args(norm: Optional[torch.nn.Module], x: torch.Tensor):
     return w.data_ptr(), float(eps)
 
 
+def _at_border(t: torch.Tensor) -> torch.Tensor:
+    """t where it starts at a 16-byte border, else a copy that does."""
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
+
+
+def _norm_weight(norm: Optional[torch.nn.Module], x: torch.Tensor):
+    """(_norm_args, the tensor that holds the weight at a 16-byte border or None)."""
+    w, eps = _norm_args(norm, x)
+    if w % 16 == 0:
+        return w, eps, None
+    copy = _at_border(norm.weight)
+    return copy.data_ptr(), eps, copy
+
+
 def fused_norm_supported(x: torch.Tensor) -> bool:
     """Whether rmsnorm / add_rmsnorm take rows of x's last dimension."""
     c = x.shape[-1]
@@ -262,9 +276,9 @@ def fused_norm_supported(x: torch.Tensor) -> bool:
 def rmsnorm(x: torch.Tensor, norm: torch.nn.Module) -> torch.Tensor:
     """`norm` (a torch.nn.RMSNorm over the last dimension) applied to x in one pass."""
     assert x.is_cuda, "This kernel requires CUDA tensors"
-    x = x.contiguous()
+    x = _at_border(x.contiguous())
     y = torch.empty_like(x)
-    w, eps = _norm_args(norm, x)
+    w, eps, _held = _norm_weight(norm, x)
     cols = x.shape[-1]
     with torch.cuda.device(x.device):
         rc = lib().verace_rmsnorm(x.data_ptr(), w, y.data_ptr(), x.numel() // cols, cols, eps,
@@ -279,9 +293,15 @@ def add_rmsnorm(h: torch.Tensor, y: torch.Tensor, y_norm: Optional[torch.nn.Modu
     (h contiguous), then out_norm(h) is returned (None without out_norm)."""
     assert h.is_cuda and h.is_contiguous(), "h must be a contiguous CUDA tensor (updated in place)"
     assert y.shape == h.shape and y.dtype == h.dtype, "h and y must match"
-    y = y.contiguous()
-    wy, ey = _norm_args(y_norm, h)
-    wn, en = _norm_args(out_norm, h)
+    if h.data_ptr() % 16:       # (on a copy, and back)
+        moved = _at_border(h)
+        n = add_rmsnorm(moved, y, y_norm, out_norm)
+        with torch.no_grad():
+            h.copy_(moved)
+        return n
+    y = _at_border(y.contiguous())
+    wy, ey, _held_y = _norm_weight(y_norm, h)
+    wn, en, _held_n = _norm_weight(out_norm, h)
     n = torch.empty_like(h) if out_norm is not None else None
     cols = h.shape[-1]
     with torch.cuda.device(h.device):
