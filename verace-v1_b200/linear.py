@@ -108,12 +108,12 @@ def _no_tangents(who, *tensors):
             raise RuntimeError(f"{who} has no forward-mode derivative")
 
 
-def _output(lead, m, n, dtype, device):
-    """Rows of n values in x's leading dimensions.  (Made in that shape: a view made inside of an autograd function may not
-    be changed in place.)"""
-    if len(lead) == 1:
+def _output(shape, m, n, dtype, device):
+    """Rows of n values in the leading dimensions of x's shape.  (Made in that shape: a view made inside of an autograd
+    function may not be changed in place.)"""
+    if len(shape) == 2:
         return torch.empty_strided((m, n), (n, 1), dtype=dtype, device=device)
-    return torch.empty(tuple(lead) + (n,), dtype=dtype, device=device)
+    return torch.empty(shape[:-1] + (n,), dtype=dtype, device=device)
 
 
 _NOTHING = contextlib.nullcontext()
@@ -129,9 +129,9 @@ def _p(t: Optional[torch.Tensor]):
 
 
 # ---------------------------------------------------------------------------- act(x Wᵀ + bias) + residual
-def _linear(lead, x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
+def _linear(shape, x2, ldx, sx, w2, ldw, sw, bias, res, ldr, m, n, k, act, out_dtype, want_pre):
     dev = x2.device
-    y = _output(lead, m, n, out_dtype, dev)
+    y = _output(shape, m, n, out_dtype, dev)
     pre = torch.empty_strided((m, n), (n, 1), dtype=torch.float32, device=dev) if want_pre else None
     L = lib()
     code = _CODE[x2.dtype]
@@ -156,7 +156,7 @@ def _fused_linear_backward(ctx, d):
             pre = pre.contiguous()
         dev, dt = x2.device, x2.dtype
         if want_x:
-            dx = _output(shape[:-1], m, k, dt, dev)
+            dx = _output(shape, m, k, dt, dev)
         if want_w:
             dw = torch.empty_strided((n, k), (k, 1), dtype=dt, device=dev)
         if want_b:
@@ -184,7 +184,7 @@ class _FusedLinear(torch.autograd.Function):
         w2, ldw = _rows(weight, n, k)
         b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         res, ldr = _residual_rows(residual, m, n)
-        y, pre = _linear(x.shape[:-1], x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
+        y, pre = _linear(x.shape, x2, ldx, None, w2, ldw, None, b, res, ldr, m, n, k, act, out_dtype, act != 0)
         ctx.save_for_backward(x2, w2, pre)
         ctx.sizes = (x.shape, m, n, k, act, out_dtype)
         return y
@@ -256,7 +256,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
         sw = _vector(w_scale, n, torch.float32, dev, "w_scale")
     res, ldr = _residual_rows(residual, m, n)
-    return _linear(lead, x2, ldx, sx, w2, ldw, sw, b, res, ldr, m, n, k, act, odt, False)[0]
+    return _linear(x.shape, x2, ldx, sx, w2, ldw, sw, b, res, ldr, m, n, k, act, odt, False)[0]
 
 
 # ---------------------------------------------------------------------------- act(x Wgᵀ) up(x Wuᵀ)
@@ -271,9 +271,9 @@ def _gate_rows(w_gate, w_up, f, k):
     return g2, u2, ldg
 
 
-def _gated(lead, x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
+def _gated(shape, x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, b1, b2, out_dtype, want_pre):
     dev = x2.device
-    h = _output(lead, m, f, out_dtype, dev)
+    h = _output(shape, m, f, out_dtype, dev)
     gate = up = None
     if want_pre:
         gate = torch.empty_strided((m, f), (f, 1), dtype=torch.float32, device=dev)
@@ -297,7 +297,7 @@ def _gated_linear_backward(ctx, d):
     (x2, ldx), (g2, u2, ldw) = _rows(x2, m, k), _gate_rows(g2, u2, f, k)     # (as in _fused_linear_backward)
     gate, up = gate.contiguous(), up.contiguous()
     dev, dt = x2.device, x2.dtype
-    dx = _output(shape[:-1], m, k, dt, dev) if want_x else None
+    dx = _output(shape, m, k, dt, dev) if want_x else None
     dg = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_g else None
     du = torch.empty_strided((f, k), (k, 1), dtype=dt, device=dev) if want_u else None
     d2 = d.contiguous()
@@ -322,7 +322,7 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, act, b1, b2, out_dtype, m, f, k):
         x2, ldx = _rows(x, m, k)
         g2, u2, ldw = _gate_rows(w_gate, w_up, f, k)
-        h, gate, up = _gated(x.shape[:-1], x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
+        h, gate, up = _gated(x.shape, x2, ldx, None, g2, u2, ldw, None, None, m, f, k, act, b1, b2, out_dtype, True)
         ctx.save_for_backward(x2, g2, u2, gate, up)
         ctx.sizes = (x.shape, m, f, k, act, b1, b2, out_dtype)
         return h
@@ -374,7 +374,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
         sx = _vector(x_scale, m, torch.float32, dev, "x_scale")
         sg = _vector(gate_scale, f, torch.float32, dev, "gate_scale")
         su = _vector(up_scale, f, torch.float32, dev, "up_scale")
-    return _gated(lead, x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, beta1, beta2, odt, False)[0]
+    return _gated(x.shape, x2, ldx, sx, g2, u2, ldw, sg, su, m, f, k, act, beta1, beta2, odt, False)[0]
 
 
 # ---------------------------------------------------------------------------- rows in 8 bits
