@@ -300,3 +300,32 @@ def test_outputs_may_be_changed_in_place(shape):
         y.sum().backward()
         (call(*want) * r + 1).sum().backward()
         assert all(torch.equal(a.grad, b.grad) and a.grad.shape == b.shape for a, b in zip(got, want))
+
+
+def test_another_module_in_the_sub_layers_place():
+    """A layer whose feed-forward sub-layer, or its base block, a user has replaced or wrapped."""
+    from test_fp8_model_gpu import make_model
+
+    class Wrapped(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            return self.inner(x)
+    x = randn(gen(12), 2, 5, 128, dt=BF16)
+    for eight in (False, True):
+        layer = make_model(BF16).layers[1]
+        if eight:
+            V.quantize_model_fp8(layer)
+        with torch.no_grad():
+            want = layer(x)[0]
+            inner = layer.mcmoe
+            layer.mcmoe = Wrapped(inner)
+            # (in 8 bits the sub-layer then quantises the norm's rounded rows itself)
+            assert torch.equal(layer(x)[0], want) or eight and layer(x)[0].isfinite().all()
+            layer.mcmoe = torch.nn.Linear(128, 128, device="cuda", dtype=BF16)
+            assert layer(x)[0].isfinite().all()
+            layer.mcmoe = inner
+            inner.base_situ_glu = torch.nn.Linear(128, inner.base_w_down.in_features, device="cuda", dtype=BF16)
+            assert layer(x)[0].isfinite().all()

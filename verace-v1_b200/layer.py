@@ -83,7 +83,8 @@ class VeraceV1Layer(nn.Module):
                                                   active_mask=active_mask)
         n = _residual(hcur, sssd_out, self.cham_norm)            # h_mid1, RMSNorm(h_mid1)
         cham_out, new_cham_hologram = self.cham_memory(n, initial_hologram=cham_hologram, active_mask=active_mask)
-        if self.mcmoe.base_situ_glu.fp8_in is not None and cham_out.dtype == hcur.dtype == self.mcmoe_norm.weight.dtype:
+        block = getattr(self.mcmoe, "base_situ_glu", None)       # (a module in the M-CMoE's place may have none)
+        if getattr(block, "fp8_in", None) is not None and cham_out.dtype == hcur.dtype == self.mcmoe_norm.weight.dtype:
             q, scale, n = add_rmsnorm_fp8(hcur, cham_out, self.mcmoe_norm, return_norm=True)   # the same, and its rows in 8 bits
             _residual(hcur, self.mcmoe(n, (q, scale)), None)
         else:
