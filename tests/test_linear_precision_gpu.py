@@ -294,3 +294,23 @@ def test_scales_far_from_1(m, k, n, rows, cols):
         over = exact > MOST
         assert bool((got[over] == math.inf).all()) and bool((got[~over].to(F64) - exact[~over]).abs().le(
             4e-6 * exact[~over].abs() + 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_long_sums_of_few_rows_and_many_outputs(dt):
+    """More tiles of weights than SMs, whose clusters split K because it is long; just below, at and beyond what eight take."""
+    g = gen(21)
+    for k in ((1 << 15) + 64, 1 << 18, (1 << 18) + 64):
+        n, m = (20000 if k < 1 << 17 else 1200), 20
+        x, w = whole(g, 4, m, k, dt=dt), whole(g, 4, n, k, dt=dt)
+        want = product_in_64(x, w)
+        assert torch.equal(V.fused_linear(x, w, out_dtype=F32).to(F64), want)
+        u = torch.zeros(n, k, device="cuda", dtype=dt)
+        u[:, 0] = 1
+        x[:, 0] = 1
+        want = torch.relu(product_in_64(x, w))
+        assert torch.equal(V.gated_linear(x, w, u, activation="relu", out_dtype=F32).to(F64), want)
+        x, w = positive(g, m, k, dt=dt), positive(g, n, k, dt=dt)
+        want, lost = product_in_64(x, w), 3.4e-4 if dt is F16 else 1.4e-3
+        assert bool(((V.fused_linear(x, w, out_dtype=F32).to(F64) - want).abs() <= lost * want).all())
+        del x, w, u, want

@@ -42,15 +42,16 @@ constexpr int FEW = 160;
 // of the running sum (and two bits more) instead of rounding the sum.  Where all terms have one sign that takes 6.4e-9 of the
 // sum a term (fp16; bf16 5e-9 to 6.2e-9, e4m3 up to 1.2e-9; 2048 x 2048 outputs, K = 2^12 ... 2^18): 2.1e-4 of it at 2^15 and
 // 8e-4 at 2^17, less than half of fp16's and of bf16's half step.  Longer sums are split, and the splits' sums added with
-// rounding.  (8 bytes an output and split: 2 to 3 % of the product's time.)
+// rounding.  (fp16, us, against sums unsplit: 4096 x 65536 x 4096 1495 to 1584 and 1530 to 1595, 4096 x 65536 x 1024 425 to 474 and
+// 394 to 469, 16 x 65536 x 16384 335 to 341 and 347 to 359.)
 inline long long run_of(int type) { return type == VERACE_F16 ? 1 << 15 : 1 << 17; }
 
-// CTAs of a cluster that share K in linear_few.cu.
+// CTAs of a cluster that share K in linear_few.cu: while there is an SM for each, or a sum would be too long.
 inline int few_splits(long long N, long long K, int segments, int type) {
   const int step = type == VERACE_E4M3 ? 128 : 64;
   const long long tiles = (N + 127) / 128, steps = (K + step - 1) / step * segments;
   int ck = 1;
-  while (ck < 8 && tiles * ck * 2 <= 148 && steps >= ck * 4) ck *= 2;
+  while (ck < 8 && ((tiles * ck * 2 <= 148 && steps >= ck * 4) || K * segments > run_of(type) * ck)) ck *= 2;
   return ck;
 }
 
