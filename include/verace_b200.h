@@ -399,7 +399,8 @@ VERACE_API int verace_rmsnorm_fp8(const void* h, const void* y, void* sum, const
  * Sums are fp32 and outputs are rounded once.  Sums of 16- and 8-bit operands are formed in the tensor core, which cuts
  *   each product to the running sum's last places instead of rounding the sum: where all terms have one sign k 6.4e-9 of it
  *   (E4M3: 1.2e-9), up to 2.1e-4 at k = 2^15 for fp16 and 8e-4 at 2^17 for bf16, where a sum is split and joined with
- *   rounding.  Sums of fp32 operands stay within 1e-6 at every length (terms of both signs, 2-norm).
+ *   rounding.  Sums of fp32 operands are 1e-7 to 2e-7 off up to k = 2^14, 4e-7 at 2^17 and 2e-6 at 2^22 (terms of both
+ *   signs, 2-norm; of one sign up to 3e-7).
  * In a backward call act'(.) times dout is rounded to dtype before it is multiplied.
  * fp32 operands enter as three bf16 parts (24 bits of every finite value; an infinity gives NaN in every output that it
  *   enters), but for up to 24 rows of x (gated: 16), which take them as they are.
