@@ -146,8 +146,9 @@ rmsnorm_kernel(const T* x, const T* w, T* y, long long rows, int cols, float eps
   const int sl = lane % L, nc = cols / 8;
   const bool act = row < rows;
   const T* xr = x + (act ? row : 0) * cols;
-  // the weights on their way to the L2, which holds no stale values
-  if (w)
+  // the weights on their way to the L2, which holds no stale values (once: asked for by every row, 131072 x 128 took 57 us
+  // instead of 13)
+  if (w && blockIdx.x == 0 && threadIdx.x < L)
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (sl + L * i < nc) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + 8 * (sl + L * i)));
